@@ -28,6 +28,12 @@ BOA_PREC_F32 = 0      # fp32 MFMA
 BOA_PREC_BF16X3 = 1   # split bf16 x3 products (fp32 weights)
 BOA_PREC_BF16W = 2    # bf16 weights, split activations
 
+BOA_DT_F32, BOA_DT_BF16, BOA_DT_F16 = 0, 1, 2  # activations of the operators (boa_amd.ops)
+BOA_LAYER_NORM_MAX_D = 4096
+BOA_CROSS_ENTROPY_MAX_V = 4096
+BOA_OPS_MAX_CHANNELS = 65536
+BOA_SCAN_MARK = 8
+
 
 class BoaError(RuntimeError):
     """Raised when a libboa_hip entry point returns a non-zero status."""
@@ -62,6 +68,7 @@ class ProfEntry(ctypes.Structure):
 
 # (name, restype, argtypes); every declaration of include/boa_hip.h appears here
 _P = ctypes.c_void_p
+_INT = ctypes.c_int
 _I32 = ctypes.c_int32
 _I64 = ctypes.c_int64
 _U64 = ctypes.c_uint64
@@ -97,6 +104,23 @@ SIGNATURES = [
     ("rcb_load", ctypes.c_int, [_P, _P, _P]),
     ("rcb_init_decoder", ctypes.c_int, [_P]),
     ("rcb_decode_step", ctypes.c_int, [_P, _P, _P, _P]),
+    ("boa_layer_norm_fwd", ctypes.c_int, [_INT, _P, _I64, _P, _P, _I64, _I32, _F32, _P, _I64, _P, _P]),
+    ("boa_layer_norm_bwd_work_bytes", _I64, [_I64, _I32]),
+    ("boa_layer_norm_bwd", ctypes.c_int, [_INT, _P, _I64, _P, _I64, _P, _P, _I64, _I32, _P, _I64, _P, _P, _I64, _P]),
+    ("boa_cross_entropy_work_bytes", _I64, []),
+    ("boa_cross_entropy_fwd", ctypes.c_int, [_INT, _P, _I64, _P, _INT, _I64, _I64, _I32, _INT, _P, _P, _P, _P, _P, _I64,
+                                             _P]),
+    ("boa_cross_entropy_bwd", ctypes.c_int, [_INT, _P, _I64, _P, _INT, _I64, _I64, _I32, _P, _P, _INT, _P, _P, _I64, _P]),
+    ("boa_causal_conv_fwd", ctypes.c_int, [_INT, _P, _I64, _I64, _P, _P, _INT, _I64, _I64, _I32, _P, _P, _P, _P, _I64, _I64, _P]),
+    ("boa_causal_conv_bwd_work_bytes", _I64, [_I64, _I64, _I32]),
+    ("boa_causal_conv_bwd", ctypes.c_int, [_INT, _P, _I64, _I64, _P, _I64, _I64, _P, _P, _INT, _I64, _I64, _I32, _P, _P, _P, _I64,
+                                           _I64, _P, _P, _I64, _P]),
+    ("boa_causal_conv_step", ctypes.c_int, [_INT, _P, _I64, _P, _P, _P, _INT, _I64, _I32, _P, _I64, _P]),
+    # boa_scan is passed as the bytes of the struct (ops._SCAN)
+    ("boa_selective_scan_work_bytes", _I64, [ctypes.c_char_p, _INT]),
+    ("boa_selective_scan_fwd", ctypes.c_int, [ctypes.c_char_p, _P, _I64, _P]),
+    ("boa_selective_scan_bwd", ctypes.c_int, [ctypes.c_char_p, _P, _I64, _P]),
+    ("boa_selective_scan_step", ctypes.c_int, [ctypes.c_char_p, _P]),
 ]
 
 _lib = None
@@ -111,8 +135,9 @@ def _bind(lib):
     return lib
 
 
-# The C ABI these signatures describe (boa_abi_version); 2: boa_decompress takes the payload's length.
-ABI_VERSION = 2
+# The C ABI these signatures describe (boa_abi_version); 2: boa_decompress takes the payload's length; 3: the operators of
+# training.
+ABI_VERSION = 3
 
 
 def load_cdll():

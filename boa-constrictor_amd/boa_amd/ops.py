@@ -1,0 +1,481 @@
+"""Operators of the model's training pass and of its streaming by single tokens, on GPU tensors.
+
+  layer_norm          rows of d values, weight and bias (nn.LayerNorm of model.py:45,51)
+  causal_conv         the mixer's depthwise convolution over 4 positions with SiLU (model.py:72)
+  selective_scan      the mixer's state space recurrence with its gate (model.py:72-81)
+  cross_entropy       next-byte loss in nats (train.py:59-63)
+  causal_conv_step, selective_scan_step   one token per sequence, states advanced in place
+
+All of them run hand-written kernels of libboa_hip.so (include/boa_hip.h) on the current stream of their tensors' device,
+synchronize nothing and can be captured into a graph.  The first four are differentiable (once): gradients reach every
+floating input but the states.  Activations are float32, bfloat16 or float16, all of a call of the same type; parameters,
+scan states and the gradients of parameters are float32; arithmetic is in float32 and each result is rounded once.  The same
+inputs give the same bits.
+
+Shapes: activations [batch, length, channels] with any batch and row strides (a last dimension that is not contiguous is
+copied); conv states [batch, 3, channels] in the activations' type, oldest position first; scan states
+[batch, 16, channels] float32; ``lens``: int32 [batch], the sequences' lengths in a padded batch.  Positions behind a
+sequence's end are not read (they may hold anything) and come out, and have gradients, as zeros; a state handed on is the one
+behind the sequence's last position, so a sequence of length 0 hands on the state that it was given.
+
+States carry no gradient: a batch that continues from a state trains on its own positions (truncated back-propagation).
+
+Captured backward passes: torch ties a parameter's gradient accumulation to the stream that first used it, so do the warm-up
+passes on the capture's side stream and let go of any eager graph of the same parameters before capturing.
+"""
+from __future__ import annotations
+
+import struct
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from boa_amd import _native as _nat
+
+__all__ = ["layer_norm", "causal_conv", "causal_conv_step", "selective_scan", "selective_scan_step", "cross_entropy",
+           "D_STATE", "D_CONV"]
+
+D_STATE, D_CONV = 16, 4
+_DTYPES = {torch.float32: _nat.BOA_DT_F32, torch.bfloat16: _nat.BOA_DT_BF16, torch.float16: _nat.BOA_DT_F16}
+_INT_BYTES = {torch.uint8: 1, torch.int32: 4, torch.int64: 8}
+
+
+# ---- argument checks -------------------------------------------------------------------------------
+def _act(who, name, t, shape=None, like=None):
+    """An activation: its type code; a tensor of `like`'s type and device, and of `shape`."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{who}: {name} must be a tensor")
+    code = _DTYPES.get(t.dtype)
+    if code is None:
+        raise TypeError(f"{who}: {name} must be float32, bfloat16 or float16 (got {t.dtype})")
+    if like is not None and (t.dtype != like.dtype or t.device != like.device):
+        raise ValueError(f"{who}: {name} must have the type and device of the other activations "
+                         f"({like.dtype}, {like.device}; got {t.dtype}, {t.device})")
+    if shape is not None and t.shape != shape:
+        raise ValueError(f"{who}: {name} must be {list(shape)} (got {list(t.shape)})")
+    return code
+
+
+def _param(who, name, t, shape, like):
+    """A float32 parameter or state of this shape on the activations' device, contiguous; None stays None."""
+    if t is None:
+        return None
+    if not isinstance(t, torch.Tensor) or t.dtype != torch.float32:
+        raise TypeError(f"{who}: {name} must be a float32 tensor")
+    if t.device != like.device or t.shape != shape:
+        raise ValueError(f"{who}: {name} must be {list(shape)} on {like.device} (got {list(t.shape)} on {t.device})")
+    return t if t.is_contiguous() else t.contiguous()
+
+
+def _state(who, t, shape, like, dtype, in_place):
+    if t is None:
+        return None
+    if not isinstance(t, torch.Tensor) or t.dtype != dtype:
+        raise TypeError(f"{who}: state must be a {dtype} tensor")
+    if t.device != like.device or t.shape != shape:
+        raise ValueError(f"{who}: state must be {list(shape)} on {like.device} (got {list(t.shape)} on {t.device})")
+    if t.requires_grad:
+        raise ValueError(f"{who}: states carry no gradient; detach() it")
+    if not t.is_contiguous():
+        if in_place:
+            raise ValueError(f"{who}: a state that is advanced in place must be contiguous")
+        t = t.contiguous()
+    return t
+
+
+def _lens(who, t, batch, like):
+    if t is None:
+        return None
+    if not isinstance(t, torch.Tensor) or t.dtype not in (torch.int32, torch.int64):
+        raise TypeError(f"{who}: lens must be an int32 tensor")
+    if t.device != like.device or t.shape != (batch,):
+        raise ValueError(f"{who}: lens must be [{batch}] on {like.device} (got {list(t.shape)} on {t.device})")
+    return t.to(torch.int32).contiguous()
+
+
+def _rows(t):
+    """The tensor with a contiguous last dimension."""
+    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+
+
+def _gpu(who, t):
+    if not t.is_cuda:
+        raise ValueError(f"{who}: the tensors must be on the GPU (got {t.device})")
+
+
+def _grad(*ts):
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts)
+
+
+class _On:
+    """The device of a tensor made current for a call, where it is another."""
+
+    def __init__(self, t):
+        i = t.device.index
+        self.guard = None if i == torch.cuda.current_device() else torch.cuda.device(i)
+
+    def __enter__(self):
+        if self.guard is not None:
+            self.guard.__enter__()
+        return torch.cuda.current_stream().cuda_stream
+
+    def __exit__(self, *a):
+        if self.guard is not None:
+            self.guard.__exit__(*a)
+
+
+def _ptr(t):
+    return 0 if t is None else t.data_ptr()
+
+
+def _work(nbytes, like):
+    return torch.empty(nbytes, dtype=torch.uint8, device=like.device) if nbytes else None
+
+
+# ---- layer norm ------------------------------------------------------------------------------------
+def _norm_fwd(x, w, b, eps, keep):
+    d = x.shape[-1]
+    rows = _rows(x.reshape(-1, d))
+    y = torch.empty_like(x, memory_format=torch.contiguous_format)
+    stats = torch.empty((rows.shape[0], 2), dtype=torch.float32, device=x.device) if keep else None
+    with _On(x) as s:
+        _nat.check(_nat.lib().boa_layer_norm_fwd(_DTYPES[x.dtype], rows.data_ptr(), rows.stride(0), _ptr(w), _ptr(b),
+                                                 rows.shape[0], d, eps, y.data_ptr(), d, _ptr(stats), s))
+    return y, stats
+
+
+class _LayerNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, w, b, eps):
+        y, stats = _norm_fwd(x, w, b, eps, True)
+        ctx.save_for_backward(x, w, stats)
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        x, w, stats = ctx.saved_tensors
+        d = x.shape[-1]
+        rows, dyr = _rows(x.reshape(-1, d)), _rows(dy.reshape(-1, d))
+        n = rows.shape[0]
+        dx = torch.empty_like(x, memory_format=torch.contiguous_format)
+        params = ctx.needs_input_grad[1] or ctx.needs_input_grad[2]
+        dwb = torch.empty((2, d), dtype=torch.float32, device=x.device) if params else None
+        lib = _nat.lib()
+        with _On(x) as s:
+            size = lib.boa_layer_norm_bwd_work_bytes(n, d) if params else 0
+            work = _work(size, x)
+            _nat.check(lib.boa_layer_norm_bwd(_DTYPES[x.dtype], dyr.data_ptr(), dyr.stride(0), rows.data_ptr(), rows.stride(0),
+                                              _ptr(w), stats.data_ptr(), n, d, dx.data_ptr(), d, _ptr(dwb), _ptr(work), size, s))
+        need = ctx.needs_input_grad
+        return dx, dwb[0] if need[1] else None, dwb[1] if need[2] else None, None
+
+
+def layer_norm(x, weight=None, bias=None, eps: float = 1e-5):
+    """``(x - mean) / sqrt(var + eps) * weight + bias`` over the last dimension (1 to 4096 values), biased variance.
+
+    x: [..., d]; weight, bias: float32 [d] or None.  Returns a contiguous tensor of x's shape and type."""
+    _act("layer_norm", "x", x)
+    if x.ndim < 1 or not 1 <= x.shape[-1] <= _nat.BOA_LAYER_NORM_MAX_D:
+        raise ValueError(f"layer_norm: x must be [..., d] with 1 <= d <= {_nat.BOA_LAYER_NORM_MAX_D} (got {list(x.shape)})")
+    if not eps >= 0.0:
+        raise ValueError(f"layer_norm: eps must not be negative (got {eps})")
+    w = _param("layer_norm", "weight", weight, x.shape[-1:], x)
+    b = _param("layer_norm", "bias", bias, x.shape[-1:], x)
+    _gpu("layer_norm", x)
+    if _grad(x, w, b):
+        return _LayerNorm.apply(x, w, b, float(eps))
+    return _norm_fwd(x, w, b, float(eps), False)[0]
+
+
+# ---- cross entropy ---------------------------------------------------------------------------------
+class _CrossEntropy(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, target, ignore, reduction, keep):
+        n, v = x.shape
+        stats = torch.empty((n, 2), dtype=torch.float32, device=x.device) if keep else None
+        each = torch.empty(n, dtype=torch.float32, device=x.device) if reduction == "none" else None
+        loss, count = (torch.empty((), dtype=torch.float32, device=x.device) if each is None else None for _ in range(2))
+        lib = _nat.lib()
+        with _On(x) as s:
+            size = lib.boa_cross_entropy_work_bytes() if each is None else 0
+            work = _work(size, x)
+            _nat.check(lib.boa_cross_entropy_fwd(_DTYPES[x.dtype], x.data_ptr(), x.stride(0), target.data_ptr(),
+                                                 target.element_size(), ignore, n, v, reduction == "mean", _ptr(stats),
+                                                 _ptr(each), _ptr(loss), _ptr(count), _ptr(work), size, s))
+        ctx.save_for_backward(x, target, stats, count)
+        ctx.ignore, ctx.reduction = ignore, reduction
+        return loss if each is None else each
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, up):
+        x, target, stats, count = ctx.saved_tensors
+        n, v = x.shape
+        up = up.to(torch.float32).contiguous()
+        dx = torch.empty((n, v), dtype=x.dtype, device=x.device)
+        with _On(x) as s:
+            _nat.check(_nat.lib().boa_cross_entropy_bwd(_DTYPES[x.dtype], x.data_ptr(), x.stride(0), target.data_ptr(),
+                                                        target.element_size(), ctx.ignore, n, v, stats.data_ptr(), up.data_ptr(),
+                                                        ctx.reduction == "none", _ptr(count) if ctx.reduction == "mean" else 0,
+                                                        dx.data_ptr(), v, s))
+        return dx, None, None, None, None
+
+
+def cross_entropy(logits, targets, *, ignore_index: int = -100, reduction: str = "mean"):
+    """``log(sum(exp(logits))) - logits[target]`` of every row, in nats: their mean over the rows that count, their sum, or
+    (reduction "none") one value per row.
+
+    logits: [..., V] (1 to 4096 symbols); targets: uint8, int32 or int64 of the leading shape.  Rows whose target is
+    ignore_index count for nothing and have no gradient (a mean over no rows is NaN); any other target outside [0, V) gives
+    NaN.  Returns float32."""
+    _act("cross_entropy", "logits", logits)
+    if logits.ndim < 1 or not 1 <= logits.shape[-1] <= _nat.BOA_CROSS_ENTROPY_MAX_V:
+        raise ValueError(f"cross_entropy: logits must be [..., V] with 1 <= V <= {_nat.BOA_CROSS_ENTROPY_MAX_V} "
+                         f"(got {list(logits.shape)})")
+    if reduction not in ("mean", "sum", "none"):
+        raise ValueError(f"cross_entropy: reduction must be mean, sum or none (got {reduction!r})")
+    if not isinstance(targets, torch.Tensor) or targets.dtype not in _INT_BYTES:
+        raise TypeError("cross_entropy: targets must be a uint8, int32 or int64 tensor")
+    if targets.device != logits.device or targets.shape != logits.shape[:-1]:
+        raise ValueError(f"cross_entropy: targets must be {list(logits.shape[:-1])} on {logits.device} "
+                         f"(got {list(targets.shape)} on {targets.device})")
+    _gpu("cross_entropy", logits)
+    rows = _rows(logits.reshape(-1, logits.shape[-1]))
+    out = _CrossEntropy.apply(rows, targets.reshape(-1).contiguous(), int(ignore_index), reduction, _grad(logits))
+    return out.reshape(targets.shape) if reduction == "none" else out
+
+
+# ---- causal convolution ----------------------------------------------------------------------------
+def _conv_fwd(x, w, b, silu, state, lens, want_state):
+    n, length, c = x.shape
+    y = torch.empty((n, length, c), dtype=x.dtype, device=x.device)
+    out = torch.empty((n, D_CONV - 1, c), dtype=x.dtype, device=x.device) if want_state else None
+    with _On(x) as s:
+        _nat.check(_nat.lib().boa_causal_conv_fwd(_DTYPES[x.dtype], x.data_ptr(), x.stride(0), x.stride(1), w.data_ptr(), _ptr(b),
+                                                  silu, n, length, c, _ptr(lens), _ptr(state), _ptr(out), y.data_ptr(),
+                                                  length * c, c, s))
+    return y, out
+
+
+class _CausalConv(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, w, b, silu, state, lens, want_state):
+        y, out = _conv_fwd(x, w, b, silu, state, lens, want_state)
+        ctx.save_for_backward(x, w, b, state, lens)
+        ctx.silu = silu
+        if out is not None:
+            ctx.mark_non_differentiable(out)
+        return y, out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy, _):
+        x, w, b, state, lens = ctx.saved_tensors
+        n, length, c = x.shape
+        dy = _rows(dy)
+        dx = torch.empty((n, length, c), dtype=x.dtype, device=x.device)
+        params = ctx.needs_input_grad[1] or ctx.needs_input_grad[2]
+        dwb = torch.empty((D_CONV + 1) * c, dtype=torch.float32, device=x.device) if params else None
+        lib = _nat.lib()
+        with _On(x) as s:
+            size = lib.boa_causal_conv_bwd_work_bytes(n, length, c) if params else 0
+            work = _work(size, x)
+            _nat.check(lib.boa_causal_conv_bwd(_DTYPES[x.dtype], dy.data_ptr(), dy.stride(0), dy.stride(1), x.data_ptr(),
+                                               x.stride(0), x.stride(1), w.data_ptr(), _ptr(b), ctx.silu, n, length, c, _ptr(lens),
+                                               _ptr(state), dx.data_ptr(), length * c, c, _ptr(dwb), _ptr(work), size, s))
+        need = ctx.needs_input_grad
+        dw = dwb[:D_CONV * c].view(w.shape) if need[1] else None
+        db = dwb[D_CONV * c:] if need[2] else None
+        return dx, dw, db, None, None, None, None
+
+
+def _conv_args(who, x, ndim, weight, bias):
+    _act(who, "x", x)
+    if x.ndim != ndim or not 1 <= x.shape[-1] <= _nat.BOA_OPS_MAX_CHANNELS:
+        raise ValueError(f"{who}: x must be {'[batch, length, channels]' if ndim == 3 else '[batch, channels]'} "
+                         f"(got {list(x.shape)})")
+    c = x.shape[-1]
+    flat = isinstance(weight, torch.Tensor) and weight.ndim == 2
+    w = _param(who, "weight", weight, torch.Size((c, D_CONV) if flat else (c, 1, D_CONV)), x)
+    if w is None:
+        raise TypeError(f"{who}: weight must be a float32 tensor")
+    return w, _param(who, "bias", bias, torch.Size((c,)), x)
+
+
+def causal_conv(x, weight, bias=None, *, silu: bool = True, state=None, lens=None, return_state: bool = False):
+    """Depthwise convolution of each channel over the last 4 positions, then SiLU unless ``silu`` is false.
+
+    x: [batch, length, channels]; weight: float32 [channels, 1, 4] (nn.Conv1d's) or [channels, 4], oldest tap first; bias:
+    float32 [channels]; state: the three positions before the first one (zeros without).  Returns y, with ``return_state``
+    also the state behind each sequence's last position, as a new tensor."""
+    w, b = _conv_args("causal_conv", x, 3, weight, bias)
+    n, _, c = x.shape
+    state = _state("causal_conv", state, (n, D_CONV - 1, c), x, x.dtype, False)
+    lens = _lens("causal_conv", lens, n, x)
+    _gpu("causal_conv", x)
+    x = _rows(x)
+    if _grad(x, w, b):
+        y, out = _CausalConv.apply(x, w, b, bool(silu), state, lens, bool(return_state))
+    else:
+        y, out = _conv_fwd(x, w, b, bool(silu), state, lens, return_state)
+    return (y, out) if return_state else y
+
+
+def causal_conv_step(x, state, weight, bias=None, *, silu: bool = True):
+    """``causal_conv`` of one position per sequence: x [batch, channels]; state [batch, 3, channels] is advanced in place.
+    Returns y [batch, channels]; no gradient."""
+    who = "causal_conv_step"
+    w, b = _conv_args(who, x, 2, weight, bias)
+    n, c = x.shape
+    if state is None:
+        raise TypeError(f"{who}: state must be a tensor")
+    state = _state(who, state, (n, D_CONV - 1, c), x, x.dtype, True)
+    if _grad(x, w, b):
+        raise ValueError(f"{who}: no gradient; call it under torch.no_grad()")
+    _gpu(who, x)
+    x = _rows(x)
+    y = torch.empty((n, c), dtype=x.dtype, device=x.device)
+    with _On(x) as s:
+        _nat.check(_nat.lib().boa_causal_conv_step(_DTYPES[x.dtype], x.data_ptr(), x.stride(0), state.data_ptr(), w.data_ptr(),
+                                                   _ptr(b), bool(silu), n, c, y.data_ptr(), c, s))
+    return y
+
+
+# ---- selective scan --------------------------------------------------------------------------------
+# boa_scan (include/boa_hip.h): dtype, channels, batch, length; u, delta, z, b, c (pointer, two strides); a, d, delta_bias,
+# lens, state_in, state_out, marks; y, dy, du, ddelta, dz, db, dc; dpar
+_SCAN = struct.Struct("@iiqq15q7q21qq")
+_NO_ROWS = (0, 0, 0)
+
+
+def _r3(t):
+    return _NO_ROWS if t is None else (t.data_ptr(), t.stride(0), t.stride(1))
+
+
+def _pack(u, delta, A, B, C, D, z, bias, lens, state_in, state_out, marks, y, back=(None,) * 6, dpar=None):
+    n, length, c = u.shape
+    return _SCAN.pack(_DTYPES[u.dtype], c, n, length, *_r3(u), *_r3(delta), *_r3(z), *_r3(B), *_r3(C), A.data_ptr(), _ptr(D),
+                      _ptr(bias), _ptr(lens), _ptr(state_in), _ptr(state_out), _ptr(marks), *_r3(y), *_r3(back[0]), *_r3(back[1]),
+                      *_r3(back[2]), *_r3(back[3]), *_r3(back[4]), *_r3(back[5]), _ptr(dpar))
+
+
+def _scalar_rows(t):
+    """B or C as the kernels read them: rows of a 16-bit type begin at multiples of 4 bytes."""
+    t = _rows(t)
+    if t.element_size() == 2 and (t.data_ptr() % 4 or any(s % 2 for s in t.stride()[:-1])):
+        t = t.clone(memory_format=torch.contiguous_format)
+    return t
+
+
+def _scan_fwd(u, delta, A, B, C, D, z, bias, state, lens, want_state, keep):
+    n, length, c = u.shape
+    y = torch.empty((n, length, c), dtype=u.dtype, device=u.device)
+    out = torch.empty((n, D_STATE, c), dtype=torch.float32, device=u.device) if want_state else None
+    marks = None
+    if keep:
+        blocks = -(-length // _nat.BOA_SCAN_MARK)
+        marks = torch.empty((n, blocks, D_STATE, c), dtype=torch.float32, device=u.device)
+    args = _pack(u, delta, A, B, C, D, z, bias, lens, state, out, marks, y)
+    lib = _nat.lib()
+    with _On(u) as s:
+        size = lib.boa_selective_scan_work_bytes(args, 0)
+        work = _work(size, u)
+        _nat.check(lib.boa_selective_scan_fwd(args, _ptr(work), size, s))
+    return y, out, marks
+
+
+class _SelectiveScan(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, u, delta, A, B, C, D, z, bias, state, lens, want_state):
+        y, out, marks = _scan_fwd(u, delta, A, B, C, D, z, bias, state, lens, want_state, True)
+        ctx.save_for_backward(u, delta, A, B, C, D, z, bias, lens, marks)
+        if out is not None:
+            ctx.mark_non_differentiable(out)
+        return y, out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy, _):
+        u, delta, A, B, C, D, z, bias, lens, marks = ctx.saved_tensors
+        n, length, c = u.shape
+        dy = _rows(dy)
+        du, ddelta = torch.empty_like(dy, memory_format=torch.contiguous_format), torch.empty_like(
+            dy, memory_format=torch.contiguous_format)
+        dz = torch.empty_like(dy, memory_format=torch.contiguous_format) if z is not None else None
+        dB, dC = (torch.empty((n, length, D_STATE), dtype=u.dtype, device=u.device) for _ in range(2))
+        dpar = torch.empty((D_STATE + 2) * c, dtype=torch.float32, device=u.device)
+        args = _pack(u, delta, A, B, C, D, z, bias, lens, None, None, marks, None, (dy, du, ddelta, dz, dB, dC), dpar)
+        lib = _nat.lib()
+        with _On(u) as s:
+            size = lib.boa_selective_scan_work_bytes(args, 1)
+            work = _work(size, u)
+            _nat.check(lib.boa_selective_scan_bwd(args, _ptr(work), size, s))
+        dA = dpar[:D_STATE * c].view(c, D_STATE)
+        dD = dpar[D_STATE * c:(D_STATE + 1) * c] if D is not None else None
+        dbias = dpar[(D_STATE + 1) * c:] if bias is not None else None
+        return du, ddelta, dA, dB, dC, dD, dz, dbias, None, None, None
+
+
+def _scan_args(who, ndim, u, delta, A, B, C, D, z, bias):
+    _act(who, "u", u)
+    if u.ndim != ndim or not 1 <= u.shape[-1] <= _nat.BOA_OPS_MAX_CHANNELS:
+        raise ValueError(f"{who}: u must be {'[batch, length, channels]' if ndim == 3 else '[batch, channels]'} "
+                         f"(got {list(u.shape)})")
+    c = u.shape[-1]
+    _act(who, "delta", delta, u.shape, u)
+    if z is not None:
+        _act(who, "z", z, u.shape, u)
+    states = u.shape[:-1] + (D_STATE,)
+    _act(who, "B", B, states, u)
+    _act(who, "C", C, states, u)
+    A = _param(who, "A", A, torch.Size((c, D_STATE)), u)
+    if A is None:
+        raise TypeError(f"{who}: A must be a float32 tensor")
+    D, bias = _param(who, "D", D, torch.Size((c,)), u), _param(who, "delta_bias", bias, torch.Size((c,)), u)
+    return _rows(u), _rows(delta), A, _scalar_rows(B), _scalar_rows(C), D, None if z is None else _rows(z), bias
+
+
+def selective_scan(u, delta, A, B, C, D=None, z=None, delta_bias=None, *, state=None, lens=None, return_state: bool = False):
+    """``h = exp(dt A) h + dt B u``, ``y = (C . h + D u) silu(z)`` along the positions, ``dt = softplus(delta + delta_bias)``.
+
+    u, delta, z: [batch, length, channels]; B, C: [batch, length, 16], shared by the channels; A: float32 [channels, 16]
+    (negative); D, delta_bias: float32 [channels].  Without z there is no gate, without D no skip.  state: [batch, 16, channels]
+    before the first position (zeros without).  Returns y, with ``return_state`` also the state behind each sequence's last
+    position, as a new tensor."""
+    who = "selective_scan"
+    args = _scan_args(who, 3, u, delta, A, B, C, D, z, delta_bias)
+    n, _, c = u.shape
+    state = _state(who, state, (n, D_STATE, c), u, torch.float32, False)
+    lens = _lens(who, lens, n, u)
+    _gpu(who, u)
+    if _grad(*args):
+        y, out = _SelectiveScan.apply(*args, state, lens, bool(return_state))
+    else:
+        y, out, _ = _scan_fwd(*args, state, lens, return_state, False)
+    return (y, out) if return_state else y
+
+
+def selective_scan_step(u, delta, A, B, C, D=None, z=None, delta_bias=None, *, state):
+    """``selective_scan`` of one position per sequence: u, delta, z [batch, channels], B, C [batch, 16]; state
+    [batch, 16, channels] is advanced in place.  Returns y [batch, channels]; no gradient."""
+    who = "selective_scan_step"
+    args = _scan_args(who, 2, u, delta, A, B, C, D, z, delta_bias)
+    n, c = u.shape
+    if state is None:
+        raise TypeError(f"{who}: state must be a tensor")
+    state = _state(who, state, (n, D_STATE, c), u, torch.float32, True)
+    if _grad(*args):
+        raise ValueError(f"{who}: no gradient; call it under torch.no_grad()")
+    _gpu(who, u)
+    y = torch.empty((n, c), dtype=u.dtype, device=u.device)
+    u, delta, A, B, C, D, z, bias = args
+
+    def r2(t):
+        return _NO_ROWS if t is None else (t.data_ptr(), t.stride(0), 0)
+
+    packed = _SCAN.pack(_DTYPES[u.dtype], c, n, 1, *r2(u), *r2(delta), *r2(z), *r2(B), *r2(C), A.data_ptr(), _ptr(D), _ptr(bias),
+                        0, 0, state.data_ptr(), 0, *r2(y), *(_NO_ROWS * 6), 0)
+    with _On(u) as s:
+        _nat.check(_nat.lib().boa_selective_scan_step(packed, s))
+    return y

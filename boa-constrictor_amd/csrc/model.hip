@@ -47,7 +47,7 @@ int boa_fail_hip(hipError_t e, const char* what, const char* file, int line) {
 }
 
 extern "C" const char* boa_last_error(void) { return g_last_error.c_str(); }
-extern "C" int boa_abi_version(void) { return 2; }  // 2: boa_decompress takes payload_words
+extern "C" int boa_abi_version(void) { return 3; }  // 2: boa_decompress takes payload_words; 3: the operators of training
 
 extern "C" int boa_is_device_pointer(const void* p) {
     hipPointerAttribute_t a;

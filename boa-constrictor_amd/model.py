@@ -6,6 +6,9 @@ its checkpoints load with ``load_state_dict`` (main.py:262-280) and the weight c
 applies.  Compute is not PyTorch: ``forward``, ``init_stream`` and ``step`` run the gfx950 kernels of
 libboa_hip.so through its C ABI.  PyTorch holds the parameters and the I/O tensors only.
 
+Training has its own path (``loss``, ``train_forward``): autograd over library matrix products and the operators of
+``boa_amd.ops`` (layer norm, causal convolution, selective scan, cross entropy), which run kernels of the same library.
+
 There is no CPU compute path.  The reference builds a mambapy model when no GPU is present
 (model.py:14-15); here step/forward raise on CPU instead of silently falling back.
 """
@@ -18,8 +21,10 @@ import os
 import numpy as np
 import torch
 import torch.nn as nn
+import torch.nn.functional as F
 
 from boa_amd import _native as _nat
+from boa_amd import ops
 from boa_amd import weights as _W
 
 __all__ = ["BoaConstrictor", "BoaBytePredictor", "MambaBlock", "Mixer"]
@@ -60,6 +65,51 @@ class Mixer(nn.Module):
         self.D = nn.Parameter(torch.ones(di))
         self.out_proj = nn.Linear(di, d_model, bias=False)
 
+    def forward(self, x, lens=None, cache=None):
+        """The mixer over x [batch, length, d_model] (model.py:59-62), differentiable in x and the parameters.
+
+        lens: the sequences' lengths in a padded batch (what lies behind a sequence's end is not read).  cache: a state of
+        ``init_cache``, which the positions continue and which is advanced in place; states carry no gradient."""
+        # two products instead of one and its halves: u and z come out contiguous, and their gradients need not be joined
+        w = self.in_proj.weight
+        u, z = F.linear(x, w[:self.d_inner]), F.linear(x, w[self.d_inner:])
+        conv, ssm = cache if cache is not None else (None, None)
+        keep = cache is not None
+        if keep and torch.is_grad_enabled():
+            conv_start = conv.clone()  # the backward pass reads it after the cache has advanced
+        else:
+            conv_start = conv
+        u = ops.causal_conv(u, self.conv1d.weight, self.conv1d.bias, state=conv_start, lens=lens, return_state=keep)
+        if keep:
+            u, conv_end = u
+        dr, B, C = self.x_proj(u).split([self.dt_rank, self.d_state, self.d_state], dim=-1)
+        delta = F.linear(dr, self.dt_proj.weight)
+        y = ops.selective_scan(u, delta, -torch.exp(self.A_log), B, C, self.D, z, self.dt_proj.bias, state=ssm, lens=lens,
+                               return_state=keep)
+        if keep:
+            y, ssm_end = y
+            conv.copy_(conv_end)
+            ssm.copy_(ssm_end)
+        return self.out_proj(y)
+
+    @torch.no_grad()
+    def step(self, x, cache):
+        """One position per sequence: x [batch, d_model]; advances the cache in place (model.py:78)."""
+        conv, ssm = cache
+        w = self.in_proj.weight
+        u, z = F.linear(x, w[:self.d_inner]), F.linear(x, w[self.d_inner:])
+        u = ops.causal_conv_step(u, conv, self.conv1d.weight, self.conv1d.bias)
+        dr, B, C = self.x_proj(u).split([self.dt_rank, self.d_state, self.d_state], dim=-1)
+        delta = F.linear(dr, self.dt_proj.weight)
+        return self.out_proj(ops.selective_scan_step(u, delta, -torch.exp(self.A_log), B, C, self.D, z, self.dt_proj.bias,
+                                                     state=ssm))
+
+    def init_cache(self, batch_size: int, dtype=torch.float32):
+        """Zero conv and scan states (model.py:68-73).  dtype: that of the activations (bfloat16 under such an autocast)."""
+        dev = self.in_proj.weight.device
+        return (torch.zeros((batch_size, self.d_conv - 1, self.d_inner), dtype=dtype, device=dev),
+                torch.zeros((batch_size, self.d_state, self.d_inner), dtype=torch.float32, device=dev))
+
 
 class MambaBlock(nn.Module):
     """model.py:42-56: x + FF(LN2(Mamba(LN1(x)))), FF = Linear(d, 4d) -> GELU -> Linear(4d, d)."""
@@ -70,6 +120,20 @@ class MambaBlock(nn.Module):
         self.mamba = Mixer(d_model)
         self.ln2 = nn.LayerNorm(d_model)
         self.ff = nn.Sequential(nn.Linear(d_model, 4 * d_model), nn.GELU(), nn.Linear(4 * d_model, d_model))
+
+    def forward(self, x, lens=None, cache=None):
+        """x [batch, length, d_model] -> the same shape, differentiable; lens and cache as ``Mixer.forward``'s."""
+        y = self.mamba(ops.layer_norm(x, self.ln1.weight, self.ln1.bias, self.ln1.eps), lens, cache)
+        return x + self.ff(ops.layer_norm(y, self.ln2.weight, self.ln2.bias, self.ln2.eps))
+
+    @torch.no_grad()
+    def step(self, x, cache):
+        """One position per sequence, x [batch, d_model]; advances the cache in place (model.py:75-81)."""
+        y = self.mamba.step(ops.layer_norm(x, self.ln1.weight, self.ln1.bias, self.ln1.eps), cache)
+        return x + self.ff(ops.layer_norm(y, self.ln2.weight, self.ln2.bias, self.ln2.eps))
+
+    def init_cache(self, batch_size: int, dtype=torch.float32):
+        return self.mamba.init_cache(batch_size, dtype)
 
 
 # Contexts of up to this many lanes hold extra workspace for tiles in flight (PIPE_LANES, model.hip): their memory grows
@@ -244,6 +308,64 @@ class BoaBytePredictor(nn.Module):
         if L:
             eng.forward(tok, out)
         return out
+
+    # ---- training ---------------------------------------------------------------------------------
+    def _embed(self, x):
+        """Embedding rows of bytes; NaN for what is no symbol of the vocabulary."""
+        w = self.embedding.weight
+        if x.dtype == torch.uint8 and len(w) >= 256:
+            return F.embedding(x.to(w.device, torch.long), w)
+        x = x.to(w.device, torch.long)
+        h = F.embedding(x.clamp(0, len(w) - 1), w)
+        return torch.where(((x < 0) | (x >= len(w)))[..., None], torch.full((), float("nan"), device=w.device), h)
+
+    def train_forward(self, x, lens=None, caches=None):
+        """Next-byte logits [B, L, V] of bytes x [B, L] with gradients for every parameter (the model must be on the GPU).
+
+        ``forward`` runs the codec's fused kernels and has no gradient; this is the training loop's forward (train.py:59).
+        It runs on the parameters as they are now: there is no copy of the weights to rebuild after an optimizer step.  Under
+        ``torch.autocast`` the products, the convolution and the scan run in its type, layer norms and residuals in float32.
+        Its logits are not bit-identical with ``forward``'s, so files are written and read with ``forward`` alone.
+
+        lens: lengths of the sequences in a padded batch.  caches: states of ``init_caches`` that the bytes continue and that
+        are advanced in place (truncated back-propagation, or streaming without an engine)."""
+        if x.ndim != 2:
+            raise ValueError(f"x must be [batch, length] (got {list(x.shape)})")
+        if lens is not None:
+            inside = torch.arange(x.shape[1], device=lens.device) < lens[:, None]
+            x = torch.where(inside, x.to(inside.device), torch.zeros((), dtype=x.dtype, device=inside.device))
+        h = self._embed(x)
+        for i, block in enumerate(self.blocks):
+            h = block(h, lens, None if caches is None else caches[i])
+        return self.head(h)
+
+    def loss(self, x, lens=None):
+        """Mean cross entropy in nats per coded byte of x [B, L]: bytes 1 .. L - 1 of each row, up to its length, under the
+        model's prediction from those before (byte 0 is stored raw); divide by ln 2 for bits per byte (train.py:9-22)."""
+        if x.ndim != 2 or x.shape[1] < 2:
+            raise ValueError(f"x must be [batch, length >= 2] (got {list(x.shape)})")
+        x = x.to(self.embedding.weight.device)
+        target, before = x[:, 1:], None
+        if lens is not None:
+            before = (lens - 1).clamp(min=0)
+            coded = torch.arange(1, x.shape[1], device=x.device) < lens[:, None]
+            target = torch.where(coded, target.to(torch.long), torch.full((), -100, device=x.device))
+        elif target.dtype not in (torch.uint8, torch.int32, torch.int64):
+            target = target.to(torch.long)
+        return ops.cross_entropy(self.train_forward(x[:, :-1], before), target, ignore_index=-100)
+
+    @torch.no_grad()
+    def train_step(self, byte_t, caches):
+        """``step`` on the parameters as they are now: bytes [B] -> logits [B, V]; advances the caches in place.  For sampling
+        from a model in training; ``init_stream`` and ``step`` run a loaded model faster."""
+        h = self._embed(byte_t.reshape(-1))
+        for block, cache in zip(self.blocks, caches):
+            h = block.step(h, cache)
+        return self.head(h)
+
+    def init_caches(self, batch_size: int, dtype=torch.float32):
+        """Zero states for ``train_forward`` and ``train_step``, one per block."""
+        return [block.init_cache(batch_size, dtype) for block in self.blocks]
 
     @torch.inference_mode()
     def init_stream(self, max_len: int, batch_size: int = 1, device=None, dtype=None):

@@ -30,7 +30,7 @@ extern "C" {
 
 /* Library identity and last error (replaces the reference's exit(1) on CUDA errors, gemm_gpu.hpp:36-43). */
 const char* boa_last_error(void);
-int boa_abi_version(void);  /* 2 (boa_decompress takes the payload length since version 2) */
+int boa_abi_version(void);  /* 3 (2: boa_decompress takes the payload length; 3: the operators of training) */
 /* Reports whether d_ptr is device memory of the HIP runtime this library is bound to (1 yes, 0 no). */
 int boa_is_device_pointer(const void* d_ptr);
 
@@ -204,6 +204,101 @@ int rcb_get_words(rcb* b, uint32_t* h_words, int64_t cap_words, int64_t* h_total
 int rcb_load(rcb* b, const uint32_t* h_words, const int32_t* h_sizes);
 int rcb_init_decoder(rcb* b);                                                        /* :293-297 */
 int rcb_decode_step(rcb* b, const float* d_probs, int32_t* d_out_syms, const uint8_t* d_mask); /* :298-305 */
+
+/* ------------------------------------------------------------------------------------------------ */
+/* Operators of the model's training pass (train.py's loop, model.py:42-81) and of its streaming by single tokens, on
+ * tensors of the caller.  No context: each call runs on the given stream of the current device, allocates nothing and
+ * synchronizes nothing, so it can be captured into a graph.  Activations are float32, bfloat16 or float16 (BOA_DT_*),
+ * with the last dimension contiguous; strides are in elements.  Parameters, their gradients, states, statistics and
+ * workspaces are float32.  Arithmetic is in float32, each result rounded once; sums have a fixed order (no atomics).
+ * Sequences may be padded: d_lens (int32 [batch], or NULL: all of `length`) gives each one's length, clamped to
+ * [0, length]; nothing behind it is read, and outputs and gradients there are zeros.                    */
+#define BOA_DT_F32 0
+#define BOA_DT_BF16 1
+#define BOA_DT_F16 2
+#define BOA_OPS_MAX_CHANNELS 65536
+
+/* Layer norm of rows of d values (nn.LayerNorm; model.py:45,51): y = (x - mean) / sqrt(var + eps) * w + b.  d_w and
+ * d_b may be NULL (1 and 0).  d_stats float32 [rows][2] receives mean and 1 / sqrt(var + eps) for the backward pass
+ * (NULL: not kept).  1 <= d <= BOA_LAYER_NORM_MAX_D.                                                    */
+#define BOA_LAYER_NORM_MAX_D 4096
+int boa_layer_norm_fwd(int dtype, const void* d_x, int64_t x_stride, const float* d_w, const float* d_b, int64_t rows,
+                       int32_t d, float eps, void* d_y, int64_t y_stride, float* d_stats, void* stream);
+/* Its gradient: d_dx [rows][d], and d_dwb float32 [2][d] (the weight's, then the bias's; NULL: not wanted), by way of
+ * d_work (boa_layer_norm_bwd_work_bytes).                                                               */
+int64_t boa_layer_norm_bwd_work_bytes(int64_t rows, int32_t d);
+int boa_layer_norm_bwd(int dtype, const void* d_dy, int64_t dy_stride, const void* d_x, int64_t x_stride, const float* d_w,
+                       const float* d_stats, int64_t rows, int32_t d, void* d_dx, int64_t dx_stride, float* d_dwb,
+                       void* d_work, int64_t work_bytes, void* stream);
+
+/* Cross entropy of rows of V logits against a target symbol each (F.cross_entropy as train.py:59-63 uses it, in nats).
+ * Targets are uint8, int32 or int64 (target_bytes 1, 4, 8); rows whose target is ignore_index count for nothing, a
+ * target outside [0, V) gives NaN.  d_losses float32 [rows] (may be NULL); d_loss and d_count, one float32 each (may both be
+ * NULL): the sum of the losses, or with `mean` their mean over the rows that count, and the number of those rows, by way of
+ * d_work (boa_cross_entropy_work_bytes).  d_stats float32 [rows][2] (may be NULL) is kept for the backward pass.
+ * 1 <= V <= BOA_CROSS_ENTROPY_MAX_V.                                                                    */
+#define BOA_CROSS_ENTROPY_MAX_V 4096
+int64_t boa_cross_entropy_work_bytes(void);
+int boa_cross_entropy_fwd(int dtype, const void* d_x, int64_t x_stride, const void* d_targets, int target_bytes,
+                          int64_t ignore_index, int64_t rows, int32_t V, int mean, float* d_stats, float* d_losses,
+                          float* d_loss, float* d_count, void* d_work, int64_t work_bytes, void* stream);
+/* Its gradient: d_dx = (softmax - onehot) * upstream.  d_up: float32 [rows] if up_rows, else one value; d_count:
+ * the forward's, for the mean (divided by the number of rows that count), or NULL.                      */
+int boa_cross_entropy_bwd(int dtype, const void* d_x, int64_t x_stride, const void* d_targets, int target_bytes,
+                          int64_t ignore_index, int64_t rows, int32_t V, const float* d_stats, const float* d_up,
+                          int up_rows, const float* d_count, void* d_dx, int64_t dx_stride, void* stream);
+
+/* Causal depthwise convolution over 4 positions with bias (d_b may be NULL) and, if silu, SiLU (the mixer's conv1d,
+ * model.py:72): x [batch][length][channels] -> y of the same shape.  d_w float32 [channels][4], oldest tap first.
+ * d_state_in [batch][3][channels] (x's type; NULL: zeros) holds the three positions before the first, oldest first;
+ * d_state_out (may be NULL; another buffer than d_state_in) receives those before each sequence's end.   */
+int boa_causal_conv_fwd(int dtype, const void* d_x, int64_t x_batch, int64_t x_row, const float* d_w, const float* d_b,
+                        int silu, int64_t batch, int64_t length, int32_t channels, const int32_t* d_lens,
+                        const void* d_state_in, void* d_state_out, void* d_y, int64_t y_batch, int64_t y_row, void* stream);
+/* Its gradient: d_dx, and d_dwb float32 [channels][4] then [channels] (the weight's and the bias's; NULL: not wanted).
+ * None for the state.                                                                                   */
+int64_t boa_causal_conv_bwd_work_bytes(int64_t batch, int64_t length, int32_t channels);
+int boa_causal_conv_bwd(int dtype, const void* d_dy, int64_t dy_batch, int64_t dy_row, const void* d_x, int64_t x_batch,
+                        int64_t x_row, const float* d_w, const float* d_b, int silu, int64_t batch, int64_t length,
+                        int32_t channels, const int32_t* d_lens, const void* d_state_in, void* d_dx, int64_t dx_batch,
+                        int64_t dx_row, float* d_dwb, void* d_work, int64_t work_bytes, void* stream);
+/* One position per sequence: x [batch][channels] -> y, d_state [batch][3][channels] shifted in place.    */
+int boa_causal_conv_step(int dtype, const void* d_x, int64_t x_stride, void* d_state, const float* d_w, const float* d_b,
+                         int silu, int64_t batch, int32_t channels, void* d_y, int64_t y_stride, void* stream);
+
+/* Selective scan (the mixer's state space recurrence, model.py:72-81) of 16 states per channel:
+ *   dt = softplus(delta + delta_bias), h_t = exp(dt a) h_(t-1) + dt b_t u_t, y_t = (c_t . h_t + d u_t) * silu(z_t)
+ * Members that a call does not use are ignored; those marked * may have a null pointer.                 */
+#define BOA_SCAN_MARK 8
+typedef struct boa_rows {
+    void* p;
+    int64_t batch_stride, row_stride;       /* elements */
+} boa_rows;
+typedef struct boa_scan {
+    int32_t dtype;                          /* of u, delta, z, b, c, y, dy and their gradients           */
+    int32_t channels;
+    int64_t batch, length;
+    boa_rows u, delta, z;                   /* [batch][length][channels]; z*: no gate                    */
+    boa_rows b, c;                          /* [batch][length][16]; 16-bit rows at multiples of 4 bytes  */
+    const float* a;                         /* [channels][16], negative                                  */
+    const float* d;                         /* * [channels]                                              */
+    const float* delta_bias;                /* * [channels]                                              */
+    const int32_t* lens;                    /* * [batch]                                                 */
+    const float* state_in;                  /* * [batch][16][channels] before the first position (zeros) */
+    float* state_out;                       /* * the same behind each sequence's last position           */
+    float* marks;                           /* [batch][ceil(length / BOA_SCAN_MARK)][16][channels]: states that the
+                                               forward pass leaves for the backward pass; * forward      */
+    boa_rows y;
+    boa_rows dy, du, ddelta, dz, db, dc;    /* backward; dz only with z                                  */
+    float* dpar;                            /* backward: [channels][16] of a, [channels] of d, [channels] of delta_bias */
+} boa_scan;
+/* Bytes of d_work that boa_selective_scan_fwd (backward = 0) or _bwd (1) needs for these sizes.          */
+int64_t boa_selective_scan_work_bytes(const boa_scan* s, int backward);
+int boa_selective_scan_fwd(const boa_scan* s, void* d_work, int64_t work_bytes, void* stream);
+/* The gradient for everything but the state.  Takes the forward's inputs and marks.                     */
+int boa_selective_scan_bwd(const boa_scan* s, void* d_work, int64_t work_bytes, void* stream);
+/* One position per sequence (length 1): advances state_out in place (lens, state_in and marks are not used). */
+int boa_selective_scan_step(const boa_scan* s, void* stream);
 
 #ifdef __cplusplus
 }
