@@ -107,21 +107,17 @@ def _grad(*ts):
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts)
 
 
-class _On:
-    """The device of a tensor made current for a call, where it is another."""
+_raw_stream, _device = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice  # cheaper than a torch.cuda.Stream
 
-    def __init__(self, t):
-        i = t.device.index
-        self.guard = None if i == torch.cuda.current_device() else torch.cuda.device(i)
 
-    def __enter__(self):
-        if self.guard is not None:
-            self.guard.__enter__()
-        return torch.cuda.current_stream().cuda_stream
-
-    def __exit__(self, *a):
-        if self.guard is not None:
-            self.guard.__exit__(*a)
+def _call(t, f, *args):
+    """An entry point (its last argument is the stream) on the current stream of a tensor's device, made current for it."""
+    i = t.device.index
+    if i == _device():
+        _nat.check(f(*args, _raw_stream(i)))
+    else:
+        with torch.cuda.device(i):
+            _nat.check(f(*args, _raw_stream(i)))
 
 
 def _ptr(t):
@@ -138,9 +134,8 @@ def _norm_fwd(x, w, b, eps, keep):
     rows = _rows(x.reshape(-1, d))
     y = torch.empty_like(x, memory_format=torch.contiguous_format)
     stats = torch.empty((rows.shape[0], 2), dtype=torch.float32, device=x.device) if keep else None
-    with _On(x) as s:
-        _nat.check(_nat.lib().boa_layer_norm_fwd(_DTYPES[x.dtype], rows.data_ptr(), rows.stride(0), _ptr(w), _ptr(b),
-                                                 rows.shape[0], d, eps, y.data_ptr(), d, _ptr(stats), s))
+    _call(x, _nat.lib().boa_layer_norm_fwd, _DTYPES[x.dtype], rows.data_ptr(), rows.stride(0), _ptr(w), _ptr(b), rows.shape[0], d,
+          eps, y.data_ptr(), d, _ptr(stats))
     return y, stats
 
 
@@ -162,11 +157,10 @@ class _LayerNorm(torch.autograd.Function):
         params = ctx.needs_input_grad[1] or ctx.needs_input_grad[2]
         dwb = torch.empty((2, d), dtype=torch.float32, device=x.device) if params else None
         lib = _nat.lib()
-        with _On(x) as s:
-            size = lib.boa_layer_norm_bwd_work_bytes(n, d) if params else 0
-            work = _work(size, x)
-            _nat.check(lib.boa_layer_norm_bwd(_DTYPES[x.dtype], dyr.data_ptr(), dyr.stride(0), rows.data_ptr(), rows.stride(0),
-                                              _ptr(w), stats.data_ptr(), n, d, dx.data_ptr(), d, _ptr(dwb), _ptr(work), size, s))
+        size = lib.boa_layer_norm_bwd_work_bytes(n, d) if params else 0
+        work = _work(size, x)
+        _call(x, lib.boa_layer_norm_bwd, _DTYPES[x.dtype], dyr.data_ptr(), dyr.stride(0), rows.data_ptr(), rows.stride(0), _ptr(w),
+              stats.data_ptr(), n, d, dx.data_ptr(), d, _ptr(dwb), _ptr(work), size)
         need = ctx.needs_input_grad
         return dx, dwb[0] if need[1] else None, dwb[1] if need[2] else None, None
 
@@ -197,12 +191,10 @@ class _CrossEntropy(torch.autograd.Function):
         each = torch.empty(n, dtype=torch.float32, device=x.device) if reduction == "none" else None
         loss, count = (torch.empty((), dtype=torch.float32, device=x.device) if each is None else None for _ in range(2))
         lib = _nat.lib()
-        with _On(x) as s:
-            size = lib.boa_cross_entropy_work_bytes() if each is None else 0
-            work = _work(size, x)
-            _nat.check(lib.boa_cross_entropy_fwd(_DTYPES[x.dtype], x.data_ptr(), x.stride(0), target.data_ptr(),
-                                                 target.element_size(), ignore, n, v, reduction == "mean", _ptr(stats),
-                                                 _ptr(each), _ptr(loss), _ptr(count), _ptr(work), size, s))
+        size = lib.boa_cross_entropy_work_bytes() if each is None else 0
+        work = _work(size, x)
+        _call(x, lib.boa_cross_entropy_fwd, _DTYPES[x.dtype], x.data_ptr(), x.stride(0), target.data_ptr(), target.element_size(),
+              ignore, n, v, reduction == "mean", _ptr(stats), _ptr(each), _ptr(loss), _ptr(count), _ptr(work), size)
         ctx.save_for_backward(x, target, stats, count)
         ctx.ignore, ctx.reduction = ignore, reduction
         return loss if each is None else each
@@ -214,11 +206,9 @@ class _CrossEntropy(torch.autograd.Function):
         n, v = x.shape
         up = up.to(torch.float32).contiguous()
         dx = torch.empty((n, v), dtype=x.dtype, device=x.device)
-        with _On(x) as s:
-            _nat.check(_nat.lib().boa_cross_entropy_bwd(_DTYPES[x.dtype], x.data_ptr(), x.stride(0), target.data_ptr(),
-                                                        target.element_size(), ctx.ignore, n, v, stats.data_ptr(), up.data_ptr(),
-                                                        ctx.reduction == "none", _ptr(count) if ctx.reduction == "mean" else 0,
-                                                        dx.data_ptr(), v, s))
+        _call(x, _nat.lib().boa_cross_entropy_bwd, _DTYPES[x.dtype], x.data_ptr(), x.stride(0), target.data_ptr(),
+              target.element_size(), ctx.ignore, n, v, stats.data_ptr(), up.data_ptr(), ctx.reduction == "none",
+              _ptr(count) if ctx.reduction == "mean" else 0, dx.data_ptr(), v)
         return dx, None, None, None, None
 
 
@@ -251,10 +241,8 @@ def _conv_fwd(x, w, b, silu, state, lens, want_state):
     n, length, c = x.shape
     y = torch.empty((n, length, c), dtype=x.dtype, device=x.device)
     out = torch.empty((n, D_CONV - 1, c), dtype=x.dtype, device=x.device) if want_state else None
-    with _On(x) as s:
-        _nat.check(_nat.lib().boa_causal_conv_fwd(_DTYPES[x.dtype], x.data_ptr(), x.stride(0), x.stride(1), w.data_ptr(), _ptr(b),
-                                                  silu, n, length, c, _ptr(lens), _ptr(state), _ptr(out), y.data_ptr(),
-                                                  length * c, c, s))
+    _call(x, _nat.lib().boa_causal_conv_fwd, _DTYPES[x.dtype], x.data_ptr(), x.stride(0), x.stride(1), w.data_ptr(), _ptr(b), silu,
+          n, length, c, _ptr(lens), _ptr(state), _ptr(out), y.data_ptr(), length * c, c)
     return y, out
 
 
@@ -278,12 +266,11 @@ class _CausalConv(torch.autograd.Function):
         params = ctx.needs_input_grad[1] or ctx.needs_input_grad[2]
         dwb = torch.empty((D_CONV + 1) * c, dtype=torch.float32, device=x.device) if params else None
         lib = _nat.lib()
-        with _On(x) as s:
-            size = lib.boa_causal_conv_bwd_work_bytes(n, length, c) if params else 0
-            work = _work(size, x)
-            _nat.check(lib.boa_causal_conv_bwd(_DTYPES[x.dtype], dy.data_ptr(), dy.stride(0), dy.stride(1), x.data_ptr(),
-                                               x.stride(0), x.stride(1), w.data_ptr(), _ptr(b), ctx.silu, n, length, c, _ptr(lens),
-                                               _ptr(state), dx.data_ptr(), length * c, c, _ptr(dwb), _ptr(work), size, s))
+        size = lib.boa_causal_conv_bwd_work_bytes(n, length, c) if params else 0
+        work = _work(size, x)
+        _call(x, lib.boa_causal_conv_bwd, _DTYPES[x.dtype], dy.data_ptr(), dy.stride(0), dy.stride(1), x.data_ptr(), x.stride(0),
+              x.stride(1), w.data_ptr(), _ptr(b), ctx.silu, n, length, c, _ptr(lens), _ptr(state), dx.data_ptr(), length * c, c,
+              _ptr(dwb), _ptr(work), size)
         need = ctx.needs_input_grad
         dw = dwb[:D_CONV * c].view(w.shape) if need[1] else None
         db = dwb[D_CONV * c:] if need[2] else None
@@ -336,9 +323,8 @@ def causal_conv_step(x, state, weight, bias=None, *, silu: bool = True):
     _gpu(who, x)
     x = _rows(x)
     y = torch.empty((n, c), dtype=x.dtype, device=x.device)
-    with _On(x) as s:
-        _nat.check(_nat.lib().boa_causal_conv_step(_DTYPES[x.dtype], x.data_ptr(), x.stride(0), state.data_ptr(), w.data_ptr(),
-                                                   _ptr(b), bool(silu), n, c, y.data_ptr(), c, s))
+    _call(x, _nat.lib().boa_causal_conv_step, _DTYPES[x.dtype], x.data_ptr(), x.stride(0), state.data_ptr(), w.data_ptr(), _ptr(b),
+          bool(silu), n, c, y.data_ptr(), c)
     return y
 
 
@@ -378,10 +364,9 @@ def _scan_fwd(u, delta, A, B, C, D, z, bias, state, lens, want_state, keep):
         marks = torch.empty((n, blocks, D_STATE, c), dtype=torch.float32, device=u.device)
     args = _pack(u, delta, A, B, C, D, z, bias, lens, state, out, marks, y)
     lib = _nat.lib()
-    with _On(u) as s:
-        size = lib.boa_selective_scan_work_bytes(args, 0)
-        work = _work(size, u)
-        _nat.check(lib.boa_selective_scan_fwd(args, _ptr(work), size, s))
+    size = lib.boa_selective_scan_work_bytes(args, 0)
+    work = _work(size, u)
+    _call(u, lib.boa_selective_scan_fwd, args, _ptr(work), size)
     return y, out, marks
 
 
@@ -407,10 +392,9 @@ class _SelectiveScan(torch.autograd.Function):
         dpar = torch.empty((D_STATE + 2) * c, dtype=torch.float32, device=u.device)
         args = _pack(u, delta, A, B, C, D, z, bias, lens, None, None, marks, None, (dy, du, ddelta, dz, dB, dC), dpar)
         lib = _nat.lib()
-        with _On(u) as s:
-            size = lib.boa_selective_scan_work_bytes(args, 1)
-            work = _work(size, u)
-            _nat.check(lib.boa_selective_scan_bwd(args, _ptr(work), size, s))
+        size = lib.boa_selective_scan_work_bytes(args, 1)
+        work = _work(size, u)
+        _call(u, lib.boa_selective_scan_bwd, args, _ptr(work), size)
         dA = dpar[:D_STATE * c].view(c, D_STATE)
         dD = dpar[D_STATE * c:(D_STATE + 1) * c] if D is not None else None
         dbias = dpar[(D_STATE + 1) * c:] if bias is not None else None
@@ -476,6 +460,5 @@ def selective_scan_step(u, delta, A, B, C, D=None, z=None, delta_bias=None, *, s
 
     packed = _SCAN.pack(_DTYPES[u.dtype], c, n, 1, *r2(u), *r2(delta), *r2(z), *r2(B), *r2(C), A.data_ptr(), _ptr(D), _ptr(bias),
                         0, 0, state.data_ptr(), 0, *r2(y), *(_NO_ROWS * 6), 0)
-    with _On(u) as s:
-        _nat.check(_nat.lib().boa_selective_scan_step(packed, s))
+    _call(u, _nat.lib().boa_selective_scan_step, packed)
     return y

@@ -329,7 +329,7 @@ extern "C" int boa_causal_conv_step(int dtype, const void* d_x, int64_t x_stride
     return with_vec(dtype, vec, [&](auto dt, auto v) {
         constexpr int DT = decltype(dt)::value, VEC = decltype(v)::value;
         const int64_t groups = ceil_div(batch * ceil_div(channels, VEC), WG);
-        if (groups > 0x7FFFFFFF) return boa_fail(BOA_ERR_ARG, "boa_causal_conv_step: batch too large");
+        if (groups > MAX_BLOCKS) return boa_fail(BOA_ERR_ARG, "boa_causal_conv_step: batch too large");
         hipLaunchKernelGGL((k_conv_step<DT, VEC>), dim3((uint32_t)groups), dim3(WG), 0, (hipStream_t)stream, d_x, x_stride,
                            d_state, d_w, d_b, batch, channels, silu, d_y, y_stride);
         BOA_HIP_TRY(hipGetLastError());

@@ -145,6 +145,9 @@ inline bool aligned16(int dtype, const void* p, int64_t stride) {
     return ((uintptr_t)p | (uintptr_t)(stride * es)) % 16 == 0;
 }
 
+// Workgroups of 256 threads that one launch dimension takes (its threads are counted in 32 bits).
+constexpr int64_t MAX_BLOCKS = 0xFFFFFF;
+
 // out[j] = sum over p < parts of part[p * width + j], j < width, in a fixed order (norm_op.hip).
 hipError_t launch_sum_parts(const float* part, int64_t parts, int64_t width, float* out, hipStream_t s);
 

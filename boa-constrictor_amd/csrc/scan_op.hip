@@ -39,9 +39,11 @@ struct ScanArgs {
     Rows u, delta, z, B, C, dy, y, du, ddelta, dz, dB, dC;
     const float *A, *D, *bias, *state_in;
     float *state_out, *marks, *part_bc, *part_par;
+    float *local, *dts;           // [batch][chunks][16][channels], [batch][chunks][channels]
     const int32_t* lens;
-    int channels, cblocks;
+    int channels, cblocks, chunks;
     int64_t batch, length, subs;  // subs: blocks of SUB positions of a sequence
+    int64_t chunk;                // positions of a chunk, a multiple of SUB
 };
 
 template <int DT>
@@ -72,6 +74,14 @@ __device__ __forceinline__ void scalar4(const typename Elem<DT>::T* p, float (&v
     }
 }
 
+// The same address, which the compiler takes for another: B and C are loaded again for the way back rather than kept (64
+// scalar registers per block).
+template <class T>
+__device__ __forceinline__ const T* again(const T* p) {
+    asm volatile("" : "+s"(p));
+    return p;
+}
+
 __device__ __forceinline__ int64_t end_of(const ScanArgs& a, int64_t b) {
     if (a.lens == nullptr) return a.length;
     const int64_t n = a.lens[b];
@@ -82,13 +92,15 @@ __device__ __forceinline__ int64_t end_of(const ScanArgs& a, int64_t b) {
 struct Place {
     int lane, q, c, cc;  // cc: c, or the last channel for the lanes past it (which take part with zeros)
     bool live;
-    int cb;
+    int cb, k;           // block of channels, chunk
     int64_t b;
-    __device__ __forceinline__ explicit Place(const ScanArgs& a) {
+    // chunks: how many of them this launch has, the first being `first`
+    __device__ __forceinline__ Place(const ScanArgs& a, int chunks, int first) {
         lane = threadIdx.x & 63;
         q = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
         cb = blockIdx.x % a.cblocks;
-        b = blockIdx.x / a.cblocks;
+        k = blockIdx.x / a.cblocks % chunks + first;
+        b = blockIdx.x / a.cblocks / chunks;
         c = cb * 64 + lane;
         live = c < a.channels;
         cc = live ? c : a.channels - 1;
@@ -104,69 +116,122 @@ __device__ __forceinline__ int64_t state_at(const ScanArgs& a, const Place& p, i
     return (r * NS + p.q * NQ + n) * a.channels + p.cc;
 }
 
-template <int DT>
+// h of this wavefront's states behind chunk j, from h before it.
+__device__ __forceinline__ void over_chunk(const ScanArgs& a, const Place& p, int j, const float (&a2)[NQ], float (&h)[NQ]) {
+    const int64_t r = p.b * a.chunks + j;
+    const float dts = a.dts[r * a.channels + p.cc];
+#pragma unroll
+    for (int n = 0; n < NQ; ++n)
+        h[n] = __builtin_fmaf(__builtin_amdgcn_exp2f(dts * a2[n]), h[n], a.local[state_at(a, p, r, n)]);
+}
+
+// LOCAL: the state that a chunk alone leaves (from zeros) and its sum of dt, for every chunk but the last; else the chunk's
+// outputs, from the state that the chunks before it leave.
+template <int DT, bool LOCAL>
 __global__ void __launch_bounds__(WG) k_scan_fwd(const ScanArgs a) {
-    __shared__ float2 s_in[SUB][64];  // dt, dt u
-    __shared__ float s_y[WAVES][SUB][64];
-    const Place p(a);
-    const int64_t end = end_of(a, p.b);
+    using E = Elem<DT>;
+    __shared__ float2 s_in[2][SUB][64];  // dt, dt u
+    __shared__ float s_y[2][LOCAL ? 1 : WAVES][SUB][64];
+    const Place p(a, LOCAL ? a.chunks - 1 : a.chunks, 0);
+    const int64_t end = end_of(a, p.b), lo = p.k * a.chunk;
+    if (LOCAL && lo + a.chunk >= end) return;  // no chunk behind this one reads its state
+    const int64_t hi = lo + a.chunk < a.length ? lo + a.chunk : a.length;  // rows to write
+    const int n_subs = lo < end ? (int)ceil_div((hi < end ? hi : end) - lo, SUB) : 0;
+    const bool gate = !LOCAL && a.z.p != nullptr;
     float a2[NQ], h[NQ];
     p.decay(a, a2);
-    const float bias = a.bias != nullptr ? a.bias[p.cc] : 0.0f, D = a.D != nullptr ? a.D[p.cc] : 0.0f;
+    const float bias = a.bias != nullptr ? a.bias[p.cc] : 0.0f, D = !LOCAL && a.D != nullptr ? a.D[p.cc] : 0.0f;
 #pragma unroll
-    for (int n = 0; n < NQ; ++n) h[n] = a.state_in != nullptr && p.live ? a.state_in[state_at(a, p, p.b, n)] : 0.0f;
+    for (int n = 0; n < NQ; ++n)
+        h[n] = !LOCAL && a.state_in != nullptr && p.live ? a.state_in[state_at(a, p, p.b, n)] : 0.0f;
 
-    const int64_t subs = ceil_div(end, SUB);
-    for (int64_t i = 0; i < subs; ++i) {
-        const int64_t t0 = i * SUB;
-        float u[MINE], z[MINE];
+    // A block's life: fetched (loads issued), prepared (dt and dt u to LDS), computed, finished (sums over the wavefronts'
+    // states, gate, stores).  One barrier per block: block i is computed while i - 1 is finished and i + 1 prepared, with
+    // two buffers each.
+    typename E::T ru[MINE], rd[MINE], rz[MINE];
+    auto fetch = [&](int i) {
+#pragma unroll
+        for (int k = 0; k < MINE; ++k) {
+            const int64_t t = min(lo + i * SUB + p.q * MINE + k, end - 1);
+            ru[k] = row<DT>(a.u, p.b, t)[p.cc];
+            rd[k] = row<DT>(a.delta, p.b, t)[p.cc];
+            if (gate) rz[k] = row<DT>(a.z, p.b, t)[p.cc];
+        }
+    };
+    float u[MINE] = {}, z[MINE] = {}, u_before[MINE], z_before[MINE];
+    auto prepare = [&](int i) {
 #pragma unroll
         for (int k = 0; k < MINE; ++k) {
             const int at = p.q * MINE + k;
-            const int64_t t = t0 + at < end ? t0 + at : end - 1;
-            u[k] = Elem<DT>::ld(row<DT>(a.u, p.b, t)[p.cc]);
-            z[k] = a.z.p != nullptr ? Elem<DT>::ld(row<DT>(a.z, p.b, t)[p.cc]) : 0.0f;
-            float dt = hw_softplus(Elem<DT>::ld(row<DT>(a.delta, p.b, t)[p.cc]) + bias);
-            if (t0 + at >= end || !p.live) dt = u[k] = 0.0f;  // the state stays as it is
-            s_in[at][p.lane] = make_float2(dt, dt * u[k]);
+            u[k] = E::ld(ru[k]);
+            if (gate) z[k] = E::ld(rz[k]);
+            float dt = hw_softplus(E::ld(rd[k]) + bias);
+            if (lo + i * SUB + at >= end || !p.live) dt = u[k] = 0.0f;  // the state stays as it is
+            s_in[i & 1][at][p.lane] = make_float2(dt, dt * u[k]);
         }
-        if (a.marks != nullptr && p.live)
+    };
+    auto finish = [&](int i) {
 #pragma unroll
-            for (int n = 0; n < NQ; ++n) a.marks[state_at(a, p, p.b * a.subs + i, n)] = h[n];
+        for (int k = 0; k < MINE; ++k) {
+            const int at = p.q * MINE + k;
+            const int64_t t = lo + i * SUB + at;
+            float y = D * u_before[k];
+#pragma unroll
+            for (int w = 0; w < WAVES; ++w) y += s_y[i & 1][LOCAL ? 0 : w][at][p.lane];
+            if (gate) y *= hw_silu(z_before[k]);
+            if (p.live && t < hi) row_mut<DT>(a.y, p.b, t)[p.c] = E::st(t < end ? y : 0.0f);
+        }
+    };
+    if (n_subs > 0) {
+        fetch(0);
+        if (!LOCAL)
+            for (int j = 0; j < p.k; ++j) over_chunk(a, p, j, a2, h);
+        prepare(0);
+        if (n_subs > 1) fetch(1);
+    }
+    float dts = 0.0f;
+    for (int i = 0; i < n_subs; ++i) {
         __syncthreads();
+        if (!LOCAL && a.marks != nullptr && p.live)
+#pragma unroll
+            for (int n = 0; n < NQ; ++n) a.marks[state_at(a, p, p.b * a.subs + lo / SUB + i, n)] = h[n];
 #pragma unroll
         for (int s = 0; s < SUB; ++s) {
-            const int64_t t = t0 + s < end ? t0 + s : end - 1;
+            const int64_t t = min(lo + i * SUB + s, end - 1);
             float B[NQ], C[NQ];
             scalar4<DT>(row<DT>(a.B, p.b, t) + p.q * NQ, B);
-            scalar4<DT>(row<DT>(a.C, p.b, t) + p.q * NQ, C);
-            const float2 in = s_in[s][p.lane];
+            if constexpr (!LOCAL) scalar4<DT>(row<DT>(a.C, p.b, t) + p.q * NQ, C);
+            const float2 in = s_in[i & 1][s][p.lane];
             float y = 0.0f;
 #pragma unroll
             for (int n = 0; n < NQ; ++n) {
                 h[n] = __builtin_fmaf(__builtin_amdgcn_exp2f(in.x * a2[n]), h[n], B[n] * in.y);
-                y = __builtin_fmaf(h[n], C[n], y);
+                if constexpr (!LOCAL) y = __builtin_fmaf(h[n], C[n], y);
             }
-            s_y[p.q][s][p.lane] = y;
+            if constexpr (LOCAL) dts += in.x;
+            else s_y[i & 1][p.q][s][p.lane] = y;
         }
-        __syncthreads();
+        if (!LOCAL && i > 0) finish(i - 1);
 #pragma unroll
-        for (int k = 0; k < MINE; ++k) {
-            const int at = p.q * MINE + k;
-            const int64_t t = t0 + at;
-            float y = D * u[k];
-#pragma unroll
-            for (int w = 0; w < WAVES; ++w) y += s_y[w][at][p.lane];
-            if (a.z.p != nullptr) y *= hw_silu(z[k]);
-            if (p.live && t < a.length) row_mut<DT>(a.y, p.b, t)[p.c] = Elem<DT>::st(t < end ? y : 0.0f);
-        }
-        __syncthreads();
+        for (int k = 0; k < MINE; ++k) u_before[k] = u[k], z_before[k] = z[k];
+        if (i + 1 < n_subs) prepare(i + 1);
+        if (i + 2 < n_subs) fetch(i + 2);
     }
-    if (p.live) {
-        if (a.state_out != nullptr)
+    if constexpr (LOCAL) {
+        if (!p.live) return;
+        const int64_t r = p.b * a.chunks + p.k;
+#pragma unroll
+        for (int n = 0; n < NQ; ++n) a.local[state_at(a, p, r, n)] = h[n];
+        if (p.q == 0) a.dts[r * a.channels + p.c] = dts;
+    } else {
+        __syncthreads();
+        if (n_subs > 0) finish(n_subs - 1);
+        if (!p.live) return;
+        // the state behind the last position: from the chunk that has it, without positions from the first
+        if (a.state_out != nullptr && (end > lo || lo == 0) && end <= lo + a.chunk)
 #pragma unroll
             for (int n = 0; n < NQ; ++n) a.state_out[state_at(a, p, p.b, n)] = h[n];
-        for (int64_t t = subs * SUB + p.q; t < a.length; t += WAVES) row_mut<DT>(a.y, p.b, t)[p.c] = Elem<DT>::st(0.0f);
+        for (int64_t t = lo + (int64_t)n_subs * SUB + p.q; t < hi; t += WAVES) row_mut<DT>(a.y, p.b, t)[p.c] = E::st(0.0f);
     }
 }
 
@@ -191,35 +256,111 @@ __device__ __forceinline__ float sum8(float (&v)[8], int lane) {
     return keep;
 }
 
+// What the backward pass prepares of a position: loaded, then dt, dt u, g and the factors that finishing it needs.
+template <int DT, bool LOCAL>
+struct BackIn {
+    using E = Elem<DT>;
+    typename E::T ru[MINE], rd[MINE], rz[MINE], ry[MINE];
+    __device__ __forceinline__ void fetch(const ScanArgs& a, const Place& p, int64_t t0, int64_t end) {
+#pragma unroll
+        for (int k = 0; k < MINE; ++k) {
+            const int64_t t = min(t0 + p.q * MINE + k, end - 1);
+            if constexpr (!LOCAL) ru[k] = row<DT>(a.u, p.b, t)[p.cc];
+            rd[k] = row<DT>(a.delta, p.b, t)[p.cc];
+            ry[k] = row<DT>(a.dy, p.b, t)[p.cc];
+            if (a.z.p != nullptr) rz[k] = row<DT>(a.z, p.b, t)[p.cc];
+        }
+    }
+};
+
+// The adjoint of the state before a chunk that the chunk's own outputs give (dh from zeros behind it), and its sum of dt, for
+// every chunk but the first.
+template <int DT>
+__global__ void __launch_bounds__(WG) k_scan_bwd_local(const ScanArgs a) {
+    using E = Elem<DT>;
+    __shared__ float2 s_in[2][SUB][64];  // dt, g
+    const Place p(a, a.chunks - 1, 1);
+    const int64_t end = end_of(a, p.b), lo = p.k * a.chunk;
+    if (lo >= end) return;
+    const int n_subs = (int)ceil_div(min(lo + a.chunk, end) - lo, SUB);
+    float a2[NQ], dh[NQ] = {}, dts = 0.0f;
+    p.decay(a, a2);
+    const float bias = a.bias != nullptr ? a.bias[p.cc] : 0.0f;
+    BackIn<DT, true> in;
+    auto prepare = [&](int i) {
+#pragma unroll
+        for (int k = 0; k < MINE; ++k) {
+            const int at = p.q * MINE + k;
+            float dt = hw_softplus(E::ld(in.rd[k]) + bias), g = E::ld(in.ry[k]);
+            if (a.z.p != nullptr) g *= hw_silu(E::ld(in.rz[k]));
+            if (lo + i * SUB + at >= end || !p.live) dt = g = 0.0f;
+            s_in[i & 1][at][p.lane] = make_float2(dt, g);
+        }
+    };
+    in.fetch(a, p, lo + (n_subs - 1) * SUB, end);
+    prepare(n_subs - 1);
+    if (n_subs > 1) in.fetch(a, p, lo + (n_subs - 2) * SUB, end);
+    for (int i = n_subs - 1; i >= 0; --i) {
+        __syncthreads();
+#pragma unroll
+        for (int s = SUB - 1; s >= 0; --s) {
+            const int64_t t = min(lo + i * SUB + s, end - 1);
+            float C[NQ];
+            scalar4<DT>(row<DT>(a.C, p.b, t) + p.q * NQ, C);
+            const float2 x = s_in[i & 1][s][p.lane];
+#pragma unroll
+            for (int n = 0; n < NQ; ++n) dh[n] = __builtin_fmaf(C[n], x.y, dh[n]) * __builtin_amdgcn_exp2f(x.x * a2[n]);
+            dts += x.x;
+        }
+        if (i > 0) prepare(i - 1);
+        if (i > 1) in.fetch(a, p, lo + (i - 2) * SUB, end);
+    }
+    if (!p.live) return;
+    const int64_t r = p.b * a.chunks + p.k;
+#pragma unroll
+    for (int n = 0; n < NQ; ++n) a.local[state_at(a, p, r, n)] = dh[n];
+    if (p.q == 0) a.dts[r * a.channels + p.c] = dts;
+}
+
 template <int DT>
 __global__ void __launch_bounds__(WG) k_scan_bwd(const ScanArgs a) {
+    using E = Elem<DT>;
     __shared__ float2 s_in[SUB][64];  // dt, dt u
     __shared__ float s_g[SUB][64];
     __shared__ float s_y[WAVES][SUB][64], s_s[WAVES][SUB][64], s_w[WAVES][SUB][64];  // partial sums over the states
-    const Place p(a);
-    const int64_t end = end_of(a, p.b);
+    const Place p(a, a.chunks, 0);
+    const int64_t end = end_of(a, p.b), lo = p.k * a.chunk;
+    const int64_t hi = min(lo + a.chunk, a.length);
+    const int n_subs = lo < end ? (int)ceil_div(min(hi, end) - lo, SUB) : 0;
+    const bool gate = a.z.p != nullptr;
     float a2[NQ], dh[NQ] = {}, dA[NQ] = {}, dA_all[NQ] = {};
     p.decay(a, a2);
     const float bias = a.bias != nullptr ? a.bias[p.cc] : 0.0f, D = a.D != nullptr ? a.D[p.cc] : 0.0f;
-    float dD = 0.0f, dbias = 0.0f;
-
-    const int64_t subs = ceil_div(end, SUB);
-    for (int64_t i = subs - 1; i >= 0; --i) {
-        const int64_t t0 = i * SUB;
+    float dD = 0.0f, dbias = 0.0f, mark[NQ] = {};
+    BackIn<DT, false> in;
+    auto fetch = [&](int i) {
+        in.fetch(a, p, lo + i * SUB, end);
+#pragma unroll
+        for (int n = 0; n < NQ; ++n) mark[n] = p.live ? a.marks[state_at(a, p, p.b * a.subs + lo / SUB + i, n)] : 0.0f;
+    };
+    if (n_subs > 0) {
+        fetch(n_subs - 1);
+        for (int j = (int)ceil_div(end, a.chunk) - 1; j > p.k; --j) over_chunk(a, p, j, a2, dh);
+    }
+    for (int i = n_subs - 1; i >= 0; --i) {
+        const int64_t t0 = lo + i * SUB;
         float u[MINE], dt[MINE], g[MINE], sig[MINE], dyz[MINE];
 #pragma unroll
         for (int k = 0; k < MINE; ++k) {
             const int at = p.q * MINE + k;
-            const int64_t t = t0 + at < end ? t0 + at : end - 1;
-            u[k] = Elem<DT>::ld(row<DT>(a.u, p.b, t)[p.cc]);
-            const float dy = Elem<DT>::ld(row<DT>(a.dy, p.b, t)[p.cc]);
-            const float pre = Elem<DT>::ld(row<DT>(a.delta, p.b, t)[p.cc]) + bias;
+            u[k] = E::ld(in.ru[k]);
+            const float dy = E::ld(in.ry[k]), pre = E::ld(in.rd[k]) + bias;
             dt[k] = hw_softplus(pre);
             sig[k] = hw_sigmoid(pre);
             g[k] = dy;
             dyz[k] = 0.0f;
-            if (a.z.p != nullptr) {
-                const float z = Elem<DT>::ld(row<DT>(a.z, p.b, t)[p.cc]), sz = hw_sigmoid(z);
+            if (gate) {
+                const float z = E::ld(in.rz[k]), sz = hw_sigmoid(z);
                 g[k] = dy * (z * sz);
                 dyz[k] = dy * __builtin_fmaf(z * sz, 1.0f - sz, sz);
             }
@@ -229,23 +370,24 @@ __global__ void __launch_bounds__(WG) k_scan_bwd(const ScanArgs a) {
         }
         float h[NQ], e[SUB][NQ], eh[SUB][NQ], bc = 0.0f;
 #pragma unroll
-        for (int n = 0; n < NQ; ++n) h[n] = p.live ? a.marks[state_at(a, p, p.b * a.subs + i, n)] : 0.0f;
+        for (int n = 0; n < NQ; ++n) h[n] = mark[n];
+        if (i > 0) fetch(i - 1);
         __syncthreads();
         float r[8];
 #pragma unroll
         for (int s = 0; s < SUB; ++s) {
-            const int64_t t = t0 + s < end ? t0 + s : end - 1;
+            const int64_t t = min(t0 + s, end - 1);
             float B[NQ], C[NQ];
             scalar4<DT>(row<DT>(a.B, p.b, t) + p.q * NQ, B);
             scalar4<DT>(row<DT>(a.C, p.b, t) + p.q * NQ, C);
-            const float2 in = s_in[s][p.lane];
+            const float2 x = s_in[s][p.lane];
             const float gs = s_g[s][p.lane];
             float y = 0.0f;
 #pragma unroll
             for (int n = 0; n < NQ; ++n) {
-                e[s][n] = __builtin_amdgcn_exp2f(in.x * a2[n]);
+                e[s][n] = __builtin_amdgcn_exp2f(x.x * a2[n]);
                 eh[s][n] = e[s][n] * h[n];
-                h[n] = __builtin_fmaf(B[n], in.y, eh[s][n]);
+                h[n] = __builtin_fmaf(B[n], x.y, eh[s][n]);
                 y = __builtin_fmaf(h[n], C[n], y);
                 r[(s & 1) * NQ + n] = gs * h[n];
             }
@@ -257,21 +399,21 @@ __global__ void __launch_bounds__(WG) k_scan_bwd(const ScanArgs a) {
         }
 #pragma unroll
         for (int s = SUB - 1; s >= 0; --s) {
-            const int64_t t = t0 + s < end ? t0 + s : end - 1;
+            const int64_t t = min(t0 + s, end - 1);
             float B[NQ], C[NQ];
-            scalar4<DT>(row<DT>(a.B, p.b, t) + p.q * NQ, B);
-            scalar4<DT>(row<DT>(a.C, p.b, t) + p.q * NQ, C);
-            const float2 in = s_in[s][p.lane];
+            scalar4<DT>(again(row<DT>(a.B, p.b, t) + p.q * NQ), B);
+            scalar4<DT>(again(row<DT>(a.C, p.b, t) + p.q * NQ), C);
+            const float2 x = s_in[s][p.lane];
             const float gs = s_g[s][p.lane];
             float sB = 0.0f, sw = 0.0f;
 #pragma unroll
             for (int n = 0; n < NQ; ++n) {
                 dh[n] = __builtin_fmaf(C[n], gs, dh[n]);
                 sB = __builtin_fmaf(dh[n], B[n], sB);
-                r[(s & 1) * NQ + n] = dh[n] * in.y;
+                r[(s & 1) * NQ + n] = dh[n] * x.y;
                 const float w = dh[n] * eh[s][n];
                 sw = __builtin_fmaf(w, a2[n], sw);
-                dA[n] = __builtin_fmaf(w, in.x, dA[n]);
+                dA[n] = __builtin_fmaf(w, x.x, dA[n]);
                 dh[n] *= e[s][n];
             }
             s_s[p.q][s][p.lane] = sB;
@@ -281,7 +423,7 @@ __global__ void __launch_bounds__(WG) k_scan_bwd(const ScanArgs a) {
                 bc = (p.lane & 7) == SUB / 2 + s / 2 ? v : bc;
             }
         }
-        a.part_bc[(((int64_t)p.cb * a.batch + p.b) * a.subs + i) * WG + threadIdx.x] = bc;
+        a.part_bc[(((int64_t)p.cb * a.batch + p.b) * a.subs + lo / SUB + i) * WG + threadIdx.x] = bc;
         __syncthreads();
 #pragma unroll
         for (int k = 0; k < MINE; ++k) {
@@ -297,10 +439,10 @@ __global__ void __launch_bounds__(WG) k_scan_bwd(const ScanArgs a) {
             const float ddelta = __builtin_fmaf(u[k], sB, sw * LN2) * sig[k], du = __builtin_fmaf(dt[k], sB, D * g[k]);
             dD = __builtin_fmaf(g[k], u[k], dD);
             dbias += ddelta;
-            if (p.live && t < a.length) {
-                row_mut<DT>(a.du, p.b, t)[p.c] = Elem<DT>::st(t < end ? du : 0.0f);
-                row_mut<DT>(a.ddelta, p.b, t)[p.c] = Elem<DT>::st(t < end ? ddelta : 0.0f);
-                if (a.z.p != nullptr) row_mut<DT>(a.dz, p.b, t)[p.c] = Elem<DT>::st(t < end ? dyz[k] * y : 0.0f);
+            if (p.live && t < hi) {
+                row_mut<DT>(a.du, p.b, t)[p.c] = E::st(t < end ? du : 0.0f);
+                row_mut<DT>(a.ddelta, p.b, t)[p.c] = E::st(t < end ? ddelta : 0.0f);
+                if (gate) row_mut<DT>(a.dz, p.b, t)[p.c] = E::st(t < end ? dyz[k] * y : 0.0f);
             }
         }
         if (i % 8 == 0)  // sums of 64 positions at a time: a long sum in one register loses digits
@@ -311,18 +453,18 @@ __global__ void __launch_bounds__(WG) k_scan_bwd(const ScanArgs a) {
             }
         __syncthreads();
     }
-    for (int64_t t = subs * SUB + p.q; t < a.length; t += WAVES)
-        if (p.live) {
-            row_mut<DT>(a.du, p.b, t)[p.c] = Elem<DT>::st(0.0f);
-            row_mut<DT>(a.ddelta, p.b, t)[p.c] = Elem<DT>::st(0.0f);
-            if (a.z.p != nullptr) row_mut<DT>(a.dz, p.b, t)[p.c] = Elem<DT>::st(0.0f);
+    if (p.live)
+        for (int64_t t = lo + (int64_t)n_subs * SUB + p.q; t < hi; t += WAVES) {
+            row_mut<DT>(a.du, p.b, t)[p.c] = E::st(0.0f);
+            row_mut<DT>(a.ddelta, p.b, t)[p.c] = E::st(0.0f);
+            if (gate) row_mut<DT>(a.dz, p.b, t)[p.c] = E::st(0.0f);
         }
-    // this sequence's sums for the parameters: [channels][16] of A, [channels] of D, [channels] of the bias
+    // this chunk's sums for the parameters: [channels][16] of A, [channels] of D, [channels] of the bias
     s_s[p.q][0][p.lane] = dD;
     s_s[p.q][1][p.lane] = dbias;
     __syncthreads();
     if (!p.live) return;
-    float* mine = a.part_par + p.b * (NS + 2) * a.channels;
+    float* mine = a.part_par + (p.b * a.chunks + p.k) * (NS + 2) * a.channels;
 #pragma unroll
     for (int n = 0; n < NQ; ++n) mine[(int64_t)p.c * NS + p.q * NQ + n] = dA_all[n];
     if (p.q < 2) {
@@ -337,13 +479,15 @@ __global__ void __launch_bounds__(WG) k_scan_bwd(const ScanArgs a) {
 template <int DT>
 __global__ void __launch_bounds__(WG) k_scan_sum_bc(const ScanArgs a) {
     const int lane = threadIdx.x & 63, q = threadIdx.x >> 6;
-    const int64_t b = blockIdx.x / a.subs, i = blockIdx.x % a.subs;
-    const int64_t end = end_of(a, b), t = i * SUB + (lane & 3) * 2 + (lane >> 5);
-    if (t >= a.length) return;
-    float v = 0.0f;
-    if (t < end)
-        for (int cb = 0; cb < a.cblocks; ++cb) v += a.part_bc[(((int64_t)cb * a.batch + b) * a.subs + i) * WG + threadIdx.x];
-    row_mut<DT>((lane & 4) ? a.dB : a.dC, b, t)[q * NQ + ((lane >> 3) & 3)] = Elem<DT>::st(v);
+    for (int64_t k = blockIdx.x; k < a.batch * a.subs; k += gridDim.x) {
+        const int64_t b = k / a.subs, i = k % a.subs;
+        const int64_t end = end_of(a, b), t = i * SUB + (lane & 3) * 2 + (lane >> 5);
+        if (t >= a.length) continue;
+        float v = 0.0f;
+        if (t < end)
+            for (int cb = 0; cb < a.cblocks; ++cb) v += a.part_bc[(((int64_t)cb * a.batch + b) * a.subs + i) * WG + threadIdx.x];
+        row_mut<DT>((lane & 4) ? a.dB : a.dC, b, t)[q * NQ + ((lane >> 3) & 3)] = Elem<DT>::st(v);
+    }
 }
 
 // One position: a lane has the 16 states of its channel.
@@ -386,10 +530,46 @@ __global__ void __launch_bounds__(WG) k_scan_step(const ScanArgs a) {
 
 Rows rows(const boa_rows& r) { return {r.p, r.batch_stride, r.row_stride}; }
 
-int64_t bc_bytes(const boa_scan* s) {
-    return ceil_div(s->channels, 64) * s->batch * ceil_div(s->length, SUB) * WG * (int64_t)sizeof(float);
+// The split over the length: chunks of a multiple of SUB positions, as many as give WANT workgroups (4 per CU), at least
+// MIN_CHUNK positions each and at most MAX_CHUNKS (each workgroup goes over the chunks before its own).
+struct Plan {
+    int chunks;
+    int64_t chunk;
+};
+constexpr int64_t WANT = 1024, MIN_CHUNK = 64, MAX_CHUNKS = 64;
+Plan plan(const boa_scan* s) {
+    const int64_t blocks = s->batch * ceil_div(s->channels, 64);
+    int64_t n = ceil_div(WANT, blocks > 0 ? blocks : 1);
+    n = n < MAX_CHUNKS ? n : MAX_CHUNKS;
+    int64_t chunk = ceil_div(ceil_div(s->length, n), SUB) * SUB;
+    chunk = chunk > MIN_CHUNK ? chunk : MIN_CHUNK;
+    n = ceil_div(s->length, chunk);
+    return {(int)(n > 1 ? n : 1), chunk};
 }
-int64_t par_bytes(const boa_scan* s) { return s->batch * (NS + 2) * (int64_t)s->channels * (int64_t)sizeof(float); }
+
+// Workspace, in floats: chunk states and sums of dt (more than one chunk), then in the backward pass the partial sums.
+struct Work {
+    int64_t local, dts, bc, par;
+    int64_t bytes() const { return (local + dts + bc + par) * (int64_t)sizeof(float); }
+};
+Work work_of(const boa_scan* s, bool backward) {
+    Work w = {};
+    if (s->batch < 1 || s->length < 1) return w;
+    const Plan p = plan(s);
+    const int64_t c = s->channels;
+    if (p.chunks > 1) w.local = s->batch * p.chunks * NS * c, w.dts = s->batch * p.chunks * c;
+    if (backward) {
+        w.bc = ceil_div(c, 64) * s->batch * ceil_div(s->length, SUB) * WG;
+        w.par = s->batch * p.chunks * (NS + 2) * c;
+    }
+    return w;
+}
+void lay_out(ScanArgs& a, const Work& w, void* d_work) {
+    a.local = static_cast<float*>(d_work);
+    a.dts = a.local + w.local;
+    a.part_bc = a.dts + w.dts;
+    a.part_par = a.part_bc + w.bc;
+}
 
 // B and C rows are read four values at a time at uniform addresses, which have to be multiples of 4 bytes.
 bool bc_aligned(const boa_scan* s, const boa_rows& r) {
@@ -412,7 +592,9 @@ int check_scan(const char* who, const boa_scan* s, ScanArgs& a) {
     a.A = s->a, a.D = s->d, a.bias = s->delta_bias, a.lens = s->lens, a.state_in = s->state_in, a.state_out = s->state_out;
     a.marks = s->marks, a.channels = s->channels, a.cblocks = (int)ceil_div(s->channels, 64);
     a.batch = s->batch, a.length = s->length, a.subs = ceil_div(s->length, SUB);
-    if (a.batch * a.cblocks > 0x7FFFFFFF || a.batch * a.subs > 0x7FFFFFFF)
+    const Plan pl = plan(s);
+    a.chunks = pl.chunks, a.chunk = pl.chunk;
+    if (a.batch > MAX_BLOCKS / ((int64_t)a.cblocks * a.chunks))
         return boa_fail(BOA_ERR_ARG, "%s: batch of %lld sequences too large", who, (long long)a.batch);
     return BOA_OK;
 }
@@ -421,7 +603,7 @@ int check_scan(const char* who, const boa_scan* s, ScanArgs& a) {
 
 extern "C" int64_t boa_selective_scan_work_bytes(const boa_scan* s, int backward) {
     if (!s || s->batch < 1 || s->length < 1 || s->channels < 1) return 0;
-    return backward ? bc_bytes(s) + par_bytes(s) : 0;
+    return work_of(s, backward != 0).bytes();
 }
 
 extern "C" int boa_selective_scan_fwd(const boa_scan* s, void* d_work, int64_t work_bytes, void* stream) {
@@ -430,9 +612,19 @@ extern "C" int boa_selective_scan_fwd(const boa_scan* s, void* d_work, int64_t w
     if (rc != BOA_OK) return rc;
     if (a.batch == 0 || (a.length == 0 && !a.state_out)) return BOA_OK;
     if (a.length > 0 && !a.y.p) return boa_fail(BOA_ERR_ARG, "boa_selective_scan_fwd: null pointer");
+    const Work w = work_of(s, false);
+    if (w.bytes() > 0 && (!d_work || work_bytes < w.bytes()))
+        return boa_fail(BOA_ERR_ARG, "boa_selective_scan_fwd: workspace of %lld bytes, needs %lld", (long long)work_bytes,
+                        (long long)w.bytes());
+    lay_out(a, w, d_work);
     return with_dtype(s->dtype, [&](auto dt) {
-        hipLaunchKernelGGL((k_scan_fwd<decltype(dt)::value>), dim3((uint32_t)(a.batch * a.cblocks)), dim3(WG), 0,
-                           (hipStream_t)stream, a);
+        constexpr int DT = decltype(dt)::value;
+        const uint32_t blocks = (uint32_t)(a.batch * a.cblocks);
+        if (a.chunks > 1) {
+            hipLaunchKernelGGL((k_scan_fwd<DT, true>), dim3(blocks * (a.chunks - 1)), dim3(WG), 0, (hipStream_t)stream, a);
+            BOA_HIP_TRY(hipGetLastError());
+        }
+        hipLaunchKernelGGL((k_scan_fwd<DT, false>), dim3(blocks * a.chunks), dim3(WG), 0, (hipStream_t)stream, a);
         BOA_HIP_TRY(hipGetLastError());
         return (int)BOA_OK;
     });
@@ -446,26 +638,30 @@ extern "C" int boa_selective_scan_bwd(const boa_scan* s, void* d_work, int64_t w
     if (!s->dpar) return boa_fail(BOA_ERR_ARG, "boa_selective_scan_bwd: null pointer");
     if (any && (!s->dy.p || !s->du.p || !s->ddelta.p || !s->db.p || !s->dc.p || !s->marks || (s->z.p && !s->dz.p)))
         return boa_fail(BOA_ERR_ARG, "boa_selective_scan_bwd: null pointer");
-    const int64_t need = boa_selective_scan_work_bytes(s, 1);
-    if (any && (!d_work || work_bytes < need))
+    const Work w = work_of(s, true);
+    if (any && (!d_work || work_bytes < w.bytes()))
         return boa_fail(BOA_ERR_ARG, "boa_selective_scan_bwd: workspace of %lld bytes, needs %lld", (long long)work_bytes,
-                        (long long)need);
+                        (long long)w.bytes());
     hipStream_t st = (hipStream_t)stream;
-    a.part_bc = static_cast<float*>(d_work);
-    a.part_par = any ? a.part_bc + bc_bytes(s) / (int64_t)sizeof(float) : nullptr;
+    lay_out(a, w, d_work);
     if (any) {
         a.dy = rows(s->dy), a.du = rows(s->du), a.ddelta = rows(s->ddelta), a.dz = rows(s->dz), a.dB = rows(s->db), a.dC = rows(s->dc);
         const int launched = with_dtype(s->dtype, [&](auto dt) {
             constexpr int DT = decltype(dt)::value;
-            hipLaunchKernelGGL((k_scan_bwd<DT>), dim3((uint32_t)(a.batch * a.cblocks)), dim3(WG), 0, st, a);
+            const uint32_t blocks = (uint32_t)(a.batch * a.cblocks);
+            if (a.chunks > 1) {
+                hipLaunchKernelGGL((k_scan_bwd_local<DT>), dim3(blocks * (a.chunks - 1)), dim3(WG), 0, st, a);
+                BOA_HIP_TRY(hipGetLastError());
+            }
+            hipLaunchKernelGGL((k_scan_bwd<DT>), dim3(blocks * a.chunks), dim3(WG), 0, st, a);
             BOA_HIP_TRY(hipGetLastError());
-            hipLaunchKernelGGL((k_scan_sum_bc<DT>), dim3((uint32_t)(a.batch * a.subs)), dim3(WG), 0, st, a);
+            hipLaunchKernelGGL((k_scan_sum_bc<DT>), dim3((uint32_t)min(a.batch * a.subs, MAX_BLOCKS)), dim3(WG), 0, st, a);
             BOA_HIP_TRY(hipGetLastError());
             return (int)BOA_OK;
         });
         if (launched != BOA_OK) return launched;
     }
-    BOA_HIP_TRY(launch_sum_parts(a.part_par, any ? a.batch : 0, (int64_t)(NS + 2) * a.channels, s->dpar, st));
+    BOA_HIP_TRY(launch_sum_parts(a.part_par, any ? a.batch * a.chunks : 0, (int64_t)(NS + 2) * a.channels, s->dpar, st));
     return BOA_OK;
 }
 
