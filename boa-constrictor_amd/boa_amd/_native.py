@@ -33,6 +33,7 @@ BOA_LAYER_NORM_MAX_D = 4096
 BOA_CROSS_ENTROPY_MAX_V = 4096
 BOA_OPS_MAX_CHANNELS = 65536
 BOA_SCAN_MARK = 8
+BOA_SCAN_MAX_ROW_STRIDE = 67108863
 
 
 class BoaError(RuntimeError):

@@ -346,9 +346,15 @@ def _pack(u, delta, A, B, C, D, z, bias, lens, state_in, state_out, marks, y, ba
                       *_r3(back[2]), *_r3(back[3]), *_r3(back[4]), *_r3(back[5]), _ptr(dpar))
 
 
-def _scalar_rows(t):
-    """B or C as the kernels read them: rows of a 16-bit type begin at multiples of 4 bytes."""
+def _scan_rows(t):
+    """Rows as the kernels read them: contiguous, not too far apart."""
     t = _rows(t)
+    return t if t.stride(-2) <= _nat.BOA_SCAN_MAX_ROW_STRIDE else t.contiguous()
+
+
+def _scalar_rows(t):
+    """The same for B and C, whose rows begin at multiples of 4 bytes."""
+    t = _scan_rows(t)
     if t.element_size() == 2 and (t.data_ptr() % 4 or any(s % 2 for s in t.stride()[:-1])):
         t = t.clone(memory_format=torch.contiguous_format)
     return t
@@ -384,7 +390,7 @@ class _SelectiveScan(torch.autograd.Function):
     def backward(ctx, dy, _):
         u, delta, A, B, C, D, z, bias, lens, marks = ctx.saved_tensors
         n, length, c = u.shape
-        dy = _rows(dy)
+        dy = _scan_rows(dy)
         du, ddelta = torch.empty_like(dy, memory_format=torch.contiguous_format), torch.empty_like(
             dy, memory_format=torch.contiguous_format)
         dz = torch.empty_like(dy, memory_format=torch.contiguous_format) if z is not None else None
@@ -417,7 +423,11 @@ def _scan_args(who, ndim, u, delta, A, B, C, D, z, bias):
     if A is None:
         raise TypeError(f"{who}: A must be a float32 tensor")
     D, bias = _param(who, "D", D, torch.Size((c,)), u), _param(who, "delta_bias", bias, torch.Size((c,)), u)
-    return _rows(u), _rows(delta), A, _scalar_rows(B), _scalar_rows(C), D, None if z is None else _rows(z), bias
+    if ndim == 3:
+        u, delta, z = _scan_rows(u), _scan_rows(delta), None if z is None else _scan_rows(z)
+    else:
+        u, delta, z = _rows(u), _rows(delta), None if z is None else _rows(z)
+    return u, delta, A, _scalar_rows(B), _scalar_rows(C), D, z, bias
 
 
 def selective_scan(u, delta, A, B, C, D=None, z=None, delta_bias=None, *, state=None, lens=None, return_state: bool = False):

@@ -25,6 +25,12 @@ using namespace boa;
 
 namespace {
 
+#ifndef BWDW
+#define BWDW 4
+#endif
+#ifndef FETCH_AT
+#define FETCH_AT 4
+#endif
 constexpr int NS = 16, WAVES = 4, NQ = NS / WAVES;
 constexpr int SUB = BOA_SCAN_MARK, MINE = SUB / WAVES;  // positions of a block, and those a wavefront prepares and finishes
 constexpr int WG = 64 * WAVES;
@@ -55,31 +61,88 @@ __device__ __forceinline__ typename Elem<DT>::T* row_mut(const Rows& a, int64_t 
     return static_cast<typename Elem<DT>::T*>(const_cast<void*>(a.p)) + b * a.b + t * a.r;
 }
 
-// Four consecutive values at a uniform address through the scalar cache (constant address space: nothing the kernel
-// writes; 16-bit rows are 4-byte aligned, which the entry points check).
+// This wavefront's states of B or C in the rows of a block, through the scalar cache (constant address space: nothing the
+// kernel writes; 16-bit rows are 4-byte aligned, and a block of rows spans less than 2 GiB, which the entry points check).
+// A row's place is a 32-bit offset from the block's first: one scalar multiplication, where 64-bit addresses of single rows
+// cost ten scalar instructions, more than the vector work of a row.
 template <int DT>
-__device__ __forceinline__ void scalar4(const typename Elem<DT>::T* p, float (&v)[NQ]) {
-    typedef __attribute__((address_space(4))) const uint32_t CWord;
-    CWord* w = (CWord*)p;
-    if constexpr (DT == DT_F32) {
+struct ScalarRows {
+    static constexpr int WORDS = NQ * (int)sizeof(typename Elem<DT>::T) / 4;
+    const char* p;   // the block's first row
+    uint32_t bytes;  // of a row
+    __device__ __forceinline__ ScalarRows(const Rows& a, int64_t b, int64_t t, int q)
+        : p((const char*)(row<DT>(a, b, t) + q * NQ)), bytes((uint32_t)a.r * (uint32_t)sizeof(typename Elem<DT>::T)) {}
+    __device__ __forceinline__ void ahead() { p += bytes * SUB; }
+    __device__ __forceinline__ void back() { p -= bytes * SUB; }
+    __device__ __forceinline__ void load(int s, uint32_t (&w)[WORDS]) const {
+        typedef __attribute__((address_space(4))) const char CByte;
+        typedef __attribute__((address_space(4))) const uint32_t CWord;
+        CWord* at = (CWord*)((CByte*)p + (uint32_t)s * bytes);
 #pragma unroll
-        for (int i = 0; i < NQ; ++i) v[i] = __uint_as_float(w[i]);
-    } else {
-#pragma unroll
-        for (int i = 0; i < NQ / 2; ++i) {
-            const uint32_t x = w[i];
-            v[2 * i] = Elem<DT>::ld((uint16_t)(x & 0xFFFFu));
-            v[2 * i + 1] = Elem<DT>::ld((uint16_t)(x >> 16));
-        }
+        for (int i = 0; i < WORDS; ++i) w[i] = at[i];
     }
+    static __device__ __forceinline__ float value(const uint32_t (&w)[WORDS], int n) {
+        if constexpr (DT == DT_F32) return __uint_as_float(w[n]);
+        else return Elem<DT>::ld((uint16_t)(n & 1 ? w[n / 2] >> 16 : w[n / 2] & 0xFFFFu));
+    }
+};
+
+// Two positions of a block as the recurrence reads them: B and C from the scalar cache, what was prepared from LDS.  A pair is
+// on its way while the one before it is computed.  Both kinds of load return out of order to one counter, so a wait is for
+// all that are under way: the pair to compute is waited for (here) before the next one is issued.
+template <int DT>
+struct Pair {
+    using S = ScalarRows<DT>;
+    uint32_t B[2][S::WORDS], C[2][S::WORDS];
+    float2 in[2];
+    float g[2];
+    __device__ __forceinline__ void here() {
+        asm volatile("" : "+v"(in[0].x), "+v"(in[0].y), "+v"(in[1].x), "+v"(in[1].y));
+    }
+    static __device__ __forceinline__ void words_here(uint32_t (&w)[2][S::WORDS]) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int i = 0; i < S::WORDS; ++i) asm volatile("" : "+s"(w[j][i]));
+    }
+    __device__ __forceinline__ float b(int j, int n) const { return S::value(B[j], n); }
+    __device__ __forceinline__ float c(int j, int n) const { return S::value(C[j], n); }
+};
+
+// The rows of a block that lanes read or write, each lane its channel: the same 32-bit offsets from the block's first row.
+template <int DT>
+struct LaneRows {
+    using T = typename Elem<DT>::T;
+    gmut<char> p;    // the block's first row
+    uint32_t bytes;  // of a row
+    __device__ __forceinline__ LaneRows(const Rows& a, int64_t b, int64_t t)
+        : p((gmut<char>)row_mut<DT>(a, b, t)), bytes((uint32_t)a.r * (uint32_t)sizeof(T)) {}
+    __device__ __forceinline__ void ahead(bool on) { p += on ? bytes * SUB : 0; }
+    __device__ __forceinline__ void back(bool on) { p -= on ? bytes * SUB : 0; }
+    // c: the lane's channel in bytes (a 32-bit offset in bytes from a uniform address: no address arithmetic in the lanes)
+    __device__ __forceinline__ gmut<T> at(int s, uint32_t c) const { return (gmut<T>)(p + (uint32_t)s * bytes + c); }
+    __device__ __forceinline__ T load(int s, uint32_t c) const { return *at(s, c); }
+    __device__ __forceinline__ void store(int s, uint32_t c, float v) const { *at(s, c) = Elem<DT>::st(v); }
+};
+
+// Element `c4` bytes from p: the same for float32 arrays.
+__device__ __forceinline__ gmut<float> lane_at(gmut<float> p, uint32_t c4) { return (gmut<float>)((gmut<char>)p + c4); }
+__device__ __forceinline__ gptr<float> lane_at(gptr<float> p, uint32_t c4) { return (gptr<float>)((gptr<char>)p + c4); }
+
+// A lane offset that the compiler takes for a new one: it would add it to the rows' addresses ahead of the loop and keep those
+// in vector registers, two for each array.
+__device__ __forceinline__ uint32_t fresh(uint32_t c) {
+    asm volatile("" : "+v"(c));
+    return c;
 }
 
-// The same address, which the compiler takes for another: B and C are loaded again for the way back rather than kept (64
-// scalar registers per block).
-template <class T>
-__device__ __forceinline__ const T* again(const T* p) {
-    asm volatile("" : "+s"(p));
-    return p;
+// A loaded value in a register of its own.  Where a float32 value is used later than the next block's load is issued, the
+// compiler otherwise takes the loaded register over, loads into another, and waits for that load at the end of the iteration
+// to move it into place.
+__device__ __forceinline__ float own_register(float v) {
+    float r;
+    asm volatile("v_mov_b32 %0, %1" : "=v"(r) : "v"(v));
+    return r;
 }
 
 __device__ __forceinline__ int64_t end_of(const ScanArgs& a, int64_t b) {
@@ -90,7 +153,8 @@ __device__ __forceinline__ int64_t end_of(const ScanArgs& a, int64_t b) {
 
 // Where a workgroup is: its channels, its sequence, this wavefront's states.
 struct Place {
-    int lane, q, c, cc;  // cc: c, or the last channel for the lanes past it (which take part with zeros)
+    int lane, q, c;
+    uint32_t cc;         // c, or the last channel for the lanes past it
     bool live;
     int cb, k;           // block of channels, chunk
     int64_t b;
@@ -103,11 +167,11 @@ struct Place {
         b = blockIdx.x / a.cblocks / chunks;
         c = cb * 64 + lane;
         live = c < a.channels;
-        cc = live ? c : a.channels - 1;
+        cc = (uint32_t)(live ? c : a.channels - 1);
     }
     __device__ __forceinline__ void decay(const ScanArgs& a, float (&a2)[NQ]) const {
 #pragma unroll
-        for (int n = 0; n < NQ; ++n) a2[n] = live ? a.A[(int64_t)cc * NS + q * NQ + n] * LOG2E : 0.0f;
+        for (int n = 0; n < NQ; ++n) a2[n] = a.A[(int64_t)cc * NS + q * NQ + n] * LOG2E;
     }
 };
 
@@ -116,108 +180,154 @@ __device__ __forceinline__ int64_t state_at(const ScanArgs& a, const Place& p, i
     return (r * NS + p.q * NQ + n) * a.channels + p.cc;
 }
 
-// h of this wavefront's states behind chunk j, from h before it.
-__device__ __forceinline__ void over_chunk(const ScanArgs& a, const Place& p, int j, const float (&a2)[NQ], float (&h)[NQ]) {
-    const int64_t r = p.b * a.chunks + j;
-    const float dts = a.dts[r * a.channels + p.cc];
+// h of this wavefront's states over the chunks j, j + step .. (n of them), the loads of four chunks in flight.
+__device__ __forceinline__ void over_chunks(const ScanArgs& a, const Place& p, int j, int step, int n_chunks, const float (&a2)[NQ],
+                                            float (&h)[NQ]) {
+    constexpr int AT_ONCE = 4;
+    for (int i0 = 0; i0 < n_chunks; i0 += AT_ONCE) {
+        float dts[AT_ONCE], l[AT_ONCE][NQ];
 #pragma unroll
-    for (int n = 0; n < NQ; ++n)
-        h[n] = __builtin_fmaf(__builtin_amdgcn_exp2f(dts * a2[n]), h[n], a.local[state_at(a, p, r, n)]);
+        for (int i = 0; i < AT_ONCE; ++i) {
+            const int64_t r = p.b * a.chunks + j + step * min(i0 + i, n_chunks - 1);
+            dts[i] = (a.dts + r * a.channels)[p.cc];
+#pragma unroll
+            for (int n = 0; n < NQ; ++n) l[i][n] = (a.local + (r * NS + p.q * NQ + n) * a.channels)[p.cc];
+        }
+#pragma unroll
+        for (int i = 0; i < AT_ONCE; ++i)
+            if (i0 + i < n_chunks)
+#pragma unroll
+                for (int n = 0; n < NQ; ++n) h[n] = __builtin_fmaf(__builtin_amdgcn_exp2f(dts[i] * a2[n]), h[n], l[i][n]);
+    }
 }
 
-// LOCAL: the state that a chunk alone leaves (from zeros) and its sum of dt, for every chunk but the last; else the chunk's
-// outputs, from the state that the chunks before it leave.
-template <int DT, bool LOCAL>
+// What a wave has to do with memory in a block is the same in every block, without branches: the hardware counts loads and
+// stores together in order, and behind a store that may or may not have been issued the compiler waits for all of them (a
+// block then takes a store's way to memory and back).  So lanes behind the last channel do what the last one does, a block
+// behind the last one is fetched as the last one, and without a gate z is u.
+enum { LOCAL, OUT, OUT_MARKS };
+
+// LOCAL: the state that a chunk alone leaves (from zeros) and its sum of dt, for every chunk but the last; OUT: the chunk's
+// outputs, from the state that the chunks before it leave; OUT_MARKS: and the state before every block.
+template <int DT, int MODE>
 __global__ void __launch_bounds__(WG) k_scan_fwd(const ScanArgs a) {
     using E = Elem<DT>;
     __shared__ float2 s_in[2][SUB][64];  // dt, dt u
-    __shared__ float s_y[2][LOCAL ? 1 : WAVES][SUB][64];
-    const Place p(a, LOCAL ? a.chunks - 1 : a.chunks, 0);
+    __shared__ float s_y[2][MODE == LOCAL ? 1 : WAVES][SUB][64];
+    const Place p(a, MODE == LOCAL ? a.chunks - 1 : a.chunks, 0);
     const int64_t end = end_of(a, p.b), lo = p.k * a.chunk;
-    if (LOCAL && lo + a.chunk >= end) return;  // no chunk behind this one reads its state
+    if (MODE == LOCAL && lo + a.chunk >= end) return;  // no chunk behind this one reads its state
     const int64_t hi = lo + a.chunk < a.length ? lo + a.chunk : a.length;  // rows to write
     const int n_subs = lo < end ? (int)ceil_div((hi < end ? hi : end) - lo, SUB) : 0;
-    const bool gate = !LOCAL && a.z.p != nullptr;
+    const bool gate = a.z.p != nullptr;
     float a2[NQ], h[NQ];
     p.decay(a, a2);
-    const float bias = a.bias != nullptr ? a.bias[p.cc] : 0.0f, D = !LOCAL && a.D != nullptr ? a.D[p.cc] : 0.0f;
+    const float bias = a.bias != nullptr ? a.bias[p.cc] : 0.0f, D = MODE != LOCAL && a.D != nullptr ? a.D[p.cc] : 0.0f;
 #pragma unroll
-    for (int n = 0; n < NQ; ++n)
-        h[n] = !LOCAL && a.state_in != nullptr && p.live ? a.state_in[state_at(a, p, p.b, n)] : 0.0f;
+    for (int n = 0; n < NQ; ++n) h[n] = MODE != LOCAL && a.state_in != nullptr ? a.state_in[state_at(a, p, p.b, n)] : 0.0f;
 
     // A block's life: fetched (loads issued), prepared (dt and dt u to LDS), computed, finished (sums over the wavefronts'
     // states, gate, stores).  One barrier per block: block i is computed while i - 1 is finished and i + 1 prepared, with
     // two buffers each.
+    const int first = p.q * MINE;  // this wavefront's first position of a block
+    uint32_t ce = p.cc * (uint32_t)sizeof(typename E::T), c4 = p.cc * 4;  // the lane's channel in bytes
+    LaneRows<DT> xu(a.u, p.b, lo), xd(a.delta, p.b, lo), xz(gate ? a.z : a.u, p.b, lo), xy(a.y, p.b, lo);
+    ScalarRows<DT> xB(a.B, p.b, lo, p.q), xC(a.C, p.b, lo, p.q);
+    gmut<float> mark = GM(a.marks) + ((p.b * a.subs + lo / SUB) * NS + p.q * NQ) * a.channels;
+    const int count = (int)(min(hi, end) - lo), rows_out = (int)(hi - lo);  // positions inside, rows to write
     typename E::T ru[MINE], rd[MINE], rz[MINE];
-    auto fetch = [&](int i) {
+    auto fetch = [&](int i) {  // i < n_subs
 #pragma unroll
         for (int k = 0; k < MINE; ++k) {
-            const int64_t t = min(lo + i * SUB + p.q * MINE + k, end - 1);
-            ru[k] = row<DT>(a.u, p.b, t)[p.cc];
-            rd[k] = row<DT>(a.delta, p.b, t)[p.cc];
-            if (gate) rz[k] = row<DT>(a.z, p.b, t)[p.cc];
+            const int s = min(first + k, count - 1 - i * SUB);
+            ru[k] = xu.load(s, ce);
+            rd[k] = xd.load(s, ce);
+            if (MODE != LOCAL) rz[k] = xz.load(s, ce);
         }
     };
-    float u[MINE] = {}, z[MINE] = {}, u_before[MINE], z_before[MINE];
-    auto prepare = [&](int i) {
+    auto prepare = [&](int i, float (&u)[MINE], float (&z)[MINE]) {
 #pragma unroll
         for (int k = 0; k < MINE; ++k) {
-            const int at = p.q * MINE + k;
-            u[k] = E::ld(ru[k]);
-            if (gate) z[k] = E::ld(rz[k]);
-            float dt = hw_softplus(E::ld(rd[k]) + bias);
-            if (lo + i * SUB + at >= end || !p.live) dt = u[k] = 0.0f;  // the state stays as it is
-            s_in[i & 1][at][p.lane] = make_float2(dt, dt * u[k]);
+            u[k] = MODE != LOCAL ? own_register(E::ld(ru[k])) : E::ld(ru[k]);
+            if (MODE != LOCAL) z[k] = own_register(E::ld(rz[k]));
+            const float dt = hw_softplus(E::ld(rd[k]) + bias);
+            // behind the end the state stays as it is
+            s_in[i & 1][first + k][p.lane] = i * SUB + first + k < count ? make_float2(dt, dt * u[k]) : make_float2(0.0f, 0.0f);
         }
     };
-    auto finish = [&](int i) {
+    // whole: all the block's positions are inside
+    auto finish = [&](int i, const float (&u)[MINE], const float (&z)[MINE], bool whole) {
 #pragma unroll
         for (int k = 0; k < MINE; ++k) {
-            const int at = p.q * MINE + k;
-            const int64_t t = lo + i * SUB + at;
-            float y = D * u_before[k];
+            const int at = first + k;
+            float y = D * u[k];
 #pragma unroll
-            for (int w = 0; w < WAVES; ++w) y += s_y[i & 1][LOCAL ? 0 : w][at][p.lane];
-            if (gate) y *= hw_silu(z_before[k]);
-            if (p.live && t < hi) row_mut<DT>(a.y, p.b, t)[p.c] = E::st(t < end ? y : 0.0f);
+            for (int w = 0; w < WAVES; ++w) y += s_y[i & 1][MODE == LOCAL ? 0 : w][at][p.lane];
+            y *= gate ? hw_silu(z[k]) : 1.0f;
+            if (whole || i * SUB + at < rows_out) xy.store(at, ce, whole || i * SUB + at < count ? y : 0.0f);
         }
+        xy.ahead(true);
     };
+    float u[MINE], z[MINE], u_before[MINE], z_before[MINE], u_next[MINE], z_next[MINE], dts = 0.0f;
     if (n_subs > 0) {
         fetch(0);
-        if (!LOCAL)
-            for (int j = 0; j < p.k; ++j) over_chunk(a, p, j, a2, h);
-        prepare(0);
-        if (n_subs > 1) fetch(1);
+        if (MODE != LOCAL) over_chunks(a, p, 0, 1, p.k, a2, h);
+        prepare(0, u, z);
+        const bool more = n_subs > 1;
+        xu.ahead(more), xd.ahead(more), xz.ahead(more);
+        fetch(more);
     }
-    float dts = 0.0f;
     for (int i = 0; i < n_subs; ++i) {
+        ce = fresh(ce), c4 = fresh(c4);
         __syncthreads();
-        if (!LOCAL && a.marks != nullptr && p.live)
+        if constexpr (MODE == OUT_MARKS) {
 #pragma unroll
-            for (int n = 0; n < NQ; ++n) a.marks[state_at(a, p, p.b * a.subs + lo / SUB + i, n)] = h[n];
-#pragma unroll
-        for (int s = 0; s < SUB; ++s) {
-            const int64_t t = min(lo + i * SUB + s, end - 1);
-            float B[NQ], C[NQ];
-            scalar4<DT>(row<DT>(a.B, p.b, t) + p.q * NQ, B);
-            if constexpr (!LOCAL) scalar4<DT>(row<DT>(a.C, p.b, t) + p.q * NQ, C);
-            const float2 in = s_in[i & 1][s][p.lane];
-            float y = 0.0f;
-#pragma unroll
-            for (int n = 0; n < NQ; ++n) {
-                h[n] = __builtin_fmaf(__builtin_amdgcn_exp2f(in.x * a2[n]), h[n], B[n] * in.y);
-                if constexpr (!LOCAL) y = __builtin_fmaf(h[n], C[n], y);
-            }
-            if constexpr (LOCAL) dts += in.x;
-            else s_y[i & 1][p.q][s][p.lane] = y;
+            for (int n = 0; n < NQ; ++n) *lane_at(mark + (uint32_t)(n * a.channels), c4) = h[n];
+            mark += NS * a.channels;
         }
-        if (!LOCAL && i > 0) finish(i - 1);
+        const int last = min(SUB, count - i * SUB) - 1;  // rows behind the end are read as the last one
+        Pair<DT> pair[2];
+        auto issue = [&](int s0, Pair<DT>& x) {
 #pragma unroll
-        for (int k = 0; k < MINE; ++k) u_before[k] = u[k], z_before[k] = z[k];
-        if (i + 1 < n_subs) prepare(i + 1);
-        if (i + 2 < n_subs) fetch(i + 2);
+            for (int j = 0; j < 2; ++j) {
+                xB.load(min(s0 + j, last), x.B[j]);
+                if constexpr (MODE != LOCAL) xC.load(min(s0 + j, last), x.C[j]);
+                x.in[j] = s_in[i & 1][s0 + j][p.lane];
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        };
+        issue(0, pair[0]);
+        if (MODE != LOCAL && i > 0) finish(i - 1, u_before, z_before, true);
+#pragma unroll
+        for (int s0 = 0; s0 < SUB; s0 += 2) {
+            Pair<DT>& x = pair[s0 / 2 % 2];
+            x.here(), x.words_here(x.B);
+            if constexpr (MODE != LOCAL) x.words_here(x.C);
+            if (s0 + 2 < SUB) issue(s0 + 2, pair[s0 / 2 % 2 ^ 1]);
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                float y = 0.0f;
+#pragma unroll
+                for (int n = 0; n < NQ; ++n) {
+                    h[n] = __builtin_fmaf(__builtin_amdgcn_exp2f(x.in[j].x * a2[n]), h[n], x.b(j, n) * x.in[j].y);
+                    if constexpr (MODE != LOCAL) y = __builtin_fmaf(h[n], x.c(j, n), y);
+                }
+                if constexpr (MODE == LOCAL) dts += x.in[j].x;
+                else s_y[i & 1][p.q][s0 + j][p.lane] = y;
+            }
+        }
+        xB.ahead(), xC.ahead();
+        prepare(i + 1, u_next, z_next);
+        const bool more = i + 2 < n_subs;
+        xu.ahead(more), xd.ahead(more), xz.ahead(more);
+        fetch(min(i + 2, n_subs - 1));
+#pragma unroll
+        for (int k = 0; k < MINE; ++k) {
+            u_before[k] = u[k], z_before[k] = z[k];
+            u[k] = u_next[k], z[k] = z_next[k];
+        }
     }
-    if constexpr (LOCAL) {
+    if constexpr (MODE == LOCAL) {
         if (!p.live) return;
         const int64_t r = p.b * a.chunks + p.k;
 #pragma unroll
@@ -225,7 +335,7 @@ __global__ void __launch_bounds__(WG) k_scan_fwd(const ScanArgs a) {
         if (p.q == 0) a.dts[r * a.channels + p.c] = dts;
     } else {
         __syncthreads();
-        if (n_subs > 0) finish(n_subs - 1);
+        if (n_subs > 0) finish(n_subs - 1, u_before, z_before, false);
         if (!p.live) return;
         // the state behind the last position: from the chunk that has it, without positions from the first
         if (a.state_out != nullptr && (end > lo || lo == 0) && end <= lo + a.chunk)
@@ -256,19 +366,34 @@ __device__ __forceinline__ float sum8(float (&v)[8], int lane) {
     return keep;
 }
 
-// What the backward pass prepares of a position: loaded, then dt, dt u, g and the factors that finishing it needs.
-template <int DT, bool LOCAL>
+// The same rows, which the compiler takes for others: on the way back B and C are loaded again rather than kept (64 scalar
+// registers per block, moved to and from vector registers for want of so many).
+template <int DT>
+__device__ __forceinline__ ScalarRows<DT> again(ScalarRows<DT> x) {
+    asm volatile("" : "+s"(x.p));
+    return x;
+}
+
+// What the backward pass loads of a block's positions, from the chunk's last block to its first.
+template <int DT, bool LOCAL_>
 struct BackIn {
     using E = Elem<DT>;
+    LaneRows<DT> xu, xd, xz, xy;
     typename E::T ru[MINE], rd[MINE], rz[MINE], ry[MINE];
-    __device__ __forceinline__ void fetch(const ScanArgs& a, const Place& p, int64_t t0, int64_t end) {
+    int first;  // this wavefront's first position of a block
+    // t: the first position of the block to start with; without a gate z is dy
+    __device__ __forceinline__ BackIn(const ScanArgs& a, const Place& p, int64_t t)
+        : xu(a.u, p.b, t), xd(a.delta, p.b, t), xz(a.z.p != nullptr ? a.z : a.dy, p.b, t), xy(a.dy, p.b, t), first(p.q * MINE) {}
+    __device__ __forceinline__ void back(bool on) { xu.back(on), xd.back(on), xz.back(on), xy.back(on); }
+    // left: positions from the block's first one to the end
+    __device__ __forceinline__ void fetch(int left, uint32_t ce) {
 #pragma unroll
         for (int k = 0; k < MINE; ++k) {
-            const int64_t t = min(t0 + p.q * MINE + k, end - 1);
-            if constexpr (!LOCAL) ru[k] = row<DT>(a.u, p.b, t)[p.cc];
-            rd[k] = row<DT>(a.delta, p.b, t)[p.cc];
-            ry[k] = row<DT>(a.dy, p.b, t)[p.cc];
-            if (a.z.p != nullptr) rz[k] = row<DT>(a.z, p.b, t)[p.cc];
+            const int s = min(first + k, left - 1);  // rows behind the end are read as the last one
+            if constexpr (!LOCAL_) ru[k] = xu.load(s, ce);
+            rd[k] = xd.load(s, ce);
+            ry[k] = xy.load(s, ce);
+            rz[k] = xz.load(s, ce);
         }
     }
 };
@@ -286,34 +411,54 @@ __global__ void __launch_bounds__(WG) k_scan_bwd_local(const ScanArgs a) {
     float a2[NQ], dh[NQ] = {}, dts = 0.0f;
     p.decay(a, a2);
     const float bias = a.bias != nullptr ? a.bias[p.cc] : 0.0f;
-    BackIn<DT, true> in;
+    const int count = (int)(min(lo + a.chunk, end) - lo);
+    const bool gate = a.z.p != nullptr;
+    uint32_t ce = p.cc * (uint32_t)sizeof(typename E::T);
+    BackIn<DT, true> in(a, p, lo + (n_subs - 1) * SUB);
+    ScalarRows<DT> xC(a.C, p.b, lo + (n_subs - 1) * SUB, p.q);
     auto prepare = [&](int i) {
 #pragma unroll
         for (int k = 0; k < MINE; ++k) {
-            const int at = p.q * MINE + k;
-            float dt = hw_softplus(E::ld(in.rd[k]) + bias), g = E::ld(in.ry[k]);
-            if (a.z.p != nullptr) g *= hw_silu(E::ld(in.rz[k]));
-            if (lo + i * SUB + at >= end || !p.live) dt = g = 0.0f;
-            s_in[i & 1][at][p.lane] = make_float2(dt, g);
+            const int at = in.first + k;
+            const float dt = hw_softplus(E::ld(in.rd[k]) + bias), g = E::ld(in.ry[k]) * (gate ? hw_silu(E::ld(in.rz[k])) : 1.0f);
+            s_in[i & 1][at][p.lane] = i * SUB + at < count ? make_float2(dt, g) : make_float2(0.0f, 0.0f);
         }
     };
-    in.fetch(a, p, lo + (n_subs - 1) * SUB, end);
+    in.fetch(count - (n_subs - 1) * SUB, ce);
     prepare(n_subs - 1);
-    if (n_subs > 1) in.fetch(a, p, lo + (n_subs - 2) * SUB, end);
+    in.back(n_subs > 1);
+    in.fetch(n_subs > 1 ? SUB : count, ce);
     for (int i = n_subs - 1; i >= 0; --i) {
+        ce = fresh(ce);
         __syncthreads();
+        const int last = min(SUB, count - i * SUB) - 1;  // rows behind the end are read as the last one
+        Pair<DT> pair[2];
+        auto issue = [&](int s0, Pair<DT>& x) {
 #pragma unroll
-        for (int s = SUB - 1; s >= 0; --s) {
-            const int64_t t = min(lo + i * SUB + s, end - 1);
-            float C[NQ];
-            scalar4<DT>(row<DT>(a.C, p.b, t) + p.q * NQ, C);
-            const float2 x = s_in[i & 1][s][p.lane];
+            for (int j = 0; j < 2; ++j) {
+                xC.load(min(s0 + j, last), x.C[j]);
+                x.in[j] = s_in[i & 1][s0 + j][p.lane];
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        };
+        issue(SUB - 2, pair[0]);
 #pragma unroll
-            for (int n = 0; n < NQ; ++n) dh[n] = __builtin_fmaf(C[n], x.y, dh[n]) * __builtin_amdgcn_exp2f(x.x * a2[n]);
-            dts += x.x;
+        for (int s0 = SUB - 2; s0 >= 0; s0 -= 2) {
+            Pair<DT>&x = pair[(SUB - 2 - s0) / 2 % 2], &next = pair[(SUB - s0) / 2 % 2];
+            x.here(), x.words_here(x.C);
+            if (s0 > 0) issue(s0 - 2, next);
+#pragma unroll
+            for (int j = 1; j >= 0; --j) {
+#pragma unroll
+                for (int n = 0; n < NQ; ++n)
+                    dh[n] = __builtin_fmaf(x.c(j, n), x.in[j].y, dh[n]) * __builtin_amdgcn_exp2f(x.in[j].x * a2[n]);
+                dts += x.in[j].x;
+            }
         }
+        xC.back();
         if (i > 0) prepare(i - 1);
-        if (i > 1) in.fetch(a, p, lo + (i - 2) * SUB, end);
+        in.back(i > 1);
+        in.fetch(min(SUB, count), ce);
     }
     if (!p.live) return;
     const int64_t r = p.b * a.chunks + p.k;
@@ -322,13 +467,15 @@ __global__ void __launch_bounds__(WG) k_scan_bwd_local(const ScanArgs a) {
     if (p.q == 0) a.dts[r * a.channels + p.c] = dts;
 }
 
-template <int DT>
-__global__ void __launch_bounds__(WG) k_scan_bwd(const ScanArgs a) {
+// ALL: every lane has a channel (channels a multiple of 64), so the stores need no lane mask.
+template <int DT, bool ALL>
+__global__ void __launch_bounds__(WG, BWDW) k_scan_bwd(const ScanArgs a) {
     using E = Elem<DT>;
     __shared__ float2 s_in[SUB][64];  // dt, dt u
     __shared__ float s_g[SUB][64];
     __shared__ float s_y[WAVES][SUB][64], s_s[WAVES][SUB][64], s_w[WAVES][SUB][64];  // partial sums over the states
     const Place p(a, a.chunks, 0);
+    const bool live = ALL || p.live;
     const int64_t end = end_of(a, p.b), lo = p.k * a.chunk;
     const int64_t hi = min(lo + a.chunk, a.length);
     const int n_subs = lo < end ? (int)ceil_div(min(hi, end) - lo, SUB) : 0;
@@ -336,99 +483,122 @@ __global__ void __launch_bounds__(WG) k_scan_bwd(const ScanArgs a) {
     float a2[NQ], dh[NQ] = {}, dA[NQ] = {}, dA_all[NQ] = {};
     p.decay(a, a2);
     const float bias = a.bias != nullptr ? a.bias[p.cc] : 0.0f, D = a.D != nullptr ? a.D[p.cc] : 0.0f;
-    float dD = 0.0f, dbias = 0.0f, mark[NQ] = {};
-    BackIn<DT, false> in;
-    auto fetch = [&](int i) {
-        in.fetch(a, p, lo + i * SUB, end);
+    float dD = 0.0f, dbias = 0.0f, mark[NQ];
+    const int count = (int)(min(hi, end) - lo), rows_out = (int)(hi - lo);
+    const int64_t t_last = lo + (int64_t)max(n_subs - 1, 0) * SUB;  // the block to start with
+    uint32_t ce = p.cc * (uint32_t)sizeof(typename E::T), c4 = p.cc * 4;  // the lane's channel in bytes
+    BackIn<DT, false> in(a, p, t_last);
+    LaneRows<DT> yu(a.du, p.b, t_last), yd(a.ddelta, p.b, t_last), yz(gate ? a.dz : a.du, p.b, t_last);
+    ScalarRows<DT> xB(a.B, p.b, t_last, p.q), xC(a.C, p.b, t_last, p.q);
+    gptr<float> marks = G(a.marks) + ((p.b * a.subs + t_last / SUB) * NS + p.q * NQ) * a.channels;
+    gmut<float> bc_out = GM(a.part_bc) + (((int64_t)p.cb * a.batch + p.b) * a.subs + t_last / SUB) * WG;
+    auto fetch = [&](int left) {
+        in.fetch(left, ce);
 #pragma unroll
-        for (int n = 0; n < NQ; ++n) mark[n] = p.live ? a.marks[state_at(a, p, p.b * a.subs + lo / SUB + i, n)] : 0.0f;
+        for (int n = 0; n < NQ; ++n) mark[n] = *lane_at(marks + (uint32_t)(n * a.channels), c4);
     };
-    if (n_subs > 0) {
-        fetch(n_subs - 1);
-        for (int j = (int)ceil_div(end, a.chunk) - 1; j > p.k; --j) over_chunk(a, p, j, a2, dh);
-    }
-    for (int i = n_subs - 1; i >= 0; --i) {
-        const int64_t t0 = lo + i * SUB;
-        float u[MINE], dt[MINE], g[MINE], sig[MINE], dyz[MINE];
+    // whole: all the block's positions are inside (all blocks but the first one here)
+    auto block = [&](int i, auto whole) {
+        constexpr bool WHOLE = decltype(whole)::value;
+        ce = fresh(ce), c4 = fresh(c4);
+        const int t0 = i * SUB;  // in the chunk
+        float u[MINE], sig[MINE], dyz[MINE];
 #pragma unroll
         for (int k = 0; k < MINE; ++k) {
-            const int at = p.q * MINE + k;
-            u[k] = E::ld(in.ru[k]);
-            const float dy = E::ld(in.ry[k]), pre = E::ld(in.rd[k]) + bias;
-            dt[k] = hw_softplus(pre);
+            const int at = in.first + k;
+            u[k] = own_register(E::ld(in.ru[k]));
+            const float dy = E::ld(in.ry[k]), pre = E::ld(in.rd[k]) + bias, z = E::ld(in.rz[k]), sz = hw_sigmoid(z);
+            float dt = hw_softplus(pre), g = dy * (gate ? z * sz : 1.0f);
             sig[k] = hw_sigmoid(pre);
-            g[k] = dy;
-            dyz[k] = 0.0f;
-            if (gate) {
-                const float z = E::ld(in.rz[k]), sz = hw_sigmoid(z);
-                g[k] = dy * (z * sz);
-                dyz[k] = dy * __builtin_fmaf(z * sz, 1.0f - sz, sz);
-            }
-            if (t0 + at >= end || !p.live) dt[k] = u[k] = g[k] = sig[k] = dyz[k] = 0.0f;
-            s_in[at][p.lane] = make_float2(dt[k], dt[k] * u[k]);
-            s_g[at][p.lane] = g[k];
+            dyz[k] = dy * __builtin_fmaf(z * sz, 1.0f - sz, sz);
+            if ((!WHOLE && t0 + at >= count) || !live) dt = g = u[k] = sig[k] = dyz[k] = 0.0f;
+            s_in[at][p.lane] = make_float2(dt, dt * u[k]);
+            s_g[at][p.lane] = g;
         }
         float h[NQ], e[SUB][NQ], eh[SUB][NQ], bc = 0.0f;
 #pragma unroll
-        for (int n = 0; n < NQ; ++n) h[n] = mark[n];
-        if (i > 0) fetch(i - 1);
+        for (int n = 0; n < NQ; ++n) h[n] = live ? mark[n] : 0.0f;
         __syncthreads();
+        const int last = WHOLE ? SUB - 1 : count - t0 - 1;  // rows behind the end are read as the last one
+        Pair<DT> pair[2];
+        auto issue = [&](int s0, Pair<DT>& x, const ScalarRows<DT>& fromB, const ScalarRows<DT>& fromC) {
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                fromB.load(min(s0 + j, last), x.B[j]);
+                fromC.load(min(s0 + j, last), x.C[j]);
+                x.in[j] = s_in[s0 + j][p.lane];
+                x.g[j] = s_g[s0 + j][p.lane];
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        };
+        auto here = [&](Pair<DT>& x) {
+            x.here(), x.words_here(x.B), x.words_here(x.C);
+            asm volatile("" : "+v"(x.g[0]), "+v"(x.g[1]));
+        };
+        issue(0, pair[0], xB, xC);
         float r[8];
 #pragma unroll
-        for (int s = 0; s < SUB; ++s) {
-            const int64_t t = min(t0 + s, end - 1);
-            float B[NQ], C[NQ];
-            scalar4<DT>(row<DT>(a.B, p.b, t) + p.q * NQ, B);
-            scalar4<DT>(row<DT>(a.C, p.b, t) + p.q * NQ, C);
-            const float2 x = s_in[s][p.lane];
-            const float gs = s_g[s][p.lane];
-            float y = 0.0f;
+        for (int s0 = 0; s0 < SUB; s0 += 2) {
+            Pair<DT>& x = pair[s0 / 2 % 2];
+            here(x);
+            if (s0 + 2 < SUB) issue(s0 + 2, pair[s0 / 2 % 2 ^ 1], xB, xC);
 #pragma unroll
-            for (int n = 0; n < NQ; ++n) {
-                e[s][n] = __builtin_amdgcn_exp2f(x.x * a2[n]);
-                eh[s][n] = e[s][n] * h[n];
-                h[n] = __builtin_fmaf(B[n], x.y, eh[s][n]);
-                y = __builtin_fmaf(h[n], C[n], y);
-                r[(s & 1) * NQ + n] = gs * h[n];
+            for (int j = 0; j < 2; ++j) {
+                const int s = s0 + j;
+                float y = 0.0f;
+#pragma unroll
+                for (int n = 0; n < NQ; ++n) {
+                    e[s][n] = __builtin_amdgcn_exp2f(x.in[j].x * a2[n]);
+                    eh[s][n] = e[s][n] * h[n];
+                    h[n] = __builtin_fmaf(x.b(j, n), x.in[j].y, eh[s][n]);
+                    y = __builtin_fmaf(h[n], x.c(j, n), y);
+                    r[j * NQ + n] = x.g[j] * h[n];
+                }
+                s_y[p.q][s][p.lane] = y;
             }
-            s_y[p.q][s][p.lane] = y;
-            if (s & 1) {  // two positions' dC: lane l has the one of position s - 1 + l / 32, state (l / 8) % 4
-                const float v = sum8(r, p.lane);
-                bc = (p.lane & 7) == s / 2 ? v : bc;
+            // the two positions' dC: lane l has the one of position s0 + l / 32, state (l / 8) % 4
+            const float v = sum8(r, p.lane);
+            bc = (p.lane & 7) == s0 / 2 ? v : bc;
+        }
+        const ScalarRows<DT> xB2 = again(xB), xC2 = again(xC);
+#pragma unroll
+        for (int s0 = SUB - 2; s0 >= 0; s0 -= 2) {
+            Pair<DT>& x = pair[s0 / 2 % 2];  // the last one is still here
+            if (s0 < SUB - 2) here(x);
+            if (s0 > 0) issue(s0 - 2, pair[s0 / 2 % 2 ^ 1], xB2, xC2);
+#pragma unroll
+            for (int j = 1; j >= 0; --j) {
+                const int s = s0 + j;
+                float sB = 0.0f, sw = 0.0f;
+#pragma unroll
+                for (int n = 0; n < NQ; ++n) {
+                    dh[n] = __builtin_fmaf(x.c(j, n), x.g[j], dh[n]);
+                    sB = __builtin_fmaf(dh[n], x.b(j, n), sB);
+                    r[j * NQ + n] = dh[n] * x.in[j].y;
+                    const float w = dh[n] * eh[s][n];
+                    sw = __builtin_fmaf(w, a2[n], sw);
+                    dA[n] = __builtin_fmaf(w, x.in[j].x, dA[n]);
+                    dh[n] *= e[s][n];
+                }
+                s_s[p.q][s][p.lane] = sB;
+                s_w[p.q][s][p.lane] = sw;
+            }
+            const float v = sum8(r, p.lane);
+            bc = (p.lane & 7) == SUB / 2 + s0 / 2 ? v : bc;
+            if (s0 == FETCH_AT) {  // the next block's loads, where registers come free
+                in.back(i > 0);
+                marks -= i > 0 ? NS * a.channels : 0;
+                fetch(i > 0 ? SUB : count - t0);
             }
         }
-#pragma unroll
-        for (int s = SUB - 1; s >= 0; --s) {
-            const int64_t t = min(t0 + s, end - 1);
-            float B[NQ], C[NQ];
-            scalar4<DT>(again(row<DT>(a.B, p.b, t) + p.q * NQ), B);
-            scalar4<DT>(again(row<DT>(a.C, p.b, t) + p.q * NQ), C);
-            const float2 x = s_in[s][p.lane];
-            const float gs = s_g[s][p.lane];
-            float sB = 0.0f, sw = 0.0f;
-#pragma unroll
-            for (int n = 0; n < NQ; ++n) {
-                dh[n] = __builtin_fmaf(C[n], gs, dh[n]);
-                sB = __builtin_fmaf(dh[n], B[n], sB);
-                r[(s & 1) * NQ + n] = dh[n] * x.y;
-                const float w = dh[n] * eh[s][n];
-                sw = __builtin_fmaf(w, a2[n], sw);
-                dA[n] = __builtin_fmaf(w, x.x, dA[n]);
-                dh[n] *= e[s][n];
-            }
-            s_s[p.q][s][p.lane] = sB;
-            s_w[p.q][s][p.lane] = sw;
-            if (!(s & 1)) {
-                const float v = sum8(r, p.lane);
-                bc = (p.lane & 7) == SUB / 2 + s / 2 ? v : bc;
-            }
-        }
-        a.part_bc[(((int64_t)p.cb * a.batch + p.b) * a.subs + lo / SUB + i) * WG + threadIdx.x] = bc;
+        xB.back(), xC.back();
+        *lane_at(bc_out, threadIdx.x * 4) = bc;
+        bc_out -= WG;
         __syncthreads();
 #pragma unroll
         for (int k = 0; k < MINE; ++k) {
-            const int at = p.q * MINE + k;
-            const int64_t t = t0 + at;
+            const int at = in.first + k, t = t0 + at;
+            const float dt = s_in[at][p.lane].x, g = s_g[at][p.lane];
             float y = D * u[k], sB = 0.0f, sw = 0.0f;
 #pragma unroll
             for (int w = 0; w < WAVES; ++w) {
@@ -436,15 +606,17 @@ __global__ void __launch_bounds__(WG) k_scan_bwd(const ScanArgs a) {
                 sB += s_s[w][at][p.lane];
                 sw += s_w[w][at][p.lane];
             }
-            const float ddelta = __builtin_fmaf(u[k], sB, sw * LN2) * sig[k], du = __builtin_fmaf(dt[k], sB, D * g[k]);
-            dD = __builtin_fmaf(g[k], u[k], dD);
+            const float ddelta = __builtin_fmaf(u[k], sB, sw * LN2) * sig[k], du = __builtin_fmaf(dt, sB, D * g);
+            dD = __builtin_fmaf(g, u[k], dD);
             dbias += ddelta;
-            if (p.live && t < hi) {
-                row_mut<DT>(a.du, p.b, t)[p.c] = E::st(t < end ? du : 0.0f);
-                row_mut<DT>(a.ddelta, p.b, t)[p.c] = E::st(t < end ? ddelta : 0.0f);
-                if (gate) row_mut<DT>(a.dz, p.b, t)[p.c] = E::st(t < end ? dyz[k] * y : 0.0f);
+            if (live && (WHOLE || t < rows_out)) {
+                const bool inside = WHOLE || t < count;
+                yu.store(at, ce, inside ? du : 0.0f);
+                yd.store(at, ce, inside ? ddelta : 0.0f);
+                yz.store(at, ce, !inside ? 0.0f : gate ? dyz[k] * y : du);  // without a gate du once more
             }
         }
+        yu.back(true), yd.back(true), yz.back(true);
         if (i % 8 == 0)  // sums of 64 positions at a time: a long sum in one register loses digits
 #pragma unroll
             for (int n = 0; n < NQ; ++n) {
@@ -452,8 +624,15 @@ __global__ void __launch_bounds__(WG) k_scan_bwd(const ScanArgs a) {
                 dA[n] = 0.0f;
             }
         __syncthreads();
+    };
+    if (n_subs > 0) {
+        fetch(count - (n_subs - 1) * SUB);
+        const int after = (int)ceil_div(end, a.chunk) - 1;
+        over_chunks(a, p, after, -1, after - p.k, a2, dh);
+        block(n_subs - 1, std::false_type());
+        for (int i = n_subs - 2; i >= 0; --i) block(i, std::true_type());
     }
-    if (p.live)
+    if (live)
         for (int64_t t = lo + (int64_t)n_subs * SUB + p.q; t < hi; t += WAVES) {
             row_mut<DT>(a.du, p.b, t)[p.c] = E::st(0.0f);
             row_mut<DT>(a.ddelta, p.b, t)[p.c] = E::st(0.0f);
@@ -463,7 +642,7 @@ __global__ void __launch_bounds__(WG) k_scan_bwd(const ScanArgs a) {
     s_s[p.q][0][p.lane] = dD;
     s_s[p.q][1][p.lane] = dbias;
     __syncthreads();
-    if (!p.live) return;
+    if (!live) return;
     float* mine = a.part_par + (p.b * a.chunks + p.k) * (NS + 2) * a.channels;
 #pragma unroll
     for (int n = 0; n < NQ; ++n) mine[(int64_t)p.c * NS + p.q * NQ + n] = dA_all[n];
@@ -500,14 +679,12 @@ __global__ void __launch_bounds__(WG) k_scan_step(const ScanArgs a) {
     if (b >= a.batch || c >= a.channels) return;
     float B[NS], C[NS];
 #pragma unroll
-    for (int i = 0; i < NS; i += NQ) {
-        float v[NQ];
-        scalar4<DT>(row<DT>(a.B, b, 0) + i, v);
+    for (int i = 0; i < WAVES; ++i) {
+        uint32_t w[ScalarRows<DT>::WORDS], v[ScalarRows<DT>::WORDS];
+        ScalarRows<DT>(a.B, b, 0, i).load(0, w);
+        ScalarRows<DT>(a.C, b, 0, i).load(0, v);
 #pragma unroll
-        for (int j = 0; j < NQ; ++j) B[i + j] = v[j];
-        scalar4<DT>(row<DT>(a.C, b, 0) + i, v);
-#pragma unroll
-        for (int j = 0; j < NQ; ++j) C[i + j] = v[j];
+        for (int j = 0; j < NQ; ++j) B[i * NQ + j] = ScalarRows<DT>::value(w, j), C[i * NQ + j] = ScalarRows<DT>::value(v, j);
     }
     float* st = a.state_out + b * NS * (int64_t)a.channels + c;
     float h[NS];
@@ -571,7 +748,9 @@ void lay_out(ScanArgs& a, const Work& w, void* d_work) {
     a.part_par = a.part_bc + w.bc;
 }
 
-// B and C rows are read four values at a time at uniform addresses, which have to be multiples of 4 bytes.
+// Rows are read at 32-bit offsets from a block's first; those of B and C four values at a time at uniform addresses, which have
+// to be multiples of 4 bytes.
+bool stride_ok(const boa_rows& r) { return !r.p || (r.row_stride >= 0 && r.row_stride <= BOA_SCAN_MAX_ROW_STRIDE); }
 bool bc_aligned(const boa_scan* s, const boa_rows& r) {
     return s->dtype == BOA_DT_F32 || ((uintptr_t)r.p % 4 == 0 && r.batch_stride % 2 == 0 && r.row_stride % 2 == 0);
 }
@@ -584,6 +763,9 @@ int check_scan(const char* who, const boa_scan* s, ScanArgs& a) {
                         BOA_OPS_MAX_CHANNELS, (long long)s->batch, (long long)s->length, s->channels);
     if (s->batch > 0 && s->length > 0) {
         if (!s->u.p || !s->delta.p || !s->b.p || !s->c.p || !s->a) return boa_fail(BOA_ERR_ARG, "%s: null pointer", who);
+        for (const boa_rows* r : {&s->u, &s->delta, &s->z, &s->b, &s->c, &s->y})
+            if (!stride_ok(*r))
+                return boa_fail(BOA_ERR_ARG, "%s: rows have to be 0 to %d values apart", who, BOA_SCAN_MAX_ROW_STRIDE);
         if (!bc_aligned(s, s->b) || !bc_aligned(s, s->c))
             return boa_fail(BOA_ERR_ARG, "%s: rows of B and C of 16-bit types have to begin at multiples of 4 bytes", who);
     }
@@ -621,10 +803,13 @@ extern "C" int boa_selective_scan_fwd(const boa_scan* s, void* d_work, int64_t w
         constexpr int DT = decltype(dt)::value;
         const uint32_t blocks = (uint32_t)(a.batch * a.cblocks);
         if (a.chunks > 1) {
-            hipLaunchKernelGGL((k_scan_fwd<DT, true>), dim3(blocks * (a.chunks - 1)), dim3(WG), 0, (hipStream_t)stream, a);
+            hipLaunchKernelGGL((k_scan_fwd<DT, LOCAL>), dim3(blocks * (a.chunks - 1)), dim3(WG), 0, (hipStream_t)stream, a);
             BOA_HIP_TRY(hipGetLastError());
         }
-        hipLaunchKernelGGL((k_scan_fwd<DT, false>), dim3(blocks * a.chunks), dim3(WG), 0, (hipStream_t)stream, a);
+        if (a.marks != nullptr)
+            hipLaunchKernelGGL((k_scan_fwd<DT, OUT_MARKS>), dim3(blocks * a.chunks), dim3(WG), 0, (hipStream_t)stream, a);
+        else
+            hipLaunchKernelGGL((k_scan_fwd<DT, OUT>), dim3(blocks * a.chunks), dim3(WG), 0, (hipStream_t)stream, a);
         BOA_HIP_TRY(hipGetLastError());
         return (int)BOA_OK;
     });
@@ -638,6 +823,9 @@ extern "C" int boa_selective_scan_bwd(const boa_scan* s, void* d_work, int64_t w
     if (!s->dpar) return boa_fail(BOA_ERR_ARG, "boa_selective_scan_bwd: null pointer");
     if (any && (!s->dy.p || !s->du.p || !s->ddelta.p || !s->db.p || !s->dc.p || !s->marks || (s->z.p && !s->dz.p)))
         return boa_fail(BOA_ERR_ARG, "boa_selective_scan_bwd: null pointer");
+    for (const boa_rows* r : {&s->dy, &s->du, &s->ddelta, &s->dz})
+        if (any && !stride_ok(*r))
+            return boa_fail(BOA_ERR_ARG, "boa_selective_scan_bwd: rows have to be 0 to %d values apart", BOA_SCAN_MAX_ROW_STRIDE);
     const Work w = work_of(s, true);
     if (any && (!d_work || work_bytes < w.bytes()))
         return boa_fail(BOA_ERR_ARG, "boa_selective_scan_bwd: workspace of %lld bytes, needs %lld", (long long)work_bytes,
@@ -653,7 +841,10 @@ extern "C" int boa_selective_scan_bwd(const boa_scan* s, void* d_work, int64_t w
                 hipLaunchKernelGGL((k_scan_bwd_local<DT>), dim3(blocks * (a.chunks - 1)), dim3(WG), 0, st, a);
                 BOA_HIP_TRY(hipGetLastError());
             }
-            hipLaunchKernelGGL((k_scan_bwd<DT>), dim3(blocks * a.chunks), dim3(WG), 0, st, a);
+            if (a.channels % 64 == 0)
+                hipLaunchKernelGGL((k_scan_bwd<DT, true>), dim3(blocks * a.chunks), dim3(WG), 0, st, a);
+            else
+                hipLaunchKernelGGL((k_scan_bwd<DT, false>), dim3(blocks * a.chunks), dim3(WG), 0, st, a);
             BOA_HIP_TRY(hipGetLastError());
             hipLaunchKernelGGL((k_scan_sum_bc<DT>), dim3((uint32_t)min(a.batch * a.subs, MAX_BLOCKS)), dim3(WG), 0, st, a);
             BOA_HIP_TRY(hipGetLastError());

@@ -270,6 +270,7 @@ int boa_causal_conv_step(int dtype, const void* d_x, int64_t x_stride, void* d_s
  *   dt = softplus(delta + delta_bias), h_t = exp(dt a) h_(t-1) + dt b_t u_t, y_t = (c_t . h_t + d u_t) * silu(z_t)
  * Members that a call does not use are ignored; those marked * may have a null pointer.                 */
 #define BOA_SCAN_MARK 8
+#define BOA_SCAN_MAX_ROW_STRIDE 67108863
 typedef struct boa_rows {
     void* p;
     int64_t batch_stride, row_stride;       /* elements */
@@ -278,8 +279,9 @@ typedef struct boa_scan {
     int32_t dtype;                          /* of u, delta, z, b, c, y, dy and their gradients           */
     int32_t channels;
     int64_t batch, length;
-    boa_rows u, delta, z;                   /* [batch][length][channels]; z*: no gate                    */
-    boa_rows b, c;                          /* [batch][length][16]; 16-bit rows at multiples of 4 bytes  */
+    boa_rows u, delta, z;                   /* [batch][length][channels]; z*: no gate; all rows 0 to
+                                               BOA_SCAN_MAX_ROW_STRIDE values apart                      */
+    boa_rows b, c;                          /* [batch][length][16]; rows at multiples of 4 bytes         */
     const float* a;                         /* [channels][16], negative                                  */
     const float* d;                         /* * [channels]                                              */
     const float* delta_bias;                /* * [channels]                                              */

@@ -139,7 +139,7 @@ def test_scan_struct_is_the_headers(tmp_path):
 def test_constants_are_the_headers():
     src = open(os.path.join(REPO, "include", "boa_hip.h")).read()
     for name in ("BOA_DT_F32", "BOA_DT_BF16", "BOA_DT_F16", "BOA_LAYER_NORM_MAX_D", "BOA_CROSS_ENTROPY_MAX_V",
-                 "BOA_OPS_MAX_CHANNELS", "BOA_SCAN_MARK"):
+                 "BOA_OPS_MAX_CHANNELS", "BOA_SCAN_MARK", "BOA_SCAN_MAX_ROW_STRIDE"):
         assert int(re.search(rf"#define {name} (\d+)", src).group(1)) == getattr(_native, name)
 
 
@@ -157,7 +157,7 @@ def test_c_abi_refuses_before_it_launches():
     fwd, bwd, step = L.boa_selective_scan_fwd, L.boa_selective_scan_bwd, L.boa_selective_scan_step
     assert fwd(None, None, 0, None) == bad
     for kw in (dict(dtype=3), dict(dtype=-1), dict(c=0), dict(c=65537), dict(n=-1), dict(length=-1), dict(p=0),
-               dict(dtype=1, b_stride=33), dict(dtype=2, p=4098), dict(n=1 << 40)):
+               dict(dtype=1, b_stride=33), dict(b_stride=1 << 26), dict(b_stride=-128), dict(dtype=2, p=4098), dict(n=1 << 40)):
         assert fwd(_pack(**kw), None, 0, None) == bad, kw
         assert step(_pack(**kw), None) == bad, kw
     assert step(_pack(), None) == bad  # more than one position
