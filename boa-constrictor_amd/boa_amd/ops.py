@@ -25,10 +25,10 @@ passes on the capture's side stream and let go of any eager graph of the same pa
 """
 from __future__ import annotations
 
+import functools
 import struct
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from boa_amd import _native as _nat
 
@@ -98,6 +98,11 @@ def _rows(t):
     return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
 
 
+def _flat(t, d):
+    """[..., d] as rows."""
+    return _rows(t if t.ndim == 2 else t.reshape(-1, d))
+
+
 def _gpu(who, t):
     if not t.is_cuda:
         raise ValueError(f"{who}: the tensors must be on the GPU (got {t.device})")
@@ -120,6 +125,17 @@ def _call(t, f, *args):
             _nat.check(f(*args, _raw_stream(i)))
 
 
+def _once(ctx):
+    """The gradients are made by kernels, which autograd cannot differentiate again."""
+    if torch.is_grad_enabled():
+        raise RuntimeError("the operators of boa_amd.ops are differentiable once (create_graph is not supported)")
+
+
+@functools.lru_cache(maxsize=256)
+def _bytes(name, *sizes):
+    return getattr(_nat.lib(), name)(*sizes)
+
+
 def _ptr(t):
     return 0 if t is None else t.data_ptr()
 
@@ -131,7 +147,7 @@ def _work(nbytes, like):
 # ---- layer norm ------------------------------------------------------------------------------------
 def _norm_fwd(x, w, b, eps, keep):
     d = x.shape[-1]
-    rows = _rows(x.reshape(-1, d))
+    rows = _flat(x, d)
     y = torch.empty_like(x, memory_format=torch.contiguous_format)
     stats = torch.empty((rows.shape[0], 2), dtype=torch.float32, device=x.device) if keep else None
     _call(x, _nat.lib().boa_layer_norm_fwd, _DTYPES[x.dtype], rows.data_ptr(), rows.stride(0), _ptr(w), _ptr(b), rows.shape[0], d,
@@ -147,22 +163,23 @@ class _LayerNorm(torch.autograd.Function):
         return y
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dy):
+        _once(ctx)
         x, w, stats = ctx.saved_tensors
         d = x.shape[-1]
-        rows, dyr = _rows(x.reshape(-1, d)), _rows(dy.reshape(-1, d))
+        rows, dyr = _flat(x, d), _flat(dy, d)
         n = rows.shape[0]
         dx = torch.empty_like(x, memory_format=torch.contiguous_format)
-        params = ctx.needs_input_grad[1] or ctx.needs_input_grad[2]
-        dwb = torch.empty((2, d), dtype=torch.float32, device=x.device) if params else None
-        lib = _nat.lib()
-        size = lib.boa_layer_norm_bwd_work_bytes(n, d) if params else 0
-        work = _work(size, x)
-        _call(x, lib.boa_layer_norm_bwd, _DTYPES[x.dtype], dyr.data_ptr(), dyr.stride(0), rows.data_ptr(), rows.stride(0), _ptr(w),
+        _, need_w, need_b, _ = ctx.needs_input_grad
+        dwb = work = None
+        size = 0
+        if need_w or need_b:
+            dwb = stats.new_empty((2, d))
+            size = _bytes("boa_layer_norm_bwd_work_bytes", n, d)
+            work = _work(size, x)
+        _call(x, _nat.lib().boa_layer_norm_bwd, _DTYPES[x.dtype], dyr.data_ptr(), dyr.stride(0), rows.data_ptr(), rows.stride(0), _ptr(w),
               stats.data_ptr(), n, d, dx.data_ptr(), d, _ptr(dwb), _ptr(work), size)
-        need = ctx.needs_input_grad
-        return dx, dwb[0] if need[1] else None, dwb[1] if need[2] else None, None
+        return dx, dwb[0] if need_w else None, dwb[1] if need_b else None, None
 
 
 def layer_norm(x, weight=None, bias=None, eps: float = 1e-5):
@@ -191,7 +208,7 @@ class _CrossEntropy(torch.autograd.Function):
         each = torch.empty(n, dtype=torch.float32, device=x.device) if reduction == "none" else None
         loss, count = (torch.empty((), dtype=torch.float32, device=x.device) if each is None else None for _ in range(2))
         lib = _nat.lib()
-        size = lib.boa_cross_entropy_work_bytes() if each is None else 0
+        size = _bytes("boa_cross_entropy_work_bytes") if each is None else 0
         work = _work(size, x)
         _call(x, lib.boa_cross_entropy_fwd, _DTYPES[x.dtype], x.data_ptr(), x.stride(0), target.data_ptr(), target.element_size(),
               ignore, n, v, reduction == "mean", _ptr(stats), _ptr(each), _ptr(loss), _ptr(count), _ptr(work), size)
@@ -200,12 +217,12 @@ class _CrossEntropy(torch.autograd.Function):
         return loss if each is None else each
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, up):
+        _once(ctx)
         x, target, stats, count = ctx.saved_tensors
         n, v = x.shape
-        up = up.to(torch.float32).contiguous()
-        dx = torch.empty((n, v), dtype=x.dtype, device=x.device)
+        up = up.contiguous()  # float32, as the loss is
+        dx = x.new_empty((n, v))
         _call(x, _nat.lib().boa_cross_entropy_bwd, _DTYPES[x.dtype], x.data_ptr(), x.stride(0), target.data_ptr(),
               target.element_size(), ctx.ignore, n, v, stats.data_ptr(), up.data_ptr(), ctx.reduction == "none",
               _ptr(count) if ctx.reduction == "mean" else 0, dx.data_ptr(), v)
@@ -231,7 +248,7 @@ def cross_entropy(logits, targets, *, ignore_index: int = -100, reduction: str =
         raise ValueError(f"cross_entropy: targets must be {list(logits.shape[:-1])} on {logits.device} "
                          f"(got {list(targets.shape)} on {targets.device})")
     _gpu("cross_entropy", logits)
-    rows = _rows(logits.reshape(-1, logits.shape[-1]))
+    rows = _flat(logits, logits.shape[-1])
     out = _CrossEntropy.apply(rows, targets.reshape(-1).contiguous(), int(ignore_index), reduction, _grad(logits))
     return out.reshape(targets.shape) if reduction == "none" else out
 
@@ -239,8 +256,8 @@ def cross_entropy(logits, targets, *, ignore_index: int = -100, reduction: str =
 # ---- causal convolution ----------------------------------------------------------------------------
 def _conv_fwd(x, w, b, silu, state, lens, want_state):
     n, length, c = x.shape
-    y = torch.empty((n, length, c), dtype=x.dtype, device=x.device)
-    out = torch.empty((n, D_CONV - 1, c), dtype=x.dtype, device=x.device) if want_state else None
+    y = x.new_empty((n, length, c))
+    out = x.new_empty((n, D_CONV - 1, c)) if want_state else None
     _call(x, _nat.lib().boa_causal_conv_fwd, _DTYPES[x.dtype], x.data_ptr(), x.stride(0), x.stride(1), w.data_ptr(), _ptr(b), silu,
           n, length, c, _ptr(lens), _ptr(state), _ptr(out), y.data_ptr(), length * c, c)
     return y, out
@@ -257,23 +274,24 @@ class _CausalConv(torch.autograd.Function):
         return y, out
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dy, _):
+        _once(ctx)
         x, w, b, state, lens = ctx.saved_tensors
         n, length, c = x.shape
         dy = _rows(dy)
-        dx = torch.empty((n, length, c), dtype=x.dtype, device=x.device)
-        params = ctx.needs_input_grad[1] or ctx.needs_input_grad[2]
-        dwb = torch.empty((D_CONV + 1) * c, dtype=torch.float32, device=x.device) if params else None
-        lib = _nat.lib()
-        size = lib.boa_causal_conv_bwd_work_bytes(n, length, c) if params else 0
-        work = _work(size, x)
-        _call(x, lib.boa_causal_conv_bwd, _DTYPES[x.dtype], dy.data_ptr(), dy.stride(0), dy.stride(1), x.data_ptr(), x.stride(0),
+        dx = x.new_empty((n, length, c))
+        need_w, need_b = ctx.needs_input_grad[1:3]
+        dwb = work = None
+        size = 0
+        if need_w or need_b:
+            dwb = w.new_empty((D_CONV + 1) * c)
+            size = _bytes("boa_causal_conv_bwd_work_bytes", n, length, c)
+            work = _work(size, x)
+        _call(x, _nat.lib().boa_causal_conv_bwd, _DTYPES[x.dtype], dy.data_ptr(), dy.stride(0), dy.stride(1), x.data_ptr(), x.stride(0),
               x.stride(1), w.data_ptr(), _ptr(b), ctx.silu, n, length, c, _ptr(lens), _ptr(state), dx.data_ptr(), length * c, c,
               _ptr(dwb), _ptr(work), size)
-        need = ctx.needs_input_grad
-        dw = dwb[:D_CONV * c].view(w.shape) if need[1] else None
-        db = dwb[D_CONV * c:] if need[2] else None
+        dw = dwb[:D_CONV * c].view(w.shape) if need_w else None
+        db = dwb[D_CONV * c:] if need_b else None
         return dx, dw, db, None, None, None, None
 
 
@@ -322,7 +340,7 @@ def causal_conv_step(x, state, weight, bias=None, *, silu: bool = True):
         raise ValueError(f"{who}: no gradient; call it under torch.no_grad()")
     _gpu(who, x)
     x = _rows(x)
-    y = torch.empty((n, c), dtype=x.dtype, device=x.device)
+    y = x.new_empty((n, c))
     _call(x, _nat.lib().boa_causal_conv_step, _DTYPES[x.dtype], x.data_ptr(), x.stride(0), state.data_ptr(), w.data_ptr(), _ptr(b),
           bool(silu), n, c, y.data_ptr(), c)
     return y
@@ -362,12 +380,11 @@ def _scalar_rows(t):
 
 def _scan_fwd(u, delta, A, B, C, D, z, bias, state, lens, want_state, keep):
     n, length, c = u.shape
-    y = torch.empty((n, length, c), dtype=u.dtype, device=u.device)
-    out = torch.empty((n, D_STATE, c), dtype=torch.float32, device=u.device) if want_state else None
+    y = u.new_empty((n, length, c))
+    out = A.new_empty((n, D_STATE, c)) if want_state else None
     marks = None
     if keep:
-        blocks = -(-length // _nat.BOA_SCAN_MARK)
-        marks = torch.empty((n, blocks, D_STATE, c), dtype=torch.float32, device=u.device)
+        marks = A.new_empty((n, -(-length // _nat.BOA_SCAN_MARK), D_STATE, c))
     args = _pack(u, delta, A, B, C, D, z, bias, lens, state, out, marks, y)
     lib = _nat.lib()
     size = lib.boa_selective_scan_work_bytes(args, 0)
@@ -386,16 +403,14 @@ class _SelectiveScan(torch.autograd.Function):
         return y, out
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dy, _):
+        _once(ctx)
         u, delta, A, B, C, D, z, bias, lens, marks = ctx.saved_tensors
         n, length, c = u.shape
         dy = _scan_rows(dy)
-        du, ddelta = torch.empty_like(dy, memory_format=torch.contiguous_format), torch.empty_like(
-            dy, memory_format=torch.contiguous_format)
-        dz = torch.empty_like(dy, memory_format=torch.contiguous_format) if z is not None else None
-        dB, dC = (torch.empty((n, length, D_STATE), dtype=u.dtype, device=u.device) for _ in range(2))
-        dpar = torch.empty((D_STATE + 2) * c, dtype=torch.float32, device=u.device)
+        du, ddelta, dz = (u.new_empty((n, length, c)) if t is not None else None for t in (u, delta, z))
+        dB, dC = (u.new_empty((n, length, D_STATE)) for _ in range(2))
+        dpar = A.new_empty((D_STATE + 2) * c)
         args = _pack(u, delta, A, B, C, D, z, bias, lens, None, None, marks, None, (dy, du, ddelta, dz, dB, dC), dpar)
         lib = _nat.lib()
         size = lib.boa_selective_scan_work_bytes(args, 1)
@@ -462,7 +477,7 @@ def selective_scan_step(u, delta, A, B, C, D=None, z=None, delta_bias=None, *, s
     if _grad(*args):
         raise ValueError(f"{who}: no gradient; call it under torch.no_grad()")
     _gpu(who, u)
-    y = torch.empty((n, c), dtype=u.dtype, device=u.device)
+    y = u.new_empty((n, c))
     u, delta, A, B, C, D, z, bias = args
 
     def r2(t):

@@ -16,9 +16,10 @@ namespace {
 
 constexpr int WG = 256, WAVES = WG / 64;
 constexpr int MAX_V = BOA_CROSS_ENTROPY_MAX_V;
-constexpr int MAX_GROUPS = 1024;
+constexpr int MAX_GROUPS = 2048;
 
-constexpr int rows_at_once(int per) { return per >= 16 ? 1 : 16 / per; }
+// Rows that a wavefront has in flight, for PER elements per lane.
+constexpr int rows_at_once(int per) { return per >= 32 ? 1 : 32 / per; }
 
 __device__ __forceinline__ int64_t target_at(const void* t, int bytes, int64_t r) {
     return bytes == 1 ? (int64_t)static_cast<const uint8_t*>(t)[r]
@@ -44,7 +45,7 @@ __global__ void __launch_bounds__(WG) k_loss_fwd(const void* xp, int64_t xs, con
     const int64_t wave = (int64_t)blockIdx.x * WAVES + wid, waves = (int64_t)gridDim.x * WAVES;
     double total = 0.0, count = 0.0;
     for (int64_t r0 = wave * ROWS; r0 < rows; r0 += waves * ROWS) {
-        float v[ROWS][PER], hit[ROWS];
+        float v[ROWS][PER];
         int64_t t[ROWS];
 #pragma unroll
         for (int r = 0; r < ROWS; ++r) {
@@ -59,7 +60,6 @@ __global__ void __launch_bounds__(WG) k_loss_fwd(const void* xp, int64_t xs, con
                 for (int j = 0; j < VEC; ++j) v[r][i * VEC + j] = e[j];
             }
             t[r] = target_at(target, target_bytes, at);
-            hit[r] = Elem<DT>::ld(x[at * xs + (t[r] >= 0 && t[r] < V ? t[r] : 0)]);
         }
 #pragma unroll
         for (int r = 0; r < ROWS; ++r) {
@@ -73,11 +73,15 @@ __global__ void __launch_bounds__(WG) k_loss_fwd(const void* xp, int64_t xs, con
             }
             m = wmax(m);
             if (__any(nan)) m = __builtin_nanf("");
-            float s = 0.0f;
+            float s = 0.0f, hit = 0.0f;  // the target's logit, from the lane that has it
 #pragma unroll
-            for (int i = 0; i < PER; ++i) s += R::col(i / VEC, lane) < V ? hw_exp(v[r][i] - m) : 0.0f;
+            for (int i = 0; i < PER; ++i) {
+                const int c = R::col(i / VEC, lane);
+                s += c < V ? hw_exp(v[r][i] - m) : 0.0f;
+                hit = c + i % VEC == t[r] ? v[r][i] : hit;
+            }
             s = wsum(s);
-            float loss = logf(s) + (m - hit[r]);
+            float loss = logf(s) + (m - wsum(hit));
             const bool kept = t[r] != ignore;
             if (t[r] < 0 || t[r] >= V) loss = __builtin_nanf("");
             if (kept) {
@@ -103,9 +107,14 @@ __global__ void __launch_bounds__(WG) k_loss_fwd(const void* xp, int64_t xs, con
 }
 
 // The workgroups' sums: their loss (over the count for the mean) and the count.
-__global__ void __launch_bounds__(MAX_GROUPS) k_loss_sum(const double2* part, int n, int mean, float* loss, float* count) {
-    __shared__ double2 s[MAX_GROUPS / 64];
-    double2 v = (int)threadIdx.x < n ? part[threadIdx.x] : make_double2(0.0, 0.0);
+constexpr int SUM_WG = 1024;
+__global__ void __launch_bounds__(SUM_WG) k_loss_sum(const double2* part, int n, int mean, float* loss, float* count) {
+    __shared__ double2 s[SUM_WG / 64];
+    double2 v = make_double2(0.0, 0.0);
+    for (int i = threadIdx.x; i < n; i += SUM_WG) {
+        v.x += part[i].x;
+        v.y += part[i].y;
+    }
     for (int o = 32; o > 0; o >>= 1) {
         v.x += __shfl_xor(v.x, o, 64);
         v.y += __shfl_xor(v.y, o, 64);
@@ -113,7 +122,7 @@ __global__ void __launch_bounds__(MAX_GROUPS) k_loss_sum(const double2* part, in
     if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = v;
     __syncthreads();
     if (threadIdx.x == 0) {
-        for (int k = 1; k < MAX_GROUPS / 64; ++k) {
+        for (int k = 1; k < SUM_WG / 64; ++k) {
             v.x += s[k].x;
             v.y += s[k].y;
         }
@@ -171,9 +180,12 @@ __global__ void __launch_bounds__(WG) k_loss_bwd(const void* xp, int64_t xs, con
     }
 }
 
+// Calls f with the row shape for V symbols: accesses of 16 bytes (8 for 16-bit rows of up to 256 symbols, which then take all
+// 64 lanes) where the rows are aligned for them, else single elements.
 template <int DT, class F>
 int with_row(int d, bool aligned, F f) {
     constexpr int W = wide<DT>();
+    if (aligned && d % 4 == 0 && d <= 256) return f(Row<DT, 4, 1>());
     if (aligned && d % W == 0) {
         const int n = (int)ceil_div(d, 64 * W);
         if (n <= 1) return f(Row<DT, W, 1>());
@@ -234,7 +246,7 @@ extern "C" int boa_cross_entropy_fwd(int dtype, const void* d_x, int64_t x_strid
         if (launched != BOA_OK) return launched;
     }
     if (d_loss) {
-        hipLaunchKernelGGL(k_loss_sum, dim3(1), dim3(MAX_GROUPS), 0, s, part, (int)groups, mean, d_loss, d_count);
+        hipLaunchKernelGGL(k_loss_sum, dim3(1), dim3(SUM_WG), 0, s, part, (int)groups, mean, d_loss, d_count);
         BOA_HIP_TRY(hipGetLastError());
     }
     return BOA_OK;

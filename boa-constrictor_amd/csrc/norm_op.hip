@@ -168,14 +168,23 @@ __global__ void __launch_bounds__(WG) k_norm_bwd(const void* dyp, int64_t dys, c
     }
 }
 
-constexpr int SUM_COLS = 32, SUM_GROUPS = 32;  // columns per workgroup, threads per column
+constexpr int SUM_COLS = 32, SUM_GROUPS = 32, SUM_AT_ONCE = 8;  // columns per workgroup, threads per column, loads in flight
 __global__ void __launch_bounds__(SUM_COLS * SUM_GROUPS) k_sum_parts(const float* part, int64_t parts, int64_t width, float* out) {
     __shared__ float s[SUM_GROUPS][SUM_COLS + 1];
     const int c = threadIdx.x % SUM_COLS, g = threadIdx.x / SUM_COLS;
     const int64_t j = (int64_t)blockIdx.x * SUM_COLS + c;
     float v = 0.0f;
     if (j < width)
-        for (int64_t p = g; p < parts; p += SUM_GROUPS) v += part[p * width + j];
+        for (int64_t p0 = g; p0 < parts; p0 += SUM_GROUPS * SUM_AT_ONCE) {
+            float t[SUM_AT_ONCE];
+#pragma unroll
+            for (int i = 0; i < SUM_AT_ONCE; ++i) {
+                const int64_t p = p0 + i * SUM_GROUPS;
+                t[i] = p < parts ? part[p * width + j] : 0.0f;
+            }
+#pragma unroll
+            for (int i = 0; i < SUM_AT_ONCE; ++i) v += t[i];
+        }
     s[g][c] = v;
     __syncthreads();
     if (g == 0 && j < width) {
@@ -192,10 +201,12 @@ int64_t bwd_groups(int64_t rows) {
     return n < 1024 ? n : 1024;
 }
 
-// Calls f with the row shape for width d: 16-byte accesses where the rows are aligned for them, else single elements.
+// Calls f with the row shape for width d: accesses of 16 bytes (8 for 16-bit rows of up to 256 values, which then take all 64
+// lanes) where the rows are aligned for them, else single elements.
 template <int DT, class F>
 int with_row(int d, bool aligned, F f) {
     constexpr int W = wide<DT>();
+    if (aligned && d % 4 == 0 && d <= 256) return f(Row<DT, 4, 1>());
     if (aligned && d % W == 0) {
         const int n = (int)ceil_div(d, 64 * W);
         if (n <= 1) return f(Row<DT, W, 1>());

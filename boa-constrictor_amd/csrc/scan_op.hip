@@ -25,12 +25,6 @@ using namespace boa;
 
 namespace {
 
-#ifndef BWDW
-#define BWDW 4
-#endif
-#ifndef FETCH_AT
-#define FETCH_AT 4
-#endif
 constexpr int NS = 16, WAVES = 4, NQ = NS / WAVES;
 constexpr int SUB = BOA_SCAN_MARK, MINE = SUB / WAVES;  // positions of a block, and those a wavefront prepares and finishes
 constexpr int WG = 64 * WAVES;
@@ -469,7 +463,7 @@ __global__ void __launch_bounds__(WG) k_scan_bwd_local(const ScanArgs a) {
 
 // ALL: every lane has a channel (channels a multiple of 64), so the stores need no lane mask.
 template <int DT, bool ALL>
-__global__ void __launch_bounds__(WG, BWDW) k_scan_bwd(const ScanArgs a) {
+__global__ void __launch_bounds__(WG, 4) k_scan_bwd(const ScanArgs a) {
     using E = Elem<DT>;
     __shared__ float2 s_in[SUB][64];  // dt, dt u
     __shared__ float s_g[SUB][64];
@@ -585,7 +579,7 @@ __global__ void __launch_bounds__(WG, BWDW) k_scan_bwd(const ScanArgs a) {
             }
             const float v = sum8(r, p.lane);
             bc = (p.lane & 7) == SUB / 2 + s0 / 2 ? v : bc;
-            if (s0 == FETCH_AT) {  // the next block's loads, where registers come free
+            if (s0 == SUB / 2) {  // the next block's loads, where registers come free
                 in.back(i > 0);
                 marks -= i > 0 ? NS * a.channels : 0;
                 fetch(i > 0 ? SUB : count - t0);
@@ -707,16 +701,22 @@ __global__ void __launch_bounds__(WG) k_scan_step(const ScanArgs a) {
 
 Rows rows(const boa_rows& r) { return {r.p, r.batch_stride, r.row_stride}; }
 
-// The split over the length: chunks of a multiple of SUB positions, as many as give WANT workgroups (4 per CU), at least
-// MIN_CHUNK positions each and at most MAX_CHUNKS (each workgroup goes over the chunks before its own).
+// The split over the length: chunks of a multiple of SUB positions, as many as give the wanted workgroups, at least MIN_CHUNK
+// positions each and at most MAX_CHUNKS (each workgroup goes over the chunks before its own).
 struct Plan {
     int chunks;
     int64_t chunk;
 };
-constexpr int64_t WANT = 1024, MIN_CHUNK = 64, MAX_CHUNKS = 64;
-Plan plan(const boa_scan* s) {
+// Workgroups: of sequences as long as the batch, six per CU in the forward pass and four in the backward pass, which is what
+// its registers let run at once (2 x 16384 positions of 512 channels: 4 and 6 per CU forward 131 and 129 us, backward 248
+// and 273; 4 x 4097 of 1024 in bfloat16 forward 92 and 88).  Where lengths differ, smaller ones even out what the CUs have to do
+// (32 sequences of up to 500 positions, 1024 channels, bfloat16: forward 84 us with 1024, 68 with 2048, 64 with 4096; backward
+// 194, 161, 142).
+int64_t wanted_workgroups(const boa_scan* s, bool backward) { return s->lens ? 4096 : backward ? 1024 : 1536; }
+constexpr int64_t MIN_CHUNK = 64, MAX_CHUNKS = 128;
+Plan plan(const boa_scan* s, bool backward) {
     const int64_t blocks = s->batch * ceil_div(s->channels, 64);
-    int64_t n = ceil_div(WANT, blocks > 0 ? blocks : 1);
+    int64_t n = ceil_div(wanted_workgroups(s, backward), blocks > 0 ? blocks : 1);
     n = n < MAX_CHUNKS ? n : MAX_CHUNKS;
     int64_t chunk = ceil_div(ceil_div(s->length, n), SUB) * SUB;
     chunk = chunk > MIN_CHUNK ? chunk : MIN_CHUNK;
@@ -732,7 +732,7 @@ struct Work {
 Work work_of(const boa_scan* s, bool backward) {
     Work w = {};
     if (s->batch < 1 || s->length < 1) return w;
-    const Plan p = plan(s);
+    const Plan p = plan(s, backward);
     const int64_t c = s->channels;
     if (p.chunks > 1) w.local = s->batch * p.chunks * NS * c, w.dts = s->batch * p.chunks * c;
     if (backward) {
@@ -755,7 +755,7 @@ bool bc_aligned(const boa_scan* s, const boa_rows& r) {
     return s->dtype == BOA_DT_F32 || ((uintptr_t)r.p % 4 == 0 && r.batch_stride % 2 == 0 && r.row_stride % 2 == 0);
 }
 
-int check_scan(const char* who, const boa_scan* s, ScanArgs& a) {
+int check_scan(const char* who, const boa_scan* s, ScanArgs& a, bool backward) {
     if (!s) return boa_fail(BOA_ERR_ARG, "%s: null arguments", who);
     if (s->dtype < BOA_DT_F32 || s->dtype > BOA_DT_F16) return boa_fail(BOA_ERR_ARG, "%s: unknown type %d", who, s->dtype);
     if (s->batch < 0 || s->length < 0 || s->channels < 1 || s->channels > BOA_OPS_MAX_CHANNELS)
@@ -774,7 +774,7 @@ int check_scan(const char* who, const boa_scan* s, ScanArgs& a) {
     a.A = s->a, a.D = s->d, a.bias = s->delta_bias, a.lens = s->lens, a.state_in = s->state_in, a.state_out = s->state_out;
     a.marks = s->marks, a.channels = s->channels, a.cblocks = (int)ceil_div(s->channels, 64);
     a.batch = s->batch, a.length = s->length, a.subs = ceil_div(s->length, SUB);
-    const Plan pl = plan(s);
+    const Plan pl = plan(s, backward);
     a.chunks = pl.chunks, a.chunk = pl.chunk;
     if (a.batch > MAX_BLOCKS / ((int64_t)a.cblocks * a.chunks))
         return boa_fail(BOA_ERR_ARG, "%s: batch of %lld sequences too large", who, (long long)a.batch);
@@ -790,7 +790,7 @@ extern "C" int64_t boa_selective_scan_work_bytes(const boa_scan* s, int backward
 
 extern "C" int boa_selective_scan_fwd(const boa_scan* s, void* d_work, int64_t work_bytes, void* stream) {
     ScanArgs a;
-    const int rc = check_scan("boa_selective_scan_fwd", s, a);
+    const int rc = check_scan("boa_selective_scan_fwd", s, a, false);
     if (rc != BOA_OK) return rc;
     if (a.batch == 0 || (a.length == 0 && !a.state_out)) return BOA_OK;
     if (a.length > 0 && !a.y.p) return boa_fail(BOA_ERR_ARG, "boa_selective_scan_fwd: null pointer");
@@ -817,7 +817,7 @@ extern "C" int boa_selective_scan_fwd(const boa_scan* s, void* d_work, int64_t w
 
 extern "C" int boa_selective_scan_bwd(const boa_scan* s, void* d_work, int64_t work_bytes, void* stream) {
     ScanArgs a;
-    const int rc = check_scan("boa_selective_scan_bwd", s, a);
+    const int rc = check_scan("boa_selective_scan_bwd", s, a, true);
     if (rc != BOA_OK) return rc;
     const bool any = a.batch > 0 && a.length > 0;
     if (!s->dpar) return boa_fail(BOA_ERR_ARG, "boa_selective_scan_bwd: null pointer");
@@ -858,7 +858,7 @@ extern "C" int boa_selective_scan_bwd(const boa_scan* s, void* d_work, int64_t w
 
 extern "C" int boa_selective_scan_step(const boa_scan* s, void* stream) {
     ScanArgs a;
-    const int rc = check_scan("boa_selective_scan_step", s, a);
+    const int rc = check_scan("boa_selective_scan_step", s, a, false);
     if (rc != BOA_OK) return rc;
     if (a.batch == 0) return BOA_OK;
     if (a.length != 1) return boa_fail(BOA_ERR_ARG, "boa_selective_scan_step: one position per sequence (got %lld)", (long long)a.length);
