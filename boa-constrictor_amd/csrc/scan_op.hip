@@ -55,6 +55,18 @@ __device__ __forceinline__ typename Elem<DT>::T* row_mut(const Rows& a, int64_t 
     return static_cast<typename Elem<DT>::T*>(const_cast<void*>(a.p)) + b * a.b + t * a.r;
 }
 
+// An offset that the compiler takes for a new one.  A lane's: an address is then a uniform one and a 32-bit offset that is seen
+// where it is used, without arithmetic in the lanes; else the sums are carried through the loop in vector registers, two for each
+// array.  A row's: else the address of every row of a block is carried in scalar registers, 32 of them.
+__device__ __forceinline__ uint32_t fresh(uint32_t& c) {
+    asm volatile("" : "+v"(c));
+    return c;
+}
+__device__ __forceinline__ uint32_t fresh_scalar(uint32_t c) {
+    asm volatile("" : "+s"(c));
+    return c;
+}
+
 // This wavefront's states of B or C in the rows of a block, through the scalar cache (constant address space: nothing the
 // kernel writes; 16-bit rows are 4-byte aligned, and a block of rows spans less than 2 GiB, which the entry points check).
 // A row's place is a 32-bit offset from the block's first: one scalar multiplication, where 64-bit addresses of single rows
@@ -68,6 +80,7 @@ struct ScalarRows {
         : p((const char*)(row<DT>(a, b, t) + q * NQ)), bytes((uint32_t)a.r * (uint32_t)sizeof(typename Elem<DT>::T)) {}
     __device__ __forceinline__ void ahead() { p += bytes * SUB; }
     __device__ __forceinline__ void back() { p -= bytes * SUB; }
+    __device__ __forceinline__ void next_block() { bytes = fresh_scalar(bytes); }
     __device__ __forceinline__ void load(int s, uint32_t (&w)[WORDS]) const {
         typedef __attribute__((address_space(4))) const char CByte;
         typedef __attribute__((address_space(4))) const uint32_t CWord;
@@ -113,22 +126,15 @@ struct LaneRows {
         : p((gmut<char>)row_mut<DT>(a, b, t)), bytes((uint32_t)a.r * (uint32_t)sizeof(T)) {}
     __device__ __forceinline__ void ahead(bool on) { p += on ? bytes * SUB : 0; }
     __device__ __forceinline__ void back(bool on) { p -= on ? bytes * SUB : 0; }
-    // c: the lane's channel in bytes (a 32-bit offset in bytes from a uniform address: no address arithmetic in the lanes)
-    __device__ __forceinline__ gmut<T> at(int s, uint32_t c) const { return (gmut<T>)(p + (uint32_t)s * bytes + c); }
-    __device__ __forceinline__ T load(int s, uint32_t c) const { return *at(s, c); }
-    __device__ __forceinline__ void store(int s, uint32_t c, float v) const { *at(s, c) = Elem<DT>::st(v); }
+    // c: the lane's channel in bytes
+    __device__ __forceinline__ gmut<T> at(int s, uint32_t& c) const { return (gmut<T>)(p + (uint32_t)s * bytes + fresh(c)); }
+    __device__ __forceinline__ T load(int s, uint32_t& c) const { return *at(s, c); }
+    __device__ __forceinline__ void store(int s, uint32_t& c, float v) const { *at(s, c) = Elem<DT>::st(v); }
 };
 
 // Element `c4` bytes from p: the same for float32 arrays.
-__device__ __forceinline__ gmut<float> lane_at(gmut<float> p, uint32_t c4) { return (gmut<float>)((gmut<char>)p + c4); }
-__device__ __forceinline__ gptr<float> lane_at(gptr<float> p, uint32_t c4) { return (gptr<float>)((gptr<char>)p + c4); }
-
-// A lane offset that the compiler takes for a new one: it would add it to the rows' addresses ahead of the loop and keep those
-// in vector registers, two for each array.
-__device__ __forceinline__ uint32_t fresh(uint32_t c) {
-    asm volatile("" : "+v"(c));
-    return c;
-}
+__device__ __forceinline__ gmut<float> lane_at(gmut<float> p, uint32_t& c4) { return (gmut<float>)((gmut<char>)p + fresh(c4)); }
+__device__ __forceinline__ gptr<float> lane_at(gptr<float> p, uint32_t& c4) { return (gptr<float>)((gptr<char>)p + fresh(c4)); }
 
 // A loaded value in a register of its own.  Where a float32 value is used later than the next block's load is issued, the
 // compiler otherwise takes the loaded register over, loads into another, and waits for that load at the end of the iteration
@@ -272,7 +278,7 @@ __global__ void __launch_bounds__(WG) k_scan_fwd(const ScanArgs a) {
         fetch(more);
     }
     for (int i = 0; i < n_subs; ++i) {
-        ce = fresh(ce), c4 = fresh(c4);
+        xB.next_block(), xC.next_block();
         __syncthreads();
         if constexpr (MODE == OUT_MARKS) {
 #pragma unroll
@@ -339,7 +345,15 @@ __global__ void __launch_bounds__(WG) k_scan_fwd(const ScanArgs a) {
     }
 }
 
-// Sums of 8 values over the wavefront; lane l gets the sum of value l / 8.
+// Sums over the wavefront of 8 values (dB or dC of two positions) of four pairs of positions.  A step of the butterfly halves
+// the values that a lane carries: where two of them meet, one half of the lanes goes on with one, the other with the other.
+// join: lanes with the bit go on with b, the others with a.  sum8: value l / 8 of lane l, still spread over its 8 lanes.
+template <int BIT, int CTRL>
+__device__ __forceinline__ float join(float a, float b, int lane) {
+    const bool up = (lane & BIT) != 0;
+    const float keep = up ? b : a, give = up ? a : b;  // in all lanes: a lane reads what another one gives
+    return keep + dpp<CTRL>(give);
+}
 __device__ __forceinline__ float sum8(float (&v)[8], int lane) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -351,13 +365,13 @@ __device__ __forceinline__ float sum8(float (&v)[8], int lane) {
         swap16(v[i], v[i + 2]);
         v[i] += v[i + 2];
     }
-    const bool up = (lane & 8) != 0;
-    float keep = up ? v[1] : v[0], give = up ? v[0] : v[1];
-    keep += dpp<DPP_ROR8>(give);
-    keep += dpp<DPP_HALF_MIRROR>(keep);
-    keep += dpp<DPP_XOR2>(keep);
-    keep += dpp<DPP_XOR1>(keep);
-    return keep;
+    return join<8, DPP_ROR8>(v[0], v[1], lane);
+}
+// Pairs 0 .. 3 (in this order): lane l gets value l / 8 of pair l / 4 % 2 + 2 (l / 2 % 2), the same in lanes 2 i and 2 i + 1.
+__device__ __forceinline__ float join01(float a, float b, int lane) { return join<4, DPP_HALF_MIRROR>(a, b, lane); }
+__device__ __forceinline__ float join0123(float a, float b, int lane) {
+    const float v = join<2, DPP_XOR2>(a, b, lane);
+    return v + dpp<DPP_XOR1>(v);
 }
 
 // The same rows, which the compiler takes for others: on the way back B and C are loaded again rather than kept (64 scalar
@@ -380,7 +394,7 @@ struct BackIn {
         : xu(a.u, p.b, t), xd(a.delta, p.b, t), xz(a.z.p != nullptr ? a.z : a.dy, p.b, t), xy(a.dy, p.b, t), first(p.q * MINE) {}
     __device__ __forceinline__ void back(bool on) { xu.back(on), xd.back(on), xz.back(on), xy.back(on); }
     // left: positions from the block's first one to the end
-    __device__ __forceinline__ void fetch(int left, uint32_t ce) {
+    __device__ __forceinline__ void fetch(int left, uint32_t& ce) {
 #pragma unroll
         for (int k = 0; k < MINE; ++k) {
             const int s = min(first + k, left - 1);  // rows behind the end are read as the last one
@@ -423,7 +437,7 @@ __global__ void __launch_bounds__(WG) k_scan_bwd_local(const ScanArgs a) {
     in.back(n_subs > 1);
     in.fetch(n_subs > 1 ? SUB : count, ce);
     for (int i = n_subs - 1; i >= 0; --i) {
-        ce = fresh(ce);
+        xC.next_block();
         __syncthreads();
         const int last = min(SUB, count - i * SUB) - 1;  // rows behind the end are read as the last one
         Pair<DT> pair[2];
@@ -480,7 +494,7 @@ __global__ void __launch_bounds__(WG, 4) k_scan_bwd(const ScanArgs a) {
     float dD = 0.0f, dbias = 0.0f, mark[NQ];
     const int count = (int)(min(hi, end) - lo), rows_out = (int)(hi - lo);
     const int64_t t_last = lo + (int64_t)max(n_subs - 1, 0) * SUB;  // the block to start with
-    uint32_t ce = p.cc * (uint32_t)sizeof(typename E::T), c4 = p.cc * 4;  // the lane's channel in bytes
+    uint32_t ce = p.cc * (uint32_t)sizeof(typename E::T), c4 = p.cc * 4, tid4 = threadIdx.x * 4;  // the lane's channel in bytes
     BackIn<DT, false> in(a, p, t_last);
     LaneRows<DT> yu(a.du, p.b, t_last), yd(a.ddelta, p.b, t_last), yz(gate ? a.dz : a.du, p.b, t_last);
     ScalarRows<DT> xB(a.B, p.b, t_last, p.q), xC(a.C, p.b, t_last, p.q);
@@ -494,7 +508,7 @@ __global__ void __launch_bounds__(WG, 4) k_scan_bwd(const ScanArgs a) {
     // whole: all the block's positions are inside (all blocks but the first one here)
     auto block = [&](int i, auto whole) {
         constexpr bool WHOLE = decltype(whole)::value;
-        ce = fresh(ce), c4 = fresh(c4);
+        xB.next_block(), xC.next_block();
         const int t0 = i * SUB;  // in the chunk
         float u[MINE], sig[MINE], dyz[MINE];
 #pragma unroll
@@ -509,7 +523,8 @@ __global__ void __launch_bounds__(WG, 4) k_scan_bwd(const ScanArgs a) {
             s_in[at][p.lane] = make_float2(dt, dt * u[k]);
             s_g[at][p.lane] = g;
         }
-        float h[NQ], e[SUB][NQ], eh[SUB][NQ], bc = 0.0f;
+        float h[NQ], e[SUB][NQ], eh[SUB][NQ], half = 0.0f, low = 0.0f, dC = 0.0f, bc = 0.0f;
+        static_assert(SUB == 8, "four pairs");
 #pragma unroll
         for (int n = 0; n < NQ; ++n) h[n] = live ? mark[n] : 0.0f;
         __syncthreads();
@@ -550,9 +565,11 @@ __global__ void __launch_bounds__(WG, 4) k_scan_bwd(const ScanArgs a) {
                 }
                 s_y[p.q][s][p.lane] = y;
             }
-            // the two positions' dC: lane l has the one of position s0 + l / 32, state (l / 8) % 4
+            // the two positions' dC: value 4 j + n
             const float v = sum8(r, p.lane);
-            bc = (p.lane & 7) == s0 / 2 ? v : bc;
+            if (s0 % 4 == 0) half = v;
+            else if (s0 == 2) low = join01(half, v, p.lane);
+            else dC = join0123(low, join01(half, v, p.lane), p.lane);
         }
         const ScalarRows<DT> xB2 = again(xB), xC2 = again(xC);
 #pragma unroll
@@ -578,7 +595,9 @@ __global__ void __launch_bounds__(WG, 4) k_scan_bwd(const ScanArgs a) {
                 s_w[p.q][s][p.lane] = sw;
             }
             const float v = sum8(r, p.lane);
-            bc = (p.lane & 7) == SUB / 2 + s0 / 2 ? v : bc;
+            if (s0 % 4 != 0) half = v;
+            else if (s0 == 4) low = join01(v, half, p.lane);
+            else bc = join0123(join01(v, half, p.lane), low, p.lane);
             if (s0 == SUB / 2) {  // the next block's loads, where registers come free
                 in.back(i > 0);
                 marks -= i > 0 ? NS * a.channels : 0;
@@ -586,7 +605,7 @@ __global__ void __launch_bounds__(WG, 4) k_scan_bwd(const ScanArgs a) {
             }
         }
         xB.back(), xC.back();
-        *lane_at(bc_out, threadIdx.x * 4) = bc;
+        *lane_at(bc_out, tid4) = (p.lane & 1) ? bc : dC;
         bc_out -= WG;
         __syncthreads();
 #pragma unroll
@@ -654,12 +673,12 @@ __global__ void __launch_bounds__(WG) k_scan_sum_bc(const ScanArgs a) {
     const int lane = threadIdx.x & 63, q = threadIdx.x >> 6;
     for (int64_t k = blockIdx.x; k < a.batch * a.subs; k += gridDim.x) {
         const int64_t b = k / a.subs, i = k % a.subs;
-        const int64_t end = end_of(a, b), t = i * SUB + (lane & 3) * 2 + (lane >> 5);
+        const int64_t end = end_of(a, b), t = i * SUB + ((lane >> 2 & 1) + (lane & 2)) * 2 + (lane >> 5);
         if (t >= a.length) continue;
         float v = 0.0f;
         if (t < end)
             for (int cb = 0; cb < a.cblocks; ++cb) v += a.part_bc[(((int64_t)cb * a.batch + b) * a.subs + i) * WG + threadIdx.x];
-        row_mut<DT>((lane & 4) ? a.dB : a.dC, b, t)[q * NQ + ((lane >> 3) & 3)] = Elem<DT>::st(v);
+        row_mut<DT>((lane & 1) ? a.dB : a.dC, b, t)[q * NQ + ((lane >> 3) & 3)] = Elem<DT>::st(v);
     }
 }
 
