@@ -479,6 +479,8 @@ def selective_scan_step(u, delta, A, B, C, D=None, z=None, delta_bias=None, *, s
     _gpu(who, u)
     y = u.new_empty((n, c))
     u, delta, A, B, C, D, z, bias = args
+    if A.data_ptr() % 16:
+        A = A.clone()
 
     def r2(t):
         return _NO_ROWS if t is None else (t.data_ptr(), t.stride(0), 0)

@@ -19,11 +19,14 @@ constexpr int MAX_V = BOA_CROSS_ENTROPY_MAX_V;
 constexpr int MAX_GROUPS = 2048;
 
 // Rows that a wavefront has in flight, for PER elements per lane.
-constexpr int rows_at_once(int per) { return per >= 32 ? 1 : 32 / per; }
+constexpr int rows_at_once(int per) { return per >= 32 ? 1 : 32 / per; }  // 8, 4, 2 or 1
 
-__device__ __forceinline__ int64_t target_at(const void* t, int bytes, int64_t r) {
-    return bytes == 1 ? (int64_t)static_cast<const uint8_t*>(t)[r]
-           : bytes == 4 ? (int64_t)static_cast<const int32_t*>(t)[r] : static_cast<const int64_t*>(t)[r];
+// Row r's symbol, or what its target is instead of one.
+constexpr int NOT_A_SYMBOL = -1, IGNORED = -2;
+__device__ __forceinline__ int symbol_at(const void* target, int bytes, int64_t ignore, int V, int64_t r) {
+    const int64_t t = bytes == 1 ? (int64_t)static_cast<const uint8_t*>(target)[r]
+                      : bytes == 4 ? (int64_t)static_cast<const int32_t*>(target)[r] : static_cast<const int64_t*>(target)[r];
+    return t == ignore ? IGNORED : t >= 0 && t < V ? (int)t : NOT_A_SYMBOL;
 }
 
 template <int DT, int VEC, int N>
@@ -31,6 +34,17 @@ struct Row {
     static constexpr int VECTOR = VEC, COUNT = N, PER = N * VEC;
     using T = typename Elem<DT>::T;
     static __device__ __forceinline__ int col(int i, int lane) { return (i * 64 + lane) * VEC; }
+    // a row, `other` behind its end; without branches, so that the loads of several rows go out together (V >= VEC)
+    static __device__ __forceinline__ void load(const T* row, int V, int lane, float other, float (&v)[PER]) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int c = col(i, lane);
+            float e[VEC];
+            ld_vec<DT, VEC>(row + (c < V ? c : V - VEC), e);
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) v[i * VEC + j] = c < V ? e[j] : other;
+        }
+    }
 };
 
 template <int DT, int VEC, int N>
@@ -45,56 +59,49 @@ __global__ void __launch_bounds__(WG) k_loss_fwd(const void* xp, int64_t xs, con
     const int64_t wave = (int64_t)blockIdx.x * WAVES + wid, waves = (int64_t)gridDim.x * WAVES;
     double total = 0.0, count = 0.0;
     for (int64_t r0 = wave * ROWS; r0 < rows; r0 += waves * ROWS) {
+        constexpr int EACH = 64 / ROWS;
+        const int64_t my_row = r0 + lane / EACH;  // of the ROWS rows the one whose values this lane ends with
         float v[ROWS][PER];
-        int64_t t[ROWS];
+#pragma unroll
+        for (int r = 0; r < ROWS; ++r) R::load(x + min(r0 + r, rows - 1) * xs, V, lane, -__builtin_huge_valf(), v[r]);
+        const int symbol = symbol_at(target, target_bytes, ignore, V, min(my_row, rows - 1));
+        // Over the lanes all the rows go together (reduce): lane l ends with those of row l / EACH, and takes that row's
+        // logarithm.  A NaN is dropped by the maximum but not by the exponentials' sum.
+        // the target's logit, by the lanes that will need it (the row is on its way to the cache already)
+        const float x_t = Elem<DT>::ld(x[min(my_row, rows - 1) * xs + (symbol >= 0 ? symbol : 0)]);
+        float m[ROWS], s[ROWS];
 #pragma unroll
         for (int r = 0; r < ROWS; ++r) {
-            const int64_t at = r0 + r < rows ? r0 + r : rows - 1;
+            m[r] = v[r][0];
 #pragma unroll
-            for (int i = 0; i < N; ++i) {
-                float e[VEC];
-#pragma unroll
-                for (int j = 0; j < VEC; ++j) e[j] = -__builtin_huge_valf();
-                if (R::col(i, lane) < V) ld_vec<DT, VEC>(x + at * xs + R::col(i, lane), e);
-#pragma unroll
-                for (int j = 0; j < VEC; ++j) v[r][i * VEC + j] = e[j];
-            }
-            t[r] = target_at(target, target_bytes, at);
+            for (int i = 1; i < PER; ++i) m[r] = fmaxf(m[r], v[r][i]);
         }
+        const float mine = reduce<Max, ROWS>(m, lane);
 #pragma unroll
         for (int r = 0; r < ROWS; ++r) {
-            if (r0 + r >= rows) break;
-            float m = v[r][0];
-            bool nan = false;  // fmaxf drops a NaN
+            m[r] = from_lane(mine, r * EACH);
+            s[r] = 0.0f;
 #pragma unroll
-            for (int i = 0; i < PER; ++i) {
-                m = fmaxf(m, v[r][i]);
-                nan |= v[r][i] != v[r][i];
-            }
-            m = wmax(m);
-            if (__any(nan)) m = __builtin_nanf("");
-            float s = 0.0f, hit = 0.0f;  // the target's logit, from the lane that has it
-#pragma unroll
-            for (int i = 0; i < PER; ++i) {
-                const int c = R::col(i / VEC, lane);
-                s += c < V ? hw_exp(v[r][i] - m) : 0.0f;
-                hit = c + i % VEC == t[r] ? v[r][i] : hit;
-            }
-            s = wsum(s);
-            float loss = logf(s) + (m - wsum(hit));
-            const bool kept = t[r] != ignore;
-            if (t[r] < 0 || t[r] >= V) loss = __builtin_nanf("");
+            for (int i = 0; i < PER; ++i) s[r] += hw_exp(v[r][i] - m[r]);  // columns behind the last: -inf
+        }
+        const float total_s = reduce<Add, ROWS>(s, lane);
+        float loss = logf(total_s) + (mine - x_t);
+        const bool kept = symbol != IGNORED;
+        if (symbol == NOT_A_SYMBOL) loss = __builtin_nanf("");
+        if (lane % EACH == 0 && my_row < rows) {
             if (kept) {
                 total += (double)loss;
                 count += 1.0;
             }
-            if (lane == 0) {
-                if (stats != nullptr) stats[r0 + r] = make_float2(m, 1.0f / s);
-                if (losses != nullptr) losses[r0 + r] = kept ? loss : 0.0f;
-            }
+            if (stats != nullptr) stats[my_row] = make_float2(mine, 1.0f / total_s);
+            if (losses != nullptr) losses[my_row] = kept ? loss : 0.0f;
         }
     }
     if (part == nullptr) return;
+    for (int o = 32; o > 0; o >>= 1) {
+        total += __shfl_xor(total, o, 64);
+        count += __shfl_xor(count, o, 64);
+    }
     if (lane == 0) sum[wid] = make_double2(total, count);
     __syncthreads();
     if (threadIdx.x == 0) {
@@ -143,35 +150,27 @@ __global__ void __launch_bounds__(WG) k_loss_bwd(const void* xp, int64_t xs, con
     const int64_t wave = (int64_t)blockIdx.x * WAVES + (threadIdx.x >> 6), waves = (int64_t)gridDim.x * WAVES;
     const float all = up_rows ? 0.0f : up[0] / (count != nullptr ? *count : 1.0f);
     for (int64_t r0 = wave * ROWS; r0 < rows; r0 += waves * ROWS) {
-        float v[ROWS][PER], scale[ROWS];
-        float2 st[ROWS];
-        int64_t t[ROWS];
+        constexpr int EACH = 64 / ROWS;
+        float v[ROWS][PER];
 #pragma unroll
-        for (int r = 0; r < ROWS; ++r) {
-            const int64_t at = r0 + r < rows ? r0 + r : rows - 1;
-#pragma unroll
-            for (int i = 0; i < N; ++i) {
-                float e[VEC] = {};
-                if (R::col(i, lane) < V) ld_vec<DT, VEC>(x + at * xs + R::col(i, lane), e);
-#pragma unroll
-                for (int j = 0; j < VEC; ++j) v[r][i * VEC + j] = e[j];
-            }
-            t[r] = target_at(target, target_bytes, at);
-            st[r] = stats[at];
-            scale[r] = up_rows ? up[at] : all;
-        }
+        for (int r = 0; r < ROWS; ++r) R::load(x + min(r0 + r, rows - 1) * xs, V, lane, 0.0f, v[r]);
+        const int64_t my_row = min(r0 + lane / EACH, rows - 1);  // a lane reads one row's values for all
+        const int my_symbol = symbol_at(target, target_bytes, ignore, V, my_row);
+        const float2 my_stats = stats[my_row];
+        const float my_scale = my_symbol == NOT_A_SYMBOL ? __builtin_nanf("") : up_rows ? up[my_row] : all;
 #pragma unroll
         for (int r = 0; r < ROWS; ++r) {
             if (r0 + r >= rows) break;
-            const bool kept = t[r] != ignore;
-            const float k = (t[r] < 0 || t[r] >= V) ? __builtin_nanf("") : scale[r];
+            const int symbol = __builtin_amdgcn_readlane(my_symbol, r * EACH);
+            const float m = from_lane(my_stats.x, r * EACH), inv = from_lane(my_stats.y, r * EACH), k = from_lane(my_scale, r * EACH);
+            const bool kept = symbol != IGNORED;
 #pragma unroll
             for (int i = 0; i < N; ++i) {
                 float e[VEC];
 #pragma unroll
                 for (int j = 0; j < VEC; ++j) {
-                    const float p = hw_exp(v[r][i * VEC + j] - st[r].x) * st[r].y;
-                    const float q = R::col(i, lane) + j == t[r] ? p - 1.0f : p;
+                    const float p = hw_exp(v[r][i * VEC + j] - m) * inv;
+                    const float q = R::col(i, lane) + j == symbol ? p - 1.0f : p;
                     e[j] = kept ? q * k : 0.0f;
                 }
                 if (R::col(i, lane) < V) st_vec<DT, VEC>(dx + (r0 + r) * dxs + R::col(i, lane), e);

@@ -26,14 +26,16 @@ struct Row {
     static constexpr int VECTOR = VEC, COUNT = N, PER = N * VEC;
     using T = typename Elem<DT>::T;
     static __device__ __forceinline__ int col(int i, int lane) { return (i * 64 + lane) * VEC; }
-    // elements beyond d read as 0 (d is a multiple of VEC, so a vector is inside or outside as a whole)
+    // elements beyond d read as 0 (d is a multiple of VEC, so a vector is inside or outside as a whole); without branches, so
+    // that the loads of several rows go out together
     static __device__ __forceinline__ void load(const T* row, int d, int lane, float (&v)[PER]) {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            float t[VEC] = {};
-            if (col(i, lane) < d) ld_vec<DT, VEC>(row + col(i, lane), t);
+            const int c = col(i, lane);
+            float t[VEC];
+            ld_vec<DT, VEC>(row + (c < d ? c : d - VEC), t);
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) v[i * VEC + j] = t[j];
+            for (int j = 0; j < VEC; ++j) v[i * VEC + j] = c < d ? t[j] : 0.0f;
         }
     }
     static __device__ __forceinline__ void store(T* row, int d, int lane, const float (&v)[PER]) {

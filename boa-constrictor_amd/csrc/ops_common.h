@@ -101,30 +101,52 @@ __device__ __forceinline__ void swap16(float& a, float& b) {
     a = __uint_as_float(r[0]);
     b = __uint_as_float(r[1]);
 }
+struct Add {
+    static __device__ __forceinline__ float of(float a, float b) { return a + b; }
+};
+struct Max {
+    static __device__ __forceinline__ float of(float a, float b) { return fmaxf(a, b); }
+};
+// R values (1, 2, 4 or 8) over the wavefront; lane l gets value l / (64 / R).  While there are several, a step of the butterfly
+// halves the values that a lane carries instead of the lanes that differ: 18 instructions for 8 values, 10 for one.
+template <int BIT, int CTRL, class Op>
+__device__ __forceinline__ float join(float a, float b, int lane) {
+    const bool up = (lane & BIT) != 0;
+    const float keep = up ? b : a, give = up ? a : b;  // in all lanes: a lane reads what another one gives
+    return Op::of(keep, dpp<CTRL>(give));
+}
+template <class Op, int R>
+__device__ __forceinline__ float reduce(const float (&x)[R], int lane) {
+    float v[R == 1 ? 2 : R];
+#pragma unroll
+    for (int i = 0; i < R; ++i) v[i] = x[i];
+    if constexpr (R == 1) v[1] = v[0];
+    constexpr int H = R >= 2 ? R / 2 : 1;  // values left after the step across halves
+#pragma unroll
+    for (int i = 0; i < H; ++i) {
+        swap32(v[i], v[i + H]);
+        v[i] = Op::of(v[i], v[i + H]);
+    }
+    constexpr int Q = R >= 4 ? R / 4 : 1;  // after the step across rows
+    if constexpr (R < 4) v[1] = v[0];
+#pragma unroll
+    for (int i = 0; i < Q; ++i) {
+        swap16(v[i], v[i + Q]);
+        v[i] = Op::of(v[i], v[i + Q]);
+    }
+    float r;
+    if constexpr (R == 8) r = join<8, DPP_ROR8, Op>(v[0], v[1], lane);
+    else r = Op::of(v[0], dpp<DPP_ROR8>(v[0]));
+    r = Op::of(r, dpp<DPP_HALF_MIRROR>(r));
+    r = Op::of(r, dpp<DPP_XOR2>(r));
+    return Op::of(r, dpp<DPP_XOR1>(r));
+}
 __device__ __forceinline__ float wsum(float v) {
-    v += dpp<DPP_XOR1>(v);
-    v += dpp<DPP_XOR2>(v);
-    v += dpp<DPP_HALF_MIRROR>(v);
-    v += dpp<DPP_ROR8>(v);
-    float w = v;
-    swap16(v, w);
-    v += w;
-    w = v;
-    swap32(v, w);
-    return v + w;
+    const float x[1] = {v};
+    return reduce<Add, 1>(x, 0);
 }
-__device__ __forceinline__ float wmax(float v) {
-    v = fmaxf(v, dpp<DPP_XOR1>(v));
-    v = fmaxf(v, dpp<DPP_XOR2>(v));
-    v = fmaxf(v, dpp<DPP_HALF_MIRROR>(v));
-    v = fmaxf(v, dpp<DPP_ROR8>(v));
-    float w = v;
-    swap16(v, w);
-    v = fmaxf(v, w);
-    w = v;
-    swap32(v, w);
-    return fmaxf(v, w);
-}
+// Lane l's value in all lanes (l the same for all).
+__device__ __forceinline__ float from_lane(float v, int l) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), l)); }
 
 __device__ __forceinline__ float hw_sigmoid(float x) { return __builtin_amdgcn_rcpf(1.0f + hw_exp(-x)); }
 

@@ -348,12 +348,6 @@ __global__ void __launch_bounds__(WG) k_scan_fwd(const ScanArgs a) {
 // Sums over the wavefront of 8 values (dB or dC of two positions) of four pairs of positions.  A step of the butterfly halves
 // the values that a lane carries: where two of them meet, one half of the lanes goes on with one, the other with the other.
 // join: lanes with the bit go on with b, the others with a.  sum8: value l / 8 of lane l, still spread over its 8 lanes.
-template <int BIT, int CTRL>
-__device__ __forceinline__ float join(float a, float b, int lane) {
-    const bool up = (lane & BIT) != 0;
-    const float keep = up ? b : a, give = up ? a : b;  // in all lanes: a lane reads what another one gives
-    return keep + dpp<CTRL>(give);
-}
 __device__ __forceinline__ float sum8(float (&v)[8], int lane) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -365,12 +359,12 @@ __device__ __forceinline__ float sum8(float (&v)[8], int lane) {
         swap16(v[i], v[i + 2]);
         v[i] += v[i + 2];
     }
-    return join<8, DPP_ROR8>(v[0], v[1], lane);
+    return join<8, DPP_ROR8, Add>(v[0], v[1], lane);
 }
 // Pairs 0 .. 3 (in this order): lane l gets value l / 8 of pair l / 4 % 2 + 2 (l / 2 % 2), the same in lanes 2 i and 2 i + 1.
-__device__ __forceinline__ float join01(float a, float b, int lane) { return join<4, DPP_HALF_MIRROR>(a, b, lane); }
+__device__ __forceinline__ float join01(float a, float b, int lane) { return join<4, DPP_HALF_MIRROR, Add>(a, b, lane); }
 __device__ __forceinline__ float join0123(float a, float b, int lane) {
-    const float v = join<2, DPP_XOR2>(a, b, lane);
+    const float v = join<2, DPP_XOR2, Add>(a, b, lane);
     return v + dpp<DPP_XOR1>(v);
 }
 
@@ -682,40 +676,52 @@ __global__ void __launch_bounds__(WG) k_scan_sum_bc(const ScanArgs a) {
     }
 }
 
-// One position: a lane has the 16 states of its channel.
+// One position: a lane has the 16 states of its channel, a wavefront 64 channels of some sequences (A and the parameters are
+// read once for all of them).  Bound by the states' way in and out.
 template <int DT>
-__global__ void __launch_bounds__(WG) k_scan_step(const ScanArgs a) {
+__global__ void __launch_bounds__(WG) k_scan_step(const ScanArgs a, int64_t walkers) {
+    using E = Elem<DT>;
     const int lane = threadIdx.x & 63;
     const int64_t k = (int64_t)blockIdx.x * WAVES + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int64_t b = k / a.cblocks;
     const int c = (int)(k % a.cblocks) * 64 + lane;
-    if (b >= a.batch || c >= a.channels) return;
-    float B[NS], C[NS];
+    const uint32_t cc = (uint32_t)(c < a.channels ? c : a.channels - 1);
+    float a2[NS];
 #pragma unroll
-    for (int i = 0; i < WAVES; ++i) {
-        uint32_t w[ScalarRows<DT>::WORDS], v[ScalarRows<DT>::WORDS];
-        ScalarRows<DT>(a.B, b, 0, i).load(0, w);
-        ScalarRows<DT>(a.C, b, 0, i).load(0, v);
-#pragma unroll
-        for (int j = 0; j < NQ; ++j) B[i * NQ + j] = ScalarRows<DT>::value(w, j), C[i * NQ + j] = ScalarRows<DT>::value(v, j);
+    for (int n = 0; n < NS; n += 4) {
+        const float4 v = reinterpret_cast<const float4*>(a.A)[cc * (NS / 4) + n / 4];
+        a2[n] = v.x * LOG2E, a2[n + 1] = v.y * LOG2E, a2[n + 2] = v.z * LOG2E, a2[n + 3] = v.w * LOG2E;
     }
-    float* st = a.state_out + b * NS * (int64_t)a.channels + c;
-    float h[NS];
+    const float bias = a.bias != nullptr ? a.bias[cc] : 0.0f, D = a.D != nullptr ? a.D[cc] : 0.0f;
+    if (c >= a.channels || k >= walkers * a.cblocks) return;
+    for (int64_t b = k / a.cblocks; b < a.batch; b += walkers) {
+        uint32_t ce = cc * (uint32_t)sizeof(typename E::T), c4 = cc * 4;
+        gmut<float> st = GM(a.state_out) + b * NS * a.channels;
+        float h[NS];
 #pragma unroll
-    for (int n = 0; n < NS; ++n) h[n] = st[n * (int64_t)a.channels];
-    const float u = Elem<DT>::ld(row<DT>(a.u, b, 0)[c]);
-    const float dt = hw_softplus(Elem<DT>::ld(row<DT>(a.delta, b, 0)[c]) + (a.bias != nullptr ? a.bias[c] : 0.0f));
-    const float du = dt * u;
-    float y = (a.D != nullptr ? a.D[c] : 0.0f) * u;
+        for (int n = 0; n < NS; ++n) h[n] = *lane_at(st + (uint32_t)(n * a.channels), c4);
+        const float u = E::ld(LaneRows<DT>(a.u, b, 0).load(0, ce));
+        const float dt = hw_softplus(E::ld(LaneRows<DT>(a.delta, b, 0).load(0, ce)) + bias);
+        const float z = a.z.p != nullptr ? E::ld(LaneRows<DT>(a.z, b, 0).load(0, ce)) : 0.0f;
+        float B[NS], C[NS];
 #pragma unroll
-    for (int n = 0; n < NS; ++n) {
-        const float e = __builtin_amdgcn_exp2f(dt * (a.A[(int64_t)c * NS + n] * LOG2E));
-        h[n] = __builtin_fmaf(e, h[n], B[n] * du);
-        y = __builtin_fmaf(h[n], C[n], y);
-        st[n * (int64_t)a.channels] = h[n];
+        for (int i = 0; i < WAVES; ++i) {
+            uint32_t w[ScalarRows<DT>::WORDS], v[ScalarRows<DT>::WORDS];
+            ScalarRows<DT>(a.B, b, 0, i).load(0, w);
+            ScalarRows<DT>(a.C, b, 0, i).load(0, v);
+#pragma unroll
+            for (int j = 0; j < NQ; ++j) B[i * NQ + j] = ScalarRows<DT>::value(w, j), C[i * NQ + j] = ScalarRows<DT>::value(v, j);
+        }
+        const float du = dt * u;
+        float y = D * u;
+#pragma unroll
+        for (int n = 0; n < NS; ++n) {
+            h[n] = __builtin_fmaf(__builtin_amdgcn_exp2f(dt * a2[n]), h[n], B[n] * du);
+            y = __builtin_fmaf(h[n], C[n], y);
+            *lane_at(st + (uint32_t)(n * a.channels), c4) = h[n];
+        }
+        if (a.z.p != nullptr) y *= hw_silu(z);
+        LaneRows<DT>(a.y, b, 0).store(0, ce, y);
     }
-    if (a.z.p != nullptr) y *= hw_silu(Elem<DT>::ld(row<DT>(a.z, b, 0)[c]));
-    row_mut<DT>(a.y, b, 0)[c] = Elem<DT>::st(y);
 }
 
 Rows rows(const boa_rows& r) { return {r.p, r.batch_stride, r.row_stride}; }
@@ -882,9 +888,12 @@ extern "C" int boa_selective_scan_step(const boa_scan* s, void* stream) {
     if (a.batch == 0) return BOA_OK;
     if (a.length != 1) return boa_fail(BOA_ERR_ARG, "boa_selective_scan_step: one position per sequence (got %lld)", (long long)a.length);
     if (!a.y.p || !a.state_out) return boa_fail(BOA_ERR_ARG, "boa_selective_scan_step: null pointer");
+    if ((uintptr_t)a.A % 16 != 0) return boa_fail(BOA_ERR_ARG, "boa_selective_scan_step: a has to begin at a multiple of 16 bytes");
+    // wavefronts for each block of channels: as many as run at once on 256 CUs (8 on each of their SIMDs), or one per sequence
+    const int64_t walkers = min(a.batch, ceil_div(8192, a.cblocks));
     return with_dtype(s->dtype, [&](auto dt) {
-        hipLaunchKernelGGL((k_scan_step<decltype(dt)::value>), dim3((uint32_t)ceil_div(a.batch * a.cblocks, WAVES)), dim3(WG), 0,
-                           (hipStream_t)stream, a);
+        hipLaunchKernelGGL((k_scan_step<decltype(dt)::value>), dim3((uint32_t)ceil_div(walkers * a.cblocks, WAVES)), dim3(WG), 0,
+                           (hipStream_t)stream, a, walkers);
         BOA_HIP_TRY(hipGetLastError());
         return (int)BOA_OK;
     });

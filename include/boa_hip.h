@@ -299,7 +299,8 @@ int64_t boa_selective_scan_work_bytes(const boa_scan* s, int backward);
 int boa_selective_scan_fwd(const boa_scan* s, void* d_work, int64_t work_bytes, void* stream);
 /* The gradient for everything but the state.  Takes the forward's inputs and marks.                     */
 int boa_selective_scan_bwd(const boa_scan* s, void* d_work, int64_t work_bytes, void* stream);
-/* One position per sequence (length 1): advances state_out in place (lens, state_in and marks are not used). */
+/* One position per sequence (length 1): advances state_out in place (lens, state_in and marks are not used).  `a` begins at
+ * a multiple of 16 bytes.                                                                                */
 int boa_selective_scan_step(const boa_scan* s, void* stream);
 
 #ifdef __cplusplus
