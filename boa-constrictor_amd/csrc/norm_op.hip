@@ -170,30 +170,9 @@ __global__ void __launch_bounds__(WG) k_norm_bwd(const void* dyp, int64_t dys, c
     }
 }
 
-constexpr int SUM_COLS = 32, SUM_GROUPS = 32, SUM_AT_ONCE = 8;  // columns per workgroup, threads per column, loads in flight
+constexpr int SUM_GROUPS = 32;
 __global__ void __launch_bounds__(SUM_COLS * SUM_GROUPS) k_sum_parts(const float* part, int64_t parts, int64_t width, float* out) {
-    __shared__ float s[SUM_GROUPS][SUM_COLS + 1];
-    const int c = threadIdx.x % SUM_COLS, g = threadIdx.x / SUM_COLS;
-    const int64_t j = (int64_t)blockIdx.x * SUM_COLS + c;
-    float v = 0.0f;
-    if (j < width)
-        for (int64_t p0 = g; p0 < parts; p0 += SUM_GROUPS * SUM_AT_ONCE) {
-            float t[SUM_AT_ONCE];
-#pragma unroll
-            for (int i = 0; i < SUM_AT_ONCE; ++i) {
-                const int64_t p = p0 + i * SUM_GROUPS;
-                t[i] = p < parts ? part[p * width + j] : 0.0f;
-            }
-#pragma unroll
-            for (int i = 0; i < SUM_AT_ONCE; ++i) v += t[i];
-        }
-    s[g][c] = v;
-    __syncthreads();
-    if (g == 0 && j < width) {
-        v = s[0][c];
-        for (int k = 1; k < SUM_GROUPS; ++k) v += s[k][c];
-        out[j] = v;
-    }
+    sum_parts<SUM_GROUPS>(part, parts, width, out, blockIdx.x);
 }
 
 int64_t fwd_groups(int64_t rows, int per) { return ceil_div(rows, WAVES * rows_at_once(per)); }

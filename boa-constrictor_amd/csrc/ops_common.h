@@ -170,7 +170,35 @@ inline bool aligned16(int dtype, const void* p, int64_t stride) {
 // Workgroups of 256 threads that one launch dimension takes (its threads are counted in 32 bits).
 constexpr int64_t MAX_BLOCKS = 0xFFFFFF;
 
-// out[j] = sum over p < parts of part[p * width + j], j < width, in a fixed order (norm_op.hip).
+// out[j] = sum over p < parts of part[p * width + j] for the SUM_COLS columns j of block `blk`, in a fixed order, by a workgroup of
+// SUM_COLS x GROUPS threads: a thread adds every GROUPS-th row, eight loads in flight, and the groups' sums follow one another.
+constexpr int SUM_COLS = 32, SUM_AT_ONCE = 8;
+template <int GROUPS>
+__device__ __forceinline__ void sum_parts(const float* part, int64_t parts, int64_t width, float* out, int64_t blk) {
+    __shared__ float s[GROUPS][SUM_COLS + 1];
+    const int c = threadIdx.x % SUM_COLS, g = threadIdx.x / SUM_COLS;
+    const int64_t j = blk * SUM_COLS + c;
+    float v = 0.0f;
+    if (j < width)
+        for (int64_t p0 = g; p0 < parts; p0 += GROUPS * SUM_AT_ONCE) {
+            float t[SUM_AT_ONCE];
+#pragma unroll
+            for (int i = 0; i < SUM_AT_ONCE; ++i) {
+                const int64_t p = p0 + i * GROUPS;
+                t[i] = p < parts ? part[p * width + j] : 0.0f;
+            }
+#pragma unroll
+            for (int i = 0; i < SUM_AT_ONCE; ++i) v += t[i];
+        }
+    s[g][c] = v;
+    __syncthreads();
+    if (g == 0 && j < width) {
+        v = s[0][c];
+        for (int k = 1; k < GROUPS; ++k) v += s[k][c];
+        out[j] = v;
+    }
+}
+// The same as a launch of its own (norm_op.hip).
 hipError_t launch_sum_parts(const float* part, int64_t parts, int64_t width, float* out, hipStream_t s);
 
 }  // namespace boa

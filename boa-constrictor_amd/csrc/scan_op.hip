@@ -661,12 +661,18 @@ __global__ void __launch_bounds__(WG, 4) k_scan_bwd(const ScanArgs a) {
     }
 }
 
-// dB and dC: the sums over the channel blocks, in the activations' type; zeros behind a sequence's end.
+// What the backward pass leaves in parts: dB and dC, the sums over the channel blocks, in the activations' type (zeros behind a
+// sequence's end), by the first bc_blocks workgroups; the parameters' gradients, the sums over the chunks, by the others.
 template <int DT>
-__global__ void __launch_bounds__(WG) k_scan_sum_bc(const ScanArgs a) {
+__global__ void __launch_bounds__(WG) k_scan_sums(const ScanArgs a, int64_t bc_blocks, float* dpar) {
+    if (blockIdx.x >= bc_blocks) {
+        sum_parts<WG / SUM_COLS>(a.part_par, a.batch * a.chunks, (int64_t)(NS + 2) * a.channels, dpar, blockIdx.x - bc_blocks);
+        return;
+    }
     const int lane = threadIdx.x & 63, q = threadIdx.x >> 6;
-    for (int64_t k = blockIdx.x; k < a.batch * a.subs; k += gridDim.x) {
+    for (int64_t k = blockIdx.x; k < a.batch * a.subs; k += bc_blocks) {
         const int64_t b = k / a.subs, i = k % a.subs;
+        // where k_scan_bwd leaves them: see join01 and join0123
         const int64_t end = end_of(a, b), t = i * SUB + ((lane >> 2 & 1) + (lane & 2)) * 2 + (lane >> 5);
         if (t >= a.length) continue;
         float v = 0.0f;
@@ -871,13 +877,16 @@ extern "C" int boa_selective_scan_bwd(const boa_scan* s, void* d_work, int64_t w
             else
                 hipLaunchKernelGGL((k_scan_bwd<DT, false>), dim3(blocks * a.chunks), dim3(WG), 0, st, a);
             BOA_HIP_TRY(hipGetLastError());
-            hipLaunchKernelGGL((k_scan_sum_bc<DT>), dim3((uint32_t)min(a.batch * a.subs, MAX_BLOCKS)), dim3(WG), 0, st, a);
+            const int64_t bc = min(a.batch * a.subs, MAX_BLOCKS / 2);
+            hipLaunchKernelGGL((k_scan_sums<DT>), dim3((uint32_t)(bc + ceil_div((int64_t)(NS + 2) * a.channels, SUM_COLS))), dim3(WG),
+                               0, st, a, bc, s->dpar);
             BOA_HIP_TRY(hipGetLastError());
             return (int)BOA_OK;
         });
         if (launched != BOA_OK) return launched;
+    } else {
+        BOA_HIP_TRY(launch_sum_parts(nullptr, 0, (int64_t)(NS + 2) * a.channels, s->dpar, st));  // zeros
     }
-    BOA_HIP_TRY(launch_sum_parts(a.part_par, any ? a.batch * a.chunks : 0, (int64_t)(NS + 2) * a.channels, s->dpar, st));
     return BOA_OK;
 }
 
