@@ -83,14 +83,16 @@ def _state(who, t, shape, like, dtype, in_place):
     return t
 
 
-def _lens(who, t, batch, like):
+def _lens(who, t, batch, length, like):
     if t is None:
         return None
     if not isinstance(t, torch.Tensor) or t.dtype not in (torch.int32, torch.int64):
         raise TypeError(f"{who}: lens must be an int32 tensor")
     if t.device != like.device or t.shape != (batch,):
         raise ValueError(f"{who}: lens must be [{batch}] on {like.device} (got {list(t.shape)} on {t.device})")
-    return t.to(torch.int32).contiguous()
+    if t.dtype == torch.int64:
+        t = t.clamp(0, length).to(torch.int32)  # what the kernels do with int32
+    return t.contiguous()
 
 
 def _rows(t):
@@ -315,9 +317,9 @@ def causal_conv(x, weight, bias=None, *, silu: bool = True, state=None, lens=Non
     float32 [channels]; state: the three positions before the first one (zeros without).  Returns y, with ``return_state``
     also the state behind each sequence's last position, as a new tensor."""
     w, b = _conv_args("causal_conv", x, 3, weight, bias)
-    n, _, c = x.shape
+    n, length, c = x.shape
     state = _state("causal_conv", state, (n, D_CONV - 1, c), x, x.dtype, False)
-    lens = _lens("causal_conv", lens, n, x)
+    lens = _lens("causal_conv", lens, n, length, x)
     _gpu("causal_conv", x)
     x = _rows(x)
     if _grad(x, w, b):
@@ -454,9 +456,9 @@ def selective_scan(u, delta, A, B, C, D=None, z=None, delta_bias=None, *, state=
     position, as a new tensor."""
     who = "selective_scan"
     args = _scan_args(who, 3, u, delta, A, B, C, D, z, delta_bias)
-    n, _, c = u.shape
+    n, length, c = u.shape
     state = _state(who, state, (n, D_STATE, c), u, torch.float32, False)
-    lens = _lens(who, lens, n, u)
+    lens = _lens(who, lens, n, length, u)
     _gpu(who, u)
     if _grad(*args):
         y, out = _SelectiveScan.apply(*args, state, lens, bool(return_state))

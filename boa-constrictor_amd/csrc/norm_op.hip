@@ -4,9 +4,10 @@
 //   mean = sum x / d, rstd = 1 / sqrt(sum (x - mean)^2 / d + eps), xh = (x - mean) rstd, y = xh w + b
 //   dx = rstd (g - mean(g) - xh mean(g xh)) with g = dy w;  dw = sum_rows dy xh, db = sum_rows dy
 //
-// Both passes are bound by memory.  A wavefront holds a row in registers, so a row is read once per pass, and takes ROWS of
-// them at a time to have enough loads in flight.  In the backward pass a wavefront adds its rows' dy xh and dy in registers,
-// a workgroup its wavefronts' through LDS, and k_sum_parts the workgroups': no atomics, so the same inputs give the same bits.
+// Both passes are bound by memory.  A wavefront (a workgroup for rows of more than 1024 values) holds a row in registers, so a
+// row is read once per pass, and takes several of them at a time to have enough loads in flight.  In the backward pass a
+// wavefront adds its rows' dy xh and dy in registers, a workgroup its wavefronts' through LDS, and k_sum_parts the workgroups':
+// no atomics, so the same inputs give the same bits.
 #include "ops_common.h"
 
 #include "../../include/boa_hip.h"
@@ -17,15 +18,18 @@ namespace {
 
 constexpr int WG = 256, WAVES = WG / 64;
 constexpr int MAX_D = BOA_LAYER_NORM_MAX_D;
+constexpr int WAVE_D = 1024;  // rows up to here are a wavefront's, wider ones a workgroup's
+static_assert(MAX_D <= 16 * WG, "16 values per thread");
 
 // Rows that a wavefront takes at a time, for PER elements per lane: 16 values in flight per lane.
 constexpr int rows_at_once(int per) { return per >= 16 ? 1 : 16 / per; }
 
-template <int DT, int VEC, int N>
+// A row over LANES threads (a wavefront, or the workgroup), N accesses of VEC elements each.
+template <int DT, int VEC, int N, int LANES_>
 struct Row {
-    static constexpr int VECTOR = VEC, COUNT = N, PER = N * VEC;
+    static constexpr int VECTOR = VEC, COUNT = N, PER = N * VEC, LANES = LANES_, TEAMS = WG / LANES;
     using T = typename Elem<DT>::T;
-    static __device__ __forceinline__ int col(int i, int lane) { return (i * 64 + lane) * VEC; }
+    static __device__ __forceinline__ int col(int i, int lane) { return (i * LANES + lane) * VEC; }
     // elements beyond d read as 0 (d is a multiple of VEC, so a vector is inside or outside as a whole); without branches, so
     // that the loads of several rows go out together
     static __device__ __forceinline__ void load(const T* row, int d, int lane, float (&v)[PER]) {
@@ -57,43 +61,60 @@ struct Row {
                 v[i * VEC + j] = (p != nullptr && c < d) ? p[c] : other;
             }
     }
+    // K sums over the row's threads
+    template <int K>
+    static __device__ __forceinline__ void sums(float (&v)[K]) {
+#pragma unroll
+        for (int k = 0; k < K; ++k) v[k] = wsum(v[k]);
+        if constexpr (LANES == WG) {
+            __shared__ float s[K][WAVES];
+            __syncthreads();  // what was here has been read
+            if ((threadIdx.x & 63) == 0)
+#pragma unroll
+                for (int k = 0; k < K; ++k) s[k][threadIdx.x >> 6] = v[k];
+            __syncthreads();
+#pragma unroll
+            for (int k = 0; k < K; ++k) {
+                v[k] = s[k][0];
+#pragma unroll
+                for (int w = 1; w < WAVES; ++w) v[k] += s[k][w];
+            }
+        }
+    }
 };
 
-template <int DT, int VEC, int N>
+template <class R, int DT>
 __global__ void __launch_bounds__(WG) k_norm_fwd(const void* xp, int64_t xs, const float* w, const float* b, int64_t rows,
                                                  int d, float eps, void* yp, int64_t ys, float2* stats) {
-    using R = Row<DT, VEC, N>;
-    constexpr int PER = R::PER, ROWS = rows_at_once(PER);
+    constexpr int PER = R::PER, ROWS = rows_at_once(PER), VEC = R::VECTOR;
     const auto* x = static_cast<const typename R::T*>(xp);
     auto* y = static_cast<typename R::T*>(yp);
-    const int lane = threadIdx.x & 63;
-    const int64_t wave = (int64_t)blockIdx.x * WAVES + (threadIdx.x >> 6), waves = (int64_t)gridDim.x * WAVES;
+    const int lane = threadIdx.x % R::LANES;
+    const int64_t team = (int64_t)blockIdx.x * R::TEAMS + threadIdx.x / R::LANES, teams = (int64_t)gridDim.x * R::TEAMS;
     float wv[PER], bv[PER];
     R::param(w, d, lane, 1.0f, wv);
     R::param(b, d, lane, 0.0f, bv);
     const float inv = 1.0f / (float)d;
-    for (int64_t r0 = wave * ROWS; r0 < rows; r0 += waves * ROWS) {
+    for (int64_t r0 = team * ROWS; r0 < rows; r0 += teams * ROWS) {
         float v[ROWS][PER];
 #pragma unroll
-        for (int r = 0; r < ROWS; ++r) {
-            const int64_t at = r0 + r < rows ? r0 + r : rows - 1;
-            R::load(x + at * xs, d, lane, v[r]);
-        }
+        for (int r = 0; r < ROWS; ++r) R::load(x + min(r0 + r, rows - 1) * xs, d, lane, v[r]);
 #pragma unroll
         for (int r = 0; r < ROWS; ++r) {
-            float s = 0.0f;
+            float s[1] = {0.0f}, q[1] = {0.0f};
 #pragma unroll
-            for (int i = 0; i < PER; ++i) s += v[r][i];
-            const float mean = wsum(s) * inv;
-            float q = 0.0f;
+            for (int i = 0; i < PER; ++i) s[0] += v[r][i];
+            R::sums(s);
+            const float mean = s[0] * inv;
 #pragma unroll
             for (int i = 0; i < PER; ++i) {
                 // beyond d the difference is not one of the row's
                 const float c = R::col(i / VEC, lane) < d ? v[r][i] - mean : 0.0f;
                 v[r][i] = c;
-                q = __builtin_fmaf(c, c, q);
+                q[0] = __builtin_fmaf(c, c, q[0]);
             }
-            const float rstd = 1.0f / sqrtf(wsum(q) * inv + eps);
+            R::sums(q);
+            const float rstd = 1.0f / sqrtf(q[0] * inv + eps);
 #pragma unroll
             for (int i = 0; i < PER; ++i) v[r][i] = __builtin_fmaf(v[r][i] * rstd, wv[i], bv[i]);
             if (r0 + r < rows) {
@@ -104,27 +125,25 @@ __global__ void __launch_bounds__(WG) k_norm_fwd(const void* xp, int64_t xs, con
     }
 }
 
-template <int DT, int VEC, int N>
+template <class R, int DT>
 __global__ void __launch_bounds__(WG) k_norm_bwd(const void* dyp, int64_t dys, const void* xp, int64_t xs, const float* w,
                                                  const float2* stats, int64_t rows, int d, void* dxp, int64_t dxs,
                                                  float* part) {
-    using R = Row<DT, VEC, N>;
-    constexpr int PER = R::PER, ROWS = rows_at_once(2 * PER);
-    __shared__ float sum[2][64 * PER];
+    constexpr int PER = R::PER, ROWS = rows_at_once(2 * PER), VEC = R::VECTOR;
     const auto* x = static_cast<const typename R::T*>(xp);
     const auto* dy = static_cast<const typename R::T*>(dyp);
     auto* dx = static_cast<typename R::T*>(dxp);
-    const int lane = threadIdx.x & 63, wv_id = threadIdx.x >> 6;
-    const int64_t wave = (int64_t)blockIdx.x * WAVES + wv_id, waves = (int64_t)gridDim.x * WAVES;
+    const int lane = threadIdx.x % R::LANES, mine = threadIdx.x / R::LANES;
+    const int64_t team = (int64_t)blockIdx.x * R::TEAMS + mine, teams = (int64_t)gridDim.x * R::TEAMS;
     float wv[PER], dw[PER] = {}, db[PER] = {};
     R::param(w, d, lane, 1.0f, wv);
     const float inv = 1.0f / (float)d;
-    for (int64_t r0 = wave * ROWS; r0 < rows; r0 += waves * ROWS) {
+    for (int64_t r0 = team * ROWS; r0 < rows; r0 += teams * ROWS) {
         float v[ROWS][PER], g[ROWS][PER];
         float2 st[ROWS];
 #pragma unroll
         for (int r = 0; r < ROWS; ++r) {
-            const int64_t at = r0 + r < rows ? r0 + r : rows - 1;
+            const int64_t at = min(r0 + r, rows - 1);
             R::load(x + at * xs, d, lane, v[r]);
             R::load(dy + at * dys, d, lane, g[r]);
             st[r] = stats[at];
@@ -132,41 +151,49 @@ __global__ void __launch_bounds__(WG) k_norm_bwd(const void* dyp, int64_t dys, c
 #pragma unroll
         for (int r = 0; r < ROWS; ++r) {
             if (r0 + r >= rows) break;
-            float m1 = 0.0f, m2 = 0.0f;
+            float m[2] = {0.0f, 0.0f};  // sums of g, and of g xh
 #pragma unroll
             for (int i = 0; i < PER; ++i) {
                 const float xh = (v[r][i] - st[r].x) * st[r].y;  // beyond d: dy is 0 there
                 dw[i] = __builtin_fmaf(g[r][i], xh, dw[i]);
                 db[i] += g[r][i];
                 const float gw = g[r][i] * wv[i];
-                m1 += gw;
-                m2 = __builtin_fmaf(gw, xh, m2);
+                m[0] += gw;
+                m[1] = __builtin_fmaf(gw, xh, m[1]);
                 v[r][i] = xh;
                 g[r][i] = gw;
             }
-            m1 = wsum(m1) * inv;
-            m2 = wsum(m2) * inv;
+            R::sums(m);
 #pragma unroll
-            for (int i = 0; i < PER; ++i) v[r][i] = (g[r][i] - m1 - v[r][i] * m2) * st[r].y;
+            for (int i = 0; i < PER; ++i) v[r][i] = (g[r][i] - m[0] * inv - v[r][i] * (m[1] * inv)) * st[r].y;
             R::store(dx + (r0 + r) * dxs, d, lane, v[r]);
         }
     }
     if (part == nullptr) return;
-    for (int k = 0; k < WAVES; ++k) {
-        if (wv_id == k) {
+    float* out = part + (int64_t)blockIdx.x * 2 * d;
+    if constexpr (R::TEAMS == 1) {
 #pragma unroll
-            for (int i = 0; i < PER; ++i) {
-                const int c = R::col(i / VEC, lane) + i % VEC;
-                sum[0][c] = (k ? sum[0][c] : 0.0f) + dw[i];
-                sum[1][c] = (k ? sum[1][c] : 0.0f) + db[i];
-            }
+        for (int i = 0; i < PER; ++i) {
+            const int c = R::col(i / VEC, lane) + i % VEC;
+            if (c < d) out[c] = dw[i], out[d + c] = db[i];
         }
-        __syncthreads();
-    }
-    float* mine = part + (int64_t)blockIdx.x * 2 * d;
-    for (int c = threadIdx.x; c < d; c += WG) {
-        mine[c] = sum[0][c];
-        mine[d + c] = sum[1][c];
+    } else {
+        __shared__ float sum[2][R::LANES * PER];
+        for (int k = 0; k < R::TEAMS; ++k) {
+            if (mine == k) {
+#pragma unroll
+                for (int i = 0; i < PER; ++i) {
+                    const int c = R::col(i / VEC, lane) + i % VEC;
+                    sum[0][c] = (k ? sum[0][c] : 0.0f) + dw[i];
+                    sum[1][c] = (k ? sum[1][c] : 0.0f) + db[i];
+                }
+            }
+            __syncthreads();
+        }
+        for (int c = threadIdx.x; c < d; c += WG) {
+            out[c] = sum[0][c];
+            out[d + c] = sum[1][c];
+        }
     }
 }
 
@@ -175,33 +202,31 @@ __global__ void __launch_bounds__(SUM_COLS * SUM_GROUPS) k_sum_parts(const float
     sum_parts<SUM_GROUPS>(part, parts, width, out, blockIdx.x);
 }
 
-int64_t fwd_groups(int64_t rows, int per) { return ceil_div(rows, WAVES * rows_at_once(per)); }
-// Workgroups of the backward pass, each of which leaves a partial row of 2 d sums: four rows or more per wavefront.
-int64_t bwd_groups(int64_t rows) {
-    const int64_t n = ceil_div(rows, 4 * WAVES);
+// Workgroups of the backward pass, each of which leaves a partial row of 2 d sums: four rows or more per wavefront (a row or
+// more per workgroup where a row takes one).
+int64_t bwd_groups(int64_t rows, int d) {
+    const int64_t n = d <= WAVE_D ? ceil_div(rows, 4 * WAVES) : rows;
     return n < 1024 ? n : 1024;
 }
 
 // Calls f with the row shape for width d: accesses of 16 bytes (8 for 16-bit rows of up to 256 values, which then take all 64
-// lanes) where the rows are aligned for them, else single elements.
+// lanes) where the rows are aligned for them, else single elements; up to 16 values per lane.
 template <int DT, class F>
 int with_row(int d, bool aligned, F f) {
     constexpr int W = wide<DT>();
-    if (aligned && d % 4 == 0 && d <= 256) return f(Row<DT, 4, 1>());
+    if (aligned && d % 4 == 0 && d <= 256) return f(Row<DT, 4, 1, 64>());
     if (aligned && d % W == 0) {
-        const int n = (int)ceil_div(d, 64 * W);
-        if (n <= 1) return f(Row<DT, W, 1>());
-        if (n <= 2) return f(Row<DT, W, 2>());
-        if (n <= 4) return f(Row<DT, W, 4>());
-        if (W * n <= 32) return f(Row<DT, W, 32 / W>());
-        return f(Row<DT, W, 64 / W>());
+        if (d <= 64 * W) return f(Row<DT, W, 1, 64>());
+        if (d <= 128 * W && d <= WAVE_D) return f(Row<DT, W, 2, 64>());
+        if (d <= WAVE_D) return f(Row<DT, W, 16 / W, 64>());
+        if (d <= WG * W) return f(Row<DT, W, 1, WG>());
+        return f(Row<DT, W, 16 / W, WG>());
     }
-    const int n = (int)ceil_div(d, 64);
-    if (n <= 4) return f(Row<DT, 1, 4>());
-    if (n <= 8) return f(Row<DT, 1, 8>());
-    if (n <= 16) return f(Row<DT, 1, 16>());
-    if (n <= 32) return f(Row<DT, 1, 32>());
-    return f(Row<DT, 1, 64>());
+    if (d <= 256) return f(Row<DT, 1, 4, 64>());
+    if (d <= 512) return f(Row<DT, 1, 8, 64>());
+    if (d <= WAVE_D) return f(Row<DT, 1, 16, 64>());
+    if (d <= 8 * WG) return f(Row<DT, 1, 8, WG>());
+    return f(Row<DT, 1, 16, WG>());
 }
 int check_norm(const char* who, int dtype, int64_t rows, int32_t d) {
     if (dtype < BOA_DT_F32 || dtype > BOA_DT_F16) return boa_fail(BOA_ERR_ARG, "%s: unknown type %d", who, dtype);
@@ -232,8 +257,8 @@ extern "C" int boa_layer_norm_fwd(int dtype, const void* d_x, int64_t x_stride, 
         constexpr int DT = decltype(dt)::value;
         return with_row<DT>(d, al, [&](auto row) {
             using R = decltype(row);
-            const int64_t groups = fwd_groups(rows, R::PER);
-            hipLaunchKernelGGL((k_norm_fwd<DT, R::VECTOR, R::COUNT>), dim3((uint32_t)(groups < 4096 ? groups : 4096)), dim3(WG), 0,
+            const int64_t groups = ceil_div(rows, R::TEAMS * rows_at_once(R::PER));
+            hipLaunchKernelGGL((k_norm_fwd<R, DT>), dim3((uint32_t)(groups < 4096 ? groups : 4096)), dim3(WG), 0,
                                (hipStream_t)stream, d_x, x_stride, d_w, d_b, rows, d, eps, d_y, y_stride,
                                reinterpret_cast<float2*>(d_stats));
             BOA_HIP_TRY(hipGetLastError());
@@ -243,7 +268,7 @@ extern "C" int boa_layer_norm_fwd(int dtype, const void* d_x, int64_t x_stride, 
 }
 
 extern "C" int64_t boa_layer_norm_bwd_work_bytes(int64_t rows, int32_t d) {
-    return rows < 1 || d < 1 ? 0 : bwd_groups(rows) * 2 * d * (int64_t)sizeof(float);
+    return rows < 1 || d < 1 ? 0 : bwd_groups(rows, d) * 2 * d * (int64_t)sizeof(float);
 }
 
 extern "C" int boa_layer_norm_bwd(int dtype, const void* d_dy, int64_t dy_stride, const void* d_x, int64_t x_stride,
@@ -258,14 +283,14 @@ extern "C" int boa_layer_norm_bwd(int dtype, const void* d_dy, int64_t dy_stride
         return boa_fail(BOA_ERR_ARG, "boa_layer_norm_bwd: null pointer");
     hipStream_t s = (hipStream_t)stream;
     float* part = d_dwb ? static_cast<float*>(d_work) : nullptr;
-    const int64_t groups = rows > 0 ? bwd_groups(rows) : 0;
+    const int64_t groups = rows > 0 ? bwd_groups(rows, d) : 0;
     if (rows > 0) {
         const bool al = aligned16(dtype, d_x, x_stride) && aligned16(dtype, d_dy, dy_stride) && aligned16(dtype, d_dx, dx_stride);
         const int launched = with_dtype(dtype, [&](auto dt) {
             constexpr int DT = decltype(dt)::value;
             return with_row<DT>(d, al, [&](auto row) {
                 using R = decltype(row);
-                hipLaunchKernelGGL((k_norm_bwd<DT, R::VECTOR, R::COUNT>), dim3((uint32_t)groups), dim3(WG), 0, s, d_dy, dy_stride,
+                hipLaunchKernelGGL((k_norm_bwd<R, DT>), dim3((uint32_t)groups), dim3(WG), 0, s, d_dy, dy_stride,
                                    d_x, x_stride, d_w, reinterpret_cast<const float2*>(d_stats), rows, d, d_dx, dx_stride, part);
                 BOA_HIP_TRY(hipGetLastError());
                 return (int)BOA_OK;

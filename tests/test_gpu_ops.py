@@ -603,6 +603,24 @@ def test_offsets_beyond_32_bits(ops):
     assert torch.equal(ops.cross_entropy(flat, t), ops.cross_entropy(flat.contiguous(), t))
 
 
+def test_differentiable_once(ops):
+    x = _randn(_gen(22), 4, 64).requires_grad_()
+    g, = torch.autograd.grad(ops.layer_norm(x).square().sum(), x, retain_graph=True)
+    assert g.isfinite().all() and not g.requires_grad
+    with pytest.raises(RuntimeError, match="differentiable once"):
+        torch.autograd.grad(ops.layer_norm(x).square().sum(), x, create_graph=True)
+
+
+def test_lengths_of_64_bits(ops):
+    """Lengths beyond 32 bits are clamped, not cut."""
+    g = _gen(23)
+    x, w = _randn(g, 3, 20, 64), _randn(g, 64, 4)
+    lens = torch.tensor([1 << 32, (1 << 32) + 7, -(1 << 33)], device="cuda")
+    assert torch.equal(ops.causal_conv(x, w, lens=lens), ops.causal_conv(x, w, lens=lens.clamp(0, 20)))
+    s = _scan_inputs(g, 3, 20, 64, torch.float32)
+    assert torch.equal(ops.selective_scan(**s, lens=lens), ops.selective_scan(**s, lens=lens.clamp(0, 20).int()))
+
+
 def test_saved_inputs_are_watched(ops):
     """An input changed in place between the passes is an error, as everywhere in torch, never a wrong gradient."""
     g = _gen(21)
