@@ -41,6 +41,15 @@ _INT_BYTES = {torch.uint8: 1, torch.int32: 4, torch.int64: 8}
 
 
 # ---- argument checks -------------------------------------------------------------------------------
+# A single-token step takes 10 us on the host, a third of it these checks: what is right is seen at once (_is), what is wrong is
+# looked at again for the message.
+_Tensor, _F32 = torch.Tensor, torch.float32
+
+
+def _is(t, dtype, shape, device):
+    return isinstance(t, _Tensor) and t.dtype is dtype and t.shape == shape and t.get_device() == device
+
+
 def _act(who, name, t, shape=None, like=None):
     """An activation: its type code; a tensor of `like`'s type and device, and of `shape`."""
     if not isinstance(t, torch.Tensor):
@@ -60,19 +69,19 @@ def _param(who, name, t, shape, like):
     """A float32 parameter or state of this shape on the activations' device, contiguous; None stays None."""
     if t is None:
         return None
+    if _is(t, _F32, shape, like.get_device()):
+        return t if t.is_contiguous() else t.contiguous()
     if not isinstance(t, torch.Tensor) or t.dtype != torch.float32:
         raise TypeError(f"{who}: {name} must be a float32 tensor")
-    if t.device != like.device or t.shape != shape:
-        raise ValueError(f"{who}: {name} must be {list(shape)} on {like.device} (got {list(t.shape)} on {t.device})")
-    return t if t.is_contiguous() else t.contiguous()
+    raise ValueError(f"{who}: {name} must be {list(shape)} on {like.device} (got {list(t.shape)} on {t.device})")
 
 
 def _state(who, t, shape, like, dtype, in_place):
     if t is None:
         return None
-    if not isinstance(t, torch.Tensor) or t.dtype != dtype:
-        raise TypeError(f"{who}: state must be a {dtype} tensor")
-    if t.device != like.device or t.shape != shape:
+    if not _is(t, dtype, shape, like.get_device()):
+        if not isinstance(t, torch.Tensor) or t.dtype != dtype:
+            raise TypeError(f"{who}: state must be a {dtype} tensor")
         raise ValueError(f"{who}: state must be {list(shape)} on {like.device} (got {list(t.shape)} on {t.device})")
     if t.requires_grad:
         raise ValueError(f"{who}: states carry no gradient; detach() it")
@@ -111,7 +120,11 @@ def _gpu(who, t):
 
 
 def _grad(*ts):
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts)
+    if torch.is_grad_enabled():
+        for t in ts:
+            if t is not None and t.requires_grad:
+                return True
+    return False
 
 
 _raw_stream, _device = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice  # cheaper than a torch.cuda.Stream
@@ -119,9 +132,11 @@ _raw_stream, _device = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDev
 
 def _call(t, f, *args):
     """An entry point (its last argument is the stream) on the current stream of a tensor's device, made current for it."""
-    i = t.device.index
+    i = t.get_device()
     if i == _device():
-        _nat.check(f(*args, _raw_stream(i)))
+        rc = f(*args, _raw_stream(i))
+        if rc:
+            _nat.check(rc)
     else:
         with torch.cuda.device(i):
             _nat.check(f(*args, _raw_stream(i)))
@@ -304,10 +319,10 @@ def _conv_args(who, x, ndim, weight, bias):
                          f"(got {list(x.shape)})")
     c = x.shape[-1]
     flat = isinstance(weight, torch.Tensor) and weight.ndim == 2
-    w = _param(who, "weight", weight, torch.Size((c, D_CONV) if flat else (c, 1, D_CONV)), x)
+    w = _param(who, "weight", weight, (c, D_CONV) if flat else (c, 1, D_CONV), x)
     if w is None:
         raise TypeError(f"{who}: weight must be a float32 tensor")
-    return w, _param(who, "bias", bias, torch.Size((c,)), x)
+    return w, _param(who, "bias", bias, (c,), x)
 
 
 def causal_conv(x, weight, bias=None, *, silu: bool = True, state=None, lens=None, return_state: bool = False):
@@ -353,6 +368,7 @@ def causal_conv_step(x, state, weight, bias=None, *, silu: bool = True):
 # lens, state_in, state_out, marks; y, dy, du, ddelta, dz, db, dc; dpar
 _SCAN = struct.Struct("@iiqq15q7q21qq")
 _NO_ROWS = (0, 0, 0)
+_NO_BACKWARD = (0,) * 19
 
 
 def _r3(t):
@@ -375,7 +391,7 @@ def _scan_rows(t):
 def _scalar_rows(t):
     """The same for B and C, whose rows begin at multiples of 4 bytes."""
     t = _scan_rows(t)
-    if t.element_size() == 2 and (t.data_ptr() % 4 or any(s % 2 for s in t.stride()[:-1])):
+    if t.dtype is not _F32 and (t.data_ptr() % 4 or any(s % 2 for s in t.stride()[:-1])):
         t = t.clone(memory_format=torch.contiguous_format)
     return t
 
@@ -429,22 +445,23 @@ def _scan_args(who, ndim, u, delta, A, B, C, D, z, bias):
     if u.ndim != ndim or not 1 <= u.shape[-1] <= _nat.BOA_OPS_MAX_CHANNELS:
         raise ValueError(f"{who}: u must be {'[batch, length, channels]' if ndim == 3 else '[batch, channels]'} "
                          f"(got {list(u.shape)})")
-    c = u.shape[-1]
-    _act(who, "delta", delta, u.shape, u)
-    if z is not None:
-        _act(who, "z", z, u.shape, u)
-    states = u.shape[:-1] + (D_STATE,)
-    _act(who, "B", B, states, u)
-    _act(who, "C", C, states, u)
-    A = _param(who, "A", A, torch.Size((c, D_STATE)), u)
+    dtype, shape, dev = u.dtype, u.shape, u.get_device()
+    c = shape[-1]
+    states = shape[:-1] + (D_STATE,)
+    if not _is(delta, dtype, shape, dev):
+        _act(who, "delta", delta, shape, u)
+    if z is not None and not _is(z, dtype, shape, dev):
+        _act(who, "z", z, shape, u)
+    if not _is(B, dtype, states, dev):
+        _act(who, "B", B, states, u)
+    if not _is(C, dtype, states, dev):
+        _act(who, "C", C, states, u)
+    A = _param(who, "A", A, (c, D_STATE), u)
     if A is None:
         raise TypeError(f"{who}: A must be a float32 tensor")
-    D, bias = _param(who, "D", D, torch.Size((c,)), u), _param(who, "delta_bias", bias, torch.Size((c,)), u)
-    if ndim == 3:
-        u, delta, z = _scan_rows(u), _scan_rows(delta), None if z is None else _scan_rows(z)
-    else:
-        u, delta, z = _rows(u), _rows(delta), None if z is None else _rows(z)
-    return u, delta, A, _scalar_rows(B), _scalar_rows(C), D, z, bias
+    D, bias = _param(who, "D", D, (c,), u), _param(who, "delta_bias", bias, (c,), u)
+    rows = _scan_rows if ndim == 3 else _rows
+    return rows(u), rows(delta), A, _scalar_rows(B), _scalar_rows(C), D, z if z is None else rows(z), bias
 
 
 def selective_scan(u, delta, A, B, C, D=None, z=None, delta_bias=None, *, state=None, lens=None, return_state: bool = False):
@@ -484,10 +501,9 @@ def selective_scan_step(u, delta, A, B, C, D=None, z=None, delta_bias=None, *, s
     if A.data_ptr() % 16:
         A = A.clone()
 
-    def r2(t):
-        return _NO_ROWS if t is None else (t.data_ptr(), t.stride(0), 0)
-
-    packed = _SCAN.pack(_DTYPES[u.dtype], c, n, 1, *r2(u), *r2(delta), *r2(z), *r2(B), *r2(C), A.data_ptr(), _ptr(D), _ptr(bias),
-                        0, 0, state.data_ptr(), 0, *r2(y), *(_NO_ROWS * 6), 0)
+    zp, zs = (0, 0) if z is None else (z.data_ptr(), z.stride(0))
+    packed = _SCAN.pack(_DTYPES[u.dtype], c, n, 1, u.data_ptr(), u.stride(0), 0, delta.data_ptr(), delta.stride(0), 0, zp, zs, 0,
+                        B.data_ptr(), B.stride(0), 0, C.data_ptr(), C.stride(0), 0, A.data_ptr(), _ptr(D), _ptr(bias), 0, 0,
+                        state.data_ptr(), 0, y.data_ptr(), c, 0, *_NO_BACKWARD)
     _call(u, _nat.lib().boa_selective_scan_step, packed)
     return y
