@@ -42,6 +42,7 @@ struct ScanArgs {
     float *local, *dts;           // [batch][chunks][16][channels], [batch][chunks][channels]
     const int32_t* lens;
     int channels, cblocks, chunks;
+    bool joined;                  // local holds the states before the chunks (k_scan_join), not those that they leave
     int64_t batch, length, subs;  // subs: blocks of SUB positions of a sequence
     int64_t chunk;                // positions of a chunk, a multiple of SUB
 };
@@ -207,6 +208,41 @@ __device__ __forceinline__ void over_chunks(const ScanArgs& a, const Place& p, i
 // behind the last one is fetched as the last one, and without a gate z is u.
 enum { LOCAL, OUT, OUT_MARKS };
 
+// Where there are many chunks, the state before each of them instead: from the ends of the chunks before it (of those behind
+// it, from the sequence's end, in the backward pass), in the places of local.  A thread takes one state through all chunks.
+constexpr int JOIN_WG = 64;  // few threads, all waiting for loads: on as many CUs as there are
+template <bool BACK>
+__global__ void __launch_bounds__(JOIN_WG) k_scan_join(const ScanArgs a) {
+    constexpr int AT_ONCE = 32;
+    const int64_t i = (int64_t)blockIdx.x * JOIN_WG + threadIdx.x;
+    if (i >= a.batch * NS * a.channels) return;
+    const int64_t b = i / (NS * a.channels);
+    const int n = (int)(i / a.channels % NS), c = (int)(i % a.channels);
+    const int64_t end = end_of(a, b);
+    const int chunks = (int)ceil_div(end, a.chunk);  // with positions inside
+    const float a2 = a.A[(int64_t)c * NS + n] * LOG2E;
+    float h = !BACK && a.state_in != nullptr ? a.state_in[i] : 0.0f;
+    for (int j0 = 0; j0 < chunks; j0 += AT_ONCE) {
+        float dts[AT_ONCE], l[AT_ONCE];
+        // the first chunk has no end of its own in the backward pass, the last one none in the forward pass
+#pragma unroll
+        for (int j = 0; j < AT_ONCE; ++j) {
+            const int at = min(j0 + j, chunks - 2), k = BACK ? chunks - 1 - at : at;
+            const int64_t r = b * a.chunks + k;
+            dts[j] = chunks > 1 ? a.dts[r * a.channels + c] : 0.0f;
+            l[j] = chunks > 1 ? a.local[(r * NS + n) * a.channels + c] : 0.0f;
+        }
+#pragma unroll
+        for (int j = 0; j < AT_ONCE; ++j) {
+            const int at = j0 + j;
+            if (at < chunks) {
+                a.local[((b * a.chunks + (BACK ? chunks - 1 - at : at)) * NS + n) * a.channels + c] = h;
+                h = __builtin_fmaf(__builtin_amdgcn_exp2f(dts[j] * a2), h, l[j]);
+            }
+        }
+    }
+}
+
 // LOCAL: the state that a chunk alone leaves (from zeros) and its sum of dt, for every chunk but the last; OUT: the chunk's
 // outputs, from the state that the chunks before it leave; OUT_MARKS: and the state before every block.
 template <int DT, int MODE>
@@ -224,7 +260,10 @@ __global__ void __launch_bounds__(WG) k_scan_fwd(const ScanArgs a) {
     p.decay(a, a2);
     const float bias = a.bias != nullptr ? a.bias[p.cc] : 0.0f, D = MODE != LOCAL && a.D != nullptr ? a.D[p.cc] : 0.0f;
 #pragma unroll
-    for (int n = 0; n < NQ; ++n) h[n] = MODE != LOCAL && a.state_in != nullptr ? a.state_in[state_at(a, p, p.b, n)] : 0.0f;
+    for (int n = 0; n < NQ; ++n)
+        h[n] = MODE == LOCAL ? 0.0f
+               : a.joined && n_subs > 0 ? a.local[state_at(a, p, p.b * a.chunks + p.k, n)]
+               : a.state_in != nullptr ? a.state_in[state_at(a, p, p.b, n)] : 0.0f;
 
     // A block's life: fetched (loads issued), prepared (dt and dt u to LDS), computed, finished (sums over the wavefronts'
     // states, gate, stores).  One barrier per block: block i is computed while i - 1 is finished and i + 1 prepared, with
@@ -271,7 +310,7 @@ __global__ void __launch_bounds__(WG) k_scan_fwd(const ScanArgs a) {
     float u[MINE], z[MINE], u_before[MINE], z_before[MINE], u_next[MINE], z_next[MINE], dts = 0.0f;
     if (n_subs > 0) {
         fetch(0);
-        if (MODE != LOCAL) over_chunks(a, p, 0, 1, p.k, a2, h);
+        if (MODE != LOCAL && !a.joined) over_chunks(a, p, 0, 1, p.k, a2, h);
         prepare(0, u, z);
         const bool more = n_subs > 1;
         xu.ahead(more), xd.ahead(more), xz.ahead(more);
@@ -634,8 +673,13 @@ __global__ void __launch_bounds__(WG, 4) k_scan_bwd(const ScanArgs a) {
     };
     if (n_subs > 0) {
         fetch(count - (n_subs - 1) * SUB);
-        const int after = (int)ceil_div(end, a.chunk) - 1;
-        over_chunks(a, p, after, -1, after - p.k, a2, dh);
+        if (a.joined) {
+#pragma unroll
+            for (int n = 0; n < NQ; ++n) dh[n] = a.local[state_at(a, p, p.b * a.chunks + p.k, n)];
+        } else {
+            const int after = (int)ceil_div(end, a.chunk) - 1;
+            over_chunks(a, p, after, -1, after - p.k, a2, dh);
+        }
         block(n_subs - 1, std::false_type());
         for (int i = n_subs - 2; i >= 0; --i) block(i, std::true_type());
     }
@@ -745,6 +789,10 @@ struct Plan {
 // 194, 161, 142).
 int64_t wanted_workgroups(const boa_scan* s, bool backward) { return s->lens ? 4096 : backward ? 1024 : 1536; }
 constexpr int64_t MIN_CHUNK = 64, MAX_CHUNKS = 128;
+// From more chunks than this on they are joined by a kernel of its own: to go over the chunks before its own costs a workgroup
+// of the last chunk 0.3 us for each, and reads them for every workgroup again (2 x 16384 positions of 512 channels: forward
+// kernel 129 us, with k_scan_join 97 + 14; backward, of 64 chunks, 247 and 233 + 11; forward, 16 chunks of 8 x 1000, 34 and 30 + 5).
+constexpr int JOIN_FROM = 32;
 Plan plan(const boa_scan* s, bool backward) {
     const int64_t blocks = s->batch * ceil_div(s->channels, 64);
     int64_t n = ceil_div(wanted_workgroups(s, backward), blocks > 0 ? blocks : 1);
@@ -806,7 +854,7 @@ int check_scan(const char* who, const boa_scan* s, ScanArgs& a, bool backward) {
     a.marks = s->marks, a.channels = s->channels, a.cblocks = (int)ceil_div(s->channels, 64);
     a.batch = s->batch, a.length = s->length, a.subs = ceil_div(s->length, SUB);
     const Plan pl = plan(s, backward);
-    a.chunks = pl.chunks, a.chunk = pl.chunk;
+    a.chunks = pl.chunks, a.chunk = pl.chunk, a.joined = pl.chunks > JOIN_FROM;
     if (a.batch > MAX_BLOCKS / ((int64_t)a.cblocks * a.chunks))
         return boa_fail(BOA_ERR_ARG, "%s: batch of %lld sequences too large", who, (long long)a.batch);
     return BOA_OK;
@@ -836,6 +884,11 @@ extern "C" int boa_selective_scan_fwd(const boa_scan* s, void* d_work, int64_t w
         if (a.chunks > 1) {
             hipLaunchKernelGGL((k_scan_fwd<DT, LOCAL>), dim3(blocks * (a.chunks - 1)), dim3(WG), 0, (hipStream_t)stream, a);
             BOA_HIP_TRY(hipGetLastError());
+            if (a.joined) {
+                hipLaunchKernelGGL((k_scan_join<false>), dim3((uint32_t)ceil_div(a.batch * NS * a.channels, JOIN_WG)), dim3(JOIN_WG), 0,
+                                   (hipStream_t)stream, a);
+                BOA_HIP_TRY(hipGetLastError());
+            }
         }
         if (a.marks != nullptr)
             hipLaunchKernelGGL((k_scan_fwd<DT, OUT_MARKS>), dim3(blocks * a.chunks), dim3(WG), 0, (hipStream_t)stream, a);
@@ -871,6 +924,11 @@ extern "C" int boa_selective_scan_bwd(const boa_scan* s, void* d_work, int64_t w
             if (a.chunks > 1) {
                 hipLaunchKernelGGL((k_scan_bwd_local<DT>), dim3(blocks * (a.chunks - 1)), dim3(WG), 0, st, a);
                 BOA_HIP_TRY(hipGetLastError());
+                if (a.joined) {
+                    hipLaunchKernelGGL((k_scan_join<true>), dim3((uint32_t)ceil_div(a.batch * NS * a.channels, JOIN_WG)), dim3(JOIN_WG), 0,
+                                       st, a);
+                    BOA_HIP_TRY(hipGetLastError());
+                }
             }
             if (a.channels % 64 == 0)
                 hipLaunchKernelGGL((k_scan_bwd<DT, true>), dim3(blocks * a.chunks), dim3(WG), 0, st, a);

@@ -351,6 +351,25 @@ def test_scan_of_padded_batches_from_a_state(ops, n, length, c, ends, gate, para
             assert torch.equal(end[i], state[i])
 
 
+@pytest.mark.parametrize("n,length,c,ends", [(1, 2300, 40, None), (2, 2500, 8, (2500, 130)), (3, 2200, 5, (0, 64, 2199))])
+def test_scan_of_many_chunks(ops, n, length, c, ends):
+    """Lengths that are split into more chunks than a workgroup goes over by itself (33 and more of 64 positions)."""
+    g = _gen(length)
+    s = {k: v.detach().requires_grad_() for k, v in _scan_inputs(g, n, length, c, torch.float32).items()}
+    state, dy = _randn(g, n, 16, c), _randn(g, n, length, c)
+    lens = None if ends is None else torch.tensor(ends, dtype=torch.int32, device="cuda")
+    y, end = ops.selective_scan(**s, state=state, lens=lens, return_state=True)
+    grads = torch.autograd.grad(y, tuple(s.values()), dy)
+    ref, k = _ref(s, state=state, lens=lens, dy=dy), _roundings(s)
+    # in these units an error at a chunk's border is one of size 1; a state is forgotten within some hundred positions, so no
+    # more than 500 positions' roundings add up
+    k = k * 500 / length
+    _check("y", y, ref["y"], k)
+    _check("state", end, ref["state"], k)
+    for name, got in zip(s, grads):
+        _check(NAMES[name], got, ref[NAMES[name]], 2 * k)
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_scan_padding_is_not_read(ops, dtype):
     g = _gen(8)
