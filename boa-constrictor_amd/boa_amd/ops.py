@@ -29,6 +29,7 @@ import functools
 import struct
 
 import torch
+from torch.autograd.graph import increment_version
 
 from boa_amd import _native as _nat
 
@@ -360,6 +361,7 @@ def causal_conv_step(x, state, weight, bias=None, *, silu: bool = True):
     y = x.new_empty((n, c))
     _call(x, _nat.lib().boa_causal_conv_step, _DTYPES[x.dtype], x.data_ptr(), x.stride(0), state.data_ptr(), w.data_ptr(), _ptr(b),
           bool(silu), n, c, y.data_ptr(), c)
+    increment_version(state)  # autograd sees the change, as it does one by an operator of torch
     return y
 
 
@@ -385,7 +387,9 @@ def _pack(u, delta, A, B, C, D, z, bias, lens, state_in, state_out, marks, y, ba
 def _scan_rows(t):
     """Rows as the kernels read them: contiguous, not too far apart."""
     t = _rows(t)
-    return t if t.stride(-2) <= _nat.BOA_SCAN_MAX_ROW_STRIDE else t.contiguous()
+    if t.stride(-2) <= _nat.BOA_SCAN_MAX_ROW_STRIDE:
+        return t
+    return t.clone(memory_format=torch.contiguous_format)  # contiguous() keeps the stride of a dimension of one
 
 
 def _scalar_rows(t):
@@ -506,4 +510,5 @@ def selective_scan_step(u, delta, A, B, C, D=None, z=None, delta_bias=None, *, s
                         B.data_ptr(), B.stride(0), 0, C.data_ptr(), C.stride(0), 0, A.data_ptr(), _ptr(D), _ptr(bias), 0, 0,
                         state.data_ptr(), 0, y.data_ptr(), c, 0, *_NO_BACKWARD)
     _call(u, _nat.lib().boa_selective_scan_step, packed)
+    increment_version(state)
     return y

@@ -259,6 +259,8 @@ extern "C" int boa_causal_conv_fwd(int dtype, const void* d_x, int64_t x_batch, 
     if (rc != BOA_OK) return rc;
     if (batch == 0 || (length == 0 && !d_state_out)) return BOA_OK;
     if (!d_w || (length > 0 && (!d_x || !d_y))) return boa_fail(BOA_ERR_ARG, "boa_causal_conv_fwd: null pointer");
+    if (d_state_out && d_state_out == d_state_in)
+        return boa_fail(BOA_ERR_ARG, "boa_causal_conv_fwd: d_state_out must be another buffer than d_state_in");
     ConvArgs a = {};
     a.x = d_x, a.xb = x_batch, a.xr = x_row, a.w = d_w, a.b = d_b, a.state_in = d_state_in, a.state_out = d_state_out;
     a.y = d_y, a.yb = y_batch, a.yr = y_row, a.lens = d_lens, a.C = channels, a.silu = silu;

@@ -873,6 +873,8 @@ extern "C" int boa_selective_scan_fwd(const boa_scan* s, void* d_work, int64_t w
     if (rc != BOA_OK) return rc;
     if (a.batch == 0 || (a.length == 0 && !a.state_out)) return BOA_OK;
     if (a.length > 0 && !a.y.p) return boa_fail(BOA_ERR_ARG, "boa_selective_scan_fwd: null pointer");
+    if (a.state_out && a.state_out == a.state_in)  // read by chunks that run beside the one that writes it
+        return boa_fail(BOA_ERR_ARG, "boa_selective_scan_fwd: state_out must be another buffer than state_in");
     const Work w = work_of(s, false);
     if (w.bytes() > 0 && (!d_work || work_bytes < w.bytes()))
         return boa_fail(BOA_ERR_ARG, "boa_selective_scan_fwd: workspace of %lld bytes, needs %lld", (long long)work_bytes,

@@ -331,6 +331,7 @@ class BoaBytePredictor(nn.Module):
         are advanced in place (truncated back-propagation, or streaming without an engine)."""
         if x.ndim != 2:
             raise ValueError(f"x must be [batch, length] (got {list(x.shape)})")
+        self._check_caches(caches)
         if lens is not None:
             inside = torch.arange(x.shape[1], device=lens.device) < lens[:, None]
             x = torch.where(inside, x.to(inside.device), torch.zeros((), dtype=x.dtype, device=inside.device))
@@ -358,10 +359,15 @@ class BoaBytePredictor(nn.Module):
     def train_step(self, byte_t, caches):
         """``step`` on the parameters as they are now: bytes [B] -> logits [B, V]; advances the caches in place.  For sampling
         from a model in training; ``init_stream`` and ``step`` run a loaded model faster."""
+        self._check_caches(caches)
         h = self._embed(byte_t.reshape(-1))
         for block, cache in zip(self.blocks, caches):
             h = block.step(h, cache)
         return self.head(h)
+
+    def _check_caches(self, caches):
+        if caches is not None and len(caches) != len(self.blocks):
+            raise ValueError(f"need a cache for each of the {len(self.blocks)} blocks (got {len(caches)})")
 
     def init_caches(self, batch_size: int, dtype=torch.float32):
         """Zero states for ``train_forward`` and ``train_step``, one per block."""

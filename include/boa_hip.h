@@ -287,7 +287,7 @@ typedef struct boa_scan {
     const float* delta_bias;                /* * [channels]                                              */
     const int32_t* lens;                    /* * [batch]                                                 */
     const float* state_in;                  /* * [batch][16][channels] before the first position (zeros) */
-    float* state_out;                       /* * the same behind each sequence's last position           */
+    float* state_out;                       /* * the same behind each sequence's last position, another buffer */
     float* marks;                           /* [batch][ceil(length / BOA_SCAN_MARK)][16][channels]: states that the
                                                forward pass leaves for the backward pass; * forward      */
     boa_rows y;

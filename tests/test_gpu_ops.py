@@ -653,3 +653,20 @@ def test_saved_inputs_are_watched(ops):
     y /= 2
     y.backward()  # the loss itself may be
     assert x.grad.isfinite().all() and math.isfinite(float(y.detach()))
+
+
+def test_saved_states_are_watched(ops):
+    """So is a state that a single-token step has advanced since a backward pass was to read it."""
+    g = _gen(22)
+    x, w, state = _randn(g, 2, 9, 64).requires_grad_(), _randn(g, 64, 4), _randn(g, 2, 3, 64)
+    y = ops.causal_conv(x, w, state=state)
+    with torch.no_grad():
+        ops.causal_conv_step(x[:, 0], state, w)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+    with torch.inference_mode():  # states without a counter
+        a, b = torch.zeros(2, 3, 64, device="cuda"), torch.zeros(2, 16, 64, device="cuda")
+        ops.causal_conv_step(x[:, 0], a, w)
+        B = x[:, 0, :16]
+        ops.selective_scan_step(x[:, 0], x[:, 1], -torch.ones(64, 16, device="cuda"), B, B, state=b)
+        assert a.abs().sum() > 0 and b.abs().sum() > 0

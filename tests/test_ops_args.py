@@ -193,3 +193,31 @@ def test_workspace_sizes():
     assert L.boa_layer_norm_bwd_work_bytes(0, 8) == 0 and L.boa_layer_norm_bwd_work_bytes(1, 8) == 64
     assert L.boa_causal_conv_bwd_work_bytes(0, 5, 8) == 0 and L.boa_causal_conv_bwd_work_bytes(2, 0, 8) == 0
     assert L.boa_selective_scan_work_bytes(None, 1) == 0
+
+
+def test_states_are_not_handed_on_in_place():
+    """The forward passes of whole sequences read the state while its successor is written."""
+    L, bad, P = _native.load_cdll(), _native.BOA_ERR_ARG, 4096
+    packed = bytearray(_pack())
+    for at in (24 + 5 * 24 + 4 * 8, 24 + 5 * 24 + 5 * 8):  # state_in, state_out
+        packed[at:at + 8] = (P).to_bytes(8, "little")
+    assert L.boa_selective_scan_fwd(bytes(packed), P, 1 << 30, None) == bad and b"another buffer" in L.boa_last_error()
+    assert L.boa_causal_conv_fwd(0, P, 64, 8, P, P, 1, 2, 8, 8, None, P, P, P, 64, 8, None) == bad
+
+
+def test_a_cache_for_every_block():
+    from model import BoaConstrictor
+
+    m = BoaConstrictor(d_model=256, num_layers=2, vocab_size=256, device="cpu")
+    with pytest.raises(ValueError, match="2 blocks"):
+        m.train_step(torch.zeros(3, dtype=torch.uint8), m.init_caches(3)[:1])
+    with pytest.raises(ValueError, match="2 blocks"):
+        m.train_forward(torch.zeros(3, 4, dtype=torch.uint8), caches=m.init_caches(3) * 2)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, BF])
+def test_far_rows_of_one_position(dtype):
+    """A dimension of one keeps any stride through contiguous(); the kernels are given rows that are near all the same."""
+    far = torch.zeros(2, 1, 16, dtype=dtype).as_strided((2, 1, 16), (16, 1 << 27, 1))
+    for near in (ops._scan_rows(far), ops._scalar_rows(far)):
+        assert near.stride() == (16, 16, 1) and near.shape == far.shape
