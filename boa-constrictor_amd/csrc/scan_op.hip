@@ -69,7 +69,7 @@ __device__ __forceinline__ uint32_t fresh_scalar(uint32_t c) {
 }
 
 // This wavefront's states of B or C in the rows of a block, through the scalar cache (constant address space: nothing the
-// kernel writes; 16-bit rows are 4-byte aligned, and a block of rows spans less than 2 GiB, which the entry points check).
+// kernel writes; 16-bit rows are 4-byte aligned, and a block of rows spans less than 4 GiB, which the entry points check).
 // A row's place is a 32-bit offset from the block's first: one scalar multiplication, where 64-bit addresses of single rows
 // cost ten scalar instructions, more than the vector work of a row.
 template <int DT>
@@ -79,8 +79,9 @@ struct ScalarRows {
     uint32_t bytes;  // of a row
     __device__ __forceinline__ ScalarRows(const Rows& a, int64_t b, int64_t t, int q)
         : p((const char*)(row<DT>(a, b, t) + q * NQ)), bytes((uint32_t)a.r * (uint32_t)sizeof(typename Elem<DT>::T)) {}
-    __device__ __forceinline__ void ahead() { p += bytes * SUB; }
-    __device__ __forceinline__ void back() { p -= bytes * SUB; }
+    __device__ __forceinline__ void ahead(bool on) { p += on ? bytes * SUB : 0; }
+    template <int ROWS = SUB>
+    __device__ __forceinline__ void back(bool on) { p -= on ? bytes * ROWS : 0; }
     __device__ __forceinline__ void next_block() { bytes = fresh_scalar(bytes); }
     __device__ __forceinline__ void load(int s, uint32_t (&w)[WORDS]) const {
         typedef __attribute__((address_space(4))) const char CByte;
@@ -95,21 +96,24 @@ struct ScalarRows {
     }
 };
 
-// Two positions of a block as the recurrence reads them: B and C from the scalar cache, what was prepared from LDS.  A pair is
-// on its way while the one before it is computed.  Both kinds of load return out of order to one counter, so a wait is for
-// all that are under way: the pair to compute is waited for (here) before the next one is issued.
-template <int DT>
-struct Pair {
+// G positions of a block as the recurrence reads them: B and C from the scalar cache, what was prepared from LDS.  A group is
+// on its way while the one before it is computed, B and C across the blocks' borders too (the states' part of 2 x 16384 positions
+// of 512 channels: forward 99 -> 95 us, of the chunks alone 70 -> 63).  Both kinds of load return out of order to one counter, so
+// a wait is for all that are under way: the group to compute is waited for (here) before the next one is issued.
+constexpr int GROUP_ONE = 4, GROUP_TWO = 2;  // where B or C is read, and where both are: 4 spills scalar registers (95, 104 us)
+template <int DT, int G>
+struct Group {
     using S = ScalarRows<DT>;
-    uint32_t B[2][S::WORDS], C[2][S::WORDS];
-    float2 in[2];
-    float g[2];
+    uint32_t B[G][S::WORDS], C[G][S::WORDS];
+    float2 in[G];
+    float g[G];
     __device__ __forceinline__ void here() {
-        asm volatile("" : "+v"(in[0].x), "+v"(in[0].y), "+v"(in[1].x), "+v"(in[1].y));
-    }
-    static __device__ __forceinline__ void words_here(uint32_t (&w)[2][S::WORDS]) {
 #pragma unroll
-        for (int j = 0; j < 2; ++j)
+        for (int j = 0; j < G; ++j) asm volatile("" : "+v"(in[j].x), "+v"(in[j].y));
+    }
+    static __device__ __forceinline__ void words_here(uint32_t (&w)[G][S::WORDS]) {
+#pragma unroll
+        for (int j = 0; j < G; ++j)
 #pragma unroll
             for (int i = 0; i < S::WORDS; ++i) asm volatile("" : "+s"(w[j][i]));
     }
@@ -126,7 +130,8 @@ struct LaneRows {
     __device__ __forceinline__ LaneRows(const Rows& a, int64_t b, int64_t t)
         : p((gmut<char>)row_mut<DT>(a, b, t)), bytes((uint32_t)a.r * (uint32_t)sizeof(T)) {}
     __device__ __forceinline__ void ahead(bool on) { p += on ? bytes * SUB : 0; }
-    __device__ __forceinline__ void back(bool on) { p -= on ? bytes * SUB : 0; }
+    template <int ROWS = SUB>
+    __device__ __forceinline__ void back(bool on) { p -= on ? bytes * ROWS : 0; }
     // c: the lane's channel in bytes
     __device__ __forceinline__ gmut<T> at(int s, uint32_t& c) const { return (gmut<T>)(p + (uint32_t)s * bytes + fresh(c)); }
     __device__ __forceinline__ T load(int s, uint32_t& c) const { return *at(s, c); }
@@ -316,35 +321,49 @@ __global__ void __launch_bounds__(WG) k_scan_fwd(const ScanArgs a) {
         xu.ahead(more), xd.ahead(more), xz.ahead(more);
         fetch(more);
     }
-    for (int i = 0; i < n_subs; ++i) {
+    // the first group of a block is on its way before the block begins
+    constexpr int G = MODE == LOCAL ? GROUP_ONE : GROUP_TWO;
+    Group<DT, G> group[2];
+    auto words = [&](int i, int s0, Group<DT, G>& x) {
         xB.next_block(), xC.next_block();
+        const int last = min(SUB, count - i * SUB) - 1;  // rows behind the end are read as the last one
+#pragma unroll
+        for (int j = 0; j < G; ++j) {
+            xB.load(min(s0 + j, last), x.B[j]);
+            if constexpr (MODE != LOCAL) xC.load(min(s0 + j, last), x.C[j]);
+        }
+    };
+    auto prepared = [&](int i, int s0, Group<DT, G>& x) {
+#pragma unroll
+        for (int j = 0; j < G; ++j) x.in[j] = s_in[i & 1][s0 + j][p.lane];
+    };
+    if (n_subs > 0) words(0, 0, group[0]);
+    for (int i = 0; i < n_subs; ++i) {
         __syncthreads();
         if constexpr (MODE == OUT_MARKS) {
 #pragma unroll
             for (int n = 0; n < NQ; ++n) *lane_at(mark + (uint32_t)(n * a.channels), c4) = h[n];
             mark += NS * a.channels;
         }
-        const int last = min(SUB, count - i * SUB) - 1;  // rows behind the end are read as the last one
-        Pair<DT> pair[2];
-        auto issue = [&](int s0, Pair<DT>& x) {
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                xB.load(min(s0 + j, last), x.B[j]);
-                if constexpr (MODE != LOCAL) xC.load(min(s0 + j, last), x.C[j]);
-                x.in[j] = s_in[i & 1][s0 + j][p.lane];
-            }
-            __builtin_amdgcn_sched_barrier(0);
-        };
-        issue(0, pair[0]);
+        prepared(i, 0, group[0]);
+        __builtin_amdgcn_sched_barrier(0);
         if (MODE != LOCAL && i > 0) finish(i - 1, u_before, z_before, true);
 #pragma unroll
-        for (int s0 = 0; s0 < SUB; s0 += 2) {
-            Pair<DT>& x = pair[s0 / 2 % 2];
+        for (int s0 = 0; s0 < SUB; s0 += G) {
+            Group<DT, G>&x = group[s0 / G % 2], &next = group[s0 / G % 2 ^ 1];
             x.here(), x.words_here(x.B);
             if constexpr (MODE != LOCAL) x.words_here(x.C);
-            if (s0 + 2 < SUB) issue(s0 + 2, pair[s0 / 2 % 2 ^ 1]);
+            if (s0 + G < SUB) {
+                words(i, s0 + G, next);
+                prepared(i, s0 + G, next);
+            } else {
+                const bool more = i + 1 < n_subs;
+                xB.ahead(more), xC.ahead(more);
+                words(more ? i + 1 : i, 0, next);
+            }
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
+            for (int j = 0; j < G; ++j) {
                 float y = 0.0f;
 #pragma unroll
                 for (int n = 0; n < NQ; ++n) {
@@ -355,7 +374,6 @@ __global__ void __launch_bounds__(WG) k_scan_fwd(const ScanArgs a) {
                 else s_y[i & 1][p.q][s0 + j][p.lane] = y;
             }
         }
-        xB.ahead(), xC.ahead();
         prepare(i + 1, u_next, z_next);
         const bool more = i + 2 < n_subs;
         xu.ahead(more), xd.ahead(more), xz.ahead(more);
@@ -415,17 +433,23 @@ __device__ __forceinline__ ScalarRows<DT> again(ScalarRows<DT> x) {
     return x;
 }
 
-// What the backward pass loads of a block's positions, from the chunk's last block to its first.
+// What the backward pass loads of a block's positions, from the chunk's last block to its first.  Where marks do not set the
+// block's size it is twice as long, for half the barriers (2 x 16384 positions of 512 channels: 78 -> 72 us; the forward pass,
+// of which more wavefronts run at once, 65 -> 69).
+constexpr int LOCAL_SUB = 2 * SUB;
 template <int DT, bool LOCAL_>
 struct BackIn {
     using E = Elem<DT>;
+    static constexpr int BLOCK = LOCAL_ ? LOCAL_SUB : SUB, MINE = BLOCK / WAVES;
     LaneRows<DT> xu, xd, xz, xy;
     typename E::T ru[MINE], rd[MINE], rz[MINE], ry[MINE];
     int first;  // this wavefront's first position of a block
     // t: the first position of the block to start with; without a gate z is dy
     __device__ __forceinline__ BackIn(const ScanArgs& a, const Place& p, int64_t t)
         : xu(a.u, p.b, t), xd(a.delta, p.b, t), xz(a.z.p != nullptr ? a.z : a.dy, p.b, t), xy(a.dy, p.b, t), first(p.q * MINE) {}
-    __device__ __forceinline__ void back(bool on) { xu.back(on), xd.back(on), xz.back(on), xy.back(on); }
+    __device__ __forceinline__ void back(bool on) {
+        xu.template back<BLOCK>(on), xd.template back<BLOCK>(on), xz.template back<BLOCK>(on), xy.template back<BLOCK>(on);
+    }
     // left: positions from the block's first one to the end
     __device__ __forceinline__ void fetch(int left, uint32_t& ce) {
 #pragma unroll
@@ -444,62 +468,73 @@ struct BackIn {
 template <int DT>
 __global__ void __launch_bounds__(WG) k_scan_bwd_local(const ScanArgs a) {
     using E = Elem<DT>;
-    __shared__ float2 s_in[2][SUB][64];  // dt, g
+    constexpr int BLOCK = LOCAL_SUB, MINE = BLOCK / WAVES;
+    __shared__ float2 s_in[2][BLOCK][64];  // dt, g
     const Place p(a, a.chunks - 1, 1);
     const int64_t end = end_of(a, p.b), lo = p.k * a.chunk;
     if (lo >= end) return;
-    const int n_subs = (int)ceil_div(min(lo + a.chunk, end) - lo, SUB);
+    const int n_subs = (int)ceil_div(min(lo + a.chunk, end) - lo, BLOCK);
     float a2[NQ], dh[NQ] = {}, dts = 0.0f;
     p.decay(a, a2);
     const float bias = a.bias != nullptr ? a.bias[p.cc] : 0.0f;
     const int count = (int)(min(lo + a.chunk, end) - lo);
     const bool gate = a.z.p != nullptr;
     uint32_t ce = p.cc * (uint32_t)sizeof(typename E::T);
-    BackIn<DT, true> in(a, p, lo + (n_subs - 1) * SUB);
-    ScalarRows<DT> xC(a.C, p.b, lo + (n_subs - 1) * SUB, p.q);
+    BackIn<DT, true> in(a, p, lo + (n_subs - 1) * BLOCK);
+    ScalarRows<DT> xC(a.C, p.b, lo + (n_subs - 1) * BLOCK, p.q);
     auto prepare = [&](int i) {
 #pragma unroll
         for (int k = 0; k < MINE; ++k) {
             const int at = in.first + k;
             const float dt = hw_softplus(E::ld(in.rd[k]) + bias), g = E::ld(in.ry[k]) * (gate ? hw_silu(E::ld(in.rz[k])) : 1.0f);
-            s_in[i & 1][at][p.lane] = i * SUB + at < count ? make_float2(dt, g) : make_float2(0.0f, 0.0f);
+            s_in[i & 1][at][p.lane] = i * BLOCK + at < count ? make_float2(dt, g) : make_float2(0.0f, 0.0f);
         }
     };
-    in.fetch(count - (n_subs - 1) * SUB, ce);
+    in.fetch(count - (n_subs - 1) * BLOCK, ce);
     prepare(n_subs - 1);
     in.back(n_subs > 1);
-    in.fetch(n_subs > 1 ? SUB : count, ce);
-    for (int i = n_subs - 1; i >= 0; --i) {
+    in.fetch(n_subs > 1 ? BLOCK : count, ce);
+    // the last group of a block, which comes first, is on its way before the block begins
+    constexpr int G = GROUP_ONE;
+    Group<DT, G> group[2];
+    auto words = [&](int i, int s0, Group<DT, G>& x) {
         xC.next_block();
-        __syncthreads();
-        const int last = min(SUB, count - i * SUB) - 1;  // rows behind the end are read as the last one
-        Pair<DT> pair[2];
-        auto issue = [&](int s0, Pair<DT>& x) {
+        const int last = min(BLOCK, count - i * BLOCK) - 1;  // rows behind the end are read as the last one
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                xC.load(min(s0 + j, last), x.C[j]);
-                x.in[j] = s_in[i & 1][s0 + j][p.lane];
+        for (int j = 0; j < G; ++j) xC.load(min(s0 + j, last), x.C[j]);
+    };
+    auto prepared = [&](int i, int s0, Group<DT, G>& x) {
+#pragma unroll
+        for (int j = 0; j < G; ++j) x.in[j] = s_in[i & 1][s0 + j][p.lane];
+    };
+    words(n_subs - 1, BLOCK - G, group[0]);
+    for (int i = n_subs - 1; i >= 0; --i) {
+        __syncthreads();
+        prepared(i, BLOCK - G, group[0]);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int s0 = BLOCK - G; s0 >= 0; s0 -= G) {
+            Group<DT, G>&x = group[(BLOCK - G - s0) / G % 2], &next = group[(BLOCK - s0) / G % 2];
+            x.here(), x.words_here(x.C);
+            if (s0 > 0) {
+                words(i, s0 - G, next);
+                prepared(i, s0 - G, next);
+            } else {
+                xC.template back<BLOCK>(i > 0);
+                words(max(i - 1, 0), BLOCK - G, next);
             }
             __builtin_amdgcn_sched_barrier(0);
-        };
-        issue(SUB - 2, pair[0]);
 #pragma unroll
-        for (int s0 = SUB - 2; s0 >= 0; s0 -= 2) {
-            Pair<DT>&x = pair[(SUB - 2 - s0) / 2 % 2], &next = pair[(SUB - s0) / 2 % 2];
-            x.here(), x.words_here(x.C);
-            if (s0 > 0) issue(s0 - 2, next);
-#pragma unroll
-            for (int j = 1; j >= 0; --j) {
+            for (int j = G - 1; j >= 0; --j) {
 #pragma unroll
                 for (int n = 0; n < NQ; ++n)
                     dh[n] = __builtin_fmaf(x.c(j, n), x.in[j].y, dh[n]) * __builtin_amdgcn_exp2f(x.in[j].x * a2[n]);
                 dts += x.in[j].x;
             }
         }
-        xC.back();
         if (i > 0) prepare(i - 1);
         in.back(i > 1);
-        in.fetch(min(SUB, count), ce);
+        in.fetch(min(BLOCK, count), ce);
     }
     if (!p.live) return;
     const int64_t r = p.b * a.chunks + p.k;
@@ -538,6 +573,15 @@ __global__ void __launch_bounds__(WG, 4) k_scan_bwd(const ScanArgs a) {
 #pragma unroll
         for (int n = 0; n < NQ; ++n) mark[n] = *lane_at(marks + (uint32_t)(n * a.channels), c4);
     };
+    // Pairs of positions; a block's first one is on its way (in pair[1]) before the block begins.
+    Group<DT, 2> pair[2];
+    auto words = [&](int s0, int last, Group<DT, 2>& x, const ScalarRows<DT>& fromB, const ScalarRows<DT>& fromC) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            fromB.load(min(s0 + j, last), x.B[j]);
+            fromC.load(min(s0 + j, last), x.C[j]);
+        }
+    };
     // whole: all the block's positions are inside (all blocks but the first one here)
     auto block = [&](int i, auto whole) {
         constexpr bool WHOLE = decltype(whole)::value;
@@ -562,26 +606,32 @@ __global__ void __launch_bounds__(WG, 4) k_scan_bwd(const ScanArgs a) {
         for (int n = 0; n < NQ; ++n) h[n] = live ? mark[n] : 0.0f;
         __syncthreads();
         const int last = WHOLE ? SUB - 1 : count - t0 - 1;  // rows behind the end are read as the last one
-        Pair<DT> pair[2];
-        auto issue = [&](int s0, Pair<DT>& x, const ScalarRows<DT>& fromB, const ScalarRows<DT>& fromC) {
+        auto prepared = [&](int s0, Group<DT, 2>& x) {
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
-                fromB.load(min(s0 + j, last), x.B[j]);
-                fromC.load(min(s0 + j, last), x.C[j]);
                 x.in[j] = s_in[s0 + j][p.lane];
                 x.g[j] = s_g[s0 + j][p.lane];
             }
+        };
+        auto issue = [&](int s0, Group<DT, 2>& x, const ScalarRows<DT>& fromB, const ScalarRows<DT>& fromC) {
+            words(s0, last, x, fromB, fromC);
+            prepared(s0, x);
             __builtin_amdgcn_sched_barrier(0);
         };
-        auto here = [&](Pair<DT>& x) {
+        auto here = [&](Group<DT, 2>& x) {
             x.here(), x.words_here(x.B), x.words_here(x.C);
             asm volatile("" : "+v"(x.g[0]), "+v"(x.g[1]));
         };
-        issue(0, pair[0], xB, xC);
+        prepared(0, pair[0]);
+        pair[1].words_here(pair[1].B), pair[1].words_here(pair[1].C);
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int w = 0; w < ScalarRows<DT>::WORDS; ++w) pair[0].B[j][w] = pair[1].B[j][w], pair[0].C[j][w] = pair[1].C[j][w];
         float r[8];
 #pragma unroll
         for (int s0 = 0; s0 < SUB; s0 += 2) {
-            Pair<DT>& x = pair[s0 / 2 % 2];
+            Group<DT, 2>& x = pair[s0 / 2 % 2];
             here(x);
             if (s0 + 2 < SUB) issue(s0 + 2, pair[s0 / 2 % 2 ^ 1], xB, xC);
 #pragma unroll
@@ -607,9 +657,15 @@ __global__ void __launch_bounds__(WG, 4) k_scan_bwd(const ScanArgs a) {
         const ScalarRows<DT> xB2 = again(xB), xC2 = again(xC);
 #pragma unroll
         for (int s0 = SUB - 2; s0 >= 0; s0 -= 2) {
-            Pair<DT>& x = pair[s0 / 2 % 2];  // the last one is still here
+            Group<DT, 2>& x = pair[s0 / 2 % 2];  // the last one is still here
             if (s0 < SUB - 2) here(x);
-            if (s0 > 0) issue(s0 - 2, pair[s0 / 2 % 2 ^ 1], xB2, xC2);
+            if (s0 > 0) {
+                issue(s0 - 2, pair[s0 / 2 % 2 ^ 1], xB2, xC2);
+            } else {
+                xB.back(i > 0), xC.back(i > 0);
+                words(0, i > 0 ? SUB - 1 : last, pair[1], xB, xC);
+                __builtin_amdgcn_sched_barrier(0);
+            }
 #pragma unroll
             for (int j = 1; j >= 0; --j) {
                 const int s = s0 + j;
@@ -637,7 +693,6 @@ __global__ void __launch_bounds__(WG, 4) k_scan_bwd(const ScanArgs a) {
                 fetch(i > 0 ? SUB : count - t0);
             }
         }
-        xB.back(), xC.back();
         *lane_at(bc_out, tid4) = (p.lane & 1) ? bc : dC;
         bc_out -= WG;
         __syncthreads();
@@ -673,6 +728,7 @@ __global__ void __launch_bounds__(WG, 4) k_scan_bwd(const ScanArgs a) {
     };
     if (n_subs > 0) {
         fetch(count - (n_subs - 1) * SUB);
+        words(0, count - (n_subs - 1) * SUB - 1, pair[1], xB, xC);
         if (a.joined) {
 #pragma unroll
             for (int n = 0; n < NQ; ++n) dh[n] = a.local[state_at(a, p, p.b * a.chunks + p.k, n)];

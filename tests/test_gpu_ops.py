@@ -622,6 +622,30 @@ def test_offsets_beyond_32_bits(ops):
     assert torch.equal(ops.cross_entropy(flat, t), ops.cross_entropy(flat.contiguous(), t))
 
 
+def test_scan_rows_as_far_apart_as_they_may_be(ops):
+    """Rows at the largest stride: a block of 16 spans almost 4 GiB, two chunks 27 GB; the bits of contiguous inputs."""
+    from boa_amd import _native
+
+    g = _gen(23)
+    length, c, far = 100, 64, _native.BOA_SCAN_MAX_ROW_STRIDE
+    big = torch.empty((length - 1) * far + 256, device="cuda")
+    s = {k: v.detach() for k, v in _scan_inputs(g, 1, length, c, torch.float32).items()}
+    state, dy = _randn(g, 1, 16, c), _randn(g, 1, length, c)
+    near, spread, at = dict(s), dict(s), 0
+    for k in ("u", "delta", "B", "C"):
+        spread[k] = torch.as_strided(big, near[k].shape, (far, far, 1), at)
+        spread[k].copy_(near[k])
+        at += near[k].shape[-1]
+    got = []
+    for t in (near, spread):
+        leaf = {k: v.requires_grad_() for k, v in t.items()}
+        y, end = ops.selective_scan(**leaf, state=state, return_state=True)
+        got.append([y, end, *torch.autograd.grad(y, tuple(leaf.values()), dy)])
+    assert all(torch.equal(p, q) for p, q in zip(*got))
+    del big, spread, leaf, got, t, y
+    torch.cuda.empty_cache()
+
+
 def test_differentiable_once(ops):
     x = _randn(_gen(22), 4, 64).requires_grad_()
     g, = torch.autograd.grad(ops.layer_norm(x).square().sum(), x, retain_graph=True)
