@@ -214,38 +214,57 @@ __device__ __forceinline__ void over_chunks(const ScanArgs& a, const Place& p, i
 enum { LOCAL, OUT, OUT_MARKS };
 
 // Where there are many chunks, the state before each of them instead: from the ends of the chunks before it (of those behind
-// it, from the sequence's end, in the backward pass), in the places of local.  A thread takes one state through all chunks.
-constexpr int JOIN_WG = 64;  // few threads, all waiting for loads: on as many CUs as there are
+// it, from the sequence's end, in the backward pass), in the places of local.  A lane takes one state through the chunks, each of
+// the four wavefronts a quarter of them, with all their loads in flight at once, and their ends meet in LDS.
+constexpr int MAX_CHUNKS = 128;
 template <bool BACK>
-__global__ void __launch_bounds__(JOIN_WG) k_scan_join(const ScanArgs a) {
-    constexpr int AT_ONCE = 32;
-    const int64_t i = (int64_t)blockIdx.x * JOIN_WG + threadIdx.x;
-    if (i >= a.batch * NS * a.channels) return;
-    const int64_t b = i / (NS * a.channels);
-    const int n = (int)(i / a.channels % NS), c = (int)(i % a.channels);
-    const int64_t end = end_of(a, b);
-    const int chunks = (int)ceil_div(end, a.chunk);  // with positions inside
-    const float a2 = a.A[(int64_t)c * NS + n] * LOG2E;
-    float h = !BACK && a.state_in != nullptr ? a.state_in[i] : 0.0f;
-    for (int j0 = 0; j0 < chunks; j0 += AT_ONCE) {
-        float dts[AT_ONCE], l[AT_ONCE];
-        // the first chunk has no end of its own in the backward pass, the last one none in the forward pass
+__global__ void __launch_bounds__(WG) k_scan_join(const ScanArgs a) {
+    constexpr int AT_ONCE = MAX_CHUNKS / WAVES;
+    __shared__ float s_e[WAVES][64], s_h[WAVES][64];
+    const int lane = threadIdx.x & 63, q = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int64_t states = (int64_t)NS * a.channels, i0 = (int64_t)blockIdx.x * 64, b0 = i0 / states;  // b0: of the first lane
+    // 32 bits are enough in a workgroup: more than two sequences have less than 64 states each
+    uint32_t i = (uint32_t)(i0 - b0 * states) + lane, of = i / (uint32_t)states;
+    const bool live = b0 + of < a.batch;
+    if (!live) of = 0, i = 0;
+    const uint32_t in = i % (uint32_t)states, n = in / (uint32_t)a.channels, c = in % (uint32_t)a.channels;
+    const int64_t b = b0 + of;
+    uint32_t l4 = (uint32_t)((of * a.chunks * states + in) * 4), dts4 = (of * a.chunks * a.channels + c) * 4;  // bytes
+    auto chunk = [&](int j) {  // the wavefront's j-th, in the order of the recurrence
+        const int at = min(q * AT_ONCE + j, a.chunks - 1);
+        return BACK ? a.chunks - 1 - at : at;
+    };
+    // what is not there (the sums of the last chunk, in the backward pass of the first one, and of those behind the end) is read
+    // all the same, but reaches no h that is kept
+    float e[AT_ONCE], l[AT_ONCE];
 #pragma unroll
-        for (int j = 0; j < AT_ONCE; ++j) {
-            const int at = min(j0 + j, chunks - 2), k = BACK ? chunks - 1 - at : at;
-            const int64_t r = b * a.chunks + k;
-            dts[j] = chunks > 1 ? a.dts[r * a.channels + c] : 0.0f;
-            l[j] = chunks > 1 ? a.local[(r * NS + n) * a.channels + c] : 0.0f;
-        }
-#pragma unroll
-        for (int j = 0; j < AT_ONCE; ++j) {
-            const int at = j0 + j;
-            if (at < chunks) {
-                a.local[((b * a.chunks + (BACK ? chunks - 1 - at : at)) * NS + n) * a.channels + c] = h;
-                h = __builtin_fmaf(__builtin_amdgcn_exp2f(dts[j] * a2), h, l[j]);
-            }
-        }
+    for (int j = 0; j < AT_ONCE; ++j) {
+        e[j] = *lane_at(G(a.dts) + (b0 * a.chunks + chunk(j)) * a.channels, dts4);
+        l[j] = *lane_at(G(a.local) + (b0 * a.chunks + chunk(j)) * states, l4);
     }
+    const int chunks = (int)ceil_div(end_of(a, b), a.chunk);  // with positions inside
+    const float a2 = a.A[(int64_t)c * NS + n] * LOG2E;
+    const float start = !BACK && a.state_in != nullptr ? a.state_in[b * states + in] : 0.0f;
+    auto inside = [&](int j) { return q * AT_ONCE + j < a.chunks && chunk(j) < chunks; };
+    float h = 0.0f, dts = 0.0f;
+#pragma unroll
+    for (int j = 0; j < AT_ONCE; ++j) {
+        const float dt = e[j];
+        e[j] = __builtin_amdgcn_exp2f(dt * a2);
+        if (inside(j)) h = __builtin_fmaf(e[j], h, l[j]), dts += dt;
+    }
+    s_e[q][lane] = __builtin_amdgcn_exp2f(dts * a2);
+    s_h[q][lane] = h;
+    __syncthreads();
+    h = start;
+    for (int w = 0; w < q; ++w) h = __builtin_fmaf(s_e[w][lane], h, s_h[w][lane]);
+    if (!live) return;
+#pragma unroll
+    for (int j = 0; j < AT_ONCE; ++j)
+        if (inside(j)) {
+            *lane_at(GM(a.local) + (b0 * a.chunks + chunk(j)) * states, l4) = h;
+            h = __builtin_fmaf(e[j], h, l[j]);
+        }
 }
 
 // LOCAL: the state that a chunk alone leaves (from zeros) and its sum of dt, for every chunk but the last; OUT: the chunk's
@@ -776,8 +795,18 @@ __global__ void __launch_bounds__(WG) k_scan_sums(const ScanArgs a, int64_t bc_b
         const int64_t end = end_of(a, b), t = i * SUB + ((lane >> 2 & 1) + (lane & 2)) * 2 + (lane >> 5);
         if (t >= a.length) continue;
         float v = 0.0f;
-        if (t < end)
-            for (int cb = 0; cb < a.cblocks; ++cb) v += a.part_bc[(((int64_t)cb * a.batch + b) * a.subs + i) * WG + threadIdx.x];
+        if (t < end) {
+            constexpr int AT_ONCE = 8;
+            const float* part = a.part_bc + k * WG + threadIdx.x;
+            const int64_t next = a.batch * a.subs * WG;  // the next block of channels
+            for (int cb = 0; cb < a.cblocks; cb += AT_ONCE) {
+                float x[AT_ONCE];
+#pragma unroll
+                for (int j = 0; j < AT_ONCE; ++j) x[j] = part[min(cb + j, a.cblocks - 1) * next];
+#pragma unroll
+                for (int j = 0; j < AT_ONCE; ++j) v += cb + j < a.cblocks ? x[j] : 0.0f;
+            }
+        }
         row_mut<DT>((lane & 1) ? a.dB : a.dC, b, t)[q * NQ + ((lane >> 3) & 3)] = Elem<DT>::st(v);
     }
 }
@@ -844,10 +873,10 @@ struct Plan {
 // (32 sequences of up to 500 positions, 1024 channels, bfloat16: forward 84 us with 1024, 68 with 2048, 64 with 4096; backward
 // 194, 161, 142).
 int64_t wanted_workgroups(const boa_scan* s, bool backward) { return s->lens ? 4096 : backward ? 1024 : 1536; }
-constexpr int64_t MIN_CHUNK = 64, MAX_CHUNKS = 128;
+constexpr int64_t MIN_CHUNK = 64;
 // From more chunks than this on they are joined by a kernel of its own: to go over the chunks before its own costs a workgroup
 // of the last chunk 0.3 us for each, and reads them for every workgroup again (2 x 16384 positions of 512 channels: forward
-// kernel 129 us, with k_scan_join 97 + 14; backward, of 64 chunks, 247 and 233 + 11; forward, 16 chunks of 8 x 1000, 34 and 30 + 5).
+// kernel 129 us, with k_scan_join 97 + 7; backward, of 64 chunks, 241 and 227 + 7; forward, 16 chunks of 8 x 1000, 34 and 30 + 5).
 constexpr int JOIN_FROM = 32;
 Plan plan(const boa_scan* s, bool backward) {
     const int64_t blocks = s->batch * ceil_div(s->channels, 64);
@@ -943,7 +972,7 @@ extern "C" int boa_selective_scan_fwd(const boa_scan* s, void* d_work, int64_t w
             hipLaunchKernelGGL((k_scan_fwd<DT, LOCAL>), dim3(blocks * (a.chunks - 1)), dim3(WG), 0, (hipStream_t)stream, a);
             BOA_HIP_TRY(hipGetLastError());
             if (a.joined) {
-                hipLaunchKernelGGL((k_scan_join<false>), dim3((uint32_t)ceil_div(a.batch * NS * a.channels, JOIN_WG)), dim3(JOIN_WG), 0,
+                hipLaunchKernelGGL((k_scan_join<false>), dim3((uint32_t)ceil_div(a.batch * NS * a.channels, 64)), dim3(WG), 0,
                                    (hipStream_t)stream, a);
                 BOA_HIP_TRY(hipGetLastError());
             }
@@ -983,7 +1012,7 @@ extern "C" int boa_selective_scan_bwd(const boa_scan* s, void* d_work, int64_t w
                 hipLaunchKernelGGL((k_scan_bwd_local<DT>), dim3(blocks * (a.chunks - 1)), dim3(WG), 0, st, a);
                 BOA_HIP_TRY(hipGetLastError());
                 if (a.joined) {
-                    hipLaunchKernelGGL((k_scan_join<true>), dim3((uint32_t)ceil_div(a.batch * NS * a.channels, JOIN_WG)), dim3(JOIN_WG), 0,
+                    hipLaunchKernelGGL((k_scan_join<true>), dim3((uint32_t)ceil_div(a.batch * NS * a.channels, 64)), dim3(WG), 0,
                                        st, a);
                     BOA_HIP_TRY(hipGetLastError());
                 }
