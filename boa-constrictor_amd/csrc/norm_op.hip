@@ -8,6 +8,9 @@
 // row is read once per pass, and takes several of them at a time to have enough loads in flight.  In the backward pass a
 // wavefront adds its rows' dy xh and dy in registers, a workgroup its wavefronts' through LDS, and k_sum_parts the workgroups':
 // no atomics, so the same inputs give the same bits.
+//
+// Measured: 262144 rows of 512 bfloat16, forward 99 us (5.4 TB/s), backward 155 and 5 for the parameters' sums (5.0 TB/s; a copy of
+// 1 GiB runs at 5.0); 8000 rows of 256 float32, 5 and 10 us.
 #include "ops_common.h"
 
 #include "../../include/boa_hip.h"
@@ -18,7 +21,9 @@ namespace {
 
 constexpr int WG = 256, WAVES = WG / 64;
 constexpr int MAX_D = BOA_LAYER_NORM_MAX_D;
-constexpr int WAVE_D = 1024;  // rows up to here are a wavefront's, wider ones a workgroup's
+// Rows up to here are a wavefront's, wider ones a workgroup's: as a wavefront's, 32 values per lane, 32768 rows of 2048 bfloat16 took
+// 123 us forward (52 as a workgroup's), and of 4096 float32, 64 values, 178 (100).
+constexpr int WAVE_D = 1024;
 static_assert(MAX_D <= 16 * WG, "16 values per thread");
 
 // Rows that a wavefront takes at a time, for PER elements per lane: 16 values in flight per lane.
@@ -51,15 +56,31 @@ struct Row {
             if (col(i, lane) < d) st_vec<DT, VEC>(row + col(i, lane), t);
         }
     }
-    // a float32 parameter row in the same places; `other` beyond d and where there is none
+    // a float32 parameter row in the same places (16-byte aligned, if the accesses are of several elements); `other` beyond d and
+    // where there is none
     static __device__ __forceinline__ void param(const float* p, int d, int lane, float other, float (&v)[PER]) {
+        constexpr int PART = VEC == 1 ? 1 : 4;
 #pragma unroll
-        for (int i = 0; i < N; ++i)
+        for (int i = 0; i < PER; i += PART) {
+            const int c = col(i / VEC, lane) + i % VEC;
+            float t[PART];
+            if (p != nullptr && c < d) ld_vec<DT_F32, PART>(p + c, t);
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) {
-                const int c = col(i, lane) + j;
-                v[i * VEC + j] = (p != nullptr && c < d) ? p[c] : other;
-            }
+            for (int j = 0; j < PART; ++j) v[i + j] = (p != nullptr && c < d) ? t[j] : other;
+        }
+    }
+    // float32 values into such places of a row that begins anywhere
+    static __device__ __forceinline__ void put(float* p, int d, int lane, const float (&v)[PER]) {
+        constexpr int PART = VEC == 1 ? 1 : 4;
+        typedef float Part __attribute__((ext_vector_type(PART), aligned(4)));
+#pragma unroll
+        for (int i = 0; i < PER; i += PART) {
+            const int c = col(i / VEC, lane) + i % VEC;
+            Part t;
+#pragma unroll
+            for (int j = 0; j < PART; ++j) t[j] = v[i + j];
+            if (c < d) *reinterpret_cast<Part*>(p + c) = t;
+        }
     }
     // K sums over the row's threads
     template <int K>
@@ -82,6 +103,14 @@ struct Row {
         }
     }
 };
+
+// And in the backward pass, which reads two arrays and has more registers in use: two rows where one is an access of 8 bytes per
+// lane (262144 rows of 256 bfloat16 87 us, 94 one at a time), else one (2 or 4 rows: float32 of 256 and 512 bfloat16 the same, 2048
+// bfloat16 99, 103 and 182).
+template <class R>
+constexpr int bwd_rows_at_once() {
+    return R::VECTOR == 4 && R::PER == 4 && sizeof(typename R::T) == 2 ? 2 : 1;
+}
 
 template <class R, int DT>
 __global__ void __launch_bounds__(WG) k_norm_fwd(const void* xp, int64_t xs, const float* w, const float* b, int64_t rows,
@@ -129,7 +158,7 @@ template <class R, int DT>
 __global__ void __launch_bounds__(WG) k_norm_bwd(const void* dyp, int64_t dys, const void* xp, int64_t xs, const float* w,
                                                  const float2* stats, int64_t rows, int d, void* dxp, int64_t dxs,
                                                  float* part) {
-    constexpr int PER = R::PER, ROWS = rows_at_once(2 * PER), VEC = R::VECTOR;
+    constexpr int PER = R::PER, ROWS = bwd_rows_at_once<R>(), VEC = R::VECTOR;
     const auto* x = static_cast<const typename R::T*>(xp);
     const auto* dy = static_cast<const typename R::T*>(dyp);
     auto* dx = static_cast<typename R::T*>(dxp);
@@ -148,35 +177,37 @@ __global__ void __launch_bounds__(WG) k_norm_bwd(const void* dyp, int64_t dys, c
             R::load(dy + at * dys, d, lane, g[r]);
             st[r] = stats[at];
         }
+        float m[2 * ROWS];  // sums of g, and of g xh
 #pragma unroll
         for (int r = 0; r < ROWS; ++r) {
-            if (r0 + r >= rows) break;
-            float m[2] = {0.0f, 0.0f};  // sums of g, and of g xh
+            const bool once = r0 + r < rows;  // the last row is read again behind the end
+            m[2 * r] = m[2 * r + 1] = 0.0f;
 #pragma unroll
             for (int i = 0; i < PER; ++i) {
                 const float xh = (v[r][i] - st[r].x) * st[r].y;  // beyond d: dy is 0 there
-                dw[i] = __builtin_fmaf(g[r][i], xh, dw[i]);
-                db[i] += g[r][i];
-                const float gw = g[r][i] * wv[i];
-                m[0] += gw;
-                m[1] = __builtin_fmaf(gw, xh, m[1]);
+                const float gd = once ? g[r][i] : 0.0f;
+                dw[i] = __builtin_fmaf(gd, xh, dw[i]);
+                db[i] += gd;
+                const float gw = gd * wv[i];
+                m[2 * r] += gw;
+                m[2 * r + 1] = __builtin_fmaf(gw, xh, m[2 * r + 1]);
                 v[r][i] = xh;
                 g[r][i] = gw;
             }
-            R::sums(m);
+        }
+        R::sums(m);
 #pragma unroll
-            for (int i = 0; i < PER; ++i) v[r][i] = (g[r][i] - m[0] * inv - v[r][i] * (m[1] * inv)) * st[r].y;
-            R::store(dx + (r0 + r) * dxs, d, lane, v[r]);
+        for (int r = 0; r < ROWS; ++r) {
+#pragma unroll
+            for (int i = 0; i < PER; ++i) v[r][i] = (g[r][i] - m[2 * r] * inv - v[r][i] * (m[2 * r + 1] * inv)) * st[r].y;
+            if (r0 + r < rows) R::store(dx + (r0 + r) * dxs, d, lane, v[r]);
         }
     }
     if (part == nullptr) return;
     float* out = part + (int64_t)blockIdx.x * 2 * d;
     if constexpr (R::TEAMS == 1) {
-#pragma unroll
-        for (int i = 0; i < PER; ++i) {
-            const int c = R::col(i / VEC, lane) + i % VEC;
-            if (c < d) out[c] = dw[i], out[d + c] = db[i];
-        }
+        R::put(out, d, lane, dw);
+        R::put(out + d, d, lane, db);
     } else {
         __shared__ float sum[2][R::LANES * PER];
         for (int k = 0; k < R::TEAMS; ++k) {
@@ -202,25 +233,30 @@ __global__ void __launch_bounds__(SUM_COLS * SUM_GROUPS) k_sum_parts(const float
     sum_parts<SUM_GROUPS>(part, parts, width, out, blockIdx.x);
 }
 
-// Workgroups of the backward pass, each of which leaves a partial row of 2 d sums: four rows or more per wavefront (a row or
-// more per workgroup where a row takes one).
+// Workgroups of the backward pass, each of which leaves a partial row of 2 d sums: 4 rows or more per team (1000 rows of 4096
+// float32 16 us, with a row per workgroup 20), and no more than run at once; of rows of more than 2048 values half of that, for the
+// partial rows' sake (16384 rows of 4096: float32 167 -> 154 us, bfloat16 103 -> 87; of 2048 bfloat16 it would be 90 -> 99).
 int64_t bwd_groups(int64_t rows, int d) {
-    const int64_t n = d <= WAVE_D ? ceil_div(rows, 4 * WAVES) : rows;
-    return n < 1024 ? n : 1024;
+    const int64_t n = ceil_div(rows, d <= WAVE_D ? 4 * WAVES : 4), most = d <= MAX_D / 2 ? 1024 : 512;
+    return n < most ? n : most;
 }
 
 // Calls f with the row shape for width d: accesses of 16 bytes (8 for 16-bit rows of up to 256 values, which then take all 64
-// lanes) where the rows are aligned for them, else single elements; up to 16 values per lane.
+// lanes) where rows and parameters are aligned for them, else single elements; up to 16 values per lane.  Backward and forward,
+// 16 bytes and single elements: 174762 rows of 384 bfloat16 129 and 148 us, 131072 of 512 float32 244 and 255.
 template <int DT, class F>
 int with_row(int d, bool aligned, F f) {
     constexpr int W = wide<DT>();
     if (aligned && d % 4 == 0 && d <= 256) return f(Row<DT, 4, 1, 64>());
     if (aligned && d % W == 0) {
-        if (d <= 64 * W) return f(Row<DT, W, 1, 64>());
-        if (d <= 128 * W && d <= WAVE_D) return f(Row<DT, W, 2, 64>());
-        if (d <= WAVE_D) return f(Row<DT, W, 16 / W, 64>());
-        if (d <= WG * W) return f(Row<DT, W, 1, WG>());
-        return f(Row<DT, W, 16 / W, WG>());
+        const bool wave = d <= WAVE_D;
+        const int64_t n = ceil_div(d, (wave ? 64 : WG) * W);
+        if (n <= 1) return wave ? f(Row<DT, W, 1, 64>()) : f(Row<DT, W, 1, WG>());
+        if (n <= 2) return wave ? f(Row<DT, W, 2, 64>()) : f(Row<DT, W, 2, WG>());
+        if constexpr (W == 4) {
+            if (n <= 3) return wave ? f(Row<DT, W, 3, 64>()) : f(Row<DT, W, 3, WG>());
+            return wave ? f(Row<DT, W, 4, 64>()) : f(Row<DT, W, 4, WG>());
+        }
     }
     if (d <= 256) return f(Row<DT, 1, 4, 64>());
     if (d <= 512) return f(Row<DT, 1, 8, 64>());
@@ -228,6 +264,7 @@ int with_row(int d, bool aligned, F f) {
     if (d <= 8 * WG) return f(Row<DT, 1, 8, WG>());
     return f(Row<DT, 1, 16, WG>());
 }
+bool params_aligned(const float* w, const float* b) { return ((uintptr_t)w | (uintptr_t)b) % 16 == 0; }
 int check_norm(const char* who, int dtype, int64_t rows, int32_t d) {
     if (dtype < BOA_DT_F32 || dtype > BOA_DT_F16) return boa_fail(BOA_ERR_ARG, "%s: unknown type %d", who, dtype);
     if (rows < 0 || d < 1 || d > MAX_D)
@@ -252,7 +289,7 @@ extern "C" int boa_layer_norm_fwd(int dtype, const void* d_x, int64_t x_stride, 
     if (rc != BOA_OK) return rc;
     if (rows == 0) return BOA_OK;
     if (!d_x || !d_y) return boa_fail(BOA_ERR_ARG, "boa_layer_norm_fwd: null pointer");
-    const bool al = aligned16(dtype, d_x, x_stride) && aligned16(dtype, d_y, y_stride);
+    const bool al = aligned16(dtype, d_x, x_stride) && aligned16(dtype, d_y, y_stride) && params_aligned(d_w, d_b);
     return with_dtype(dtype, [&](auto dt) {
         constexpr int DT = decltype(dt)::value;
         return with_row<DT>(d, al, [&](auto row) {
@@ -285,7 +322,8 @@ extern "C" int boa_layer_norm_bwd(int dtype, const void* d_dy, int64_t dy_stride
     float* part = d_dwb ? static_cast<float*>(d_work) : nullptr;
     const int64_t groups = rows > 0 ? bwd_groups(rows, d) : 0;
     if (rows > 0) {
-        const bool al = aligned16(dtype, d_x, x_stride) && aligned16(dtype, d_dy, dy_stride) && aligned16(dtype, d_dx, dx_stride);
+        const bool al = aligned16(dtype, d_x, x_stride) && aligned16(dtype, d_dy, dy_stride) && aligned16(dtype, d_dx, dx_stride) &&
+                        params_aligned(d_w, nullptr);
         const int launched = with_dtype(dtype, [&](auto dt) {
             constexpr int DT = decltype(dt)::value;
             return with_row<DT>(d, al, [&](auto row) {
