@@ -9,6 +9,9 @@
 // per run (and three times more at the runs' borders, from cache).  The backward pass computes p again instead of
 // reading it.  Positions before the first come from the state (zeros without one); positions from a sequence's length on are
 // not read and are written as zeros.
+//
+// Measured: 64 x 1500 positions of 512 channels, float32: forward 75 us (393 MB: 5.2 TB/s), backward 130 (590 MB: 4.5; with dy and x
+// in part still in the last cache 53 and 91); bfloat16 36 and 77.  One position of 64 x 512, 3 us.
 #include "ops_common.h"
 
 #include "../../include/boa_hip.h"
@@ -19,7 +22,9 @@ namespace {
 
 constexpr int TAPS = 4, PAST = TAPS - 1;
 constexpr int LANES = 64, RUNS = 4, WG = LANES * RUNS;  // a wavefront: 64 channel vectors of one run
-constexpr int RUN = 16;                                 // positions of a run
+// Positions of a run: of 8, 16 and 32 the case above takes 72, 75 and 83 us forward and 130, 130 and 131 backward, in bfloat16
+// 35, 36 and 44, and 87, 77 and 71; a single sequence of 1000 positions 6, 6 and 10, and 11, 12 and 19.
+constexpr int RUN = 16;
 constexpr int MAX_GROUPS = 1024;                        // workgroups along the runs
 
 struct ConvArgs {
@@ -225,6 +230,8 @@ __global__ void __launch_bounds__(WG) k_conv_step(const void* xp, int64_t xs, vo
     for (int q = 0; q < PAST; ++q) *reinterpret_cast<typename W::V*>(st + q * (int64_t)C) = r[q + 1];
 }
 
+// Four channels at a time where all rows are aligned for it (else one): the case above, forward and backward, 205 us (208 with
+// single ones), in bfloat16 113 (326).
 bool vec_ok(int dtype, const void* p, int64_t s0, int64_t s1) {
     const int64_t bytes = dtype == BOA_DT_F32 ? 16 : 8;
     return (uintptr_t)p % bytes == 0 && s0 % 4 == 0 && s1 % 4 == 0;

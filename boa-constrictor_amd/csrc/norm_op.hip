@@ -21,8 +21,8 @@ namespace {
 
 constexpr int WG = 256, WAVES = WG / 64;
 constexpr int MAX_D = BOA_LAYER_NORM_MAX_D;
-// Rows up to here are a wavefront's, wider ones a workgroup's: as a wavefront's, 32 values per lane, 32768 rows of 2048 bfloat16 took
-// 123 us forward (52 as a workgroup's), and of 4096 float32, 64 values, 178 (100).
+// Rows up to here are a wavefront's, wider ones a workgroup's.  As a wavefront's, forward and backward, 32768 rows of 2048 float32 take
+// 97 and 160 us (as a workgroup's 99 and 161), 16384 of 4096 106 and 316 (97 and 155).
 constexpr int WAVE_D = 1024;
 static_assert(MAX_D <= 16 * WG, "16 values per thread");
 

@@ -16,7 +16,13 @@
 // channel) is shared out: of SUB = 8 positions a wavefront prepares two (softplus, gate) and finishes two (the sum over
 // states, the gate, the stores), through LDS.  The forward pass of a training step leaves the state at every SUB positions
 // ("marks", 8 bytes per (position, channel)); the backward pass walks the blocks of SUB positions from the last one,
-// computes each forward again from its mark with e and e h in registers, then backward.
+// computes each forward again from its mark with e and e h in registers, then backward.  Where the batch has too few
+// workgroups the length is split into chunks: a first kernel computes what each chunk alone leaves (forward its last state, backward
+// the adjoint before it), and the main one goes on from those of the chunks before its own.
+//
+// Measured, float32 of 2 x 16384 positions and 512 channels: chunks alone 64 us, joined 7, forward 97 (of the vector units' cycles
+// 0.67 and 0.68), backward 72 + 7 + 227 (0.7, 0.84) + 13 for the sums, where one pass over the data would take 54 and 94 us of
+// memory; 8 x 1000 of 512: 20 + 33 and 20 + 64 + 4; a prompt of 4 x 4097 and 1024 channels in bfloat16: 62 + 90.
 #include "ops_common.h"
 
 #include "../../include/boa_hip.h"
@@ -562,7 +568,8 @@ __global__ void __launch_bounds__(WG) k_scan_bwd_local(const ScanArgs a) {
     if (p.q == 0) a.dts[r * a.channels + p.c] = dts;
 }
 
-// ALL: every lane has a channel (channels a multiple of 64), so the stores need no lane mask.
+// ALL: every lane has a channel (channels a multiple of 64), so the stores need no lane mask (2 x 16384 positions: the whole backward
+// pass 289 us for 512 channels, 322 for 511, whose rows are not aligned either).
 template <int DT, bool ALL>
 __global__ void __launch_bounds__(WG, 4) k_scan_bwd(const ScanArgs a) {
     using E = Elem<DT>;
@@ -812,7 +819,7 @@ __global__ void __launch_bounds__(WG) k_scan_sums(const ScanArgs a, int64_t bc_b
 }
 
 // One position: a lane has the 16 states of its channel, a wavefront 64 channels of some sequences (A and the parameters are
-// read once for all of them).  Bound by the states' way in and out.
+// read once for all of them).  Bound by the states' way in and out: 1000 x 1024, 23 us (131 MB: 5.7 TB/s); 1 x 512, 3.5 us.
 template <int DT>
 __global__ void __launch_bounds__(WG) k_scan_step(const ScanArgs a, int64_t walkers) {
     using E = Elem<DT>;
