@@ -7,8 +7,9 @@
 // 1 / sum_r are kept, 8 bytes per row) and writes their gradient.  Both are bound by memory.  A row whose target is
 // ignore_index counts for nothing (its gradient is 0); one whose target is not a symbol gives NaN, in its loss and its gradient.
 //
-// Measured: 262144 rows of 256 bfloat16, forward 32 to 42 us (134 MB: 4.2 TB/s and less), backward 43 (268 MB: 6.2 TB/s, the logits
-// in part still in the last cache); float32 49 (5.5 TB/s) and 112 (4.8).  8000 rows of 256 float32, 4.5, 5.4 and 2.6 for the sum.
+// Measured: 262144 rows of 256 bfloat16, forward 39 us (134 MB: 3.4 TB/s, with the gradient of the pass before still on its way to
+// memory; 32 alone), backward 42 (268 MB: 6.4 TB/s, the logits in part still in the last cache); float32 49 (5.5 TB/s) and 112
+// (4.8).  8000 rows of 256 float32, 4.5 and 5.4, and 2.6 for the sum.
 #include "ops_common.h"
 
 #include "../../include/boa_hip.h"
@@ -19,7 +20,7 @@ namespace {
 
 constexpr int WG = 256, WAVES = WG / 64;
 constexpr int MAX_V = BOA_CROSS_ENTROPY_MAX_V;
-constexpr int MAX_GROUPS = 2048;
+constexpr int MAX_GROUPS = 4096;  // 262144 rows of 256 bfloat16: 39 us, with 2048 42, with 8192 38 and 0.7 more for their sum
 
 // Rows that a wavefront has in flight, for PER elements per lane.
 constexpr int rows_at_once(int per) { return per >= 32 ? 1 : 32 / per; }  // 8, 4, 2 or 1

@@ -21,7 +21,7 @@
 // the adjoint before it), and the main one goes on from those of the chunks before its own.
 //
 // Measured, float32 of 2 x 16384 positions and 512 channels: chunks alone 64 us, joined 7, forward 97 (of the vector units' cycles
-// 0.67 and 0.68), backward 72 + 7 + 227 (0.7, 0.84) + 13 for the sums, where one pass over the data would take 54 and 94 us of
+// 0.74 and 0.68), backward 72 + 7 + 229 (0.71, 0.85) + 13 for the sums, where one pass over the data would take 54 and 94 us of
 // memory; 8 x 1000 of 512: 20 + 33 and 20 + 64 + 4; a prompt of 4 x 4097 and 1024 channels in bfloat16: 62 + 90.
 #include "ops_common.h"
 
