@@ -258,6 +258,7 @@ class BoaBytePredictor(nn.Module):
         return eng
 
     def release_engines(self):
+        """Gives the contexts' memory back; the next use lays the weights out as they are then."""
         self._engines.clear()
 
     def plan_wave_lanes(self, n_chunks: int, chunk_len: int, cap: int = 65536) -> int:
@@ -325,7 +326,9 @@ class BoaBytePredictor(nn.Module):
         ``forward`` runs the codec's fused kernels and has no gradient; this is the training loop's forward (train.py:59).
         It runs on the parameters as they are now: there is no copy of the weights to rebuild after an optimizer step.  Under
         ``torch.autocast`` the products, the convolution and the scan run in its type, layer norms and residuals in float32.
-        Its logits are not bit-identical with ``forward``'s, so files are written and read with ``forward`` alone.
+        Its logits are not bit-identical with ``forward``'s, so files are written and read with ``forward`` alone.  ``forward`` and
+        the codec lay the weights out anew when they have changed, but do not see what a replayed graph has written: call
+        ``release_engines()`` behind the replays of a captured update.
 
         lens: lengths of the sequences in a padded batch.  caches: states of ``init_caches`` that the bytes continue and that
         are advanced in place (truncated back-propagation, or streaming without an engine)."""

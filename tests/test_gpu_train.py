@@ -200,3 +200,29 @@ def test_captured_training_step(gpu):
         assert _rel(loss, want.cpu()) <= 1e-6
         for p, q in zip(params, eager.parameters()):
             assert _rel(p, q.cpu()) <= 1e-6
+
+
+def test_weights_trained_by_a_graph_compress(gpu):
+    """The codec does not see what a replayed graph writes; release_engines() makes it look."""
+    import codec
+
+    m, _ = _model(1)
+    data = np.random.default_rng(7).integers(0, 4, 300).astype(np.uint8)
+    w = m.head[2].weight
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side), torch.no_grad():
+        w.mul_(1.0)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph), torch.no_grad():
+        w.mul_(0.5)
+    before = codec.compress_payload(m, [data])[0]
+    graph.replay()
+    m.release_engines()
+    got = codec.compress_payload(m, [data])[0]
+    other, _ = _model(1)
+    with torch.no_grad():
+        other.head[2].weight.mul_(0.5)
+    want = codec.compress_payload(other, [data])[0]
+    assert np.array_equal(got, want) and not np.array_equal(got, before)
