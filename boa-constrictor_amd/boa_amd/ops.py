@@ -219,31 +219,36 @@ def layer_norm(x, weight=None, bias=None, eps: float = 1e-5):
 
 # ---- cross entropy ---------------------------------------------------------------------------------
 class _CrossEntropy(torch.autograd.Function):
+    # In one allocation: the forward pass's workspace, the number of rows that count, and what the backward pass needs of each row.
     @staticmethod
     def forward(ctx, x, target, ignore, reduction, keep):
         n, v = x.shape
-        stats = torch.empty((n, 2), dtype=torch.float32, device=x.device) if keep else None
-        each = torch.empty(n, dtype=torch.float32, device=x.device) if reduction == "none" else None
-        loss, count = (torch.empty((), dtype=torch.float32, device=x.device) if each is None else None for _ in range(2))
         lib = _nat.lib()
-        size = _bytes("boa_cross_entropy_work_bytes") if each is None else 0
-        work = _work(size, x)
+        size = 0 if reduction == "none" else _bytes("boa_cross_entropy_work_bytes")
+        buf = torch.empty(size + 16 + (8 * n if keep else 0), dtype=torch.uint8, device=x.device)
+        work = buf.data_ptr()
+        count, stats = work + size, work + size + 16
+        loss = torch.empty(n if reduction == "none" else (), dtype=torch.float32, device=x.device)
+        each, all_rows = (loss.data_ptr(), 0) if reduction == "none" else (0, loss.data_ptr())
         _call(x, lib.boa_cross_entropy_fwd, _DTYPES[x.dtype], x.data_ptr(), x.stride(0), target.data_ptr(), target.element_size(),
-              ignore, n, v, reduction == "mean", _ptr(stats), _ptr(each), _ptr(loss), _ptr(count), _ptr(work), size)
-        ctx.save_for_backward(x, target, stats, count)
-        ctx.ignore, ctx.reduction = ignore, reduction
-        return loss if each is None else each
+              ignore, n, v, reduction == "mean", stats if keep else 0, each, all_rows, count if all_rows else 0,
+              work if all_rows else 0, size)
+        if keep:
+            ctx.save_for_backward(x, target, buf)
+            ctx.ignore, ctx.reduction, ctx.size = ignore, reduction, size
+        return loss
 
     @staticmethod
     def backward(ctx, up):
         _once(ctx)
-        x, target, stats, count = ctx.saved_tensors
+        x, target, buf = ctx.saved_tensors
         n, v = x.shape
         up = up.contiguous()  # float32, as the loss is
         dx = x.new_empty((n, v))
+        count = buf.data_ptr() + ctx.size
         _call(x, _nat.lib().boa_cross_entropy_bwd, _DTYPES[x.dtype], x.data_ptr(), x.stride(0), target.data_ptr(),
-              target.element_size(), ctx.ignore, n, v, stats.data_ptr(), up.data_ptr(), ctx.reduction == "none",
-              _ptr(count) if ctx.reduction == "mean" else 0, dx.data_ptr(), v)
+              target.element_size(), ctx.ignore, n, v, count + 16, up.data_ptr(), ctx.reduction == "none",
+              count if ctx.reduction == "mean" else 0, dx.data_ptr(), v)
         return dx, None, None, None, None
 
 
