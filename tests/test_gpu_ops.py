@@ -69,6 +69,25 @@ def test_norm(ops, rows, d, dtype):
     _check("db", db, ref["db"], rows, torch.float32)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,d,params", [(41, 384, 4), (41, 768, 4), (11, 1152, 4), (11, 1536, 4), (9, 2500, 4), (6, 4000, 4),
+                                           (20011, 64, 4), (17001, 200, 4), (4501, 1152, 4), (2101, 2500, 4), (2101, 2501, 4),
+                                           (50, 256, 1), (50, 512, 2), (9, 2048, 3)])
+def test_norm_widths_loops_and_parameters_anywhere(ops, rows, d, params, dtype):
+    """More widths, rows that take several steps of a workgroup, parameters that begin at any multiple of 4 bytes."""
+    g = _gen(rows * d)
+    x, dy = _randn(g, rows, d, dtype=dtype, scale=2, mean=0.5).requires_grad_(), _randn(g, rows, d, dtype=dtype)
+    w, b = (_randn(g, d + 4)[params:][:d].detach().requires_grad_() for _ in range(2))
+    y = ops.layer_norm(x, w, b)
+    dx, dw, db = torch.autograd.grad(y, (x, w, b), dy)
+    ref = R.norm(x, w, b, dy)
+    n = 4 * (d / 64 + 8) + 16
+    _check("y", y, ref["y"], n, dtype)
+    _check("dx", dx, ref["dx"], 2 * n, dtype)
+    _check("dw", dw, ref["dw"], n + rows, torch.float32)
+    _check("db", db, ref["db"], rows, torch.float32)
+
+
 def test_norm_without_parameters_and_odd_layouts(ops):
     g = _gen(1)
     wide = _randn(g, 6, 5, 300)
@@ -694,3 +713,70 @@ def test_saved_states_are_watched(ops):
         B = x[:, 0, :16]
         ops.selective_scan_step(x[:, 0], x[:, 1], -torch.ones(64, 16, device="cuda"), B, B, state=b)
         assert a.abs().sum() > 0 and b.abs().sum() > 0
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_many_rows_are_each_as_alone(ops, dtype):
+    """More rows, runs and sequences than the workgroups take in one step: the bits of smaller calls."""
+    g = _gen(24)
+    x = _randn(g, 140003, 40, dtype=dtype, scale=3).requires_grad_()
+    t = torch.randint(0, 40, (140003,), generator=g, device="cuda", dtype=torch.uint8)
+    up = _randn(g, 140003)
+    y = ops.cross_entropy(x, t, reduction="none")
+    dx, = torch.autograd.grad(y, (x,), up)
+    for at in range(0, 140003, 50000):
+        part = x.detach()[at:at + 50000].requires_grad_()
+        z = ops.cross_entropy(part, t[at:at + 50000], reduction="none")
+        assert torch.equal(z, y[at:at + 50000])
+        assert torch.equal(torch.autograd.grad(z, (part,), up[at:at + 50000])[0], dx[at:at + 50000])
+    mean = ops.cross_entropy(x.detach(), t)
+    # summed in 64 bits, rounded once
+    assert abs(float(mean) - float(y.detach().double().mean())) <= (2.0 ** -24 + 2.0 ** -34) * float(mean)
+
+    for c, n, length in ((3, 150001, 2), (8, 9001, 17)):
+        w, b = _randn(g, c, 4), _randn(g, c)
+        x, dy = _randn(g, n, length, c, dtype=dtype).requires_grad_(), _randn(g, n, length, c, dtype=dtype)
+        y = ops.causal_conv(x, w, b)
+        dx, = torch.autograd.grad(y, (x,), dy)
+        for at in range(0, n, 70000):
+            part = x.detach()[at:at + 70000].requires_grad_()
+            z = ops.causal_conv(part, w, b)
+            assert torch.equal(z, y[at:at + 70000])
+            assert torch.equal(torch.autograd.grad(z, (part,), dy[at:at + 70000])[0], dx[at:at + 70000])
+
+    n, c = 20001, 70
+    act = [_randn(g, n, c, dtype=dtype) for _ in range(3)] + [_randn(g, n, 16, dtype=dtype) for _ in range(2)]
+    A, D, bias, state = -torch.rand(c, 16, device="cuda") * 16, _randn(g, c), _randn(g, c), _randn(g, n, 16, c)
+    st = state.clone()
+    y = ops.selective_scan_step(act[0], act[1], A, act[3], act[4], D, act[2], bias, state=st)
+    for at in range(0, n, 6000):
+        u, delta, z, B, C = (v[at:at + 6000] for v in act)
+        s = state[at:at + 6000].clone()
+        assert torch.equal(ops.selective_scan_step(u, delta, A, B, C, D, z, bias, state=s), y[at:at + 6000])
+        assert torch.equal(s, st[at:at + 6000])
+
+
+def test_scan_of_the_most_channels(ops):
+    """65536 channels: each as in a call of its own; dB and dC, here of terms without signs, are the sums over the calls."""
+    g = _gen(25)
+    n, length, c, step = 1, 60, 65536, 4096 + 64  # 60 positions: never split
+    s = {k: v if v is None else (v.abs() if k in "uBC" else v).detach().requires_grad_()
+         for k, v in _scan_inputs(g, n, length, c, torch.float32, gate=False).items()}
+    s.pop("z")
+    dy = _randn(g, n, length, c).abs()
+    y, end = ops.selective_scan(**s, return_state=True)
+    got = dict(zip(s, torch.autograd.grad(y, tuple(s.values()), dy)))
+    sums = {k: torch.zeros(n, length, 16, dtype=torch.float64, device="cuda") for k in "BC"}
+    for at in range(0, c, step):
+        cut = slice(at, min(at + step, c))
+        part = {k: (v if k in "BC" else v[cut] if k in ("A", "D", "delta_bias") else v[..., cut]).detach().requires_grad_()
+                for k, v in s.items()}
+        z, e = ops.selective_scan(**part, return_state=True)
+        assert torch.equal(z, y[..., cut]) and torch.equal(e, end[..., cut])
+        for k, v in zip(part, torch.autograd.grad(z, tuple(part.values()), dy[..., cut])):
+            if k in "BC":
+                sums[k] += v.double()
+            else:
+                assert torch.equal(v, got[k][cut] if k in ("A", "D", "delta_bias") else got[k][..., cut])
+    for k in "BC":  # a butterfly over 64 channels, then 1024 or 65 blocks of them one after another, in 32 bits
+        assert ((got[k].double() - sums[k]).abs() <= (6 + 1024 + 6 + 65) * 2.0 ** -24 * sums[k]).all()
