@@ -111,8 +111,11 @@ def _rows(t):
 
 
 def _flat(t, d):
-    """[..., d] as rows."""
-    return _rows(t if t.ndim == 2 else t.reshape(-1, d))
+    """[..., d] as rows: a tensor that holds them, their stride, their number."""
+    if t.is_contiguous():
+        return t, d, t.numel() // d
+    t = _rows(t if t.ndim == 2 else t.reshape(-1, d))
+    return t, t.stride(0), t.shape[0]
 
 
 def _gpu(who, t):
@@ -165,11 +168,11 @@ def _work(nbytes, like):
 # ---- layer norm ------------------------------------------------------------------------------------
 def _norm_fwd(x, w, b, eps, keep):
     d = x.shape[-1]
-    rows = _flat(x, d)
+    rows, stride, n = _flat(x, d)
     y = torch.empty_like(x, memory_format=torch.contiguous_format)
-    stats = torch.empty((rows.shape[0], 2), dtype=torch.float32, device=x.device) if keep else None
-    _call(x, _nat.lib().boa_layer_norm_fwd, _DTYPES[x.dtype], rows.data_ptr(), rows.stride(0), _ptr(w), _ptr(b), rows.shape[0], d,
-          eps, y.data_ptr(), d, _ptr(stats))
+    stats = torch.empty((n, 2), dtype=torch.float32, device=x.device) if keep else None
+    _call(x, _nat.lib().boa_layer_norm_fwd, _DTYPES[x.dtype], rows.data_ptr(), stride, _ptr(w), _ptr(b), n, d, eps, y.data_ptr(), d,
+          _ptr(stats))
     return y, stats
 
 
@@ -185,8 +188,8 @@ class _LayerNorm(torch.autograd.Function):
         _once(ctx)
         x, w, stats = ctx.saved_tensors
         d = x.shape[-1]
-        rows, dyr = _flat(x, d), _flat(dy, d)
-        n = rows.shape[0]
+        rows, stride, n = _flat(x, d)
+        dyr, dy_stride, _ = _flat(dy, d)
         dx = torch.empty_like(x, memory_format=torch.contiguous_format)
         _, need_w, need_b, _ = ctx.needs_input_grad
         dwb = work = None
@@ -195,7 +198,7 @@ class _LayerNorm(torch.autograd.Function):
             dwb = stats.new_empty((2, d))
             size = _bytes("boa_layer_norm_bwd_work_bytes", n, d)
             work = _work(size, x)
-        _call(x, _nat.lib().boa_layer_norm_bwd, _DTYPES[x.dtype], dyr.data_ptr(), dyr.stride(0), rows.data_ptr(), rows.stride(0), _ptr(w),
+        _call(x, _nat.lib().boa_layer_norm_bwd, _DTYPES[x.dtype], dyr.data_ptr(), dy_stride, rows.data_ptr(), stride, _ptr(w),
               stats.data_ptr(), n, d, dx.data_ptr(), d, _ptr(dwb), _ptr(work), size)
         return dx, dwb[0] if need_w else None, dwb[1] if need_b else None, None
 
@@ -222,15 +225,16 @@ class _CrossEntropy(torch.autograd.Function):
     # In one allocation: the forward pass's workspace, the number of rows that count, and what the backward pass needs of each row.
     @staticmethod
     def forward(ctx, x, target, ignore, reduction, keep):
-        n, v = x.shape
+        v = x.shape[-1]
+        rows, stride, n = _flat(x, v)
         lib = _nat.lib()
         size = 0 if reduction == "none" else _bytes("boa_cross_entropy_work_bytes")
         buf = torch.empty(size + 16 + (8 * n if keep else 0), dtype=torch.uint8, device=x.device)
         work = buf.data_ptr()
         count, stats = work + size, work + size + 16
-        loss = torch.empty(n if reduction == "none" else (), dtype=torch.float32, device=x.device)
+        loss = torch.empty(x.shape[:-1] if reduction == "none" else (), dtype=torch.float32, device=x.device)
         each, all_rows = (loss.data_ptr(), 0) if reduction == "none" else (0, loss.data_ptr())
-        _call(x, lib.boa_cross_entropy_fwd, _DTYPES[x.dtype], x.data_ptr(), x.stride(0), target.data_ptr(), target.element_size(),
+        _call(x, lib.boa_cross_entropy_fwd, _DTYPES[x.dtype], rows.data_ptr(), stride, target.data_ptr(), target.element_size(),
               ignore, n, v, reduction == "mean", stats if keep else 0, each, all_rows, count if all_rows else 0,
               work if all_rows else 0, size)
         if keep:
@@ -242,11 +246,12 @@ class _CrossEntropy(torch.autograd.Function):
     def backward(ctx, up):
         _once(ctx)
         x, target, buf = ctx.saved_tensors
-        n, v = x.shape
+        v = x.shape[-1]
+        rows, stride, n = _flat(x, v)
         up = up.contiguous()  # float32, as the loss is
-        dx = x.new_empty((n, v))
+        dx = x.new_empty(x.shape)
         count = buf.data_ptr() + ctx.size
-        _call(x, _nat.lib().boa_cross_entropy_bwd, _DTYPES[x.dtype], x.data_ptr(), x.stride(0), target.data_ptr(),
+        _call(x, _nat.lib().boa_cross_entropy_bwd, _DTYPES[x.dtype], rows.data_ptr(), stride, target.data_ptr(),
               target.element_size(), ctx.ignore, n, v, count + 16, up.data_ptr(), ctx.reduction == "none",
               count if ctx.reduction == "mean" else 0, dx.data_ptr(), v)
         return dx, None, None, None, None
@@ -271,9 +276,7 @@ def cross_entropy(logits, targets, *, ignore_index: int = -100, reduction: str =
         raise ValueError(f"cross_entropy: targets must be {list(logits.shape[:-1])} on {logits.device} "
                          f"(got {list(targets.shape)} on {targets.device})")
     _gpu("cross_entropy", logits)
-    rows = _flat(logits, logits.shape[-1])
-    out = _CrossEntropy.apply(rows, targets.reshape(-1).contiguous(), int(ignore_index), reduction, _grad(logits))
-    return out.reshape(targets.shape) if reduction == "none" else out
+    return _CrossEntropy.apply(logits, targets.contiguous(), int(ignore_index), reduction, _grad(logits))
 
 
 # ---- causal convolution ----------------------------------------------------------------------------
@@ -313,7 +316,7 @@ class _CausalConv(torch.autograd.Function):
         _call(x, _nat.lib().boa_causal_conv_bwd, _DTYPES[x.dtype], dy.data_ptr(), dy.stride(0), dy.stride(1), x.data_ptr(), x.stride(0),
               x.stride(1), w.data_ptr(), _ptr(b), ctx.silu, n, length, c, _ptr(lens), _ptr(state), dx.data_ptr(), length * c, c,
               _ptr(dwb), _ptr(work), size)
-        dw = dwb[:D_CONV * c].view(w.shape) if need_w else None
+        dw = dwb.as_strided(w.shape, w.stride()) if need_w else None
         db = dwb[D_CONV * c:] if need_b else None
         return dx, dw, db, None, None, None, None
 
@@ -443,7 +446,7 @@ class _SelectiveScan(torch.autograd.Function):
         size = lib.boa_selective_scan_work_bytes(args, 1)
         work = _work(size, u)
         _call(u, lib.boa_selective_scan_bwd, args, _ptr(work), size)
-        dA = dpar[:D_STATE * c].view(c, D_STATE)
+        dA = dpar.as_strided((c, D_STATE), (D_STATE, 1))
         dD = dpar[D_STATE * c:(D_STATE + 1) * c] if D is not None else None
         dbias = dpar[(D_STATE + 1) * c:] if bias is not None else None
         return du, ddelta, dA, dB, dC, dD, dz, dbias, None, None, None
