@@ -103,8 +103,8 @@ struct ScalarRows {
 };
 
 // G positions of a block as the recurrence reads them: B and C from the scalar cache, what was prepared from LDS.  A group is
-// on its way while the one before it is computed, B and C across the blocks' borders too (the states' part of 2 x 16384 positions
-// of 512 channels: forward 99 -> 95 us, of the chunks alone 70 -> 63).  Both kinds of load return out of order to one counter, so
+// on its way while the one before it is computed, B and C across the blocks' borders too (2 x 16384 positions of 512 channels: forward
+// 99 -> 95 us, the chunks alone 70 -> 63).  Both kinds of load return out of order to one counter, so
 // a wait is for all that are under way: the group to compute is waited for (here) before the next one is issued.
 constexpr int GROUP_ONE = 4, GROUP_TWO = 2;  // where B or C is read, and where both are: 4 spills scalar registers (95, 104 us)
 template <int DT, int G>
@@ -220,12 +220,12 @@ __device__ __forceinline__ void over_chunks(const ScanArgs& a, const Place& p, i
 enum { LOCAL, OUT, OUT_MARKS };
 
 // Where there are many chunks, the state before each of them instead: from the ends of the chunks before it (of those behind
-// it, from the sequence's end, in the backward pass), in the places of local.  A lane takes one state through the chunks, each of
-// the four wavefronts a quarter of them, with all their loads in flight at once, and their ends meet in LDS.
-constexpr int MAX_CHUNKS = 128;
+// it, from the sequence's end, in the backward pass), in the places of local.  A lane takes one state through 32 chunks with all their
+// loads in flight at once, a workgroup has as many wavefronts as that takes, and their ends meet in LDS.
+constexpr int JOIN_EACH = 32, MAX_CHUNKS = JOIN_EACH * WAVES;
 template <bool BACK>
 __global__ void __launch_bounds__(WG) k_scan_join(const ScanArgs a) {
-    constexpr int AT_ONCE = MAX_CHUNKS / WAVES;
+    constexpr int AT_ONCE = JOIN_EACH;
     __shared__ float s_e[WAVES][64], s_h[WAVES][64];
     const int lane = threadIdx.x & 63, q = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int64_t states = (int64_t)NS * a.channels, i0 = (int64_t)blockIdx.x * 64, b0 = i0 / states;  // b0: of the first lane
@@ -869,7 +869,7 @@ __global__ void __launch_bounds__(WG) k_scan_step(const ScanArgs a, int64_t walk
 Rows rows(const boa_rows& r) { return {r.p, r.batch_stride, r.row_stride}; }
 
 // The split over the length: chunks of a multiple of SUB positions, as many as give the wanted workgroups, at least MIN_CHUNK
-// positions each and at most MAX_CHUNKS (each workgroup goes over the chunks before its own).
+// positions each and at most MAX_CHUNKS.
 struct Plan {
     int chunks;
     int64_t chunk;
@@ -883,7 +883,8 @@ int64_t wanted_workgroups(const boa_scan* s, bool backward) { return s->lens ? 4
 constexpr int64_t MIN_CHUNK = 64;
 // From more chunks than this on they are joined by a kernel of its own: to go over the chunks before its own costs a workgroup
 // of the last chunk 0.3 us for each, and reads them for every workgroup again (2 x 16384 positions of 512 channels: forward
-// kernel 129 us, with k_scan_join 97 + 7; backward, of 64 chunks, 241 and 227 + 7; forward, 16 chunks of 8 x 1000, 34 and 30 + 5).
+// kernel 129 us, with k_scan_join 97 + 7; backward, of 64 chunks, 241 and 228 + 7; 24 chunks of the prompt above 89 and 84 + 7; 16 of
+// 8 x 1000 forward 32.5 and 28.7 + 6, backward 63.5 and 57.5 + 6).
 constexpr int JOIN_FROM = 32;
 Plan plan(const boa_scan* s, bool backward) {
     const int64_t blocks = s->batch * ceil_div(s->channels, 64);
@@ -894,6 +895,9 @@ Plan plan(const boa_scan* s, bool backward) {
     n = ceil_div(s->length, chunk);
     return {(int)(n > 1 ? n : 1), chunk};
 }
+
+dim3 join_grid(const ScanArgs& a) { return dim3((uint32_t)ceil_div(a.batch * NS * a.channels, 64)); }
+dim3 join_block(const ScanArgs& a) { return dim3(64 * (uint32_t)ceil_div(a.chunks, JOIN_EACH)); }
 
 // Workspace, in floats: chunk states and sums of dt (more than one chunk), then in the backward pass the partial sums.
 struct Work {
@@ -979,8 +983,7 @@ extern "C" int boa_selective_scan_fwd(const boa_scan* s, void* d_work, int64_t w
             hipLaunchKernelGGL((k_scan_fwd<DT, LOCAL>), dim3(blocks * (a.chunks - 1)), dim3(WG), 0, (hipStream_t)stream, a);
             BOA_HIP_TRY(hipGetLastError());
             if (a.joined) {
-                hipLaunchKernelGGL((k_scan_join<false>), dim3((uint32_t)ceil_div(a.batch * NS * a.channels, 64)), dim3(WG), 0,
-                                   (hipStream_t)stream, a);
+                hipLaunchKernelGGL((k_scan_join<false>), join_grid(a), join_block(a), 0, (hipStream_t)stream, a);
                 BOA_HIP_TRY(hipGetLastError());
             }
         }
@@ -1019,8 +1022,7 @@ extern "C" int boa_selective_scan_bwd(const boa_scan* s, void* d_work, int64_t w
                 hipLaunchKernelGGL((k_scan_bwd_local<DT>), dim3(blocks * (a.chunks - 1)), dim3(WG), 0, st, a);
                 BOA_HIP_TRY(hipGetLastError());
                 if (a.joined) {
-                    hipLaunchKernelGGL((k_scan_join<true>), dim3((uint32_t)ceil_div(a.batch * NS * a.channels, 64)), dim3(WG), 0,
-                                       st, a);
+                    hipLaunchKernelGGL((k_scan_join<true>), join_grid(a), join_block(a), 0, st, a);
                     BOA_HIP_TRY(hipGetLastError());
                 }
             }
