@@ -7,8 +7,9 @@
   causal_conv_step, selective_scan_step   one token per sequence, states advanced in place
 
 All of them run hand-written kernels of libboa_hip.so (include/boa_hip.h) on the current stream of their tensors' device,
-synchronize nothing and can be captured into a graph.  The first four are differentiable (once): gradients reach every
-floating input but the states.  Activations are float32, bfloat16 or float16, all of a call of the same type; parameters,
+synchronize nothing and can be captured into a graph.  The first four are differentiable (once, backward): gradients reach
+every floating input but the states; inputs with a tangent of forward-mode differentiation are refused, and so is every call
+that torch.jit.trace or make_fx records.  Activations are float32, bfloat16 or float16, all of a call of the same type; parameters,
 scan states and the gradients of parameters are float32; arithmetic is in float32 and each result is rounded once.  The same
 inputs give the same bits.
 
@@ -29,6 +30,7 @@ import functools
 import struct
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.graph import increment_version
 
 from boa_amd import _native as _nat
@@ -146,10 +148,24 @@ def _call(t, f, *args):
             _nat.check(f(*args, _raw_stream(i)))
 
 
-def _once(ctx):
+_tracing, _mode, _PROXY = torch._C._get_tracing_state, torch._C._get_dispatch_mode, torch._C._TorchDispatchModeKey.PROXY
+
+
+def _plain(who, *ts):
+    """Refuses what a kernel behind a pointer would drop without a word: tangents, and the recording of the call by a tracer."""
+    if forward_ad._current_level >= 0 and torch._C._is_fwd_grad_enabled():
+        for t in ts:
+            if isinstance(t, _Tensor) and forward_ad.unpack_dual(t).tangent is not None:
+                raise RuntimeError(f"{who}: forward-mode differentiation is not supported")
+    if _tracing() is not None or _mode(_PROXY) is not None:
+        raise RuntimeError(f"{who}: cannot be traced (torch.jit.trace, make_fx)")
+
+
+def _once(who, dy):
     """The gradients are made by kernels, which autograd cannot differentiate again."""
     if torch.is_grad_enabled():
         raise RuntimeError("the operators of boa_amd.ops are differentiable once (create_graph is not supported)")
+    _plain(who, dy)
 
 
 @functools.lru_cache(maxsize=256)
@@ -185,7 +201,7 @@ class _LayerNorm(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dy):
-        _once(ctx)
+        _once("layer_norm", dy)
         x, w, stats = ctx.saved_tensors
         d = x.shape[-1]
         rows, stride, n = _flat(x, d)
@@ -207,6 +223,7 @@ def layer_norm(x, weight=None, bias=None, eps: float = 1e-5):
     """``(x - mean) / sqrt(var + eps) * weight + bias`` over the last dimension (1 to 4096 values), biased variance.
 
     x: [..., d]; weight, bias: float32 [d] or None.  Returns a contiguous tensor of x's shape and type."""
+    _plain("layer_norm", x, weight, bias)
     _act("layer_norm", "x", x)
     if x.ndim < 1 or not 1 <= x.shape[-1] <= _nat.BOA_LAYER_NORM_MAX_D:
         raise ValueError(f"layer_norm: x must be [..., d] with 1 <= d <= {_nat.BOA_LAYER_NORM_MAX_D} (got {list(x.shape)})")
@@ -244,7 +261,7 @@ class _CrossEntropy(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, up):
-        _once(ctx)
+        _once("cross_entropy", up)
         x, target, buf = ctx.saved_tensors
         v = x.shape[-1]
         rows, stride, n = _flat(x, v)
@@ -264,6 +281,7 @@ def cross_entropy(logits, targets, *, ignore_index: int = -100, reduction: str =
     logits: [..., V] (1 to 4096 symbols); targets: uint8, int32 or int64 of the leading shape.  Rows whose target is
     ignore_index count for nothing and have no gradient (a mean over no rows is NaN); any other target outside [0, V) gives
     NaN.  Returns float32."""
+    _plain("cross_entropy", logits)
     _act("cross_entropy", "logits", logits)
     if logits.ndim < 1 or not 1 <= logits.shape[-1] <= _nat.BOA_CROSS_ENTROPY_MAX_V:
         raise ValueError(f"cross_entropy: logits must be [..., V] with 1 <= V <= {_nat.BOA_CROSS_ENTROPY_MAX_V} "
@@ -301,7 +319,7 @@ class _CausalConv(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dy, _):
-        _once(ctx)
+        _once("causal_conv", dy)
         x, w, b, state, lens = ctx.saved_tensors
         n, length, c = x.shape
         dy = _rows(dy)
@@ -340,6 +358,7 @@ def causal_conv(x, weight, bias=None, *, silu: bool = True, state=None, lens=Non
     x: [batch, length, channels]; weight: float32 [channels, 1, 4] (nn.Conv1d's) or [channels, 4], oldest tap first; bias:
     float32 [channels]; state: the three positions before the first one (zeros without).  Returns y, with ``return_state``
     also the state behind each sequence's last position, as a new tensor."""
+    _plain("causal_conv", x, weight, bias, state)
     w, b = _conv_args("causal_conv", x, 3, weight, bias)
     n, length, c = x.shape
     state = _state("causal_conv", state, (n, D_CONV - 1, c), x, x.dtype, False)
@@ -357,6 +376,7 @@ def causal_conv_step(x, state, weight, bias=None, *, silu: bool = True):
     """``causal_conv`` of one position per sequence: x [batch, channels]; state [batch, 3, channels] is advanced in place.
     Returns y [batch, channels]; no gradient."""
     who = "causal_conv_step"
+    _plain(who, x, state, weight, bias)
     w, b = _conv_args(who, x, 2, weight, bias)
     n, c = x.shape
     if state is None:
@@ -434,7 +454,7 @@ class _SelectiveScan(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dy, _):
-        _once(ctx)
+        _once("selective_scan", dy)
         u, delta, A, B, C, D, z, bias, lens, marks = ctx.saved_tensors
         n, length, c = u.shape
         dy = _scan_rows(dy)
@@ -484,6 +504,7 @@ def selective_scan(u, delta, A, B, C, D=None, z=None, delta_bias=None, *, state=
     before the first position (zeros without).  Returns y, with ``return_state`` also the state behind each sequence's last
     position, as a new tensor."""
     who = "selective_scan"
+    _plain(who, u, delta, A, B, C, D, z, delta_bias, state)
     args = _scan_args(who, 3, u, delta, A, B, C, D, z, delta_bias)
     n, length, c = u.shape
     state = _state(who, state, (n, D_STATE, c), u, torch.float32, False)
@@ -500,6 +521,7 @@ def selective_scan_step(u, delta, A, B, C, D=None, z=None, delta_bias=None, *, s
     """``selective_scan`` of one position per sequence: u, delta, z [batch, channels], B, C [batch, 16]; state
     [batch, 16, channels] is advanced in place.  Returns y [batch, channels]; no gradient."""
     who = "selective_scan_step"
+    _plain(who, u, delta, A, B, C, D, z, delta_bias, state)
     args = _scan_args(who, 2, u, delta, A, B, C, D, z, delta_bias)
     n, c = u.shape
     if state is None:
