@@ -15,6 +15,7 @@ There is no CPU compute path.  The reference builds a mambapy model when no GPU 
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 import os
 
@@ -37,6 +38,26 @@ DEFAULT_TILE_LEN = int(os.environ.get("BOA_TILE_LEN", "64"))
 # same mode.
 PRECISIONS = {"f32": _nat.BOA_PREC_F32, "bf16x3": _nat.BOA_PREC_BF16X3, "bf16w": _nat.BOA_PREC_BF16W}
 DEFAULT_PRECISION = os.environ.get("BOA_PRECISION", "f32")
+
+
+def _no_grad(f):
+    """torch.no_grad() for a step that may be called between training passes of one autocast region.  Autocast keeps the weights
+    that it has cast for the rest of the region; those cast without a gradient would leave the passes behind them without one,
+    so they are not kept (unless the caller's whole code is without gradients)."""
+
+    @functools.wraps(f)
+    def call(*args, **kw):
+        if not torch.is_grad_enabled():
+            return f(*args, **kw)
+        kept = torch.is_autocast_cache_enabled()
+        torch.set_autocast_cache_enabled(False)
+        try:
+            with torch.no_grad():
+                return f(*args, **kw)
+        finally:
+            torch.set_autocast_cache_enabled(kept)
+
+    return call
 
 
 class Mixer(nn.Module):
@@ -92,7 +113,7 @@ class Mixer(nn.Module):
             ssm.copy_(ssm_end)
         return self.out_proj(y)
 
-    @torch.no_grad()
+    @_no_grad
     def step(self, x, cache):
         """One position per sequence: x [batch, d_model]; advances the cache in place (model.py:78)."""
         conv, ssm = cache
@@ -126,7 +147,7 @@ class MambaBlock(nn.Module):
         y = self.mamba(ops.layer_norm(x, self.ln1.weight, self.ln1.bias, self.ln1.eps), lens, cache)
         return x + self.ff(ops.layer_norm(y, self.ln2.weight, self.ln2.bias, self.ln2.eps))
 
-    @torch.no_grad()
+    @_no_grad
     def step(self, x, cache):
         """One position per sequence, x [batch, d_model]; advances the cache in place (model.py:75-81)."""
         y = self.mamba.step(ops.layer_norm(x, self.ln1.weight, self.ln1.bias, self.ln1.eps), cache)
@@ -358,7 +379,7 @@ class BoaBytePredictor(nn.Module):
             target = target.to(torch.long)
         return ops.cross_entropy(self.train_forward(x[:, :-1], before), target, ignore_index=-100)
 
-    @torch.no_grad()
+    @_no_grad
     def train_step(self, byte_t, caches):
         """``step`` on the parameters as they are now: bytes [B] -> logits [B, V]; advances the caches in place.  For sampling
         from a model in training; ``init_stream`` and ``step`` run a loaded model faster."""
