@@ -174,7 +174,14 @@ def _bytes(name, *sizes):
 
 
 def _ptr(t):
-    return 0 if t is None else t.data_ptr()
+    """The address of an input that may be absent.  A tensor that stands for others (a subclass that wraps them, a fake one) has
+    none, which would be taken for absence."""
+    if t is None:
+        return 0
+    p = t.data_ptr()
+    if not p and t.numel():
+        raise ValueError(f"boa_amd.ops: a {type(t).__name__} of shape {list(t.shape)} without memory of its own")
+    return p
 
 
 def _work(nbytes, like):
@@ -402,7 +409,7 @@ _NO_BACKWARD = (0,) * 19
 
 
 def _r3(t):
-    return _NO_ROWS if t is None else (t.data_ptr(), t.stride(0), t.stride(1))
+    return _NO_ROWS if t is None else (_ptr(t), t.stride(0), t.stride(1))
 
 
 def _pack(u, delta, A, B, C, D, z, bias, lens, state_in, state_out, marks, y, back=(None,) * 6, dpar=None):
@@ -535,7 +542,7 @@ def selective_scan_step(u, delta, A, B, C, D=None, z=None, delta_bias=None, *, s
     if A.data_ptr() % 16:
         A = A.clone()
 
-    zp, zs = (0, 0) if z is None else (z.data_ptr(), z.stride(0))
+    zp, zs = (0, 0) if z is None else (_ptr(z), z.stride(0))
     packed = _SCAN.pack(_DTYPES[u.dtype], c, n, 1, u.data_ptr(), u.stride(0), 0, delta.data_ptr(), delta.stride(0), 0, zp, zs, 0,
                         B.data_ptr(), B.stride(0), 0, C.data_ptr(), C.stride(0), 0, A.data_ptr(), _ptr(D), _ptr(bias), 0, 0,
                         state.data_ptr(), 0, y.data_ptr(), c, 0, *_NO_BACKWARD)
