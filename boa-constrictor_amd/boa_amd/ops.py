@@ -148,7 +148,8 @@ def _call(t, f, *args):
             _nat.check(f(*args, _raw_stream(i)))
 
 
-_tracing, _mode, _PROXY = torch._C._get_tracing_state, torch._C._get_dispatch_mode, torch._C._TorchDispatchModeKey.PROXY
+_tracing, _modes, _mode, _PROXY = (torch._C._is_tracing, torch._C._len_torch_dispatch_stack, torch._C._get_dispatch_mode,
+                                   torch._C._TorchDispatchModeKey.PROXY)
 
 
 def _plain(who, *ts):
@@ -157,7 +158,7 @@ def _plain(who, *ts):
         for t in ts:
             if isinstance(t, _Tensor) and forward_ad.unpack_dual(t).tangent is not None:
                 raise RuntimeError(f"{who}: forward-mode differentiation is not supported")
-    if _tracing() is not None or _mode(_PROXY) is not None:
+    if _tracing() or (_modes() and _mode(_PROXY) is not None):
         raise RuntimeError(f"{who}: cannot be traced (torch.jit.trace, make_fx)")
 
 
