@@ -969,7 +969,7 @@ extern "C" int boa_selective_scan_fwd(const boa_scan* s, void* d_work, int64_t w
     const int rc = check_scan("boa_selective_scan_fwd", s, a, false);
     if (rc != BOA_OK) return rc;
     if (a.batch == 0 || (a.length == 0 && !a.state_out)) return BOA_OK;
-    if (a.length > 0 && !a.y.p) return boa_fail(BOA_ERR_ARG, "boa_selective_scan_fwd: null pointer");
+    if (!a.A || (a.length > 0 && !a.y.p)) return boa_fail(BOA_ERR_ARG, "boa_selective_scan_fwd: null pointer");
     if (a.state_out && a.state_out == a.state_in)  // read by chunks that run beside the one that writes it
         return boa_fail(BOA_ERR_ARG, "boa_selective_scan_fwd: state_out must be another buffer than state_in");
     const Work w = work_of(s, false);

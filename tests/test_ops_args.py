@@ -221,3 +221,14 @@ def test_far_rows_of_one_position(dtype):
     far = torch.zeros(2, 1, 16, dtype=dtype).as_strided((2, 1, 16), (16, 1 << 27, 1))
     for near in (ops._scan_rows(far), ops._scalar_rows(far)):
         assert near.stride() == (16, 16, 1) and near.shape == far.shape
+
+
+def test_a_scan_of_no_positions_needs_its_parameters():
+    """It hands on the state by the kernel that reads them."""
+    L, bad, P = _native.load_cdll(), _native.BOA_ERR_ARG, 4096
+    packed = bytearray(_pack(length=0))
+    at_a, at_state_out = 24 + 5 * 24, 24 + 5 * 24 + 5 * 8
+    packed[at_a:at_a + 8] = bytes(8)
+    assert L.boa_selective_scan_fwd(bytes(packed), None, 0, None) == _native.BOA_OK  # no state wanted: nothing to do
+    packed[at_state_out:at_state_out + 8] = P.to_bytes(8, "little")
+    assert L.boa_selective_scan_fwd(bytes(packed), None, 0, None) == bad and b"null pointer" in L.boa_last_error()
