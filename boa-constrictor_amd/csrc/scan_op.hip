@@ -927,11 +927,13 @@ void lay_out(ScanArgs& a, const Work& w, void* d_work) {
 // Rows are read at 32-bit offsets from a block's first; those of B and C four values at a time at uniform addresses, which have
 // to be multiples of 4 bytes.
 bool stride_ok(const boa_rows& r) { return !r.p || (r.row_stride >= 0 && r.row_stride <= BOA_SCAN_MAX_ROW_STRIDE); }
-bool bc_aligned(const boa_scan* s, const boa_rows& r) {
-    return s->dtype == BOA_DT_F32 || ((uintptr_t)r.p % 4 == 0 && r.batch_stride % 2 == 0 && r.row_stride % 2 == 0);
+bool bc_aligned(const boa_scan* s, const boa_rows& r, bool step) {
+    return s->dtype == BOA_DT_F32 || ((uintptr_t)r.p % 4 == 0 && r.batch_stride % 2 == 0 && (step || r.row_stride % 2 == 0));
 }
 
-int check_scan(const char* who, const boa_scan* s, ScanArgs& a, bool backward) {
+// Looks at the members that the call uses: a step has no rows one behind the other, the backward pass no y.
+enum Pass { FORWARD, BACKWARD, STEP };
+int check_scan(const char* who, const boa_scan* s, ScanArgs& a, Pass pass) {
     if (!s) return boa_fail(BOA_ERR_ARG, "%s: null arguments", who);
     if (s->dtype < BOA_DT_F32 || s->dtype > BOA_DT_F16) return boa_fail(BOA_ERR_ARG, "%s: unknown type %d", who, s->dtype);
     if (s->batch < 0 || s->length < 0 || s->channels < 1 || s->channels > BOA_OPS_MAX_CHANNELS)
@@ -939,10 +941,10 @@ int check_scan(const char* who, const boa_scan* s, ScanArgs& a, bool backward) {
                         BOA_OPS_MAX_CHANNELS, (long long)s->batch, (long long)s->length, s->channels);
     if (s->batch > 0 && s->length > 0) {
         if (!s->u.p || !s->delta.p || !s->b.p || !s->c.p || !s->a) return boa_fail(BOA_ERR_ARG, "%s: null pointer", who);
-        for (const boa_rows* r : {&s->u, &s->delta, &s->z, &s->b, &s->c, &s->y})
-            if (!stride_ok(*r))
+        for (const boa_rows* r : {&s->u, &s->delta, &s->z, &s->b, &s->c, pass == FORWARD ? &s->y : &s->u})
+            if (pass != STEP && !stride_ok(*r))
                 return boa_fail(BOA_ERR_ARG, "%s: rows have to be 0 to %d values apart", who, BOA_SCAN_MAX_ROW_STRIDE);
-        if (!bc_aligned(s, s->b) || !bc_aligned(s, s->c))
+        if (!bc_aligned(s, s->b, pass == STEP) || !bc_aligned(s, s->c, pass == STEP))
             return boa_fail(BOA_ERR_ARG, "%s: rows of B and C of 16-bit types have to begin at multiples of 4 bytes", who);
     }
     a = ScanArgs{};
@@ -950,7 +952,7 @@ int check_scan(const char* who, const boa_scan* s, ScanArgs& a, bool backward) {
     a.A = s->a, a.D = s->d, a.bias = s->delta_bias, a.lens = s->lens, a.state_in = s->state_in, a.state_out = s->state_out;
     a.marks = s->marks, a.channels = s->channels, a.cblocks = (int)ceil_div(s->channels, 64);
     a.batch = s->batch, a.length = s->length, a.subs = ceil_div(s->length, SUB);
-    const Plan pl = plan(s, backward);
+    const Plan pl = plan(s, pass == BACKWARD);
     a.chunks = pl.chunks, a.chunk = pl.chunk, a.joined = pl.chunks > JOIN_FROM;
     if (a.batch > MAX_BLOCKS / ((int64_t)a.cblocks * a.chunks))
         return boa_fail(BOA_ERR_ARG, "%s: batch of %lld sequences too large", who, (long long)a.batch);
@@ -966,7 +968,7 @@ extern "C" int64_t boa_selective_scan_work_bytes(const boa_scan* s, int backward
 
 extern "C" int boa_selective_scan_fwd(const boa_scan* s, void* d_work, int64_t work_bytes, void* stream) {
     ScanArgs a;
-    const int rc = check_scan("boa_selective_scan_fwd", s, a, false);
+    const int rc = check_scan("boa_selective_scan_fwd", s, a, FORWARD);
     if (rc != BOA_OK) return rc;
     if (a.batch == 0 || (a.length == 0 && !a.state_out)) return BOA_OK;
     if (!a.A || (a.length > 0 && !a.y.p)) return boa_fail(BOA_ERR_ARG, "boa_selective_scan_fwd: null pointer");
@@ -999,13 +1001,13 @@ extern "C" int boa_selective_scan_fwd(const boa_scan* s, void* d_work, int64_t w
 
 extern "C" int boa_selective_scan_bwd(const boa_scan* s, void* d_work, int64_t work_bytes, void* stream) {
     ScanArgs a;
-    const int rc = check_scan("boa_selective_scan_bwd", s, a, true);
+    const int rc = check_scan("boa_selective_scan_bwd", s, a, BACKWARD);
     if (rc != BOA_OK) return rc;
     const bool any = a.batch > 0 && a.length > 0;
     if (!s->dpar) return boa_fail(BOA_ERR_ARG, "boa_selective_scan_bwd: null pointer");
     if (any && (!s->dy.p || !s->du.p || !s->ddelta.p || !s->db.p || !s->dc.p || !s->marks || (s->z.p && !s->dz.p)))
         return boa_fail(BOA_ERR_ARG, "boa_selective_scan_bwd: null pointer");
-    for (const boa_rows* r : {&s->dy, &s->du, &s->ddelta, &s->dz})
+    for (const boa_rows* r : {&s->dy, &s->du, &s->ddelta, s->z.p ? &s->dz : &s->du})
         if (any && !stride_ok(*r))
             return boa_fail(BOA_ERR_ARG, "boa_selective_scan_bwd: rows have to be 0 to %d values apart", BOA_SCAN_MAX_ROW_STRIDE);
     const Work w = work_of(s, true);
@@ -1047,7 +1049,7 @@ extern "C" int boa_selective_scan_bwd(const boa_scan* s, void* d_work, int64_t w
 
 extern "C" int boa_selective_scan_step(const boa_scan* s, void* stream) {
     ScanArgs a;
-    const int rc = check_scan("boa_selective_scan_step", s, a, false);
+    const int rc = check_scan("boa_selective_scan_step", s, a, STEP);
     if (rc != BOA_OK) return rc;
     if (a.batch == 0) return BOA_OK;
     if (a.length != 1) return boa_fail(BOA_ERR_ARG, "boa_selective_scan_step: one position per sequence (got %lld)", (long long)a.length);

@@ -232,3 +232,32 @@ def test_a_scan_of_no_positions_needs_its_parameters():
     assert L.boa_selective_scan_fwd(bytes(packed), None, 0, None) == _native.BOA_OK  # no state wanted: nothing to do
     packed[at_state_out:at_state_out + 8] = P.to_bytes(8, "little")
     assert L.boa_selective_scan_fwd(bytes(packed), None, 0, None) == bad and b"null pointer" in L.boa_last_error()
+
+
+def _put(packed, member, value, at=0):
+    """`value` as the at-th 8 bytes of a member of boa_scan."""
+    order = ["u", "delta", "z", "b", "c", "a", "d", "delta_bias", "lens", "state_in", "state_out", "marks", "y", "dy", "du",
+             "ddelta", "dz", "db", "dc", "dpar"]
+    pointers = ("a", "d", "delta_bias", "lens", "state_in", "state_out", "marks", "dpar")
+    i = 24 + sum(8 if m in pointers else 24 for m in order[:order.index(member)]) + 8 * at
+    packed[i:i + 8] = value.to_bytes(8, "little", signed=True)
+
+
+@pytest.mark.parametrize("far", [-5, 1 << 40])
+def test_members_that_a_call_does_not_use_are_ignored(far):
+    """Row strides of a step, y of a backward pass, dz without z: each call goes on to the next refusal (and launches nothing)."""
+    L, bad, P = _native.load_cdll(), _native.BOA_ERR_ARG, 4096
+    packed = bytearray(_pack(dtype=1, length=1))
+    for m in ("u", "delta", "z", "b", "c", "y"):
+        _put(packed, m, far, 2)
+    assert L.boa_selective_scan_step(bytes(packed), None) == bad and b"null pointer" in L.boa_last_error()  # no state
+    packed = bytearray(_pack())
+    _put(packed, "y", far, 2)
+    assert L.boa_selective_scan_bwd(bytes(packed), P, 0, None) == bad and b"workspace" in L.boa_last_error()
+    _put(packed, "dz", far, 2)
+    assert L.boa_selective_scan_bwd(bytes(packed), P, 0, None) == bad and b"rows have to be" in L.boa_last_error()
+    _put(packed, "z", 0)
+    assert L.boa_selective_scan_bwd(bytes(packed), P, 0, None) == bad and b"workspace" in L.boa_last_error()
+    packed = bytearray(_pack())
+    _put(packed, "y", far, 2)  # the forward pass writes y
+    assert L.boa_selective_scan_fwd(bytes(packed), P, 0, None) == bad and b"rows have to be" in L.boa_last_error()
