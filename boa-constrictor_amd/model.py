@@ -346,7 +346,9 @@ class BoaBytePredictor(nn.Module):
 
         ``forward`` runs the codec's fused kernels and has no gradient; this is the training loop's forward (train.py:59).
         It runs on the parameters as they are now: there is no copy of the weights to rebuild after an optimizer step.  Under
-        ``torch.autocast`` the products, the convolution and the scan run in its type, layer norms and residuals in float32.
+        ``torch.autocast`` the products, the convolution and the scan take and give its type, and so does a block's second layer
+        norm, whose rows come from a product and go to one; the first layer norm and the residuals are float32, and the
+        operators' arithmetic always is.
         Its logits are not bit-identical with ``forward``'s, so files are written and read with ``forward`` alone.  ``forward`` and
         the codec lay the weights out anew when they have changed, but do not see what a replayed graph has written: call
         ``release_engines()`` behind the replays of a captured update.
