@@ -4,8 +4,10 @@
 //   dx_rj = (exp(x_rj - m_r) / sum_r - [j = t]) * upstream (divided by the number of rows that count, for the mean)
 //
 // A wavefront holds a row in registers: the forward pass reads the logits once, the backward pass once more (m_r and
-// 1 / sum_r are kept, 8 bytes per row) and writes their gradient.  Both are bound by memory.  A row whose target is
-// ignore_index counts for nothing (its gradient is 0); one whose target is not a symbol gives NaN, in its loss and its gradient.
+// 1 / sum_r are kept, 8 bytes per row) and writes their gradient.  Both are bound by memory, but for the forward pass in 16
+// bits, which has 14 vector instructions per logit to its 2 bytes (the vector units are busy for 0.62 of the cycles).  A row
+// whose target is ignore_index counts for nothing (its gradient is 0); one whose target is not a symbol gives NaN, in its loss
+// and its gradient.
 //
 // Measured: 262144 rows of 256 bfloat16, forward 39 us (134 MB: 3.4 TB/s, with the gradient of the pass before still on its way to
 // memory; 32 alone), backward 42 (268 MB: 6.4 TB/s, the logits in part still in the last cache); float32 49 (5.5 TB/s) and 112

@@ -879,7 +879,10 @@ struct Plan {
 // its registers let run at once (2 x 16384 positions of 512 channels: 4 and 6 per CU forward 131 and 129 us, backward 248
 // and 273; 4 x 4097 of 1024 in bfloat16 forward 92 and 88).  Where lengths differ, smaller ones even out what the CUs have to do
 // (32 sequences of up to 500 positions, 1024 channels, bfloat16: forward 84 us with 1024, 68 with 2048, 64 with 4096; backward
-// 194, 161, 142).
+// 194, 161, 142).  The number is reached by rounding up, so a batch that has almost as many by itself is cut in two: 1000 positions
+// of 512 channels, float32, forward with 96, 128 and 191 sequences 321, 398 and 571 us (not split 283, 321, 443), backward 696, 876
+// and 1270 (684, 830, 1237); up to 500 positions of 1024, bfloat16, 64, 128 and 192 sequences, forward 151, 294, 390 (125, 193,
+// 249), backward 327, 638, 891 (296, 510, 692).
 int64_t wanted_workgroups(const boa_scan* s, bool backward) { return s->lens ? 4096 : backward ? 1024 : 1536; }
 constexpr int64_t MIN_CHUNK = 64;
 // From more chunks than this on they are joined by a kernel of its own: to go over the chunks before its own costs a workgroup
