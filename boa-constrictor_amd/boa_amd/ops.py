@@ -163,10 +163,14 @@ def _plain(who, *ts):
 
 
 def _once(who, dy):
-    """The gradients are made by kernels, which autograd cannot differentiate again."""
+    """The upstream gradient in memory: autograd hands zeros and negations on without writing them.  The gradients are made by
+    kernels, which autograd cannot differentiate again."""
     if torch.is_grad_enabled():
         raise RuntimeError("the operators of boa_amd.ops are differentiable once (create_graph is not supported)")
     _plain(who, dy)
+    if dy._is_zerotensor():
+        return torch.zeros(dy.shape, dtype=dy.dtype, device=dy.device)
+    return dy.resolve_neg()
 
 
 @functools.lru_cache(maxsize=256)
@@ -209,7 +213,7 @@ class _LayerNorm(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dy):
-        _once("layer_norm", dy)
+        dy = _once("layer_norm", dy)
         x, w, stats = ctx.saved_tensors
         d = x.shape[-1]
         rows, stride, n = _flat(x, d)
@@ -269,7 +273,7 @@ class _CrossEntropy(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, up):
-        _once("cross_entropy", up)
+        up = _once("cross_entropy", up)
         x, target, buf = ctx.saved_tensors
         v = x.shape[-1]
         rows, stride, n = _flat(x, v)
@@ -327,7 +331,7 @@ class _CausalConv(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dy, _):
-        _once("causal_conv", dy)
+        dy = _once("causal_conv", dy)
         x, w, b, state, lens = ctx.saved_tensors
         n, length, c = x.shape
         dy = _rows(dy)
@@ -462,7 +466,7 @@ class _SelectiveScan(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dy, _):
-        _once("selective_scan", dy)
+        dy = _once("selective_scan", dy)
         u, delta, A, B, C, D, z, bias, lens, marks = ctx.saved_tensors
         n, length, c = u.shape
         dy = _scan_rows(dy)

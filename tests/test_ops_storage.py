@@ -52,3 +52,30 @@ def test_empty_tensors_have_no_address_and_pass(launched):
     assert ops._ptr(torch.empty(0, C)) == 0
     ops.causal_conv(torch.zeros(0, L, C), torch.zeros(C, 4), state=torch.zeros(0, 3, C), lens=torch.zeros(0, dtype=torch.int32))
     assert len(launched) == 1
+
+
+def test_upstream_gradients_that_are_not_in_memory():
+    """Zeros that autograd hands on without memory (of sgn), and a negation that is left to the reader (of a conjugate's imaginary part,
+    with one channel, so that nothing copies it)."""
+    got = []
+
+    class Op(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, x):
+            return x.clone()
+
+        @staticmethod
+        def backward(ctx, dy):
+            before = dy
+            dy = ops._once("op", dy)
+            got.append((before.data_ptr(), before.is_neg(), dy))
+            return dy.clone()
+
+    x = torch.randn(N, L, 1, requires_grad=True)
+    torch.sgn(Op.apply(x)).sum().backward()
+    address, _, dy = got.pop()
+    assert not address and dy.data_ptr() and not dy._is_zerotensor() and not dy.any() and dy.shape == x.shape
+    up = torch._neg_view(torch.ones(N, L, 1))
+    Op.apply(x).backward(up)
+    _, neg, dy = got.pop()
+    assert neg and not dy.is_neg() and torch.equal(dy, -torch.ones(N, L, 1))
