@@ -112,6 +112,11 @@ def _rows(t):
     return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
 
 
+def _written(*ts):
+    """Tensors of one channel with lazy negations written out (imaginary parts of conjugates; wider ones have gaps and are copied)."""
+    return tuple(t.resolve_neg() if isinstance(t, _Tensor) else t for t in ts)
+
+
 def _flat(t, d):
     """[..., d] as rows: a tensor that holds them, their stride, their number."""
     if t.is_contiguous():
@@ -241,6 +246,8 @@ def layer_norm(x, weight=None, bias=None, eps: float = 1e-5):
         raise ValueError(f"layer_norm: x must be [..., d] with 1 <= d <= {_nat.BOA_LAYER_NORM_MAX_D} (got {list(x.shape)})")
     if not eps >= 0.0:
         raise ValueError(f"layer_norm: eps must not be negative (got {eps})")
+    if x.shape[-1] == 1:
+        weight, bias = _written(weight, bias)
     w = _param("layer_norm", "weight", weight, x.shape[-1:], x)
     b = _param("layer_norm", "bias", bias, x.shape[-1:], x)
     _gpu("layer_norm", x)
@@ -357,11 +364,13 @@ def _conv_args(who, x, ndim, weight, bias):
         raise ValueError(f"{who}: x must be {'[batch, length, channels]' if ndim == 3 else '[batch, channels]'} "
                          f"(got {list(x.shape)})")
     c = x.shape[-1]
+    if c == 1:
+        x, bias = _written(x, bias)
     flat = isinstance(weight, torch.Tensor) and weight.ndim == 2
     w = _param(who, "weight", weight, (c, D_CONV) if flat else (c, 1, D_CONV), x)
     if w is None:
         raise TypeError(f"{who}: weight must be a float32 tensor")
-    return w, _param(who, "bias", bias, (c,), x)
+    return x, w, _param(who, "bias", bias, (c,), x)
 
 
 def causal_conv(x, weight, bias=None, *, silu: bool = True, state=None, lens=None, return_state: bool = False):
@@ -371,7 +380,7 @@ def causal_conv(x, weight, bias=None, *, silu: bool = True, state=None, lens=Non
     float32 [channels]; state: the three positions before the first one (zeros without).  Returns y, with ``return_state``
     also the state behind each sequence's last position, as a new tensor."""
     _plain("causal_conv", x, weight, bias, state)
-    w, b = _conv_args("causal_conv", x, 3, weight, bias)
+    x, w, b = _conv_args("causal_conv", x, 3, weight, bias)
     n, length, c = x.shape
     state = _state("causal_conv", state, (n, D_CONV - 1, c), x, x.dtype, False)
     lens = _lens("causal_conv", lens, n, length, x)
@@ -389,7 +398,7 @@ def causal_conv_step(x, state, weight, bias=None, *, silu: bool = True):
     Returns y [batch, channels]; no gradient."""
     who = "causal_conv_step"
     _plain(who, x, state, weight, bias)
-    w, b = _conv_args(who, x, 2, weight, bias)
+    x, w, b = _conv_args(who, x, 2, weight, bias)
     n, c = x.shape
     if state is None:
         raise TypeError(f"{who}: state must be a tensor")
@@ -491,6 +500,8 @@ def _scan_args(who, ndim, u, delta, A, B, C, D, z, bias):
                          f"(got {list(u.shape)})")
     dtype, shape, dev = u.dtype, u.shape, u.get_device()
     c = shape[-1]
+    if c == 1:
+        u, delta, z, D, bias = _written(u, delta, z, D, bias)
     states = shape[:-1] + (D_STATE,)
     if not _is(delta, dtype, shape, dev):
         _act(who, "delta", delta, shape, u)

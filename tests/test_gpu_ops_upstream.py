@@ -25,3 +25,37 @@ def test_zeros_without_memory_and_negations(gpu):
         want = torch.autograd.grad(call(), leaves, -up)
         got = torch.autograd.grad(call(), leaves, torch._neg_view(up))
         assert all(torch.equal(p, q) for p, q in zip(got, want)) and any(v.any() for v in want)
+
+
+def test_one_channel_of_conjugates(gpu):
+    """Imaginary parts of conjugates are negated where they are read; with one channel their rows count as contiguous."""
+    from boa_amd import ops
+
+    g = _gen(2)
+
+    def imag(*shape):
+        v = torch.complex(_randn(g, *shape), _randn(g, *shape)).conj().imag
+        assert v.is_neg()
+        return v
+
+    x, w, b = imag(2, 30)[..., None], _randn(g, 1, 4), imag(1)
+    state, up = _randn(g, 2, 3, 1), _randn(g, 2, 30, 1)
+    s = {**_scan_inputs(g, 2, 30, 1, torch.float32), "u": x, "delta": imag(2, 30)[..., None], "z": imag(2, 30)[..., None], "D": b,
+         "delta_bias": imag(1)}
+    assert x.is_neg() and ops._rows(x) is x
+    written = lambda t: t.resolve_neg().clone()  # noqa: E731
+
+    def passes(f):
+        x1, b1, s1 = f(x).requires_grad_(), f(b).requires_grad_(), {k: f(v).requires_grad_() for k, v in s.items()}
+        y = ops.causal_conv(x1, w, b1)
+        z = ops.selective_scan(**s1)
+        n = ops.layer_norm(x1, None, b1)
+        out = [y, z, n, *torch.autograd.grad(y, (x1, b1), up), *torch.autograd.grad(z, tuple(s1.values()), up),
+               *torch.autograd.grad(n, (b1,), up)]
+        with torch.no_grad():
+            st, h = state.clone(), torch.zeros(2, 16, 1, device="cuda")
+            at = {k: v[:, 0] if k in ("u", "delta", "B", "C", "z") else v for k, v in s1.items()}
+            out += [ops.causal_conv_step(x1[:, 0], st, w, b1), st, ops.selective_scan_step(**at, state=h), h]
+        return out
+
+    assert all(torch.equal(p, q) for p, q in zip(passes(lambda t: t.detach()), passes(lambda t: written(t.detach()))))
