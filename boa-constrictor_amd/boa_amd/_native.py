@@ -34,6 +34,8 @@ BOA_CROSS_ENTROPY_MAX_V = 4096
 BOA_OPS_MAX_CHANNELS = 65536
 BOA_SCAN_MARK = 8
 BOA_SCAN_MAX_ROW_STRIDE = 67108863
+BOA_SAMPLE_MAX_V = 4096
+BOA_ATTENTION_MAX_KEY, BOA_ATTENTION_MAX_VALUE, BOA_ATTENTION_MAX_HEADS = 128, 512, 4096
 
 
 class BoaError(RuntimeError):
@@ -74,6 +76,7 @@ _I32 = ctypes.c_int32
 _I64 = ctypes.c_int64
 _U64 = ctypes.c_uint64
 _F32 = ctypes.c_float
+_F64 = ctypes.c_double
 SIGNATURES = [
     ("boa_last_error", ctypes.c_char_p, []),
     ("boa_abi_version", ctypes.c_int, []),
@@ -122,6 +125,16 @@ SIGNATURES = [
     ("boa_selective_scan_fwd", ctypes.c_int, [ctypes.c_char_p, _P, _I64, _P]),
     ("boa_selective_scan_bwd", ctypes.c_int, [ctypes.c_char_p, _P, _I64, _P]),
     ("boa_selective_scan_step", ctypes.c_int, [ctypes.c_char_p, _P]),
+    # and boa_attention (ops._ATTENTION)
+    ("boa_linear_attention_work_bytes", _I64, [ctypes.c_char_p, _INT]),
+    ("boa_linear_attention_fwd", ctypes.c_int, [ctypes.c_char_p, _P, _I64, _P]),
+    ("boa_linear_attention_bwd", ctypes.c_int, [ctypes.c_char_p, _P, _I64, _P, _I64, _P]),
+    ("boa_linear_attention_step", ctypes.c_int, [ctypes.c_char_p, _P]),
+    # grads, counts and dtypes as the bytes of arrays
+    ("boa_grad_norm_work_bytes", _I64, [_I32]),
+    ("boa_grad_norm", ctypes.c_int, [_I32, ctypes.c_char_p, ctypes.c_char_p, ctypes.c_char_p, _INT, _P, _P, _I64, _P]),
+    ("boa_clip_grads", ctypes.c_int, [_I32, ctypes.c_char_p, ctypes.c_char_p, ctypes.c_char_p, _INT, _F64, _P, _P, _I64, _P]),
+    ("boa_sample", ctypes.c_int, [_INT, _P, _I64, _I64, _I32, _P, _F64, _P, _I32, _P, _F64, _P, _F64, _P, _P, _P]),
 ]
 
 _lib = None
@@ -137,8 +150,8 @@ def _bind(lib):
 
 
 # The C ABI these signatures describe (boa_abi_version); 2: boa_decompress takes the payload's length; 3: the operators of
-# training.
-ABI_VERSION = 3
+# training; 4: linear attention, gradient norm, sampling.
+ABI_VERSION = 4
 
 
 def load_cdll():

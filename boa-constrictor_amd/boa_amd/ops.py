@@ -26,7 +26,9 @@ passes on the capture's side stream and let go of any eager graph of the same pa
 """
 from __future__ import annotations
 
+import array
 import functools
+import math
 import struct
 
 import torch
@@ -36,7 +38,7 @@ from torch.autograd.graph import increment_version
 from boa_amd import _native as _nat
 
 __all__ = ["layer_norm", "causal_conv", "causal_conv_step", "selective_scan", "selective_scan_step", "cross_entropy",
-           "D_STATE", "D_CONV"]
+           "linear_attention", "linear_attention_step", "grad_norm", "clip_grad_norm_", "sample", "D_STATE", "D_CONV"]
 
 D_STATE, D_CONV = 16, 4
 _DTYPES = {torch.float32: _nat.BOA_DT_F32, torch.bfloat16: _nat.BOA_DT_BF16, torch.float16: _nat.BOA_DT_F16}
@@ -565,3 +567,269 @@ def selective_scan_step(u, delta, A, B, C, D=None, z=None, delta_bias=None, *, s
     _call(u, _nat.lib().boa_selective_scan_step, packed)
     increment_version(state)
     return y
+
+
+# ---- linear attention ------------------------------------------------------------------------------
+# boa_attention (include/boa_hip.h): dtype, heads, groups, key, value, decay_per_head, scale, unused; batch, length; q, k, v, y
+# (pointer, three strides); decay and its strides; lens, state_in, state_out; dy, dq, dk, dv; ddecay
+_ATTENTION = struct.Struct("@6ifi2q16q4q3q16qq")
+_NO_HEADS = (0, 0, 0, 0)
+
+
+def _r4(t):
+    return _NO_HEADS if t is None else (t.data_ptr(), *t.stride()[:-1])
+
+
+def _pack_attention(q, k, v, g, scale, lens, state_in, state_out, y, back=(None,) * 4, dg=None):
+    n, length, groups, key = q.shape
+    gs = (0, 0, 1) if g.ndim == 1 else g.stride()
+    return _ATTENTION.pack(_DTYPES[q.dtype], v.shape[2], groups, key, v.shape[3], g.ndim == 1, scale, 0, n, length, *_r4(q), *_r4(k),
+                           *_r4(v), *_r4(y), g.data_ptr(), *gs, _ptr(lens), _ptr(state_in), _ptr(state_out), *_r4(back[0]),
+                           *_r4(back[1]), *_r4(back[2]), *_r4(back[3]), _ptr(dg))
+
+
+def _attention_fwd(q, k, v, g, scale, state, lens, want_state):
+    n, length, heads, value = v.shape
+    y = v.new_empty((n, length, heads, value))
+    out = g.new_empty((n, heads, q.shape[3], value)) if want_state else None
+    args = _pack_attention(q, k, v, g, scale, lens, state, out, y)
+    lib = _nat.lib()
+    size = lib.boa_linear_attention_work_bytes(args, 0)
+    work = _work(size, q)
+    _call(q, lib.boa_linear_attention_fwd, args, _ptr(work), size)
+    return y, out, work
+
+
+class _LinearAttention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, g, scale, state, lens, want_state):
+        y, out, work = _attention_fwd(q, k, v, g, scale, state, lens, want_state)
+        ctx.save_for_backward(q, k, v, g, lens, work)  # the states before the chunks are in the workspace
+        ctx.scale = scale
+        if out is not None:
+            ctx.mark_non_differentiable(out)
+        return y, out
+
+    @staticmethod
+    def backward(ctx, dy, _):
+        dy = _once("linear_attention", dy)
+        q, k, v, g, lens, fwd = ctx.saved_tensors
+        dy = _rows(dy)
+        dq, dk, dv, dg = (t.new_empty(t.shape) for t in (q, k, v, g))
+        args = _pack_attention(q, k, v, g, ctx.scale, lens, None, None, None, (dy, dq, dk, dv), dg)
+        lib = _nat.lib()
+        size = lib.boa_linear_attention_work_bytes(args, 1)
+        work = _work(size, q)
+        _call(q, lib.boa_linear_attention_bwd, args, _ptr(fwd), 0 if fwd is None else fwd.numel(), _ptr(work), size)
+        return dq, dk, dv, dg, None, None, None, None
+
+
+def _attention_args(who, ndim, q, k, v, g, scale):
+    _act(who, "q", q)
+    lead = "batch, length" if ndim == 4 else "batch"
+    if q.ndim != ndim or not 1 <= q.shape[-1] <= _nat.BOA_ATTENTION_MAX_KEY or not q.shape[-2]:
+        raise ValueError(f"{who}: q must be [{lead}, groups, key] with 1 <= key <= {_nat.BOA_ATTENTION_MAX_KEY} (got {list(q.shape)})")
+    dev = q.get_device()
+    if not _is(k, q.dtype, q.shape, dev):
+        _act(who, "k", k, q.shape, q)
+    _act(who, "v", v, None, q)
+    if v.ndim != ndim or v.shape[:-2] != q.shape[:-2] or not 1 <= v.shape[-1] <= _nat.BOA_ATTENTION_MAX_VALUE:
+        raise ValueError(f"{who}: v must be [{lead}, heads, value] with 1 <= value <= {_nat.BOA_ATTENTION_MAX_VALUE}, {lead} as q's "
+                         f"(got {list(v.shape)} and {list(q.shape)})")
+    heads = v.shape[-2]
+    if not 1 <= heads <= _nat.BOA_ATTENTION_MAX_HEADS or heads % q.shape[-2]:
+        raise ValueError(f"{who}: the heads of v must be a multiple of q's and k's, at most {_nat.BOA_ATTENTION_MAX_HEADS} "
+                         f"(got {heads} and {q.shape[-2]})")
+    if not isinstance(g, _Tensor) or g.dtype is not _F32:
+        raise TypeError(f"{who}: log_decay must be a float32 tensor")
+    if g.get_device() != dev or (g.shape != (heads,) and g.shape != v.shape[:-1]):
+        raise ValueError(f"{who}: log_decay must be [{heads}] or {list(v.shape[:-1])} on {q.device} (got {list(g.shape)} on {g.device})")
+    if g.ndim == 1 and g.stride(0) != 1:
+        g = g.contiguous()
+    if q.shape[-1] == 1:
+        q, k = _written(q, k)
+    if v.shape[-1] == 1:
+        v, = _written(v)
+    g, = _written(g)
+    scale = q.shape[-1] ** -0.5 if scale is None else float(scale)
+    return _rows(q), _rows(k), _rows(v), g, scale
+
+
+def linear_attention(q, k, v, log_decay, *, scale=None, state=None, lens=None, return_state: bool = False):
+    """``S = exp(log_decay) S + k v^T``, ``y = scale S^T q`` along the positions: a state of key x value values per head, which
+    ``selective_scan`` would have as 16 per channel with a decay each.
+
+    q, k: [batch, length, groups, key] (1 to 128), each group shared by heads / groups consecutive heads; v: [batch, length, heads,
+    value] (1 to 512); log_decay: float32 [heads], or [batch, length, heads] for one of each position's own, 0 or negative (-inf
+    forgets everything before); scale: 1 / sqrt(key) unless given.  state: float32 [batch, heads, key, value] before the first
+    position (zeros without).  Returns y [batch, length, heads, value], with ``return_state`` also the state behind each
+    sequence's last position, as a new tensor."""
+    who = "linear_attention"
+    _plain(who, q, k, v, log_decay, state)
+    q, k, v, g, scale = _attention_args(who, 4, q, k, v, log_decay, scale)
+    n, length, heads, value = v.shape
+    state = _state(who, state, (n, heads, q.shape[-1], value), q, torch.float32, False)
+    lens = _lens(who, lens, n, length, q)
+    _gpu(who, q)
+    if _grad(q, k, v, g):
+        y, out = _LinearAttention.apply(q, k, v, g, scale, state, lens, bool(return_state))
+    else:
+        y, out, _ = _attention_fwd(q, k, v, g, scale, state, lens, return_state)
+    return (y, out) if return_state else y
+
+
+def linear_attention_step(q, k, v, log_decay, *, state, scale=None):
+    """``linear_attention`` of one position per sequence: q, k [batch, groups, key], v [batch, heads, value], log_decay [heads] or
+    [batch, heads]; state [batch, heads, key, value] is advanced in place.  Returns y [batch, heads, value]; no gradient."""
+    who = "linear_attention_step"
+    _plain(who, q, k, v, log_decay, state)
+    q, k, v, g, scale = _attention_args(who, 3, q, k, v, log_decay, scale)
+    n, heads, value = v.shape
+    key = q.shape[-1]
+    if state is None:
+        raise TypeError(f"{who}: state must be a tensor")
+    state = _state(who, state, (n, heads, key, value), q, torch.float32, True)
+    if _grad(q, k, v, g):
+        raise ValueError(f"{who}: no gradient; call it under torch.no_grad()")
+    _gpu(who, q)
+    y = v.new_empty((n, heads, value))
+    per_head = g.ndim == 1
+    packed = _ATTENTION.pack(_DTYPES[q.dtype], heads, q.shape[1], key, value, per_head, scale, 0, n, 1, q.data_ptr(), q.stride(0), 0,
+                             q.stride(1), k.data_ptr(), k.stride(0), 0, k.stride(1), v.data_ptr(), v.stride(0), 0, v.stride(1),
+                             y.data_ptr(), heads * value, 0, value, g.data_ptr(), 0 if per_head else g.stride(0), 0,
+                             1 if per_head else g.stride(1), 0, 0, state.data_ptr(), *(_NO_HEADS * 4), 0)
+    _call(q, _nat.lib().boa_linear_attention_step, packed)
+    increment_version(state)
+    return y
+
+
+# ---- gradient norm ---------------------------------------------------------------------------------
+def _grads(who, parameters):
+    """The gradients of parameters (those that have one), and their addresses, sizes and types as the bytes of C arrays."""
+    if isinstance(parameters, _Tensor):
+        parameters = (parameters,)
+    grads = [g for g in [p.grad for p in parameters] if g is not None]
+    if not grads:
+        return grads, None
+    _plain(who, *grads)
+    dev = grads[0].device
+    for g in grads:
+        if g.dtype not in _DTYPES or g.layout is not torch.strided:
+            raise TypeError(f"{who}: gradients must be dense float32, bfloat16 or float16 (got {g.layout}, {g.dtype})")
+        if g.device != dev:
+            raise ValueError(f"{who}: the gradients must be on one device (got {dev} and {g.device})")
+    _gpu(who, grads[0])
+    return grads, dev
+
+
+def _arrays(grads):
+    return (array.array("q", [_ptr(g) for g in grads]).tobytes(), array.array("q", [g.numel() for g in grads]).tobytes(),
+            array.array("i", [_DTYPES[g.dtype] for g in grads]).tobytes())
+
+
+def _norm_type(who, norm_type):
+    if norm_type not in (2, math.inf):
+        raise ValueError(f"{who}: norm_type must be 2 or inf (got {norm_type})")
+    return norm_type != 2
+
+
+def grad_norm(parameters, *, norm_type: float = 2.0):
+    """The norm of the gradients of all parameters together, as if they were one vector: 2-norm, or (inf) the largest magnitude.
+
+    parameters: a tensor or an iterable of them; those without a gradient count for nothing.  Gradients may be float32, bfloat16
+    and float16 in one call, on one device.  Returns float32 on it, without waiting for it."""
+    who = "grad_norm"
+    largest = _norm_type(who, norm_type)
+    grads, dev = _grads(who, parameters)
+    if not grads:
+        return torch.zeros(())
+    grads = [g if g.is_contiguous() else g.contiguous() for g in grads if not g._is_zerotensor()]
+    lib, n = _nat.lib(), len(grads)
+    size = lib.boa_grad_norm_work_bytes(n)
+    norm, work = torch.empty((), dtype=torch.float32, device=dev), torch.empty(size, dtype=torch.uint8, device=dev)
+    _call(norm, lib.boa_grad_norm, n, *_arrays(grads), largest, norm.data_ptr(), work.data_ptr(), size)
+    return norm
+
+
+def clip_grad_norm_(parameters, max_norm: float, *, norm_type: float = 2.0):
+    """Scales the gradients of all parameters in place by ``min(1, max_norm / (norm + 1e-6))``, ``norm`` theirs together, between
+    ``loss.backward()`` and the optimizer's step.  Returns the norm that they had (``grad_norm``).
+
+    The call waits for nothing, so a norm that is no number makes the gradients so too (an infinite one makes them zeros, and NaN
+    where they were infinite)."""
+    who = "clip_grad_norm_"
+    largest = _norm_type(who, norm_type)
+    max_norm = float(max_norm)
+    if not max_norm >= 0.0:
+        raise ValueError(f"{who}: max_norm must not be negative (got {max_norm})")
+    all_grads, dev = _grads(who, parameters)
+    if not all_grads:
+        return torch.zeros(())
+    grads, copies = [], []
+    for g in all_grads:
+        if g.is_contiguous():
+            if not g._is_zerotensor():
+                grads.append(g)
+        else:
+            if any(s == 0 and n > 1 for s, n in zip(g.stride(), g.shape)):
+                raise ValueError(f"{who}: a gradient whose values share memory (strides {g.stride()}) cannot be scaled in place")
+            grads.append(g.contiguous())
+            copies.append((g, grads[-1]))
+    lib, n = _nat.lib(), len(grads)
+    size = lib.boa_grad_norm_work_bytes(n)
+    norm, work = torch.empty((), dtype=torch.float32, device=dev), torch.empty(size, dtype=torch.uint8, device=dev)
+    _call(norm, lib.boa_clip_grads, n, *_arrays(grads), largest, max_norm, norm.data_ptr(), work.data_ptr(), size)
+    with torch.no_grad():
+        for g, scaled in copies:
+            g.copy_(scaled)
+    increment_version(grads)
+    return norm
+
+
+# ---- drawing symbols -------------------------------------------------------------------------------
+def _limit(who, name, v, shape, like, dtype, lo, hi):
+    """A limit of all rows as a number, or one of each row as a contiguous tensor: (number, tensor)."""
+    if not isinstance(v, _Tensor):
+        if not lo <= v <= hi:
+            raise ValueError(f"{who}: {name} must be {lo} to {hi} (got {v})")
+        return v, None
+    if v.dtype is not dtype:
+        raise TypeError(f"{who}: {name} must be a number or a {dtype} tensor (got {v.dtype})")
+    if v.shape != shape or v.get_device() != like.get_device():
+        raise ValueError(f"{who}: {name} must be a number or {list(shape)} on {like.device} (got {list(v.shape)} on {v.device})")
+    return 0, v.resolve_neg().contiguous()
+
+
+def sample(logits, u, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+    """Symbols drawn from logits [..., V] (1 to 4096 symbols) by given random numbers u, float32 of the leading shape in [0, 1).
+
+    The weights are exp((x - max) / temperature).  Of all symbols the top_k likeliest are kept (0: all), of those the fewest
+    likeliest whose weights sum to top_p of theirs, of those the ones with at least min_p of the likeliest one's weight; equal
+    logits count in the symbols' order.  Returns, int64 of the leading shape, the first symbol up to and with which the kept
+    weights sum to more than u of them all: the same numbers draw the same symbols.  Temperature 0 takes the likeliest symbol.
+    Each limit is a number, or a tensor of the leading shape (float32; top_k int32, where 0 or less keeps all).  A row that is no
+    distribution (a NaN in it or its numbers, nothing above -inf) gives -1.  No gradient."""
+    who = "sample"
+    _plain(who, logits, u)
+    _act(who, "logits", logits)
+    if logits.ndim < 1 or not 1 <= logits.shape[-1] <= _nat.BOA_SAMPLE_MAX_V:
+        raise ValueError(f"{who}: logits must be [..., V] with 1 <= V <= {_nat.BOA_SAMPLE_MAX_V} (got {list(logits.shape)})")
+    shape = logits.shape[:-1]
+    if not isinstance(u, _Tensor) or u.dtype is not _F32:
+        raise TypeError(f"{who}: u must be a float32 tensor")
+    if u.shape != shape or u.get_device() != logits.get_device():
+        raise ValueError(f"{who}: u must be {list(shape)} on {logits.device} (got {list(u.shape)} on {u.device})")
+    t, ts = _limit(who, "temperature", temperature, shape, logits, _F32, 0.0, math.inf)
+    k, ks = _limit(who, "top_k", top_k, shape, logits, torch.int32, 0, 0x7FFFFFFF)
+    p, ps = _limit(who, "top_p", top_p, shape, logits, _F32, 0.0, 1.0)
+    m, ms = _limit(who, "min_p", min_p, shape, logits, _F32, 0.0, 1.0)
+    _gpu(who, logits)
+    v = logits.shape[-1]
+    if v == 1:
+        logits, = _written(logits)
+    rows, stride, n = _flat(logits, v)
+    u = u.resolve_neg().contiguous()
+    out = torch.empty(shape, dtype=torch.int64, device=logits.device)
+    _call(logits, _nat.lib().boa_sample, _DTYPES[logits.dtype], rows.data_ptr(), stride, n, v, _ptr(u), t, _ptr(ts), k, _ptr(ks), p,
+          _ptr(ps), m, _ptr(ms), out.data_ptr())
+    return out

@@ -355,6 +355,10 @@ class BoaBytePredictor(nn.Module):
 
         lens: lengths of the sequences in a padded batch.  caches: states of ``init_caches`` that the bytes continue and that
         are advanced in place (truncated back-propagation, or streaming without an engine)."""
+        return self.head(self._hidden(x, lens, caches))
+
+    def _hidden(self, x, lens=None, caches=None):
+        """What the blocks make of bytes x [B, L], before the head."""
         if x.ndim != 2:
             raise ValueError(f"x must be [batch, length] (got {list(x.shape)})")
         self._check_caches(caches)
@@ -364,7 +368,7 @@ class BoaBytePredictor(nn.Module):
         h = self._embed(x)
         for i, block in enumerate(self.blocks):
             h = block(h, lens, None if caches is None else caches[i])
-        return self.head(h)
+        return h
 
     def loss(self, x, lens=None):
         """Mean cross entropy in nats per coded byte of x [B, L]: bytes 1 .. L - 1 of each row, up to its length, under the
@@ -390,6 +394,34 @@ class BoaBytePredictor(nn.Module):
         for block, cache in zip(self.blocks, caches):
             h = block.step(h, cache)
         return self.head(h)
+
+    @_no_grad
+    def generate(self, x, steps: int, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, u=None, generator=None):
+        """Bytes that the model, with its parameters as they are now, goes on with behind prompts x [B, L >= 1]: int64 [B, steps].
+
+        Each is drawn by ``ops.sample`` (temperature, top_k, top_p, min_p: numbers, or one per prompt) from the prediction
+        behind those before it, by the numbers u, float32 [steps, B] in [0, 1), or by ``generator``'s.  The same numbers
+        give the same bytes.  Where the logits hold a NaN the byte is -1, and so are those behind it."""
+        if x.ndim != 2 or x.shape[1] < 1:
+            raise ValueError(f"x must be [batch, length >= 1] (got {list(x.shape)})")
+        if steps < 0:
+            raise ValueError(f"steps must not be negative (got {steps})")
+        n, dev = x.shape[0], self.embedding.weight.device
+        if u is None:
+            u = torch.rand((steps, n), generator=generator, device=dev)
+        elif u.shape != (steps, n):
+            raise ValueError(f"u must be {[steps, n]} (got {list(u.shape)})")
+        out = torch.empty((n, steps), dtype=torch.int64, device=dev)
+        if steps == 0:
+            return out
+        mixed = torch.is_autocast_enabled("cuda")
+        caches = self.init_caches(n, torch.get_autocast_dtype("cuda") if mixed else torch.float32)
+        logits = self.head(self._hidden(x, caches=caches)[:, -1])
+        for i in range(steps):
+            out[:, i] = ops.sample(logits, u[i], temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p)
+            if i + 1 < steps:
+                logits = self.train_step(out[:, i], caches)
+        return out
 
     def _check_caches(self, caches):
         if caches is not None and len(caches) != len(self.blocks):

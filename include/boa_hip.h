@@ -30,7 +30,8 @@ extern "C" {
 
 /* Library identity and last error (replaces the reference's exit(1) on CUDA errors, gemm_gpu.hpp:36-43). */
 const char* boa_last_error(void);
-int boa_abi_version(void);  /* 3 (2: boa_decompress takes the payload length; 3: the operators of training) */
+int boa_abi_version(void);  /* 4 (2: boa_decompress takes the payload length; 3: the operators of training; 4: linear
+                               attention, gradient norm, sampling) */
 /* Reports whether d_ptr is device memory of the HIP runtime this library is bound to (1 yes, 0 no). */
 int boa_is_device_pointer(const void* d_ptr);
 
@@ -302,6 +303,64 @@ int boa_selective_scan_bwd(const boa_scan* s, void* d_work, int64_t work_bytes, 
 /* One position per sequence (length 1): advances state_out in place (lens, state_in and marks are not used).  `a` begins at
  * a multiple of 16 bytes.                                                                                */
 int boa_selective_scan_step(const boa_scan* s, void* stream);
+
+/* Linear attention with a decay for each head: a state of `key` x `value` values per head and sequence,
+ *   S_t = e^(decay_t) S_(t-1) + k_t v_t^T, y_t = scale S_t^T q_t
+ * The sibling of the selective scan for states that share one decay, whose products then run on the matrix cores.  q and k have
+ * `groups` heads, each shared by heads / groups consecutive heads of v.  Members that a call does not use are ignored; those
+ * marked * may have a null pointer.                                                                     */
+#define BOA_ATTENTION_MAX_KEY 128
+#define BOA_ATTENTION_MAX_VALUE 512
+#define BOA_ATTENTION_MAX_HEADS 4096
+typedef struct boa_heads {
+    void* p;
+    int64_t batch_stride, row_stride, head_stride;  /* elements */
+} boa_heads;
+typedef struct boa_attention {
+    int32_t dtype;                          /* of q, k, v, y, dy and their gradients                     */
+    int32_t heads, groups, key, value;
+    int32_t decay_per_head;                 /* decay is [heads], the same at all positions               */
+    float scale;
+    int32_t unused;
+    int64_t batch, length;
+    boa_heads q, k, v, y;                   /* [batch][length][groups][key] (q, k), [batch][length][heads][value] */
+    const float* decay;                     /* log of the decay: [batch][length][heads] or [heads]       */
+    int64_t decay_batch_stride, decay_row_stride, decay_head_stride;
+    const int32_t* lens;                    /* * [batch]                                                 */
+    const float* state_in;                  /* * [batch][heads][key][value] before the first position (zeros) */
+    float* state_out;                       /* * the same behind each sequence's last position, another buffer */
+    boa_heads dy, dq, dk, dv;               /* backward                                                  */
+    float* ddecay;                          /* backward: [batch][length][heads] or [heads]               */
+} boa_attention;
+/* Bytes of d_work, at a multiple of 16, that boa_linear_attention_fwd (backward = 0) or _bwd (1) needs for these sizes. */
+int64_t boa_linear_attention_work_bytes(const boa_attention* s, int backward);
+int boa_linear_attention_fwd(const boa_attention* s, void* d_work, int64_t work_bytes, void* stream);
+/* The gradient for everything but the state.  Takes the forward's inputs and its workspace as it left it. */
+int boa_linear_attention_bwd(const boa_attention* s, const void* d_fwd_work, int64_t fwd_work_bytes, void* d_work,
+                             int64_t work_bytes, void* stream);
+/* One position per sequence (length 1): advances state_out in place (lens and state_in are not used).    */
+int boa_linear_attention_step(const boa_attention* s, void* stream);
+
+/* The norm of n gradients together: sqrt of the sum of all squares, or (largest) the largest magnitude, float32 at d_norm; sums are
+ * in 64 bits.  grads, counts (values) and dtypes are host arrays; a gradient's values are contiguous.  Two launches for up to 180
+ * tensors; d_work (boa_grad_norm_work_bytes) at a multiple of 8.                                         */
+int64_t boa_grad_norm_work_bytes(int32_t n);
+int boa_grad_norm(int32_t n, const void* const* d_grads, const int64_t* counts, const int32_t* dtypes, int largest,
+                  float* d_norm, void* d_work, int64_t work_bytes, void* stream);
+/* The same, and every gradient times min(1, max_norm / (norm + 1e-6)) in place.  No two of them may share memory. */
+int boa_clip_grads(int32_t n, void* const* d_grads, const int64_t* counts, const int32_t* dtypes, int largest, double max_norm,
+                   float* d_norm, void* d_work, int64_t work_bytes, void* stream);
+
+/* Symbols drawn from rows of V logits by a number each (d_u float32 [rows], in [0, 1)): weights e^((x - max) / temperature), of
+ * which are kept the top_k largest (0 or less: all), of those the fewest largest whose sum is at least top_p of theirs, of those
+ * whoever has at least min_p of the largest one's; d_out int64 [rows] receives the first symbol up to and with which the weights
+ * sum to more than u of all.  Among equal logits the lower symbol counts as larger.  Temperature 0 takes the largest.  Each limit
+ * is one value, or one per row by a pointer (float32, int32 [rows]).  A row that is no distribution (a NaN in it or in
+ * its numbers, or nothing above -inf) gives -1.  1 <= V <= BOA_SAMPLE_MAX_V.                              */
+#define BOA_SAMPLE_MAX_V 4096
+int boa_sample(int dtype, const void* d_x, int64_t x_stride, int64_t rows, int32_t V, const float* d_u, double temperature,
+               const float* d_temperature, int32_t top_k, const int32_t* d_top_k, double top_p, const float* d_top_p,
+               double min_p, const float* d_min_p, int64_t* d_out, void* stream);
 
 #ifdef __cplusplus
 }
