@@ -4,10 +4,12 @@
 //   theirs; of those whoever has at least min_p of the largest; drawn: the first i, in the symbols' order, with w_0 + ... + w_i > u sum(w)
 //   Among equals the lower index counts as larger.  Temperature 0 takes the largest.
 //
-// Weights and sums are in 64 bits, so that which symbol a number falls on does not hang on the order in which 32-bit sums are
-// rounded.  A row is held in registers by one wavefront, or by four for more than 1024 symbols.  Nothing is sorted: the key of the
-// last symbol that a limit keeps is found bit by bit, by counting (or adding the weights of) the keys above, with the logits as
-// unsigned integers of the same order.
+// Weights and the sums that decide are in 64 bits, so that which symbol a number falls on does not hang on the order in which 32-bit
+// sums are rounded.  A row is held in registers by one wavefront, or by four for more than 1024 symbols.  Nothing is sorted: the
+// key of the last symbol that a limit keeps is found bit by bit, by counting (or adding the weights of) the keys above, with the
+// logits as unsigned integers of the same order, until one symbol is left that it can be.  The weights are added in 32 bits
+// there; whether the symbol found is the one is decided by two sums in 64, and where it is not (a border within 32 bits'
+// rounding) the search is done again with those.
 #include "ops_common.h"
 
 #include "../../include/boa_hip.h"
@@ -30,6 +32,49 @@ struct Args {
     int64_t* out;
 };
 
+// Inclusive sum over the lanes before, by permutations in registers: inside rows of 16, then from the rows before.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double from_before(double v) {
+    const u32x2 w = __builtin_bit_cast(u32x2, v);
+    const u32x2 r = {(uint32_t)__builtin_amdgcn_update_dpp(0, (int)w[0], CTRL, ROWS, 0xF, false),
+                     (uint32_t)__builtin_amdgcn_update_dpp(0, (int)w[1], CTRL, ROWS, 0xF, false)};
+    return __builtin_bit_cast(double, r);
+}
+template <int CTRL, int ROWS>
+__device__ __forceinline__ float from_before(float v) {
+    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, ROWS, 0xF, false));
+}
+constexpr int DPP_SHR1 = 0x111, DPP_SHR2 = 0x112, DPP_SHR4 = 0x114, DPP_SHR8 = 0x118, DPP_BCAST15 = 0x142, DPP_BCAST31 = 0x143;
+template <class T>
+__device__ __forceinline__ T scan(T v) {
+    v += from_before<DPP_SHR1, 0xF>(v);
+    v += from_before<DPP_SHR2, 0xF>(v);
+    v += from_before<DPP_SHR4, 0xF>(v);
+    v += from_before<DPP_SHR8, 0xF>(v);
+    v += from_before<DPP_BCAST15, 0xA>(v);
+    return v + from_before<DPP_BCAST31, 0xC>(v);
+}
+__device__ __forceinline__ double last_lane(double v) {
+    const u32x2 w = __builtin_bit_cast(u32x2, v);
+    const u32x2 r = {(uint32_t)__builtin_amdgcn_readlane((int)w[0], 63), (uint32_t)__builtin_amdgcn_readlane((int)w[1], 63)};
+    return __builtin_bit_cast(double, r);
+}
+__device__ __forceinline__ float last_lane(float v) { return from_lane(v, 63); }
+// The largest of all lanes, the same way.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t max_with(uint32_t v) {
+    return max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xF, false));
+}
+__device__ __forceinline__ uint32_t wave_largest(uint32_t v) {
+    v = max_with<DPP_SHR1, 0xF>(v);
+    v = max_with<DPP_SHR2, 0xF>(v);
+    v = max_with<DPP_SHR4, 0xF>(v);
+    v = max_with<DPP_SHR8, 0xF>(v);
+    v = max_with<DPP_BCAST15, 0xA>(v);
+    v = max_with<DPP_BCAST31, 0xC>(v);
+    return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
+}
+
 // Sums over the lanes of a row: of a wavefront, or of four (ROW_WAVES) by way of LDS.
 template <int ROW_WAVES>
 struct Over {
@@ -44,15 +89,15 @@ struct Over {
         __syncthreads();
         return join(join(at[0], at[1]), join(at[2], at[3]));
     }
-    __device__ __forceinline__ double sum(double v) {
-        for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
-        return waves(v, [](double a, double b) { return a + b; });
+    template <class T>
+    __device__ __forceinline__ T sum(T v) {
+        return (T)waves((double)last_lane(scan(v)), [](double a, double b) { return a + b; });
     }
     __device__ __forceinline__ int count(int of_wave) {
         return ROW_WAVES == 1 ? of_wave : (int)waves((double)of_wave, [](double a, double b) { return a + b; });
     }
     __device__ __forceinline__ uint32_t largest(uint32_t v) {
-        for (int o = 32; o > 0; o >>= 1) v = max(v, (uint32_t)__shfl_xor((int)v, o, 64));
+        v = wave_largest(v);
         return ROW_WAVES == 1 ? v : (uint32_t)waves((double)v, [](double a, double b) { return a > b ? a : b; });
     }
     // of the wavefronts before this one, and of all of them
@@ -79,6 +124,7 @@ __device__ __forceinline__ uint32_t key_of(float x) {
     const uint32_t b = __float_as_uint(x + 0.0f);  // -0 is 0
     return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
+__device__ __forceinline__ float value_of(uint32_t key) { return __uint_as_float(key & 0x80000000u ? key & 0x7FFFFFFFu : ~key); }
 constexpr uint32_t KEY_OF_NOTHING = 0x007FFFFFu;  // -inf
 
 template <int DT, int VEC, int N, int ROW_WAVES>
@@ -117,6 +163,26 @@ __global__ void __launch_bounds__(WG) k_sample(const Args a) {
         for (int i = 0; i < PER; ++i) top = max(top, key[i]);
         top = over.largest(top);
         const bool bad = over.count(__popcll(__ballot(nan))) > 0 || top <= KEY_OF_NOTHING || u != u || t != t || p != p || least != least;
+        // The largest key of which `enough` holds, where it holds of all smaller ones: bit by bit, until one symbol is left between the
+        // keys that are known to be enough and those that are not (bits below a 16-bit logit's last are all the same).
+        const auto search = [&](auto enough) {
+            uint32_t last = 0u;
+            int with = a.V, above = 0;  // symbols from `last` on, and from the first key known not to be enough on
+            constexpr int LAST_BIT = DT == DT_F32 ? 0 : DT == DT_BF16 ? 16 : 13;
+            for (int bit = 31; bit >= LAST_BIT && with - above > 1; --bit) {
+                const uint32_t c = last | 1u << bit;
+                int n = 0;
+#pragma unroll
+                for (int i = 0; i < PER; ++i) n += __popcll(__ballot(key[i] >= c));
+                n = over.count(n);
+                if (enough(c, n)) last = c, with = n;
+                else above = n;
+            }
+            uint32_t found = 0u;  // the smallest from there on, as the largest complement
+#pragma unroll
+            for (int i = 0; i < PER; ++i) found = max(found, key[i] >= max(last, 1u) ? ~key[i] : 0u);
+            return ~over.largest(found);
+        };
         // keeps of the symbols with this key the first n, by their index
         const auto keep_first = [&](uint32_t of, int n) {
 #pragma unroll
@@ -147,13 +213,7 @@ __global__ void __launch_bounds__(WG) k_sample(const Args a) {
                 for (int i = 0; i < PER; ++i) key[i] = key[i] == top ? top : 0u;
                 keep_first(top, 1);
             } else if (k > 0 && k < a.V) {
-                uint32_t last = 0u;
-                for (uint32_t bit = 0x80000000u; bit != 0u; bit >>= 1) {
-                    int n = 0;
-#pragma unroll
-                    for (int i = 0; i < PER; ++i) n += __popcll(__ballot(key[i] >= (last | bit)));
-                    if (over.count(n) >= k) last |= bit;
-                }
+                const uint32_t last = search([&](uint32_t, int n) { return n >= k; });
                 int above = 0, with = 0;
 #pragma unroll
                 for (int i = 0; i < PER; ++i) {
@@ -167,43 +227,40 @@ __global__ void __launch_bounds__(WG) k_sample(const Args a) {
             }
         }
         // weights of what is kept
-        const float largest = __uint_as_float(top & 0x80000000u ? top & 0x7FFFFFFFu : ~top);
+        const float largest = value_of(top);
         const double by = t > 0.0 ? 1.0 / t : 1.0;
+        // an infinity is as large as itself, and infinitely far from all others whatever the temperature
+        const auto weight = [&](float x) {
+            const double d = (double)x - (double)largest;
+            return x == largest ? 1.0 : d == -__builtin_huge_val() ? 0.0 : exp(d * by);
+        };
         double w[PER];
 #pragma unroll
-        for (int i = 0; i < PER; ++i) {
-            const double d = (double)v[i] - (double)largest;
-            // an infinity is as large as itself, and infinitely far from all others whatever the temperature
-            const double e = v[i] == largest ? 1.0 : d == -__builtin_huge_val() ? 0.0 : exp(d * by);
-            w[i] = key[i] == 0u || bad ? 0.0 : e;
-        }
+        for (int i = 0; i < PER; ++i) w[i] = key[i] == 0u || bad ? 0.0 : weight(v[i]);
         if (!bad && p > 0.0 && p < 1.0) {
-            double sum = 0.0;
+            const auto from = [&](uint32_t c, auto zero) {
+                auto sum = zero;
 #pragma unroll
-            for (int i = 0; i < PER; ++i) sum += w[i];
-            const double want = p * over.sum(sum);
-            uint32_t last = 0u;
-            for (uint32_t bit = 0x80000000u; bit != 0u; bit >>= 1) {
-                double s = 0.0;
-#pragma unroll
-                for (int i = 0; i < PER; ++i) s += key[i] >= (last | bit) ? w[i] : 0.0;
-                if (over.sum(s) >= want) last |= bit;
+                for (int i = 0; i < PER; ++i) sum += key[i] >= c ? (decltype(zero))w[i] : zero;
+                return over.sum(sum);
+            };
+            const double want = p * from(1u, 0.0);
+            uint32_t last = search([&](uint32_t c, int) { return from(c, 0.0f) >= (float)want; });
+            double above = from(last + 1u, 0.0);
+            if (above >= want || from(last, 0.0) < want) {
+                last = search([&](uint32_t c, int) { return from(c, 0.0) >= want; });
+                above = from(last + 1u, 0.0);
             }
             // of those that are equal to the last as many as it takes
-            double above = 0.0, one = 0.0;
             int equal = 0;
 #pragma unroll
-            for (int i = 0; i < PER; ++i) {
-                above += key[i] > last ? w[i] : 0.0;
-                one = key[i] == last ? w[i] : one;
-                equal += __popcll(__ballot(key[i] == last && last != 0u));
-            }
-            above = over.sum(above);
+            for (int i = 0; i < PER; ++i) equal += __popcll(__ballot(key[i] == last));
             equal = over.count(equal);
-            for (int o = 32; o > 0; o >>= 1) one = fmax(one, __shfl_xor(one, o, 64));
-            one = over.waves(one, [](double x, double y) { return x > y ? x : y; });
             int n = 1;
-            while (n < equal && above + n * one < want) ++n;
+            if (equal > 1) {
+                const double one = weight(value_of(last));
+                while (n < equal && above + n * one < want) ++n;
+            }
 #pragma unroll
             for (int i = 0; i < PER; ++i)
                 if (key[i] < last) key[i] = 0u;
@@ -219,17 +276,11 @@ __global__ void __launch_bounds__(WG) k_sample(const Args a) {
             double s = 0.0;
 #pragma unroll
             for (int j = 0; j < VEC; ++j) s += w[i * VEC + j];
-            double scan = s;
-#pragma unroll
-            for (int o = 1; o < 64; o <<= 1) {
-                const double y = __shfl_up(scan, o, 64);
-                if (lane >= o) scan += y;
-            }
+            const double with = scan(s);
             double total;
-            const double waves_before = over.before(__shfl(scan, 63, 64), total);
-            double lanes_before = __shfl_up(scan, 1, 64);
-            lanes_before = lane == 0 ? 0.0 : lanes_before;
-            upto[i] = all + (waves_before + lanes_before);
+            const double waves_before = over.before(last_lane(with), total);
+            const double lanes_before = __shfl_up(with, 1, 64);
+            upto[i] = all + (waves_before + (lane == 0 ? 0.0 : lanes_before));
             all += total;
         }
         const double at = (double)u * all;
