@@ -26,9 +26,9 @@ passes on the capture's side stream and let go of any eager graph of the same pa
 """
 from __future__ import annotations
 
-import array
 import functools
 import math
+import operator
 import struct
 
 import torch
@@ -704,27 +704,45 @@ def linear_attention_step(q, k, v, log_decay, *, state, scale=None):
 
 
 # ---- gradient norm ---------------------------------------------------------------------------------
-def _grads(who, parameters):
-    """The gradients of parameters (those that have one), and their addresses, sizes and types as the bytes of C arrays."""
+# A model has hundreds of gradients, and each look at one costs Python 70 ns: few looks, without calls of functions of our own.
+_grad_of, _contiguous, _address, _size = operator.attrgetter("grad"), _Tensor.is_contiguous, _Tensor.data_ptr, _Tensor.numel
+
+
+def _grads(who, parameters, in_place):
+    """The gradients of parameters, those that have one and memory for it; their number, addresses, sizes and types as the bytes of C
+    arrays; copies of those that are not contiguous, with the originals; their device."""
     if isinstance(parameters, _Tensor):
         parameters = (parameters,)
-    grads = [g for g in [p.grad for p in parameters] if g is not None]
+    grads = [g for g in map(_grad_of, parameters) if g is not None]
+    copies = []
     if not grads:
-        return grads, None
+        return grads, None, copies, None
     _plain(who, *grads)
+    try:
+        codes = [_DTYPES[g.dtype] for g in grads]
+        at = list(map(_address, grads))
+    except (KeyError, RuntimeError):  # sparse ones have no address
+        raise TypeError(f"{who}: gradients must be dense float32, bfloat16 or float16 "
+                        f"(got {', '.join(sorted({f'{g.layout}, {g.dtype}' for g in grads}))})") from None
     dev = grads[0].device
-    for g in grads:
-        if g.dtype not in _DTYPES or g.layout is not torch.strided:
-            raise TypeError(f"{who}: gradients must be dense float32, bfloat16 or float16 (got {g.layout}, {g.dtype})")
-        if g.device != dev:
-            raise ValueError(f"{who}: the gradients must be on one device (got {dev} and {g.device})")
+    if len(set(map(_Tensor.get_device, grads))) > 1:
+        raise ValueError(f"{who}: the gradients must be on one device (got {', '.join(sorted({str(g.device) for g in grads}))})")
     _gpu(who, grads[0])
-    return grads, dev
-
-
-def _arrays(grads):
-    return (array.array("q", [_ptr(g) for g in grads]).tobytes(), array.array("q", [g.numel() for g in grads]).tobytes(),
-            array.array("i", [_DTYPES[g.dtype] for g in grads]).tobytes())
+    if not all(map(_contiguous, grads)):
+        for i, g in enumerate(grads):
+            if not g.is_contiguous():
+                if in_place and any(s == 0 and n > 1 for s, n in zip(g.stride(), g.shape)):
+                    raise ValueError(f"{who}: a gradient whose values share memory (strides {g.stride()}) cannot be scaled in place")
+                grads[i] = g.contiguous()
+                at[i] = grads[i].data_ptr()
+                copies.append((g, grads[i]))
+    if not all(at):  # empty ones, and zeros that autograd has not written; what stands for others without memory is refused
+        for g in grads:
+            if not g._is_zerotensor():
+                _ptr(g)
+        grads, at, codes = zip(*[x for x in zip(grads, at, codes) if x[1]]) if any(at) else ((), (), ())
+    n = len(grads)
+    return grads, (n, struct.pack(f"{n}q", *at), struct.pack(f"{n}q", *map(_size, grads)), struct.pack(f"{n}i", *codes)), copies, dev
 
 
 def _norm_type(who, norm_type):
@@ -740,14 +758,13 @@ def grad_norm(parameters, *, norm_type: float = 2.0):
     and float16 in one call, on one device.  Returns float32 on it, without waiting for it."""
     who = "grad_norm"
     largest = _norm_type(who, norm_type)
-    grads, dev = _grads(who, parameters)
-    if not grads:
+    grads, arrays, _, dev = _grads(who, parameters, False)
+    if dev is None:
         return torch.zeros(())
-    grads = [g if g.is_contiguous() else g.contiguous() for g in grads if not g._is_zerotensor()]
-    lib, n = _nat.lib(), len(grads)
-    size = lib.boa_grad_norm_work_bytes(n)
+    lib = _nat.lib()
+    size = _bytes("boa_grad_norm_work_bytes", len(grads))
     norm, work = torch.empty((), dtype=torch.float32, device=dev), torch.empty(size, dtype=torch.uint8, device=dev)
-    _call(norm, lib.boa_grad_norm, n, *_arrays(grads), largest, norm.data_ptr(), work.data_ptr(), size)
+    _call(norm, lib.boa_grad_norm, *arrays, largest, norm.data_ptr(), work.data_ptr(), size)
     return norm
 
 
@@ -762,27 +779,19 @@ def clip_grad_norm_(parameters, max_norm: float, *, norm_type: float = 2.0):
     max_norm = float(max_norm)
     if not max_norm >= 0.0:
         raise ValueError(f"{who}: max_norm must not be negative (got {max_norm})")
-    all_grads, dev = _grads(who, parameters)
-    if not all_grads:
+    grads, arrays, copies, dev = _grads(who, parameters, True)
+    if dev is None:
         return torch.zeros(())
-    grads, copies = [], []
-    for g in all_grads:
-        if g.is_contiguous():
-            if not g._is_zerotensor():
-                grads.append(g)
-        else:
-            if any(s == 0 and n > 1 for s, n in zip(g.stride(), g.shape)):
-                raise ValueError(f"{who}: a gradient whose values share memory (strides {g.stride()}) cannot be scaled in place")
-            grads.append(g.contiguous())
-            copies.append((g, grads[-1]))
-    lib, n = _nat.lib(), len(grads)
-    size = lib.boa_grad_norm_work_bytes(n)
+    lib = _nat.lib()
+    size = _bytes("boa_grad_norm_work_bytes", len(grads))
     norm, work = torch.empty((), dtype=torch.float32, device=dev), torch.empty(size, dtype=torch.uint8, device=dev)
-    _call(norm, lib.boa_clip_grads, n, *_arrays(grads), largest, max_norm, norm.data_ptr(), work.data_ptr(), size)
-    with torch.no_grad():
-        for g, scaled in copies:
-            g.copy_(scaled)
-    increment_version(grads)
+    _call(norm, lib.boa_clip_grads, *arrays, largest, max_norm, norm.data_ptr(), work.data_ptr(), size)
+    if copies:
+        with torch.no_grad():
+            for g, scaled in copies:
+                g.copy_(scaled)
+    if grads:
+        increment_version(grads)
     return norm
 
 
