@@ -128,7 +128,8 @@ SIGNATURES = [
     # and boa_attention (ops._ATTENTION)
     ("boa_linear_attention_work_bytes", _I64, [ctypes.c_char_p, _INT]),
     ("boa_linear_attention_fwd", ctypes.c_int, [ctypes.c_char_p, _P, _I64, _P]),
-    ("boa_linear_attention_bwd", ctypes.c_int, [ctypes.c_char_p, _P, _I64, _P, _I64, _P]),
+    ("boa_linear_attention_marks_bytes", _I64, [ctypes.c_char_p]),
+    ("boa_linear_attention_bwd", ctypes.c_int, [ctypes.c_char_p, _P, _I64, _P]),
     ("boa_linear_attention_step", ctypes.c_int, [ctypes.c_char_p, _P]),
     # grads, counts and dtypes as the bytes of arrays
     ("boa_grad_norm_work_bytes", _I64, [_I32]),

@@ -571,8 +571,8 @@ def selective_scan_step(u, delta, A, B, C, D=None, z=None, delta_bias=None, *, s
 
 # ---- linear attention ------------------------------------------------------------------------------
 # boa_attention (include/boa_hip.h): dtype, heads, groups, key, value, decay_per_head, scale, unused; batch, length; q, k, v, y
-# (pointer, three strides); decay and its strides; lens, state_in, state_out; dy, dq, dk, dv; ddecay
-_ATTENTION = struct.Struct("@6ifi2q16q4q3q16qq")
+# (pointer, three strides); decay and its strides; lens, state_in, state_out, marks; dy, dq, dk, dv; ddecay
+_ATTENTION = struct.Struct("@6ifi2q16q4q4q16qq")
 _NO_HEADS = (0, 0, 0, 0)
 
 
@@ -580,31 +580,33 @@ def _r4(t):
     return _NO_HEADS if t is None else (t.data_ptr(), *t.stride()[:-1])
 
 
-def _pack_attention(q, k, v, g, scale, lens, state_in, state_out, y, back=(None,) * 4, dg=None):
+def _pack_attention(q, k, v, g, scale, lens, state_in, state_out, marks, y, back=(None,) * 4, dg=None):
     n, length, groups, key = q.shape
     gs = (0, 0, 1) if g.ndim == 1 else g.stride()
     return _ATTENTION.pack(_DTYPES[q.dtype], v.shape[2], groups, key, v.shape[3], g.ndim == 1, scale, 0, n, length, *_r4(q), *_r4(k),
-                           *_r4(v), *_r4(y), g.data_ptr(), *gs, _ptr(lens), _ptr(state_in), _ptr(state_out), *_r4(back[0]),
-                           *_r4(back[1]), *_r4(back[2]), *_r4(back[3]), _ptr(dg))
+                           *_r4(v), *_r4(y), g.data_ptr(), *gs, _ptr(lens), _ptr(state_in), _ptr(state_out), _ptr(marks),
+                           *_r4(back[0]), *_r4(back[1]), *_r4(back[2]), *_r4(back[3]), _ptr(dg))
 
 
-def _attention_fwd(q, k, v, g, scale, state, lens, want_state):
+def _attention_fwd(q, k, v, g, scale, state, lens, want_state, keep):
     n, length, heads, value = v.shape
     y = v.new_empty((n, length, heads, value))
     out = g.new_empty((n, heads, q.shape[3], value)) if want_state else None
-    args = _pack_attention(q, k, v, g, scale, lens, state, out, y)
+    # the states before every 64th position, of keys and values padded to multiples of 64
+    marks = g.new_empty((n * heads, -(-value // 64), -(-length // 64), -(-q.shape[3] // 64) * 4096)) if keep else None
+    args = _pack_attention(q, k, v, g, scale, lens, state, out, marks, y)
     lib = _nat.lib()
     size = lib.boa_linear_attention_work_bytes(args, 0)
     work = _work(size, q)
     _call(q, lib.boa_linear_attention_fwd, args, _ptr(work), size)
-    return y, out, work
+    return y, out, marks
 
 
 class _LinearAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, g, scale, state, lens, want_state):
-        y, out, work = _attention_fwd(q, k, v, g, scale, state, lens, want_state)
-        ctx.save_for_backward(q, k, v, g, lens, work)  # the states before the chunks are in the workspace
+        y, out, marks = _attention_fwd(q, k, v, g, scale, state, lens, want_state, True)
+        ctx.save_for_backward(q, k, v, g, lens, marks)
         ctx.scale = scale
         if out is not None:
             ctx.mark_non_differentiable(out)
@@ -613,14 +615,14 @@ class _LinearAttention(torch.autograd.Function):
     @staticmethod
     def backward(ctx, dy, _):
         dy = _once("linear_attention", dy)
-        q, k, v, g, lens, fwd = ctx.saved_tensors
+        q, k, v, g, lens, marks = ctx.saved_tensors
         dy = _rows(dy)
         dq, dk, dv, dg = (t.new_empty(t.shape) for t in (q, k, v, g))
-        args = _pack_attention(q, k, v, g, ctx.scale, lens, None, None, None, (dy, dq, dk, dv), dg)
+        args = _pack_attention(q, k, v, g, ctx.scale, lens, None, None, marks, None, (dy, dq, dk, dv), dg)
         lib = _nat.lib()
         size = lib.boa_linear_attention_work_bytes(args, 1)
         work = _work(size, q)
-        _call(q, lib.boa_linear_attention_bwd, args, _ptr(fwd), 0 if fwd is None else fwd.numel(), _ptr(work), size)
+        _call(q, lib.boa_linear_attention_bwd, args, _ptr(work), size)
         return dq, dk, dv, dg, None, None, None, None
 
 
@@ -674,7 +676,7 @@ def linear_attention(q, k, v, log_decay, *, scale=None, state=None, lens=None, r
     if _grad(q, k, v, g):
         y, out = _LinearAttention.apply(q, k, v, g, scale, state, lens, bool(return_state))
     else:
-        y, out, _ = _attention_fwd(q, k, v, g, scale, state, lens, return_state)
+        y, out, _ = _attention_fwd(q, k, v, g, scale, state, lens, return_state, False)
     return (y, out) if return_state else y
 
 
@@ -697,7 +699,7 @@ def linear_attention_step(q, k, v, log_decay, *, state, scale=None):
     packed = _ATTENTION.pack(_DTYPES[q.dtype], heads, q.shape[1], key, value, per_head, scale, 0, n, 1, q.data_ptr(), q.stride(0), 0,
                              q.stride(1), k.data_ptr(), k.stride(0), 0, k.stride(1), v.data_ptr(), v.stride(0), 0, v.stride(1),
                              y.data_ptr(), heads * value, 0, value, g.data_ptr(), 0 if per_head else g.stride(0), 0,
-                             1 if per_head else g.stride(1), 0, 0, state.data_ptr(), *(_NO_HEADS * 4), 0)
+                             1 if per_head else g.stride(1), 0, 0, state.data_ptr(), 0, *(_NO_HEADS * 4), 0)
     _call(q, _nat.lib().boa_linear_attention_step, packed)
     increment_version(state)
     return y

@@ -16,8 +16,13 @@
 // passes over the chunk, e^(G_end) <S, dS>.  All of them are sums of what is there; nothing is a difference of sums over the
 // whole length, whose rounding would grow with it.
 //
-// Four kernels: the states before every chunk (one workgroup walks a piece of the length with the state in registers; pieces
-// are joined by a small kernel), then every chunk by itself, forward or backward.
+// Forward, a workgroup walks a piece of the length with the state in registers; where the length is split, a first kernel finds
+// what each piece leaves by itself, and a small one joins them.  Backward, the gradients of the states behind every chunk are laid
+// down by a walk from the end, and then every chunk is done by itself.
+//
+// Everywhere a wavefront has 16 columns of a product's result: its own 16 positions i (or j) in what is made of A and dA, so that
+// these stay in its registers, where a result tile (column in the lane, four consecutive rows per lane) is the next product's
+// operand as it is; its own 16 of every 64 keys in a state.
 #include "ops_common.h"
 
 #include "../../include/boa_hip.h"
@@ -41,14 +46,15 @@ struct Args {
     const int32_t* lens;
     const float* state_in;
     float* state_out;
-    float* marks;   // [batch heads][value tiles][chunks][NP * PV] states before each chunk (backward: dS behind it), of its piece alone
-    float* starts;  // [batch heads][value tiles][pieces][NP * PV] what the pieces before leave (pieces > 1)
-    float* pre;     // [batch heads][chunks] decay from the start of its piece
+    float* marks;   // [batch heads][value tiles][chunks][NP * PV]: forward (or null) the states before the chunks, backward what lies
+                    // behind each chunk of its piece adds to the gradient of the state behind it
+    float* starts;  // [batch heads][value tiles][pieces][NP * PV] what each piece leaves, then what it starts from (pieces > 1)
+    float* pre;     // backward: [batch heads][chunks] decay from the chunk's end to its piece's
     double* fall;   // [batch heads][pieces] log2 of the piece's decay
-    const float *fmarks, *fstarts, *fpre;  // backward: the forward's
-    float *part_q, *part_k;                // backward: [batch][length][heads * value tiles][key], or null: dq, dk are written
-    float* dg;                             // backward: [value tiles][batch][length][heads], or null
-    float* dg_sum;                         // backward: [batch * chunks * value tiles][heads], or null
+    const float* fmarks;     // backward: the forward's
+    float *part_q, *part_k;  // backward: [batch][length][heads * value tiles][key], or null: dq, dk are written
+    float* dg;               // backward: [value tiles][batch][length][heads], or null
+    float* dg_sum;           // backward: [batch * chunks * value tiles][heads], or null
     int64_t batch, length, chunks;
     int32_t heads, share, key, value, tiles, pieces, per_piece;
     float scale;
@@ -56,11 +62,14 @@ struct Args {
 };
 enum { W_Q = 1, W_K = 2, W_V = 4, W_DY = 8, W_Y = 16, W_DQ = 32, W_DK = 64, W_DV = 128 };
 
-// How products of a type run: elements in LDS, parts that a float32 value is split into, K of a step.
-//   bfloat16: inputs as they are.  What is computed on the way (A, dA, states) is split into parts of 8 bits each: two for what
-//   ends in a result of 16 bits, three (24 bits) for the states and whatever goes into dg, which are float32.  One rounding to 8
-//   bits instead would be as large as the result's own rounding.
+// How products of a type run: elements in LDS, K of a step, parts that a float32 value is split into.
+//   bfloat16: inputs as they are.  What is computed on the way (A, dA, states, decayed keys) is split into parts of 8 bits each:
+//   two for what ends in a result of 16 bits, three (24 bits) for the states and whatever goes into dg, which are float32.  One
+//   rounding to 8 bits instead would be as large as the result's own rounding.
 //   float32, and float16, whose range the parts of a float32 value do not fit: float32 products (v_mfma_f32_16x16x4_f32).
+// A fragment holds VEC elements along K per lane: `row` of a tile with K along memory, `col` of one with K across; element e of lane
+// group g is k = VEC g + e.  `mixed` is `col` in the order of register tiles, k = 16 (e / 4) + 4 g + e % 4: element e of
+// `registers` is row 4 g + e % 4 of tile e / 4 of a result.
 template <int DT> struct Mat {
     using E = float;
     using Frag = f32x4;
@@ -70,23 +79,30 @@ template <int DT> struct Mat {
         for (int i = 0; i < 4; ++i) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[i], b[i], c, 0, 0, 0);
         return c;
     }
-    // rows of the fragment along K in memory
     static __device__ __forceinline__ Frag row(const E* t, int ld, int row0, int k0, int lane) {
         return *reinterpret_cast<const Frag*>(t + (row0 + (lane & 15)) * ld + k0 + (lane >> 4) * VEC);
     }
-    // and across: element [k][row]
     static __device__ __forceinline__ Frag col(const E* t, int ld, int row0, int k0, int lane) {
         const E* p = t + (k0 + (lane >> 4) * VEC) * ld + row0 + (lane & 15);
         return Frag{p[0], p[ld], p[2 * ld], p[3 * ld]};
     }
-    static __device__ __forceinline__ float value(E v) { return v; }
-    static __device__ __forceinline__ Frag finite(Frag f) {
+    static __device__ __forceinline__ Frag mixed(const E* t, int ld, int row0, int k0, int lane) { return col(t, ld, row0, k0, lane); }
+    static __device__ __forceinline__ void widen(const Frag& f, float (&x)[VEC]) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) f[i] = __builtin_isfinite(f[i]) ? f[i] : 0.0f;
-        return f;
+        for (int i = 0; i < VEC; ++i) x[i] = f[i];
     }
+    template <int PARTS>
+    static __device__ __forceinline__ void split(const float (&x)[VEC], Frag (&f)[PARTS]) {
+        f[0] = Frag{x[0], x[1], x[2], x[3]};
+    }
+    static __device__ __forceinline__ floatx4 load4(const E* p) { return *reinterpret_cast<const floatx4*>(p); }
 };
 typedef short s16x4 __attribute__((ext_vector_type(4)));
+// What is left of f behind its part hi; nothing behind an infinite one.
+__device__ __forceinline__ float rest(float f, float hi) {
+    const float r = f - hi;
+    return r == r ? r : 0.0f;
+}
 template <> struct Mat<DT_BF16> {
     using E = uint16_t;
     using Frag = bf16x8;
@@ -99,93 +115,153 @@ template <> struct Mat<DT_BF16> {
     }
     // The transposing read: of 16 lanes, lane i gives the address of 4 elements of row i / 4 at column 4 (i % 4) and gets column i of
     // the four rows.
-    static __device__ __forceinline__ Frag col(const E* t, int ld, int row0, int k0, int lane) {
+    static __device__ __forceinline__ Frag across(const E* t, int ld, int row0, int k, int apart, int lane) {
         const int l = lane & 15;
-        const E* p = t + (k0 + (lane >> 4) * VEC + (l >> 2)) * ld + row0 + (l & 3) * 4;
+        const E* p = t + (k + (l >> 2)) * ld + row0 + (l & 3) * 4;
         using P = __attribute__((address_space(3))) s16x4*;
         struct {
             s16x4 a, b;
-        } r = {__builtin_amdgcn_ds_read_tr16_b64_v4i16((P)p), __builtin_amdgcn_ds_read_tr16_b64_v4i16((P)(p + 4 * ld))};
+        } r = {__builtin_amdgcn_ds_read_tr16_b64_v4i16((P)p), __builtin_amdgcn_ds_read_tr16_b64_v4i16((P)(p + apart * ld))};
         return __builtin_bit_cast(Frag, r);
     }
-    static __device__ __forceinline__ float value(E v) { return __uint_as_float((uint32_t)v << 16); }
-    static __device__ __forceinline__ Frag finite(Frag f) {
-        u32x4 w = __builtin_bit_cast(u32x4, f);
+    static __device__ __forceinline__ Frag col(const E* t, int ld, int row0, int k0, int lane) {
+        return across(t, ld, row0, k0 + (lane >> 4) * VEC, 4, lane);
+    }
+    static __device__ __forceinline__ Frag mixed(const E* t, int ld, int row0, int k0, int lane) {
+        return across(t, ld, row0, k0 + (lane >> 4) * 4, 16, lane);
+    }
+    static __device__ __forceinline__ void widen(const Frag& f, float (&x)[VEC]) { Raw<DT_BF16, VEC>::unpack(__builtin_bit_cast(u32x4, f), x); }
+    template <int PARTS>
+    static __device__ __forceinline__ void split(const float (&x)[VEC], Frag (&f)[PARTS]) {
+        float v[VEC];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) w[i] &= ((w[i] & 0x7F80u) != 0x7F80u ? 0xFFFFu : 0u) | ((w[i] & 0x7F800000u) != 0x7F800000u ? 0xFFFF0000u : 0u);
-        return __builtin_bit_cast(Frag, w);
+        for (int i = 0; i < VEC; ++i) v[i] = x[i];
+#pragma unroll
+        for (int s = 0; s < PARTS; ++s) {
+            u32x4 w;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                w[i] = bf16_pk(v[2 * i], v[2 * i + 1]);
+                v[2 * i] = rest(v[2 * i], __uint_as_float(w[i] << 16));
+                v[2 * i + 1] = rest(v[2 * i + 1], __uint_as_float(w[i] & 0xFFFF0000u));
+            }
+            f[s] = __builtin_bit_cast(Frag, w);
+        }
+    }
+    static __device__ __forceinline__ floatx4 load4(const E* p) {
+        float v[4];
+        ld_vec<DT_BF16, 4>(p, v);
+        return floatx4{v[0], v[1], v[2], v[3]};
+    }
+};
+// Step s of a product over 64 positions whose second operand is in registers, four tiles of 16 rows.
+template <class M, int PARTS>
+__device__ __forceinline__ void registers(const floatx4 (&t)[4], int s, typename M::Frag (&f)[PARTS]) {
+    float x[M::VEC];
+#pragma unroll
+    for (int e = 0; e < M::VEC; ++e) x[e] = t[s * (M::VEC / 4) + e / 4][e % 4];
+    M::template split<PARTS>(x, f);
+}
+// Whether step s has anything of the tiles first .. last.
+template <class M>
+__device__ __forceinline__ bool has(int s, int first, int last) {
+    constexpr int T = M::VEC / 4;
+    return s * T <= last && s * T + T - 1 >= first;
+}
+
+// Infinities and NaN of a first operand that meet a second one which is held in parts, or is zero where a position may not be reached:
+// zero times those would be NaN.  They are left out of the product (`finite`), and added as what they are: products of ones count
+// those of each sign that meet a factor of each sign.  Whatever they do not reach keeps its bits.
+template <class M>
+struct Odd {
+    floatx4 up = {0.0f, 0.0f, 0.0f, 0.0f}, down = up, nan = up;
+    static __device__ __forceinline__ typename M::Frag finite(const typename M::Frag& f) {
+        float x[M::VEC];
+        M::widen(f, x);
+#pragma unroll
+        for (int e = 0; e < M::VEC; ++e) x[e] = __builtin_isfinite(x[e]) ? x[e] : 0.0f;
+        typename M::Frag r[1];
+        M::template split<1>(x, r);
+        return r[0];
+    }
+    // a: the first operand; w: the second's values, of which `in` count
+    __device__ __forceinline__ void step(const typename M::Frag& a, const float (&w)[M::VEC], const bool (&in)[M::VEC]) {
+        float x[M::VEC];
+        M::widen(a, x);
+        const auto count = [&](auto of, auto to, floatx4 c) {
+            typename M::Frag fo[1], ft[1];
+            float y[M::VEC], z[M::VEC];
+#pragma unroll
+            for (int e = 0; e < M::VEC; ++e) y[e] = of(x[e]) ? 1.0f : 0.0f, z[e] = in[e] && to(w[e]) ? 1.0f : 0.0f;
+            M::template split<1>(y, fo);
+            M::template split<1>(z, ft);
+            return M::mma(fo[0], ft[0], c);
+        };
+        const auto above = [](float f) { return f == __builtin_huge_valf(); };
+        const auto below = [](float f) { return f == -__builtin_huge_valf(); };
+        const auto plus = [](float f) { return f > 0.0f; };
+        const auto minus = [](float f) { return f < 0.0f; };
+        up = count(below, minus, count(above, plus, up));
+        down = count(above, minus, count(below, plus, down));
+        nan = count([](float f) { return f != f; }, [](float) { return true; }, nan);
+        nan = count([](float f) { return __builtin_isinf(f); }, [](float f) { return !(f > 0.0f) && !(f < 0.0f); }, nan);
+    }
+    __device__ __forceinline__ void add_to(floatx4& v) const {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            if (up[r] > 0.0f) v[r] += __builtin_huge_valf();
+            if (down[r] > 0.0f) v[r] -= __builtin_huge_valf();
+            if (nan[r] > 0.0f) v[r] = __builtin_nanf("");
+        }
     }
 };
 
-// acc[ta][tb] += A B over K from k0 to k1: A's rows from a0 on, B's from b0 on (16 each), held along K in memory (false) or across
-// (true), in AS and BS parts that are a_part and b_part elements apart (one of the two has a single part).  FINITE: without
-// those of A's elements that are infinite or NaN.
-template <class M, bool ACOL, bool BCOL, int AS, int BS, bool FINITE = false, int TA, int TB>
-__device__ __forceinline__ void product(floatx4 (&acc)[TA][TB], const typename M::E* a, int a_part, int lda, int a0,
-                                        const typename M::E* b, int b_part, int ldb, int b0, int k0, int k1, int lane) {
-    static_assert(AS == 1 || BS == 1, "");
-    for (int k = k0; k < k1; k += M::STEP) {
-        typename M::Frag fb[TB][BS];
-#pragma unroll
-        for (int j = 0; j < TB; ++j)
-#pragma unroll
-            for (int s = 0; s < BS; ++s)
-                fb[j][s] = BCOL ? M::col(b + s * b_part, ldb, b0 + 16 * j, k, lane) : M::row(b + s * b_part, ldb, b0 + 16 * j, k, lane);
-#pragma unroll
-        for (int i = 0; i < TA; ++i) {
-            typename M::Frag fa[AS];
-#pragma unroll
-            for (int s = 0; s < AS; ++s) {
-                fa[s] = ACOL ? M::col(a + s * a_part, lda, a0 + 16 * i, k, lane) : M::row(a + s * a_part, lda, a0 + 16 * i, k, lane);
-                if constexpr (FINITE) fa[s] = M::finite(fa[s]);
-            }
-#pragma unroll
-            for (int s = 0; s < AS * BS; ++s)
-#pragma unroll
-                for (int j = 0; j < TB; ++j) acc[i][j] = M::mma(fa[AS > 1 ? s : 0], fb[j][BS > 1 ? s : 0], acc[i][j]);
-        }
-    }
-}
-
-// acc += A B for a B that is zero outside a triangle: with UPTO, B is held along K and k <= column counts, without it across and
-// k >= column.  A is held across ([k][row]).  Where A has infinities or NaN, the zeros of B would make NaN of them and a position
-// would reach those before it (or behind, backward): they are left out of the matrix product and added element by element, so that
-// whatever they do not reach keeps its bits.
-template <class M, bool UPTO, int BS, int TA, int TB>
-__device__ __forceinline__ void product_within(floatx4 (&acc)[TA][TB], bool finite, const typename M::E* a, int lda, int a0,
-                                               const typename M::E* b, int b_part, int ldb, int b0, int lane) {
-    const int k0 = UPTO ? 0 : b0, k1 = UPTO ? b0 + 16 * TB : CHUNK;  // b0 is a multiple of M::STEP
+// acc[ta] += A B over 64 positions k: A's rows from a0 on, held across in LDS; B (16 columns) in registers, four tiles of 16 k, of which
+// those from `first` to `last` are not all zero.  inside(k) says whether B's k of this lane's column counts; B is zero where it
+// does not, and where A is not `finite` its zeros are kept apart.
+template <class M, int PARTS, int TA, class F>
+__device__ __forceinline__ void product_within(floatx4 (&acc)[TA], bool finite, const typename M::E* a, int lda, int a0, const floatx4 (&b)[4],
+                                               int first, int last, int lane, F inside) {
+    using Frag = typename M::Frag;
     if (finite) {
-        product<M, true, !UPTO, 1, BS>(acc, a, 0, lda, a0, b, b_part, ldb, b0, k0, k1, lane);
+#pragma unroll
+        for (int s = 0; s < CHUNK / M::STEP; ++s) {
+            if (!has<M>(s, first, last)) continue;
+            Frag fb[PARTS];
+            registers<M, PARTS>(b, s, fb);
+#pragma unroll
+            for (int i = 0; i < TA; ++i) {
+                const Frag fa = M::mixed(a, lda, a0 + 16 * i, s * M::STEP, lane);
+#pragma unroll
+                for (int p = 0; p < PARTS; ++p) acc[i] = M::mma(fa, fb[p], acc[i]);
+            }
+        }
         return;
     }
-    product<M, true, !UPTO, 1, BS, true>(acc, a, 0, lda, a0, b, b_part, ldb, b0, k0, k1, lane);
 #pragma unroll
-    for (int i = 0; i < TA; ++i)
+    for (int i = 0; i < TA; ++i) {
+        Odd<M> odd;
 #pragma unroll
-        for (int j = 0; j < TB; ++j)
+        for (int s = 0; s < CHUNK / M::STEP; ++s) {
+            if (!has<M>(s, first, last)) continue;
+            Frag fb[PARTS];
+            registers<M, PARTS>(b, s, fb);
+            const Frag fa = M::mixed(a, lda, a0 + 16 * i, s * M::STEP, lane), clean = Odd<M>::finite(fa);
+            float w[M::VEC];
+            bool in[M::VEC];
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int row = a0 + 16 * i + 4 * (lane >> 4) + r, col = b0 + 16 * j + (lane & 15);
-                float v = acc[i][j][r];
-#pragma unroll 1
-                for (int k = k0; k < k1; ++k) {
-                    const float x = M::value(a[k * lda + row]);
-                    if (__builtin_isfinite(x) || (UPTO ? k > col : k < col)) continue;
-                    float w = 0.0f;
-#pragma unroll
-                    for (int s = 0; s < BS; ++s) w += M::value(b[s * b_part + (UPTO ? col * ldb + k : k * ldb + col)]);
-                    v = __builtin_fmaf(x, w, v);
-                }
-                acc[i][j][r] = v;
+            for (int e = 0; e < M::VEC; ++e) {
+                w[e] = b[s * (M::VEC / 4) + e / 4][e % 4];
+                in[e] = inside(s * M::STEP + 16 * (e / 4) + 4 * (lane >> 4) + e % 4);
             }
+#pragma unroll
+            for (int p = 0; p < PARTS; ++p) acc[i] = M::mma(clean, fb[p], acc[i]);
+            odd.step(fa, w, in);
+        }
+        odd.add_to(acc[i]);
+    }
 }
 
-// A value that is no infinity minus itself: the parts behind an infinite first one are zero.
-__device__ __forceinline__ float rest(float f, float hi) {
-    const float r = f - hi;
-    return r == r ? r : 0.0f;
-}
 // Four consecutive values into LDS, in PARTS parts that are `part` elements apart.
 template <class M, int PARTS>
 __device__ __forceinline__ void put4(typename M::E* p, int part, floatx4 v) {
@@ -266,19 +342,6 @@ struct Tile {
             }
         }
     }
-    // each row times its weight, in three parts (one in float32)
-    __device__ __forceinline__ void store_weighted(typename M::E* t, const float* weight) const {
-#pragma unroll
-        for (int i = 0; i < PER; ++i) {
-            const int at = threadIdx.x + i * WG, r = at / ROW, c = at % ROW * V;
-            const float w = weight[r];
-            float f[V];
-            unpack(i, f);
-#pragma unroll
-            for (int e = 0; e < V; e += 4)
-                put4<M, M::THREE>(t + r * LD + c + e, SIZE, floatx4{f[e] * w, f[e + 1] * w, f[e + 2] * w, f[e + 3] * w});
-        }
-    }
 };
 
 // log2 of the decay from a chunk's start up to and with each position (lane), summed in 64 bits; a decay of zero (-inf) as
@@ -289,12 +352,7 @@ __device__ __forceinline__ double decays(const Args& a, int64_t b, int h, int64_
         g = (double)static_cast<const float*>(a.g.p)[b * a.g.bs + (t0 + lane) * a.g.rs + h * a.g.hs] * LOG2E;
         g = g < -200.0 ? -200.0 : g;
     }
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const double x = __shfl_up(g, o, 64);
-        if (lane >= o) g += x;
-    }
-    return g;
+    return scan(g);
 }
 __device__ __forceinline__ float2 in_two(double g) {
     const float hi = (float)g;
@@ -313,56 +371,115 @@ __device__ __forceinline__ typename Elem<DT>::T* row_of(const Heads& x, int64_t 
     return static_cast<typename Elem<DT>::T*>(x.p) + b * x.bs + t * x.rs + h * x.hs;
 }
 
-// Where a wavefront's values of a state lie: tile [tn][tp], value r of lane l is row n, column p of the state.
+// A state in a wavefront's registers: tile [tp][tn], value r of lane l is value 16 tp + 4 (l / 16) + r of key 64 tn + 16 wave + l % 16.
 template <int NP>
 struct State {
-    static constexpr int TN = NP / 32, TP = 2, SIZE = NP * PV;
-    floatx4 v[TN][TP];
-    static __device__ __forceinline__ int n(int tn, int lane, int wave) { return (wave & 1) * (NP / 2) + tn * 16 + 4 * (lane >> 4); }
-    static __device__ __forceinline__ int p(int tp, int lane, int wave) { return (wave >> 1) * 32 + tp * 16 + (lane & 15); }
-    static __device__ __forceinline__ int at(int tn, int tp, int lane, int wave) { return (((wave * TN + tn) * TP + tp) * 64 + lane) * 4; }
+    static constexpr int TN = NP / 64, TP = PV / 16, SIZE = NP * PV;
+    floatx4 v[TP][TN];
+    static __device__ __forceinline__ int n(int tn, int lane, int wave) { return 64 * tn + 16 * wave + (lane & 15); }
+    static __device__ __forceinline__ int p(int tp, int lane) { return 16 * tp + 4 * (lane >> 4); }
+    static __device__ __forceinline__ int at(int tp, int tn, int lane, int wave) { return (((wave * TN + tn) * TP + tp) * 64 + lane) * 4; }
+    template <class F>
+    __device__ __forceinline__ void each(F f) {
+#pragma unroll
+        for (int i = 0; i < TP; ++i)
+#pragma unroll
+            for (int j = 0; j < TN; ++j) f(i, j, v[i][j]);
+    }
+    __device__ __forceinline__ void zero() {
+        each([](int, int, floatx4& x) { x = floatx4{0.0f, 0.0f, 0.0f, 0.0f}; });
+    }
     __device__ __forceinline__ void load(const float* m, int lane, int wave) {
-#pragma unroll
-        for (int i = 0; i < TN; ++i)
-#pragma unroll
-            for (int j = 0; j < TP; ++j) v[i][j] = *reinterpret_cast<const floatx4*>(m + at(i, j, lane, wave));
+        each([&](int i, int j, floatx4& x) { x = *reinterpret_cast<const floatx4*>(m + at(i, j, lane, wave)); });
     }
     __device__ __forceinline__ void add(const float* m, float f, int lane, int wave) {
+        each([&](int i, int j, floatx4& x) {
+            const floatx4 y = *reinterpret_cast<const floatx4*>(m + at(i, j, lane, wave));
 #pragma unroll
-        for (int i = 0; i < TN; ++i)
-#pragma unroll
-            for (int j = 0; j < TP; ++j) {
-                const floatx4 x = *reinterpret_cast<const floatx4*>(m + at(i, j, lane, wave));
-#pragma unroll
-                for (int r = 0; r < 4; ++r) v[i][j][r] = __builtin_fmaf(f, x[r], v[i][j][r]);
-            }
+            for (int r = 0; r < 4; ++r) x[r] = __builtin_fmaf(f, y[r], x[r]);
+        });
     }
-    __device__ __forceinline__ void store(float* m, int lane, int wave) const {
-#pragma unroll
-        for (int i = 0; i < TN; ++i)
-#pragma unroll
-            for (int j = 0; j < TP; ++j) *reinterpret_cast<floatx4*>(m + at(i, j, lane, wave)) = v[i][j];
+    __device__ __forceinline__ void store(float* m, int lane, int wave) {
+        each([&](int i, int j, floatx4& x) { *reinterpret_cast<floatx4*>(m + at(i, j, lane, wave)) = x; });
     }
-    // Into LDS as rows of a column's values along n, zeros (which what lies behind key and value need not be) behind them.
+    // the caller's [key][value]
+    __device__ __forceinline__ void from_caller(const float* s, int key, int value, int p0, int lane, int wave) {
+        each([&](int i, int j, floatx4& x) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+                if (n(j, lane, wave) < key && p0 + p(i, lane) + r < value) x[r] = s[n(j, lane, wave) * value + p0 + p(i, lane) + r];
+        });
+    }
+    __device__ __forceinline__ void to_caller(float* s, int key, int value, int p0, int lane, int wave) {
+        each([&](int i, int j, floatx4& x) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+                if (n(j, lane, wave) < key && p0 + p(i, lane) + r < value) s[n(j, lane, wave) * value + p0 + p(i, lane) + r] = x[r];
+        });
+    }
+    // Into LDS as [key][value], zeros (which what lies behind key and value need not be) behind them.
     template <class M, int PARTS>
-    __device__ __forceinline__ void put(typename M::E* t, int key, int value, int lane, int wave) const {
-        constexpr int LD = NP + M::PAD;
+    __device__ __forceinline__ void put(typename M::E* t, int key, int value, int lane, int wave) {
+        constexpr int LD = PV + M::PAD;
+        each([&](int i, int j, floatx4& x) {
+            floatx4 y = x;
 #pragma unroll
-        for (int i = 0; i < TN; ++i)
-#pragma unroll
-            for (int j = 0; j < TP; ++j) {
-                floatx4 x = v[i][j];
-#pragma unroll
-                for (int r = 0; r < 4; ++r)
-                    if (n(i, lane, wave) + r >= key || p(j, lane, wave) >= value) x[r] = 0.0f;
-                put4<M, PARTS>(t + p(j, lane, wave) * LD + n(i, lane, wave), PV * LD, x);
-            }
+            for (int r = 0; r < 4; ++r)
+                if (n(j, lane, wave) >= key || p(i, lane) + r >= value) y[r] = 0.0f;
+            put4<M, PARTS>(t + n(j, lane, wave) * LD + p(i, lane), NP * LD, y);
+        });
     }
 };
 
-// ---- states before every chunk ----------------------------------------------------------------------
-// A workgroup walks the chunks of a piece, forward over k v^T, or (BACK) from the last one over scale e^(G_i) q dy^T, and leaves the
-// state that it reaches each chunk with.  Where the length is one piece it starts from the caller's state and hands it on.
+// One step of a state's update over STEP positions: s += (y)^T (x weight), y's fragments given; x (tile [position][key]) of the
+// wavefront's own keys is weighted in registers.
+template <class M, int NP, int LDX>
+__device__ __forceinline__ void update(State<NP>& s, bool finite, const typename M::Frag (&fy)[State<NP>::TP], const typename M::E* tx,
+                                       const float* weight, int step, int lane, int wave) {
+#pragma unroll
+    for (int j = 0; j < State<NP>::TN; ++j) {
+        float x[M::VEC];
+        M::widen(M::mixed(tx, LDX, 64 * j + 16 * wave, step * M::STEP, lane), x);
+#pragma unroll
+        for (int e = 0; e < M::VEC; e += 4) {
+            const f32x4 w = *reinterpret_cast<const f32x4*>(weight + step * M::STEP + 4 * e + 4 * (lane >> 4));
+#pragma unroll
+            for (int c = 0; c < 4; ++c) x[e + c] *= w[c];
+        }
+        typename M::Frag fx[M::THREE];
+        M::template split<M::THREE>(x, fx);
+        if (finite || M::THREE == 1) {
+#pragma unroll
+            for (int i = 0; i < State<NP>::TP; ++i)
+#pragma unroll
+                for (int p = 0; p < M::THREE; ++p) s.v[i][j] = M::mma(fy[i], fx[p], s.v[i][j]);
+        } else {
+            bool in[M::VEC];
+#pragma unroll
+            for (int e = 0; e < M::VEC; ++e) in[e] = true;
+#pragma unroll
+            for (int i = 0; i < State<NP>::TP; ++i) {
+                const typename M::Frag clean = Odd<M>::finite(fy[i]);
+                Odd<M> odd;
+#pragma unroll
+                for (int p = 0; p < M::THREE; ++p) s.v[i][j] = M::mma(clean, fx[p], s.v[i][j]);
+                odd.step(fy[i], x, in);
+                odd.add_to(s.v[i][j]);
+            }
+        }
+    }
+}
+template <int NP>
+__device__ __forceinline__ void times(State<NP>& s, float f) {
+    s.each([&](int, int, floatx4& x) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) x[r] *= f;
+    });
+}
+
+// ---- states by themselves ---------------------------------------------------------------------------
+// A workgroup walks the chunks of a piece from a state of zeros, forward over k v^T or (BACK) from the last one over scale e^(G_i)
+// q dy^T; leaves what it ends with, and backward also what it reaches each chunk with.
 template <int DT, int NP, bool BACK>
 __global__ void __launch_bounds__(WG) k_attn_states(const Args a) {
     using M = Mat<DT>;
@@ -370,9 +487,9 @@ __global__ void __launch_bounds__(WG) k_attn_states(const Args a) {
     using TY = Tile<DT, PV>;
     using S = State<NP>;
     __shared__ __attribute__((aligned(16))) typename M::E tx[TX::SIZE];
-    __shared__ __attribute__((aligned(16))) typename M::E ty[M::THREE * TY::SIZE];
-    __shared__ float weight[CHUNK];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    __shared__ __attribute__((aligned(16))) typename M::E ty[TY::SIZE];
+    __shared__ __attribute__((aligned(16))) float weight[CHUNK];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int piece = (int)(blockIdx.x % a.pieces), tile = (int)(blockIdx.x / a.pieces % a.tiles);
     const int64_t bh = blockIdx.x / a.pieces / a.tiles, b = bh / a.heads;
     const int h = (int)(bh % a.heads);
@@ -384,20 +501,7 @@ __global__ void __launch_bounds__(WG) k_attn_states(const Args a) {
     float* marks = a.marks + (bh * a.tiles + tile) * a.chunks * S::SIZE;
 
     S s;
-#pragma unroll
-    for (int i = 0; i < S::TN; ++i)
-#pragma unroll
-        for (int j = 0; j < S::TP; ++j) {
-            s.v[i][j] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
-            if (!BACK && a.pieces == 1 && a.state_in != nullptr) {
-                const int p = tile * PV + S::p(j, lane, wave);
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const int n = S::n(i, lane, wave) + r;
-                    if (n < a.key && p < a.value) s.v[i][j][r] = a.state_in[(bh * a.key + n) * a.value + p];
-                }
-            }
-        }
+    s.zero();
     double passed = 0.0;
     TX x;
     TY y;
@@ -413,41 +517,30 @@ __global__ void __launch_bounds__(WG) k_attn_states(const Args a) {
     if (n > 0) fetch(BACK ? c1 - 1 : c0);
     for (int64_t m = 0; m < n; ++m) {
         const int64_t c = BACK ? c1 - 1 - m : c0 + m;
-        s.store(marks + c * S::SIZE, lane, wave);
-        if (a.pre != nullptr && tile == 0 && threadIdx.x == 0) a.pre[bh * a.chunks + c] = __builtin_amdgcn_exp2f((float)passed);
-        const double all = __shfl(g, 63, 64);
-        if (wave == 0) weight[lane] = BACK ? a.scale * __builtin_amdgcn_exp2f((float)g) : __builtin_amdgcn_exp2f((float)(all - g));
-        __syncthreads();
+        if constexpr (BACK) {
+            s.store(marks + c * S::SIZE, lane, wave);
+            if (a.pieces > 1 && tile == 0 && threadIdx.x == 0) a.pre[bh * a.chunks + c] = __builtin_amdgcn_exp2f((float)passed);
+        }
+        const double all = last_lane(g);
         x.store(tx);
-        y.store_weighted(ty, weight);
-        __syncthreads();
+        y.store(ty);
+        if (wave == 0) weight[lane] = BACK ? a.scale * __builtin_amdgcn_exp2f((float)g) : __builtin_amdgcn_exp2f((float)(all - g));
+        const bool finite = __syncthreads_and(M::THREE == 1 || y.finite());
         if (m + 1 < n) fetch(BACK ? c - 1 : c + 1);
-        const float f = __builtin_amdgcn_exp2f((float)all);
         passed += all;
+        times(s, __builtin_amdgcn_exp2f((float)all));
 #pragma unroll
-        for (int i = 0; i < S::TN; ++i)
+        for (int k = 0; k < CHUNK / M::STEP; ++k) {
+            typename M::Frag fy[S::TP];
 #pragma unroll
-            for (int j = 0; j < S::TP; ++j)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) s.v[i][j][r] *= f;
-        product<M, true, true, 1, M::THREE>(s.v, tx, 0, TX::LD, (wave & 1) * (NP / 2), ty, TY::SIZE, TY::LD, (wave >> 1) * 32, 0, CHUNK, lane);
+            for (int i = 0; i < S::TP; ++i) fy[i] = M::mixed(ty, TY::LD, 16 * i, k * M::STEP, lane);
+            update<M, NP, TX::LD>(s, finite, fy, tx, weight, k, lane, wave);
+        }
         __syncthreads();
     }
     if (a.pieces > 1) {
         s.store(a.starts + ((bh * a.tiles + tile) * a.pieces + piece) * S::SIZE, lane, wave);
         if (tile == 0 && threadIdx.x == 0) a.fall[bh * a.pieces + piece] = passed;
-    } else if (!BACK && a.state_out != nullptr) {
-#pragma unroll
-        for (int i = 0; i < S::TN; ++i)
-#pragma unroll
-            for (int j = 0; j < S::TP; ++j) {
-                const int p = tile * PV + S::p(j, lane, wave);
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const int k = S::n(i, lane, wave) + r;
-                    if (k < a.key && p < a.value) a.state_out[(bh * a.key + k) * a.value + p] = s.v[i][j][r];
-                }
-            }
     }
 }
 
@@ -462,13 +555,13 @@ __global__ void __launch_bounds__(WG) k_attn_join(const Args a) {
     const int tile = (int)(bht % a.tiles), lane = threadIdx.x & 63;
     const int block = part * (WG / 64) + (threadIdx.x >> 6);  // (wave * TN + tn) * TP + tp
     const int tp = block % S::TP, tn = block / S::TP % S::TN, wave = block / S::TP / S::TN;
-    const int n = S::n(tn, lane, wave), p = tile * PV + S::p(tp, lane, wave);
+    const int n = S::n(tn, lane, wave), p = tile * PV + S::p(tp, lane);
     float* at = a.starts + bht * a.pieces * S::SIZE + block * 256 + lane * 4;
     floatx4 s = {0.0f, 0.0f, 0.0f, 0.0f};
     if (!BACK && a.state_in != nullptr)
 #pragma unroll
         for (int r = 0; r < 4; ++r)
-            if (n + r < a.key && p < a.value) s[r] = a.state_in[(bh * a.key + n + r) * a.value + p];
+            if (n < a.key && p + r < a.value) s[r] = a.state_in[(bh * a.key + n) * a.value + p + r];
     for (int i0 = 0; i0 < a.pieces; i0 += AT_ONCE) {
         floatx4 own[AT_ONCE];
         float f[AT_ONCE];
@@ -490,7 +583,7 @@ __global__ void __launch_bounds__(WG) k_attn_join(const Args a) {
     if (!BACK && a.state_out != nullptr)
 #pragma unroll
         for (int r = 0; r < 4; ++r)
-            if (n + r < a.key && p < a.value) a.state_out[(bh * a.key + n + r) * a.value + p] = s[r];
+            if (n < a.key && p + r < a.value) a.state_out[(bh * a.key + n) * a.value + p + r] = s[r];
 }
 
 // Four consecutive columns of a row of a result.
@@ -505,116 +598,132 @@ __device__ __forceinline__ void write4(typename Elem<DT>::T* p, int col, int col
             if (col + r < cols) p[col + r] = Elem<DT>::st(v[r]);
     }
 }
-
-struct Place {
-    int64_t c, bh, b, t0, end;
-    int tile, h, rows, vcols;
-    __device__ __forceinline__ Place(const Args& a) {
-        c = blockIdx.x % a.chunks;
-        tile = (int)(blockIdx.x / a.chunks % a.tiles);
-        bh = blockIdx.x / a.chunks / a.tiles;
-        b = bh / a.heads;
-        h = (int)(bh % a.heads);
-        t0 = c * CHUNK;
-        end = end_of(a, b);
-        rows = (int)max((int64_t)0, min((int64_t)CHUNK, end - t0));  // that hold something
-        vcols = min(PV, a.value - tile * PV);
-    }
-};
-// Zeros for the rows of a chunk from `from` on.
+// Zeros in the columns col0 .. of the rows [from, to).
 template <int DT>
-__device__ __forceinline__ void zero_rows(const Args& a, const Place& w, const Heads& x, int h, int col0, int cols, int from) {
-    const int last = (int)min((int64_t)CHUNK, a.length - w.t0);
-    for (int i = threadIdx.x; i < (last - from) * cols; i += WG)
-        row_of<DT>(x, w.b, w.t0 + from + i / cols, h)[col0 + i % cols] = Elem<DT>::st(0.0f);
+__device__ __forceinline__ void zero_rows(const Heads& x, int64_t b, int h, int col0, int cols, int64_t from, int64_t to) {
+    for (int64_t i = threadIdx.x; i < (to - from) * cols; i += WG) row_of<DT>(x, b, from + i / cols, h)[col0 + i % cols] = Elem<DT>::st(0.0f);
 }
 
-// ---- forward, a chunk ---------------------------------------------------------------------------------
+// ---- forward ------------------------------------------------------------------------------------------
+template <int DT, int NP>
+struct FwdLds {
+    using M = Mat<DT>;
+    static constexpr int Q = 0, K = Tile<DT, NP>::SIZE, V = 2 * K, S = V + Tile<DT, PV>::SIZE, LDS_STATE = PV + M::PAD, PART = NP * LDS_STATE;
+    static constexpr int BYTES = (int)sizeof(typename M::E) * (S + M::TWO * PART);
+};
 template <int DT, int NP>
 __global__ void __launch_bounds__(WG) k_attn_fwd(const Args a) {
     using M = Mat<DT>;
     using E = typename M::E;
+    using Frag = typename M::Frag;
     using TN = Tile<DT, NP>;
     using TV = Tile<DT, PV>;
     using S = State<NP>;
-    constexpr int SA = CHUNK * (CHUNK + M::PAD), LA = CHUNK + M::PAD;
+    using L = FwdLds<DT, NP>;
     extern __shared__ __attribute__((aligned(16))) char lds[];
-    E* tq = reinterpret_cast<E*>(lds);
-    E* tk = tq + TN::SIZE;
-    E* tv = tk + TN::SIZE;
-    E* ts = tv + TV::SIZE;                   // [PV][NP] in two parts
-    E* ta = ts + M::TWO * PV * TN::LD;       // [CHUNK][CHUNK] in two parts
+    E* tq = reinterpret_cast<E*>(lds) + L::Q;
+    E* tk = reinterpret_cast<E*>(lds) + L::K;
+    E* tv = reinterpret_cast<E*>(lds) + L::V;
+    E* ts = reinterpret_cast<E*>(lds) + L::S;  // [NP][PV] in two parts
     __shared__ float2 G[CHUNK];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const Place w(a);
-    if (w.rows < CHUNK) zero_rows<DT>(a, w, a.y, w.h, w.tile * PV, w.vcols, w.rows);
-    if (w.rows == 0) return;
+    __shared__ __attribute__((aligned(16))) float weight[CHUNK];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l15 = lane & 15, row4 = 4 * (lane >> 4);
+    // a wavefront's own positions i: the later ones have more before them, so workgroups beside each other have them the other way round
+    const int own = blockIdx.x & 1 ? WAVES - 1 - wave : wave;
+    const int piece = (int)(blockIdx.x % a.pieces), tile = (int)(blockIdx.x / a.pieces % a.tiles);
+    const int64_t bh = blockIdx.x / a.pieces / a.tiles, b = bh / a.heads;
+    const int h = (int)(bh % a.heads);
+    const int64_t end = end_of(a, b), bht = bh * a.tiles + tile;
+    const int64_t c0 = (int64_t)piece * a.per_piece, c1 = min(c0 + a.per_piece, (end + CHUNK - 1) / CHUNK);
+    const int vcols = min(PV, a.value - tile * PV);
+    const int64_t behind = min((c0 + a.per_piece) * CHUNK, a.length);
+    if (end < behind) zero_rows<DT>(a.y, b, h, tile * PV, vcols, max(end, c0 * CHUNK), behind);
+
+    S s;
+    s.zero();
+    if (a.pieces > 1) s.load(a.starts + (bht * a.pieces + piece) * S::SIZE, lane, wave);
+    else if (a.state_in != nullptr) s.from_caller(a.state_in + bh * a.key * a.value, a.key, a.value, tile * PV, lane, wave);
     TN q, k;
     TV v;
-    S s;
-    const int64_t bht = w.bh * a.tiles + w.tile;
-    s.load(a.marks + (bht * a.chunks + w.c) * S::SIZE, lane, wave);
-    q.load(row_of<DT>(a.q, w.b, w.t0, w.h / a.share), a.q.rs, w.rows, a.key, a.wide & W_Q);
-    k.load(row_of<DT>(a.k, w.b, w.t0, w.h / a.share), a.k.rs, w.rows, a.key, a.wide & W_K);
-    v.load(row_of<DT>(a.v, w.b, w.t0, w.h) + w.tile * PV, a.v.rs, w.rows, w.vcols, a.wide & W_V);
-    const double g = decays(a, w.b, w.h, w.t0, w.rows, lane);
-    if (wave == 0) G[lane] = in_two(g);
-    if (a.pieces > 1)
-        s.add(a.starts + (bht * a.pieces + w.c / a.per_piece) * S::SIZE, a.pre[w.bh * a.chunks + w.c], lane, wave);
-    q.store(tq);
-    k.store(tk);
-    v.store(tv);
-    s.template put<M, M::TWO>(ts, a.key, w.vcols, lane, wave);
-    const bool finite = __syncthreads_and(v.finite());
-    const int i0 = (wave & 1) * 32, j0 = (wave >> 1) * 32, l15 = lane & 15, row4 = 4 * (lane >> 4);
-    // A_ij of 32 x 32 positions (rows j, column i), into LDS along j
-    if (j0 <= i0) {
-        floatx4 acc[2][2] = {};
-        product<M, false, false, 1, 1>(acc, tk, 0, TN::LD, j0, tq, 0, TN::LD, i0, 0, NP, lane);
-#pragma unroll
-        for (int ti = 0; ti < 2; ++ti) {
-            const int i = i0 + 16 * ti + l15;
-            const float2 gi = G[i];
-#pragma unroll
-            for (int tj = 0; tj < 2; ++tj) {
-                const int j = j0 + 16 * tj + row4;
-                floatx4 x;
-#pragma unroll
-                for (int r = 0; r < 4; ++r)
-                    x[r] = j + r <= i && i < w.rows ? acc[tj][ti][r] * (a.scale * fall_between(gi, G[j + r])) : 0.0f;
-                put4<M, M::TWO>(ta + i * LA + j, SA, x);
-            }
+    double g = 0.0;
+    const auto fetch = [&](int64_t c) {
+        const int64_t t0 = c * CHUNK;
+        const int rows = (int)min((int64_t)CHUNK, end - t0);
+        q.load(row_of<DT>(a.q, b, t0, h / a.share), a.q.rs, rows, a.key, a.wide & W_Q);
+        k.load(row_of<DT>(a.k, b, t0, h / a.share), a.k.rs, rows, a.key, a.wide & W_K);
+        v.load(row_of<DT>(a.v, b, t0, h) + tile * PV, a.v.rs, rows, vcols, a.wide & W_V);
+        g = decays(a, b, h, t0, rows, lane);
+    };
+    if (c0 < c1) fetch(c0);
+    for (int64_t c = c0; c < c1; ++c) {
+        const int64_t t0 = c * CHUNK;
+        const int rows = (int)min((int64_t)CHUNK, end - t0);
+        const double all = last_lane(g);
+        q.store(tq);
+        k.store(tk);
+        v.store(tv);
+        s.template put<M, M::TWO>(ts, a.key, vcols, lane, wave);
+        if (wave == 0) {
+            G[lane] = in_two(g);
+            weight[lane] = __builtin_amdgcn_exp2f((float)(all - g));
         }
-    }
-    // y of 32 positions (columns) and 32 values (rows): what the state gives, then the chunk's own
-    const int p0 = j0;
-    floatx4 y[2][2] = {};
-    product<M, false, false, M::TWO, 1>(y, ts, PV * TN::LD, TN::LD, p0, tq, 0, TN::LD, i0, 0, NP, lane);
+        const bool finite = __syncthreads_and(v.finite());
+        if (a.marks != nullptr) s.store(a.marks + (bht * a.chunks + c) * S::SIZE, lane, wave);
+        if (c + 1 < c1) fetch(c + 1);
+
+        // q . k of all positions j (rows) and the own ones (columns), and what the state gives
+        floatx4 A[4] = {}, y[S::TP] = {};
 #pragma unroll
-    for (int ti = 0; ti < 2; ++ti) {
-        const float2 gi = G[i0 + 16 * ti + l15];
+        for (int n = 0; n < NP; n += M::STEP) {
+            const Frag fq = M::row(tq, TN::LD, 16 * own, n, lane);
+#pragma unroll
+            for (int t = 0; t < 4; ++t)
+                if (t <= own) A[t] = M::mma(M::row(tk, TN::LD, 16 * t, n, lane), fq, A[t]);
+#pragma unroll
+            for (int p = 0; p < S::TP; ++p)
+#pragma unroll
+                for (int i = 0; i < M::TWO; ++i) y[p] = M::mma(M::col(ts + i * L::PART, L::LDS_STATE, 16 * p, n, lane), fq, y[p]);
+        }
+        const int i = 16 * own + l15;
+        const float2 gi = G[i];
         const float f = a.scale * __builtin_amdgcn_exp2f(gi.x + gi.y);
 #pragma unroll
-        for (int tp = 0; tp < 2; ++tp)
+        for (int p = 0; p < S::TP; ++p)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) y[tp][ti][r] *= f;
+            for (int r = 0; r < 4; ++r) y[p][r] *= f;
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+            if (t <= own)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const int j = 16 * t + row4 + r;
+                    A[t][r] = j <= i && i < rows ? A[t][r] * (a.scale * fall_between(gi, G[j])) : 0.0f;
+                }
+        times(s, __builtin_amdgcn_exp2f((float)all));
+        if (!finite) product_within<M, M::TWO>(y, false, tv, TV::LD, 0, A, 0, own, lane, [&](int j) { return j <= i && i < rows; });
+#pragma unroll
+        for (int k = 0; k < CHUNK / M::STEP; ++k) {
+            Frag fv[S::TP];
+#pragma unroll
+            for (int p = 0; p < S::TP; ++p) fv[p] = M::mixed(tv, TV::LD, 16 * p, k * M::STEP, lane);
+            if (finite && has<M>(k, 0, own)) {
+                Frag fa[M::TWO];
+                registers<M, M::TWO>(A, k, fa);
+#pragma unroll
+                for (int p = 0; p < S::TP; ++p)
+#pragma unroll
+                    for (int x = 0; x < M::TWO; ++x) y[p] = M::mma(fv[p], fa[x], y[p]);
+            }
+            update<M, NP, TN::LD>(s, finite, fv, tk, weight, k, lane, wave);
+        }
+        if (i < rows) {
+            auto* out = row_of<DT>(a.y, b, t0 + i, h) + tile * PV;
+#pragma unroll
+            for (int p = 0; p < S::TP; ++p) write4<DT>(out, 16 * p + row4, vcols, a.wide & W_Y, y[p]);
+        }
+        __syncthreads();
     }
-    __syncthreads();
-    product_within<M, true, M::TWO>(y, finite, tv, TV::LD, p0, ta, SA, LA, i0, lane);
-#pragma unroll
-    for (int ti = 0; ti < 2; ++ti) {
-        const int i = i0 + 16 * ti + l15;
-        if (i >= w.rows) continue;
-        auto* out = row_of<DT>(a.y, w.b, w.t0 + i, w.h) + w.tile * PV;
-#pragma unroll
-        for (int tp = 0; tp < 2; ++tp) write4<DT>(out, p0 + 16 * tp + row4, w.vcols, a.wide & W_Y, y[tp][ti]);
-    }
-}
-template <int DT, int NP>
-constexpr int fwd_lds() {
-    using M = Mat<DT>;
-    return (int)sizeof(typename M::E) * (2 * Tile<DT, NP>::SIZE + Tile<DT, PV>::SIZE + M::TWO * PV * Tile<DT, NP>::LD +
-                                         M::TWO * CHUNK * (CHUNK + M::PAD));
+    if (a.pieces == 1 && a.state_out != nullptr) s.to_caller(a.state_out + bh * a.key * a.value, a.key, a.value, tile * PV, lane, wave);
 }
 
 // ---- backward, a chunk --------------------------------------------------------------------------------
@@ -624,7 +733,7 @@ __device__ __forceinline__ float over_rows(float v) {
     return v + __shfl_xor(v, 32, 64);
 }
 // Of the 16 columns of a row of lanes the sum from a lane's own to the last one.
-constexpr int DPP_SHL1 = 0x101, DPP_SHL2 = 0x102, DPP_SHL4 = 0x104, DPP_SHL8 = 0x108, DPP_FROM_FIRST = 0x150;
+constexpr int DPP_SHL1 = 0x101, DPP_SHL2 = 0x102, DPP_SHL4 = 0x104, DPP_SHL8 = 0x108;
 __device__ __forceinline__ float from_here(float v) {
     v += dpp<DPP_SHL1>(v);
     v += dpp<DPP_SHL2>(v);
@@ -632,262 +741,261 @@ __device__ __forceinline__ float from_here(float v) {
     return v + dpp<DPP_SHL8>(v);
 }
 
+// In LDS: first S and dS, each [NP][PV] in three parts, with v and dy; then q and k in their places; last dS again in q's.
+template <int DT, int NP>
+struct BwdLds {
+    using M = Mat<DT>;
+    static constexpr int LDS_STATE = PV + M::PAD, PART = NP * LDS_STATE;
+    static constexpr int ONE = M::THREE * PART > Tile<DT, NP>::SIZE ? M::THREE * PART : Tile<DT, NP>::SIZE;
+    static constexpr int Q = 0, K = ONE, V = 2 * ONE, D = V + Tile<DT, PV>::SIZE;
+    static constexpr int BYTES = (int)sizeof(typename M::E) * (D + Tile<DT, PV>::SIZE);
+};
 template <int DT, int NP>
 __global__ void __launch_bounds__(WG) k_attn_bwd(const Args a) {
     using M = Mat<DT>;
     using E = typename M::E;
+    using Frag = typename M::Frag;
     using TN = Tile<DT, NP>;
     using TV = Tile<DT, PV>;
     using S = State<NP>;
-    constexpr int SA = CHUNK * (CHUNK + M::PAD), LA = CHUNK + M::PAD, SS = PV * TN::LD, NT = NP / 32;
+    using L = BwdLds<DT, NP>;
+    constexpr int NT = NP / 16, LS = L::LDS_STATE;
     extern __shared__ __attribute__((aligned(16))) char lds[];
-    E* tq = reinterpret_cast<E*>(lds);
-    E* tk = tq + TN::SIZE;
-    E* tv = tk + TN::SIZE;
-    E* td = tv + TV::SIZE;           // dy
-    E* ts = td + TV::SIZE;           // [PV][NP] in three parts: S, then dS
-    E* ta = ts + M::THREE * SS;      // [CHUNK][CHUNK] in two parts: dA, then A
+    E* tq = reinterpret_cast<E*>(lds) + L::Q;
+    E* tk = reinterpret_cast<E*>(lds) + L::K;
+    E* tv = reinterpret_cast<E*>(lds) + L::V;
+    E* td = reinterpret_cast<E*>(lds) + L::D;  // dy
     __shared__ float2 G[CHUNK];
-    __shared__ float pairs[2][CHUNK], over_middle[CHUNK / 2], from_before[2][CHUNK], to_behind[2][CHUNK], through[WAVES];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l15 = lane & 15, row4 = 4 * (lane >> 4);
-    const Place w(a);
-    const int part = w.h * a.tiles + w.tile, parts = a.heads * a.tiles;
-    const int present = (int)min((int64_t)CHUNK, a.length - w.t0);
-    float* dg = a.dg == nullptr ? nullptr : a.dg + ((w.tile * a.batch + w.b) * a.length + w.t0) * a.heads + w.h;
-    float* dg_sum = a.dg_sum == nullptr ? nullptr : a.dg_sum + ((w.b * a.chunks + w.c) * a.tiles + w.tile) * a.heads + w.h;
-    const auto part_row = [&](float* p, int i) { return p + ((w.b * a.length + w.t0 + i) * parts + part) * a.key; };
-    if (w.rows < CHUNK) {
-        zero_rows<DT>(a, w, a.dv, w.h, w.tile * PV, w.vcols, w.rows);
+    __shared__ float pairs[CHUNK], middle[WAVES - 1][CHUNK], from_state[CHUNK], to_behind[CHUNK], through[WAVES];
+    const int lane = threadIdx.x & 63, own = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l15 = lane & 15, row4 = 4 * (lane >> 4);
+    const int64_t c = blockIdx.x % a.chunks, bht = blockIdx.x / a.chunks, bh = bht / a.tiles, b = bh / a.heads, t0 = c * CHUNK;
+    const int tile = (int)(bht % a.tiles), h = (int)(bh % a.heads);
+    const int64_t end = end_of(a, b);
+    const int present = (int)min((int64_t)CHUNK, a.length - t0);
+    const int rows = (int)max((int64_t)0, min((int64_t)CHUNK, end - t0));  // that hold something
+    const int vcols = min(PV, a.value - tile * PV);
+    float* dg = a.dg == nullptr ? nullptr : a.dg + ((tile * a.batch + b) * a.length + t0) * a.heads + h;
+    float* dg_sum = a.dg_sum == nullptr ? nullptr : a.dg_sum + ((b * a.chunks + c) * a.tiles + tile) * a.heads + h;
+    const auto part_row = [&](float* p, int64_t i) { return p + ((b * a.length + t0 + i) * (a.heads * a.tiles) + h * a.tiles + tile) * a.key; };
+    if (rows < present) {
+        zero_rows<DT>(a.dv, b, h, tile * PV, vcols, t0 + rows, t0 + present);
         if (a.part_q == nullptr) {
-            zero_rows<DT>(a, w, a.dq, w.h, 0, a.key, w.rows);
-            zero_rows<DT>(a, w, a.dk, w.h, 0, a.key, w.rows);
+            zero_rows<DT>(a.dq, b, h, 0, a.key, t0 + rows, t0 + present);
+            zero_rows<DT>(a.dk, b, h, 0, a.key, t0 + rows, t0 + present);
         } else {
-            for (int i = threadIdx.x; i < (present - w.rows) * a.key; i += WG) {
-                part_row(a.part_q, w.rows + i / a.key)[i % a.key] = 0.0f;
-                part_row(a.part_k, w.rows + i / a.key)[i % a.key] = 0.0f;
+            for (int i = threadIdx.x; i < (present - rows) * a.key; i += WG) {
+                part_row(a.part_q, rows + i / a.key)[i % a.key] = 0.0f;
+                part_row(a.part_k, rows + i / a.key)[i % a.key] = 0.0f;
             }
         }
     }
-    if (w.rows == 0) {
+    if (rows == 0) {
         if (dg != nullptr && (int)threadIdx.x < present) dg[(int64_t)threadIdx.x * a.heads] = 0.0f;
         if (dg_sum != nullptr && threadIdx.x == 0) *dg_sum = 0.0f;
         return;
     }
-    S s, ds;
+    S ds;
     TN q, k;
-    TV v, d;
-    const int64_t bht = w.bh * a.tiles + w.tile, mark = (bht * a.chunks + w.c) * S::SIZE;
-    const int64_t start = (bht * a.pieces + w.c / a.per_piece) * S::SIZE;
-    q.load(row_of<DT>(a.q, w.b, w.t0, w.h / a.share), a.q.rs, w.rows, a.key, a.wide & W_Q);
-    k.load(row_of<DT>(a.k, w.b, w.t0, w.h / a.share), a.k.rs, w.rows, a.key, a.wide & W_K);
-    v.load(row_of<DT>(a.v, w.b, w.t0, w.h) + w.tile * PV, a.v.rs, w.rows, w.vcols, a.wide & W_V);
-    d.load(row_of<DT>(a.dy, w.b, w.t0, w.h) + w.tile * PV, a.dy.rs, w.rows, w.vcols, a.wide & W_DY);
-    s.load(a.fmarks + mark, lane, wave);
-    ds.load(a.marks + mark, lane, wave);
-    const double g = decays(a, w.b, w.h, w.t0, w.rows, lane);
-    const double all = __shfl(g, 63, 64);
-    const float2 g_end = in_two(all);
-    if (wave == 0) G[lane] = in_two(g);
-    if (a.pieces > 1) {
-        s.add(a.fstarts + start, a.fpre[w.bh * a.chunks + w.c], lane, wave);
-        ds.add(a.starts + start, a.pre[w.bh * a.chunks + w.c], lane, wave);
-    }
-    q.store(tq);
-    k.store(tk);
-    v.store(tv);
-    d.store(td);
-    s.template put<M, M::THREE>(ts, a.key, w.vcols, lane, wave);
-    // what passes over the chunk
+    bool finite;
     {
+        S s;
+        TV v, d;
+        const int64_t mark = (bht * a.chunks + c) * S::SIZE;
+        s.load(a.fmarks + mark, lane, own);
+        ds.load(a.marks + mark, lane, own);
+        v.load(row_of<DT>(a.v, b, t0, h) + tile * PV, a.v.rs, rows, vcols, a.wide & W_V);
+        d.load(row_of<DT>(a.dy, b, t0, h) + tile * PV, a.dy.rs, rows, vcols, a.wide & W_DY);
+        q.load(row_of<DT>(a.q, b, t0, h / a.share), a.q.rs, rows, a.key, a.wide & W_Q);
+        k.load(row_of<DT>(a.k, b, t0, h / a.share), a.k.rs, rows, a.key, a.wide & W_K);
+        if (a.pieces > 1) ds.add(a.starts + (bht * a.pieces + c / a.per_piece) * S::SIZE, a.pre[bh * a.chunks + c], lane, own);
+        const double g = decays(a, b, h, t0, rows, lane);
+        if (own == 0) G[lane] = in_two(g);
+        v.store(tv);
+        d.store(td);
+        s.template put<M, M::THREE>(tq, a.key, vcols, lane, own);
+        ds.template put<M, M::THREE>(tk, a.key, vcols, lane, own);
+        // what passes over the chunk
         float x = 0.0f;
 #pragma unroll
-        for (int i = 0; i < S::TN; ++i)
+        for (int i = 0; i < S::TP; ++i)
 #pragma unroll
-            for (int j = 0; j < S::TP; ++j)
+            for (int j = 0; j < S::TN; ++j)
 #pragma unroll
                 for (int r = 0; r < 4; ++r)
-                    if (S::n(i, lane, wave) + r < a.key && S::p(j, lane, wave) < w.vcols) x = __builtin_fmaf(s.v[i][j][r], ds.v[i][j][r], x);
+                    if (S::n(j, lane, own) < a.key && S::p(i, lane) + r < vcols) x = __builtin_fmaf(s.v[i][j][r], ds.v[i][j][r], x);
         x = wsum(x);
-        if (lane == 0) through[wave] = x;
+        if (lane == 0) through[own] = x;
+        finite = __syncthreads_and(q.finite() && k.finite() && d.finite());
     }
-    const bool finite = __syncthreads_and(q.finite() && k.finite() && d.finite());
-
-    // A and dA of 32 x 32 positions (rows j, column i)
-    const int i0 = (wave & 1) * 32, j0 = (wave >> 1) * 32;
-    floatx4 A[2][2] = {}, dA[2][2] = {};
-    if (j0 <= i0) {
-        product<M, false, false, 1, 1>(A, tk, 0, TN::LD, j0, tq, 0, TN::LD, i0, 0, NP, lane);
-        product<M, false, false, 1, 1>(dA, tv, 0, TV::LD, j0, td, 0, TV::LD, i0, 0, PV, lane);
-        floatx4 m[2][2];
+    const int me = 16 * own + l15;  // the own position, as i of dq and as j of dk and dv
+    const float2 mine = G[me], g_end = G[CHUNK - 1];
+    const float to_end = fall_between(g_end, mine), from_start = a.scale * __builtin_amdgcn_exp2f(mine.x + mine.y);
+    floatx4 dq[NT] = {}, dk[NT] = {};
 #pragma unroll
-        for (int ti = 0; ti < 2; ++ti) {
-            const int i = i0 + 16 * ti + l15;
-            const float2 gi = G[i];
+    for (int p = 0; p < PV; p += M::STEP) {
+        const Frag fd = M::row(td, TV::LD, 16 * own, p, lane), fv = M::row(tv, TV::LD, 16 * own, p, lane);
 #pragma unroll
-            for (int tj = 0; tj < 2; ++tj) {
-                const int j = j0 + 16 * tj + row4;
+        for (int n = 0; n < NT; ++n)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const bool in = j + r <= i && i < w.rows;
-                    const float f = a.scale * fall_between(gi, G[j + r]);
-                    A[tj][ti][r] = in ? A[tj][ti][r] * f : 0.0f;
-                    m[tj][ti][r] = in ? A[tj][ti][r] * dA[tj][ti][r] : 0.0f;
-                    dA[tj][ti][r] = in ? dA[tj][ti][r] * f : 0.0f;
-                }
-                put4<M, M::TWO>(ta + i * LA + j, SA, dA[tj][ti]);
+            for (int x = 0; x < M::THREE; ++x) {
+                dq[n] = M::mma(M::row(tq + x * L::PART, LS, 16 * n, p, lane), fd, dq[n]);
+                dk[n] = M::mma(M::row(tk + x * L::PART, LS, 16 * n, p, lane), fv, dk[n]);
             }
-        }
-        // the pairs that a position t (as i) lies between: sums of M_ij over i >= t of these 32, then over j < t
-        float at[2] = {0.0f, 0.0f};
+    }
+    __syncthreads();
+    q.store(tq);
+    k.store(tk);
+    __syncthreads();
+    {
+        float x = 0.0f, y = 0.0f;
 #pragma unroll
-        for (int tj = 0; tj < 2; ++tj)
+        for (int n = 0; n < NT; ++n) {
+            const floatx4 fq = M::load4(tq + me * TN::LD + 16 * n + row4), fk = M::load4(tk + me * TN::LD + 16 * n + row4);
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                const float second = from_here(m[tj][1][r]), first = from_here(m[tj][0][r]) + dpp<DPP_FROM_FIRST>(second);
-                const int j = j0 + 16 * tj + row4 + r;
-                at[0] += j < i0 + l15 ? first : 0.0f;
-                at[1] += j < i0 + 16 + l15 ? second : 0.0f;
-                if (i0 > j0 && l15 == 0) over_middle[j] = first;
+                dq[n][r] *= from_start;
+                dk[n][r] *= to_end;
+                x = __builtin_fmaf(dq[n][r], fq[r], x);
+                y = __builtin_fmaf(dk[n][r], fk[r], y);
             }
-#pragma unroll
-        for (int ti = 0; ti < 2; ++ti) {
-            const float x = over_rows(at[ti]);
-            if (lane < 16) pairs[wave >> 1][i0 + 16 * ti + l15] = x;
         }
-    } else if (lane < 32) {
-        pairs[wave >> 1][i0 + lane] = 0.0f;
+        x = over_rows(x);
+        y = over_rows(y);
+        if (lane < 16) from_state[me] = x, to_behind[me] = y;
     }
-    __syncthreads();
-
-    // key halves by the wavefront's second bit here, positions by its first
-    const int n0 = (wave >> 1) * (NP / 2);
+    // the own positions as i: rows are positions j before them
     {
-        floatx4 o[NT][2] = {};
-        product<M, true, false, M::THREE, 1>(o, ts, SS, TN::LD, n0, td, 0, TV::LD, i0, 0, PV, lane);
+        floatx4 A[4] = {}, dA[4] = {};
 #pragma unroll
-        for (int ti = 0; ti < 2; ++ti) {
-            const int i = i0 + 16 * ti + l15;
-            const float2 gi = G[i];
-            const float f = a.scale * __builtin_amdgcn_exp2f(gi.x + gi.y);
-            float x = 0.0f;
+        for (int n = 0; n < NP; n += M::STEP) {
+            const Frag f = M::row(tq, TN::LD, 16 * own, n, lane);
 #pragma unroll
-            for (int tn = 0; tn < NT; ++tn)
+            for (int t = 0; t < 4; ++t)
+                if (t <= own) A[t] = M::mma(M::row(tk, TN::LD, 16 * t, n, lane), f, A[t]);
+        }
+#pragma unroll
+        for (int p = 0; p < PV; p += M::STEP) {
+            const Frag f = M::row(td, TV::LD, 16 * own, p, lane);
+#pragma unroll
+            for (int t = 0; t < 4; ++t)
+                if (t <= own) dA[t] = M::mma(M::row(tv, TV::LD, 16 * t, p, lane), f, dA[t]);
+        }
+        // the pairs that a position t of the own ones lies between: of M_ij the sum over the own i >= t, then over j < t; and all own i
+        // for the positions of the tiles before
+        float at = 0.0f;
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+            if (t <= own)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    o[tn][ti][r] *= f;
-                    x = __builtin_fmaf(o[tn][ti][r], M::value(tq[i * TN::LD + n0 + 16 * tn + row4 + r]), x);
+                    const int j = 16 * t + row4 + r;
+                    const bool in = j <= me && me < rows;
+                    const float w = a.scale * fall_between(mine, G[j]);
+                    const float m = in ? A[t][r] * w * dA[t][r] : 0.0f;
+                    dA[t][r] = in ? dA[t][r] * w : 0.0f;
+                    const float sum = from_here(m);
+                    at += j < me ? sum : 0.0f;
+                    if (t < own && l15 == 0) middle[own - 1][j] = sum;
                 }
-            x = over_rows(x);
-            if (lane < 16) from_before[wave >> 1][i] = x;
-        }
-        product_within<M, true, M::TWO>(o, finite, tk, TN::LD, n0, ta, SA, LA, i0, lane);
+        at = over_rows(at);
+        if (lane < 16) pairs[me] = at;
+        product_within<M, M::TWO>(dq, finite, tk, TN::LD, 0, dA, 0, own, lane, [&](int j) { return j <= me && me < rows; });
+        if (me < rows) {
 #pragma unroll
-        for (int ti = 0; ti < 2; ++ti) {
-            const int i = i0 + 16 * ti + l15;
-            if (i >= w.rows) continue;
-#pragma unroll
-            for (int tn = 0; tn < NT; ++tn) {
-                if (a.part_q == nullptr) write4<DT>(row_of<DT>(a.dq, w.b, w.t0 + i, w.h), n0 + 16 * tn + row4, a.key, a.wide & W_DQ, o[tn][ti]);
-                else write4<DT_F32>(part_row(a.part_q, i), n0 + 16 * tn + row4, a.key, a.key % 4 == 0, o[tn][ti]);
+            for (int n = 0; n < NT; ++n) {
+                if (a.part_q == nullptr) write4<DT>(row_of<DT>(a.dq, b, t0 + me, h), 16 * n + row4, a.key, a.wide & W_DQ, dq[n]);
+                else write4<DT_F32>(part_row(a.part_q, me), 16 * n + row4, a.key, a.key % 4 == 0, dq[n]);
             }
         }
     }
-    __syncthreads();
-    ds.template put<M, M::THREE>(ts, a.key, w.vcols, lane, wave);
-    __syncthreads();
+    // the own positions as j: rows are positions i behind them
+    floatx4 dv[S::TP] = {};
     {
-        const int c0 = i0;  // the columns are positions j here
-        floatx4 o[NT][2] = {};
-        product<M, true, false, M::THREE, 1>(o, ts, SS, TN::LD, n0, tv, 0, TV::LD, c0, 0, PV, lane);
+        floatx4 A[4] = {}, dA[4] = {};
 #pragma unroll
-        for (int tj = 0; tj < 2; ++tj) {
-            const int j = c0 + 16 * tj + l15;
-            const float f = fall_between(g_end, G[j]);
-            float x = 0.0f;
+        for (int n = 0; n < NP; n += M::STEP) {
+            const Frag f = M::row(tk, TN::LD, 16 * own, n, lane);
 #pragma unroll
-            for (int tn = 0; tn < NT; ++tn)
+            for (int t = 0; t < 4; ++t)
+                if (t >= own) A[t] = M::mma(M::row(tq, TN::LD, 16 * t, n, lane), f, A[t]);
+        }
+#pragma unroll
+        for (int p = 0; p < PV; p += M::STEP) {
+            const Frag f = M::row(tv, TV::LD, 16 * own, p, lane);
+#pragma unroll
+            for (int t = 0; t < 4; ++t)
+                if (t >= own) dA[t] = M::mma(M::row(td, TV::LD, 16 * t, p, lane), f, dA[t]);
+        }
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+            if (t >= own)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    o[tn][tj][r] *= f;
-                    x = __builtin_fmaf(o[tn][tj][r], M::value(tk[j * TN::LD + n0 + 16 * tn + row4 + r]), x);
+                    const int i = 16 * t + row4 + r;
+                    const bool in = i >= me && i < rows;
+                    const float w = a.scale * fall_between(G[i], mine);
+                    A[t][r] = in ? A[t][r] * w : 0.0f;
+                    dA[t][r] = in ? dA[t][r] * w : 0.0f;
                 }
-            x = over_rows(x);
-            if (lane < 16) to_behind[wave >> 1][j] = x;
-        }
-        product_within<M, false, M::TWO>(o, finite, tq, TN::LD, n0, ta, SA, LA, c0, lane);
+        const auto inside = [&](int i) { return i >= me && i < rows; };
+        product_within<M, M::TWO>(dk, finite, tq, TN::LD, 0, dA, own, 3, lane, inside);
+        product_within<M, M::TWO>(dv, finite, td, TV::LD, 0, A, own, 3, lane, inside);
+        if (me < rows) {
 #pragma unroll
-        for (int tj = 0; tj < 2; ++tj) {
-            const int j = c0 + 16 * tj + l15;
-            if (j >= w.rows) continue;
-#pragma unroll
-            for (int tn = 0; tn < NT; ++tn) {
-                if (a.part_k == nullptr) write4<DT>(row_of<DT>(a.dk, w.b, w.t0 + j, w.h), n0 + 16 * tn + row4, a.key, a.wide & W_DK, o[tn][tj]);
-                else write4<DT_F32>(part_row(a.part_k, j), n0 + 16 * tn + row4, a.key, a.key % 4 == 0, o[tn][tj]);
+            for (int n = 0; n < NT; ++n) {
+                if (a.part_k == nullptr) write4<DT>(row_of<DT>(a.dk, b, t0 + me, h), 16 * n + row4, a.key, a.wide & W_DK, dk[n]);
+                else write4<DT_F32>(part_row(a.part_k, me), 16 * n + row4, a.key, a.key % 4 == 0, dk[n]);
             }
         }
     }
     __syncthreads();
-    if (j0 <= i0) {
-#pragma unroll
-        for (int ti = 0; ti < 2; ++ti)
-#pragma unroll
-            for (int tj = 0; tj < 2; ++tj) put4<M, M::TWO>(ta + (i0 + 16 * ti + l15) * LA + j0 + 16 * tj + row4, SA, A[tj][ti]);
-    }
+    ds.template put<M, M::TWO>(tq, a.key, vcols, lane, own);
     __syncthreads();
     {
-        const int p0 = j0, c0 = i0;
-        floatx4 o[2][2] = {};
-        product<M, false, false, M::THREE, 1>(o, ts, SS, TN::LD, p0, tk, 0, TN::LD, c0, 0, NP, lane);
+        floatx4 far[S::TP] = {};
 #pragma unroll
-        for (int tj = 0; tj < 2; ++tj) {
-            const float f = fall_between(g_end, G[c0 + 16 * tj + l15]);
+        for (int n = 0; n < NP; n += M::STEP) {
+            const Frag f = M::row(tk, TN::LD, 16 * own, n, lane);
 #pragma unroll
-            for (int tp = 0; tp < 2; ++tp)
+            for (int p = 0; p < S::TP; ++p)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) o[tp][tj][r] *= f;
+                for (int x = 0; x < M::TWO; ++x) far[p] = M::mma(M::col(tq + x * L::PART, LS, 16 * p, n, lane), f, far[p]);
         }
-        product_within<M, false, M::TWO>(o, finite, td, TV::LD, p0, ta, SA, LA, c0, lane);
+        if (me < rows) {
+            auto* out = row_of<DT>(a.dv, b, t0 + me, h) + tile * PV;
 #pragma unroll
-        for (int tj = 0; tj < 2; ++tj) {
-            const int j = c0 + 16 * tj + l15;
-            if (j >= w.rows) continue;
-            auto* out = row_of<DT>(a.dv, w.b, w.t0 + j, w.h) + w.tile * PV;
+            for (int p = 0; p < S::TP; ++p) {
 #pragma unroll
-            for (int tp = 0; tp < 2; ++tp) write4<DT>(out, p0 + 16 * tp + row4, w.vcols, a.wide & W_DV, o[tp][tj]);
+                for (int r = 0; r < 4; ++r) dv[p][r] = __builtin_fmaf(to_end, far[p][r], dv[p][r]);
+                write4<DT>(out, 16 * p + row4, vcols, a.wide & W_DV, dv[p]);
+            }
         }
     }
     // dg, by one wavefront (lane = position)
-    if (wave == 0 && (dg != nullptr || dg_sum != nullptr)) {
-        // of the chunk's own pairs those of its second half with its first are missing for the first half's positions
-        const double over = ((double)through[0] + (double)through[1] + (double)through[2] + (double)through[3]) * (double)__builtin_amdgcn_exp2f((float)all);
-        const bool in = lane < w.rows;
-        double behind = in ? (double)to_behind[0][lane] + (double)to_behind[1][lane] : 0.0;
-        double middle = lane < CHUNK / 2 ? (double)over_middle[lane] : 0.0;
-        double later = in ? (double)from_before[0][lane] + (double)from_before[1][lane] : 0.0;
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const double x = __shfl_up(behind, o, 64), y = __shfl_up(middle, o, 64), z = __shfl_down(later, o, 64);
-            if (lane >= o) behind += x, middle += y;
-            if (lane + o < 64) later += z;
-        }
-        behind = __shfl_up(behind, 1, 64), middle = __shfl_up(middle, 1, 64);  // of the positions before
-        double x = (double)pairs[0][lane] + (double)pairs[1][lane] + later + over;
+    if (own == 0 && (dg != nullptr || dg_sum != nullptr)) {
+        const double over = ((double)through[0] + (double)through[1] + (double)through[2] + (double)through[3]) *
+                            (double)__builtin_amdgcn_exp2f(g_end.x + g_end.y);
+        const bool in = lane < rows;
+        // from the states before: positions i from t on (summed from the last one); to the positions behind the chunk: j before t
+        const int last = CHUNK - 1 - lane;
+        double later = scan(last < rows ? (double)from_state[last] : 0.0);
+        later = __shfl(later, CHUNK - 1 - lane, 64);
+        double x = (double)pairs[lane] + later + over;
+        const double behind = __shfl_up(scan(in ? (double)to_behind[lane] : 0.0), 1, 64);
         if (lane > 0) x += behind;
-        if (lane > 0 && lane < CHUNK / 2) x += middle;
+        // and of the chunk's own pairs those with an i of a later tile than t's
+#pragma unroll
+        for (int t = 1; t < WAVES; ++t) {
+            const double before = __shfl_up(scan(lane < 16 * t ? (double)middle[t - 1][lane] : 0.0), 1, 64);
+            if (lane > 0 && lane < 16 * t) x += before;
+        }
         if (!in) x = 0.0;
         if (dg != nullptr && lane < present) dg[(int64_t)lane * a.heads] = (float)x;
         if (dg_sum != nullptr) {
-            double sum = x;
-            for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
+            const double sum = last_lane(scan(x));
             if (lane == 0) *dg_sum = (float)sum;
         }
     }
-}
-template <int DT, int NP>
-constexpr int bwd_lds() {
-    using M = Mat<DT>;
-    return (int)sizeof(typename M::E) * (2 * Tile<DT, NP>::SIZE + 2 * Tile<DT, PV>::SIZE + M::THREE * PV * Tile<DT, NP>::LD +
-                                         M::TWO * CHUNK * (CHUNK + M::PAD));
 }
 
 // dq and dk of a group's key from its heads' parts (and those of their value tiles), in their order; dg from its value tiles.
@@ -982,18 +1090,19 @@ bool wide_rows(int dtype, const boa_heads& x, int cols) {
 }
 
 // The split: pieces of whole chunks, as many as give the wanted workgroups.
-constexpr int64_t WANTED = 1024;
+constexpr int64_t WANTED = 512, WANTED_BACK = 1024;
 struct Plan {
     int np, tiles;
     int64_t chunks, bh;
     int32_t pieces, per_piece;
-    explicit Plan(const boa_attention& s) {
+    bool back;
+    Plan(const boa_attention& s, bool backward) : back(backward) {
         np = s.key <= 64 ? 64 : 128;
         tiles = (int)ceil_div(s.value, PV);
         chunks = ceil_div(s.length, CHUNK);
         bh = s.batch * s.heads;
         const int64_t each = bh * tiles;
-        int64_t n = each > 0 ? ceil_div(WANTED, each) : 1;
+        int64_t n = each > 0 ? ceil_div(back ? WANTED_BACK : WANTED, each) : 1;
         n = n < chunks ? n : chunks;
         per_piece = (int32_t)(n > 1 ? ceil_div(chunks, n) : chunks > 1 ? chunks : 1);
         pieces = (int32_t)(chunks > 1 ? ceil_div(chunks, per_piece) : 1);
@@ -1001,20 +1110,26 @@ struct Plan {
     int64_t state() const { return (int64_t)np * PV; }
     int64_t marks() const { return bh * tiles * chunks * state(); }
     int64_t starts() const { return pieces > 1 ? bh * tiles * pieces * state() : 0; }
-    int64_t states_bytes() const { return 4 * (marks() + starts()) + (pieces > 1 ? (4 * bh * chunks + 8 * bh * pieces + 15) / 16 * 16 : 0); }
-    // [marks][starts][fall][pre] from p on
+    // [starts][fall][pre], backward behind [marks]
+    int64_t bytes() const {
+        return (back ? 4 * marks() : 0) + 4 * starts() + (pieces > 1 ? (8 * bh * pieces + (back ? 4 * bh * chunks : 0) + 15) / 16 * 16 : 0);
+    }
     void place(Args& a, void* p) const {
-        a.marks = static_cast<float*>(p);
-        a.starts = a.marks + marks();
+        a.starts = static_cast<float*>(p);
+        if (back) {
+            a.marks = a.starts;
+            a.starts += marks();
+        }
         a.fall = reinterpret_cast<double*>(a.starts + starts());
-        a.pre = pieces > 1 ? reinterpret_cast<float*>(a.fall + bh * pieces) : nullptr;
+        a.pre = reinterpret_cast<float*>(a.fall + bh * pieces);
+        a.pieces = pieces, a.per_piece = per_piece;
     }
 };
 
 bool parts_wanted(const boa_attention& s, const Plan& p) { return s.heads / s.groups * p.tiles > 1; }
 
 int64_t bwd_bytes(const boa_attention& s, const Plan& p) {
-    int64_t n = p.states_bytes();
+    int64_t n = p.bytes();
     if (parts_wanted(s, p)) n += 2 * 4 * s.batch * s.length * s.heads * p.tiles * s.key;
     if (s.decay_per_head) n += 4 * s.batch * p.chunks * p.tiles * s.heads;
     else if (p.tiles > 1) n += 4 * p.tiles * s.batch * s.length * s.heads;
@@ -1045,8 +1160,7 @@ Args args_of(const boa_attention& s, const Plan& p) {
            s.decay_per_head ? 1 : s.decay_head_stride};
     a.lens = s.lens, a.state_in = s.state_in, a.state_out = s.state_out;
     a.batch = s.batch, a.length = s.length, a.chunks = p.chunks;
-    a.heads = s.heads, a.share = s.heads / s.groups, a.key = s.key, a.value = s.value, a.tiles = p.tiles;
-    a.pieces = p.pieces, a.per_piece = p.per_piece, a.scale = s.scale;
+    a.heads = s.heads, a.share = s.heads / s.groups, a.key = s.key, a.value = s.value, a.tiles = p.tiles, a.scale = s.scale;
     const struct {
         uint32_t bit;
         const boa_heads& x;
@@ -1070,7 +1184,7 @@ int with_key(int np, F f) {
     return np == 64 ? f(std::integral_constant<int, 64>()) : f(std::integral_constant<int, 128>());
 }
 
-// The states before every chunk (backward: their gradients behind it).
+// What the pieces leave, and backward what every chunk's end is reached with.
 template <int DT, int NP, bool BACK>
 int launch_states(const Args& a, const Plan& p, hipStream_t s) {
     hipLaunchKernelGGL((k_attn_states<DT, NP, BACK>), dim3((uint32_t)(p.bh * p.tiles * p.pieces)), dim3(WG), 0, s, a);
@@ -1086,41 +1200,46 @@ int launch_states(const Args& a, const Plan& p, hipStream_t s) {
 
 extern "C" int64_t boa_linear_attention_work_bytes(const boa_attention* s, int backward) {
     if (check_sizes("boa_linear_attention_work_bytes", s) != BOA_OK) return -1;
-    const Plan p(*s);
-    return backward ? bwd_bytes(*s, p) : p.states_bytes();
+    const Plan p(*s, backward != 0);
+    return backward ? bwd_bytes(*s, p) : p.bytes();
+}
+
+extern "C" int64_t boa_linear_attention_marks_bytes(const boa_attention* s) {
+    if (check_sizes("boa_linear_attention_marks_bytes", s) != BOA_OK) return -1;
+    return 4 * Plan(*s, false).marks();
 }
 
 extern "C" int boa_linear_attention_fwd(const boa_attention* s, void* d_work, int64_t work_bytes, void* stream) {
     const int rc = check_sizes("boa_linear_attention_fwd", s);
     if (rc != BOA_OK) return rc;
     if (s->batch == 0) return BOA_OK;
-    if (!s->decay || (s->length > 0 && (!s->q.p || !s->k.p || !s->v.p || !s->y.p)))
-        return boa_fail(BOA_ERR_ARG, "boa_linear_attention_fwd: null pointer");
-    const Plan p(*s);
-    if (p.states_bytes() > 0 && (!d_work || (uintptr_t)d_work % 16 || work_bytes < p.states_bytes()))
+    if (!s->decay || (s->length > 0 && (!s->q.p || !s->k.p || !s->v.p || !s->y.p)) || (uintptr_t)s->marks % 16)
+        return boa_fail(BOA_ERR_ARG, "boa_linear_attention_fwd: null pointer, or marks not at a multiple of 16 bytes");
+    const Plan p(*s, false);
+    if (p.bytes() > 0 && (!d_work || (uintptr_t)d_work % 16 || work_bytes < p.bytes()))
         return boa_fail(BOA_ERR_ARG, "boa_linear_attention_fwd: workspace of %lld bytes, needs %lld at a multiple of 16", (long long)work_bytes,
-                        (long long)p.states_bytes());
+                        (long long)p.bytes());
     Args a = args_of(*s, p);
     p.place(a, d_work);
+    a.marks = s->marks;
+    hipStream_t st = (hipStream_t)stream;
     return with_dtype(s->dtype, [&](auto dt) {
         return with_key(p.np, [&](auto np) {
-            constexpr int DT = decltype(dt)::value, NP = decltype(np)::value;
-            const int done = launch_states<DT, NP, false>(a, p, (hipStream_t)stream);
-            if (done != BOA_OK || p.chunks == 0) return done;
-            constexpr int LDS = fwd_lds<DT, NP>();
+            constexpr int DT = decltype(dt)::value, NP = decltype(np)::value, LDS = FwdLds<DT, NP>::BYTES;
+            if (p.pieces > 1)
+                if (const int no = launch_states<DT, NP, false>(a, p, st)) return no;
             if (const int no = allow_lds(k_attn_fwd<DT, NP>, LDS)) return no;
-            hipLaunchKernelGGL((k_attn_fwd<DT, NP>), dim3((uint32_t)(p.bh * p.tiles * p.chunks)), dim3(WG), LDS, (hipStream_t)stream, a);
+            hipLaunchKernelGGL((k_attn_fwd<DT, NP>), dim3((uint32_t)(p.bh * p.tiles * p.pieces)), dim3(WG), LDS, st, a);
             BOA_HIP_TRY(hipGetLastError());
             return (int)BOA_OK;
         });
     });
 }
 
-extern "C" int boa_linear_attention_bwd(const boa_attention* s, const void* d_fwd_work, int64_t fwd_work_bytes, void* d_work, int64_t work_bytes,
-                                        void* stream) {
+extern "C" int boa_linear_attention_bwd(const boa_attention* s, void* d_work, int64_t work_bytes, void* stream) {
     const int rc = check_sizes("boa_linear_attention_bwd", s);
     if (rc != BOA_OK) return rc;
-    const Plan p(*s);
+    const Plan p(*s, true);
     if (!s->decay || !s->ddecay) return boa_fail(BOA_ERR_ARG, "boa_linear_attention_bwd: null pointer");
     const int64_t need = bwd_bytes(*s, p);
     hipStream_t st = (hipStream_t)stream;
@@ -1128,18 +1247,16 @@ extern "C" int boa_linear_attention_bwd(const boa_attention* s, const void* d_fw
         if (s->decay_per_head) BOA_HIP_TRY(launch_sum_parts(nullptr, 0, s->heads, s->ddecay, st));
         return BOA_OK;
     }
-    if (!s->q.p || !s->k.p || !s->v.p || !s->dy.p || !s->dq.p || !s->dk.p || !s->dv.p)
-        return boa_fail(BOA_ERR_ARG, "boa_linear_attention_bwd: null pointer");
-    if (!d_fwd_work || fwd_work_bytes < p.states_bytes() || !d_work || work_bytes < need || ((uintptr_t)d_fwd_work | (uintptr_t)d_work) % 16)
-        return boa_fail(BOA_ERR_ARG,
-                        "boa_linear_attention_bwd: workspaces of %lld (the forward's) and %lld bytes, needs %lld and %lld at multiples of 16",
-                        (long long)fwd_work_bytes, (long long)work_bytes, (long long)p.states_bytes(), (long long)need);
+    if (!s->q.p || !s->k.p || !s->v.p || !s->dy.p || !s->dq.p || !s->dk.p || !s->dv.p || !s->marks || (uintptr_t)s->marks % 16)
+        return boa_fail(BOA_ERR_ARG, "boa_linear_attention_bwd: null pointer, or marks not at a multiple of 16 bytes");
+    if (!d_work || work_bytes < need || (uintptr_t)d_work % 16)
+        return boa_fail(BOA_ERR_ARG, "boa_linear_attention_bwd: workspace of %lld bytes, needs %lld at a multiple of 16", (long long)work_bytes,
+                        (long long)need);
     Args a = args_of(*s, p);
-    p.place(a, const_cast<void*>(d_fwd_work));
-    a.fmarks = a.marks, a.fstarts = a.starts, a.fpre = a.pre;
     p.place(a, d_work);
+    a.fmarks = s->marks;
     a.state_in = nullptr, a.state_out = nullptr;
-    float* rest = reinterpret_cast<float*>(static_cast<char*>(d_work) + p.states_bytes());
+    float* rest = reinterpret_cast<float*>(static_cast<char*>(d_work) + p.bytes());
     if (parts_wanted(*s, p)) {
         const int64_t each = s->batch * s->length * s->heads * p.tiles * s->key;
         a.part_q = rest, a.part_k = rest + each;
@@ -1149,10 +1266,8 @@ extern "C" int boa_linear_attention_bwd(const boa_attention* s, const void* d_fw
     else a.dg = p.tiles > 1 ? rest : s->ddecay;
     return with_dtype(s->dtype, [&](auto dt) {
         return with_key(p.np, [&](auto np) {
-            constexpr int DT = decltype(dt)::value, NP = decltype(np)::value;
-            const int done = launch_states<DT, NP, true>(a, p, st);
-            if (done != BOA_OK) return done;
-            constexpr int LDS = bwd_lds<DT, NP>();
+            constexpr int DT = decltype(dt)::value, NP = decltype(np)::value, LDS = BwdLds<DT, NP>::BYTES;
+            if (const int no = launch_states<DT, NP, true>(a, p, st)) return no;
             if (const int no = allow_lds(k_attn_bwd<DT, NP>, LDS)) return no;
             hipLaunchKernelGGL((k_attn_bwd<DT, NP>), dim3((uint32_t)(p.bh * p.tiles * p.chunks)), dim3(WG), LDS, st, a);
             BOA_HIP_TRY(hipGetLastError());
@@ -1184,7 +1299,7 @@ extern "C" int boa_linear_attention_step(const boa_attention* s, void* stream) {
     if (s->batch == 0) return BOA_OK;
     if (!s->q.p || !s->k.p || !s->v.p || !s->y.p || !s->decay || !s->state_out)
         return boa_fail(BOA_ERR_ARG, "boa_linear_attention_step: null pointer");
-    const Plan p(*s);
+    const Plan p(*s, false);
     const Args a = args_of(*s, p);
     const bool vec = s->value % 4 == 0 && (uintptr_t)s->state_out % 16 == 0;
     const dim3 grid((uint32_t)(p.bh < MAX_BLOCKS ? p.bh : MAX_BLOCKS));

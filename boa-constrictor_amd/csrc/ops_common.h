@@ -148,6 +148,35 @@ __device__ __forceinline__ float wsum(float v) {
 // Lane l's value in all lanes (l the same for all).
 __device__ __forceinline__ float from_lane(float v, int l) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), l)); }
 
+// Inclusive sum over the lanes before, by permutations in registers: inside rows of 16, then from the rows before.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double from_before(double v) {
+    const u32x2 w = __builtin_bit_cast(u32x2, v);
+    const u32x2 r = {(uint32_t)__builtin_amdgcn_update_dpp(0, (int)w[0], CTRL, ROWS, 0xF, false),
+                     (uint32_t)__builtin_amdgcn_update_dpp(0, (int)w[1], CTRL, ROWS, 0xF, false)};
+    return __builtin_bit_cast(double, r);
+}
+template <int CTRL, int ROWS>
+__device__ __forceinline__ float from_before(float v) {
+    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, ROWS, 0xF, false));
+}
+constexpr int DPP_SHR1 = 0x111, DPP_SHR2 = 0x112, DPP_SHR4 = 0x114, DPP_SHR8 = 0x118, DPP_BCAST15 = 0x142, DPP_BCAST31 = 0x143;
+template <class T>
+__device__ __forceinline__ T scan(T v) {
+    v += from_before<DPP_SHR1, 0xF>(v);
+    v += from_before<DPP_SHR2, 0xF>(v);
+    v += from_before<DPP_SHR4, 0xF>(v);
+    v += from_before<DPP_SHR8, 0xF>(v);
+    v += from_before<DPP_BCAST15, 0xA>(v);
+    return v + from_before<DPP_BCAST31, 0xC>(v);
+}
+__device__ __forceinline__ double last_lane(double v) {
+    const u32x2 w = __builtin_bit_cast(u32x2, v);
+    const u32x2 r = {(uint32_t)__builtin_amdgcn_readlane((int)w[0], 63), (uint32_t)__builtin_amdgcn_readlane((int)w[1], 63)};
+    return __builtin_bit_cast(double, r);
+}
+__device__ __forceinline__ float last_lane(float v) { return from_lane(v, 63); }
+
 __device__ __forceinline__ float hw_sigmoid(float x) { return __builtin_amdgcn_rcpf(1.0f + hw_exp(-x)); }
 
 __host__ __device__ inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }

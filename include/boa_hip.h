@@ -329,15 +329,17 @@ typedef struct boa_attention {
     const int32_t* lens;                    /* * [batch]                                                 */
     const float* state_in;                  /* * [batch][heads][key][value] before the first position (zeros) */
     float* state_out;                       /* * the same behind each sequence's last position, another buffer */
+    float* marks;                           /* states that the forward pass leaves for the backward pass, at a multiple of 16
+                                               bytes; * forward                                          */
     boa_heads dy, dq, dk, dv;               /* backward                                                  */
     float* ddecay;                          /* backward: [batch][length][heads] or [heads]               */
 } boa_attention;
 /* Bytes of d_work, at a multiple of 16, that boa_linear_attention_fwd (backward = 0) or _bwd (1) needs for these sizes. */
 int64_t boa_linear_attention_work_bytes(const boa_attention* s, int backward);
+int64_t boa_linear_attention_marks_bytes(const boa_attention* s);  /* and of marks */
 int boa_linear_attention_fwd(const boa_attention* s, void* d_work, int64_t work_bytes, void* stream);
-/* The gradient for everything but the state.  Takes the forward's inputs and its workspace as it left it. */
-int boa_linear_attention_bwd(const boa_attention* s, const void* d_fwd_work, int64_t fwd_work_bytes, void* d_work,
-                             int64_t work_bytes, void* stream);
+/* The gradient for everything but the state.  Takes the forward's inputs and marks.                     */
+int boa_linear_attention_bwd(const boa_attention* s, void* d_work, int64_t work_bytes, void* stream);
 /* One position per sequence (length 1): advances state_out in place (lens and state_in are not used).    */
 int boa_linear_attention_step(const boa_attention* s, void* stream);
 

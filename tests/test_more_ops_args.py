@@ -170,13 +170,13 @@ def test_tensors_without_memory_are_not_taken_for_absent_ones(monkeypatch):
 
 
 # ---- the C ABI: every refusal comes before any launch ------------------------------------------------
-def _packed(dtype=0, heads=4, groups=2, key=6, value=3, n=2, length=5, p=16, decay=16, state_out=0, ddecay=16):
+def _packed(dtype=0, heads=4, groups=2, key=6, value=3, n=2, length=5, p=16, decay=16, state_out=0, ddecay=16, marks=16):
     rows = (p, 1, 1, 1)
-    return ops._ATTENTION.pack(dtype, heads, groups, key, value, 0, 1.0, 0, n, length, *(rows * 4), decay, 1, 1, 1, 0, 0, state_out, *(rows * 4), ddecay)
+    return ops._ATTENTION.pack(dtype, heads, groups, key, value, 0, 1.0, 0, n, length, *(rows * 4), decay, 1, 1, 1, 0, 0, state_out, marks, *(rows * 4), ddecay)
 
 
 def test_the_struct_has_the_headers_size():
-    assert ops._ATTENTION.size == 6 * 4 + 8 + 16 + 4 * 32 + 8 + 24 + 24 + 4 * 32 + 8
+    assert ops._ATTENTION.size == 6 * 4 + 8 + 16 + 4 * 32 + 8 + 24 + 32 + 4 * 32 + 8
 
 
 @pytest.mark.parametrize("kw", [dict(dtype=3), dict(heads=0), dict(groups=0), dict(groups=3), dict(heads=8192, groups=2), dict(key=0), dict(key=129),
@@ -187,7 +187,7 @@ def test_c_attention_sizes(kw):
     assert lib.boa_linear_attention_work_bytes(s, 0) == -1 and lib.boa_linear_attention_work_bytes(s, 1) == -1
     big = ctypes.c_void_p(16)
     assert lib.boa_linear_attention_fwd(s, big, 1 << 62, None) == _native.BOA_ERR_ARG
-    assert lib.boa_linear_attention_bwd(s, big, 1 << 62, big, 1 << 62, None) == _native.BOA_ERR_ARG
+    assert lib.boa_linear_attention_bwd(s, big, 1 << 62, None) == _native.BOA_ERR_ARG
     assert lib.boa_linear_attention_step(s, None) == _native.BOA_ERR_ARG
 
 
@@ -197,15 +197,17 @@ def test_c_attention_pointers_and_workspaces():
     s = _packed(n=1, length=200)
     need, back = lib.boa_linear_attention_work_bytes(s, 0), lib.boa_linear_attention_work_bytes(s, 1)
     assert 0 < need < back
-    for bad in (_packed(p=0), _packed(decay=0)):
+    assert lib.boa_linear_attention_bwd(_packed(marks=0), big, 1 << 62, None) == _native.BOA_ERR_ARG
+    assert lib.boa_linear_attention_marks_bytes(_packed(n=1, length=200)) == 4 * 4 * 4 * 64 * 64
+    assert lib.boa_linear_attention_marks_bytes(_packed(dtype=3)) == -1
+    for bad in (_packed(p=0), _packed(decay=0), _packed(marks=8)):
         assert lib.boa_linear_attention_fwd(bad, big, 1 << 62, None) == _native.BOA_ERR_ARG
-        assert lib.boa_linear_attention_bwd(bad, big, 1 << 62, big, 1 << 62, None) == _native.BOA_ERR_ARG
-    assert lib.boa_linear_attention_bwd(_packed(ddecay=0), big, 1 << 62, big, 1 << 62, None) == _native.BOA_ERR_ARG
+        assert lib.boa_linear_attention_bwd(bad, big, 1 << 62, None) == _native.BOA_ERR_ARG
+    assert lib.boa_linear_attention_bwd(_packed(ddecay=0), big, 1 << 62, None) == _native.BOA_ERR_ARG
     for work, size in ((None, need), (big, need - 1), (odd, need)):
         assert lib.boa_linear_attention_fwd(s, work, size, None) == _native.BOA_ERR_ARG
-        assert lib.boa_linear_attention_bwd(s, work, size, big, back, None) == _native.BOA_ERR_ARG
     for work, size in ((None, back), (big, back - 1), (odd, back)):
-        assert lib.boa_linear_attention_bwd(s, big, need, work, size, None) == _native.BOA_ERR_ARG
+        assert lib.boa_linear_attention_bwd(s, work, size, None) == _native.BOA_ERR_ARG
     assert lib.boa_linear_attention_step(_packed(length=2, state_out=16), None) == _native.BOA_ERR_ARG
     assert lib.boa_linear_attention_step(_packed(length=1), None) == _native.BOA_ERR_ARG
     assert lib.boa_linear_attention_fwd(None, big, 0, None) == _native.BOA_ERR_ARG
