@@ -96,6 +96,13 @@ template <int DT> struct Mat {
         f[0] = Frag{x[0], x[1], x[2], x[3]};
     }
     static __device__ __forceinline__ floatx4 load4(const E* p) { return *reinterpret_cast<const floatx4*>(p); }
+    static __device__ __forceinline__ float value(E v) { return v; }
+    // zeros in the place of infinities and NaN
+    static __device__ __forceinline__ Frag finite(Frag f) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) f[i] = __builtin_isfinite(f[i]) ? f[i] : 0.0f;
+        return f;
+    }
 };
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 // What is left of f behind its part hi; nothing behind an infinite one.
@@ -153,6 +160,13 @@ template <> struct Mat<DT_BF16> {
         ld_vec<DT_BF16, 4>(p, v);
         return floatx4{v[0], v[1], v[2], v[3]};
     }
+    static __device__ __forceinline__ float value(E v) { return Elem<DT_BF16>::ld(v); }
+    static __device__ __forceinline__ Frag finite(const Frag& f) {
+        u32x4 w = __builtin_bit_cast(u32x4, f);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] &= ((w[i] & 0x7F80u) != 0x7F80u ? 0xFFFFu : 0u) | ((w[i] & 0x7F800000u) != 0x7F800000u ? 0xFFFF0000u : 0u);
+        return __builtin_bit_cast(Frag, w);
+    }
 };
 // Step s of a product over 64 positions whose second operand is in registers, four tiles of 16 rows.
 template <class M, int PARTS>
@@ -169,96 +183,46 @@ __device__ __forceinline__ bool has(int s, int first, int last) {
     return s * T <= last && s * T + T - 1 >= first;
 }
 
-// Infinities and NaN of a first operand that meet a second one which is held in parts, or is zero where a position may not be reached:
-// zero times those would be NaN.  They are left out of the product (`finite`), and added as what they are: products of ones count
-// those of each sign that meet a factor of each sign.  Whatever they do not reach keeps its bits.
-template <class M>
-struct Odd {
-    floatx4 up = {0.0f, 0.0f, 0.0f, 0.0f}, down = up, nan = up;
-    static __device__ __forceinline__ typename M::Frag finite(const typename M::Frag& f) {
-        float x[M::VEC];
-        M::widen(f, x);
+// Row k (the same for all lanes) of the lane's column of a register operand of four tiles.
+__device__ __forceinline__ float row_of_tiles(const floatx4 (&t)[4], int k, int lane) {
+    float x = 0.0f;
 #pragma unroll
-        for (int e = 0; e < M::VEC; ++e) x[e] = __builtin_isfinite(x[e]) ? x[e] : 0.0f;
-        typename M::Frag r[1];
-        M::template split<1>(x, r);
-        return r[0];
-    }
-    // a: the first operand; w: the second's values, of which `in` count
-    __device__ __forceinline__ void step(const typename M::Frag& a, const float (&w)[M::VEC], const bool (&in)[M::VEC]) {
-        float x[M::VEC];
-        M::widen(a, x);
-        const auto count = [&](auto of, auto to, floatx4 c) {
-            typename M::Frag fo[1], ft[1];
-            float y[M::VEC], z[M::VEC];
-#pragma unroll
-            for (int e = 0; e < M::VEC; ++e) y[e] = of(x[e]) ? 1.0f : 0.0f, z[e] = in[e] && to(w[e]) ? 1.0f : 0.0f;
-            M::template split<1>(y, fo);
-            M::template split<1>(z, ft);
-            return M::mma(fo[0], ft[0], c);
-        };
-        const auto above = [](float f) { return f == __builtin_huge_valf(); };
-        const auto below = [](float f) { return f == -__builtin_huge_valf(); };
-        const auto plus = [](float f) { return f > 0.0f; };
-        const auto minus = [](float f) { return f < 0.0f; };
-        up = count(below, minus, count(above, plus, up));
-        down = count(above, minus, count(below, plus, down));
-        nan = count([](float f) { return f != f; }, [](float) { return true; }, nan);
-        nan = count([](float f) { return __builtin_isinf(f); }, [](float f) { return !(f > 0.0f) && !(f < 0.0f); }, nan);
-    }
-    __device__ __forceinline__ void add_to(floatx4& v) const {
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            if (up[r] > 0.0f) v[r] += __builtin_huge_valf();
-            if (down[r] > 0.0f) v[r] -= __builtin_huge_valf();
-            if (nan[r] > 0.0f) v[r] = __builtin_nanf("");
-        }
-    }
-};
+    for (int i = 0; i < 16; ++i)
+        if ((k >> 4) * 4 + (k & 3) == i) x = t[i / 4][i % 4];
+    return __shfl(x, 16 * ((k >> 2) & 3) + (lane & 15), 64);
+}
 
-// acc[ta] += A B over 64 positions k: A's rows from a0 on, held across in LDS; B (16 columns) in registers, four tiles of 16 k, of which
+// acc[ta] += A B over 64 positions k: A's rows from 0 on, held across in LDS; B (16 columns) in registers, four tiles of 16 k, of which
 // those from `first` to `last` are not all zero.  inside(k) says whether B's k of this lane's column counts; B is zero where it
-// does not, and where A is not `finite` its zeros are kept apart.
+// does not.  If A has infinities or NaN (it is not `finite`), those times such zeros would be NaN, and a position would reach others
+// that it comes behind: they are left out of the product and added one by one, so that whatever they do not reach keeps its bits.
 template <class M, int PARTS, int TA, class F>
-__device__ __forceinline__ void product_within(floatx4 (&acc)[TA], bool finite, const typename M::E* a, int lda, int a0, const floatx4 (&b)[4],
+__device__ __forceinline__ void product_within(floatx4 (&acc)[TA], bool finite, const typename M::E* a, int lda, const floatx4 (&b)[4],
                                                int first, int last, int lane, F inside) {
-    using Frag = typename M::Frag;
-    if (finite) {
 #pragma unroll
-        for (int s = 0; s < CHUNK / M::STEP; ++s) {
-            if (!has<M>(s, first, last)) continue;
-            Frag fb[PARTS];
-            registers<M, PARTS>(b, s, fb);
+    for (int s = 0; s < CHUNK / M::STEP; ++s) {
+        if (!has<M>(s, first, last)) continue;
+        typename M::Frag fb[PARTS];
+        registers<M, PARTS>(b, s, fb);
 #pragma unroll
-            for (int i = 0; i < TA; ++i) {
-                const Frag fa = M::mixed(a, lda, a0 + 16 * i, s * M::STEP, lane);
+        for (int i = 0; i < TA; ++i) {
+            typename M::Frag fa = M::mixed(a, lda, 16 * i, s * M::STEP, lane);
+            if (!finite) fa = M::finite(fa);
 #pragma unroll
-                for (int p = 0; p < PARTS; ++p) acc[i] = M::mma(fa, fb[p], acc[i]);
-            }
+            for (int p = 0; p < PARTS; ++p) acc[i] = M::mma(fa, fb[p], acc[i]);
         }
-        return;
     }
+    if (finite) return;
+#pragma unroll 1
+    for (int k = 16 * first; k < 16 * last + 16; ++k) {
+        const float w = row_of_tiles(b, k, lane);
+        const bool in = inside(k);
 #pragma unroll
-    for (int i = 0; i < TA; ++i) {
-        Odd<M> odd;
+        for (int i = 0; i < TA; ++i) {
+            const floatx4 x = M::load4(a + k * lda + 16 * i + 4 * (lane >> 4));
 #pragma unroll
-        for (int s = 0; s < CHUNK / M::STEP; ++s) {
-            if (!has<M>(s, first, last)) continue;
-            Frag fb[PARTS];
-            registers<M, PARTS>(b, s, fb);
-            const Frag fa = M::mixed(a, lda, a0 + 16 * i, s * M::STEP, lane), clean = Odd<M>::finite(fa);
-            float w[M::VEC];
-            bool in[M::VEC];
-#pragma unroll
-            for (int e = 0; e < M::VEC; ++e) {
-                w[e] = b[s * (M::VEC / 4) + e / 4][e % 4];
-                in[e] = inside(s * M::STEP + 16 * (e / 4) + 4 * (lane >> 4) + e % 4);
-            }
-#pragma unroll
-            for (int p = 0; p < PARTS; ++p) acc[i] = M::mma(clean, fb[p], acc[i]);
-            odd.step(fa, w, in);
+            for (int r = 0; r < 4; ++r) acc[i][r] = in && !__builtin_isfinite(x[r]) ? __builtin_fmaf(x[r], w, acc[i][r]) : acc[i][r];
         }
-        odd.add_to(acc[i]);
     }
 }
 
@@ -283,16 +247,24 @@ template <int DT, int COLS>
 struct Tile {
     using M = Mat<DT>;
     using T = typename Elem<DT>::T;
-    static constexpr int V = wide<DT>(), PER = CHUNK * COLS / (WG * V), ROW = COLS / V, LD = COLS + M::PAD, SIZE = CHUNK * LD;
+    static constexpr int V = wide<DT>(), PER = CHUNK * COLS / (WG * V), ROW = COLS / V;  // accesses of a thread, of a row
+    static_assert(WG % ROW == 0, "");
+    static constexpr int LD = COLS + M::PAD, SIZE = CHUNK * LD;
     u32x4 v[PER];
     // rows from p on, `rows` and `cols` of them
     __device__ __forceinline__ void load(const T* p, int64_t stride, int rows, int cols, bool wide16) {
+        const int r0 = threadIdx.x / ROW, c = threadIdx.x % ROW * V;  // WG / ROW rows apart
+        p += r0 * stride + c;
+        if (wide16 && rows == CHUNK && cols == COLS) {
+#pragma unroll
+            for (int i = 0; i < PER; ++i) v[i] = *reinterpret_cast<const u32x4*>(p + i * (WG / ROW * stride));
+            return;
+        }
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
-            const int at = threadIdx.x + i * WG, r = at / ROW, c = at % ROW * V;
             v[i] = u32x4{0u, 0u, 0u, 0u};
-            if (r < rows && c < cols) {
-                const T* q = p + r * stride + c;
+            if (r0 + i * (WG / ROW) < rows && c < cols) {
+                const T* q = p + i * (WG / ROW * stride);
                 if (wide16) {
                     v[i] = *reinterpret_cast<const u32x4*>(q);
                 } else {
@@ -346,10 +318,13 @@ struct Tile {
 
 // log2 of the decay from a chunk's start up to and with each position (lane), summed in 64 bits; a decay of zero (-inf) as
 // 2^-200, which is zero in float32 whatever it is multiplied with, so that differences stay numbers.
-__device__ __forceinline__ double decays(const Args& a, int64_t b, int h, int64_t t0, int rows, int lane) {
+__device__ __forceinline__ const float* decays_of(const Args& a, int64_t b, int h) {
+    return static_cast<const float*>(a.g.p) + b * a.g.bs + h * a.g.hs;
+}
+__device__ __forceinline__ double decays(const float* p, int64_t stride, int rows, int lane) {
     double g = 0.0;
     if (lane < rows) {
-        g = (double)static_cast<const float*>(a.g.p)[b * a.g.bs + (t0 + lane) * a.g.rs + h * a.g.hs] * LOG2E;
+        g = (double)p[lane * stride] * LOG2E;
         g = g < -200.0 ? -200.0 : g;
     }
     return scan(g);
@@ -434,7 +409,7 @@ struct State {
 // One step of a state's update over STEP positions: s += (y)^T (x weight), y's fragments given; x (tile [position][key]) of the
 // wavefront's own keys is weighted in registers.
 template <class M, int NP, int LDX>
-__device__ __forceinline__ void update(State<NP>& s, bool finite, const typename M::Frag (&fy)[State<NP>::TP], const typename M::E* tx,
+__device__ __forceinline__ void update(State<NP>& s, const typename M::Frag (&fy)[State<NP>::TP], const typename M::E* tx,
                                        const float* weight, int step, int lane, int wave) {
 #pragma unroll
     for (int j = 0; j < State<NP>::TN; ++j) {
@@ -448,25 +423,27 @@ __device__ __forceinline__ void update(State<NP>& s, bool finite, const typename
         }
         typename M::Frag fx[M::THREE];
         M::template split<M::THREE>(x, fx);
-        if (finite || M::THREE == 1) {
 #pragma unroll
-            for (int i = 0; i < State<NP>::TP; ++i)
+        for (int i = 0; i < State<NP>::TP; ++i)
 #pragma unroll
-                for (int p = 0; p < M::THREE; ++p) s.v[i][j] = M::mma(fy[i], fx[p], s.v[i][j]);
-        } else {
-            bool in[M::VEC];
+            for (int p = 0; p < M::THREE; ++p) s.v[i][j] = M::mma(fy[i], fx[p], s.v[i][j]);
+    }
+}
+// What infinities and NaN of y (tile [position][value]) add to it, where x's values are held in parts and zeros among these would make
+// NaN of all of them.
+template <class M, int NP, int LDX, int LDY>
+__device__ __forceinline__ void update_odd(State<NP>& s, const typename M::E* ty, const typename M::E* tx, const float* weight, int lane,
+                                           int wave) {
+#pragma unroll 1
+    for (int k = 0; k < CHUNK; ++k) {
+        float w[State<NP>::TN];
 #pragma unroll
-            for (int e = 0; e < M::VEC; ++e) in[e] = true;
+        for (int j = 0; j < State<NP>::TN; ++j) w[j] = weight[k] * M::value(tx[k * LDX + 64 * j + 16 * wave + (lane & 15)]);
+        s.each([&](int i, int j, floatx4& v) {
+            const floatx4 y = M::load4(ty + k * LDY + 16 * i + 4 * (lane >> 4));
 #pragma unroll
-            for (int i = 0; i < State<NP>::TP; ++i) {
-                const typename M::Frag clean = Odd<M>::finite(fy[i]);
-                Odd<M> odd;
-#pragma unroll
-                for (int p = 0; p < M::THREE; ++p) s.v[i][j] = M::mma(clean, fx[p], s.v[i][j]);
-                odd.step(fy[i], x, in);
-                odd.add_to(s.v[i][j]);
-            }
-        }
+            for (int r = 0; r < 4; ++r) v[r] = __builtin_isfinite(y[r]) ? v[r] : __builtin_fmaf(y[r], w[j], v[r]);
+        });
     }
 }
 template <int NP>
@@ -481,7 +458,7 @@ __device__ __forceinline__ void times(State<NP>& s, float f) {
 // A workgroup walks the chunks of a piece from a state of zeros, forward over k v^T or (BACK) from the last one over scale e^(G_i)
 // q dy^T; leaves what it ends with, and backward also what it reaches each chunk with.
 template <int DT, int NP, bool BACK>
-__global__ void __launch_bounds__(WG) k_attn_states(const Args a) {
+__global__ void __launch_bounds__(WG, 2) k_attn_states(const Args a) {
     using M = Mat<DT>;
     using TX = Tile<DT, NP>;
     using TY = Tile<DT, PV>;
@@ -506,12 +483,15 @@ __global__ void __launch_bounds__(WG) k_attn_states(const Args a) {
     TX x;
     TY y;
     double g = 0.0;
+    const auto* xp = row_of<DT>(X, b, 0, h / a.share);
+    const auto* yp = row_of<DT>(Y, b, 0, h) + tile * PV;
+    const float* gp = decays_of(a, b, h);
     const auto fetch = [&](int64_t c) {
         const int64_t t0 = c * CHUNK;
         const int rows = (int)min((int64_t)CHUNK, end - t0);
-        x.load(row_of<DT>(X, b, t0, h / a.share), X.rs, rows, a.key, wx);
-        y.load(row_of<DT>(Y, b, t0, h) + tile * PV, Y.rs, rows, vcols, wy);
-        g = decays(a, b, h, t0, rows, lane);
+        x.load(xp + t0 * X.rs, X.rs, rows, a.key, wx);
+        y.load(yp + t0 * Y.rs, Y.rs, rows, vcols, wy);
+        g = decays(gp + t0 * a.g.rs, a.g.rs, rows, lane);
     };
     const int64_t n = c1 - c0;
     if (n > 0) fetch(BACK ? c1 - 1 : c0);
@@ -525,7 +505,8 @@ __global__ void __launch_bounds__(WG) k_attn_states(const Args a) {
         x.store(tx);
         y.store(ty);
         if (wave == 0) weight[lane] = BACK ? a.scale * __builtin_amdgcn_exp2f((float)g) : __builtin_amdgcn_exp2f((float)(all - g));
-        const bool finite = __syncthreads_and(M::THREE == 1 || y.finite());
+        const bool odd = M::THREE > 1 && !__syncthreads_and(y.finite());
+        if (M::THREE == 1) __syncthreads();
         if (m + 1 < n) fetch(BACK ? c - 1 : c + 1);
         passed += all;
         times(s, __builtin_amdgcn_exp2f((float)all));
@@ -533,9 +514,13 @@ __global__ void __launch_bounds__(WG) k_attn_states(const Args a) {
         for (int k = 0; k < CHUNK / M::STEP; ++k) {
             typename M::Frag fy[S::TP];
 #pragma unroll
-            for (int i = 0; i < S::TP; ++i) fy[i] = M::mixed(ty, TY::LD, 16 * i, k * M::STEP, lane);
-            update<M, NP, TX::LD>(s, finite, fy, tx, weight, k, lane, wave);
+            for (int i = 0; i < S::TP; ++i) {
+                fy[i] = M::mixed(ty, TY::LD, 16 * i, k * M::STEP, lane);
+                if (odd) fy[i] = M::finite(fy[i]);
+            }
+            update<M, NP, TX::LD>(s, fy, tx, weight, k, lane, wave);
         }
+        if (odd) update_odd<M, NP, TX::LD, TY::LD>(s, ty, tx, weight, lane, wave);
         __syncthreads();
     }
     if (a.pieces > 1) {
@@ -612,7 +597,7 @@ struct FwdLds {
     static constexpr int BYTES = (int)sizeof(typename M::E) * (S + M::TWO * PART);
 };
 template <int DT, int NP>
-__global__ void __launch_bounds__(WG) k_attn_fwd(const Args a) {
+__global__ void __launch_bounds__(WG, DT == DT_F32 && NP == 128 ? 1 : 2) k_attn_fwd(const Args a) {
     using M = Mat<DT>;
     using E = typename M::E;
     using Frag = typename M::Frag;
@@ -646,13 +631,19 @@ __global__ void __launch_bounds__(WG) k_attn_fwd(const Args a) {
     TN q, k;
     TV v;
     double g = 0.0;
+    const auto* qp = row_of<DT>(a.q, b, 0, h / a.share);
+    const auto* kp = row_of<DT>(a.k, b, 0, h / a.share);
+    const auto* vp = row_of<DT>(a.v, b, 0, h) + tile * PV;
+    const float* gp = decays_of(a, b, h);
+    auto* yp = row_of<DT>(a.y, b, 0, h) + tile * PV;
+    float* marks = a.marks == nullptr ? nullptr : a.marks + bht * a.chunks * S::SIZE;
     const auto fetch = [&](int64_t c) {
         const int64_t t0 = c * CHUNK;
         const int rows = (int)min((int64_t)CHUNK, end - t0);
-        q.load(row_of<DT>(a.q, b, t0, h / a.share), a.q.rs, rows, a.key, a.wide & W_Q);
-        k.load(row_of<DT>(a.k, b, t0, h / a.share), a.k.rs, rows, a.key, a.wide & W_K);
-        v.load(row_of<DT>(a.v, b, t0, h) + tile * PV, a.v.rs, rows, vcols, a.wide & W_V);
-        g = decays(a, b, h, t0, rows, lane);
+        q.load(qp + t0 * a.q.rs, a.q.rs, rows, a.key, a.wide & W_Q);
+        k.load(kp + t0 * a.k.rs, a.k.rs, rows, a.key, a.wide & W_K);
+        v.load(vp + t0 * a.v.rs, a.v.rs, rows, vcols, a.wide & W_V);
+        g = decays(gp + t0 * a.g.rs, a.g.rs, rows, lane);
     };
     if (c0 < c1) fetch(c0);
     for (int64_t c = c0; c < c1; ++c) {
@@ -668,7 +659,7 @@ __global__ void __launch_bounds__(WG) k_attn_fwd(const Args a) {
             weight[lane] = __builtin_amdgcn_exp2f((float)(all - g));
         }
         const bool finite = __syncthreads_and(v.finite());
-        if (a.marks != nullptr) s.store(a.marks + (bht * a.chunks + c) * S::SIZE, lane, wave);
+        if (marks != nullptr) s.store(marks + c * S::SIZE, lane, wave);
         if (c + 1 < c1) fetch(c + 1);
 
         // q . k of all positions j (rows) and the own ones (columns), and what the state gives
@@ -700,12 +691,15 @@ __global__ void __launch_bounds__(WG) k_attn_fwd(const Args a) {
                     A[t][r] = j <= i && i < rows ? A[t][r] * (a.scale * fall_between(gi, G[j])) : 0.0f;
                 }
         times(s, __builtin_amdgcn_exp2f((float)all));
-        if (!finite) product_within<M, M::TWO>(y, false, tv, TV::LD, 0, A, 0, own, lane, [&](int j) { return j <= i && i < rows; });
+        if (!finite) product_within<M, M::TWO>(y, false, tv, TV::LD, A, 0, own, lane, [&](int j) { return j <= i && i < rows; });
 #pragma unroll
         for (int k = 0; k < CHUNK / M::STEP; ++k) {
             Frag fv[S::TP];
 #pragma unroll
-            for (int p = 0; p < S::TP; ++p) fv[p] = M::mixed(tv, TV::LD, 16 * p, k * M::STEP, lane);
+            for (int p = 0; p < S::TP; ++p) {
+                fv[p] = M::mixed(tv, TV::LD, 16 * p, k * M::STEP, lane);
+                if (!finite && M::THREE > 1) fv[p] = M::finite(fv[p]);
+            }
             if (finite && has<M>(k, 0, own)) {
                 Frag fa[M::TWO];
                 registers<M, M::TWO>(A, k, fa);
@@ -714,10 +708,11 @@ __global__ void __launch_bounds__(WG) k_attn_fwd(const Args a) {
 #pragma unroll
                     for (int x = 0; x < M::TWO; ++x) y[p] = M::mma(fv[p], fa[x], y[p]);
             }
-            update<M, NP, TN::LD>(s, finite, fv, tk, weight, k, lane, wave);
+            update<M, NP, TN::LD>(s, fv, tk, weight, k, lane, wave);
         }
+        if (!finite && M::THREE > 1) update_odd<M, NP, TN::LD, TV::LD>(s, tv, tk, weight, lane, wave);
         if (i < rows) {
-            auto* out = row_of<DT>(a.y, b, t0 + i, h) + tile * PV;
+            auto* out = yp + (t0 + i) * a.y.rs;
 #pragma unroll
             for (int p = 0; p < S::TP; ++p) write4<DT>(out, 16 * p + row4, vcols, a.wide & W_Y, y[p]);
         }
@@ -751,7 +746,7 @@ struct BwdLds {
     static constexpr int BYTES = (int)sizeof(typename M::E) * (D + Tile<DT, PV>::SIZE);
 };
 template <int DT, int NP>
-__global__ void __launch_bounds__(WG) k_attn_bwd(const Args a) {
+__global__ void __launch_bounds__(WG, 2) k_attn_bwd(const Args a) {
     using M = Mat<DT>;
     using E = typename M::E;
     using Frag = typename M::Frag;
@@ -808,7 +803,7 @@ __global__ void __launch_bounds__(WG) k_attn_bwd(const Args a) {
         q.load(row_of<DT>(a.q, b, t0, h / a.share), a.q.rs, rows, a.key, a.wide & W_Q);
         k.load(row_of<DT>(a.k, b, t0, h / a.share), a.k.rs, rows, a.key, a.wide & W_K);
         if (a.pieces > 1) ds.add(a.starts + (bht * a.pieces + c / a.per_piece) * S::SIZE, a.pre[bh * a.chunks + c], lane, own);
-        const double g = decays(a, b, h, t0, rows, lane);
+        const double g = decays(decays_of(a, b, h) + t0 * a.g.rs, a.g.rs, rows, lane);
         if (own == 0) G[lane] = in_two(g);
         v.store(tv);
         d.store(td);
@@ -899,7 +894,7 @@ __global__ void __launch_bounds__(WG) k_attn_bwd(const Args a) {
                 }
         at = over_rows(at);
         if (lane < 16) pairs[me] = at;
-        product_within<M, M::TWO>(dq, finite, tk, TN::LD, 0, dA, 0, own, lane, [&](int j) { return j <= me && me < rows; });
+        product_within<M, M::TWO>(dq, finite, tk, TN::LD, dA, 0, own, lane, [&](int j) { return j <= me && me < rows; });
         if (me < rows) {
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
@@ -938,8 +933,8 @@ __global__ void __launch_bounds__(WG) k_attn_bwd(const Args a) {
                     dA[t][r] = in ? dA[t][r] * w : 0.0f;
                 }
         const auto inside = [&](int i) { return i >= me && i < rows; };
-        product_within<M, M::TWO>(dk, finite, tq, TN::LD, 0, dA, own, 3, lane, inside);
-        product_within<M, M::TWO>(dv, finite, td, TV::LD, 0, A, own, 3, lane, inside);
+        product_within<M, M::TWO>(dk, finite, tq, TN::LD, dA, own, 3, lane, inside);
+        product_within<M, M::TWO>(dv, finite, td, TV::LD, A, own, 3, lane, inside);
         if (me < rows) {
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
