@@ -321,13 +321,11 @@ struct Tile {
 __device__ __forceinline__ const float* decays_of(const Args& a, int64_t b, int h) {
     return static_cast<const float*>(a.g.p) + b * a.g.bs + h * a.g.hs;
 }
-__device__ __forceinline__ double decays(const float* p, int64_t stride, int rows, int lane) {
-    double g = 0.0;
-    if (lane < rows) {
-        g = (double)p[lane * stride] * LOG2E;
-        g = g < -200.0 ? -200.0 : g;
-    }
-    return scan(g);
+// a position's own, and from it the sum
+__device__ __forceinline__ float decay_at(const float* p, int64_t stride, int rows, int lane) { return lane < rows ? p[lane * stride] : 0.0f; }
+__device__ __forceinline__ double decays(float own) {
+    const double g = (double)own * LOG2E;
+    return scan(g < -200.0 ? -200.0 : g);
 }
 __device__ __forceinline__ float2 in_two(double g) {
     const float hi = (float)g;
@@ -482,7 +480,7 @@ __global__ void __launch_bounds__(WG, 2) k_attn_states(const Args a) {
     double passed = 0.0;
     TX x;
     TY y;
-    double g = 0.0;
+    float g_own = 0.0f;
     const auto* xp = row_of<DT>(X, b, 0, h / a.share);
     const auto* yp = row_of<DT>(Y, b, 0, h) + tile * PV;
     const float* gp = decays_of(a, b, h);
@@ -491,7 +489,7 @@ __global__ void __launch_bounds__(WG, 2) k_attn_states(const Args a) {
         const int rows = (int)min((int64_t)CHUNK, end - t0);
         x.load(xp + t0 * X.rs, X.rs, rows, a.key, wx);
         y.load(yp + t0 * Y.rs, Y.rs, rows, vcols, wy);
-        g = decays(gp + t0 * a.g.rs, a.g.rs, rows, lane);
+        g_own = decay_at(gp + t0 * a.g.rs, a.g.rs, rows, lane);
     };
     const int64_t n = c1 - c0;
     if (n > 0) fetch(BACK ? c1 - 1 : c0);
@@ -501,7 +499,7 @@ __global__ void __launch_bounds__(WG, 2) k_attn_states(const Args a) {
             s.store(marks + c * S::SIZE, lane, wave);
             if (a.pieces > 1 && tile == 0 && threadIdx.x == 0) a.pre[bh * a.chunks + c] = __builtin_amdgcn_exp2f((float)passed);
         }
-        const double all = last_lane(g);
+        const double g = decays(g_own), all = last_lane(g);
         x.store(tx);
         y.store(ty);
         if (wave == 0) weight[lane] = BACK ? a.scale * __builtin_amdgcn_exp2f((float)g) : __builtin_amdgcn_exp2f((float)(all - g));
@@ -630,7 +628,7 @@ __global__ void __launch_bounds__(WG, DT == DT_F32 && NP == 128 ? 1 : 2) k_attn_
     else if (a.state_in != nullptr) s.from_caller(a.state_in + bh * a.key * a.value, a.key, a.value, tile * PV, lane, wave);
     TN q, k;
     TV v;
-    double g = 0.0;
+    float g_own = 0.0f;
     const auto* qp = row_of<DT>(a.q, b, 0, h / a.share);
     const auto* kp = row_of<DT>(a.k, b, 0, h / a.share);
     const auto* vp = row_of<DT>(a.v, b, 0, h) + tile * PV;
@@ -643,13 +641,13 @@ __global__ void __launch_bounds__(WG, DT == DT_F32 && NP == 128 ? 1 : 2) k_attn_
         q.load(qp + t0 * a.q.rs, a.q.rs, rows, a.key, a.wide & W_Q);
         k.load(kp + t0 * a.k.rs, a.k.rs, rows, a.key, a.wide & W_K);
         v.load(vp + t0 * a.v.rs, a.v.rs, rows, vcols, a.wide & W_V);
-        g = decays(gp + t0 * a.g.rs, a.g.rs, rows, lane);
+        g_own = decay_at(gp + t0 * a.g.rs, a.g.rs, rows, lane);
     };
     if (c0 < c1) fetch(c0);
     for (int64_t c = c0; c < c1; ++c) {
         const int64_t t0 = c * CHUNK;
         const int rows = (int)min((int64_t)CHUNK, end - t0);
-        const double all = last_lane(g);
+        const double g = decays(g_own), all = last_lane(g);
         q.store(tq);
         k.store(tk);
         v.store(tv);
@@ -803,7 +801,7 @@ __global__ void __launch_bounds__(WG, 2) k_attn_bwd(const Args a) {
         q.load(row_of<DT>(a.q, b, t0, h / a.share), a.q.rs, rows, a.key, a.wide & W_Q);
         k.load(row_of<DT>(a.k, b, t0, h / a.share), a.k.rs, rows, a.key, a.wide & W_K);
         if (a.pieces > 1) ds.add(a.starts + (bht * a.pieces + c / a.per_piece) * S::SIZE, a.pre[bh * a.chunks + c], lane, own);
-        const double g = decays(decays_of(a, b, h) + t0 * a.g.rs, a.g.rs, rows, lane);
+        const double g = decays(decay_at(decays_of(a, b, h) + t0 * a.g.rs, a.g.rs, rows, lane));
         if (own == 0) G[lane] = in_two(g);
         v.store(tv);
         d.store(td);
@@ -1085,7 +1083,7 @@ bool wide_rows(int dtype, const boa_heads& x, int cols) {
 }
 
 // The split: pieces of whole chunks, as many as give the wanted workgroups.
-constexpr int64_t WANTED = 512, WANTED_BACK = 1024;
+constexpr int64_t WANTED = 512;
 struct Plan {
     int np, tiles;
     int64_t chunks, bh;
@@ -1097,7 +1095,7 @@ struct Plan {
         chunks = ceil_div(s.length, CHUNK);
         bh = s.batch * s.heads;
         const int64_t each = bh * tiles;
-        int64_t n = each > 0 ? ceil_div(back ? WANTED_BACK : WANTED, each) : 1;
+        int64_t n = each > 0 ? ceil_div(WANTED, each) : 1;
         n = n < chunks ? n : chunks;
         per_piece = (int32_t)(n > 1 ? ceil_div(chunks, n) : chunks > 1 ? chunks : 1);
         pieces = (int32_t)(chunks > 1 ? ceil_div(chunks, per_piece) : 1);
