@@ -74,6 +74,7 @@ template <int DT> struct Mat {
     using E = float;
     using Frag = f32x4;
     static constexpr int STEP = 16, VEC = 4, TWO = 1, THREE = 1, PAD = 4;
+    static constexpr bool SKIP = true;  // tiles that are all zero are left out: the matrix cores bound it
     static __device__ __forceinline__ floatx4 mma(const Frag& a, const Frag& b, floatx4 c) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[i], b[i], c, 0, 0, 0);
@@ -114,6 +115,7 @@ template <> struct Mat<DT_BF16> {
     using E = uint16_t;
     using Frag = bf16x8;
     static constexpr int STEP = 32, VEC = 8, TWO = 2, THREE = 3, PAD = 8;
+    static constexpr bool SKIP = false;  // branches would cost more
     static __device__ __forceinline__ floatx4 mma(const Frag& a, const Frag& b, floatx4 c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
     }
@@ -176,13 +178,6 @@ __device__ __forceinline__ void registers(const floatx4 (&t)[4], int s, typename
     for (int e = 0; e < M::VEC; ++e) x[e] = t[s * (M::VEC / 4) + e / 4][e % 4];
     M::template split<PARTS>(x, f);
 }
-// Whether step s has anything of the tiles first .. last.
-template <class M>
-__device__ __forceinline__ bool has(int s, int first, int last) {
-    constexpr int T = M::VEC / 4;
-    return s * T <= last && s * T + T - 1 >= first;
-}
-
 // Row k (the same for all lanes) of the lane's column of a register operand of four tiles.
 __device__ __forceinline__ float row_of_tiles(const floatx4 (&t)[4], int k, int lane) {
     float x = 0.0f;
@@ -199,20 +194,22 @@ __device__ __forceinline__ float row_of_tiles(const floatx4 (&t)[4], int k, int 
 template <class M, int PARTS, int TA, class F>
 __device__ __forceinline__ void product_within(floatx4 (&acc)[TA], bool finite, const typename M::E* a, int lda, const floatx4 (&b)[4],
                                                int first, int last, int lane, F inside) {
+    const auto all = [&](auto clean) {
 #pragma unroll
-    for (int s = 0; s < CHUNK / M::STEP; ++s) {
-        if (!has<M>(s, first, last)) continue;
-        typename M::Frag fb[PARTS];
-        registers<M, PARTS>(b, s, fb);
+        for (int s = 0; s < CHUNK / M::STEP; ++s) {
+            if (M::SKIP && (s < first || s > last)) continue;  // a step is a tile there
+            typename M::Frag fb[PARTS];
+            registers<M, PARTS>(b, s, fb);
 #pragma unroll
-        for (int i = 0; i < TA; ++i) {
-            typename M::Frag fa = M::mixed(a, lda, 16 * i, s * M::STEP, lane);
-            if (!finite) fa = M::finite(fa);
+            for (int i = 0; i < TA; ++i) {
+                const typename M::Frag fa = clean(M::mixed(a, lda, 16 * i, s * M::STEP, lane));
 #pragma unroll
-            for (int p = 0; p < PARTS; ++p) acc[i] = M::mma(fa, fb[p], acc[i]);
+                for (int p = 0; p < PARTS; ++p) acc[i] = M::mma(fa, fb[p], acc[i]);
+            }
         }
-    }
-    if (finite) return;
+    };
+    if (finite) return all([](const typename M::Frag& f) { return f; });
+    all([](const typename M::Frag& f) { return M::finite(f); });
 #pragma unroll 1
     for (int k = 16 * first; k < 16 * last + 16; ++k) {
         const float w = row_of_tiles(b, k, lane);
@@ -223,6 +220,21 @@ __device__ __forceinline__ void product_within(floatx4 (&acc)[TA], bool finite, 
 #pragma unroll
             for (int r = 0; r < 4; ++r) acc[i][r] = in && !__builtin_isfinite(x[r]) ? __builtin_fmaf(x[r], w, acc[i][r]) : acc[i][r];
         }
+    }
+}
+// The products of 16 columns (rows `own` .. of b) with the tiles from `first` to `last` of a's rows, both held along K.
+template <class M, int K>
+__device__ __forceinline__ void scores(floatx4 (&acc)[4], const typename M::E* a, const typename M::E* b, int ld, int own, int first, int last,
+                                       int lane) {
+    typename M::Frag fb[K / M::STEP];
+#pragma unroll
+    for (int s = 0; s < K / M::STEP; ++s) fb[s] = M::row(b, ld, own, s * M::STEP, lane);
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+        acc[t] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+        if (M::SKIP && (t < first || t > last)) continue;
+#pragma unroll
+        for (int s = 0; s < K / M::STEP; ++s) acc[t] = M::mma(M::row(a, ld, 16 * t, s * M::STEP, lane), fb[s], acc[t]);
     }
 }
 
@@ -333,6 +345,34 @@ __device__ __forceinline__ float2 in_two(double g) {
 }
 // 2^(a - b)
 __device__ __forceinline__ float fall_between(float2 a, float2 b) { return __builtin_amdgcn_exp2f((a.x - b.x) + (a.y - b.y)); }
+// The sums of a chunk's logarithms in LDS, in two parts.
+struct Falls {
+    float x[CHUNK], y[CHUNK];
+    __device__ __forceinline__ void put(int i, float2 g) { x[i] = g.x, y[i] = g.y; }
+    __device__ __forceinline__ float2 at(int i) const { return make_float2(x[i], y[i]); }
+};
+// The factors between the own position and the four rows of each tile that a lane has: of the own one behind them, or of them behind it.
+template <bool OWN_BEHIND>
+__device__ __forceinline__ void falls(const Falls& g, float2 own, float scale, int lane, floatx4 (&f)[4]) {
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+        const f32x4 x = *reinterpret_cast<const f32x4*>(g.x + 16 * t + 4 * (lane >> 4)), y = *reinterpret_cast<const f32x4*>(g.y + 16 * t + 4 * (lane >> 4));
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const float2 o = make_float2(x[r], y[r]);
+            f[t][r] = scale * (OWN_BEHIND ? fall_between(own, o) : fall_between(o, own));
+        }
+    }
+}
+// Whether any value that the workgroup's threads have is not finite, by way of a barrier: each wavefront says so in LDS.
+__device__ __forceinline__ void say_finite(int* said, bool finite, int lane, int wave) {
+    const bool all = __ballot(!finite) == 0;
+    if (lane == 0) said[wave] = all;
+}
+__device__ __forceinline__ bool heard_finite(const int* said) {
+    const int all = said[0] & said[1] & said[2] & said[3];
+    return __builtin_amdgcn_readfirstlane(all) != 0;
+}
 
 __device__ __forceinline__ int64_t end_of(const Args& a, int64_t b) {
     if (a.lens == nullptr) return a.length;
@@ -464,6 +504,7 @@ __global__ void __launch_bounds__(WG, 2) k_attn_states(const Args a) {
     __shared__ __attribute__((aligned(16))) typename M::E tx[TX::SIZE];
     __shared__ __attribute__((aligned(16))) typename M::E ty[TY::SIZE];
     __shared__ __attribute__((aligned(16))) float weight[CHUNK];
+    __shared__ int said[WAVES];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int piece = (int)(blockIdx.x % a.pieces), tile = (int)(blockIdx.x / a.pieces % a.tiles);
     const int64_t bh = blockIdx.x / a.pieces / a.tiles, b = bh / a.heads;
@@ -503,22 +544,27 @@ __global__ void __launch_bounds__(WG, 2) k_attn_states(const Args a) {
         x.store(tx);
         y.store(ty);
         if (wave == 0) weight[lane] = BACK ? a.scale * __builtin_amdgcn_exp2f((float)g) : __builtin_amdgcn_exp2f((float)(all - g));
-        const bool odd = M::THREE > 1 && !__syncthreads_and(y.finite());
-        if (M::THREE == 1) __syncthreads();
+        if constexpr (M::THREE > 1) say_finite(said, y.finite(), lane, wave);
+        __syncthreads();
+        const bool finite = M::THREE == 1 || heard_finite(said);
         if (m + 1 < n) fetch(BACK ? c - 1 : c + 1);
         passed += all;
         times(s, __builtin_amdgcn_exp2f((float)all));
+        const auto all_steps = [&](auto clean) {
 #pragma unroll
-        for (int k = 0; k < CHUNK / M::STEP; ++k) {
-            typename M::Frag fy[S::TP];
+            for (int k = 0; k < CHUNK / M::STEP; ++k) {
+                typename M::Frag fy[S::TP];
 #pragma unroll
-            for (int i = 0; i < S::TP; ++i) {
-                fy[i] = M::mixed(ty, TY::LD, 16 * i, k * M::STEP, lane);
-                if (odd) fy[i] = M::finite(fy[i]);
+                for (int i = 0; i < S::TP; ++i) fy[i] = clean(M::mixed(ty, TY::LD, 16 * i, k * M::STEP, lane));
+                update<M, NP, TX::LD>(s, fy, tx, weight, k, lane, wave);
             }
-            update<M, NP, TX::LD>(s, fy, tx, weight, k, lane, wave);
+        };
+        if (finite) {
+            all_steps([](const typename M::Frag& f) { return f; });
+        } else {
+            all_steps([](const typename M::Frag& f) { return M::finite(f); });
+            update_odd<M, NP, TX::LD, TY::LD>(s, ty, tx, weight, lane, wave);
         }
-        if (odd) update_odd<M, NP, TX::LD, TY::LD>(s, ty, tx, weight, lane, wave);
         __syncthreads();
     }
     if (a.pieces > 1) {
@@ -595,7 +641,7 @@ struct FwdLds {
     static constexpr int BYTES = (int)sizeof(typename M::E) * (S + M::TWO * PART);
 };
 template <int DT, int NP>
-__global__ void __launch_bounds__(WG, DT == DT_F32 && NP == 128 ? 1 : 2) k_attn_fwd(const Args a) {
+__global__ void __launch_bounds__(WG, NP == 128 ? 1 : 2) k_attn_fwd(const Args a) {
     using M = Mat<DT>;
     using E = typename M::E;
     using Frag = typename M::Frag;
@@ -608,8 +654,9 @@ __global__ void __launch_bounds__(WG, DT == DT_F32 && NP == 128 ? 1 : 2) k_attn_
     E* tk = reinterpret_cast<E*>(lds) + L::K;
     E* tv = reinterpret_cast<E*>(lds) + L::V;
     E* ts = reinterpret_cast<E*>(lds) + L::S;  // [NP][PV] in two parts
-    __shared__ float2 G[CHUNK];
+    __shared__ __attribute__((aligned(16))) Falls G;
     __shared__ __attribute__((aligned(16))) float weight[CHUNK];
+    __shared__ int said[WAVES];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l15 = lane & 15, row4 = 4 * (lane >> 4);
     // a wavefront's own positions i: the later ones have more before them, so workgroups beside each other have them the other way round
     const int own = blockIdx.x & 1 ? WAVES - 1 - wave : wave;
@@ -643,6 +690,20 @@ __global__ void __launch_bounds__(WG, DT == DT_F32 && NP == 128 ? 1 : 2) k_attn_
         v.load(vp + t0 * a.v.rs, a.v.rs, rows, vcols, a.wide & W_V);
         g_own = decay_at(gp + t0 * a.g.rs, a.g.rs, rows, lane);
     };
+    // a chunk's results are written while the next one is on: what has been stored late would be waited for with the next tiles
+    floatx4 y[S::TP];
+    const auto write = [&](int64_t t0) {
+        const int64_t t = t0 + 16 * own + l15;
+        if (t >= end) return;
+        auto* out = yp + t * a.y.rs;
+        if ((a.wide & W_Y) && vcols == PV) {
+#pragma unroll
+            for (int p = 0; p < S::TP; ++p) write4<DT>(out, 16 * p + row4, PV, true, y[p]);
+        } else {
+#pragma unroll
+            for (int p = 0; p < S::TP; ++p) write4<DT>(out, 16 * p + row4, vcols, false, y[p]);
+        }
+    };
     if (c0 < c1) fetch(c0);
     for (int64_t c = c0; c < c1; ++c) {
         const int64_t t0 = c * CHUNK;
@@ -653,69 +714,78 @@ __global__ void __launch_bounds__(WG, DT == DT_F32 && NP == 128 ? 1 : 2) k_attn_
         v.store(tv);
         s.template put<M, M::TWO>(ts, a.key, vcols, lane, wave);
         if (wave == 0) {
-            G[lane] = in_two(g);
+            G.put(lane, in_two(g));
             weight[lane] = __builtin_amdgcn_exp2f((float)(all - g));
         }
-        const bool finite = __syncthreads_and(v.finite());
+        say_finite(said, v.finite(), lane, wave);
+        __syncthreads();
+        const bool finite = heard_finite(said);
+        if (c > c0) write(t0 - CHUNK);
         if (marks != nullptr) s.store(marks + c * S::SIZE, lane, wave);
         if (c + 1 < c1) fetch(c + 1);
 
         // q . k of all positions j (rows) and the own ones (columns), and what the state gives
-        floatx4 A[4] = {}, y[S::TP] = {};
+        floatx4 A[4], f[4];
+        scores<M, NP>(A, tk, tq, TN::LD, 16 * own, 0, own, lane);
+#pragma unroll
+        for (int p = 0; p < S::TP; ++p) y[p] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int n = 0; n < NP; n += M::STEP) {
             const Frag fq = M::row(tq, TN::LD, 16 * own, n, lane);
-#pragma unroll
-            for (int t = 0; t < 4; ++t)
-                if (t <= own) A[t] = M::mma(M::row(tk, TN::LD, 16 * t, n, lane), fq, A[t]);
 #pragma unroll
             for (int p = 0; p < S::TP; ++p)
 #pragma unroll
                 for (int i = 0; i < M::TWO; ++i) y[p] = M::mma(M::col(ts + i * L::PART, L::LDS_STATE, 16 * p, n, lane), fq, y[p]);
         }
         const int i = 16 * own + l15;
-        const float2 gi = G[i];
-        const float f = a.scale * __builtin_amdgcn_exp2f(gi.x + gi.y);
+        const float2 gi = G.at(i);
+        const float from_start = a.scale * __builtin_amdgcn_exp2f(gi.x + gi.y);
+        falls<true>(G, gi, a.scale, lane, f);
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int j = 16 * t + row4 + r;
+                const float x = A[t][r] * f[t][r];
+                A[t][r] = j <= i && i < rows ? x : 0.0f;
+            }
 #pragma unroll
         for (int p = 0; p < S::TP; ++p)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) y[p][r] *= f;
-#pragma unroll
-        for (int t = 0; t < 4; ++t)
-            if (t <= own)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const int j = 16 * t + row4 + r;
-                    A[t][r] = j <= i && i < rows ? A[t][r] * (a.scale * fall_between(gi, G[j])) : 0.0f;
-                }
+            for (int r = 0; r < 4; ++r) y[p][r] *= from_start;
         times(s, __builtin_amdgcn_exp2f((float)all));
-        if (!finite) product_within<M, M::TWO>(y, false, tv, TV::LD, A, 0, own, lane, [&](int j) { return j <= i && i < rows; });
+        if (finite) {
 #pragma unroll
-        for (int k = 0; k < CHUNK / M::STEP; ++k) {
-            Frag fv[S::TP];
+            for (int k = 0; k < CHUNK / M::STEP; ++k) {
+                Frag fv[S::TP], fa[M::TWO];
 #pragma unroll
-            for (int p = 0; p < S::TP; ++p) {
-                fv[p] = M::mixed(tv, TV::LD, 16 * p, k * M::STEP, lane);
-                if (!finite && M::THREE > 1) fv[p] = M::finite(fv[p]);
+                for (int p = 0; p < S::TP; ++p) fv[p] = M::mixed(tv, TV::LD, 16 * p, k * M::STEP, lane);
+                if (!M::SKIP || k <= own) {
+                    registers<M, M::TWO>(A, k, fa);
+#pragma unroll
+                    for (int p = 0; p < S::TP; ++p)
+#pragma unroll
+                        for (int x = 0; x < M::TWO; ++x) y[p] = M::mma(fv[p], fa[x], y[p]);
+                }
+                update<M, NP, TN::LD>(s, fv, tk, weight, k, lane, wave);
             }
-            if (finite && has<M>(k, 0, own)) {
-                Frag fa[M::TWO];
-                registers<M, M::TWO>(A, k, fa);
+        } else {
+            product_within<M, M::TWO>(y, false, tv, TV::LD, A, 0, own, lane, [&](int j) { return j <= i && i < rows; });
 #pragma unroll
-                for (int p = 0; p < S::TP; ++p)
+            for (int k = 0; k < CHUNK / M::STEP; ++k) {
+                Frag fv[S::TP];
 #pragma unroll
-                    for (int x = 0; x < M::TWO; ++x) y[p] = M::mma(fv[p], fa[x], y[p]);
+                for (int p = 0; p < S::TP; ++p) {
+                    fv[p] = M::mixed(tv, TV::LD, 16 * p, k * M::STEP, lane);
+                    if constexpr (M::THREE > 1) fv[p] = M::finite(fv[p]);
+                }
+                update<M, NP, TN::LD>(s, fv, tk, weight, k, lane, wave);
             }
-            update<M, NP, TN::LD>(s, fv, tk, weight, k, lane, wave);
-        }
-        if (!finite && M::THREE > 1) update_odd<M, NP, TN::LD, TV::LD>(s, tv, tk, weight, lane, wave);
-        if (i < rows) {
-            auto* out = yp + (t0 + i) * a.y.rs;
-#pragma unroll
-            for (int p = 0; p < S::TP; ++p) write4<DT>(out, 16 * p + row4, vcols, a.wide & W_Y, y[p]);
+            if constexpr (M::THREE > 1) update_odd<M, NP, TN::LD, TV::LD>(s, tv, tk, weight, lane, wave);
         }
         __syncthreads();
     }
+    if (c0 < c1) write((c1 - 1) * CHUNK);
     if (a.pieces == 1 && a.state_out != nullptr) s.to_caller(a.state_out + bh * a.key * a.value, a.key, a.value, tile * PV, lane, wave);
 }
 
@@ -758,8 +828,10 @@ __global__ void __launch_bounds__(WG, 2) k_attn_bwd(const Args a) {
     E* tk = reinterpret_cast<E*>(lds) + L::K;
     E* tv = reinterpret_cast<E*>(lds) + L::V;
     E* td = reinterpret_cast<E*>(lds) + L::D;  // dy
-    __shared__ float2 G[CHUNK];
-    __shared__ float pairs[CHUNK], middle[WAVES - 1][CHUNK], from_state[CHUNK], to_behind[CHUNK], through[WAVES];
+    __shared__ __attribute__((aligned(16))) Falls G;
+    __shared__ int said[WAVES];
+    __shared__ __attribute__((aligned(16))) float middle[WAVES - 1][CHUNK];
+    __shared__ float pairs[CHUNK], from_state[CHUNK], to_behind[CHUNK], through[WAVES];
     const int lane = threadIdx.x & 63, own = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l15 = lane & 15, row4 = 4 * (lane >> 4);
     const int64_t c = blockIdx.x % a.chunks, bht = blockIdx.x / a.chunks, bh = bht / a.tiles, b = bh / a.heads, t0 = c * CHUNK;
     const int tile = (int)(bht % a.tiles), h = (int)(bh % a.heads);
@@ -802,7 +874,7 @@ __global__ void __launch_bounds__(WG, 2) k_attn_bwd(const Args a) {
         k.load(row_of<DT>(a.k, b, t0, h / a.share), a.k.rs, rows, a.key, a.wide & W_K);
         if (a.pieces > 1) ds.add(a.starts + (bht * a.pieces + c / a.per_piece) * S::SIZE, a.pre[bh * a.chunks + c], lane, own);
         const double g = decays(decay_at(decays_of(a, b, h) + t0 * a.g.rs, a.g.rs, rows, lane));
-        if (own == 0) G[lane] = in_two(g);
+        if (own == 0) G.put(lane, in_two(g));
         v.store(tv);
         d.store(td);
         s.template put<M, M::THREE>(tq, a.key, vcols, lane, own);
@@ -818,10 +890,12 @@ __global__ void __launch_bounds__(WG, 2) k_attn_bwd(const Args a) {
                     if (S::n(j, lane, own) < a.key && S::p(i, lane) + r < vcols) x = __builtin_fmaf(s.v[i][j][r], ds.v[i][j][r], x);
         x = wsum(x);
         if (lane == 0) through[own] = x;
-        finite = __syncthreads_and(q.finite() && k.finite() && d.finite());
+        say_finite(said, q.finite() && k.finite() && d.finite(), lane, own);
+        __syncthreads();
+        finite = heard_finite(said);
     }
     const int me = 16 * own + l15;  // the own position, as i of dq and as j of dk and dv
-    const float2 mine = G[me], g_end = G[CHUNK - 1];
+    const float2 mine = G.at(me), g_end = G.at(CHUNK - 1);
     const float to_end = fall_between(g_end, mine), from_start = a.scale * __builtin_amdgcn_exp2f(mine.x + mine.y);
     floatx4 dq[NT] = {}, dk[NT] = {};
 #pragma unroll
@@ -858,38 +932,31 @@ __global__ void __launch_bounds__(WG, 2) k_attn_bwd(const Args a) {
     }
     // the own positions as i: rows are positions j before them
     {
-        floatx4 A[4] = {}, dA[4] = {};
-#pragma unroll
-        for (int n = 0; n < NP; n += M::STEP) {
-            const Frag f = M::row(tq, TN::LD, 16 * own, n, lane);
-#pragma unroll
-            for (int t = 0; t < 4; ++t)
-                if (t <= own) A[t] = M::mma(M::row(tk, TN::LD, 16 * t, n, lane), f, A[t]);
-        }
-#pragma unroll
-        for (int p = 0; p < PV; p += M::STEP) {
-            const Frag f = M::row(td, TV::LD, 16 * own, p, lane);
-#pragma unroll
-            for (int t = 0; t < 4; ++t)
-                if (t <= own) dA[t] = M::mma(M::row(tv, TV::LD, 16 * t, p, lane), f, dA[t]);
-        }
+        floatx4 A[4], dA[4], f[4];
+        scores<M, NP>(A, tk, tq, TN::LD, 16 * own, 0, own, lane);
+        scores<M, PV>(dA, tv, td, TV::LD, 16 * own, 0, own, lane);
+        falls<true>(G, mine, a.scale, lane, f);
         // the pairs that a position t of the own ones lies between: of M_ij the sum over the own i >= t, then over j < t; and all own i
         // for the positions of the tiles before
         float at = 0.0f;
 #pragma unroll
-        for (int t = 0; t < 4; ++t)
-            if (t <= own)
+        for (int t = 0; t < 4; ++t) {
+            if (t > own) continue;
+            floatx4 sums;
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const int j = 16 * t + row4 + r;
-                    const bool in = j <= me && me < rows;
-                    const float w = a.scale * fall_between(mine, G[j]);
-                    const float m = in ? A[t][r] * w * dA[t][r] : 0.0f;
-                    dA[t][r] = in ? dA[t][r] * w : 0.0f;
-                    const float sum = from_here(m);
-                    at += j < me ? sum : 0.0f;
-                    if (t < own && l15 == 0) middle[own - 1][j] = sum;
-                }
+            for (int r = 0; r < 4; ++r) {
+                const int j = 16 * t + row4 + r;
+                const bool in = j <= me && me < rows;
+                const float x = dA[t][r] * f[t][r], m = A[t][r] * x;
+                dA[t][r] = in ? x : 0.0f;
+                sums[r] = from_here(in ? m : 0.0f);
+                at += j < me ? sums[r] : 0.0f;
+            }
+            if (t < own && l15 == 0) *reinterpret_cast<floatx4*>(&middle[own - 1][16 * t + row4]) = sums;
+        }
+#pragma unroll
+        for (int t = 1; t < 4; ++t)
+            if (t > own) dA[t] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
         at = over_rows(at);
         if (lane < 16) pairs[me] = at;
         product_within<M, M::TWO>(dq, finite, tk, TN::LD, dA, 0, own, lane, [&](int j) { return j <= me && me < rows; });
@@ -904,32 +971,20 @@ __global__ void __launch_bounds__(WG, 2) k_attn_bwd(const Args a) {
     // the own positions as j: rows are positions i behind them
     floatx4 dv[S::TP] = {};
     {
-        floatx4 A[4] = {}, dA[4] = {};
-#pragma unroll
-        for (int n = 0; n < NP; n += M::STEP) {
-            const Frag f = M::row(tk, TN::LD, 16 * own, n, lane);
-#pragma unroll
-            for (int t = 0; t < 4; ++t)
-                if (t >= own) A[t] = M::mma(M::row(tq, TN::LD, 16 * t, n, lane), f, A[t]);
-        }
-#pragma unroll
-        for (int p = 0; p < PV; p += M::STEP) {
-            const Frag f = M::row(tv, TV::LD, 16 * own, p, lane);
-#pragma unroll
-            for (int t = 0; t < 4; ++t)
-                if (t >= own) dA[t] = M::mma(M::row(td, TV::LD, 16 * t, p, lane), f, dA[t]);
-        }
+        floatx4 A[4], dA[4], f[4];
+        scores<M, NP>(A, tq, tk, TN::LD, 16 * own, own, 3, lane);
+        scores<M, PV>(dA, td, tv, TV::LD, 16 * own, own, 3, lane);
+        falls<false>(G, mine, a.scale, lane, f);
 #pragma unroll
         for (int t = 0; t < 4; ++t)
-            if (t >= own)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const int i = 16 * t + row4 + r;
-                    const bool in = i >= me && i < rows;
-                    const float w = a.scale * fall_between(G[i], mine);
-                    A[t][r] = in ? A[t][r] * w : 0.0f;
-                    dA[t][r] = in ? dA[t][r] * w : 0.0f;
-                }
+            for (int r = 0; r < 4; ++r) {
+                const int i = 16 * t + row4 + r;
+                const bool in = i >= me && i < rows;
+                const float x = A[t][r] * f[t][r], y = dA[t][r] * f[t][r];
+                A[t][r] = in ? x : 0.0f;
+                dA[t][r] = in ? y : 0.0f;
+            }
         const auto inside = [&](int i) { return i >= me && i < rows; };
         product_within<M, M::TWO>(dk, finite, tq, TN::LD, dA, own, 3, lane, inside);
         product_within<M, M::TWO>(dv, finite, td, TV::LD, A, own, 3, lane, inside);
