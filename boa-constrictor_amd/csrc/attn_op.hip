@@ -254,6 +254,13 @@ __device__ __forceinline__ void put4(typename M::E* p, int part, floatx4 v) {
     }
 }
 
+// The same number (uniform), which the compiler takes for another one: what is computed from it stays where it is written.  Masks of
+// the columns that a head has would otherwise be made before a loop over chunks and be kept, more than there are scalar registers.
+__device__ __forceinline__ int here(int x) {
+    asm volatile("" : "+s"(x));
+    return x;
+}
+
 // A tile of CHUNK rows and COLS columns on its way from memory to LDS; zeros behind the last row and column.
 template <int DT, int COLS>
 struct Tile {
@@ -272,6 +279,7 @@ struct Tile {
             for (int i = 0; i < PER; ++i) v[i] = *reinterpret_cast<const u32x4*>(p + i * (WG / ROW * stride));
             return;
         }
+        cols = here(cols);
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
             v[i] = u32x4{0u, 0u, 0u, 0u};
@@ -434,6 +442,11 @@ struct State {
     template <class M, int PARTS>
     __device__ __forceinline__ void put(typename M::E* t, int key, int value, int lane, int wave) {
         constexpr int LD = PV + M::PAD;
+        if (key == NP && value == PV) {
+            each([&](int i, int j, floatx4& x) { put4<M, PARTS>(t + n(j, lane, wave) * LD + p(i, lane), NP * LD, x); });
+            return;
+        }
+        key = here(key), value = here(value);
         each([&](int i, int j, floatx4& x) {
             floatx4 y = x;
 #pragma unroll
@@ -701,7 +714,7 @@ __global__ void __launch_bounds__(WG, NP == 128 ? 1 : 2) k_attn_fwd(const Args a
             for (int p = 0; p < S::TP; ++p) write4<DT>(out, 16 * p + row4, PV, true, y[p]);
         } else {
 #pragma unroll
-            for (int p = 0; p < S::TP; ++p) write4<DT>(out, 16 * p + row4, vcols, false, y[p]);
+            for (int p = 0; p < S::TP; ++p) write4<DT>(out, 16 * p + row4, here(vcols), false, y[p]);
         }
     };
     if (c0 < c1) fetch(c0);
