@@ -52,11 +52,11 @@ struct Args {
     float* pre;     // backward: [batch heads][chunks] decay from the chunk's end to its piece's
     double* fall;   // [batch heads][pieces] log2 of the piece's decay
     const float* fmarks;     // backward: the forward's
-    float *part_q, *part_k;  // backward: [batch][length][heads * value tiles][key], or null: dq, dk are written
+    float *part_q, *part_k;  // backward: [batch][length][parts of each group][key], or null: dq, dk are written
     float* dg;               // backward: [value tiles][batch][length][heads], or null
     float* dg_sum;           // backward: [batch * chunks * value tiles][heads], or null
     int64_t batch, length, chunks;
-    int32_t heads, share, key, value, tiles, pieces, per_piece;
+    int32_t heads, share, in_turn, key, value, tiles, pieces, per_piece;
     float scale;
     uint32_t wide;  // bit per tensor: read or written 16 bytes at a time (W_*)
 };
@@ -261,6 +261,12 @@ __device__ __forceinline__ int here(int x) {
     return x;
 }
 
+// The same for a lane's number: addresses and masks that are made from it.
+__device__ __forceinline__ int here_lane(int x) {
+    asm volatile("" : "+v"(x));
+    return x;
+}
+
 // A tile of CHUNK rows and COLS columns on its way from memory to LDS; zeros behind the last row and column.
 template <int DT, int COLS>
 struct Tile {
@@ -296,22 +302,18 @@ struct Tile {
                         }
                 }
             }
+            __builtin_amdgcn_sched_barrier(0);  // else all elements' loads are on their way at once, in registers of their own
         }
     }
+    // An exponent of ones and one more carry into the sign's place.
     __device__ __forceinline__ bool finite() const {
-        bool ok = true;
+        constexpr uint32_t SIGNS = DT == DT_F32 ? 0x80000000u : 0x80008000u, ONE = DT == DT_F32 ? 0x00800000u : DT == DT_BF16 ? 0x00800080u : 0x04000400u;
+        uint32_t any = 0u;
 #pragma unroll
         for (int i = 0; i < PER; ++i)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                if constexpr (DT == DT_F32) {
-                    ok &= (v[i][e] & 0x7F800000u) != 0x7F800000u;
-                } else {
-                    constexpr uint32_t m = DT == DT_BF16 ? 0x7F80u : 0x7C00u;
-                    ok &= (v[i][e] & m) != m && (v[i][e] >> 16 & m) != m;
-                }
-            }
-        return ok;
+            for (int e = 0; e < 4; ++e) any |= (v[i][e] & ~SIGNS) + ONE;
+        return (any & SIGNS) == 0u;
     }
     __device__ __forceinline__ void unpack(int i, float (&f)[V]) const {
 #pragma unroll
@@ -640,10 +642,28 @@ __device__ __forceinline__ void write4(typename Elem<DT>::T* p, int col, int col
             if (col + r < cols) p[col + r] = Elem<DT>::st(v[r]);
     }
 }
+// A row of dq or dk, where it is one head's own, or its part of a sum.
+template <int DT, int NT>
+__device__ __forceinline__ void write_key(float* part, typename Elem<DT>::T* out, int key, bool wide16, int row4, const floatx4 (&v)[NT]) {
+    if (part != nullptr) {
+        const bool four = key % 4 == 0;
+#pragma unroll
+        for (int n = 0; n < NT; ++n) write4<DT_F32>(part, 16 * n + row4, here(key), four, v[n]);
+    } else if (wide16 && key == 16 * NT) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n) write4<DT>(out, 16 * n + row4, 16 * NT, true, v[n]);
+    } else {
+#pragma unroll
+        for (int n = 0; n < NT; ++n) write4<DT>(out, 16 * n + row4, here(key), false, v[n]);
+    }
+}
 // Zeros in the columns col0 .. of the rows [from, to).
 template <int DT>
 __device__ __forceinline__ void zero_rows(const Heads& x, int64_t b, int h, int col0, int cols, int64_t from, int64_t to) {
-    for (int64_t i = threadIdx.x; i < (to - from) * cols; i += WG) row_of<DT>(x, b, from + i / cols, h)[col0 + i % cols] = Elem<DT>::st(0.0f);
+#pragma unroll 1
+    for (int64_t t = from + threadIdx.x / 64; t < to; t += WG / 64)
+#pragma unroll 1
+        for (int i = threadIdx.x % 64; i < cols; i += 64) row_of<DT>(x, b, t, h)[col0 + i] = Elem<DT>::st(0.0f);
 }
 
 // ---- forward ------------------------------------------------------------------------------------------
@@ -817,17 +837,19 @@ __device__ __forceinline__ float from_here(float v) {
     return v + dpp<DPP_SHL8>(v);
 }
 
-// In LDS: first S and dS, each [NP][PV] in three parts, with v and dy; then q and k in their places; last dS again in q's.
+// In LDS: k, v and dy, and in one place after another dS and S, each [NP][PV] in three parts, and q.
 template <int DT, int NP>
 struct BwdLds {
     using M = Mat<DT>;
     static constexpr int LDS_STATE = PV + M::PAD, PART = NP * LDS_STATE;
     static constexpr int ONE = M::THREE * PART > Tile<DT, NP>::SIZE ? M::THREE * PART : Tile<DT, NP>::SIZE;
-    static constexpr int Q = 0, K = ONE, V = 2 * ONE, D = V + Tile<DT, PV>::SIZE;
+    static constexpr int Q = 0, K = ONE, V = K + Tile<DT, NP>::SIZE, D = V + Tile<DT, PV>::SIZE;
     static constexpr int BYTES = (int)sizeof(typename M::E) * (D + Tile<DT, PV>::SIZE);
 };
-template <int DT, int NP>
-__global__ void __launch_bounds__(WG, 2) k_attn_bwd(const Args a) {
+// A workgroup has one chunk, and of a group `in_turn` heads one after another: their queries and keys are read once, and what the
+// heads give to dq and dk is summed in registers.
+template <int DT, int NP, bool TURNS>
+__global__ void __launch_bounds__(WG, NP == 128 ? 1 : 2) k_attn_bwd(const Args a) {
     using M = Mat<DT>;
     using E = typename M::E;
     using Frag = typename M::Frag;
@@ -844,218 +866,279 @@ __global__ void __launch_bounds__(WG, 2) k_attn_bwd(const Args a) {
     __shared__ __attribute__((aligned(16))) Falls G;
     __shared__ int said[WAVES];
     __shared__ __attribute__((aligned(16))) float middle[WAVES - 1][CHUNK];
-    __shared__ float pairs[CHUNK], from_state[CHUNK], to_behind[CHUNK], through[WAVES];
-    const int lane = threadIdx.x & 63, own = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l15 = lane & 15, row4 = 4 * (lane >> 4);
-    const int64_t c = blockIdx.x % a.chunks, bht = blockIdx.x / a.chunks, bh = bht / a.tiles, b = bh / a.heads, t0 = c * CHUNK;
-    const int tile = (int)(bht % a.tiles), h = (int)(bh % a.heads);
+    __shared__ float pairs[CHUNK], from_state[CHUNK], to_behind[CHUNK], through[2][WAVES];
+    const int first_own = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t chunks = (uint32_t)a.chunks, rest = blockIdx.x / chunks, turns = (uint32_t)(a.share / a.in_turn);
+    const int64_t c = blockIdx.x - rest * chunks, t0 = c * CHUNK;
+    const int tile = (int)(rest % (uint32_t)a.tiles);
+    const uint32_t set = rest / (uint32_t)a.tiles, bg = set / turns;  // a group's heads in turn; a sequence's group
+    const uint32_t groups = (uint32_t)(a.heads / a.share);
+    const int64_t b = bg / groups;
+    const int gr = (int)(bg % groups), h0 = gr * a.share + (int)(set % turns) * a.in_turn;
     const int64_t end = end_of(a, b);
     const int present = (int)min((int64_t)CHUNK, a.length - t0);
-    const int rows = (int)max((int64_t)0, min((int64_t)CHUNK, end - t0));  // that hold something
+    const int all_rows = (int)max((int64_t)0, min((int64_t)CHUNK, end - t0));  // that hold something
     const int vcols = min(PV, a.value - tile * PV);
-    float* dg = a.dg == nullptr ? nullptr : a.dg + ((tile * a.batch + b) * a.length + t0) * a.heads + h;
-    float* dg_sum = a.dg_sum == nullptr ? nullptr : a.dg_sum + ((b * a.chunks + c) * a.tiles + tile) * a.heads + h;
-    const auto part_row = [&](float* p, int64_t i) { return p + ((b * a.length + t0 + i) * (a.heads * a.tiles) + h * a.tiles + tile) * a.key; };
-    if (rows < present) {
-        zero_rows<DT>(a.dv, b, h, tile * PV, vcols, t0 + rows, t0 + present);
+    const auto part_row = [&](float* p, int64_t i) {
+        return p + (((b * a.length + t0 + i) * groups + gr) * turns * a.tiles + (set % turns) * a.tiles + tile) * a.key;
+    };
+    if (all_rows < present) {
+        for (int h = h0; h < h0 + a.in_turn; ++h) zero_rows<DT>(a.dv, b, h, tile * PV, vcols, t0 + all_rows, t0 + present);
         if (a.part_q == nullptr) {
-            zero_rows<DT>(a.dq, b, h, 0, a.key, t0 + rows, t0 + present);
-            zero_rows<DT>(a.dk, b, h, 0, a.key, t0 + rows, t0 + present);
+            zero_rows<DT>(a.dq, b, gr, 0, a.key, t0 + all_rows, t0 + present);
+            zero_rows<DT>(a.dk, b, gr, 0, a.key, t0 + all_rows, t0 + present);
         } else {
-            for (int i = threadIdx.x; i < (present - rows) * a.key; i += WG) {
-                part_row(a.part_q, rows + i / a.key)[i % a.key] = 0.0f;
-                part_row(a.part_k, rows + i / a.key)[i % a.key] = 0.0f;
-            }
+            for (int i = all_rows + threadIdx.x / 64; i < present; i += WG / 64)
+                for (int n = threadIdx.x % 64; n < a.key; n += 64) part_row(a.part_q, i)[n] = 0.0f, part_row(a.part_k, i)[n] = 0.0f;
         }
     }
-    if (rows == 0) {
-        if (dg != nullptr && (int)threadIdx.x < present) dg[(int64_t)threadIdx.x * a.heads] = 0.0f;
-        if (dg_sum != nullptr && threadIdx.x == 0) *dg_sum = 0.0f;
+    const auto dg_of = [&](int h) { return a.dg == nullptr ? nullptr : a.dg + ((tile * a.batch + b) * a.length + t0) * a.heads + h; };
+    const auto dg_sum_of = [&](int h) { return a.dg_sum == nullptr ? nullptr : a.dg_sum + ((b * a.chunks + c) * a.tiles + tile) * a.heads + h; };
+    if (all_rows == 0) {
+        for (int h = h0; h < h0 + a.in_turn; ++h) {
+            if (a.dg != nullptr && (int)threadIdx.x < present) dg_of(h)[(int64_t)threadIdx.x * a.heads] = 0.0f;
+            if (a.dg_sum != nullptr && threadIdx.x == 0) *dg_sum_of(h) = 0.0f;
+        }
         return;
     }
-    S ds;
-    TN q, k;
-    bool finite;
-    {
-        S s;
+    floatx4 all_dq[NT] = {}, all_dk[NT] = {};
+    bool finite_k = false;
+    for (int turn = 0; turn < (TURNS ? a.in_turn : 1); ++turn) {
+        const int lane = TURNS ? here_lane(threadIdx.x & 63) : threadIdx.x & 63, own = TURNS ? here(first_own) : first_own;
+        const int rows = TURNS ? here(all_rows) : all_rows;
+        const int l15 = lane & 15, row4 = 4 * (lane >> 4), me = 16 * own + l15;  // the own position, as i of dq and as j of dk and dv
+        const int h = h0 + turn;
+        const int64_t bht = (b * a.heads + h) * a.tiles + tile, mark = (bht * a.chunks + c) * S::SIZE;
+        S s, ds;
+        TN q;
         TV v, d;
-        const int64_t mark = (bht * a.chunks + c) * S::SIZE;
-        s.load(a.fmarks + mark, lane, own);
         ds.load(a.marks + mark, lane, own);
         v.load(row_of<DT>(a.v, b, t0, h) + tile * PV, a.v.rs, rows, vcols, a.wide & W_V);
         d.load(row_of<DT>(a.dy, b, t0, h) + tile * PV, a.dy.rs, rows, vcols, a.wide & W_DY);
-        q.load(row_of<DT>(a.q, b, t0, h / a.share), a.q.rs, rows, a.key, a.wide & W_Q);
-        k.load(row_of<DT>(a.k, b, t0, h / a.share), a.k.rs, rows, a.key, a.wide & W_K);
-        if (a.pieces > 1) ds.add(a.starts + (bht * a.pieces + c / a.per_piece) * S::SIZE, a.pre[bh * a.chunks + c], lane, own);
-        const double g = decays(decay_at(decays_of(a, b, h) + t0 * a.g.rs, a.g.rs, rows, lane));
-        if (own == 0) G.put(lane, in_two(g));
-        v.store(tv);
-        d.store(td);
-        s.template put<M, M::THREE>(tq, a.key, vcols, lane, own);
-        ds.template put<M, M::THREE>(tk, a.key, vcols, lane, own);
-        // what passes over the chunk
-        float x = 0.0f;
+        s.load(a.fmarks + mark, lane, own);
+        const float g_own = decay_at(decays_of(a, b, h) + t0 * a.g.rs, a.g.rs, rows, lane);
+        q.load(row_of<DT>(a.q, b, t0, gr), a.q.rs, rows, a.key, a.wide & W_Q);
+        if (turn == 0) {
+            TN k;
+            k.load(row_of<DT>(a.k, b, t0, gr), a.k.rs, rows, a.key, a.wide & W_K);
+            k.store(tk);
+            finite_k = k.finite();
+        }
+        {
+            if (a.pieces > 1)
+                ds.add(a.starts + (bht * a.pieces + c / a.per_piece) * S::SIZE, a.pre[(b * a.heads + h) * a.chunks + c], lane, own);
+            const double g = decays(g_own);
+            if (own == 0) G.put(lane, in_two(g));
+            {  // what passes over the chunk; behind key and value there may be anything
+                float x = 0.0f;
+                const bool full = a.key == NP && vcols == PV;
+                const int key = here(a.key), value = here(vcols);
+                s.each([&](int i, int j, floatx4& y) {
+                    if (full) {
 #pragma unroll
-        for (int i = 0; i < S::TP; ++i)
+                        for (int r = 0; r < 4; ++r) x = __builtin_fmaf(y[r], ds.v[i][j][r], x);
+                    } else {
 #pragma unroll
-            for (int j = 0; j < S::TN; ++j)
+                        for (int r = 0; r < 4; ++r) {
+                            const float z = __builtin_fmaf(y[r], ds.v[i][j][r], x);
+                            x = S::n(j, lane, own) < key && S::p(i, lane) + r < value ? z : x;
+                        }
+                    }
+                });
+                x = wsum(x);
+                if (lane == 0) through[turn & 1][own] = x;
+            }
+            v.store(tv);
+            d.store(td);
+            ds.template put<M, M::THREE>(tq, a.key, vcols, lane, own);
+            say_finite(said, finite_k && q.finite() && d.finite(), lane, own);
+            __syncthreads();
+            const bool finite = heard_finite(said);
+            const float2 mine = G.at(me), g_end = G.at(CHUNK - 1);
+            const float to_end = fall_between(g_end, mine), from_start = a.scale * __builtin_amdgcn_exp2f(mine.x + mine.y);
+            floatx4 dq[NT], dk[NT], dv[S::TP];
+            // what the positions behind the chunk give to dk and dv, by way of dS
 #pragma unroll
-                for (int r = 0; r < 4; ++r)
-                    if (S::n(j, lane, own) < a.key && S::p(i, lane) + r < vcols) x = __builtin_fmaf(s.v[i][j][r], ds.v[i][j][r], x);
-        x = wsum(x);
-        if (lane == 0) through[own] = x;
-        say_finite(said, q.finite() && k.finite() && d.finite(), lane, own);
-        __syncthreads();
-        finite = heard_finite(said);
+            for (int n = 0; n < NT; ++n) dk[n] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int p = 0; p < S::TP; ++p) dv[p] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int p = 0; p < PV; p += M::STEP) {
+                const Frag f = M::row(tv, TV::LD, 16 * own, p, lane);
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int x = 0; x < M::THREE; ++x) dk[n] = M::mma(M::row(tq + x * L::PART, LS, 16 * n, p, lane), f, dk[n]);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+#pragma unroll
+            for (int n = 0; n < NP; n += M::STEP) {
+                const Frag f = M::row(tk, TN::LD, 16 * own, n, lane);
+#pragma unroll
+                for (int p = 0; p < S::TP; ++p)
+#pragma unroll
+                    for (int x = 0; x < M::TWO; ++x) dv[p] = M::mma(M::col(tq + x * L::PART, LS, 16 * p, n, lane), f, dv[p]);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            {
+                float x = 0.0f;
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    const floatx4 f = M::load4(tk + me * TN::LD + 16 * n + row4);
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        dk[n][r] *= to_end;
+                        x = __builtin_fmaf(dk[n][r], f[r], x);
+                    }
+                }
+                x = over_rows(x);
+                if (lane < 16) to_behind[me] = x;
+#pragma unroll
+                for (int p = 0; p < S::TP; ++p)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) dv[p][r] *= to_end;
+            }
+            __syncthreads();
+            // and what the state before the chunk gives to dq
+            s.template put<M, M::THREE>(tq, a.key, vcols, lane, own);
+            __syncthreads();
+#pragma unroll
+            for (int n = 0; n < NT; ++n) dq[n] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int p = 0; p < PV; p += M::STEP) {
+                const Frag f = M::row(td, TV::LD, 16 * own, p, lane);
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int x = 0; x < M::THREE; ++x) dq[n] = M::mma(M::row(tq + x * L::PART, LS, 16 * n, p, lane), f, dq[n]);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            __syncthreads();
+            q.store(tq);
+            __syncthreads();
+            {
+                float x = 0.0f;
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    const floatx4 f = M::load4(tq + me * TN::LD + 16 * n + row4);
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        dq[n][r] *= from_start;
+                        x = __builtin_fmaf(dq[n][r], f[r], x);
+                    }
+                }
+                x = over_rows(x);
+                if (lane < 16) from_state[me] = x;
+            }
+            // the own positions as i: rows are positions j before them
+            __builtin_amdgcn_sched_barrier(0);
+            {
+                floatx4 A[4], dA[4], f[4];
+                scores<M, NP>(A, tk, tq, TN::LD, 16 * own, 0, own, lane);
+                __builtin_amdgcn_sched_barrier(0);
+                scores<M, PV>(dA, tv, td, TV::LD, 16 * own, 0, own, lane);
+                __builtin_amdgcn_sched_barrier(0);
+                falls<true>(G, mine, a.scale, lane, f);
+                // the pairs that a position t of the own ones lies between: of M_ij the sum over the own i >= t, then over j < t; and all
+                // own i for the positions of the tiles before
+                float at = 0.0f;
+#pragma unroll
+                for (int t = 0; t < 4; ++t) {
+                    if (t > own) continue;
+                    floatx4 sums;
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const int j = 16 * t + row4 + r;
+                        const bool in = j <= me && me < rows;
+                        const float x = dA[t][r] * f[t][r], m = A[t][r] * x;
+                        dA[t][r] = in ? x : 0.0f;
+                        sums[r] = from_here(in ? m : 0.0f);
+                        at += j < me ? sums[r] : 0.0f;
+                    }
+                    if (t < own && l15 == 0) *reinterpret_cast<floatx4*>(&middle[own - 1][16 * t + row4]) = sums;
+                }
+#pragma unroll
+                for (int t = 1; t < 4; ++t)
+                    if (t > own) dA[t] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+                at = over_rows(at);
+                if (lane < 16) pairs[me] = at;
+                product_within<M, M::TWO>(dq, finite, tk, TN::LD, dA, 0, own, lane, [&](int j) { return j <= me && me < rows; });
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) all_dq[n][r] = TURNS ? all_dq[n][r] + dq[n][r] : dq[n][r];
+            }
+            // the own positions as j: rows are positions i behind them
+            __builtin_amdgcn_sched_barrier(0);
+            {
+                floatx4 A[4], dA[4], f[4];
+                scores<M, NP>(A, tq, tk, TN::LD, 16 * own, own, 3, lane);
+                __builtin_amdgcn_sched_barrier(0);
+                scores<M, PV>(dA, td, tv, TV::LD, 16 * own, own, 3, lane);
+                __builtin_amdgcn_sched_barrier(0);
+                falls<false>(G, mine, a.scale, lane, f);
+#pragma unroll
+                for (int t = 0; t < 4; ++t) {
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const int i = 16 * t + row4 + r;
+                        const bool in = i >= me && i < rows;
+                        const float x = A[t][r] * f[t][r], y = dA[t][r] * f[t][r];
+                        A[t][r] = in ? x : 0.0f;
+                        dA[t][r] = in ? y : 0.0f;
+                    }
+                }
+                const auto inside = [&](int i) { return i >= me && i < rows; };
+                product_within<M, M::TWO>(dk, finite, tq, TN::LD, dA, own, 3, lane, inside);
+                __builtin_amdgcn_sched_barrier(0);
+                product_within<M, M::TWO>(dv, finite, td, TV::LD, A, own, 3, lane, inside);
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) all_dk[n][r] = TURNS ? all_dk[n][r] + dk[n][r] : dk[n][r];
+                if (me < rows) {
+                    auto* out = row_of<DT>(a.dv, b, t0 + me, h) + tile * PV;
+                    if ((a.wide & W_DV) && vcols == PV) {
+#pragma unroll
+                        for (int p = 0; p < S::TP; ++p) write4<DT>(out, 16 * p + row4, PV, true, dv[p]);
+                    } else {
+#pragma unroll
+                        for (int p = 0; p < S::TP; ++p) write4<DT>(out, 16 * p + row4, here(vcols), false, dv[p]);
+                    }
+                }
+            }
+            __syncthreads();
+            // dg, by one wavefront (lane = position)
+            if (own == 0) {
+                const double over = ((double)through[turn & 1][0] + (double)through[turn & 1][1] + (double)through[turn & 1][2] + (double)through[turn & 1][3]) *
+                                    (double)__builtin_amdgcn_exp2f(g_end.x + g_end.y);
+                const bool in = lane < rows;
+                // from the states before: positions i from t on (summed from the last one); to the positions behind the chunk: j before t
+                const int last = CHUNK - 1 - lane;
+                const double later = __shfl(scan(last < rows ? (double)from_state[last] : 0.0), CHUNK - 1 - lane, 64);
+                double x = (double)pairs[lane] + later + over;
+                const double behind = __shfl_up(scan(in ? (double)to_behind[lane] : 0.0), 1, 64);
+                if (lane > 0) x += behind;
+                // and of the chunk's own pairs those with an i of a later tile than t's
+#pragma unroll
+                for (int t = 1; t < WAVES; ++t) {
+                    const double before = __shfl_up(scan(lane < 16 * t ? (double)middle[t - 1][lane] : 0.0), 1, 64);
+                    if (lane > 0 && lane < 16 * t) x += before;
+                }
+                if (!in) x = 0.0;
+                if (a.dg != nullptr && lane < present) dg_of(h)[(int64_t)lane * a.heads] = (float)x;
+                if (a.dg_sum != nullptr) {
+                    const double sum = last_lane(scan(x));
+                    if (lane == 0) *dg_sum_of(h) = (float)sum;
+                }
+            }
+        }
     }
-    const int me = 16 * own + l15;  // the own position, as i of dq and as j of dk and dv
-    const float2 mine = G.at(me), g_end = G.at(CHUNK - 1);
-    const float to_end = fall_between(g_end, mine), from_start = a.scale * __builtin_amdgcn_exp2f(mine.x + mine.y);
-    floatx4 dq[NT] = {}, dk[NT] = {};
-#pragma unroll
-    for (int p = 0; p < PV; p += M::STEP) {
-        const Frag fd = M::row(td, TV::LD, 16 * own, p, lane), fv = M::row(tv, TV::LD, 16 * own, p, lane);
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int x = 0; x < M::THREE; ++x) {
-                dq[n] = M::mma(M::row(tq + x * L::PART, LS, 16 * n, p, lane), fd, dq[n]);
-                dk[n] = M::mma(M::row(tk + x * L::PART, LS, 16 * n, p, lane), fv, dk[n]);
-            }
-    }
-    __syncthreads();
-    q.store(tq);
-    k.store(tk);
-    __syncthreads();
-    {
-        float x = 0.0f, y = 0.0f;
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-            const floatx4 fq = M::load4(tq + me * TN::LD + 16 * n + row4), fk = M::load4(tk + me * TN::LD + 16 * n + row4);
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                dq[n][r] *= from_start;
-                dk[n][r] *= to_end;
-                x = __builtin_fmaf(dq[n][r], fq[r], x);
-                y = __builtin_fmaf(dk[n][r], fk[r], y);
-            }
-        }
-        x = over_rows(x);
-        y = over_rows(y);
-        if (lane < 16) from_state[me] = x, to_behind[me] = y;
-    }
-    // the own positions as i: rows are positions j before them
-    {
-        floatx4 A[4], dA[4], f[4];
-        scores<M, NP>(A, tk, tq, TN::LD, 16 * own, 0, own, lane);
-        scores<M, PV>(dA, tv, td, TV::LD, 16 * own, 0, own, lane);
-        falls<true>(G, mine, a.scale, lane, f);
-        // the pairs that a position t of the own ones lies between: of M_ij the sum over the own i >= t, then over j < t; and all own i
-        // for the positions of the tiles before
-        float at = 0.0f;
-#pragma unroll
-        for (int t = 0; t < 4; ++t) {
-            if (t > own) continue;
-            floatx4 sums;
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int j = 16 * t + row4 + r;
-                const bool in = j <= me && me < rows;
-                const float x = dA[t][r] * f[t][r], m = A[t][r] * x;
-                dA[t][r] = in ? x : 0.0f;
-                sums[r] = from_here(in ? m : 0.0f);
-                at += j < me ? sums[r] : 0.0f;
-            }
-            if (t < own && l15 == 0) *reinterpret_cast<floatx4*>(&middle[own - 1][16 * t + row4]) = sums;
-        }
-#pragma unroll
-        for (int t = 1; t < 4; ++t)
-            if (t > own) dA[t] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
-        at = over_rows(at);
-        if (lane < 16) pairs[me] = at;
-        product_within<M, M::TWO>(dq, finite, tk, TN::LD, dA, 0, own, lane, [&](int j) { return j <= me && me < rows; });
-        if (me < rows) {
-#pragma unroll
-            for (int n = 0; n < NT; ++n) {
-                if (a.part_q == nullptr) write4<DT>(row_of<DT>(a.dq, b, t0 + me, h), 16 * n + row4, a.key, a.wide & W_DQ, dq[n]);
-                else write4<DT_F32>(part_row(a.part_q, me), 16 * n + row4, a.key, a.key % 4 == 0, dq[n]);
-            }
-        }
-    }
-    // the own positions as j: rows are positions i behind them
-    floatx4 dv[S::TP] = {};
-    {
-        floatx4 A[4], dA[4], f[4];
-        scores<M, NP>(A, tq, tk, TN::LD, 16 * own, own, 3, lane);
-        scores<M, PV>(dA, td, tv, TV::LD, 16 * own, own, 3, lane);
-        falls<false>(G, mine, a.scale, lane, f);
-#pragma unroll
-        for (int t = 0; t < 4; ++t)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int i = 16 * t + row4 + r;
-                const bool in = i >= me && i < rows;
-                const float x = A[t][r] * f[t][r], y = dA[t][r] * f[t][r];
-                A[t][r] = in ? x : 0.0f;
-                dA[t][r] = in ? y : 0.0f;
-            }
-        const auto inside = [&](int i) { return i >= me && i < rows; };
-        product_within<M, M::TWO>(dk, finite, tq, TN::LD, dA, own, 3, lane, inside);
-        product_within<M, M::TWO>(dv, finite, td, TV::LD, A, own, 3, lane, inside);
-        if (me < rows) {
-#pragma unroll
-            for (int n = 0; n < NT; ++n) {
-                if (a.part_k == nullptr) write4<DT>(row_of<DT>(a.dk, b, t0 + me, h), 16 * n + row4, a.key, a.wide & W_DK, dk[n]);
-                else write4<DT_F32>(part_row(a.part_k, me), 16 * n + row4, a.key, a.key % 4 == 0, dk[n]);
-            }
-        }
-    }
-    __syncthreads();
-    ds.template put<M, M::TWO>(tq, a.key, vcols, lane, own);
-    __syncthreads();
-    {
-        floatx4 far[S::TP] = {};
-#pragma unroll
-        for (int n = 0; n < NP; n += M::STEP) {
-            const Frag f = M::row(tk, TN::LD, 16 * own, n, lane);
-#pragma unroll
-            for (int p = 0; p < S::TP; ++p)
-#pragma unroll
-                for (int x = 0; x < M::TWO; ++x) far[p] = M::mma(M::col(tq + x * L::PART, LS, 16 * p, n, lane), f, far[p]);
-        }
-        if (me < rows) {
-            auto* out = row_of<DT>(a.dv, b, t0 + me, h) + tile * PV;
-#pragma unroll
-            for (int p = 0; p < S::TP; ++p) {
-#pragma unroll
-                for (int r = 0; r < 4; ++r) dv[p][r] = __builtin_fmaf(to_end, far[p][r], dv[p][r]);
-                write4<DT>(out, 16 * p + row4, vcols, a.wide & W_DV, dv[p]);
-            }
-        }
-    }
-    // dg, by one wavefront (lane = position)
-    if (own == 0 && (dg != nullptr || dg_sum != nullptr)) {
-        const double over = ((double)through[0] + (double)through[1] + (double)through[2] + (double)through[3]) *
-                            (double)__builtin_amdgcn_exp2f(g_end.x + g_end.y);
-        const bool in = lane < rows;
-        // from the states before: positions i from t on (summed from the last one); to the positions behind the chunk: j before t
-        const int last = CHUNK - 1 - lane;
-        double later = scan(last < rows ? (double)from_state[last] : 0.0);
-        later = __shfl(later, CHUNK - 1 - lane, 64);
-        double x = (double)pairs[lane] + later + over;
-        const double behind = __shfl_up(scan(in ? (double)to_behind[lane] : 0.0), 1, 64);
-        if (lane > 0) x += behind;
-        // and of the chunk's own pairs those with an i of a later tile than t's
-#pragma unroll
-        for (int t = 1; t < WAVES; ++t) {
-            const double before = __shfl_up(scan(lane < 16 * t ? (double)middle[t - 1][lane] : 0.0), 1, 64);
-            if (lane > 0 && lane < 16 * t) x += before;
-        }
-        if (!in) x = 0.0;
-        if (dg != nullptr && lane < present) dg[(int64_t)lane * a.heads] = (float)x;
-        if (dg_sum != nullptr) {
-            const double sum = last_lane(scan(x));
-            if (lane == 0) *dg_sum = (float)sum;
-        }
+    const int me = 16 * first_own + (threadIdx.x & 15), row4 = 4 * ((threadIdx.x & 63) >> 4);
+    if (me < all_rows) {
+        write_key<DT>(a.part_q == nullptr ? nullptr : part_row(a.part_q, me), row_of<DT>(a.dq, b, t0 + me, gr), a.key, a.wide & W_DQ, row4, all_dq);
+        write_key<DT>(a.part_k == nullptr ? nullptr : part_row(a.part_k, me), row_of<DT>(a.dk, b, t0 + me, gr), a.key, a.wide & W_DK, row4, all_dk);
     }
 }
 
@@ -1063,7 +1146,7 @@ __global__ void __launch_bounds__(WG, 2) k_attn_bwd(const Args a) {
 template <int DT>
 __global__ void __launch_bounds__(WG) k_attn_sum(const Args a, const float* part, Heads out, int groups) {
     const int64_t n = a.batch * a.length * groups * a.key;
-    const int each = a.share * a.tiles;
+    const int each = a.share / a.in_turn * a.tiles;
     for (int64_t i = (int64_t)blockIdx.x * WG + threadIdx.x; i < n; i += (int64_t)gridDim.x * WG) {
         const int col = (int)(i % a.key), gr = (int)(i / a.key % groups);
         const int64_t bt = i / a.key / groups;
@@ -1187,11 +1270,19 @@ struct Plan {
     }
 };
 
-bool parts_wanted(const boa_attention& s, const Plan& p) { return s.heads / s.groups * p.tiles > 1; }
+// Heads of a group that a workgroup of the backward pass takes in turn: as many as leave two for each CU twice over.
+int in_turn(const boa_attention& s, const Plan& p) {
+    const int share = s.heads / s.groups;
+    for (int n = share; n > 1; --n)
+        if (share % n == 0 && p.bh / n * p.tiles * p.chunks >= 2 * WANTED) return n;
+    return 1;
+}
+// Parts of a group's dq and dk, which are then summed.
+int64_t group_parts(const boa_attention& s, const Plan& p) { return (int64_t)(s.heads / s.groups / in_turn(s, p)) * p.tiles; }
 
 int64_t bwd_bytes(const boa_attention& s, const Plan& p) {
     int64_t n = p.bytes();
-    if (parts_wanted(s, p)) n += 2 * 4 * s.batch * s.length * s.heads * p.tiles * s.key;
+    if (group_parts(s, p) > 1) n += 2 * 4 * s.batch * s.length * s.groups * group_parts(s, p) * s.key;
     if (s.decay_per_head) n += 4 * s.batch * p.chunks * p.tiles * s.heads;
     else if (p.tiles > 1) n += 4 * p.tiles * s.batch * s.length * s.heads;
     return n;
@@ -1318,8 +1409,9 @@ extern "C" int boa_linear_attention_bwd(const boa_attention* s, void* d_work, in
     a.fmarks = s->marks;
     a.state_in = nullptr, a.state_out = nullptr;
     float* rest = reinterpret_cast<float*>(static_cast<char*>(d_work) + p.bytes());
-    if (parts_wanted(*s, p)) {
-        const int64_t each = s->batch * s->length * s->heads * p.tiles * s->key;
+    a.in_turn = in_turn(*s, p);
+    if (group_parts(*s, p) > 1) {
+        const int64_t each = s->batch * s->length * s->groups * group_parts(*s, p) * s->key;
         a.part_q = rest, a.part_k = rest + each;
         rest += 2 * each;
     }
@@ -1329,8 +1421,14 @@ extern "C" int boa_linear_attention_bwd(const boa_attention* s, void* d_work, in
         return with_key(p.np, [&](auto np) {
             constexpr int DT = decltype(dt)::value, NP = decltype(np)::value, LDS = BwdLds<DT, NP>::BYTES;
             if (const int no = launch_states<DT, NP, true>(a, p, st)) return no;
-            if (const int no = allow_lds(k_attn_bwd<DT, NP>, LDS)) return no;
-            hipLaunchKernelGGL((k_attn_bwd<DT, NP>), dim3((uint32_t)(p.bh * p.tiles * p.chunks)), dim3(WG), LDS, st, a);
+            const dim3 grid((uint32_t)(p.bh / a.in_turn * p.tiles * p.chunks));
+            if (a.in_turn > 1) {
+                if (const int no = allow_lds(k_attn_bwd<DT, NP, true>, LDS)) return no;
+                hipLaunchKernelGGL((k_attn_bwd<DT, NP, true>), grid, dim3(WG), LDS, st, a);
+            } else {
+                if (const int no = allow_lds(k_attn_bwd<DT, NP, false>, LDS)) return no;
+                hipLaunchKernelGGL((k_attn_bwd<DT, NP, false>), grid, dim3(WG), LDS, st, a);
+            }
             BOA_HIP_TRY(hipGetLastError());
             if (a.part_q != nullptr) {
                 const int64_t n = ceil_div(s->batch * s->length * s->groups * s->key, WG);
