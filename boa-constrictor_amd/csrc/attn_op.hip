@@ -60,7 +60,7 @@ struct Args {
     float scale;
     uint32_t wide;  // bit per tensor: read or written 16 bytes at a time (W_*)
 };
-enum { W_Q = 1, W_K = 2, W_V = 4, W_DY = 8, W_Y = 16, W_DQ = 32, W_DK = 64, W_DV = 128 };
+enum { W_Q = 1, W_K = 2, W_V = 4, W_DY = 8, W_Y = 16, W_DQ = 32, W_DK = 64, W_DV = 128, W_FWD = W_Q | W_K | W_V, W_BACK = W_FWD | W_DY };
 
 // How products of a type run: elements in LDS, K of a step, parts that a float32 value is split into.
 //   bfloat16: inputs as they are.  What is computed on the way (A, dA, states, decayed keys) is split into parts of 8 bits each:
@@ -276,11 +276,12 @@ struct Tile {
     static_assert(WG % ROW == 0, "");
     static constexpr int LD = COLS + M::PAD, SIZE = CHUNK * LD;
     u32x4 v[PER];
-    // rows from p on, `rows` and `cols` of them
-    __device__ __forceinline__ void load(const T* p, int64_t stride, int rows, int cols, bool wide16) {
-        const int r0 = threadIdx.x / ROW, c = threadIdx.x % ROW * V;  // WG / ROW rows apart
+    // rows from p on, `rows` and `cols` of them; WIDE: aligned for accesses of 16 bytes
+    template <bool WIDE>
+    __device__ __forceinline__ void load(const T* p, int64_t stride, int rows, int cols, int tid) {
+        const int r0 = tid / ROW, c = tid % ROW * V;  // WG / ROW rows apart
         p += r0 * stride + c;
-        if (wide16 && rows == CHUNK && cols == COLS) {
+        if (WIDE && rows == CHUNK && cols == COLS) {
 #pragma unroll
             for (int i = 0; i < PER; ++i) v[i] = *reinterpret_cast<const u32x4*>(p + i * (WG / ROW * stride));
             return;
@@ -289,9 +290,9 @@ struct Tile {
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
             v[i] = u32x4{0u, 0u, 0u, 0u};
+            const T* q = p + i * (WG / ROW * stride);
             if (r0 + i * (WG / ROW) < rows && c < cols) {
-                const T* q = p + i * (WG / ROW * stride);
-                if (wide16) {
+                if constexpr (WIDE) {
                     v[i] = *reinterpret_cast<const u32x4*>(q);
                 } else {
 #pragma unroll
@@ -322,10 +323,10 @@ struct Tile {
             else f[e] = Elem<DT>::ld((uint16_t)(v[i][e / 2] >> (16 * (e & 1))));
         }
     }
-    __device__ __forceinline__ void store(typename M::E* t) const {
+    __device__ __forceinline__ void store(typename M::E* t, int tid) const {
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
-            const int at = threadIdx.x + i * WG, r = at / ROW, c = at % ROW * V;
+            const int at = tid + i * WG, r = at / ROW, c = at % ROW * V;
             if constexpr (DT == DT_F16) {
                 float f[V];
                 unpack(i, f);
@@ -361,18 +362,18 @@ struct Falls {
     __device__ __forceinline__ void put(int i, float2 g) { x[i] = g.x, y[i] = g.y; }
     __device__ __forceinline__ float2 at(int i) const { return make_float2(x[i], y[i]); }
 };
-// The factors between the own position and the four rows of each tile that a lane has: of the own one behind them, or of them behind it.
+// The factors between the own position and the four rows that a lane has of tile t: of the own one behind them, or of them behind it.
 template <bool OWN_BEHIND>
-__device__ __forceinline__ void falls(const Falls& g, float2 own, float scale, int lane, floatx4 (&f)[4]) {
+__device__ __forceinline__ floatx4 falls(const Falls& g, float2 own, float scale, int lane, int t) {
+    const int at = 16 * t + 4 * (lane >> 4);
+    const f32x4 x = *reinterpret_cast<const f32x4*>(g.x + at), y = *reinterpret_cast<const f32x4*>(g.y + at);
+    floatx4 f;
 #pragma unroll
-    for (int t = 0; t < 4; ++t) {
-        const f32x4 x = *reinterpret_cast<const f32x4*>(g.x + 16 * t + 4 * (lane >> 4)), y = *reinterpret_cast<const f32x4*>(g.y + 16 * t + 4 * (lane >> 4));
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const float2 o = make_float2(x[r], y[r]);
-            f[t][r] = scale * (OWN_BEHIND ? fall_between(own, o) : fall_between(o, own));
-        }
+    for (int r = 0; r < 4; ++r) {
+        const float2 o = make_float2(x[r], y[r]);
+        f[r] = scale * (OWN_BEHIND ? fall_between(own, o) : fall_between(o, own));
     }
+    return f;
 }
 // Whether any value that the workgroup's threads have is not finite, by way of a barrier: each wavefront says so in LDS.
 __device__ __forceinline__ void say_finite(int* said, bool finite, int lane, int wave) {
@@ -510,7 +511,7 @@ __device__ __forceinline__ void times(State<NP>& s, float f) {
 // ---- states by themselves ---------------------------------------------------------------------------
 // A workgroup walks the chunks of a piece from a state of zeros, forward over k v^T or (BACK) from the last one over scale e^(G_i)
 // q dy^T; leaves what it ends with, and backward also what it reaches each chunk with.
-template <int DT, int NP, bool BACK>
+template <int DT, int NP, bool BACK, bool WIDE>
 __global__ void __launch_bounds__(WG, 2) k_attn_states(const Args a) {
     using M = Mat<DT>;
     using TX = Tile<DT, NP>;
@@ -527,7 +528,6 @@ __global__ void __launch_bounds__(WG, 2) k_attn_states(const Args a) {
     const int64_t end = end_of(a, b);
     const int64_t c0 = (int64_t)piece * a.per_piece, c1 = min(c0 + a.per_piece, (end + CHUNK - 1) / CHUNK);
     const Heads &X = BACK ? a.q : a.k, &Y = BACK ? a.dy : a.v;
-    const bool wx = (a.wide & (BACK ? W_Q : W_K)) != 0, wy = (a.wide & (BACK ? W_DY : W_V)) != 0;
     const int vcols = min(PV, a.value - tile * PV);
     float* marks = a.marks + (bh * a.tiles + tile) * a.chunks * S::SIZE;
 
@@ -540,29 +540,30 @@ __global__ void __launch_bounds__(WG, 2) k_attn_states(const Args a) {
     const auto* xp = row_of<DT>(X, b, 0, h / a.share);
     const auto* yp = row_of<DT>(Y, b, 0, h) + tile * PV;
     const float* gp = decays_of(a, b, h);
-    const auto fetch = [&](int64_t c) {
+    const auto fetch = [&](int64_t c, int tid) {
         const int64_t t0 = c * CHUNK;
         const int rows = (int)min((int64_t)CHUNK, end - t0);
-        x.load(xp + t0 * X.rs, X.rs, rows, a.key, wx);
-        y.load(yp + t0 * Y.rs, Y.rs, rows, vcols, wy);
-        g_own = decay_at(gp + t0 * a.g.rs, a.g.rs, rows, lane);
+        x.template load<WIDE>(xp + t0 * X.rs, X.rs, rows, a.key, tid);
+        y.template load<WIDE>(yp + t0 * Y.rs, Y.rs, rows, vcols, tid);
+        g_own = decay_at(gp + t0 * a.g.rs, a.g.rs, rows, tid & 63);
     };
     const int64_t n = c1 - c0;
-    if (n > 0) fetch(BACK ? c1 - 1 : c0);
+    if (n > 0) fetch(BACK ? c1 - 1 : c0, threadIdx.x);
     for (int64_t m = 0; m < n; ++m) {
+        const int tid = threadIdx.x;
         const int64_t c = BACK ? c1 - 1 - m : c0 + m;
         if constexpr (BACK) {
             s.store(marks + c * S::SIZE, lane, wave);
             if (a.pieces > 1 && tile == 0 && threadIdx.x == 0) a.pre[bh * a.chunks + c] = __builtin_amdgcn_exp2f((float)passed);
         }
         const double g = decays(g_own), all = last_lane(g);
-        x.store(tx);
-        y.store(ty);
+        x.store(tx, tid);
+        y.store(ty, tid);
         if (wave == 0) weight[lane] = BACK ? a.scale * __builtin_amdgcn_exp2f((float)g) : __builtin_amdgcn_exp2f((float)(all - g));
         if constexpr (M::THREE > 1) say_finite(said, y.finite(), lane, wave);
         __syncthreads();
         const bool finite = M::THREE == 1 || heard_finite(said);
-        if (m + 1 < n) fetch(BACK ? c - 1 : c + 1);
+        if (m + 1 < n) fetch(BACK ? c - 1 : c + 1, tid);
         passed += all;
         times(s, __builtin_amdgcn_exp2f((float)all));
         const auto all_steps = [&](auto clean) {
@@ -673,7 +674,7 @@ struct FwdLds {
     static constexpr int Q = 0, K = Tile<DT, NP>::SIZE, V = 2 * K, S = V + Tile<DT, PV>::SIZE, LDS_STATE = PV + M::PAD, PART = NP * LDS_STATE;
     static constexpr int BYTES = (int)sizeof(typename M::E) * (S + M::TWO * PART);
 };
-template <int DT, int NP>
+template <int DT, int NP, bool WIDE>
 __global__ void __launch_bounds__(WG, NP == 128 ? 1 : 2) k_attn_fwd(const Args a) {
     using M = Mat<DT>;
     using E = typename M::E;
@@ -690,7 +691,7 @@ __global__ void __launch_bounds__(WG, NP == 128 ? 1 : 2) k_attn_fwd(const Args a
     __shared__ __attribute__((aligned(16))) Falls G;
     __shared__ __attribute__((aligned(16))) float weight[CHUNK];
     __shared__ int said[WAVES];
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l15 = lane & 15, row4 = 4 * (lane >> 4);
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     // a wavefront's own positions i: the later ones have more before them, so workgroups beside each other have them the other way round
     const int own = blockIdx.x & 1 ? WAVES - 1 - wave : wave;
     const int piece = (int)(blockIdx.x % a.pieces), tile = (int)(blockIdx.x / a.pieces % a.tiles);
@@ -715,36 +716,46 @@ __global__ void __launch_bounds__(WG, NP == 128 ? 1 : 2) k_attn_fwd(const Args a
     const float* gp = decays_of(a, b, h);
     auto* yp = row_of<DT>(a.y, b, 0, h) + tile * PV;
     float* marks = a.marks == nullptr ? nullptr : a.marks + bht * a.chunks * S::SIZE;
-    const auto fetch = [&](int64_t c) {
+    const auto fetch = [&](int64_t c, int tid) {
         const int64_t t0 = c * CHUNK;
         const int rows = (int)min((int64_t)CHUNK, end - t0);
-        q.load(qp + t0 * a.q.rs, a.q.rs, rows, a.key, a.wide & W_Q);
-        k.load(kp + t0 * a.k.rs, a.k.rs, rows, a.key, a.wide & W_K);
-        v.load(vp + t0 * a.v.rs, a.v.rs, rows, vcols, a.wide & W_V);
-        g_own = decay_at(gp + t0 * a.g.rs, a.g.rs, rows, lane);
+        q.template load<WIDE>(qp + t0 * a.q.rs, a.q.rs, rows, a.key, tid);
+        k.template load<WIDE>(kp + t0 * a.k.rs, a.k.rs, rows, a.key, tid);
+        v.template load<WIDE>(vp + t0 * a.v.rs, a.v.rs, rows, vcols, tid);
+        g_own = decay_at(gp + t0 * a.g.rs, a.g.rs, rows, tid & 63);
     };
     // a chunk's results are written while the next one is on: what has been stored late would be waited for with the next tiles
-    floatx4 y[S::TP];
-    const auto write = [&](int64_t t0) {
-        const int64_t t = t0 + 16 * own + l15;
+    using Out = Raw<DT, 4>;
+    typename Out::V done[S::TP];
+    const auto write = [&](int64_t t0, int tid) {
+        const int row4 = 4 * ((tid & 63) >> 4);
+        const int64_t t = t0 + 16 * own + (tid & 15);
         if (t >= end) return;
-        auto* out = yp + t * a.y.rs;
+        auto* out = yp + t * a.y.rs + row4;
         if ((a.wide & W_Y) && vcols == PV) {
 #pragma unroll
-            for (int p = 0; p < S::TP; ++p) write4<DT>(out, 16 * p + row4, PV, true, y[p]);
+            for (int p = 0; p < S::TP; ++p) *reinterpret_cast<typename Out::V*>(out + 16 * p) = done[p];
         } else {
 #pragma unroll
-            for (int p = 0; p < S::TP; ++p) write4<DT>(out, 16 * p + row4, here(vcols), false, y[p]);
+            for (int p = 0; p < S::TP; ++p) {
+                const int cols = here(vcols);
+                float v[4];
+                Out::unpack(done[p], v);
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                    if (16 * p + row4 + r < cols) out[16 * p + r] = Elem<DT>::st(v[r]);
+            }
         }
     };
-    if (c0 < c1) fetch(c0);
+    if (c0 < c1) fetch(c0, threadIdx.x);
     for (int64_t c = c0; c < c1; ++c) {
+        const int tid = here_lane(threadIdx.x), lane = tid & 63, l15 = lane & 15, row4 = 4 * (lane >> 4);
         const int64_t t0 = c * CHUNK;
         const int rows = (int)min((int64_t)CHUNK, end - t0);
         const double g = decays(g_own), all = last_lane(g);
-        q.store(tq);
-        k.store(tk);
-        v.store(tv);
+        q.store(tq, tid);
+        k.store(tk, tid);
+        v.store(tv, tid);
         s.template put<M, M::TWO>(ts, a.key, vcols, lane, wave);
         if (wave == 0) {
             G.put(lane, in_two(g));
@@ -753,13 +764,14 @@ __global__ void __launch_bounds__(WG, NP == 128 ? 1 : 2) k_attn_fwd(const Args a
         say_finite(said, v.finite(), lane, wave);
         __syncthreads();
         const bool finite = heard_finite(said);
-        if (c > c0) write(t0 - CHUNK);
+        if (c > c0) write(t0 - CHUNK, tid);
         if (marks != nullptr) s.store(marks + c * S::SIZE, lane, wave);
-        if (c + 1 < c1) fetch(c + 1);
+        if (c + 1 < c1) fetch(c + 1, tid);
 
         // q . k of all positions j (rows) and the own ones (columns), and what the state gives
-        floatx4 A[4], f[4];
+        floatx4 A[4], y[S::TP];
         scores<M, NP>(A, tk, tq, TN::LD, 16 * own, 0, own, lane);
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int p = 0; p < S::TP; ++p) y[p] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
@@ -770,22 +782,25 @@ __global__ void __launch_bounds__(WG, NP == 128 ? 1 : 2) k_attn_fwd(const Args a
 #pragma unroll
                 for (int i = 0; i < M::TWO; ++i) y[p] = M::mma(M::col(ts + i * L::PART, L::LDS_STATE, 16 * p, n, lane), fq, y[p]);
         }
+        __builtin_amdgcn_sched_barrier(0);
         const int i = 16 * own + l15;
         const float2 gi = G.at(i);
         const float from_start = a.scale * __builtin_amdgcn_exp2f(gi.x + gi.y);
-        falls<true>(G, gi, a.scale, lane, f);
 #pragma unroll
-        for (int t = 0; t < 4; ++t)
+        for (int t = 0; t < 4; ++t) {
+            const floatx4 f = falls<true>(G, gi, a.scale, lane, t);
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 const int j = 16 * t + row4 + r;
-                const float x = A[t][r] * f[t][r];
+                const float x = A[t][r] * f[r];
                 A[t][r] = j <= i && i < rows ? x : 0.0f;
             }
+        }
 #pragma unroll
         for (int p = 0; p < S::TP; ++p)
 #pragma unroll
             for (int r = 0; r < 4; ++r) y[p][r] *= from_start;
+        __builtin_amdgcn_sched_barrier(0);
         times(s, __builtin_amdgcn_exp2f((float)all));
         if (finite) {
 #pragma unroll
@@ -800,7 +815,9 @@ __global__ void __launch_bounds__(WG, NP == 128 ? 1 : 2) k_attn_fwd(const Args a
 #pragma unroll
                         for (int x = 0; x < M::TWO; ++x) y[p] = M::mma(fv[p], fa[x], y[p]);
                 }
+                __builtin_amdgcn_sched_barrier(0);
                 update<M, NP, TN::LD>(s, fv, tk, weight, k, lane, wave);
+                __builtin_amdgcn_sched_barrier(0);
             }
         } else {
             product_within<M, M::TWO>(y, false, tv, TV::LD, A, 0, own, lane, [&](int j) { return j <= i && i < rows; });
@@ -816,9 +833,14 @@ __global__ void __launch_bounds__(WG, NP == 128 ? 1 : 2) k_attn_fwd(const Args a
             }
             if constexpr (M::THREE > 1) update_odd<M, NP, TN::LD, TV::LD>(s, tv, tk, weight, lane, wave);
         }
+#pragma unroll
+        for (int p = 0; p < S::TP; ++p) {
+            const float v[4] = {y[p][0], y[p][1], y[p][2], y[p][3]};
+            done[p] = Out::pack(v);
+        }
         __syncthreads();
     }
-    if (c0 < c1) write((c1 - 1) * CHUNK);
+    if (c0 < c1) write((c1 - 1) * CHUNK, threadIdx.x);
     if (a.pieces == 1 && a.state_out != nullptr) s.to_caller(a.state_out + bh * a.key * a.value, a.key, a.value, tile * PV, lane, wave);
 }
 
@@ -848,7 +870,7 @@ struct BwdLds {
 };
 // A workgroup has one chunk, and of a group `in_turn` heads one after another: their queries and keys are read once, and what the
 // heads give to dq and dk is summed in registers.
-template <int DT, int NP, bool TURNS>
+template <int DT, int NP, bool TURNS, bool WIDE>
 __global__ void __launch_bounds__(WG, NP == 128 ? 1 : 2) k_attn_bwd(const Args a) {
     using M = Mat<DT>;
     using E = typename M::E;
@@ -904,7 +926,7 @@ __global__ void __launch_bounds__(WG, NP == 128 ? 1 : 2) k_attn_bwd(const Args a
     floatx4 all_dq[NT] = {}, all_dk[NT] = {};
     bool finite_k = false;
     for (int turn = 0; turn < (TURNS ? a.in_turn : 1); ++turn) {
-        const int lane = TURNS ? here_lane(threadIdx.x & 63) : threadIdx.x & 63, own = TURNS ? here(first_own) : first_own;
+        const int tid = TURNS ? here_lane(threadIdx.x) : threadIdx.x, lane = tid & 63, own = TURNS ? here(first_own) : first_own;
         const int rows = TURNS ? here(all_rows) : all_rows;
         const int l15 = lane & 15, row4 = 4 * (lane >> 4), me = 16 * own + l15;  // the own position, as i of dq and as j of dk and dv
         const int h = h0 + turn;
@@ -913,15 +935,15 @@ __global__ void __launch_bounds__(WG, NP == 128 ? 1 : 2) k_attn_bwd(const Args a
         TN q;
         TV v, d;
         ds.load(a.marks + mark, lane, own);
-        v.load(row_of<DT>(a.v, b, t0, h) + tile * PV, a.v.rs, rows, vcols, a.wide & W_V);
-        d.load(row_of<DT>(a.dy, b, t0, h) + tile * PV, a.dy.rs, rows, vcols, a.wide & W_DY);
+        v.template load<WIDE>(row_of<DT>(a.v, b, t0, h) + tile * PV, a.v.rs, rows, vcols, tid);
+        d.template load<WIDE>(row_of<DT>(a.dy, b, t0, h) + tile * PV, a.dy.rs, rows, vcols, tid);
         s.load(a.fmarks + mark, lane, own);
         const float g_own = decay_at(decays_of(a, b, h) + t0 * a.g.rs, a.g.rs, rows, lane);
-        q.load(row_of<DT>(a.q, b, t0, gr), a.q.rs, rows, a.key, a.wide & W_Q);
+        q.template load<WIDE>(row_of<DT>(a.q, b, t0, gr), a.q.rs, rows, a.key, tid);
         if (turn == 0) {
             TN k;
-            k.load(row_of<DT>(a.k, b, t0, gr), a.k.rs, rows, a.key, a.wide & W_K);
-            k.store(tk);
+            k.template load<WIDE>(row_of<DT>(a.k, b, t0, gr), a.k.rs, rows, a.key, tid);
+            k.store(tk, tid);
             finite_k = k.finite();
         }
         {
@@ -948,8 +970,8 @@ __global__ void __launch_bounds__(WG, NP == 128 ? 1 : 2) k_attn_bwd(const Args a
                 x = wsum(x);
                 if (lane == 0) through[turn & 1][own] = x;
             }
-            v.store(tv);
-            d.store(td);
+            v.store(tv, tid);
+            d.store(td, tid);
             ds.template put<M, M::THREE>(tq, a.key, vcols, lane, own);
             say_finite(said, finite_k && q.finite() && d.finite(), lane, own);
             __syncthreads();
@@ -1014,7 +1036,7 @@ __global__ void __launch_bounds__(WG, NP == 128 ? 1 : 2) k_attn_bwd(const Args a
                 __builtin_amdgcn_sched_barrier(0);
             }
             __syncthreads();
-            q.store(tq);
+            q.store(tq, tid);
             __syncthreads();
             {
                 float x = 0.0f;
@@ -1033,24 +1055,24 @@ __global__ void __launch_bounds__(WG, NP == 128 ? 1 : 2) k_attn_bwd(const Args a
             // the own positions as i: rows are positions j before them
             __builtin_amdgcn_sched_barrier(0);
             {
-                floatx4 A[4], dA[4], f[4];
+                floatx4 A[4], dA[4];
                 scores<M, NP>(A, tk, tq, TN::LD, 16 * own, 0, own, lane);
                 __builtin_amdgcn_sched_barrier(0);
                 scores<M, PV>(dA, tv, td, TV::LD, 16 * own, 0, own, lane);
                 __builtin_amdgcn_sched_barrier(0);
-                falls<true>(G, mine, a.scale, lane, f);
                 // the pairs that a position t of the own ones lies between: of M_ij the sum over the own i >= t, then over j < t; and all
                 // own i for the positions of the tiles before
                 float at = 0.0f;
 #pragma unroll
                 for (int t = 0; t < 4; ++t) {
                     if (t > own) continue;
+                    const floatx4 f = falls<true>(G, mine, a.scale, lane, t);
                     floatx4 sums;
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
                         const int j = 16 * t + row4 + r;
                         const bool in = j <= me && me < rows;
-                        const float x = dA[t][r] * f[t][r], m = A[t][r] * x;
+                        const float x = dA[t][r] * f[r], m = A[t][r] * x;
                         dA[t][r] = in ? x : 0.0f;
                         sums[r] = from_here(in ? m : 0.0f);
                         at += j < me ? sums[r] : 0.0f;
@@ -1071,19 +1093,19 @@ __global__ void __launch_bounds__(WG, NP == 128 ? 1 : 2) k_attn_bwd(const Args a
             // the own positions as j: rows are positions i behind them
             __builtin_amdgcn_sched_barrier(0);
             {
-                floatx4 A[4], dA[4], f[4];
+                floatx4 A[4], dA[4];
                 scores<M, NP>(A, tq, tk, TN::LD, 16 * own, own, 3, lane);
                 __builtin_amdgcn_sched_barrier(0);
                 scores<M, PV>(dA, td, tv, TV::LD, 16 * own, own, 3, lane);
                 __builtin_amdgcn_sched_barrier(0);
-                falls<false>(G, mine, a.scale, lane, f);
 #pragma unroll
                 for (int t = 0; t < 4; ++t) {
+                    const floatx4 f = falls<false>(G, mine, a.scale, lane, t);
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
                         const int i = 16 * t + row4 + r;
                         const bool in = i >= me && i < rows;
-                        const float x = A[t][r] * f[t][r], y = dA[t][r] * f[t][r];
+                        const float x = A[t][r] * f[r], y = dA[t][r] * f[r];
                         A[t][r] = in ? x : 0.0f;
                         dA[t][r] = in ? y : 0.0f;
                     }
@@ -1142,9 +1164,11 @@ __global__ void __launch_bounds__(WG, NP == 128 ? 1 : 2) k_attn_bwd(const Args a
     }
 }
 
-// dq and dk of a group's key from its heads' parts (and those of their value tiles), in their order; dg from its value tiles.
+// dq (blockIdx.y 0) and dk of a group's key from its parts, in their order.
 template <int DT>
-__global__ void __launch_bounds__(WG) k_attn_sum(const Args a, const float* part, Heads out, int groups) {
+__global__ void __launch_bounds__(WG) k_attn_sum(const Args a, int groups) {
+    const float* part = blockIdx.y == 0 ? a.part_q : a.part_k;
+    const Heads out = blockIdx.y == 0 ? a.dq : a.dk;
     const int64_t n = a.batch * a.length * groups * a.key;
     const int each = a.share / a.in_turn * a.tiles;
     for (int64_t i = (int64_t)blockIdx.x * WG + threadIdx.x; i < n; i += (int64_t)gridDim.x * WG) {
@@ -1156,6 +1180,7 @@ __global__ void __launch_bounds__(WG) k_attn_sum(const Args a, const float* part
         row_of<DT>(out, bt / a.length, bt % a.length, gr)[col] = Elem<DT>::st(v);
     }
 }
+// dg from its value tiles.
 __global__ void __launch_bounds__(WG) k_attn_sum_tiles(const float* part, float* out, int64_t n, int tiles) {
     for (int64_t i = (int64_t)blockIdx.x * WG + threadIdx.x; i < n; i += (int64_t)gridDim.x * WG) {
         float v = part[i];
@@ -1331,15 +1356,17 @@ int allow_lds(K* kernel, int bytes) {
     return BOA_OK;
 }
 
+// Calls f with the padded key and whether all inputs are aligned as constants.
 template <class F>
-int with_key(int np, F f) {
-    return np == 64 ? f(std::integral_constant<int, 64>()) : f(std::integral_constant<int, 128>());
+int with_key(int np, bool wide, F f) {
+    const auto with = [&](auto n) { return wide ? f(n, std::true_type()) : f(n, std::false_type()); };
+    return np == 64 ? with(std::integral_constant<int, 64>()) : with(std::integral_constant<int, 128>());
 }
 
 // What the pieces leave, and backward what every chunk's end is reached with.
-template <int DT, int NP, bool BACK>
+template <int DT, int NP, bool BACK, bool WIDE>
 int launch_states(const Args& a, const Plan& p, hipStream_t s) {
-    hipLaunchKernelGGL((k_attn_states<DT, NP, BACK>), dim3((uint32_t)(p.bh * p.tiles * p.pieces)), dim3(WG), 0, s, a);
+    hipLaunchKernelGGL((k_attn_states<DT, NP, BACK, WIDE>), dim3((uint32_t)(p.bh * p.tiles * p.pieces)), dim3(WG), 0, s, a);
     BOA_HIP_TRY(hipGetLastError());
     if (p.pieces > 1) {
         hipLaunchKernelGGL((k_attn_join<NP, BACK>), dim3((uint32_t)(p.bh * p.tiles * (State<NP>::SIZE / (WG * 4)))), dim3(WG), 0, s, a);
@@ -1376,12 +1403,13 @@ extern "C" int boa_linear_attention_fwd(const boa_attention* s, void* d_work, in
     a.marks = s->marks;
     hipStream_t st = (hipStream_t)stream;
     return with_dtype(s->dtype, [&](auto dt) {
-        return with_key(p.np, [&](auto np) {
+        return with_key(p.np, (a.wide & W_FWD) == W_FWD, [&](auto np, auto wide) {
+            constexpr bool WIDE = decltype(wide)::value;
             constexpr int DT = decltype(dt)::value, NP = decltype(np)::value, LDS = FwdLds<DT, NP>::BYTES;
             if (p.pieces > 1)
-                if (const int no = launch_states<DT, NP, false>(a, p, st)) return no;
-            if (const int no = allow_lds(k_attn_fwd<DT, NP>, LDS)) return no;
-            hipLaunchKernelGGL((k_attn_fwd<DT, NP>), dim3((uint32_t)(p.bh * p.tiles * p.pieces)), dim3(WG), LDS, st, a);
+                if (const int no = launch_states<DT, NP, false, WIDE>(a, p, st)) return no;
+            if (const int no = allow_lds(k_attn_fwd<DT, NP, WIDE>, LDS)) return no;
+            hipLaunchKernelGGL((k_attn_fwd<DT, NP, WIDE>), dim3((uint32_t)(p.bh * p.tiles * p.pieces)), dim3(WG), LDS, st, a);
             BOA_HIP_TRY(hipGetLastError());
             return (int)BOA_OK;
         });
@@ -1418,24 +1446,22 @@ extern "C" int boa_linear_attention_bwd(const boa_attention* s, void* d_work, in
     if (s->decay_per_head) a.dg_sum = rest;
     else a.dg = p.tiles > 1 ? rest : s->ddecay;
     return with_dtype(s->dtype, [&](auto dt) {
-        return with_key(p.np, [&](auto np) {
+        return with_key(p.np, (a.wide & W_BACK) == W_BACK, [&](auto np, auto wide) {
+            constexpr bool WIDE = decltype(wide)::value;
             constexpr int DT = decltype(dt)::value, NP = decltype(np)::value, LDS = BwdLds<DT, NP>::BYTES;
-            if (const int no = launch_states<DT, NP, true>(a, p, st)) return no;
+            if (const int no = launch_states<DT, NP, true, WIDE>(a, p, st)) return no;
             const dim3 grid((uint32_t)(p.bh / a.in_turn * p.tiles * p.chunks));
             if (a.in_turn > 1) {
-                if (const int no = allow_lds(k_attn_bwd<DT, NP, true>, LDS)) return no;
-                hipLaunchKernelGGL((k_attn_bwd<DT, NP, true>), grid, dim3(WG), LDS, st, a);
+                if (const int no = allow_lds(k_attn_bwd<DT, NP, true, WIDE>, LDS)) return no;
+                hipLaunchKernelGGL((k_attn_bwd<DT, NP, true, WIDE>), grid, dim3(WG), LDS, st, a);
             } else {
-                if (const int no = allow_lds(k_attn_bwd<DT, NP, false>, LDS)) return no;
-                hipLaunchKernelGGL((k_attn_bwd<DT, NP, false>), grid, dim3(WG), LDS, st, a);
+                if (const int no = allow_lds(k_attn_bwd<DT, NP, false, WIDE>, LDS)) return no;
+                hipLaunchKernelGGL((k_attn_bwd<DT, NP, false, WIDE>), grid, dim3(WG), LDS, st, a);
             }
             BOA_HIP_TRY(hipGetLastError());
             if (a.part_q != nullptr) {
                 const int64_t n = ceil_div(s->batch * s->length * s->groups * s->key, WG);
-                const dim3 grid((uint32_t)(n < MAX_BLOCKS ? n : MAX_BLOCKS));
-                hipLaunchKernelGGL((k_attn_sum<DT>), grid, dim3(WG), 0, st, a, a.part_q, a.dq, s->groups);
-                BOA_HIP_TRY(hipGetLastError());
-                hipLaunchKernelGGL((k_attn_sum<DT>), grid, dim3(WG), 0, st, a, a.part_k, a.dk, s->groups);
+                hipLaunchKernelGGL((k_attn_sum<DT>), dim3((uint32_t)(n < MAX_BLOCKS ? n : MAX_BLOCKS), 2), dim3(WG), 0, st, a, s->groups);
                 BOA_HIP_TRY(hipGetLastError());
             }
             if (a.dg_sum != nullptr) {
