@@ -135,25 +135,35 @@ __global__ void __launch_bounds__(WG) k_sample(const Args a) {
         for (int i = 0; i < PER; ++i) top = max(top, key[i]);
         top = over.largest(top);
         const bool bad = over.count(__popcll(__ballot(nan))) > 0 || top <= KEY_OF_NOTHING || u != u || t != t || p != p || least != least;
-        // The largest key of which `enough` holds, where it holds of all smaller ones: bit by bit, until one symbol is left between the
-        // keys that are known to be enough and those that are not (bits below a 16-bit logit's last are all the same).
+        // The largest key of which `enough` holds, where it holds of all smaller ones: bit by bit, from the first in which the keys
+        // differ, until one symbol is left between those that are known to be enough and those that are not (bits below a
+        // 16-bit logit's last are all the same).
         const auto search = [&](auto enough) {
-            uint32_t last = 0u;
-            int with = a.V, above = 0;  // symbols from `last` on, and from the first key known not to be enough on
             constexpr int LAST_BIT = DT == DT_F32 ? 0 : DT == DT_BF16 ? 16 : 13;
-            for (int bit = 31; bit >= LAST_BIT && with - above > 1; --bit) {
-                const uint32_t c = last | 1u << bit;
+            const auto smallest_from = [&](uint32_t c) {  // as the largest complement
+                uint32_t found = 0u;
+#pragma unroll
+                for (int i = 0; i < PER; ++i) found = max(found, key[i] >= c ? ~key[i] : 0u);
+                return ~over.largest(found);
+            };
+            const auto count_from = [&](uint32_t c) {
                 int n = 0;
 #pragma unroll
                 for (int i = 0; i < PER; ++i) n += __popcll(__ballot(key[i] >= c));
-                n = over.count(n);
+                return over.count(n);
+            };
+            uint32_t last = smallest_from(1u);
+            if (last == top) return last;
+            const int first_bit = 31 - __clz(last ^ top);
+            last &= ~((2u << first_bit) - 1u);
+            int with = count_from(max(last, 1u)), above = 0;  // symbols from `last` on, and from the first key known not to be enough on
+            for (int bit = first_bit; bit >= LAST_BIT && with - above > 1; --bit) {
+                const uint32_t c = last | 1u << bit;
+                const int n = count_from(c);
                 if (enough(c, n)) last = c, with = n;
                 else above = n;
             }
-            uint32_t found = 0u;  // the smallest from there on, as the largest complement
-#pragma unroll
-            for (int i = 0; i < PER; ++i) found = max(found, key[i] >= max(last, 1u) ? ~key[i] : 0u);
-            return ~over.largest(found);
+            return smallest_from(max(last, 1u));
         };
         // keeps of the symbols with this key the first n, by their index
         const auto keep_first = [&](uint32_t of, int n) {
