@@ -588,6 +588,13 @@ def _pack_attention(q, k, v, g, scale, lens, state_in, state_out, marks, y, back
                            *_r4(back[0]), *_r4(back[1]), *_r4(back[2]), *_r4(back[3]), _ptr(dg))
 
 
+def _attention_work(lib, args, backward):
+    size = lib.boa_linear_attention_work_bytes(args, backward)
+    if size < 0:
+        _nat.check(_nat.BOA_ERR_ARG)
+    return size
+
+
 def _attention_fwd(q, k, v, g, scale, state, lens, want_state, keep):
     n, length, heads, value = v.shape
     y = v.new_empty((n, length, heads, value))
@@ -596,7 +603,7 @@ def _attention_fwd(q, k, v, g, scale, state, lens, want_state, keep):
     marks = g.new_empty((n * heads, -(-value // 64), -(-length // 64), -(-q.shape[3] // 64) * 4096)) if keep else None
     args = _pack_attention(q, k, v, g, scale, lens, state, out, marks, y)
     lib = _nat.lib()
-    size = lib.boa_linear_attention_work_bytes(args, 0)
+    size = _attention_work(lib, args, 0)
     work = _work(size, q)
     _call(q, lib.boa_linear_attention_fwd, args, _ptr(work), size)
     return y, out, marks
@@ -620,7 +627,7 @@ class _LinearAttention(torch.autograd.Function):
         dq, dk, dv, dg = (t.new_empty(t.shape) for t in (q, k, v, g))
         args = _pack_attention(q, k, v, g, ctx.scale, lens, None, None, marks, None, (dy, dq, dk, dv), dg)
         lib = _nat.lib()
-        size = lib.boa_linear_attention_work_bytes(args, 1)
+        size = _attention_work(lib, args, 1)
         work = _work(size, q)
         _call(q, lib.boa_linear_attention_bwd, args, _ptr(work), size)
         return dq, dk, dv, dg, None, None, None, None
@@ -735,6 +742,8 @@ def _grads(who, parameters, in_place):
             if not g.is_contiguous():
                 if in_place and any(s == 0 and n > 1 for s, n in zip(g.stride(), g.shape)):
                     raise ValueError(f"{who}: a gradient whose values share memory (strides {g.stride()}) cannot be scaled in place")
+                if in_place and at.count(at[i]) > 1 and at[i]:
+                    raise ValueError(f"{who}: two gradients share memory and cannot be scaled in place")
                 grads[i] = g.contiguous()
                 at[i] = grads[i].data_ptr()
                 copies.append((g, grads[i]))
@@ -803,7 +812,7 @@ def _limit(who, name, v, shape, like, dtype, lo, hi):
     if not isinstance(v, _Tensor):
         if not lo <= v <= hi:
             raise ValueError(f"{who}: {name} must be {lo} to {hi} (got {v})")
-        return v, None
+        return operator.index(v) if dtype is torch.int32 else float(v), None
     if v.dtype is not dtype:
         raise TypeError(f"{who}: {name} must be a number or a {dtype} tensor (got {v.dtype})")
     if v.shape != shape or v.get_device() != like.get_device():
@@ -821,7 +830,7 @@ def sample(logits, u, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     Each limit is a number, or a tensor of the leading shape (float32; top_k int32, where 0 or less keeps all).  A row that is no
     distribution (a NaN in it or its numbers, nothing above -inf) gives -1.  No gradient."""
     who = "sample"
-    _plain(who, logits, u)
+    _plain(who, logits, u, temperature, top_p, min_p)
     _act(who, "logits", logits)
     if logits.ndim < 1 or not 1 <= logits.shape[-1] <= _nat.BOA_SAMPLE_MAX_V:
         raise ValueError(f"{who}: logits must be [..., V] with 1 <= V <= {_nat.BOA_SAMPLE_MAX_V} (got {list(logits.shape)})")

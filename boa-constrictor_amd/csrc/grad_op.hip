@@ -23,6 +23,7 @@ constexpr int MOST = 180;        // tensors of a launch: 21 bytes each of the 4 
 constexpr int MAX_GROUPS = 1024;  // workgroups of a norm launch, and its partial sums
 constexpr int AT_ONCE = 4;        // accesses of 16 bytes that a thread has in flight
 constexpr int SPAN = WG * AT_ONCE * 16;  // bytes of a block
+constexpr int64_t MOST_BYTES = INT64_C(1) << 39;  // of a tensor
 
 struct Table {
     void* p[MOST];          // down to a multiple of 16 bytes
@@ -161,8 +162,8 @@ int check_grads(const char* who, int32_t n, const void* const* grads, const int6
     if (n < 0 || (n > 0 && (!grads || !counts || !dtypes))) return boa_fail(BOA_ERR_ARG, "%s: null pointer", who);
     for (int32_t i = 0; i < n; ++i) {
         if (dtypes[i] < BOA_DT_F32 || dtypes[i] > BOA_DT_F16) return boa_fail(BOA_ERR_ARG, "%s: unknown type %d", who, dtypes[i]);
-        // a tensor's blocks are counted in 32 bits
-        if (counts[i] < 0 || counts[i] > INT64_C(1) << 40 || (counts[i] > 0 && !grads[i]) || (uintptr_t)grads[i] % element_bytes(dtypes[i]))
+        // blocks are counted in 32 bits; no tensor is longer than a device's memory
+        if (counts[i] < 0 || counts[i] > MOST_BYTES / element_bytes(dtypes[i]) || (counts[i] > 0 && !grads[i]) || (uintptr_t)grads[i] % element_bytes(dtypes[i]))
             return boa_fail(BOA_ERR_ARG, "%s: tensor %d of %lld values at %p", who, i, (long long)counts[i], grads[i]);
     }
     if (!work || (uintptr_t)work % 8 || work_bytes < boa_grad_norm_work_bytes(n))
@@ -218,10 +219,10 @@ int with_norm(int largest, F f) {
 
 }  // namespace
 
-// The partial sums of as many launches as n tensors may take: one for MOST of them, and one more for each that is too long to go
-// with others.
+// The partial sums of as many launches as n tensors may take: one for MOST of them, and more where 63 or more of the longest fill
+// one (2^25 blocks each of 2^31).
 extern "C" int64_t boa_grad_norm_work_bytes(int32_t n) {
-    return (n > 0 ? 2 * ceil_div(n, MOST) + 1 : 1) * (int64_t)MAX_GROUPS * (int64_t)sizeof(double);
+    return (n > 0 ? 3 * ceil_div(n, MOST) + 1 : 1) * (int64_t)MAX_GROUPS * (int64_t)sizeof(double);
 }
 
 extern "C" int boa_grad_norm(int32_t n, const void* const* d_grads, const int64_t* counts, const int32_t* dtypes, int largest, float* d_norm,

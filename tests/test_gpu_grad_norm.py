@@ -148,6 +148,21 @@ def test_gradients_that_share_memory_are_refused(gpu):
     ops.grad_norm(params)
 
 
+def test_a_gradient_given_twice_that_is_not_contiguous_is_refused(gpu):
+    p, = _params([(64, 32)], 8)
+    p.grad = p.grad.t().contiguous().t()
+    before = p.grad.clone()
+    with pytest.raises(ValueError, match="share memory"):
+        ops.clip_grad_norm_([p, p], 0.1)
+    assert torch.equal(p.grad, before)
+    p.grad = p.grad.t().contiguous().t()
+    q = torch.nn.Parameter(torch.zeros(32, 64, device="cuda"))
+    q.grad = p.grad.t()
+    with pytest.raises(ValueError, match="share memory"):
+        ops.clip_grad_norm_([q, p], 0.1)
+    assert torch.equal(p.grad, before)
+
+
 def test_autograd_sees_that_gradients_were_scaled(gpu):
     p, = _params([(10,)], 9)
     version = p.grad._version

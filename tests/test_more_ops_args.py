@@ -3,6 +3,7 @@ import array
 import ctypes
 import math
 
+import numpy as np
 import pytest
 import torch
 from torch.autograd import forward_ad
@@ -276,3 +277,35 @@ def test_generate_refuses():
             m.generate(*args, **kw)
     with pytest.raises(ValueError, match="on the GPU"):
         m.generate(x, 4)
+
+
+def test_limits_are_numbers_of_their_kind():
+    like, shape = torch.zeros(2, 256), (2,)
+    for v in (5.0, np.float32(5), "5"):
+        with pytest.raises(TypeError):
+            ops._limit("sample", "top_k", v, shape, like, torch.int32, 0, 9)
+    for v in (np.int64(5), np.uint8(5), 5):
+        got, none = ops._limit("sample", "top_k", v, shape, like, torch.int32, 0, 9)
+        assert type(got) is int and got == 5 and none is None
+    for v in (np.float32(0.5), np.float64(0.5), 0.5):
+        got, none = ops._limit("sample", "top_p", v, shape, like, torch.float32, 0.0, 1.0)
+        assert type(got) is float and got == 0.5 and none is None
+    for name in ("temperature", "top_p", "min_p"):
+        with forward_ad.dual_level(), pytest.raises(RuntimeError, match="forward-mode"):
+            ops.sample(like, torch.zeros(2), **{name: forward_ad.make_dual(torch.ones(2), torch.ones(2))})
+
+
+def test_c_tensors_longer_than_any_memory():
+    lib = _native.load_cdll()
+    work, norm = ctypes.c_void_p(16), ctypes.c_void_p(16)
+    for dtype, n in ((0, (1 << 37) + 1), (1, (1 << 38) + 1), (2, (1 << 38) + 1)):
+        a = (array.array("q", [64]).tobytes(), array.array("q", [n]).tobytes(), array.array("i", [dtype]).tobytes())
+        size = lib.boa_grad_norm_work_bytes(1)
+        assert lib.boa_grad_norm(1, *a, 0, norm, work, size, None) == _native.BOA_ERR_ARG
+        assert lib.boa_clip_grads(1, *a, 0, 1.0, norm, work, size, None) == _native.BOA_ERR_ARG
+
+
+def test_more_sequences_than_a_launch_takes_are_named(monkeypatch):
+    monkeypatch.setattr(_native, "_lib", _native.load_cdll())
+    with pytest.raises(ValueError, match="too many for a launch"):
+        ops._attention_work(_native._lib, _packed(n=1 << 40), 0)
