@@ -23,6 +23,12 @@
 // Everywhere a wavefront has 16 columns of a product's result: its own 16 positions i (or j) in what is made of A and dA, so that
 // these stay in its registers, where a result tile (column in the lane, four consecutive rows per lane) is the next product's
 // operand as it is; its own 16 of every 64 keys in a state.
+//
+// Measured with 64 keys and 64 values a head (copies of the sizes moved here reach 5 to 6 TB/s, float32 products of libraries 150
+// TFLOP/s), kernels in us; 4 x 4097 positions x 16 heads of 4 groups in bfloat16: states 22, joined 6, forward 50 (136 MB and as
+// much of k and v again); 2 x 16384 x 8 heads in float32: forward 38 + 7 + 110, backward 44 + 7 + 254 (539 MB, and 27 GFLOP of
+// products, 183 us at the libraries' rate); 32 x 500 x 16 heads of 4 groups in bfloat16: forward 44, backward 21 + 109; one position
+// of 1000 x 16 heads: 83 (532 MB, 6.4 TB/s).  What bounds each stands at its kernel.
 #include "ops_common.h"
 
 #include "../../include/boa_hip.h"
@@ -74,7 +80,7 @@ template <int DT> struct Mat {
     using E = float;
     using Frag = f32x4;
     static constexpr int STEP = 16, VEC = 4, TWO = 1, THREE = 1, PAD = 4;
-    static constexpr bool SKIP = true;  // tiles that are all zero are left out: the matrix cores bound it
+    static constexpr bool SKIP = true;  // all-zero tiles are left out: 2 x 16384 x 8 backward 293 -> 254 us
     static __device__ __forceinline__ floatx4 mma(const Frag& a, const Frag& b, floatx4 c) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[i], b[i], c, 0, 0, 0);
@@ -115,7 +121,7 @@ template <> struct Mat<DT_BF16> {
     using E = uint16_t;
     using Frag = bf16x8;
     static constexpr int STEP = 32, VEC = 8, TWO = 2, THREE = 3, PAD = 8;
-    static constexpr bool SKIP = false;  // branches would cost more
+    static constexpr bool SKIP = false;  // a step is two tiles, and takes an eighth of float32's time a tile
     static __device__ __forceinline__ floatx4 mma(const Frag& a, const Frag& b, floatx4 c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
     }
@@ -276,7 +282,8 @@ struct Tile {
     static_assert(WG % ROW == 0, "");
     static constexpr int LD = COLS + M::PAD, SIZE = CHUNK * LD;
     u32x4 v[PER];
-    // rows from p on, `rows` and `cols` of them; WIDE: aligned for accesses of 16 bytes
+    // rows from p on, `rows` and `cols` of them; WIDE: aligned for accesses of 16 bytes (the other way takes 1.5 to 2.7 times a
+    // kernel's time on the same data: prompt of 4 x 4097 x 16 heads in bfloat16 114 + 62 us for 50 + 22)
     template <bool WIDE>
     __device__ __forceinline__ void load(const T* p, int64_t stride, int rows, int cols, int tid) {
         const int r0 = tid / ROW, c = tid % ROW * V;  // WG / ROW rows apart
@@ -510,7 +517,9 @@ __device__ __forceinline__ void times(State<NP>& s, float f) {
 
 // ---- states by themselves ---------------------------------------------------------------------------
 // A workgroup walks the chunks of a piece from a state of zeros, forward over k v^T or (BACK) from the last one over scale e^(G_i)
-// q dy^T; leaves what it ends with, and backward also what it reaches each chunk with.
+// q dy^T; leaves what it ends with, and backward also what it reaches each chunk with.  The state stays in registers; two
+// workgroups on a CU hide each other's loads.  A chunk takes a workgroup about 2.7 us, of which a product of 64 x 64 x 64 is the
+// smallest part: it waits for the next chunk's loads and LDS (k and v at 4.1 TB/s in bfloat16, 3.7 in float32 over 2 x 16384 x 8).
 template <int DT, int NP, bool BACK, bool WIDE>
 __global__ void __launch_bounds__(WG, 2) k_attn_states(const Args a) {
     using M = Mat<DT>;
@@ -590,7 +599,8 @@ __global__ void __launch_bounds__(WG, 2) k_attn_states(const Args a) {
 }
 
 // What each piece leaves by itself becomes the state that it starts from (backward: the gradient of the state behind it), eight
-// pieces' loads at a time.  A thread has four values of a state.
+// pieces' loads at a time.  A thread has four values of a state.  Bound by the latency of loads that follow one another: 6 to 7 us
+// for the 8 to 32 pieces that fill the card.
 template <int NP, bool BACK>
 __global__ void __launch_bounds__(WG) k_attn_join(const Args a) {
     using S = State<NP>;
@@ -668,6 +678,10 @@ __device__ __forceinline__ void zero_rows(const Heads& x, int64_t b, int h, int 
 }
 
 // ---- forward ------------------------------------------------------------------------------------------
+// A workgroup walks a piece with the state in registers, and lays it into LDS (split in two parts for bfloat16) for the product
+// with q; the next chunk's q, k and v are loaded into registers while this one's products run.  Bound in bfloat16 by vector work
+// (56% of the SIMDs' time: decays, splits, masks) and LDS, at 2.7 TB/s of inputs and results; in float32 by the matrix cores' rate
+// for it and LDS together, 110 us for 16 GFLOP.
 template <int DT, int NP>
 struct FwdLds {
     using M = Mat<DT>;
@@ -868,6 +882,10 @@ struct BwdLds {
     static constexpr int Q = 0, K = ONE, V = K + Tile<DT, NP>::SIZE, D = V + Tile<DT, PV>::SIZE;
     static constexpr int BYTES = (int)sizeof(typename M::E) * (D + Tile<DT, PV>::SIZE);
 };
+// The products of one chunk take no turn behind another's, so there is a workgroup for each and nothing is carried: 4096 of them at
+// 2 x 16384 x 8 in float32, 254 us of which the matrix cores are busy for 100; loads at a chunk's start take a quarter, and two
+// workgroups on a CU (LDS allows no third) hide half of each other's.  Walking chunks with the next one's tiles loaded ahead needs
+// more registers than there are.
 // A workgroup has one chunk, and of a group `in_turn` heads one after another: their queries and keys are read once, and what the
 // heads give to dq and dk is summed in registers.
 template <int DT, int NP, bool TURNS, bool WIDE>
@@ -1191,7 +1209,8 @@ __global__ void __launch_bounds__(WG) k_attn_sum_tiles(const float* part, float*
 
 // ---- one position -------------------------------------------------------------------------------------
 // A workgroup per head of a sequence: a thread has VEC values of every ROWS-th row of the state, read and written once; the rows'
-// products with q are summed over the wavefront's lanes, then through LDS.
+// products with q are summed over the wavefront's lanes, then through LDS.  Bound by memory: 1000 x 16 heads of 64 x 64 take 83 us
+// (6.4 TB/s) with accesses of 16 bytes, 121 with those of 4.
 template <int DT, int VEC>
 __global__ void __launch_bounds__(WG) k_attn_step(const Args a) {
     constexpr int LANES = 64 / VEC, ROWS = WG / LANES, AT_ONCE = 4;  // lanes of a row of PV values, rows at a time
@@ -1258,7 +1277,9 @@ bool wide_rows(int dtype, const boa_heads& x, int cols) {
             (uintptr_t)(cols * es)) % 16 == 0;
 }
 
-// The split: pieces of whole chunks, as many as give the wanted workgroups.
+// The split: pieces of whole chunks, as many as give the wanted workgroups, two for each CU.  Forward of 4 x 4097 x 16 heads in
+// bfloat16 with 256, 512, 768 and 1024 wanted: 92, 61, 73 and 67 us; of 2 x 16384 x 8 in float32: 153, 125, 165 and 126.  Backward
+// 1024 and 512 take the same time walking, but joining 13 us against 7.5.
 constexpr int64_t WANTED = 512;
 struct Plan {
     int np, tiles;
@@ -1296,6 +1317,7 @@ struct Plan {
 };
 
 // Heads of a group that a workgroup of the backward pass takes in turn: as many as leave two for each CU twice over.
+// 32 x 500 x 16 heads of 4 groups: 109 us so, 135 + 45 for the sums over heads with each head by itself, 121 + 36 with two in turn.
 int in_turn(const boa_attention& s, const Plan& p) {
     const int share = s.heads / s.groups;
     for (int n = share; n > 1; --n)
