@@ -1,21 +1,25 @@
-"""Operators of the model's training pass and of its streaming by single tokens, on GPU tensors.
+"""Operators of a model's training pass and of its streaming by single tokens, on GPU tensors.
 
   layer_norm          rows of d values, weight and bias (nn.LayerNorm of model.py:45,51)
   causal_conv         the mixer's depthwise convolution over 4 positions with SiLU (model.py:72)
   selective_scan      the mixer's state space recurrence with its gate (model.py:72-81)
   cross_entropy       next-byte loss in nats (train.py:59-63)
-  causal_conv_step, selective_scan_step   one token per sequence, states advanced in place
+  linear_attention    a recurrence like the scan's whose state is a key x value matrix per head
+  causal_conv_step, selective_scan_step, linear_attention_step   one token per sequence, states advanced in place
+  grad_norm, clip_grad_norm_   the norm of all gradients together, and their scaling by it (before optimizer.step() of train.py:63)
+  sample              next symbols drawn from logits by given random numbers, with temperature, top_k, top_p and min_p
 
 All of them run hand-written kernels of libboa_hip.so (include/boa_hip.h) on the current stream of their tensors' device,
-synchronize nothing and can be captured into a graph.  The first four are differentiable (once, backward): gradients reach
+synchronize nothing and can be captured into a graph.  The first five are differentiable (once, backward): gradients reach
 every floating input but the states; inputs with a tangent of forward-mode differentiation are refused, and so is every call
 that torch.jit.trace or make_fx records.  Activations are float32, bfloat16 or float16, all of a call of the same type; parameters,
 scan states and the gradients of parameters are float32; arithmetic is in float32 and each result is rounded once.  The same
 inputs give the same bits.
 
 Shapes: activations [batch, length, channels] with any batch and row strides (a last dimension that is not contiguous is
-copied); conv states [batch, 3, channels] in the activations' type, oldest position first; scan states
-[batch, 16, channels] float32; ``lens``: int32 [batch], the sequences' lengths in a padded batch.  Positions behind a
+copied), of linear attention [batch, length, heads, key or value] with any strides but the last; conv states
+[batch, 3, channels] in the activations' type, oldest position first; scan states [batch, 16, channels] and attention's
+[batch, heads, key, value] float32; ``lens``: int32 [batch], the sequences' lengths in a padded batch.  Positions behind a
 sequence's end are not read (they may hold anything) and come out, and have gradients, as zeros; a state handed on is the one
 behind the sequence's last position, so a sequence of length 0 hands on the state that it was given.
 

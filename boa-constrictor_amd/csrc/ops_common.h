@@ -1,5 +1,6 @@
-// Shared parts of the training and single-token operators (norm_op.hip, loss_op.hip, conv_op.hip, scan_op.hip): element
-// types, row loads and stores, sums over a wavefront without the LDS, and the sum of partial rows.
+// Shared parts of the training and single-token operators (norm_op.hip, loss_op.hip, conv_op.hip, scan_op.hip, attn_op.hip,
+// grad_op.hip, sample_op.hip): element types, row loads and stores, sums and scans over a wavefront without the LDS, and the sum of
+// partial rows.
 //
 // Every operator takes its activations as float32, bfloat16 or float16 and computes in float32; a result is rounded to the
 // activations' type once, when it is stored.  Parameters, their gradients, states and statistics are float32.
