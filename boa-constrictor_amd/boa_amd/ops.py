@@ -718,7 +718,8 @@ def linear_attention_step(q, k, v, log_decay, *, state, scale=None):
 
 # ---- gradient norm ---------------------------------------------------------------------------------
 # A model has hundreds of gradients, and each look at one costs Python 70 ns: few looks, without calls of functions of our own.
-_grad_of, _contiguous, _address, _size = operator.attrgetter("grad"), _Tensor.is_contiguous, _Tensor.data_ptr, _Tensor.numel
+_grad_of, _type_of = operator.attrgetter("grad"), operator.attrgetter("dtype")
+_contiguous, _address, _size = _Tensor.is_contiguous, _Tensor.data_ptr, _Tensor.numel
 
 
 def _grads(who, parameters, in_place):
@@ -732,7 +733,8 @@ def _grads(who, parameters, in_place):
         return grads, None, copies, None
     _plain(who, *grads)
     try:
-        codes = [_DTYPES[g.dtype] for g in grads]
+        types = set(map(_type_of, grads))
+        codes = [_DTYPES[types.pop()]] * len(grads) if len(types) == 1 else [_DTYPES[g.dtype] for g in grads]
         at = list(map(_address, grads))
     except (KeyError, RuntimeError):  # sparse ones have no address
         raise TypeError(f"{who}: gradients must be dense float32, bfloat16 or float16 "
