@@ -25,7 +25,7 @@
 // operand as it is; its own 16 of every 64 keys in a state.
 //
 // Measured with 64 keys and 64 values a head (copies of the sizes moved here reach 5 to 6 TB/s, float32 products of libraries 150
-// TFLOP/s), kernels in us; 4 x 4097 positions x 16 heads of 4 groups in bfloat16: states 22, joined 6, forward 50 (136 MB and as
+// TFLOP/s), kernels in us; 4 x 4097 positions x 16 heads of 4 groups in bfloat16: states 21, joined 6, forward 50 (136 MB and as
 // much of k and v again); 2 x 16384 x 8 heads in float32: forward 38 + 7 + 110, backward 44 + 7 + 254 (539 MB, and 27 GFLOP of
 // products, 183 us at the libraries' rate); 32 x 500 x 16 heads of 4 groups in bfloat16: forward 44, backward 21 + 109; one position
 // of 1000 x 16 heads: 83 (532 MB, 6.4 TB/s).  What bounds each stands at its kernel.
@@ -64,9 +64,7 @@ struct Args {
     int64_t batch, length, chunks;
     int32_t heads, share, in_turn, key, value, tiles, pieces, per_piece;
     float scale;
-    uint32_t wide;  // bit per tensor: read or written 16 bytes at a time (W_*)
 };
-enum { W_Q = 1, W_K = 2, W_V = 4, W_DY = 8, W_Y = 16, W_DQ = 32, W_DK = 64, W_DV = 128, W_FWD = W_Q | W_K | W_V, W_BACK = W_FWD | W_DY };
 
 // How products of a type run: elements in LDS, K of a step, parts that a float32 value is split into.
 //   bfloat16: inputs as they are.  What is computed on the way (A, dA, states, decayed keys) is split into parts of 8 bits each:
@@ -273,6 +271,20 @@ __device__ __forceinline__ int here_lane(int x) {
     return x;
 }
 
+// 16 bytes at any element's address: the hardware takes them as it takes aligned ones.
+typedef u32x4 AnyAt __attribute__((aligned(2)));
+// The value without its first n elements of ES bytes (fewer than 16 bytes); zeros behind.
+template <int ES>
+__device__ __forceinline__ u32x4 shifted(u32x4 v, int n) {
+    if (n & (8 / ES)) v = u32x4{v[2], v[3], 0u, 0u};
+    if (n & (4 / ES)) v = u32x4{v[1], v[2], v[3], 0u};
+    if constexpr (ES == 2)
+        if (n & 1)
+            v = u32x4{__builtin_amdgcn_alignbit(v[1], v[0], 16), __builtin_amdgcn_alignbit(v[2], v[1], 16), __builtin_amdgcn_alignbit(v[3], v[2], 16),
+                      v[3] >> 16};
+    return v;
+}
+
 // A tile of CHUNK rows and COLS columns on its way from memory to LDS; zeros behind the last row and column.
 template <int DT, int COLS>
 struct Tile {
@@ -282,35 +294,44 @@ struct Tile {
     static_assert(WG % ROW == 0, "");
     static constexpr int LD = COLS + M::PAD, SIZE = CHUNK * LD;
     u32x4 v[PER];
-    // rows from p on, `rows` and `cols` of them; WIDE: aligned for accesses of 16 bytes (the other way takes 1.5 to 2.7 times a
-    // kernel's time on the same data: prompt of 4 x 4097 x 16 heads in bfloat16 114 + 62 us for 50 + 22)
-    template <bool WIDE>
+    // rows from p on, `rows` and `cols` of them; EVEN: cols are a multiple of V.  A row's last access, where it would pass the row's
+    // end, is one that ends there, shifted down.  On the same data (all cases above) that takes 1 to 30% longer than EVEN, and
+    // element by element 1.5 to 2.7 times as long.
+    template <bool EVEN>
     __device__ __forceinline__ void load(const T* p, int64_t stride, int rows, int cols, int tid) {
         const int r0 = tid / ROW, c = tid % ROW * V;  // WG / ROW rows apart
         p += r0 * stride + c;
-        if (WIDE && rows == CHUNK && cols == COLS) {
+        if (EVEN && rows == CHUNK && cols == COLS) {
 #pragma unroll
-            for (int i = 0; i < PER; ++i) v[i] = *reinterpret_cast<const u32x4*>(p + i * (WG / ROW * stride));
+            for (int i = 0; i < PER; ++i) v[i] = *reinterpret_cast<const AnyAt*>(p + i * (WG / ROW * stride));
             return;
         }
         cols = here(cols);
 #pragma unroll
-        for (int i = 0; i < PER; ++i) {
-            v[i] = u32x4{0u, 0u, 0u, 0u};
-            const T* q = p + i * (WG / ROW * stride);
-            if (r0 + i * (WG / ROW) < rows && c < cols) {
-                if constexpr (WIDE) {
-                    v[i] = *reinterpret_cast<const u32x4*>(q);
-                } else {
+        for (int i = 0; i < PER; ++i) v[i] = u32x4{0u, 0u, 0u, 0u};
+        if (c >= cols) return;
+        if (EVEN || cols >= V) {
+            const int over = EVEN ? 0 : max(c + V - cols, 0);
+            p -= over;
 #pragma unroll
-                    for (int e = 0; e < V; ++e)
-                        if (c + e < cols) {
+            for (int i = 0; i < PER; ++i)
+                if (r0 + i * (WG / ROW) < rows) v[i] = *reinterpret_cast<const AnyAt*>(p + i * (WG / ROW * stride));
+            if constexpr (!EVEN)
+#pragma unroll
+                for (int i = 0; i < PER; ++i) v[i] = shifted<sizeof(T)>(v[i], over);
+        } else {
+#pragma unroll
+            for (int i = 0; i < PER; ++i) {
+                const T* q = p + i * (WG / ROW * stride);
+                if (r0 + i * (WG / ROW) < rows)
+#pragma unroll
+                    for (int e = 0; e < V - 1; ++e)
+                        if (e < cols) {
                             if constexpr (sizeof(T) == 4) v[i][e] = __float_as_uint(q[e]);
                             else v[i][e / 2] |= (uint32_t)q[e] << (16 * (e & 1));
                         }
-                }
+                __builtin_amdgcn_sched_barrier(0);  // else all elements' loads are on their way at once, in registers of their own
             }
-            __builtin_amdgcn_sched_barrier(0);  // else all elements' loads are on their way at once, in registers of their own
         }
     }
     // An exponent of ones and one more carry into the sign's place.
@@ -520,7 +541,7 @@ __device__ __forceinline__ void times(State<NP>& s, float f) {
 // q dy^T; leaves what it ends with, and backward also what it reaches each chunk with.  The state stays in registers; two
 // workgroups on a CU hide each other's loads.  A chunk takes a workgroup about 2.7 us, of which a product of 64 x 64 x 64 is the
 // smallest part: it waits for the next chunk's loads and LDS (k and v at 4.1 TB/s in bfloat16, 3.7 in float32 over 2 x 16384 x 8).
-template <int DT, int NP, bool BACK, bool WIDE>
+template <int DT, int NP, bool BACK, bool EVEN>
 __global__ void __launch_bounds__(WG, 2) k_attn_states(const Args a) {
     using M = Mat<DT>;
     using TX = Tile<DT, NP>;
@@ -552,8 +573,8 @@ __global__ void __launch_bounds__(WG, 2) k_attn_states(const Args a) {
     const auto fetch = [&](int64_t c, int tid) {
         const int64_t t0 = c * CHUNK;
         const int rows = (int)min((int64_t)CHUNK, end - t0);
-        x.template load<WIDE>(xp + t0 * X.rs, X.rs, rows, a.key, tid);
-        y.template load<WIDE>(yp + t0 * Y.rs, Y.rs, rows, vcols, tid);
+        x.template load<EVEN>(xp + t0 * X.rs, X.rs, rows, a.key, tid);
+        y.template load<EVEN>(yp + t0 * Y.rs, Y.rs, rows, vcols, tid);
         g_own = decay_at(gp + t0 * a.g.rs, a.g.rs, rows, tid & 63);
     };
     const int64_t n = c1 - c0;
@@ -643,10 +664,11 @@ __global__ void __launch_bounds__(WG) k_attn_join(const Args a) {
 
 // Four consecutive columns of a row of a result.
 template <int DT>
-__device__ __forceinline__ void write4(typename Elem<DT>::T* p, int col, int cols, bool wide16, floatx4 v) {
-    if (wide16 && col < cols) {
+__device__ __forceinline__ void write4(typename Elem<DT>::T* p, int col, int cols, floatx4 v) {
+    if (col + 4 <= cols) {
+        using Any __attribute__((aligned(2))) = typename Raw<DT, 4>::V;
         const float f[4] = {v[0], v[1], v[2], v[3]};
-        st_vec<DT, 4>(p + col, f);
+        *reinterpret_cast<Any*>(p + col) = Raw<DT, 4>::pack(f);
     } else {
 #pragma unroll
         for (int r = 0; r < 4; ++r)
@@ -655,17 +677,16 @@ __device__ __forceinline__ void write4(typename Elem<DT>::T* p, int col, int col
 }
 // A row of dq or dk, where it is one head's own, or its part of a sum.
 template <int DT, int NT>
-__device__ __forceinline__ void write_key(float* part, typename Elem<DT>::T* out, int key, bool wide16, int row4, const floatx4 (&v)[NT]) {
+__device__ __forceinline__ void write_key(float* part, typename Elem<DT>::T* out, int key, int row4, const floatx4 (&v)[NT]) {
     if (part != nullptr) {
-        const bool four = key % 4 == 0;
 #pragma unroll
-        for (int n = 0; n < NT; ++n) write4<DT_F32>(part, 16 * n + row4, here(key), four, v[n]);
-    } else if (wide16 && key == 16 * NT) {
+        for (int n = 0; n < NT; ++n) write4<DT_F32>(part, 16 * n + row4, here(key), v[n]);
+    } else if (key == 16 * NT) {
 #pragma unroll
-        for (int n = 0; n < NT; ++n) write4<DT>(out, 16 * n + row4, 16 * NT, true, v[n]);
+        for (int n = 0; n < NT; ++n) write4<DT>(out, 16 * n + row4, 16 * NT, v[n]);
     } else {
 #pragma unroll
-        for (int n = 0; n < NT; ++n) write4<DT>(out, 16 * n + row4, here(key), false, v[n]);
+        for (int n = 0; n < NT; ++n) write4<DT>(out, 16 * n + row4, here(key), v[n]);
     }
 }
 // Zeros in the columns col0 .. of the rows [from, to).
@@ -688,7 +709,7 @@ struct FwdLds {
     static constexpr int Q = 0, K = Tile<DT, NP>::SIZE, V = 2 * K, S = V + Tile<DT, PV>::SIZE, LDS_STATE = PV + M::PAD, PART = NP * LDS_STATE;
     static constexpr int BYTES = (int)sizeof(typename M::E) * (S + M::TWO * PART);
 };
-template <int DT, int NP, bool WIDE>
+template <int DT, int NP, bool EVEN>
 __global__ void __launch_bounds__(WG, NP == 128 ? 1 : 2) k_attn_fwd(const Args a) {
     using M = Mat<DT>;
     using E = typename M::E;
@@ -733,9 +754,9 @@ __global__ void __launch_bounds__(WG, NP == 128 ? 1 : 2) k_attn_fwd(const Args a
     const auto fetch = [&](int64_t c, int tid) {
         const int64_t t0 = c * CHUNK;
         const int rows = (int)min((int64_t)CHUNK, end - t0);
-        q.template load<WIDE>(qp + t0 * a.q.rs, a.q.rs, rows, a.key, tid);
-        k.template load<WIDE>(kp + t0 * a.k.rs, a.k.rs, rows, a.key, tid);
-        v.template load<WIDE>(vp + t0 * a.v.rs, a.v.rs, rows, vcols, tid);
+        q.template load<EVEN>(qp + t0 * a.q.rs, a.q.rs, rows, a.key, tid);
+        k.template load<EVEN>(kp + t0 * a.k.rs, a.k.rs, rows, a.key, tid);
+        v.template load<EVEN>(vp + t0 * a.v.rs, a.v.rs, rows, vcols, tid);
         g_own = decay_at(gp + t0 * a.g.rs, a.g.rs, rows, tid & 63);
     };
     // a chunk's results are written while the next one is on: what has been stored late would be waited for with the next tiles
@@ -746,18 +767,21 @@ __global__ void __launch_bounds__(WG, NP == 128 ? 1 : 2) k_attn_fwd(const Args a
         const int64_t t = t0 + 16 * own + (tid & 15);
         if (t >= end) return;
         auto* out = yp + t * a.y.rs + row4;
-        if ((a.wide & W_Y) && vcols == PV) {
+        using Any __attribute__((aligned(2))) = typename Out::V;
+        if (vcols == PV) {
 #pragma unroll
-            for (int p = 0; p < S::TP; ++p) *reinterpret_cast<typename Out::V*>(out + 16 * p) = done[p];
+            for (int p = 0; p < S::TP; ++p) *reinterpret_cast<Any*>(out + 16 * p) = done[p];
         } else {
 #pragma unroll
             for (int p = 0; p < S::TP; ++p) {
-                const int cols = here(vcols);
+                const int cols = here(vcols) - 16 * p - row4;
                 float v[4];
                 Out::unpack(done[p], v);
+                if (cols >= 4) *reinterpret_cast<Any*>(out + 16 * p) = done[p];
+                else
 #pragma unroll
-                for (int r = 0; r < 4; ++r)
-                    if (16 * p + row4 + r < cols) out[16 * p + r] = Elem<DT>::st(v[r]);
+                    for (int r = 0; r < 3; ++r)
+                        if (r < cols) out[16 * p + r] = Elem<DT>::st(v[r]);
             }
         }
     };
@@ -888,7 +912,7 @@ struct BwdLds {
 // more registers than there are.
 // A workgroup has one chunk, and of a group `in_turn` heads one after another: their queries and keys are read once, and what the
 // heads give to dq and dk is summed in registers.
-template <int DT, int NP, bool TURNS, bool WIDE>
+template <int DT, int NP, bool TURNS, bool EVEN>
 __global__ void __launch_bounds__(WG, NP == 128 ? 1 : 2) k_attn_bwd(const Args a) {
     using M = Mat<DT>;
     using E = typename M::E;
@@ -953,14 +977,14 @@ __global__ void __launch_bounds__(WG, NP == 128 ? 1 : 2) k_attn_bwd(const Args a
         TN q;
         TV v, d;
         ds.load(a.marks + mark, lane, own);
-        v.template load<WIDE>(row_of<DT>(a.v, b, t0, h) + tile * PV, a.v.rs, rows, vcols, tid);
-        d.template load<WIDE>(row_of<DT>(a.dy, b, t0, h) + tile * PV, a.dy.rs, rows, vcols, tid);
+        v.template load<EVEN>(row_of<DT>(a.v, b, t0, h) + tile * PV, a.v.rs, rows, vcols, tid);
+        d.template load<EVEN>(row_of<DT>(a.dy, b, t0, h) + tile * PV, a.dy.rs, rows, vcols, tid);
         s.load(a.fmarks + mark, lane, own);
         const float g_own = decay_at(decays_of(a, b, h) + t0 * a.g.rs, a.g.rs, rows, lane);
-        q.template load<WIDE>(row_of<DT>(a.q, b, t0, gr), a.q.rs, rows, a.key, tid);
+        q.template load<EVEN>(row_of<DT>(a.q, b, t0, gr), a.q.rs, rows, a.key, tid);
         if (turn == 0) {
             TN k;
-            k.template load<WIDE>(row_of<DT>(a.k, b, t0, gr), a.k.rs, rows, a.key, tid);
+            k.template load<EVEN>(row_of<DT>(a.k, b, t0, gr), a.k.rs, rows, a.key, tid);
             k.store(tk, tid);
             finite_k = k.finite();
         }
@@ -1139,12 +1163,12 @@ __global__ void __launch_bounds__(WG, NP == 128 ? 1 : 2) k_attn_bwd(const Args a
                     for (int r = 0; r < 4; ++r) all_dk[n][r] = TURNS ? all_dk[n][r] + dk[n][r] : dk[n][r];
                 if (me < rows) {
                     auto* out = row_of<DT>(a.dv, b, t0 + me, h) + tile * PV;
-                    if ((a.wide & W_DV) && vcols == PV) {
+                    if (vcols == PV) {
 #pragma unroll
-                        for (int p = 0; p < S::TP; ++p) write4<DT>(out, 16 * p + row4, PV, true, dv[p]);
+                        for (int p = 0; p < S::TP; ++p) write4<DT>(out, 16 * p + row4, PV, dv[p]);
                     } else {
 #pragma unroll
-                        for (int p = 0; p < S::TP; ++p) write4<DT>(out, 16 * p + row4, here(vcols), false, dv[p]);
+                        for (int p = 0; p < S::TP; ++p) write4<DT>(out, 16 * p + row4, here(vcols), dv[p]);
                     }
                 }
             }
@@ -1177,8 +1201,8 @@ __global__ void __launch_bounds__(WG, NP == 128 ? 1 : 2) k_attn_bwd(const Args a
     }
     const int me = 16 * first_own + (threadIdx.x & 15), row4 = 4 * ((threadIdx.x & 63) >> 4);
     if (me < all_rows) {
-        write_key<DT>(a.part_q == nullptr ? nullptr : part_row(a.part_q, me), row_of<DT>(a.dq, b, t0 + me, gr), a.key, a.wide & W_DQ, row4, all_dq);
-        write_key<DT>(a.part_k == nullptr ? nullptr : part_row(a.part_k, me), row_of<DT>(a.dk, b, t0 + me, gr), a.key, a.wide & W_DK, row4, all_dk);
+        write_key<DT>(a.part_q == nullptr ? nullptr : part_row(a.part_q, me), row_of<DT>(a.dq, b, t0 + me, gr), a.key, row4, all_dq);
+        write_key<DT>(a.part_k == nullptr ? nullptr : part_row(a.part_k, me), row_of<DT>(a.dk, b, t0 + me, gr), a.key, row4, all_dk);
     }
 }
 
@@ -1208,12 +1232,12 @@ __global__ void __launch_bounds__(WG) k_attn_sum_tiles(const float* part, float*
 }
 
 // ---- one position -------------------------------------------------------------------------------------
-// A workgroup per head of a sequence: a thread has VEC values of every ROWS-th row of the state, read and written once; the rows'
+// A workgroup per head of a sequence: a thread has four values of every ROWS-th row of the state, read and written once; the rows'
 // products with q are summed over the wavefront's lanes, then through LDS.  Bound by memory: 1000 x 16 heads of 64 x 64 take 83 us
-// (6.4 TB/s) with accesses of 16 bytes, 121 with those of 4.
-template <int DT, int VEC>
+// (6.4 TB/s) with accesses of 16 bytes, 121 with those of 4.  EVEN: values are a multiple of four (63 of them take 9% longer than 64).
+template <int DT, bool EVEN>
 __global__ void __launch_bounds__(WG) k_attn_step(const Args a) {
-    constexpr int LANES = 64 / VEC, ROWS = WG / LANES, AT_ONCE = 4;  // lanes of a row of PV values, rows at a time
+    constexpr int VEC = 4, LANES = 64 / VEC, ROWS = WG / LANES, AT_ONCE = 4;  // lanes of a row of PV values, rows at a time
     __shared__ float part[WAVES][PV];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int col = threadIdx.x % LANES * VEC, row = threadIdx.x / LANES;
@@ -1226,11 +1250,12 @@ __global__ void __launch_bounds__(WG) k_attn_step(const Args a) {
         const float f = hw_exp(static_cast<const float*>(a.g.p)[b * a.g.bs + h * a.g.hs]);
         for (int p0 = 0; p0 < a.value; p0 += PV) {
             const int p = p0 + col;
-            const bool in = p < a.value;
+            const int have = a.value - p;  // values from p on
+            const bool whole = EVEN ? have > 0 : have >= VEC;
             float* st = a.state_out + bh * a.key * a.value + p;
             float vv[VEC], y[VEC];
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) vv[e] = in ? Elem<DT>::ld(v[p + e]) : 0.0f, y[e] = 0.0f;
+            for (int e = 0; e < VEC; ++e) vv[e] = (EVEN ? whole : e < have) ? Elem<DT>::ld(v[p + e]) : 0.0f, y[e] = 0.0f;
             for (int n0 = row; n0 < a.key; n0 += ROWS * AT_ONCE) {
                 float s[AT_ONCE][VEC], kn[AT_ONCE], qn[AT_ONCE];
 #pragma unroll
@@ -1238,18 +1263,29 @@ __global__ void __launch_bounds__(WG) k_attn_step(const Args a) {
                     const int n = min(n0 + i * ROWS, a.key - 1);
                     kn[i] = Elem<DT>::ld(k[n]);
                     qn[i] = Elem<DT>::ld(q[n]);
-                    if (in) ld_vec<DT_F32, VEC>(st + (int64_t)n * a.value, s[i]);
+                    if (whole) {
+                        Raw<DT_F32, VEC>::unpack(*reinterpret_cast<const AnyAt*>(st + (int64_t)n * a.value), s[i]);
+                    } else if (!EVEN) {
+#pragma unroll
+                        for (int e = 0; e < VEC; ++e) s[i][e] = e < have ? st[(int64_t)n * a.value + e] : 0.0f;
+                    }
                 }
 #pragma unroll
                 for (int i = 0; i < AT_ONCE; ++i) {
                     const int n = n0 + i * ROWS;
-                    if (n >= a.key || !in) continue;
+                    if (n >= a.key || (EVEN && !whole)) continue;
 #pragma unroll
                     for (int e = 0; e < VEC; ++e) {
                         s[i][e] = __builtin_fmaf(f, s[i][e], kn[i] * vv[e]);
                         y[e] = __builtin_fmaf(qn[i], s[i][e], y[e]);
                     }
-                    st_vec<DT_F32, VEC>(st + (int64_t)n * a.value, s[i]);
+                    if (EVEN || whole) {
+                        *reinterpret_cast<AnyAt*>(st + (int64_t)n * a.value) = Raw<DT_F32, VEC>::pack(s[i]);
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < VEC - 1; ++e)
+                            if (e < have) st[(int64_t)n * a.value + e] = s[i][e];
+                    }
                 }
             }
 #pragma unroll
@@ -1270,12 +1306,6 @@ __global__ void __launch_bounds__(WG) k_attn_step(const Args a) {
 
 // ---- host ---------------------------------------------------------------------------------------------
 Heads heads_of(const boa_heads& x) { return {x.p, x.batch_stride, x.row_stride, x.head_stride}; }
-
-bool wide_rows(int dtype, const boa_heads& x, int cols) {
-    const int64_t es = dtype == DT_F32 ? 4 : 2;
-    return ((uintptr_t)x.p | (uintptr_t)(x.batch_stride * es) | (uintptr_t)(x.row_stride * es) | (uintptr_t)(x.head_stride * es) |
-            (uintptr_t)(cols * es)) % 16 == 0;
-}
 
 // The split: pieces of whole chunks, as many as give the wanted workgroups, two for each CU.  Forward of 4 x 4097 x 16 heads in
 // bfloat16 with 256, 512, 768 and 1024 wanted: 92, 61, 73 and 67 us; of 2 x 16384 x 8 in float32: 153, 125, 165 and 126.  Backward
@@ -1360,14 +1390,6 @@ Args args_of(const boa_attention& s, const Plan& p) {
     a.lens = s.lens, a.state_in = s.state_in, a.state_out = s.state_out;
     a.batch = s.batch, a.length = s.length, a.chunks = p.chunks;
     a.heads = s.heads, a.share = s.heads / s.groups, a.key = s.key, a.value = s.value, a.tiles = p.tiles, a.scale = s.scale;
-    const struct {
-        uint32_t bit;
-        const boa_heads& x;
-        int cols;
-    } all[] = {{W_Q, s.q, s.key}, {W_K, s.k, s.key}, {W_V, s.v, s.value}, {W_DY, s.dy, s.value}, {W_Y, s.y, s.value}, {W_DQ, s.dq, s.key},
-               {W_DK, s.dk, s.key}, {W_DV, s.dv, s.value}};
-    for (const auto& t : all)
-        if (wide_rows(s.dtype, t.x, t.cols)) a.wide |= t.bit;
     return a;
 }
 
@@ -1378,17 +1400,20 @@ int allow_lds(K* kernel, int bytes) {
     return BOA_OK;
 }
 
-// Calls f with the padded key and whether all inputs are aligned as constants.
+// Whether no access of 16 bytes passes a row's end.  Kernels that know it need no shifts, and fewer registers.
+bool even(const boa_attention& s) { return (s.key | s.value) % (s.dtype == BOA_DT_F32 ? 4 : 8) == 0; }
+
+// Calls f with the padded key and `even` as constants.
 template <class F>
-int with_key(int np, bool wide, F f) {
-    const auto with = [&](auto n) { return wide ? f(n, std::true_type()) : f(n, std::false_type()); };
+int with_key(int np, bool even, F f) {
+    const auto with = [&](auto n) { return even ? f(n, std::true_type()) : f(n, std::false_type()); };
     return np == 64 ? with(std::integral_constant<int, 64>()) : with(std::integral_constant<int, 128>());
 }
 
 // What the pieces leave, and backward what every chunk's end is reached with.
-template <int DT, int NP, bool BACK, bool WIDE>
+template <int DT, int NP, bool BACK, bool EVEN>
 int launch_states(const Args& a, const Plan& p, hipStream_t s) {
-    hipLaunchKernelGGL((k_attn_states<DT, NP, BACK, WIDE>), dim3((uint32_t)(p.bh * p.tiles * p.pieces)), dim3(WG), 0, s, a);
+    hipLaunchKernelGGL((k_attn_states<DT, NP, BACK, EVEN>), dim3((uint32_t)(p.bh * p.tiles * p.pieces)), dim3(WG), 0, s, a);
     BOA_HIP_TRY(hipGetLastError());
     if (p.pieces > 1) {
         hipLaunchKernelGGL((k_attn_join<NP, BACK>), dim3((uint32_t)(p.bh * p.tiles * (State<NP>::SIZE / (WG * 4)))), dim3(WG), 0, s, a);
@@ -1425,13 +1450,13 @@ extern "C" int boa_linear_attention_fwd(const boa_attention* s, void* d_work, in
     a.marks = s->marks;
     hipStream_t st = (hipStream_t)stream;
     return with_dtype(s->dtype, [&](auto dt) {
-        return with_key(p.np, (a.wide & W_FWD) == W_FWD, [&](auto np, auto wide) {
-            constexpr bool WIDE = decltype(wide)::value;
+        return with_key(p.np, even(*s), [&](auto np, auto even) {
+            constexpr bool EVEN = decltype(even)::value;
             constexpr int DT = decltype(dt)::value, NP = decltype(np)::value, LDS = FwdLds<DT, NP>::BYTES;
             if (p.pieces > 1)
-                if (const int no = launch_states<DT, NP, false, WIDE>(a, p, st)) return no;
-            if (const int no = allow_lds(k_attn_fwd<DT, NP, WIDE>, LDS)) return no;
-            hipLaunchKernelGGL((k_attn_fwd<DT, NP, WIDE>), dim3((uint32_t)(p.bh * p.tiles * p.pieces)), dim3(WG), LDS, st, a);
+                if (const int no = launch_states<DT, NP, false, EVEN>(a, p, st)) return no;
+            if (const int no = allow_lds(k_attn_fwd<DT, NP, EVEN>, LDS)) return no;
+            hipLaunchKernelGGL((k_attn_fwd<DT, NP, EVEN>), dim3((uint32_t)(p.bh * p.tiles * p.pieces)), dim3(WG), LDS, st, a);
             BOA_HIP_TRY(hipGetLastError());
             return (int)BOA_OK;
         });
@@ -1468,17 +1493,17 @@ extern "C" int boa_linear_attention_bwd(const boa_attention* s, void* d_work, in
     if (s->decay_per_head) a.dg_sum = rest;
     else a.dg = p.tiles > 1 ? rest : s->ddecay;
     return with_dtype(s->dtype, [&](auto dt) {
-        return with_key(p.np, (a.wide & W_BACK) == W_BACK, [&](auto np, auto wide) {
-            constexpr bool WIDE = decltype(wide)::value;
+        return with_key(p.np, even(*s), [&](auto np, auto even) {
+            constexpr bool EVEN = decltype(even)::value;
             constexpr int DT = decltype(dt)::value, NP = decltype(np)::value, LDS = BwdLds<DT, NP>::BYTES;
-            if (const int no = launch_states<DT, NP, true, WIDE>(a, p, st)) return no;
+            if (const int no = launch_states<DT, NP, true, EVEN>(a, p, st)) return no;
             const dim3 grid((uint32_t)(p.bh / a.in_turn * p.tiles * p.chunks));
             if (a.in_turn > 1) {
-                if (const int no = allow_lds(k_attn_bwd<DT, NP, true, WIDE>, LDS)) return no;
-                hipLaunchKernelGGL((k_attn_bwd<DT, NP, true, WIDE>), grid, dim3(WG), LDS, st, a);
+                if (const int no = allow_lds(k_attn_bwd<DT, NP, true, EVEN>, LDS)) return no;
+                hipLaunchKernelGGL((k_attn_bwd<DT, NP, true, EVEN>), grid, dim3(WG), LDS, st, a);
             } else {
-                if (const int no = allow_lds(k_attn_bwd<DT, NP, false, WIDE>, LDS)) return no;
-                hipLaunchKernelGGL((k_attn_bwd<DT, NP, false, WIDE>), grid, dim3(WG), LDS, st, a);
+                if (const int no = allow_lds(k_attn_bwd<DT, NP, false, EVEN>, LDS)) return no;
+                hipLaunchKernelGGL((k_attn_bwd<DT, NP, false, EVEN>), grid, dim3(WG), LDS, st, a);
             }
             BOA_HIP_TRY(hipGetLastError());
             if (a.part_q != nullptr) {
@@ -1508,12 +1533,11 @@ extern "C" int boa_linear_attention_step(const boa_attention* s, void* stream) {
         return boa_fail(BOA_ERR_ARG, "boa_linear_attention_step: null pointer");
     const Plan p(*s, false);
     const Args a = args_of(*s, p);
-    const bool vec = s->value % 4 == 0 && (uintptr_t)s->state_out % 16 == 0;
     const dim3 grid((uint32_t)(p.bh < MAX_BLOCKS ? p.bh : MAX_BLOCKS));
     return with_dtype(s->dtype, [&](auto dt) {
         constexpr int DT = decltype(dt)::value;
-        if (vec) hipLaunchKernelGGL((k_attn_step<DT, 4>), grid, dim3(WG), 0, (hipStream_t)stream, a);
-        else hipLaunchKernelGGL((k_attn_step<DT, 1>), grid, dim3(WG), 0, (hipStream_t)stream, a);
+        if (s->value % 4 == 0) hipLaunchKernelGGL((k_attn_step<DT, true>), grid, dim3(WG), 0, (hipStream_t)stream, a);
+        else hipLaunchKernelGGL((k_attn_step<DT, false>), grid, dim3(WG), 0, (hipStream_t)stream, a);
         BOA_HIP_TRY(hipGetLastError());
         return (int)BOA_OK;
     });
