@@ -26,7 +26,7 @@
 //
 // Measured with 64 keys and 64 values a head (copies of the sizes moved here reach 5 to 6 TB/s, float32 products of libraries 150
 // TFLOP/s), kernels in us; 4 x 4097 positions x 16 heads of 4 groups in bfloat16: states 21, joined 6, forward 50 (136 MB and as
-// much of k and v again); 2 x 16384 x 8 heads in float32: forward 38 + 7 + 110, backward 44 + 7 + 254 (539 MB, and 27 GFLOP of
+// much of k and v again); 2 x 16384 x 8 heads in float32: forward 38 + 7 + 110, backward 44 + 7 + 224 (539 MB, and 27 GFLOP of
 // products, 183 us at the libraries' rate); 32 x 500 x 16 heads of 4 groups in bfloat16: forward 44, backward 21 + 109; one position
 // of 1000 x 16 heads: 83 (532 MB, 6.4 TB/s).  What bounds each stands at its kernel.
 #include "ops_common.h"
@@ -78,7 +78,7 @@ template <int DT> struct Mat {
     using E = float;
     using Frag = f32x4;
     static constexpr int STEP = 16, VEC = 4, TWO = 1, THREE = 1, PAD = 4;
-    static constexpr bool SKIP = true;  // all-zero tiles are left out: 2 x 16384 x 8 backward 293 -> 254 us
+    static constexpr bool SKIP = true;  // all-zero tiles are left out (2 x 16384 x 8 backward 293 -> 254 us)
     static __device__ __forceinline__ floatx4 mma(const Frag& a, const Frag& b, floatx4 c) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[i], b[i], c, 0, 0, 0);
@@ -897,30 +897,33 @@ __device__ __forceinline__ float from_here(float v) {
     return v + dpp<DPP_SHL8>(v);
 }
 
-// In LDS: k, v and dy, and in one place after another dS and S, each [NP][PV] in three parts, and q.
-template <int DT, int NP>
+// In LDS: k, v and dy, and in one place after another dS and S, each [NP][PV] in three parts, and q.  SHARED: v's place becomes k's.
+template <int DT, int NP, bool SHARED>
 struct BwdLds {
     using M = Mat<DT>;
     static constexpr int LDS_STATE = PV + M::PAD, PART = NP * LDS_STATE;
     static constexpr int ONE = M::THREE * PART > Tile<DT, NP>::SIZE ? M::THREE * PART : Tile<DT, NP>::SIZE;
-    static constexpr int Q = 0, K = ONE, V = K + Tile<DT, NP>::SIZE, D = V + Tile<DT, PV>::SIZE;
+    static constexpr int Q = 0, K = ONE, V = SHARED ? K : K + Tile<DT, NP>::SIZE, D = V + Tile<DT, PV>::SIZE;
     static constexpr int BYTES = (int)sizeof(typename M::E) * (D + Tile<DT, PV>::SIZE);
 };
 // The products of one chunk take no turn behind another's, so there is a workgroup for each and nothing is carried: 4096 of them at
-// 2 x 16384 x 8 in float32, 254 us of which the matrix cores are busy for 100; loads at a chunk's start take a quarter, and two
-// workgroups on a CU (LDS allows no third) hide half of each other's.  Walking chunks with the next one's tiles loaded ahead needs
-// more registers than there are.
+// 2 x 16384 x 8 in float32, 224 us of which the matrix cores are busy for 120.  Loads at a chunk's start take a quarter of its time,
+// which other workgroups on the CU hide: with up to 64 keys three of them, if what is made of v comes before anything of k, so
+// that one place in LDS does for both (four places and two workgroups: 255 us; 2 x 8192 x 16 in bfloat16 113 and 144).  Not in
+// turns, which keep k and need more registers, nor in bfloat16 of odd widths.  Walking chunks with the next one's tiles loaded
+// ahead needs more registers than there are.
 // A workgroup has one chunk, and of a group `in_turn` heads one after another: their queries and keys are read once, and what the
 // heads give to dq and dk is summed in registers.
 template <int DT, int NP, bool TURNS, bool EVEN>
-__global__ void __launch_bounds__(WG, NP == 128 ? 1 : 2) k_attn_bwd(const Args a) {
+__global__ void __launch_bounds__(WG, NP == 128 ? 1 : TURNS || (DT == DT_BF16 && !EVEN) ? 2 : 3) k_attn_bwd(const Args a) {
     using M = Mat<DT>;
     using E = typename M::E;
     using Frag = typename M::Frag;
     using TN = Tile<DT, NP>;
     using TV = Tile<DT, PV>;
     using S = State<NP>;
-    using L = BwdLds<DT, NP>;
+    constexpr bool SHARED = !TURNS && NP == PV;
+    using L = BwdLds<DT, NP, SHARED>;
     constexpr int NT = NP / 16, LS = L::LDS_STATE;
     extern __shared__ __attribute__((aligned(16))) char lds[];
     E* tq = reinterpret_cast<E*>(lds) + L::Q;
@@ -930,7 +933,11 @@ __global__ void __launch_bounds__(WG, NP == 128 ? 1 : 2) k_attn_bwd(const Args a
     __shared__ __attribute__((aligned(16))) Falls G;
     __shared__ int said[WAVES];
     __shared__ __attribute__((aligned(16))) float middle[WAVES - 1][CHUNK];
-    __shared__ float pairs[CHUNK], from_state[CHUNK], to_behind[CHUNK], through[2][WAVES];
+    __shared__ float through[2][WAVES];
+    // a position's parts of dg, behind its row of dy
+    const auto part_of = [&](int which, int i) -> float& { return reinterpret_cast<float*>(td + i * TV::LD + PV)[which]; };
+    enum { PAIRS, FROM_STATE, TO_BEHIND };
+    static_assert(M::PAD * sizeof(E) >= 3 * sizeof(float), "");
     const int first_own = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t chunks = (uint32_t)a.chunks, rest = blockIdx.x / chunks, turns = (uint32_t)(a.share / a.in_turn);
     const int64_t c = blockIdx.x - rest * chunks, t0 = c * CHUNK;
@@ -981,11 +988,12 @@ __global__ void __launch_bounds__(WG, NP == 128 ? 1 : 2) k_attn_bwd(const Args a
         d.template load<EVEN>(row_of<DT>(a.dy, b, t0, h) + tile * PV, a.dy.rs, rows, vcols, tid);
         s.load(a.fmarks + mark, lane, own);
         const float g_own = decay_at(decays_of(a, b, h) + t0 * a.g.rs, a.g.rs, rows, lane);
-        q.template load<EVEN>(row_of<DT>(a.q, b, t0, gr), a.q.rs, rows, a.key, tid);
-        if (turn == 0) {
-            TN k;
+        const auto load_q = [&] { q.template load<EVEN>(row_of<DT>(a.q, b, t0, gr), a.q.rs, rows, a.key, tid); };
+        if (!SHARED) load_q();
+        TN k;
+        if (!TURNS || turn == 0) {
             k.template load<EVEN>(row_of<DT>(a.k, b, t0, gr), a.k.rs, rows, a.key, tid);
-            k.store(tk, tid);
+            if (!SHARED) k.store(tk, tid);
             finite_k = k.finite();
         }
         {
@@ -1015,12 +1023,11 @@ __global__ void __launch_bounds__(WG, NP == 128 ? 1 : 2) k_attn_bwd(const Args a
             v.store(tv, tid);
             d.store(td, tid);
             ds.template put<M, M::THREE>(tq, a.key, vcols, lane, own);
-            say_finite(said, finite_k && q.finite() && d.finite(), lane, own);
+            const bool finite_kd = finite_k && d.finite();
             __syncthreads();
-            const bool finite = heard_finite(said);
             const float2 mine = G.at(me), g_end = G.at(CHUNK - 1);
             const float to_end = fall_between(g_end, mine), from_start = a.scale * __builtin_amdgcn_exp2f(mine.x + mine.y);
-            floatx4 dq[NT], dk[NT], dv[S::TP];
+            floatx4 dq[NT], dk[NT], dv[S::TP], dA_i[4], dA_j[4];  // dy . v with the own positions as i, as j
             // what the positions behind the chunk give to dk and dv, by way of dS
 #pragma unroll
             for (int n = 0; n < NT; ++n) dk[n] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
@@ -1034,6 +1041,15 @@ __global__ void __launch_bounds__(WG, NP == 128 ? 1 : 2) k_attn_bwd(const Args a
 #pragma unroll
                     for (int x = 0; x < M::THREE; ++x) dk[n] = M::mma(M::row(tq + x * L::PART, LS, 16 * n, p, lane), f, dk[n]);
                 __builtin_amdgcn_sched_barrier(0);
+            }
+            if constexpr (SHARED) {
+                scores<M, PV>(dA_i, tv, td, TV::LD, 16 * own, 0, own, lane);
+                __builtin_amdgcn_sched_barrier(0);
+                scores<M, PV>(dA_j, td, tv, TV::LD, 16 * own, own, 3, lane);
+                __syncthreads();
+                k.store(tk, tid);
+                load_q();
+                __syncthreads();
             }
 #pragma unroll
             for (int n = 0; n < NP; n += M::STEP) {
@@ -1056,7 +1072,7 @@ __global__ void __launch_bounds__(WG, NP == 128 ? 1 : 2) k_attn_bwd(const Args a
                     }
                 }
                 x = over_rows(x);
-                if (lane < 16) to_behind[me] = x;
+                if (lane < 16) part_of(TO_BEHIND, me) = x;
 #pragma unroll
                 for (int p = 0; p < S::TP; ++p)
 #pragma unroll
@@ -1079,7 +1095,9 @@ __global__ void __launch_bounds__(WG, NP == 128 ? 1 : 2) k_attn_bwd(const Args a
             }
             __syncthreads();
             q.store(tq, tid);
+            say_finite(said, finite_kd && q.finite(), lane, own);
             __syncthreads();
+            const bool finite = heard_finite(said);
             {
                 float x = 0.0f;
 #pragma unroll
@@ -1092,15 +1110,15 @@ __global__ void __launch_bounds__(WG, NP == 128 ? 1 : 2) k_attn_bwd(const Args a
                     }
                 }
                 x = over_rows(x);
-                if (lane < 16) from_state[me] = x;
+                if (lane < 16) part_of(FROM_STATE, me) = x;
             }
             // the own positions as i: rows are positions j before them
             __builtin_amdgcn_sched_barrier(0);
             {
-                floatx4 A[4], dA[4];
+                floatx4 A[4], (&dA)[4] = dA_i;
                 scores<M, NP>(A, tk, tq, TN::LD, 16 * own, 0, own, lane);
                 __builtin_amdgcn_sched_barrier(0);
-                scores<M, PV>(dA, tv, td, TV::LD, 16 * own, 0, own, lane);
+                if (!SHARED) scores<M, PV>(dA, tv, td, TV::LD, 16 * own, 0, own, lane);
                 __builtin_amdgcn_sched_barrier(0);
                 // the pairs that a position t of the own ones lies between: of M_ij the sum over the own i >= t, then over j < t; and all
                 // own i for the positions of the tiles before
@@ -1125,7 +1143,7 @@ __global__ void __launch_bounds__(WG, NP == 128 ? 1 : 2) k_attn_bwd(const Args a
                 for (int t = 1; t < 4; ++t)
                     if (t > own) dA[t] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
                 at = over_rows(at);
-                if (lane < 16) pairs[me] = at;
+                if (lane < 16) part_of(PAIRS, me) = at;
                 product_within<M, M::TWO>(dq, finite, tk, TN::LD, dA, 0, own, lane, [&](int j) { return j <= me && me < rows; });
 #pragma unroll
                 for (int n = 0; n < NT; ++n)
@@ -1135,10 +1153,10 @@ __global__ void __launch_bounds__(WG, NP == 128 ? 1 : 2) k_attn_bwd(const Args a
             // the own positions as j: rows are positions i behind them
             __builtin_amdgcn_sched_barrier(0);
             {
-                floatx4 A[4], dA[4];
+                floatx4 A[4], (&dA)[4] = dA_j;
                 scores<M, NP>(A, tq, tk, TN::LD, 16 * own, own, 3, lane);
                 __builtin_amdgcn_sched_barrier(0);
-                scores<M, PV>(dA, td, tv, TV::LD, 16 * own, own, 3, lane);
+                if (!SHARED) scores<M, PV>(dA, td, tv, TV::LD, 16 * own, own, 3, lane);
                 __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
                 for (int t = 0; t < 4; ++t) {
@@ -1180,9 +1198,9 @@ __global__ void __launch_bounds__(WG, NP == 128 ? 1 : 2) k_attn_bwd(const Args a
                 const bool in = lane < rows;
                 // from the states before: positions i from t on (summed from the last one); to the positions behind the chunk: j before t
                 const int last = CHUNK - 1 - lane;
-                const double later = __shfl(scan(last < rows ? (double)from_state[last] : 0.0), CHUNK - 1 - lane, 64);
-                double x = (double)pairs[lane] + later + over;
-                const double behind = __shfl_up(scan(in ? (double)to_behind[lane] : 0.0), 1, 64);
+                const double later = __shfl(scan(last < rows ? (double)part_of(FROM_STATE, last) : 0.0), CHUNK - 1 - lane, 64);
+                double x = (double)part_of(PAIRS, lane) + later + over;
+                const double behind = __shfl_up(scan(in ? (double)part_of(TO_BEHIND, lane) : 0.0), 1, 64);
                 if (lane > 0) x += behind;
                 // and of the chunk's own pairs those with an i of a later tile than t's
 #pragma unroll
@@ -1495,13 +1513,15 @@ extern "C" int boa_linear_attention_bwd(const boa_attention* s, void* d_work, in
     return with_dtype(s->dtype, [&](auto dt) {
         return with_key(p.np, even(*s), [&](auto np, auto even) {
             constexpr bool EVEN = decltype(even)::value;
-            constexpr int DT = decltype(dt)::value, NP = decltype(np)::value, LDS = BwdLds<DT, NP>::BYTES;
+            constexpr int DT = decltype(dt)::value, NP = decltype(np)::value;
             if (const int no = launch_states<DT, NP, true, EVEN>(a, p, st)) return no;
             const dim3 grid((uint32_t)(p.bh / a.in_turn * p.tiles * p.chunks));
             if (a.in_turn > 1) {
+                constexpr int LDS = BwdLds<DT, NP, false>::BYTES;
                 if (const int no = allow_lds(k_attn_bwd<DT, NP, true, EVEN>, LDS)) return no;
                 hipLaunchKernelGGL((k_attn_bwd<DT, NP, true, EVEN>), grid, dim3(WG), LDS, st, a);
             } else {
+                constexpr int LDS = BwdLds<DT, NP, NP == PV>::BYTES;
                 if (const int no = allow_lds(k_attn_bwd<DT, NP, false, EVEN>, LDS)) return no;
                 hipLaunchKernelGGL((k_attn_bwd<DT, NP, false, EVEN>), grid, dim3(WG), LDS, st, a);
             }
