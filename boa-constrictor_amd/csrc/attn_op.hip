@@ -701,7 +701,7 @@ __device__ __forceinline__ void zero_rows(const Heads& x, int64_t b, int h, int 
 // ---- forward ------------------------------------------------------------------------------------------
 // A workgroup walks a piece with the state in registers, and lays it into LDS (split in two parts for bfloat16) for the product
 // with q; the next chunk's q, k and v are loaded into registers while this one's products run.  Bound in bfloat16 by vector work
-// (56% of the SIMDs' time: decays, splits, masks) and LDS, at 2.7 TB/s of inputs and results; in float32 by the matrix cores' rate
+// (55% of the SIMDs' time: decays, splits, masks) and LDS, at 2.7 TB/s of inputs and results; in float32 by the matrix cores' rate
 // for it and LDS together, 110 us for 16 GFLOP.
 template <int DT, int NP>
 struct FwdLds {
@@ -907,7 +907,7 @@ struct BwdLds {
     static constexpr int BYTES = (int)sizeof(typename M::E) * (D + Tile<DT, PV>::SIZE);
 };
 // The products of one chunk take no turn behind another's, so there is a workgroup for each and nothing is carried: 4096 of them at
-// 2 x 16384 x 8 in float32, 224 us of which the matrix cores are busy for 120.  Loads at a chunk's start take a quarter of its time,
+// 2 x 16384 x 8 in float32, 224 us of which the matrix cores are busy for 59%.  Loads at a chunk's start take a quarter of its time,
 // which other workgroups on the CU hide: with up to 64 keys three of them, if what is made of v comes before anything of k, so
 // that one place in LDS does for both (four places and two workgroups: 255 us; 2 x 8192 x 16 in bfloat16 113 and 144).  Not in
 // turns, which keep k and need more registers, nor in bfloat16 of odd widths.  Walking chunks with the next one's tiles loaded
@@ -1365,7 +1365,9 @@ struct Plan {
 };
 
 // Heads of a group that a workgroup of the backward pass takes in turn: as many as leave two for each CU twice over.
-// 32 x 500 x 16 heads of 4 groups: 109 us so, 135 + 45 for the sums over heads with each head by itself, 121 + 36 with two in turn.
+// 32 x 500 x 16 heads of 4 groups in bfloat16: 109 us so, 135 + 45 for the sums over heads with each head by itself, 121 + 36 with
+// two in turn.  Forward and backward of 2 x 8192 x 16 heads of 8 groups, whole groups in turn: 404 us in float32 and 248 in bfloat16,
+// each head by itself 451 and 298; where only a part of a group can be (2 to 4 of 4 to 16 heads) it is 10% less to 11% more.
 int in_turn(const boa_attention& s, const Plan& p) {
     const int share = s.heads / s.groups;
     for (int n = share; n > 1; --n)
@@ -1411,7 +1413,7 @@ Args args_of(const boa_attention& s, const Plan& p) {
     return a;
 }
 
-// Kernels whose LDS passes 64 KB are told so, once per kernel and device (the call is of no stream and may run under capture).
+// Kernels whose LDS passes 64 KB are told so before each launch: it is of the current device, of no stream, and may run under capture.
 template <class K>
 int allow_lds(K* kernel, int bytes) {
     BOA_HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes));

@@ -7,6 +7,10 @@
 // Sums and the factor are in 64 bits: squares of large float32 values (and of scaled float16 gradients) stay in range, a norm that
 // float32 cannot hold still scales, and it costs nothing beside the memory that bounds both.  Where the factor is 1 nothing is
 // written.
+//
+// Measured: 141 gradients of 32 MB in float32 7 us for the sums (4.4 TB/s) and 12 for the scaling (5.4, from the last-level cache in
+// part); 277 of 122 MB in bfloat16, two launches of each, 25 and 51 (4.9 and 4.8 TB/s).  Bound by memory, and below some 100 MB by
+// the host, which looks at each gradient: 58 and 111 us.
 #include <algorithm>
 #include <vector>
 
