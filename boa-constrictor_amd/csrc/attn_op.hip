@@ -67,9 +67,8 @@ struct Args {
 };
 
 // How products of a type run: elements in LDS, K of a step, parts that a float32 value is split into.
-//   bfloat16: inputs as they are.  What is computed on the way (A, dA, states, decayed keys) is split into parts of 8 bits each:
-//   two for what ends in a result of 16 bits, three (24 bits) for the states and whatever goes into dg, which are float32.  One
-//   rounding to 8 bits instead would be as large as the result's own rounding.
+//   bfloat16: inputs as they are.  What is computed on the way (A, dA, states, decayed keys) is split into three parts of 8 bits
+//   each, float32's 24: with two, terms that cancel would leave an error beyond the result's own rounding.
 //   float32, and float16, whose range the parts of a float32 value do not fit: float32 products (v_mfma_f32_16x16x4_f32).
 // A fragment holds VEC elements along K per lane: `row` of a tile with K along memory, `col` of one with K across; element e of lane
 // group g is k = VEC g + e.  `mixed` is `col` in the order of register tiles, k = 16 (e / 4) + 4 g + e % 4: element e of
@@ -77,7 +76,7 @@ struct Args {
 template <int DT> struct Mat {
     using E = float;
     using Frag = f32x4;
-    static constexpr int STEP = 16, VEC = 4, TWO = 1, THREE = 1, PAD = 4;
+    static constexpr int STEP = 16, VEC = 4, PARTS = 1, PAD = 4;
     static constexpr bool SKIP = true;  // all-zero tiles are left out (2 x 16384 x 8 backward 293 -> 254 us)
     static __device__ __forceinline__ floatx4 mma(const Frag& a, const Frag& b, floatx4 c) {
 #pragma unroll
@@ -96,7 +95,6 @@ template <int DT> struct Mat {
 #pragma unroll
         for (int i = 0; i < VEC; ++i) x[i] = f[i];
     }
-    template <int PARTS>
     static __device__ __forceinline__ void split(const float (&x)[VEC], Frag (&f)[PARTS]) {
         f[0] = Frag{x[0], x[1], x[2], x[3]};
     }
@@ -118,7 +116,7 @@ __device__ __forceinline__ float rest(float f, float hi) {
 template <> struct Mat<DT_BF16> {
     using E = uint16_t;
     using Frag = bf16x8;
-    static constexpr int STEP = 32, VEC = 8, TWO = 2, THREE = 3, PAD = 8;
+    static constexpr int STEP = 32, VEC = 8, PARTS = 3, PAD = 8;
     static constexpr bool SKIP = false;  // a step is two tiles, and takes an eighth of float32's time a tile
     static __device__ __forceinline__ floatx4 mma(const Frag& a, const Frag& b, floatx4 c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
@@ -144,7 +142,6 @@ template <> struct Mat<DT_BF16> {
         return across(t, ld, row0, k0 + (lane >> 4) * 4, 16, lane);
     }
     static __device__ __forceinline__ void widen(const Frag& f, float (&x)[VEC]) { Raw<DT_BF16, VEC>::unpack(__builtin_bit_cast(u32x4, f), x); }
-    template <int PARTS>
     static __device__ __forceinline__ void split(const float (&x)[VEC], Frag (&f)[PARTS]) {
         float v[VEC];
 #pragma unroll
@@ -175,12 +172,12 @@ template <> struct Mat<DT_BF16> {
     }
 };
 // Step s of a product over 64 positions whose second operand is in registers, four tiles of 16 rows.
-template <class M, int PARTS>
-__device__ __forceinline__ void registers(const floatx4 (&t)[4], int s, typename M::Frag (&f)[PARTS]) {
+template <class M>
+__device__ __forceinline__ void registers(const floatx4 (&t)[4], int s, typename M::Frag (&f)[M::PARTS]) {
     float x[M::VEC];
 #pragma unroll
     for (int e = 0; e < M::VEC; ++e) x[e] = t[s * (M::VEC / 4) + e / 4][e % 4];
-    M::template split<PARTS>(x, f);
+    M::split(x, f);
 }
 // Row k (the same for all lanes) of the lane's column of a register operand of four tiles.
 __device__ __forceinline__ float row_of_tiles(const floatx4 (&t)[4], int k, int lane) {
@@ -195,20 +192,20 @@ __device__ __forceinline__ float row_of_tiles(const floatx4 (&t)[4], int k, int 
 // those from `first` to `last` are not all zero.  inside(k) says whether B's k of this lane's column counts; B is zero where it
 // does not.  If A has infinities or NaN (it is not `finite`), those times such zeros would be NaN, and a position would reach others
 // that it comes behind: they are left out of the product and added one by one, so that whatever they do not reach keeps its bits.
-template <class M, int PARTS, int TA, class F>
+template <class M, int TA, class F>
 __device__ __forceinline__ void product_within(floatx4 (&acc)[TA], bool finite, const typename M::E* a, int lda, const floatx4 (&b)[4],
                                                int first, int last, int lane, F inside) {
     const auto all = [&](auto clean) {
 #pragma unroll
         for (int s = 0; s < CHUNK / M::STEP; ++s) {
             if (M::SKIP && (s < first || s > last)) continue;  // a step is a tile there
-            typename M::Frag fb[PARTS];
-            registers<M, PARTS>(b, s, fb);
+            typename M::Frag fb[M::PARTS];
+            registers<M>(b, s, fb);
 #pragma unroll
             for (int i = 0; i < TA; ++i) {
                 const typename M::Frag fa = clean(M::mixed(a, lda, 16 * i, s * M::STEP, lane));
 #pragma unroll
-                for (int p = 0; p < PARTS; ++p) acc[i] = M::mma(fa, fb[p], acc[i]);
+                for (int p = 0; p < M::PARTS; ++p) acc[i] = M::mma(fa, fb[p], acc[i]);
             }
         }
     };
@@ -242,14 +239,14 @@ __device__ __forceinline__ void scores(floatx4 (&acc)[4], const typename M::E* a
     }
 }
 
-// Four consecutive values into LDS, in PARTS parts that are `part` elements apart.
-template <class M, int PARTS>
+// Four consecutive values into LDS, in parts that are `part` elements apart.
+template <class M>
 __device__ __forceinline__ void put4(typename M::E* p, int part, floatx4 v) {
     if constexpr (sizeof(typename M::E) == 4) {
         *reinterpret_cast<f32x4*>(p) = f32x4{v[0], v[1], v[2], v[3]};
     } else {
 #pragma unroll
-        for (int s = 0; s < PARTS; ++s) {
+        for (int s = 0; s < M::PARTS; ++s) {
             const u32x2 w = {bf16_pk(v[0], v[1]), bf16_pk(v[2], v[3])};
             *reinterpret_cast<u32x2*>(p + s * part) = w;
             v = floatx4{rest(v[0], __uint_as_float(w[0] << 16)), rest(v[1], __uint_as_float(w[0] & 0xFFFF0000u)),
@@ -470,11 +467,11 @@ struct State {
         });
     }
     // Into LDS as [key][value], zeros (which what lies behind key and value need not be) behind them.
-    template <class M, int PARTS>
+    template <class M>
     __device__ __forceinline__ void put(typename M::E* t, int key, int value, int lane, int wave) {
         constexpr int LD = PV + M::PAD;
         if (key == NP && value == PV) {
-            each([&](int i, int j, floatx4& x) { put4<M, PARTS>(t + n(j, lane, wave) * LD + p(i, lane), NP * LD, x); });
+            each([&](int i, int j, floatx4& x) { put4<M>(t + n(j, lane, wave) * LD + p(i, lane), NP * LD, x); });
             return;
         }
         key = here(key), value = here(value);
@@ -483,7 +480,7 @@ struct State {
 #pragma unroll
             for (int r = 0; r < 4; ++r)
                 if (n(j, lane, wave) >= key || p(i, lane) + r >= value) y[r] = 0.0f;
-            put4<M, PARTS>(t + n(j, lane, wave) * LD + p(i, lane), NP * LD, y);
+            put4<M>(t + n(j, lane, wave) * LD + p(i, lane), NP * LD, y);
         });
     }
 };
@@ -503,12 +500,12 @@ __device__ __forceinline__ void update(State<NP>& s, const typename M::Frag (&fy
 #pragma unroll
             for (int c = 0; c < 4; ++c) x[e + c] *= w[c];
         }
-        typename M::Frag fx[M::THREE];
-        M::template split<M::THREE>(x, fx);
+        typename M::Frag fx[M::PARTS];
+        M::split(x, fx);
 #pragma unroll
         for (int i = 0; i < State<NP>::TP; ++i)
 #pragma unroll
-            for (int p = 0; p < M::THREE; ++p) s.v[i][j] = M::mma(fy[i], fx[p], s.v[i][j]);
+            for (int p = 0; p < M::PARTS; ++p) s.v[i][j] = M::mma(fy[i], fx[p], s.v[i][j]);
     }
 }
 // What infinities and NaN of y (tile [position][value]) add to it, where x's values are held in parts and zeros among these would make
@@ -590,9 +587,9 @@ __global__ void __launch_bounds__(WG, 2) k_attn_states(const Args a) {
         x.store(tx, tid);
         y.store(ty, tid);
         if (wave == 0) weight[lane] = BACK ? a.scale * __builtin_amdgcn_exp2f((float)g) : __builtin_amdgcn_exp2f((float)(all - g));
-        if constexpr (M::THREE > 1) say_finite(said, y.finite(), lane, wave);
+        if constexpr (M::PARTS > 1) say_finite(said, y.finite(), lane, wave);
         __syncthreads();
-        const bool finite = M::THREE == 1 || heard_finite(said);
+        const bool finite = M::PARTS == 1 || heard_finite(said);
         if (m + 1 < n) fetch(BACK ? c - 1 : c + 1, tid);
         passed += all;
         times(s, __builtin_amdgcn_exp2f((float)all));
@@ -699,7 +696,7 @@ __device__ __forceinline__ void zero_rows(const Heads& x, int64_t b, int h, int 
 }
 
 // ---- forward ------------------------------------------------------------------------------------------
-// A workgroup walks a piece with the state in registers, and lays it into LDS (split in two parts for bfloat16) for the product
+// A workgroup walks a piece with the state in registers, and lays it into LDS (in parts for bfloat16) for the product
 // with q; the next chunk's q, k and v are loaded into registers while this one's products run.  Bound in bfloat16 by vector work
 // (55% of the SIMDs' time: decays, splits, masks) and LDS, at 2.7 TB/s of inputs and results; in float32 by the matrix cores' rate
 // for it and LDS together, 110 us for 16 GFLOP.
@@ -707,7 +704,7 @@ template <int DT, int NP>
 struct FwdLds {
     using M = Mat<DT>;
     static constexpr int Q = 0, K = Tile<DT, NP>::SIZE, V = 2 * K, S = V + Tile<DT, PV>::SIZE, LDS_STATE = PV + M::PAD, PART = NP * LDS_STATE;
-    static constexpr int BYTES = (int)sizeof(typename M::E) * (S + M::TWO * PART);
+    static constexpr int BYTES = (int)sizeof(typename M::E) * (S + M::PARTS * PART);
 };
 template <int DT, int NP, bool EVEN>
 __global__ void __launch_bounds__(WG, NP == 128 ? 1 : 2) k_attn_fwd(const Args a) {
@@ -722,7 +719,7 @@ __global__ void __launch_bounds__(WG, NP == 128 ? 1 : 2) k_attn_fwd(const Args a
     E* tq = reinterpret_cast<E*>(lds) + L::Q;
     E* tk = reinterpret_cast<E*>(lds) + L::K;
     E* tv = reinterpret_cast<E*>(lds) + L::V;
-    E* ts = reinterpret_cast<E*>(lds) + L::S;  // [NP][PV] in two parts
+    E* ts = reinterpret_cast<E*>(lds) + L::S;  // [NP][PV] in parts
     __shared__ __attribute__((aligned(16))) Falls G;
     __shared__ __attribute__((aligned(16))) float weight[CHUNK];
     __shared__ int said[WAVES];
@@ -794,7 +791,7 @@ __global__ void __launch_bounds__(WG, NP == 128 ? 1 : 2) k_attn_fwd(const Args a
         q.store(tq, tid);
         k.store(tk, tid);
         v.store(tv, tid);
-        s.template put<M, M::TWO>(ts, a.key, vcols, lane, wave);
+        s.template put<M>(ts, a.key, vcols, lane, wave);
         if (wave == 0) {
             G.put(lane, in_two(g));
             weight[lane] = __builtin_amdgcn_exp2f((float)(all - g));
@@ -818,7 +815,7 @@ __global__ void __launch_bounds__(WG, NP == 128 ? 1 : 2) k_attn_fwd(const Args a
 #pragma unroll
             for (int p = 0; p < S::TP; ++p)
 #pragma unroll
-                for (int i = 0; i < M::TWO; ++i) y[p] = M::mma(M::col(ts + i * L::PART, L::LDS_STATE, 16 * p, n, lane), fq, y[p]);
+                for (int i = 0; i < M::PARTS; ++i) y[p] = M::mma(M::col(ts + i * L::PART, L::LDS_STATE, 16 * p, n, lane), fq, y[p]);
         }
         __builtin_amdgcn_sched_barrier(0);
         const int i = 16 * own + l15;
@@ -843,33 +840,33 @@ __global__ void __launch_bounds__(WG, NP == 128 ? 1 : 2) k_attn_fwd(const Args a
         if (finite) {
 #pragma unroll
             for (int k = 0; k < CHUNK / M::STEP; ++k) {
-                Frag fv[S::TP], fa[M::TWO];
+                Frag fv[S::TP], fa[M::PARTS];
 #pragma unroll
                 for (int p = 0; p < S::TP; ++p) fv[p] = M::mixed(tv, TV::LD, 16 * p, k * M::STEP, lane);
                 if (!M::SKIP || k <= own) {
-                    registers<M, M::TWO>(A, k, fa);
+                    registers<M>(A, k, fa);
 #pragma unroll
                     for (int p = 0; p < S::TP; ++p)
 #pragma unroll
-                        for (int x = 0; x < M::TWO; ++x) y[p] = M::mma(fv[p], fa[x], y[p]);
+                        for (int x = 0; x < M::PARTS; ++x) y[p] = M::mma(fv[p], fa[x], y[p]);
                 }
                 __builtin_amdgcn_sched_barrier(0);
                 update<M, NP, TN::LD>(s, fv, tk, weight, k, lane, wave);
                 __builtin_amdgcn_sched_barrier(0);
             }
         } else {
-            product_within<M, M::TWO>(y, false, tv, TV::LD, A, 0, own, lane, [&](int j) { return j <= i && i < rows; });
+            product_within<M>(y, false, tv, TV::LD, A, 0, own, lane, [&](int j) { return j <= i && i < rows; });
 #pragma unroll
             for (int k = 0; k < CHUNK / M::STEP; ++k) {
                 Frag fv[S::TP];
 #pragma unroll
                 for (int p = 0; p < S::TP; ++p) {
                     fv[p] = M::mixed(tv, TV::LD, 16 * p, k * M::STEP, lane);
-                    if constexpr (M::THREE > 1) fv[p] = M::finite(fv[p]);
+                    if constexpr (M::PARTS > 1) fv[p] = M::finite(fv[p]);
                 }
                 update<M, NP, TN::LD>(s, fv, tk, weight, k, lane, wave);
             }
-            if constexpr (M::THREE > 1) update_odd<M, NP, TN::LD, TV::LD>(s, tv, tk, weight, lane, wave);
+            if constexpr (M::PARTS > 1) update_odd<M, NP, TN::LD, TV::LD>(s, tv, tk, weight, lane, wave);
         }
 #pragma unroll
         for (int p = 0; p < S::TP; ++p) {
@@ -902,7 +899,7 @@ template <int DT, int NP, bool SHARED>
 struct BwdLds {
     using M = Mat<DT>;
     static constexpr int LDS_STATE = PV + M::PAD, PART = NP * LDS_STATE;
-    static constexpr int ONE = M::THREE * PART > Tile<DT, NP>::SIZE ? M::THREE * PART : Tile<DT, NP>::SIZE;
+    static constexpr int ONE = M::PARTS * PART > Tile<DT, NP>::SIZE ? M::PARTS * PART : Tile<DT, NP>::SIZE;
     static constexpr int Q = 0, K = ONE, V = SHARED ? K : K + Tile<DT, NP>::SIZE, D = V + Tile<DT, PV>::SIZE;
     static constexpr int BYTES = (int)sizeof(typename M::E) * (D + Tile<DT, PV>::SIZE);
 };
@@ -1022,11 +1019,11 @@ __global__ void __launch_bounds__(WG, NP == 128 ? 1 : TURNS || (DT == DT_BF16 &&
             }
             v.store(tv, tid);
             d.store(td, tid);
-            ds.template put<M, M::THREE>(tq, a.key, vcols, lane, own);
+            ds.template put<M>(tq, a.key, vcols, lane, own);
             const bool finite_kd = finite_k && d.finite();
             __syncthreads();
-            const float2 mine = G.at(me), g_end = G.at(CHUNK - 1);
-            const float to_end = fall_between(g_end, mine), from_start = a.scale * __builtin_amdgcn_exp2f(mine.x + mine.y);
+            const float2 mine = G.at(me);
+            const float to_end = fall_between(G.at(CHUNK - 1), mine), from_start = a.scale * __builtin_amdgcn_exp2f(mine.x + mine.y);
             floatx4 dq[NT], dk[NT], dv[S::TP], dA_i[4], dA_j[4];  // dy . v with the own positions as i, as j
             // what the positions behind the chunk give to dk and dv, by way of dS
 #pragma unroll
@@ -1039,7 +1036,7 @@ __global__ void __launch_bounds__(WG, NP == 128 ? 1 : TURNS || (DT == DT_BF16 &&
 #pragma unroll
                 for (int n = 0; n < NT; ++n)
 #pragma unroll
-                    for (int x = 0; x < M::THREE; ++x) dk[n] = M::mma(M::row(tq + x * L::PART, LS, 16 * n, p, lane), f, dk[n]);
+                    for (int x = 0; x < M::PARTS; ++x) dk[n] = M::mma(M::row(tq + x * L::PART, LS, 16 * n, p, lane), f, dk[n]);
                 __builtin_amdgcn_sched_barrier(0);
             }
             if constexpr (SHARED) {
@@ -1057,7 +1054,7 @@ __global__ void __launch_bounds__(WG, NP == 128 ? 1 : TURNS || (DT == DT_BF16 &&
 #pragma unroll
                 for (int p = 0; p < S::TP; ++p)
 #pragma unroll
-                    for (int x = 0; x < M::TWO; ++x) dv[p] = M::mma(M::col(tq + x * L::PART, LS, 16 * p, n, lane), f, dv[p]);
+                    for (int x = 0; x < M::PARTS; ++x) dv[p] = M::mma(M::col(tq + x * L::PART, LS, 16 * p, n, lane), f, dv[p]);
                 __builtin_amdgcn_sched_barrier(0);
             }
             {
@@ -1080,7 +1077,7 @@ __global__ void __launch_bounds__(WG, NP == 128 ? 1 : TURNS || (DT == DT_BF16 &&
             }
             __syncthreads();
             // and what the state before the chunk gives to dq
-            s.template put<M, M::THREE>(tq, a.key, vcols, lane, own);
+            s.template put<M>(tq, a.key, vcols, lane, own);
             __syncthreads();
 #pragma unroll
             for (int n = 0; n < NT; ++n) dq[n] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
@@ -1090,7 +1087,7 @@ __global__ void __launch_bounds__(WG, NP == 128 ? 1 : TURNS || (DT == DT_BF16 &&
 #pragma unroll
                 for (int n = 0; n < NT; ++n)
 #pragma unroll
-                    for (int x = 0; x < M::THREE; ++x) dq[n] = M::mma(M::row(tq + x * L::PART, LS, 16 * n, p, lane), f, dq[n]);
+                    for (int x = 0; x < M::PARTS; ++x) dq[n] = M::mma(M::row(tq + x * L::PART, LS, 16 * n, p, lane), f, dq[n]);
                 __builtin_amdgcn_sched_barrier(0);
             }
             __syncthreads();
@@ -1144,7 +1141,7 @@ __global__ void __launch_bounds__(WG, NP == 128 ? 1 : TURNS || (DT == DT_BF16 &&
                     if (t > own) dA[t] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
                 at = over_rows(at);
                 if (lane < 16) part_of(PAIRS, me) = at;
-                product_within<M, M::TWO>(dq, finite, tk, TN::LD, dA, 0, own, lane, [&](int j) { return j <= me && me < rows; });
+                product_within<M>(dq, finite, tk, TN::LD, dA, 0, own, lane, [&](int j) { return j <= me && me < rows; });
 #pragma unroll
                 for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -1171,9 +1168,9 @@ __global__ void __launch_bounds__(WG, NP == 128 ? 1 : TURNS || (DT == DT_BF16 &&
                     }
                 }
                 const auto inside = [&](int i) { return i >= me && i < rows; };
-                product_within<M, M::TWO>(dk, finite, tq, TN::LD, dA, own, 3, lane, inside);
+                product_within<M>(dk, finite, tq, TN::LD, dA, own, 3, lane, inside);
                 __builtin_amdgcn_sched_barrier(0);
-                product_within<M, M::TWO>(dv, finite, td, TV::LD, A, own, 3, lane, inside);
+                product_within<M>(dv, finite, td, TV::LD, A, own, 3, lane, inside);
                 __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
                 for (int n = 0; n < NT; ++n)
@@ -1193,6 +1190,7 @@ __global__ void __launch_bounds__(WG, NP == 128 ? 1 : TURNS || (DT == DT_BF16 &&
             __syncthreads();
             // dg, by one wavefront (lane = position)
             if (own == 0) {
+                const float2 g_end = G.at(CHUNK - 1);
                 const double over = ((double)through[turn & 1][0] + (double)through[turn & 1][1] + (double)through[turn & 1][2] + (double)through[turn & 1][3]) *
                                     (double)__builtin_amdgcn_exp2f(g_end.x + g_end.y);
                 const bool in = lane < rows;
