@@ -1457,7 +1457,7 @@ extern "C" int boa_linear_attention_fwd(const boa_attention* s, void* d_work, in
     const int rc = check_sizes("boa_linear_attention_fwd", s);
     if (rc != BOA_OK) return rc;
     if (s->batch == 0) return BOA_OK;
-    if (!s->decay || (s->length > 0 && (!s->q.p || !s->k.p || !s->v.p || !s->y.p)) || (uintptr_t)s->marks % 16)
+    if ((s->length > 0 && (!s->decay || !s->q.p || !s->k.p || !s->v.p || !s->y.p)) || (uintptr_t)s->marks % 16)
         return boa_fail(BOA_ERR_ARG, "boa_linear_attention_fwd: null pointer, or marks not at a multiple of 16 bytes");
     const Plan p(*s, false);
     if (p.bytes() > 0 && (!d_work || (uintptr_t)d_work % 16 || work_bytes < p.bytes()))
@@ -1485,10 +1485,12 @@ extern "C" int boa_linear_attention_bwd(const boa_attention* s, void* d_work, in
     const int rc = check_sizes("boa_linear_attention_bwd", s);
     if (rc != BOA_OK) return rc;
     const Plan p(*s, true);
-    if (!s->decay || !s->ddecay) return boa_fail(BOA_ERR_ARG, "boa_linear_attention_bwd: null pointer");
     const int64_t need = bwd_bytes(*s, p);
     hipStream_t st = (hipStream_t)stream;
-    if (s->batch == 0 || s->length == 0) {
+    const bool empty = s->batch == 0 || s->length == 0;  // no decay is read, and a gradient for each position has none either
+    if ((!empty && !s->decay) || ((!empty || s->decay_per_head) && !s->ddecay))
+        return boa_fail(BOA_ERR_ARG, "boa_linear_attention_bwd: null pointer");
+    if (empty) {
         if (s->decay_per_head) BOA_HIP_TRY(launch_sum_parts(nullptr, 0, s->heads, s->ddecay, st));
         return BOA_OK;
     }
