@@ -58,11 +58,11 @@ struct Args {
     float* pre;     // backward: [batch heads][chunks] decay from the chunk's end to its piece's
     double* fall;   // [batch heads][pieces] log2 of the piece's decay
     const float* fmarks;     // backward: the forward's
-    float *part_q, *part_k;  // backward: [batch][length][parts of each group][key], or null: dq, dk are written
+    float *part_q, *part_k;  // backward: [batch][length][groups][parts][key], or null: dq, dk are written
     float* dg;               // backward: [value tiles][batch][length][heads], or null
     float* dg_sum;           // backward: [batch * chunks * value tiles][heads], or null
     int64_t batch, length, chunks;
-    int32_t heads, share, in_turn, key, value, tiles, pieces, per_piece;
+    int32_t heads, share, parts, key, value, tiles, pieces, per_piece;
     float scale;
 };
 
@@ -909,8 +909,8 @@ struct BwdLds {
 // that one place in LDS does for both (four places and two workgroups: 255 us; 2 x 8192 x 16 in bfloat16 113 and 144).  Not in
 // turns, which keep k and need more registers, nor in bfloat16 of odd widths.  Walking chunks with the next one's tiles loaded
 // ahead needs more registers than there are.
-// A workgroup has one chunk, and of a group `in_turn` heads one after another: their queries and keys are read once, and what the
-// heads give to dq and dk is summed in registers.
+// A workgroup has one chunk of a head, or (TURNS) of all heads of a group one after another: their queries and keys are read once, and
+// what the heads give to dq and dk is summed in registers.
 template <int DT, int NP, bool TURNS, bool EVEN>
 __global__ void __launch_bounds__(WG, NP == 128 ? 1 : TURNS || (DT == DT_BF16 && !EVEN) ? 2 : 3) k_attn_bwd(const Args a) {
     using M = Mat<DT>;
@@ -936,22 +936,23 @@ __global__ void __launch_bounds__(WG, NP == 128 ? 1 : TURNS || (DT == DT_BF16 &&
     enum { PAIRS, FROM_STATE, TO_BEHIND };
     static_assert(M::PAD * sizeof(E) >= 3 * sizeof(float), "");
     const int first_own = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const uint32_t chunks = (uint32_t)a.chunks, rest = blockIdx.x / chunks, turns = (uint32_t)(a.share / a.in_turn);
+    const uint32_t chunks = (uint32_t)a.chunks, rest = blockIdx.x / chunks;
     const int64_t c = blockIdx.x - rest * chunks, t0 = c * CHUNK;
     const int tile = (int)(rest % (uint32_t)a.tiles);
-    const uint32_t set = rest / (uint32_t)a.tiles, bg = set / turns;  // a group's heads in turn; a sequence's group
+    const uint32_t turns = TURNS ? (uint32_t)a.share : 1u, sets = (uint32_t)a.share / turns;  // heads of a workgroup, workgroups of a group
+    const uint32_t set = rest / (uint32_t)a.tiles, bg = set / sets;  // bg: a sequence's group
     const uint32_t groups = (uint32_t)(a.heads / a.share);
     const int64_t b = bg / groups;
-    const int gr = (int)(bg % groups), h0 = gr * a.share + (int)(set % turns) * a.in_turn;
+    const int gr = (int)(bg % groups), h0 = gr * a.share + (int)(set % sets), h1 = h0 + (int)turns;
     const int64_t end = end_of(a, b);
     const int present = (int)min((int64_t)CHUNK, a.length - t0);
     const int all_rows = (int)max((int64_t)0, min((int64_t)CHUNK, end - t0));  // that hold something
     const int vcols = min(PV, a.value - tile * PV);
     const auto part_row = [&](float* p, int64_t i) {
-        return p + (((b * a.length + t0 + i) * groups + gr) * turns * a.tiles + (set % turns) * a.tiles + tile) * a.key;
+        return p + (((b * a.length + t0 + i) * groups + gr) * sets * a.tiles + (set % sets) * a.tiles + tile) * a.key;
     };
     if (all_rows < present) {
-        for (int h = h0; h < h0 + a.in_turn; ++h) zero_rows<DT>(a.dv, b, h, tile * PV, vcols, t0 + all_rows, t0 + present);
+        for (int h = h0; h < h1; ++h) zero_rows<DT>(a.dv, b, h, tile * PV, vcols, t0 + all_rows, t0 + present);
         if (a.part_q == nullptr) {
             zero_rows<DT>(a.dq, b, gr, 0, a.key, t0 + all_rows, t0 + present);
             zero_rows<DT>(a.dk, b, gr, 0, a.key, t0 + all_rows, t0 + present);
@@ -963,7 +964,7 @@ __global__ void __launch_bounds__(WG, NP == 128 ? 1 : TURNS || (DT == DT_BF16 &&
     const auto dg_of = [&](int h) { return a.dg == nullptr ? nullptr : a.dg + ((tile * a.batch + b) * a.length + t0) * a.heads + h; };
     const auto dg_sum_of = [&](int h) { return a.dg_sum == nullptr ? nullptr : a.dg_sum + ((b * a.chunks + c) * a.tiles + tile) * a.heads + h; };
     if (all_rows == 0) {
-        for (int h = h0; h < h0 + a.in_turn; ++h) {
+        for (int h = h0; h < h1; ++h) {
             if (a.dg != nullptr && (int)threadIdx.x < present) dg_of(h)[(int64_t)threadIdx.x * a.heads] = 0.0f;
             if (a.dg_sum != nullptr && threadIdx.x == 0) *dg_sum_of(h) = 0.0f;
         }
@@ -971,7 +972,7 @@ __global__ void __launch_bounds__(WG, NP == 128 ? 1 : TURNS || (DT == DT_BF16 &&
     }
     floatx4 all_dq[NT] = {}, all_dk[NT] = {};
     bool finite_k = false;
-    for (int turn = 0; turn < (TURNS ? a.in_turn : 1); ++turn) {
+    for (int turn = 0; turn < (TURNS ? a.share : 1); ++turn) {
         const int tid = TURNS ? here_lane(threadIdx.x) : threadIdx.x, lane = tid & 63, own = TURNS ? here(first_own) : first_own;
         const int rows = TURNS ? here(all_rows) : all_rows;
         const int l15 = lane & 15, row4 = 4 * (lane >> 4), me = 16 * own + l15;  // the own position, as i of dq and as j of dk and dv
@@ -1228,7 +1229,7 @@ __global__ void __launch_bounds__(WG) k_attn_sum(const Args a, int groups) {
     const float* part = blockIdx.y == 0 ? a.part_q : a.part_k;
     const Heads out = blockIdx.y == 0 ? a.dq : a.dk;
     const int64_t n = a.batch * a.length * groups * a.key;
-    const int each = a.share / a.in_turn * a.tiles;
+    const int each = a.parts;
     for (int64_t i = (int64_t)blockIdx.x * WG + threadIdx.x; i < n; i += (int64_t)gridDim.x * WG) {
         const int col = (int)(i % a.key), gr = (int)(i / a.key % groups);
         const int64_t bt = i / a.key / groups;
@@ -1362,18 +1363,18 @@ struct Plan {
     }
 };
 
-// Heads of a group that a workgroup of the backward pass takes in turn: as many as leave two for each CU twice over.
-// 32 x 500 x 16 heads of 4 groups in bfloat16: 109 us so, 135 + 45 for the sums over heads with each head by itself, 121 + 36 with
-// two in turn.  Forward and backward of 2 x 8192 x 16 heads of 8 groups, whole groups in turn: 404 us in float32 and 248 in bfloat16,
-// each head by itself 451 and 298; where only a part of a group can be (2 to 4 of 4 to 16 heads) it is 10% less to 11% more.
-int in_turn(const boa_attention& s, const Plan& p) {
+// Whether a workgroup of the backward pass takes the heads of a group in turn: where that leaves two workgroups for each place on a CU
+// (two places, with more than 64 keys one), else each head by itself.
+// 32 x 500 x 16 heads of 4 groups in bfloat16: 109 us so, 135 + 45 for the sums over heads with each head by itself.  Forward and
+// backward of 2 x 8192 x 16 heads of 8 groups: 404 us in float32 and 248 in bfloat16, each head by itself 451 and 298; of 4 x 4096 x 16
+// heads of 2 groups and 128 keys 746 and 493, each by itself 903 and 631.  (A part of a group in turn: of 300 x 65 x 8 heads and 64 x
+// 500 x 8 heads of one group in bfloat16 247 and 215 us, each by itself 205 and 230.)
+bool in_turn(const boa_attention& s, const Plan& p) {
     const int share = s.heads / s.groups;
-    for (int n = share; n > 1; --n)
-        if (share % n == 0 && p.bh / n * p.tiles * p.chunks >= 2 * WANTED) return n;
-    return 1;
+    return share > 1 && p.bh / share * p.tiles * p.chunks >= (p.np == 64 ? 2 : 1) * WANTED;
 }
 // Parts of a group's dq and dk, which are then summed.
-int64_t group_parts(const boa_attention& s, const Plan& p) { return (int64_t)(s.heads / s.groups / in_turn(s, p)) * p.tiles; }
+int group_parts(const boa_attention& s, const Plan& p) { return (in_turn(s, p) ? 1 : s.heads / s.groups) * p.tiles; }
 
 int64_t bwd_bytes(const boa_attention& s, const Plan& p) {
     int64_t n = p.bytes();
@@ -1504,9 +1505,10 @@ extern "C" int boa_linear_attention_bwd(const boa_attention* s, void* d_work, in
     a.fmarks = s->marks;
     a.state_in = nullptr, a.state_out = nullptr;
     float* rest = reinterpret_cast<float*>(static_cast<char*>(d_work) + p.bytes());
-    a.in_turn = in_turn(*s, p);
-    if (group_parts(*s, p) > 1) {
-        const int64_t each = s->batch * s->length * s->groups * group_parts(*s, p) * s->key;
+    const bool turns = in_turn(*s, p);
+    a.parts = group_parts(*s, p);
+    if (a.parts > 1) {
+        const int64_t each = s->batch * s->length * s->groups * a.parts * s->key;
         a.part_q = rest, a.part_k = rest + each;
         rest += 2 * each;
     }
@@ -1517,8 +1519,8 @@ extern "C" int boa_linear_attention_bwd(const boa_attention* s, void* d_work, in
             constexpr bool EVEN = decltype(even)::value;
             constexpr int DT = decltype(dt)::value, NP = decltype(np)::value;
             if (const int no = launch_states<DT, NP, true, EVEN>(a, p, st)) return no;
-            const dim3 grid((uint32_t)(p.bh / a.in_turn * p.tiles * p.chunks));
-            if (a.in_turn > 1) {
+            const dim3 grid((uint32_t)(p.bh / (turns ? a.share : 1) * p.tiles * p.chunks));
+            if (turns) {
                 constexpr int LDS = BwdLds<DT, NP, false>::BYTES;
                 if (const int no = allow_lds(k_attn_bwd<DT, NP, true, EVEN>, LDS)) return no;
                 hipLaunchKernelGGL((k_attn_bwd<DT, NP, true, EVEN>), grid, dim3(WG), LDS, st, a);
