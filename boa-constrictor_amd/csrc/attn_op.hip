@@ -108,10 +108,13 @@ template <int DT> struct Mat {
     }
 };
 typedef short s16x4 __attribute__((ext_vector_type(4)));
-// What is left of f behind its part hi; nothing behind an infinite one.
-__device__ __forceinline__ float rest(float f, float hi) {
-    const float r = f - hi;
-    return r == r ? r : 0.0f;
+// Parts of float32 values: the upper halves, cut off rather than rounded, so that three of them are the value itself, and finite where it
+// is finite.
+__device__ __forceinline__ uint32_t uppers(float lo, float hi) { return __builtin_amdgcn_perm(__float_as_uint(hi), __float_as_uint(lo), 0x07060302u); }
+// What is left of f behind its upper half; nothing behind an infinite one.
+__device__ __forceinline__ float rest(float f) {
+    const float r = f - __uint_as_float(__float_as_uint(f) & 0xFFFF0000u);
+    return fabsf(f) == __builtin_inff() ? 0.0f : r;
 }
 template <> struct Mat<DT_BF16> {
     using E = uint16_t;
@@ -151,9 +154,9 @@ template <> struct Mat<DT_BF16> {
             u32x4 w;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                w[i] = bf16_pk(v[2 * i], v[2 * i + 1]);
-                v[2 * i] = rest(v[2 * i], __uint_as_float(w[i] << 16));
-                v[2 * i + 1] = rest(v[2 * i + 1], __uint_as_float(w[i] & 0xFFFF0000u));
+                w[i] = uppers(v[2 * i], v[2 * i + 1]);
+                v[2 * i] = rest(v[2 * i]);
+                v[2 * i + 1] = rest(v[2 * i + 1]);
             }
             f[s] = __builtin_bit_cast(Frag, w);
         }
@@ -176,7 +179,10 @@ template <class M>
 __device__ __forceinline__ void registers(const floatx4 (&t)[4], int s, typename M::Frag (&f)[M::PARTS]) {
     float x[M::VEC];
 #pragma unroll
-    for (int e = 0; e < M::VEC; ++e) x[e] = t[s * (M::VEC / 4) + e / 4][e % 4];
+    for (int e = 0; e < M::VEC; ++e) {
+        x[e] = t[s * (M::VEC / 4) + e / 4][e % 4];
+        if (M::PARTS > 1) asm volatile("" : "+v"(x[e]));  // else the splits of all steps are made ahead, and kept
+    }
     M::split(x, f);
 }
 // Row k (the same for all lanes) of the lane's column of a register operand of four tiles.
@@ -247,10 +253,9 @@ __device__ __forceinline__ void put4(typename M::E* p, int part, floatx4 v) {
     } else {
 #pragma unroll
         for (int s = 0; s < M::PARTS; ++s) {
-            const u32x2 w = {bf16_pk(v[0], v[1]), bf16_pk(v[2], v[3])};
+            const u32x2 w = {uppers(v[0], v[1]), uppers(v[2], v[3])};
             *reinterpret_cast<u32x2*>(p + s * part) = w;
-            v = floatx4{rest(v[0], __uint_as_float(w[0] << 16)), rest(v[1], __uint_as_float(w[0] & 0xFFFF0000u)),
-                        rest(v[2], __uint_as_float(w[1] << 16)), rest(v[3], __uint_as_float(w[1] & 0xFFFF0000u))};
+            v = floatx4{rest(v[0]), rest(v[1]), rest(v[2]), rest(v[3])};
         }
     }
 }
