@@ -98,6 +98,9 @@ template <int DT> struct Mat {
     static __device__ __forceinline__ void split(const float (&x)[VEC], Frag (&f)[PARTS]) {
         f[0] = Frag{x[0], x[1], x[2], x[3]};
     }
+    // An operand times a factor: all of it, or a power of two now and the rest of it (`behind`) times the product.
+    static __device__ __forceinline__ Frag scaled(const Frag& f, float by) { return Frag{f[0] * by, f[1] * by, f[2] * by, f[3] * by}; }
+    static __device__ __forceinline__ float behind(float) { return 1.0f; }
     static __device__ __forceinline__ floatx4 load4(const E* p) { return *reinterpret_cast<const floatx4*>(p); }
     static __device__ __forceinline__ float value(E v) { return v; }
     // zeros in the place of infinities and NaN
@@ -160,6 +163,17 @@ template <> struct Mat<DT_BF16> {
             }
             f[s] = __builtin_bit_cast(Frag, w);
         }
+    }
+    // A power of two leaves a bfloat16 value one, down to the smallest ones.
+    static __device__ __forceinline__ Frag scaled(const Frag& f, float by) {
+        const float two = __uint_as_float(__float_as_uint(by) & 0x7F800000u);
+        u32x4 w = __builtin_bit_cast(u32x4, f);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = uppers(__uint_as_float(w[i] << 16) * two, __uint_as_float(w[i] & 0xFFFF0000u) * two);
+        return __builtin_bit_cast(Frag, w);
+    }
+    static __device__ __forceinline__ float behind(float by) {
+        return by == by ? __uint_as_float((__float_as_uint(by) & 0x807FFFFFu) | 0x3F800000u) : by;
     }
     static __device__ __forceinline__ floatx4 load4(const E* p) {
         float v[4];
@@ -405,14 +419,23 @@ __device__ __forceinline__ floatx4 falls(const Falls& g, float2 own, float scale
     }
     return f;
 }
-// Whether any value that the workgroup's threads have is not finite, by way of a barrier: each wavefront says so in LDS.
-__device__ __forceinline__ void say_finite(int* said, bool finite, int lane, int wave) {
-    const bool all = __ballot(!finite) == 0;
+// Whether all values that the workgroup's threads have are finite, by way of a barrier: each wavefront says so in LDS, of one set of
+// values or (in bit 1) of two.
+__device__ __forceinline__ void say_finite(int* said, bool finite, int lane, int wave, bool other = true) {
+    const int all = (__ballot(!finite) == 0 ? 1 : 0) | (__ballot(!other) == 0 ? 2 : 0);
     if (lane == 0) said[wave] = all;
 }
-__device__ __forceinline__ bool heard_finite(const int* said) {
-    const int all = said[0] & said[1] & said[2] & said[3];
-    return __builtin_amdgcn_readfirstlane(all) != 0;
+__device__ __forceinline__ int heard(const int* said) { return __builtin_amdgcn_readfirstlane(said[0] & said[1] & said[2] & said[3]); }
+__device__ __forceinline__ bool heard_finite(const int* said) { return (heard(said) & 1) != 0; }
+
+// Whether a pair of positions with this decay between them counts.  A score of finite values may pass float32's range and is nothing all
+// the same behind a decay of zero; where an infinity or NaN is among the values that scores are made of (not FINITE), it is not.
+template <bool FINITE>
+__device__ __forceinline__ bool counts(float f) { return !FINITE || f != 0.0f; }
+template <class F>
+__device__ __forceinline__ void where_finite(bool finite, F f) {
+    if (finite) f(std::true_type());
+    else f(std::false_type());
 }
 
 __device__ __forceinline__ int64_t end_of(const Args& a, int64_t b) {
@@ -801,9 +824,10 @@ __global__ void __launch_bounds__(WG, NP == 128 ? 1 : 2) k_attn_fwd(const Args a
             G.put(lane, in_two(g));
             weight[lane] = __builtin_amdgcn_exp2f((float)(all - g));
         }
-        say_finite(said, v.finite(), lane, wave);
+        say_finite(said, v.finite(), lane, wave, k.finite());
         __syncthreads();
-        const bool finite = heard_finite(said);
+        const int all_finite = heard(said);
+        const bool finite = (all_finite & 1) != 0, finite_k = (all_finite & 2) != 0;
         if (c > c0) write(t0 - CHUNK, tid);
         if (marks != nullptr) s.store(marks + c * S::SIZE, lane, wave);
         if (c + 1 < c1) fetch(c + 1, tid);
@@ -812,34 +836,36 @@ __global__ void __launch_bounds__(WG, NP == 128 ? 1 : 2) k_attn_fwd(const Args a
         floatx4 A[4], y[S::TP];
         scores<M, NP>(A, tk, tq, TN::LD, 16 * own, 0, own, lane);
         __builtin_amdgcn_sched_barrier(0);
+        const int i = 16 * own + l15;
+        const float2 gi = G.at(i);
+        const float from_start = a.scale * __builtin_amdgcn_exp2f(gi.x + gi.y);
 #pragma unroll
         for (int p = 0; p < S::TP; ++p) y[p] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int n = 0; n < NP; n += M::STEP) {
-            const Frag fq = M::row(tq, TN::LD, 16 * own, n, lane);
+            const Frag fq = M::scaled(M::row(tq, TN::LD, 16 * own, n, lane), from_start);
 #pragma unroll
             for (int p = 0; p < S::TP; ++p)
 #pragma unroll
                 for (int i = 0; i < M::PARTS; ++i) y[p] = M::mma(M::col(ts + i * L::PART, L::LDS_STATE, 16 * p, n, lane), fq, y[p]);
         }
         __builtin_amdgcn_sched_barrier(0);
-        const int i = 16 * own + l15;
-        const float2 gi = G.at(i);
-        const float from_start = a.scale * __builtin_amdgcn_exp2f(gi.x + gi.y);
+        where_finite(finite_k, [&](auto clean) {  // a query that is not finite reaches its own position, with no decay
 #pragma unroll
-        for (int t = 0; t < 4; ++t) {
-            const floatx4 f = falls<true>(G, gi, a.scale, lane, t);
+            for (int t = 0; t < 4; ++t) {
+                const floatx4 f = falls<true>(G, gi, a.scale, lane, t);
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int j = 16 * t + row4 + r;
-                const float x = A[t][r] * f[r];
-                A[t][r] = j <= i && i < rows ? x : 0.0f;
+                for (int r = 0; r < 4; ++r) {
+                    const int j = 16 * t + row4 + r;
+                    const float x = A[t][r] * f[r];
+                    A[t][r] = j <= i && i < rows && counts<decltype(clean)::value>(f[r]) ? x : 0.0f;
+                }
             }
-        }
+        });
 #pragma unroll
         for (int p = 0; p < S::TP; ++p)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) y[p][r] *= from_start;
+            for (int r = 0; r < 4; ++r) y[p][r] *= M::behind(from_start);
         __builtin_amdgcn_sched_barrier(0);
         times(s, __builtin_amdgcn_exp2f((float)all));
         if (finite) {
@@ -1006,16 +1032,17 @@ __global__ void __launch_bounds__(WG, NP == 128 ? 1 : TURNS || (DT == DT_BF16 &&
             if (own == 0) G.put(lane, in_two(g));
             {  // what passes over the chunk; behind key and value there may be anything
                 float x = 0.0f;
+                const float fall = __builtin_amdgcn_exp2f((float)last_lane(g));
                 const bool full = a.key == NP && vcols == PV;
                 const int key = here(a.key), value = here(vcols);
                 s.each([&](int i, int j, floatx4& y) {
                     if (full) {
 #pragma unroll
-                        for (int r = 0; r < 4; ++r) x = __builtin_fmaf(y[r], ds.v[i][j][r], x);
+                        for (int r = 0; r < 4; ++r) x = __builtin_fmaf(y[r] * fall, ds.v[i][j][r], x);
                     } else {
 #pragma unroll
                         for (int r = 0; r < 4; ++r) {
-                            const float z = __builtin_fmaf(y[r], ds.v[i][j][r], x);
+                            const float z = __builtin_fmaf(y[r] * fall, ds.v[i][j][r], x);
                             x = S::n(j, lane, own) < key && S::p(i, lane) + r < value ? z : x;
                         }
                     }
@@ -1026,7 +1053,7 @@ __global__ void __launch_bounds__(WG, NP == 128 ? 1 : TURNS || (DT == DT_BF16 &&
             v.store(tv, tid);
             d.store(td, tid);
             ds.template put<M>(tq, a.key, vcols, lane, own);
-            const bool finite_kd = finite_k && d.finite();
+            const bool finite_kvd = finite_k && v.finite() && d.finite();
             __syncthreads();
             const float2 mine = G.at(me);
             const float to_end = fall_between(G.at(CHUNK - 1), mine), from_start = a.scale * __builtin_amdgcn_exp2f(mine.x + mine.y);
@@ -1038,7 +1065,7 @@ __global__ void __launch_bounds__(WG, NP == 128 ? 1 : TURNS || (DT == DT_BF16 &&
             for (int p = 0; p < S::TP; ++p) dv[p] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (int p = 0; p < PV; p += M::STEP) {
-                const Frag f = M::row(tv, TV::LD, 16 * own, p, lane);
+                const Frag f = M::scaled(M::row(tv, TV::LD, 16 * own, p, lane), to_end);
 #pragma unroll
                 for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -1056,7 +1083,7 @@ __global__ void __launch_bounds__(WG, NP == 128 ? 1 : TURNS || (DT == DT_BF16 &&
             }
 #pragma unroll
             for (int n = 0; n < NP; n += M::STEP) {
-                const Frag f = M::row(tk, TN::LD, 16 * own, n, lane);
+                const Frag f = M::scaled(M::row(tk, TN::LD, 16 * own, n, lane), to_end);
 #pragma unroll
                 for (int p = 0; p < S::TP; ++p)
 #pragma unroll
@@ -1070,7 +1097,7 @@ __global__ void __launch_bounds__(WG, NP == 128 ? 1 : TURNS || (DT == DT_BF16 &&
                     const floatx4 f = M::load4(tk + me * TN::LD + 16 * n + row4);
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
-                        dk[n][r] *= to_end;
+                        dk[n][r] *= M::behind(to_end);
                         x = __builtin_fmaf(dk[n][r], f[r], x);
                     }
                 }
@@ -1079,7 +1106,7 @@ __global__ void __launch_bounds__(WG, NP == 128 ? 1 : TURNS || (DT == DT_BF16 &&
 #pragma unroll
                 for (int p = 0; p < S::TP; ++p)
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) dv[p][r] *= to_end;
+                    for (int r = 0; r < 4; ++r) dv[p][r] *= M::behind(to_end);
             }
             __syncthreads();
             // and what the state before the chunk gives to dq
@@ -1089,7 +1116,7 @@ __global__ void __launch_bounds__(WG, NP == 128 ? 1 : TURNS || (DT == DT_BF16 &&
             for (int n = 0; n < NT; ++n) dq[n] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (int p = 0; p < PV; p += M::STEP) {
-                const Frag f = M::row(td, TV::LD, 16 * own, p, lane);
+                const Frag f = M::scaled(M::row(td, TV::LD, 16 * own, p, lane), from_start);
 #pragma unroll
                 for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -1098,7 +1125,7 @@ __global__ void __launch_bounds__(WG, NP == 128 ? 1 : TURNS || (DT == DT_BF16 &&
             }
             __syncthreads();
             q.store(tq, tid);
-            say_finite(said, finite_kd && q.finite(), lane, own);
+            say_finite(said, finite_kvd && q.finite(), lane, own);
             __syncthreads();
             const bool finite = heard_finite(said);
             {
@@ -1108,7 +1135,7 @@ __global__ void __launch_bounds__(WG, NP == 128 ? 1 : TURNS || (DT == DT_BF16 &&
                     const floatx4 f = M::load4(tq + me * TN::LD + 16 * n + row4);
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
-                        dq[n][r] *= from_start;
+                        dq[n][r] *= M::behind(from_start);
                         x = __builtin_fmaf(dq[n][r], f[r], x);
                     }
                 }
@@ -1126,22 +1153,24 @@ __global__ void __launch_bounds__(WG, NP == 128 ? 1 : TURNS || (DT == DT_BF16 &&
                 // the pairs that a position t of the own ones lies between: of M_ij the sum over the own i >= t, then over j < t; and all
                 // own i for the positions of the tiles before
                 float at = 0.0f;
+                where_finite(finite, [&](auto clean) {
 #pragma unroll
-                for (int t = 0; t < 4; ++t) {
-                    if (t > own) continue;
-                    const floatx4 f = falls<true>(G, mine, a.scale, lane, t);
-                    floatx4 sums;
+                    for (int t = 0; t < 4; ++t) {
+                        if (t > own) continue;
+                        const floatx4 f = falls<true>(G, mine, a.scale, lane, t);
+                        floatx4 sums;
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        const int j = 16 * t + row4 + r;
-                        const bool in = j <= me && me < rows;
-                        const float x = dA[t][r] * f[r], m = A[t][r] * x;
-                        dA[t][r] = in ? x : 0.0f;
-                        sums[r] = from_here(in ? m : 0.0f);
-                        at += j < me ? sums[r] : 0.0f;
+                        for (int r = 0; r < 4; ++r) {
+                            const int j = 16 * t + row4 + r;
+                            const bool in = j <= me && me < rows && counts<decltype(clean)::value>(f[r]);
+                            const float x = dA[t][r] * f[r], m = A[t][r] * x;
+                            dA[t][r] = in ? x : 0.0f;
+                            sums[r] = from_here(in ? m : 0.0f);
+                            at += j < me ? sums[r] : 0.0f;
+                        }
+                        if (t < own && l15 == 0) *reinterpret_cast<floatx4*>(&middle[own - 1][16 * t + row4]) = sums;
                     }
-                    if (t < own && l15 == 0) *reinterpret_cast<floatx4*>(&middle[own - 1][16 * t + row4]) = sums;
-                }
+                });
 #pragma unroll
                 for (int t = 1; t < 4; ++t)
                     if (t > own) dA[t] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
@@ -1161,18 +1190,20 @@ __global__ void __launch_bounds__(WG, NP == 128 ? 1 : TURNS || (DT == DT_BF16 &&
                 __builtin_amdgcn_sched_barrier(0);
                 if (!SHARED) scores<M, PV>(dA, td, tv, TV::LD, 16 * own, own, 3, lane);
                 __builtin_amdgcn_sched_barrier(0);
+                where_finite(finite, [&](auto clean) {
 #pragma unroll
-                for (int t = 0; t < 4; ++t) {
-                    const floatx4 f = falls<false>(G, mine, a.scale, lane, t);
+                    for (int t = 0; t < 4; ++t) {
+                        const floatx4 f = falls<false>(G, mine, a.scale, lane, t);
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        const int i = 16 * t + row4 + r;
-                        const bool in = i >= me && i < rows;
-                        const float x = A[t][r] * f[r], y = dA[t][r] * f[r];
-                        A[t][r] = in ? x : 0.0f;
-                        dA[t][r] = in ? y : 0.0f;
+                        for (int r = 0; r < 4; ++r) {
+                            const int i = 16 * t + row4 + r;
+                            const bool in = i >= me && i < rows && counts<decltype(clean)::value>(f[r]);
+                            const float x = A[t][r] * f[r], y = dA[t][r] * f[r];
+                            A[t][r] = in ? x : 0.0f;
+                            dA[t][r] = in ? y : 0.0f;
+                        }
                     }
-                }
+                });
                 const auto inside = [&](int i) { return i >= me && i < rows; };
                 product_within<M>(dk, finite, tq, TN::LD, dA, own, 3, lane, inside);
                 __builtin_amdgcn_sched_barrier(0);
@@ -1196,9 +1227,8 @@ __global__ void __launch_bounds__(WG, NP == 128 ? 1 : TURNS || (DT == DT_BF16 &&
             __syncthreads();
             // dg, by one wavefront (lane = position)
             if (own == 0) {
-                const float2 g_end = G.at(CHUNK - 1);
-                const double over = ((double)through[turn & 1][0] + (double)through[turn & 1][1] + (double)through[turn & 1][2] + (double)through[turn & 1][3]) *
-                                    (double)__builtin_amdgcn_exp2f(g_end.x + g_end.y);
+                const float(&over_of)[WAVES] = through[turn & 1];
+                const double over = (double)over_of[0] + (double)over_of[1] + (double)over_of[2] + (double)over_of[3];
                 const bool in = lane < rows;
                 // from the states before: positions i from t on (summed from the last one); to the positions behind the chunk: j before t
                 const int last = CHUNK - 1 - lane;
@@ -1284,7 +1314,7 @@ __global__ void __launch_bounds__(WG) k_attn_step(const Args a) {
                 for (int i = 0; i < AT_ONCE; ++i) {
                     const int n = min(n0 + i * ROWS, a.key - 1);
                     kn[i] = Elem<DT>::ld(k[n]);
-                    qn[i] = Elem<DT>::ld(q[n]);
+                    qn[i] = a.scale * Elem<DT>::ld(q[n]);
                     if (whole) {
                         Raw<DT_F32, VEC>::unpack(*reinterpret_cast<const AnyAt*>(st + (int64_t)n * a.value), s[i]);
                     } else if (!EVEN) {
@@ -1319,7 +1349,7 @@ __global__ void __launch_bounds__(WG) k_attn_step(const Args a) {
             __syncthreads();
             if (threadIdx.x < PV && p0 + (int)threadIdx.x < a.value) {
                 const int c = threadIdx.x;
-                row_of<DT>(a.y, b, 0, h)[p0 + c] = Elem<DT>::st(a.scale * ((part[0][c] + part[1][c]) + (part[2][c] + part[3][c])));
+                row_of<DT>(a.y, b, 0, h)[p0 + c] = Elem<DT>::st((part[0][c] + part[1][c]) + (part[2][c] + part[3][c]));
             }
             __syncthreads();
         }
