@@ -676,7 +676,8 @@ def linear_attention(q, k, v, log_decay, *, scale=None, state=None, lens=None, r
     value] (1 to 512); log_decay: float32 [heads], or [batch, length, heads] for one of each position's own, 0 or negative (-inf
     forgets everything before); scale: 1 / sqrt(key) unless given.  state: float32 [batch, heads, key, value] before the first
     position (zeros without).  Returns y [batch, length, heads, value], with ``return_state`` also the state behind each
-    sequence's last position, as a new tensor."""
+    sequence's last position, as a new tensor.  Products q . k of near positions are made before scale and decay: beyond float32's
+    range they are infinite (nothing behind a decay of zero)."""
     who = "linear_attention"
     _plain(who, q, k, v, log_decay, state)
     q, k, v, g, scale = _attention_args(who, 4, q, k, v, log_decay, scale)

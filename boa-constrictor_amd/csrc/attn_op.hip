@@ -25,10 +25,11 @@
 // operand as it is; its own 16 of every 64 keys in a state.
 //
 // Measured with 64 keys and 64 values a head (copies of the sizes moved here reach 5 to 6 TB/s, float32 products of libraries 150
-// TFLOP/s), kernels in us; 4 x 4097 positions x 16 heads of 4 groups in bfloat16: states 21, joined 6, forward 50 (136 MB and as
-// much of k and v again); 2 x 16384 x 8 heads in float32: forward 38 + 7 + 110, backward 44 + 7 + 224 (539 MB, and 27 GFLOP of
-// products, 183 us at the libraries' rate); 32 x 500 x 16 heads of 4 groups in bfloat16: forward 44, backward 21 + 109; one position
-// of 1000 x 16 heads: 83 (532 MB, 6.4 TB/s).  What bounds each stands at its kernel.
+// TFLOP/s), kernels in us; 4 x 4097 positions x 16 heads of 16 groups in bfloat16: states 21, joined 6, forward 59 (136 MB and as
+// much of k and v again); 2 x 16384 x 8 heads in float32: forward 38 + 7 + 112, backward 44 + 7 + 219 (539 MB, and 22 GFLOP of
+// products that are needed, 149 us at the libraries' rate; 27 are done, with the scores in both orientations and k and v walked
+// twice); 32 x up to 500 x 16 heads of 4 groups in bfloat16: forward 44 to 52, backward 18 to 20 + 126; one position of 1000 x 16
+// heads: 83 (532 MB, 6.4 TB/s).  What bounds each stands at its kernel.
 #include "ops_common.h"
 
 #include "../../include/boa_hip.h"
@@ -69,7 +70,8 @@ struct Args {
 // How products of a type run: elements in LDS, K of a step, parts that a float32 value is split into.
 //   bfloat16: inputs as they are.  What is computed on the way (A, dA, states, decayed keys) is split into three parts of 8 bits
 //   each, float32's 24: with two, terms that cancel would leave an error beyond the result's own rounding.
-//   float32, and float16, whose range the parts of a float32 value do not fit: float32 products (v_mfma_f32_16x16x4_f32).
+//   float32 and float16: float32 products (v_mfma_f32_16x16x4_f32).  Parts of A, dA and states do not fit float16's range; q . k and
+//   dy . v, whose operands are float16, would fit its products but are made like the rest.
 // A fragment holds VEC elements along K per lane: `row` of a tile with K along memory, `col` of one with K across; element e of lane
 // group g is k = VEC g + e.  `mixed` is `col` in the order of register tiles, k = 16 (e / 4) + 4 g + e % 4: element e of
 // `registers` is row 4 g + e % 4 of tile e / 4 of a result.
@@ -564,8 +566,9 @@ __device__ __forceinline__ void times(State<NP>& s, float f) {
 // ---- states by themselves ---------------------------------------------------------------------------
 // A workgroup walks the chunks of a piece from a state of zeros, forward over k v^T or (BACK) from the last one over scale e^(G_i)
 // q dy^T; leaves what it ends with, and backward also what it reaches each chunk with.  The state stays in registers; two
-// workgroups on a CU hide each other's loads.  A chunk takes a workgroup about 2.7 us, of which a product of 64 x 64 x 64 is the
-// smallest part: it waits for the next chunk's loads and LDS (k and v at 4.1 TB/s in bfloat16, 3.7 in float32 over 2 x 16384 x 8).
+// workgroups on a CU hide each other's loads.  A chunk takes a workgroup about 2.4 us, of which a product of 64 x 64 x 64 is the
+// smallest part: nothing is full (vector 58%, matrix 17%, LDS 24% of the cycles in bfloat16; 18, 47 and 22% in float32), it waits for
+// the next chunk's loads and at two barriers (k and v at 3.2 TB/s in bfloat16, 3.5 in float32 over 2 x 16384 x 8).
 template <int DT, int NP, bool BACK, bool EVEN>
 __global__ void __launch_bounds__(WG, 2) k_attn_states(const Args a) {
     using M = Mat<DT>;
@@ -725,9 +728,10 @@ __device__ __forceinline__ void zero_rows(const Heads& x, int64_t b, int h, int 
 
 // ---- forward ------------------------------------------------------------------------------------------
 // A workgroup walks a piece with the state in registers, and lays it into LDS (in parts for bfloat16) for the product
-// with q; the next chunk's q, k and v are loaded into registers while this one's products run.  Bound in bfloat16 by vector work
-// (55% of the SIMDs' time: decays, splits, masks) and LDS, at 2.7 TB/s of inputs and results; in float32 by the matrix cores' rate
-// for it and LDS together, 110 us for 16 GFLOP.
+// with q; the next chunk's q, k and v are loaded into registers while this one's products run.  Nothing is full: in bfloat16 (59 us, 2.3
+// TB/s of inputs and results) vector work has 64% of the SIMDs' cycles (decays, splits into parts, masks), the matrix cores 19%, LDS
+// 34%, 41% of that conflicts; in float32 the matrix cores are busy for 50%: 112 us for 7.0 GFLOP, 62 TFLOP/s.  The rest is waiting,
+// at two barriers a chunk with two workgroups on a CU.
 template <int DT, int NP>
 struct FwdLds {
     using M = Mat<DT>;
@@ -935,11 +939,12 @@ struct BwdLds {
     static constexpr int BYTES = (int)sizeof(typename M::E) * (D + Tile<DT, PV>::SIZE);
 };
 // The products of one chunk take no turn behind another's, so there is a workgroup for each and nothing is carried: 4096 of them at
-// 2 x 16384 x 8 in float32, 224 us of which the matrix cores are busy for 59%.  Loads at a chunk's start take a quarter of its time,
-// which other workgroups on the CU hide: with up to 64 keys three of them, if what is made of v comes before anything of k, so
-// that one place in LDS does for both (four places and two workgroups: 255 us; 2 x 8192 x 16 in bfloat16 113 and 144).  Not in
+// 2 x 16384 x 8 in float32, 219 us for 16 GFLOP, of which the matrix cores are busy for 58%.  Loads at a chunk's start take a quarter of
+// its time, which other workgroups on the CU hide: with up to 64 keys three of them, if what is made of v comes before anything of
+// k, so that one place in LDS does for both (four places and two workgroups: 248 us; 2 x 8192 x 16 in bfloat16 128 and 159).  Not in
 // turns, which keep k and need more registers, nor in bfloat16 of odd widths.  Walking chunks with the next one's tiles loaded
-// ahead needs more registers than there are.
+// ahead needs more registers than there are.  In turn nothing is full (bfloat16: vector 48%, matrix 14%, LDS 31% of the cycles): seven
+// barriers a head, and scalar registers for the tensors' addresses that are kept in vector lanes (127 to 180 in turn, 88 to 101 else).
 // A workgroup has one chunk of a head, or (TURNS) of all heads of a group one after another: their queries and keys are read once, and
 // what the heads give to dq and dk is summed in registers.
 template <int DT, int NP, bool TURNS, bool EVEN>
@@ -1360,8 +1365,9 @@ __global__ void __launch_bounds__(WG) k_attn_step(const Args a) {
 Heads heads_of(const boa_heads& x) { return {x.p, x.batch_stride, x.row_stride, x.head_stride}; }
 
 // The split: pieces of whole chunks, as many as give the wanted workgroups, two for each CU.  Forward of 4 x 4097 x 16 heads in
-// bfloat16 with 256, 512, 768 and 1024 wanted: 92, 61, 73 and 67 us; of 2 x 16384 x 8 in float32: 153, 125, 165 and 126.  Backward
-// 1024 and 512 take the same time walking, but joining 13 us against 7.5.
+// bfloat16 with 256, 512, 768 and 1024 wanted: 109, 86, 88 and 89 us of kernels; of 2 x 16384 x 8 in float32: 194, 158, 192 and 166.
+// Backward 1024 and 512 take the same time walking, but joining 13 us against 7.5.  Padding counts as work here and in in_turn: the
+// lengths are on the device.
 constexpr int64_t WANTED = 512;
 struct Plan {
     int np, tiles;
@@ -1400,10 +1406,10 @@ struct Plan {
 
 // Whether a workgroup of the backward pass takes the heads of a group in turn: where that leaves two workgroups for each place on a CU
 // (two places, with more than 64 keys one), else each head by itself.
-// 32 x 500 x 16 heads of 4 groups in bfloat16: 109 us so, 135 + 45 for the sums over heads with each head by itself.  Forward and
-// backward of 2 x 8192 x 16 heads of 8 groups: 404 us in float32 and 248 in bfloat16, each head by itself 451 and 298; of 4 x 4096 x 16
-// heads of 2 groups and 128 keys 746 and 493, each by itself 903 and 631.  (A part of a group in turn: of 300 x 65 x 8 heads and 64 x
-// 500 x 8 heads of one group in bfloat16 247 and 215 us, each by itself 205 and 230.)
+// 32 x up to 500 x 16 heads of 4 groups in bfloat16: 127 us so, 112 + 42 for the sums over heads with each head by itself; 2 x 8192 x 16
+// heads of 8 groups: 234 in float32 and 160 in bfloat16, each by itself 218 + 66 and 143 + 65; 4 x 4096 x 16 heads of 2 groups and 128
+// keys: 454 and 317, each by itself 519 + 90 and 380 + 85.  (A part of a group in turn: forward and backward of 300 x 65 x 8 heads and
+// 64 x 500 x 8 heads of one group in bfloat16 247 and 215 us, each by itself 205 and 230.)
 bool in_turn(const boa_attention& s, const Plan& p) {
     const int share = s.heads / s.groups;
     return share > 1 && p.bh / share * p.tiles * p.chunks >= (p.np == 64 ? 2 : 1) * WANTED;

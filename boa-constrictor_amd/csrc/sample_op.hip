@@ -13,7 +13,8 @@
 //
 // Measured with top_k 50 and top_p 0.95: 65536 x 256 float32 122 us, 16384 x 1024 104, 4096 x 4096 139 (0.5 to 0.6 TB/s); a single
 // row 6, whose steps follow one another.  Bound by vector work: a search's step is a compare, a count or a sum over the lanes, about
-// 30 steps a row; exponentials in 64 bits are the rest.
+// 30 steps a row; exponentials in 64 bits are the rest.  Above 256 symbols 11 to 62 scalar registers are kept in
+// vector lanes (counts of the keys).
 #include "ops_common.h"
 
 #include "../../include/boa_hip.h"
